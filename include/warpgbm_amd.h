@@ -227,6 +227,124 @@ int wgbm_importance_add(float* acc, int32_t n_feats, int32_t num_eras, const flo
                         const int64_t* node, const int64_t* feat_start, void* stream);
 
 /* ------------------------------------------------------------------------
+ * Losses of class scores and of paired scores, with their gradients (no
+ * counterpart in the reference, whose losses are squared error and softmax
+ * cross entropy): what a boosting round with the engine's objective 2 fits.
+ *
+ * All sums are float32 (sums over the rows of a sequence, over the pairs of a
+ * sequence and over all rows: float64), in an order that depends on the sizes
+ * only: results are the same in every run.  Gradients are rounded to the
+ * scores' type once.  The calls allocate nothing and may be captured into a
+ * HIP graph; `workspace` (device memory, 16-byte aligned, of the bytes that the
+ * matching _workspace call returns, -1 for arguments it refuses) is written
+ * before it is read and must not be shared by calls that may overlap.
+ * ------------------------------------------------------------------------ */
+#define WGBM_F32 0
+#define WGBM_BF16 1
+#define WGBM_F16 2
+
+/* Scores [n_rows, n_classes] of one of the types above, or a gradient of
+ * them: element (i, k) at data[i * row_stride + k * class_stride], strides in
+ * elements.  Either class_stride is 1 (row-major, row_stride >= n_classes) or
+ * row_stride is 1 (class-major, class_stride >= n_rows: the engine's scores).
+ * n_classes at most 2^24.  A score of -inf is a class that the row may not
+ * take; a row whose scores are all -inf has no class and counts as left out
+ * (results 0).  NaN shows in the results of its row. */
+typedef struct wgbm_scores {
+  void* data;
+  int32_t dtype;
+  int64_t n_rows;
+  int32_t n_classes;
+  int64_t row_stride;
+  int64_t class_stride;
+} wgbm_scores;
+
+/* log_prob[i] = log softmax(scores[i])[labels[i]], and norm [n_rows][2]: the
+ * row's maximum m and log(sum exp(s - m)).  A row whose label is outside
+ * [0, n_classes) has log_prob 0; a row without a class has log_prob 0 and norm
+ * (-inf, 0). */
+int64_t wgbm_class_log_probs_workspace(const wgbm_scores* scores);
+int wgbm_class_log_probs(const wgbm_scores* scores, const int32_t* labels, float* log_prob,
+                         float* norm, void* workspace, int64_t workspace_bytes, void* stream);
+/* grad[i][k] = grad_log_prob[i] * (1[k = labels[i]] - softmax(scores[i])[k]);
+ * 0 for rows without a label or a class and where grad_log_prob is 0.  norm as
+ * written by wgbm_class_log_probs. */
+int wgbm_class_log_probs_grad(const wgbm_scores* scores, const int32_t* labels, const float* norm,
+                              const float* grad_log_prob, const wgbm_scores* grad, void* stream);
+
+/* Clipped policy loss with a KL term, per row, and its gradient:
+ *   ratio = exp(logp[action] - old_log_prob),
+ *   loss = weight * (-min(ratio A, clip(ratio, 1 - clip_low, 1 + clip_high) A) + kl_coef * KL),
+ * KL = exp(x) - x - 1 with x = ref_log_prob - logp[action] (the sampled
+ * estimate), or sum_k p_k (log p_k - log q_k) for q = softmax(ref_scores), or
+ * absent when neither is given.  Whether a ratio is clipped is decided as in
+ * float64.  weight NULL: 1.  A row of weight 0 or whose action is outside
+ * [0, n_classes) is not read: loss, log_prob, kl and gradient 0.  A class of
+ * probability 0 takes no part in the exact KL; one that only the reference
+ * excludes makes it infinite.  kl may be NULL; grad NULL: no gradient;
+ * accumulate != 0 adds to grad instead of overwriting it.  grad must not
+ * overlap an input. */
+typedef struct wgbm_policy_args {
+  const int32_t* actions;          /* [n_rows] */
+  const float* old_log_prob;       /* [n_rows] */
+  const float* advantage;          /* [n_rows] */
+  const float* weight;             /* [n_rows] or NULL */
+  const float* ref_log_prob;       /* [n_rows] or NULL */
+  const wgbm_scores* ref_scores;   /* of the scores' shape, type and order, or NULL */
+  double clip_low;                 /* [0, 1] */
+  double clip_high;                /* [0, inf) */
+  float kl_coef;
+} wgbm_policy_args;
+int64_t wgbm_policy_loss_workspace(const wgbm_scores* scores);
+int wgbm_policy_loss(const wgbm_scores* scores, const wgbm_policy_args* args, float* loss,
+                     float* log_prob, float* kl, const wgbm_scores* grad, int32_t accumulate,
+                     void* workspace, int64_t workspace_bytes, void* stream);
+
+/* Balance loss over the n' rows with mask != 0 (mask NULL: all) that have a
+ * class: counts[k] (int64) = rows with class k among their top_k classes (the
+ * lower class first among equal scores; -inf and NaN are never taken), f_k =
+ * counts[k] / (n' top_k), prob[k] = mean of softmax(scores)[k],
+ *   *loss = coef * n_classes * sum_k f_k prob[k],
+ * grad as for the policy loss, with f held constant (0 in rows left out; with
+ * accumulate those keep what they hold).  n_classes at most 4096, top_k at
+ * most 8.  Without a row that counts everything is 0. */
+int64_t wgbm_balance_loss_workspace(const wgbm_scores* scores);
+int wgbm_balance_loss(const wgbm_scores* scores, const uint8_t* mask, int32_t top_k, float coef,
+                      float* loss, int64_t* counts, float* prob, const wgbm_scores* grad,
+                      int32_t accumulate, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* Preference loss of pairs of sequences of rows (paired log ratios): with
+ * u_i = log_prob[i] - ref_log_prob[i] and U_s the sum of u over the rows
+ * sequence_start[s] .. sequence_start[s + 1] of sequence s (none: U_s = 0),
+ *   margin[p] = U[preferred] - U[other],
+ *   loss[p] = weight[p] * ((1 - e) log(1 + exp(-beta margin)) + e log(1 + exp(beta margin))),
+ * e = label_smoothing, and grad[i] = sum over the pairs that hold i's sequence.
+ * Rows behind the last sequence have gradient 0.  Without sequence_start every
+ * row is a sequence.  pairs [n_pairs][2]: sequence numbers, which the call
+ * takes as valid (0 .. n_sequences - 1), as it does the offsets (from 0, not
+ * descending, at most n_rows); incidence [2 n_pairs]: the numbers
+ * 2 * pair + side (0 preferred, 1 other) grouped by sequence,
+ * incidence_start [n_sequences + 1] their offsets.  A pair of weight 0 is not
+ * read.  grad NULL: no gradient (incidence may be NULL then). */
+typedef struct wgbm_preference_args {
+  const float* log_prob;            /* [n_rows] */
+  const float* ref_log_prob;        /* [n_rows] or NULL (0) */
+  int64_t n_rows;
+  const int64_t* sequence_start;    /* [n_sequences + 1] or NULL */
+  int64_t n_sequences;
+  const int32_t* pairs;
+  int64_t n_pairs;
+  const int32_t* incidence;
+  const int64_t* incidence_start;
+  const float* weight;              /* [n_pairs] or NULL (1) */
+  float beta;
+  float label_smoothing;            /* [0, 0.5] */
+} wgbm_preference_args;
+int64_t wgbm_preference_loss_workspace(const wgbm_preference_args* args);
+int wgbm_preference_loss(const wgbm_preference_args* args, float* loss, float* margin, float* grad,
+                         void* workspace, int64_t workspace_bytes, void* stream);
+
+/* ------------------------------------------------------------------------
  * Level-wise boosting engine (the caller of the four operators:
  * warpgbm/core.py grow_forest 692-744, grow_forest_multiclass 746-818,
  * grow_tree 597-658).

@@ -45,6 +45,15 @@ SIGNATURES = {
     "wgbm_predict_heap_path": (C.c_int, [_i64, _i64, _i32, _i32, _i32]),
     "wgbm_importance_add": (C.c_int, [_p, _i32, _i32, _p, _p, _p, _p]),
     "wgbm_softmax_rows": (C.c_int, [_p, _i64, _i32, _p]),
+    "wgbm_class_log_probs_workspace": (_i64, [_p]),
+    "wgbm_class_log_probs": (C.c_int, [_p, _p, _p, _p, _p, _i64, _p]),
+    "wgbm_class_log_probs_grad": (C.c_int, [_p, _p, _p, _p, _p, _p]),
+    "wgbm_policy_loss_workspace": (_i64, [_p]),
+    "wgbm_policy_loss": (C.c_int, [_p, _p, _p, _p, _p, _p, _i32, _p, _i64, _p]),
+    "wgbm_balance_loss_workspace": (_i64, [_p]),
+    "wgbm_balance_loss": (C.c_int, [_p, _p, _i32, _f32, _p, _p, _p, _p, _i32, _p, _i64, _p]),
+    "wgbm_preference_loss_workspace": (_i64, [_p]),
+    "wgbm_preference_loss": (C.c_int, [_p, _p, _p, _p, _p, _i64, _p]),
     "wgbm_engine_create": (C.c_int, [C.POINTER(_p), _p]),
     "wgbm_engine_round": (C.c_int, [_p, _p, _p, _p, _i32, _p, _p]),
     "wgbm_engine_set_tuning": (C.c_int, [_p, _i32, _i64]),
@@ -88,6 +97,48 @@ class TreeRecord(C.Structure):
         ("count", _p),
         ("gain", _p),
         ("H", _i32),
+    ]
+
+
+class Scores(C.Structure):
+    _fields_ = [
+        ("data", _p),
+        ("dtype", _i32),
+        ("n_rows", _i64),
+        ("n_classes", _i32),
+        ("row_stride", _i64),
+        ("class_stride", _i64),
+    ]
+
+
+class PolicyArgs(C.Structure):
+    _fields_ = [
+        ("actions", _p),
+        ("old_log_prob", _p),
+        ("advantage", _p),
+        ("weight", _p),
+        ("ref_log_prob", _p),
+        ("ref_scores", C.POINTER(Scores)),
+        ("clip_low", C.c_double),
+        ("clip_high", C.c_double),
+        ("kl_coef", _f32),
+    ]
+
+
+class PreferenceArgs(C.Structure):
+    _fields_ = [
+        ("log_prob", _p),
+        ("ref_log_prob", _p),
+        ("n_rows", _i64),
+        ("sequence_start", _p),
+        ("n_sequences", _i64),
+        ("pairs", _p),
+        ("n_pairs", _i64),
+        ("incidence", _p),
+        ("incidence_start", _p),
+        ("weight", _p),
+        ("beta", _f32),
+        ("label_smoothing", _f32),
     ]
 
 

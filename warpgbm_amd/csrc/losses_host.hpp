@@ -1,0 +1,70 @@
+// Host declarations of the losses (losses.hip, losses_balance.hip,
+// preference.hip).
+#pragma once
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "losses.hpp"
+
+namespace wgbm {
+
+// waves that fill the GPU (256 CUs, 16 waves each)
+constexpr int64_t kLossWaves = 4096;
+
+// runs a statement with T the element type of a dtype code
+#define LOSS_TYPES(dtype, ...)        \
+  do {                                \
+    if ((dtype) == kF32) {            \
+      using T = float;                \
+      __VA_ARGS__;                    \
+    } else if ((dtype) == kBF16) {    \
+      using T = __bf16;               \
+      __VA_ARGS__;                    \
+    } else {                          \
+      using T = _Float16;             \
+      __VA_ARGS__;                    \
+    }                                 \
+  } while (0)
+
+int32_t loss_splits(int64_t n, int32_t K, bool cm);
+
+size_t log_probs_workspace(int64_t n, int32_t K, bool cm);
+int class_log_probs(const ScoresView& s, const int32_t* label, const uint8_t* mask,
+                    float* log_prob, float* norm, void* ws, hipStream_t st);
+int class_log_probs_grad(const ScoresView& s, const int32_t* label, const float* norm,
+                         const float* grad, const ScoresView& out, hipStream_t st);
+
+size_t policy_workspace(int64_t n, int32_t K, bool cm);
+int policy_loss(const ScoresView& s, const ScoresView& ref, const PolicyRows& g,
+                const ScoresView& out, bool accumulate, void* ws, hipStream_t st);
+
+struct BalanceOut {
+  float* loss;
+  int64_t* counts;
+  float* prob;
+};
+size_t balance_workspace(int64_t n, int32_t K, bool cm);
+int balance_loss(const ScoresView& s, const uint8_t* mask, int32_t top_k, float coef,
+                 const BalanceOut& o, const ScoresView& out, bool accumulate, void* ws,
+                 hipStream_t st);
+
+struct PreferenceArgs {
+  const float* log_prob;
+  const float* ref;
+  int64_t n_rows;
+  const int64_t* seg_start;  // null: every row is a sequence of its own
+  int64_t n_seg;
+  const int32_t* pairs;      // [n_pairs][2]: preferred, other
+  int64_t n_pairs;
+  const int32_t* inc;        // [2 n_pairs]: 2 * pair + side, grouped by sequence
+  const int64_t* inc_start;  // [n_seg + 1]
+  const float* weight;
+  float beta, smooth;
+  float* loss;
+  float* margin;
+  float* grad;
+};
+size_t preference_workspace(int64_t n_seg, int64_t n_pairs, bool segments);
+int preference_loss(const PreferenceArgs& a, void* ws, hipStream_t st);
+
+}  // namespace wgbm

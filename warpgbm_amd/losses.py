@@ -1,0 +1,356 @@
+"""Losses of class scores and of paired scores, with their gradients.
+
+What a boosting round of the objectives "policy", "preference" and
+"policy_preference" fits its trees to, as operators on GPU tensors: each call
+returns the per-row (per-pair) losses and the gradient with respect to the
+scores, computed by the HIP library through the C ABI of
+``include/warpgbm_amd.h``.  The reference has no counterpart (its losses are
+squared error and softmax cross entropy, warpgbm/core.py:186-214, 719).
+
+Scores are [n rows, K classes] in float32, bfloat16 or float16, with either the
+classes of a row next to each other (``scores`` contiguous, or rows with a
+stride) or the rows of a class (``scores_cm.t()`` of the engine's class-major
+[K, n]).  Per-row inputs are contiguous.  A score of -inf is a class that the
+row may not take; a row whose scores are all -inf counts as left out.  Rows
+left out (weight 0, mask false, label outside [0, K)) are not read: their
+results and gradients are 0, whatever their scores hold.
+
+Launches go on torch's current stream of the scores' device; nothing
+synchronises except the construction of a :class:`PreferencePlan`.  Outputs and
+working memory come from torch's allocator, so calls may be captured into a
+HIP graph.  Wrong types, shapes, devices or layouts raise ``RuntimeError``.
+"""
+from __future__ import annotations
+
+import ctypes as C
+from collections import namedtuple
+
+import numpy as np
+import torch
+
+from . import _lib
+
+ClassLogProbs = namedtuple("ClassLogProbs", ["log_prob", "norm"])
+PolicyLoss = namedtuple("PolicyLoss", ["loss", "log_prob", "kl", "grad"])
+BalanceLoss = namedtuple("BalanceLoss", ["loss", "counts", "prob", "grad"])
+PreferenceLoss = namedtuple("PreferenceLoss", ["loss", "margin", "grad"])
+
+_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+
+
+def _vector(t, name, dtype, n, device):
+    """A contiguous [n] tensor of dtype on device; its address."""
+    if not isinstance(t, torch.Tensor):
+        raise RuntimeError(f"{name} must be a torch.Tensor")
+    if t.dtype != dtype:
+        raise RuntimeError(f"{name} must have dtype {dtype}, got {t.dtype}")
+    if t.device != device:
+        raise RuntimeError(f"{name} must be on {device}, got {t.device}")
+    if t.dim() != 1 or t.shape[0] != n:
+        raise RuntimeError(f"{name} must have shape ({n},), got {tuple(t.shape)}")
+    if not t.is_contiguous():
+        raise RuntimeError(f"{name} must be contiguous")
+    return t.data_ptr()
+
+
+def _matrix(t, name):
+    """The C view of a [n, K] tensor of scores."""
+    if not isinstance(t, torch.Tensor):
+        raise RuntimeError(f"{name} must be a torch.Tensor")
+    code = _DTYPES.get(t.dtype)
+    if code is None:
+        raise RuntimeError(f"{name} must be float32, bfloat16 or float16, got {t.dtype}")
+    if not t.is_cuda:
+        raise RuntimeError(f"{name} must be a GPU tensor, got device {t.device}")
+    if t.dim() != 2:
+        raise RuntimeError(f"{name} must be 2-D, got shape {tuple(t.shape)}")
+    n, K = t.shape
+    if K < 1:
+        raise RuntimeError(f"{name} must have at least one class")
+    rs, ks = t.stride()
+    # the stride of a dimension of one element says nothing
+    if K == 1 or n == 0:
+        rs, ks = max(rs, K), 1
+    elif n == 1:
+        rs = K if ks == 1 else 1
+    if not ((ks == 1 and rs >= K) or (rs == 1 and ks >= n)):
+        raise RuntimeError(f"{name} must have the classes of a row or the rows of a class next to "
+                           f"each other (no overlap), got strides {tuple(t.stride())}")
+    return _lib.Scores(t.data_ptr(), code, n, K, rs, ks)
+
+
+def _like(v, scores):
+    """A new matrix of the scores' shape, type and order, and its view."""
+    n, K = scores.shape
+    if v.row_stride == 1 and v.class_stride != 1:
+        t = torch.empty_strided((n, K), (1, max(n, 2)), dtype=scores.dtype, device=scores.device)
+        return t, _lib.Scores(t.data_ptr(), v.dtype, n, K, 1, max(n, 2))
+    t = torch.empty((n, K), dtype=scores.dtype, device=scores.device)
+    return t, _lib.Scores(t.data_ptr(), v.dtype, n, K, K, 1)
+
+
+def _grad(grad, v, scores, with_grad):
+    """The gradient's matrix: a given one (added to), a new one, or none."""
+    if grad is None:
+        return _like(v, scores) if with_grad else (None, None)
+    if not with_grad:
+        raise RuntimeError("grad given, but with_grad is False")
+    g = _matrix(grad, "grad")
+    if grad.device != scores.device or grad.dtype != scores.dtype or grad.shape != scores.shape:
+        raise RuntimeError("grad must have the shape, dtype and device of scores")
+    if (g.row_stride == 1 and g.class_stride != 1) != (v.row_stride == 1 and v.class_stride != 1):
+        raise RuntimeError("grad must have its rows or classes next to each other as scores has")
+    if grad.data_ptr() == scores.data_ptr() and scores.numel():
+        raise RuntimeError("grad must not be the scores' memory")
+    return grad, g
+
+
+class _on:
+    """The scores' device as the current one (HIP launches go to the device
+    that is current), at no cost where it already is."""
+
+    def __init__(self, device):
+        self.index = device.index
+        self.back = None
+
+    def __enter__(self):
+        now = torch.cuda.current_device()
+        if self.index is not None and now != self.index:
+            torch.cuda.set_device(self.index)
+            self.back = now
+
+    def __exit__(self, *exc):
+        if self.back is not None:
+            torch.cuda.set_device(self.back)
+
+
+def _workspace(nbytes, device, what):
+    if nbytes < 0:
+        _lib.check(1000, what)
+    return torch.empty(max(int(nbytes), 16), dtype=torch.uint8, device=device)
+
+
+def class_log_probs(scores, labels) -> ClassLogProbs:
+    """Log-probability of each row's label under softmax(scores), and the norm
+    [n, 2] of every row (its maximum m and log(sum exp(s - m))), which
+    :func:`class_log_probs_grad` takes.  labels: int32 [n]; a row whose label is
+    outside [0, K) has none and log-probability 0."""
+    v = _matrix(scores, "scores")
+    n, dev = scores.shape[0], scores.device
+    lab = _vector(labels, "labels", torch.int32, n, dev)
+    lib = _lib.load()
+    with _on(dev):
+        log_prob = torch.empty(n, dtype=torch.float32, device=dev)
+        norm = torch.empty((n, 2), dtype=torch.float32, device=dev)
+        ws = _workspace(lib.wgbm_class_log_probs_workspace(C.byref(v)), dev, "class_log_probs")
+        rc = lib.wgbm_class_log_probs(C.byref(v), lab, log_prob.data_ptr(), norm.data_ptr(),
+                                      ws.data_ptr(), ws.numel(), _lib.current_stream_ptr(dev))
+    _lib.check(rc, "class_log_probs")
+    return ClassLogProbs(log_prob, norm)
+
+
+def class_log_probs_grad(scores, labels, norm, grad_log_prob) -> torch.Tensor:
+    """Gradient with respect to the scores of sum_i grad_log_prob[i] *
+    log_prob[i], in the scores' type and order."""
+    v = _matrix(scores, "scores")
+    n, dev = scores.shape[0], scores.device
+    lab = _vector(labels, "labels", torch.int32, n, dev)
+    g = _vector(grad_log_prob, "grad_log_prob", torch.float32, n, dev)
+    if not isinstance(norm, torch.Tensor) or tuple(norm.shape) != (n, 2):
+        raise RuntimeError(f"norm must be a ({n}, 2) tensor")
+    nrm = _vector(norm.view(-1) if norm.is_contiguous() else norm, "norm", torch.float32, 2 * n,
+                  dev)
+    lib = _lib.load()
+    with _on(dev):
+        out, ov = _like(v, scores)
+        rc = lib.wgbm_class_log_probs_grad(C.byref(v), lab, nrm, g, C.byref(ov),
+                                           _lib.current_stream_ptr(dev))
+    _lib.check(rc, "class_log_probs_grad")
+    return out
+
+
+def policy_loss(scores, actions, old_log_prob, advantage, *, weight=None, ref_log_prob=None,
+                ref_scores=None, clip=(0.2, 0.2), kl_coef=0.0, grad=None,
+                with_grad=True) -> PolicyLoss:
+    """Clipped policy loss with a KL term, per row, and its gradient.
+
+    ratio = exp(logp[action] - old_log_prob) and
+    ``loss = weight * (-min(ratio * advantage, clip(ratio, 1 - clip[0], 1 +
+    clip[1]) * advantage) + kl_coef * KL)``; KL is the sampled estimate
+    exp(x) - x - 1 with x = ref_log_prob - logp[action], or the divergence of
+    softmax(scores) from softmax(ref_scores) over all classes (ref_scores: the
+    scores' shape, type and order), or absent when neither is given.  Whether a
+    ratio is clipped is decided as in float64.
+
+    actions int32 [n]; old_log_prob, advantage, weight, ref_log_prob float32
+    [n].  Rows of weight 0 are left out.  ``loss``, ``log_prob`` and ``kl`` (None
+    without a reference; not weighted) are float32 [n]; ``grad`` is the gradient
+    of the losses' sum, added to a given ``grad``, None with
+    ``with_grad=False``."""
+    v = _matrix(scores, "scores")
+    n, dev = scores.shape[0], scores.device
+    if ref_scores is not None and ref_log_prob is not None:
+        raise RuntimeError("ref_scores and ref_log_prob exclude each other")
+    try:
+        low, high = (float(c) for c in clip)
+    except (TypeError, ValueError):
+        raise RuntimeError(f"clip must be a pair of numbers, got {clip!r}") from None
+    f32 = torch.float32
+    rv = None
+    if ref_scores is not None:
+        rv = _matrix(ref_scores, "ref_scores")
+        if ref_scores.device != dev:
+            raise RuntimeError(f"ref_scores must be on {dev}, got {ref_scores.device}")
+    args = _lib.PolicyArgs(
+        _vector(actions, "actions", torch.int32, n, dev),
+        _vector(old_log_prob, "old_log_prob", f32, n, dev),
+        _vector(advantage, "advantage", f32, n, dev),
+        _vector(weight, "weight", f32, n, dev) if weight is not None else None,
+        _vector(ref_log_prob, "ref_log_prob", f32, n, dev) if ref_log_prob is not None else None,
+        C.pointer(rv) if rv is not None else None, low, high, float(kl_coef))
+    lib = _lib.load()
+    with _on(dev):
+        out, gv = _grad(grad, v, scores, with_grad)
+        loss = torch.empty(n, dtype=f32, device=dev)
+        log_prob = torch.empty(n, dtype=f32, device=dev)
+        kl = None
+        if ref_scores is not None or ref_log_prob is not None:
+            kl = torch.empty(n, dtype=f32, device=dev)
+        ws = _workspace(lib.wgbm_policy_loss_workspace(C.byref(v)), dev, "policy_loss")
+        rc = lib.wgbm_policy_loss(
+            C.byref(v), C.byref(args), loss.data_ptr(), log_prob.data_ptr(),
+            kl.data_ptr() if kl is not None else None,
+            C.byref(gv) if gv is not None else None, int(grad is not None), ws.data_ptr(),
+            ws.numel(), _lib.current_stream_ptr(dev))
+    _lib.check(rc, "policy_loss")
+    return PolicyLoss(loss, log_prob, kl, out)
+
+
+def balance_loss(scores, *, top_k=1, mask=None, coef=1.0, grad=None,
+                 with_grad=True) -> BalanceLoss:
+    """How evenly rows fall on classes: ``loss = coef * K * sum_k f_k * prob_k``
+    with f_k the share of class k among the top_k choices of the rows that count
+    (``counts``, int64 [K]; the lower class first among equal scores) and prob_k
+    the mean of softmax(scores) (float32 [K]).  The least value, coef, is that
+    of even classes.
+
+    mask: bool [n], the rows that count (None: all).  The gradient (of prob, the
+    counts held constant) is added to a given ``grad``.  At most 4096 classes,
+    top_k at most 8 and K."""
+    v = _matrix(scores, "scores")
+    n, dev = scores.shape[0], scores.device
+    K = scores.shape[1]
+    if mask is not None:
+        mask = _vector(mask, "mask", torch.bool, n, dev)
+    lib = _lib.load()
+    with _on(dev):
+        out, gv = _grad(grad, v, scores, with_grad)
+        loss = torch.empty((), dtype=torch.float32, device=dev)
+        counts = torch.empty(K, dtype=torch.int64, device=dev)
+        prob = torch.empty(K, dtype=torch.float32, device=dev)
+        ws = _workspace(lib.wgbm_balance_loss_workspace(C.byref(v)), dev, "balance_loss")
+        rc = lib.wgbm_balance_loss(
+            C.byref(v), mask, int(top_k), float(coef), loss.data_ptr(), counts.data_ptr(),
+            prob.data_ptr(), C.byref(gv) if gv is not None else None, int(grad is not None),
+            ws.data_ptr(), ws.numel(), _lib.current_stream_ptr(dev))
+    _lib.check(rc, "balance_loss")
+    return BalanceLoss(loss, counts, prob, out)
+
+
+class PreferencePlan:
+    """Pairs of sequences laid out for :func:`preference_loss`, once for all
+    rounds of a fit.
+
+    pairs: integers [P, 2], (preferred, other) sequence numbers; n_rows: rows of
+    the log-probabilities; segments: offsets [S + 1] of the sequences' rows
+    (from 0, not descending, at most n_rows; an empty sequence has a log ratio
+    of 0, rows behind the last one belong to none), or None when every row is a
+    sequence of its own.  Arrays or tensors; ``device`` where they are not
+    already on a GPU.  The construction checks them (it waits for the GPU) and
+    keeps copies."""
+
+    def __init__(self, pairs, n_rows, segments=None, device=None):
+        pairs = self._whole_numbers(pairs, "pairs")
+        if pairs.dim() != 2 or pairs.shape[1] != 2:
+            raise RuntimeError(f"pairs must have shape (P, 2), got {tuple(pairs.shape)}")
+        if device is None:
+            device = pairs.device if pairs.is_cuda else torch.device("cuda")
+        device = torch.device(device)
+        if device.type == "cuda" and device.index is None:
+            device = torch.device("cuda", torch.cuda.current_device())
+        self.device = device
+        self.n_rows = int(n_rows)
+        if self.n_rows < 0:
+            raise RuntimeError("n_rows must not be negative")
+        P = pairs.shape[0]
+        if P >= 1 << 30:
+            raise RuntimeError("at most 2^30 - 1 pairs")
+        self.n_pairs = P
+        self.sequence_start = None
+        S = self.n_rows
+        if segments is not None:
+            seg = self._whole_numbers(segments, "segments").to(device=device, dtype=torch.int64)
+            if seg.dim() != 1 or seg.shape[0] < 1:
+                raise RuntimeError("segments must be the offsets [S + 1] of S sequences")
+            S = seg.shape[0] - 1
+            if int(seg[0]) != 0 or int(seg[-1]) > self.n_rows or bool((seg[1:] < seg[:-1]).any()):
+                raise RuntimeError(f"segments must ascend from 0 to at most n_rows={self.n_rows}")
+            self.sequence_start = seg.clone()
+        if S >= 1 << 31:
+            raise RuntimeError("too many sequences")
+        self.n_sequences = S
+        pairs = pairs.to(device=device, dtype=torch.int64)
+        if P and (int(pairs.min()) < 0 or int(pairs.max()) >= S):
+            raise RuntimeError(f"pairs must hold sequence numbers in [0, {S})")
+        self.pairs = pairs.to(torch.int32).contiguous().clone()
+        # the numbers 2 * pair + side grouped by sequence (a stable sort: in
+        # pair order), and each sequence's range of them
+        ends = self.pairs.reshape(-1)
+        order = torch.sort(ends, stable=True)
+        self.incidence = order.indices.to(torch.int32)
+        self.incidence_start = torch.searchsorted(
+            order.values, torch.arange(S + 1, dtype=torch.int32, device=device))
+
+    @staticmethod
+    def _whole_numbers(a, name):
+        t = a if isinstance(a, torch.Tensor) else torch.from_numpy(np.ascontiguousarray(a))
+        if t.dtype not in (torch.int32, torch.int64):
+            raise RuntimeError(f"{name} must be int32 or int64, got {t.dtype}")
+        return t
+
+
+def preference_loss(log_prob, plan, *, ref_log_prob=None, weight=None, beta=1.0,
+                    label_smoothing=0.0, with_grad=True) -> PreferenceLoss:
+    """Loss of the plan's pairs, and its gradient with respect to log_prob.
+
+    With U_s the sum over sequence s of log_prob - ref_log_prob, ``margin =
+    U[preferred] - U[other]`` and ``loss = weight * ((1 - e) * softplus(-beta *
+    margin) + e * softplus(beta * margin))``, e = label_smoothing, one per pair;
+    ``grad`` is the gradient of the losses' sum (None with
+    ``with_grad=False``).  log_prob, ref_log_prob: float32 [n_rows], any scores
+    of rows (a scorer's without a reference give the pairwise logistic loss);
+    weight: float32 [P], pairs of weight 0 are left out (margin 0)."""
+    if not isinstance(plan, PreferencePlan):
+        raise RuntimeError("plan must be a PreferencePlan")
+    n, dev = plan.n_rows, plan.device
+    f32 = torch.float32
+    lp = _vector(log_prob, "log_prob", f32, n, dev)
+    rp = _vector(ref_log_prob, "ref_log_prob", f32, n, dev) if ref_log_prob is not None else None
+    P = plan.n_pairs
+    w = _vector(weight, "weight", f32, P, dev) if weight is not None else None
+    seg = plan.sequence_start
+    args = _lib.PreferenceArgs(
+        lp, rp, n, seg.data_ptr() if seg is not None else None, plan.n_sequences,
+        plan.pairs.data_ptr(), P, plan.incidence.data_ptr(), plan.incidence_start.data_ptr(), w,
+        float(beta), float(label_smoothing))
+    lib = _lib.load()
+    with _on(dev):
+        loss = torch.empty(P, dtype=f32, device=dev)
+        margin = torch.empty(P, dtype=f32, device=dev)
+        grad = torch.empty(n, dtype=f32, device=dev) if with_grad else None
+        ws = _workspace(lib.wgbm_preference_loss_workspace(C.byref(args)), dev, "preference_loss")
+        rc = lib.wgbm_preference_loss(C.byref(args), loss.data_ptr(), margin.data_ptr(),
+                                      grad.data_ptr() if grad is not None else None,
+                                      ws.data_ptr(), ws.numel(), _lib.current_stream_ptr(dev))
+    _lib.check(rc, "preference_loss")
+    return PreferenceLoss(loss, margin, grad)
