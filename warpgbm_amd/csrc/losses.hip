@@ -6,38 +6,10 @@
 // row, and the gradient is written by an elementwise pass over the scores.
 #include <algorithm>
 
-#include "losses.hpp"
+#include "losses_frames.hpp"
 #include "losses_host.hpp"
 
 namespace wgbm {
-
-// ---------------------------------------------------------------------------
-// 16 bytes of a row: VE classes next to each other.  Rows of an odd length
-// start at any multiple of the element size; global loads and stores of this
-// GPU take such addresses.
-// ---------------------------------------------------------------------------
-template <typename T>
-struct Chunk {
-  static constexpr int VE = 16 / (int)sizeof(T);
-  T v[VE];
-};
-template <typename T>
-__device__ __forceinline__ Chunk<T> load_chunk(const T* p) {
-  Chunk<T> c;
-  __builtin_memcpy(&c, p, 16);
-  return c;
-}
-template <typename T>
-__device__ __forceinline__ void store_chunk(T* p, const Chunk<T>& c) {
-  __builtin_memcpy(p, &c, 16);
-}
-
-// label of row i, -1 where it has none
-__device__ __forceinline__ int32_t row_label(const int32_t* label, int64_t i, int32_t K) {
-  if (!label) return -1;
-  const int32_t a = label[i];
-  return a >= 0 && a < K ? a : -1;
-}
 
 // statistics of the classes [k0, k1), k0 + step * j, of one row by one thread
 template <typename T, bool REF>
@@ -137,8 +109,8 @@ __global__ __launch_bounds__(256) void log_prob_rows_kernel(ScoresView s,
   const int32_t lab = row_label(label, i, s.K);
   const float sa = lab >= 0 ? to_f32(((const T*)s.data)[i * s.rs + lab * s.ks]) : 0.0f;
   const LogProb lp = row_log_prob(a, sa);
-  if (log_prob) log_prob[i] = lp.live && lab >= 0 ? lp.logp : 0.0f;
-  norm[i] = lp.live ? make_float2(lp.m, lp.l) : make_float2(-__builtin_inff(), 0.0f);
+  if (log_prob) log_prob[i] = lp.live && lab >= 0 ? (float)lp.logp : 0.0f;
+  norm[i] = lp.live ? make_float2(lp.m, (float)lp.l) : make_float2(-__builtin_inff(), 0.0f);
 }
 
 // log p of the label in float64, by the 64 lanes of a wave
@@ -218,15 +190,18 @@ struct LogProbGrad {
     const float2 v = norm[i];
     if (v.x == -__builtin_inff()) return c;
     c.m = v.x;
-    c.l = v.y;
+    c.iz = v.y;  // (the sum's logarithm)
     c.c0 = -g;
     c.label = a;
     c.live = 1;
     return c;
   }
+  __device__ __forceinline__ float at(const RowCoef& c, float s, float) const {
+    return c.c0 * loss_expf((s - c.m) - c.iz);
+  }
   // the label's from its own logarithm: 1 - p without a difference
   __device__ __forceinline__ float at_label(const RowCoef& c, float s) const {
-    return c.c0 * expm1f((s - c.m) - c.l);
+    return c.c0 * expm1f((s - c.m) - c.iz);
   }
 };
 
@@ -235,6 +210,9 @@ struct PolicyGrad {
   const RowCoef* coef;
   static constexpr bool kRef = REF;
   __device__ __forceinline__ RowCoef row(int64_t i, int32_t) const { return coef[i]; }
+  __device__ __forceinline__ float at(const RowCoef& c, float s, float r) const {
+    return coef_grad<REF>(c, s, r);
+  }
   __device__ __forceinline__ float at_label(const RowCoef& c, float) const { return c.gl; }
 };
 
@@ -260,7 +238,7 @@ __global__ __launch_bounds__(256) void score_grad_kernel(ScoresView s, ScoresVie
     for (int32_t k = k0; k < k1; ++k) {
       const float v = to_f32(p[k * s.ks]);
       const float r = G::kRef ? to_f32(q[k * ref.ks]) : 0.0f;
-      float x = k == c.label ? g.at_label(c, v) : coef_grad<G::kRef>(c, v, r);
+      float x = k == c.label ? g.at_label(c, v) : g.at(c, v, r);
       if (accumulate) x += to_f32(o[k * out.ks]);
       o[k * out.ks] = from_f32<T>(x);
     }
@@ -297,7 +275,7 @@ __global__ __launch_bounds__(256) void score_grad_kernel(ScoresView s, ScoresVie
       for (int j = 0; j < VE; ++j) {
         const float sv = to_f32(v.v[j]);
         const float rv = G::kRef ? to_f32(r.v[j]) : 0.0f;
-        float x = k + j == c.label ? g.at_label(c, sv) : coef_grad<G::kRef>(c, sv, rv);
+        float x = k + j == c.label ? g.at_label(c, sv) : g.at(c, sv, rv);
         if (accumulate) x += to_f32(old.v[j]);
         v.v[j] = from_f32<T>(x);
       }
@@ -378,6 +356,14 @@ static int log_probs_t(const ScoresView& s, const int32_t* label, const uint8_t*
 
 int class_log_probs(const ScoresView& s, const int32_t* label, const uint8_t* mask,
                     float* log_prob, float* norm, void* ws, hipStream_t st) {
+  if (log_prob) {
+    bool done = false;
+    const auto rows = s.dtype == kF32    ? log_probs_rows_f32
+                      : s.dtype == kBF16 ? log_probs_rows_bf16
+                                         : log_probs_rows_f16;
+    const int r = rows(s, label, log_prob, norm, st, &done);
+    if (r || done) return r;
+  }
   LOSS_TYPES(s.dtype, return log_probs_t<T>(s, label, mask, log_prob, norm, ws, st));
 }
 
@@ -404,6 +390,12 @@ static int policy_t(const ScoresView& s, const ScoresView& ref, const PolicyRows
 
 int policy_loss(const ScoresView& s, const ScoresView& ref, const PolicyRows& g,
                 const ScoresView& out, bool accumulate, void* ws, hipStream_t st) {
+  bool done = false;
+  const auto rows = s.dtype == kF32    ? policy_rows_f32
+                    : s.dtype == kBF16 ? policy_rows_bf16
+                                       : policy_rows_f16;
+  const int r = rows(s, ref, g, out, accumulate, st, &done);
+  if (r || done) return r;
   if (ref.data) LOSS_TYPES(s.dtype, return (policy_t<T, true>(s, ref, g, out, accumulate, ws, st)));
   LOSS_TYPES(s.dtype, return (policy_t<T, false>(s, ref, g, out, accumulate, ws, st)));
 }

@@ -40,11 +40,11 @@ struct PolicyRows {
   float* kl;
 };
 
-// what a row's gradient is made of: with d = s - m, p_k = exp(d_k - l),
+// what a row's gradient is made of: with d = s - m, p_k = exp(d_k) * iz,
 //   g_k = p_k * (c1 * (d_k - (r_k - mr)) + c0),  and at the label g_a = gl
 // (c1 and mr only with reference scores).  live = 0: the row's gradient is 0.
 struct RowCoef {
-  float m, l, c0, c1, mr, gl;
+  float m, iz, c0, c1, mr, gl;
   int32_t label;
   int32_t live;
 };
@@ -144,9 +144,13 @@ __device__ __forceinline__ RowStats join_stats(RowStats a, RowStats b) {
 // ---------------------------------------------------------------------------
 // what follows from a row's statistics
 // ---------------------------------------------------------------------------
+// (float64 from the row's sum on: the logarithm of many classes' sum, some
+// ten, would lose a digit in float32 that the ratio and the divergence of a
+// policy near its reference need)
 struct LogProb {
-  float logp, m, l;  // l = log of the sum of e^(s - m)
-  bool live;         // the row has a class
+  double logp, l;  // l = log of the sum of e^(s - m)
+  float m;
+  bool live;  // the row has a class
 };
 
 // sa: the label's score
@@ -155,8 +159,8 @@ __device__ __forceinline__ LogProb row_log_prob(const RowStats& a, float sa) {
   LogProb o;
   o.live = !(z == 0.0f);  // (NaN is live: it shows in the results)
   o.m = safe_max(a.m);
-  o.l = logf(z);
-  o.logp = (sa - o.m) - o.l;
+  o.l = log((double)z);
+  o.logp = ((double)sa - (double)o.m) - o.l;
   return o;
 }
 
@@ -180,19 +184,19 @@ __device__ __forceinline__ PolicyRow policy_row(const RowStats& st, float sa, fl
                                                 int32_t label, const double* exact_logp) {
   PolicyRow o;
   const LogProb lp = row_log_prob(st, sa);
+  const float z = st.z + st.za;
   o.c.m = lp.m;
-  o.c.l = lp.l;
+  o.c.iz = 1.0f / z;
   o.c.label = label;
   o.c.live = lp.live;
   o.near = false;
   if (!lp.live) {
     o.loss = o.logp = o.kl = 0.0f;
-    o.c.c0 = o.c.c1 = o.c.mr = o.c.gl = 0.0f;
+    o.c.c0 = o.c.c1 = o.c.mr = o.c.gl = o.c.iz = 0.0f;
     return o;
   }
-  const float z = st.z + st.za;
-  o.logp = lp.logp;
-  const float x = lp.logp - old;
+  o.logp = (float)lp.logp;
+  const float x = (float)(lp.logp - (double)old);
   const float ratio = expf(x);
   // positive advantages stop above the upper border, negative ones below the
   // lower
@@ -205,9 +209,9 @@ __device__ __forceinline__ PolicyRow policy_row(const RowStats& st, float sa, fl
     } else {
       const float edge = up ? g.log_hi : g.log_lo;
       stop = up ? x > edge : x < edge;
-      // float32's error: 2^-24 of |logp|, |old| and 1, and of the sum for each
-      // class that one thread adds to it (160 of them are within this bound)
-      o.near = fabsf(x - edge) < 1e-5f * (1.0f + fabsf(lp.logp) + fabsf(old));
+      // the sum's error is 2^-24 for each class that one thread adds to it
+      // (256 of them are within this bound), that of x and edge 2^-24 of theirs
+      o.near = fabsf(x - edge) < 2e-5f * (1.0f + fabsf(edge));
     }
   }
   float value = stop ? -A * (float)(up ? g.clip_hi : g.clip_lo) : -A * ratio;
@@ -216,15 +220,19 @@ __device__ __forceinline__ PolicyRow policy_row(const RowStats& st, float sa, fl
   o.kl = 0.0f;
   float wk = 0.0f, base = 0.0f;
   if (REF) {
-    const float lr = logf(st.zr);
-    o.kl = st.u / z - lp.l + lr;
-    base = lr - lp.l - o.kl;  // log p_k - log q_k - KL = (d_k - dr_k) + base
+    const double lr = log((double)st.zr) - lp.l;
+    const double kl = (double)st.u / (double)z + lr;
+    o.kl = (float)kl;
+    base = (float)(lr - kl);  // log p_k - log q_k - KL = (d_k - dr_k) + base
     value += g.kl_coef * o.kl;
     wk = w * g.kl_coef;
   } else if (g.ref_log_prob) {
-    const float d = g.ref_log_prob[i] - lp.logp;
+    const float d = (float)((double)g.ref_log_prob[i] - lp.logp);
     const float e = expm1f(d);
     o.kl = e - d;
+    // near 0 the difference loses what the series keeps
+    if (fabsf(d) < 0.03125f)
+      o.kl = d * d * fmaf(d, fmaf(d, fmaf(d, 1.0f / 120.0f, 1.0f / 24.0f), 1.0f / 6.0f), 0.5f);
     value += g.kl_coef * o.kl;
     c -= g.kl_coef * e;
   }
@@ -242,10 +250,10 @@ __device__ __forceinline__ PolicyRow policy_row(const RowStats& st, float sa, fl
 // gradient at a class that is not the label
 template <bool REF>
 __device__ __forceinline__ float coef_grad(const RowCoef& c, float s, float r) {
-  const float d = s - c.m, p = loss_expf(d - c.l);
+  const float d = s - c.m, e = loss_expf(d);
   float t = c.c0;
-  if (REF) t = p == 0.0f ? 0.0f : fmaf(c.c1, d - (r - c.mr), t);
-  return p * t;
+  if (REF) t = e == 0.0f ? 0.0f : fmaf(c.c1, d - (r - c.mr), t);
+  return e * c.iz * t;
 }
 
 }  // namespace wgbm

@@ -1,0 +1,273 @@
+// Frames: how a row's scores sit in the registers of the threads that share
+// it.  A frame loads a row's classes once; the losses make their passes
+// (maximum, sums, gradient) over the registers.
+#pragma once
+#include "losses.hpp"
+
+namespace wgbm {
+
+// 16 bytes of a row: VE classes next to each other.  Rows of an odd length
+// start at any multiple of the element size; global loads and stores of this
+// GPU take such addresses.
+template <typename T>
+struct Chunk {
+  static constexpr int VE = 16 / (int)sizeof(T);
+  T v[VE];
+};
+template <typename T>
+__device__ __forceinline__ Chunk<T> load_chunk(const T* p) {
+  Chunk<T> c;
+  __builtin_memcpy(&c, p, 16);
+  return c;
+}
+template <typename T>
+__device__ __forceinline__ void store_chunk(T* p, const Chunk<T>& c) {
+  __builtin_memcpy(p, &c, 16);
+}
+
+// label of row i, -1 where it has none
+__device__ __forceinline__ int32_t row_label(const int32_t* label, int64_t i, int32_t K) {
+  if (!label) return -1;
+  const int32_t a = label[i];
+  return a >= 0 && a < K ? a : -1;
+}
+
+// ---------------------------------------------------------------------------
+// reductions over a group of G lanes (a power of two up to 64, aligned); every
+// lane gets the same bits (each step combines two values that commute)
+// ---------------------------------------------------------------------------
+template <int CTRL>
+__device__ __forceinline__ float dpp_f32(float x) {
+  return __builtin_bit_cast(
+      float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), CTRL, 0xf, 0xf, true));
+}
+struct AddF {
+  __device__ __forceinline__ float operator()(float a, float b) const { return a + b; }
+};
+struct MaxF {
+  __device__ __forceinline__ float operator()(float a, float b) const { return fmaxf(a, b); }
+};
+template <int G, typename Op>
+__device__ __forceinline__ float lanes_reduce(float x, Op op) {
+  if (G >= 2) x = op(x, dpp_f32<0xB1>(x));   // lanes 1 0 3 2
+  if (G >= 4) x = op(x, dpp_f32<0x4E>(x));   // lanes 2 3 0 1
+  if (G >= 8) x = op(x, dpp_f32<0x141>(x));  // the other quad of eight
+  if (G >= 16) x = op(x, dpp_f32<0x140>(x));  // the other half of sixteen
+  if (G >= 32) x = op(x, __shfl_xor(x, 16));
+  if (G >= 64) x = op(x, __shfl_xor(x, 32));
+  return x;
+}
+
+// over a whole workgroup of NW waves: each wave's value through LDS (buf: NW
+// words that no other reduction of this row uses), joined in wave order
+template <int NW, typename Op>
+__device__ __forceinline__ float waves_reduce(float x, Op op, float* buf) {
+  x = lanes_reduce<64>(x, op);
+  if ((threadIdx.x & 63) == 0) buf[threadIdx.x >> 6] = x;
+  __syncthreads();
+  x = buf[0];
+#pragma unroll
+  for (int w = 1; w < NW; ++w) x = op(x, buf[w]);
+  return x;
+}
+
+// ---------------------------------------------------------------------------
+// RowFrame: classes next to each other.  G threads share a row; thread t holds
+// the chunks t, t + G, ... (NC of them): classes (c * G + t) * VE .. + VE.
+//
+// Every load is whole and unconditional, so that all of a thread's are in
+// flight together: a chunk that would pass the row's end is read VE classes
+// before it (K >= VE), and its classes that belong to other threads (or to
+// none) are then set to -inf.  Class of (chunk c, element e) = first(c) + e;
+// elements below skip(c) are not this thread's.
+// ---------------------------------------------------------------------------
+template <typename T_, int G_, int NC_>
+struct RowFrame {
+  using T = T_;
+  static constexpr int G = G_, NC = NC_, VE = Chunk<T>::VE, N = NC * VE;
+  static constexpr int kThreads = G <= 256 ? 256 : G, kMax = kThreads;
+  static constexpr bool kBarrier = G > 64, kSlices = false;
+  static constexpr int kRows = kThreads / G;  // rows of a workgroup
+  static constexpr int kBuf = G > 64 ? G / 64 : 1;
+  int32_t t, K;  // this thread's place in its group
+
+  __device__ __forceinline__ RowFrame(const ScoresView& s) : t(threadIdx.x % G), K(s.K) {}
+  static __device__ __forceinline__ int64_t row(int64_t block) {
+    return block * kRows + threadIdx.x / G;
+  }
+  __device__ __forceinline__ bool first_lane() const { return t == 0; }
+  __device__ __forceinline__ int32_t want(int c) const { return (c * G + t) * VE; }
+  __device__ __forceinline__ int32_t first(int c) const {
+    const int32_t k = want(c);
+    return k < K - VE ? k : K - VE;
+  }
+  __device__ __forceinline__ int32_t skip(int c) const { return want(c) - first(c); }
+
+  struct Regs {
+    Chunk<T> c[NC];
+  };
+  __device__ __forceinline__ void load(Regs& r, const ScoresView& s, int64_t i) const {
+    const T* p = (const T*)s.data + i * s.rs;
+#pragma unroll
+    for (int c = 0; c < NC; ++c) r.c[c] = load_chunk<T>(p + first(c));
+  }
+  __device__ __forceinline__ void trim(Regs& r) const {
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+      const int32_t sk = skip(c);
+      if (__any(sk > 0)) {
+#pragma unroll
+        for (int e = 0; e < VE; ++e)
+          r.c[c].v[e] = e < sk ? (T)(-__builtin_inff()) : r.c[c].v[e];
+      }
+    }
+  }
+  static __device__ __forceinline__ float value(const Regs& r, int j) {
+    return to_f32(r.c[j / VE].v[j % VE]);
+  }
+  __device__ __forceinline__ int32_t cls(int j) const { return first(j / VE) + j % VE; }
+
+  // reductions over the row; buf as for waves_reduce (kBuf words each)
+  template <typename Op>
+  __device__ __forceinline__ float reduce(float x, Op op, float* buf) const {
+    if (G <= 64) return lanes_reduce<(G < 64 ? G : 64)>(x, op);
+    return waves_reduce<(G > 64 ? G / 64 : 1)>(x, op, buf);
+  }
+
+  // (one row a group: its lanes agree)
+  __device__ __forceinline__ bool any(bool x) const { return x; }
+  // sum of e^(s - m) over the row in float64, from memory; buf: kBuf words
+  __device__ __forceinline__ double wide_sum(const ScoresView& s, int64_t i, float m,
+                                             double* buf) const {
+    const T* p = (const T*)s.data + i * s.rs;
+    double z = 0.0;
+    for (int32_t k = t; k < K; k += G) z += exp((double)to_f32(p[k]) - (double)m);
+    for (int o = (G < 64 ? G : 64) / 2; o; o >>= 1) z += __shfl_xor(z, o);
+    if (G <= 64) return z;
+    if ((threadIdx.x & 63) == 0) buf[threadIdx.x >> 6] = z;
+    __syncthreads();
+    z = 0.0;
+    for (int w = 0; w < kBuf; ++w) z += buf[w];
+    return z;
+  }
+
+  // out[cls(j)] (+)= f(j) for this thread's classes
+  template <typename F>
+  __device__ __forceinline__ void store(const ScoresView& o, int64_t i, bool accumulate, F f) const {
+    T* p = (T*)o.data + i * o.rs;
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+      const int32_t k = want(c), sk = skip(c), at = first(c);
+      if (sk >= VE) continue;
+      float x[VE];
+#pragma unroll
+      for (int e = 0; e < VE; ++e) x[e] = f(c * VE + e);
+      if (sk == 0) {
+        Chunk<T> v;
+        if (accumulate) {
+          const Chunk<T> old = load_chunk<T>(p + k);
+#pragma unroll
+          for (int e = 0; e < VE; ++e) x[e] += to_f32(old.v[e]);
+        }
+#pragma unroll
+        for (int e = 0; e < VE; ++e) v.v[e] = from_f32<T>(x[e]);
+        store_chunk<T>(p + k, v);
+      } else {
+#pragma unroll
+        for (int e = 0; e < VE; ++e)
+          if (e >= sk) p[at + e] = from_f32<T>(accumulate ? x[e] + to_f32(p[at + e]) : x[e]);
+      }
+    }
+  }
+  __device__ __forceinline__ void store_zero(const ScoresView& o, int64_t i) const {
+    store(o, i, false, [](int) { return 0.0f; });
+  }
+};
+
+// ---------------------------------------------------------------------------
+// ClassFrame: a thread per row and slice of its classes, the rows of a class
+// next to each other (one load instruction reads 64 rows of a class).  The
+// slices w = 0 .. S-1 are the waves of a workgroup; slice w holds the classes
+// w, w + S, ... (N of them).  With S = 1 a workgroup's waves hold rows of
+// their own; rows may then also be short and next to each other (any strides).
+// Classes past the last are read as the last one and set to -inf.
+// ---------------------------------------------------------------------------
+template <typename T_, int N_, bool SLICES>
+struct ClassFrame {
+  using T = T_;
+  static constexpr int N = N_;
+  static constexpr int kMax = SLICES ? 1024 : 256;
+  static constexpr bool kBarrier = SLICES, kSlices = SLICES;
+  static constexpr int kBuf = SLICES ? 16 * 64 : 1;
+  int32_t w, S, K;
+
+  __device__ __forceinline__ ClassFrame(const ScoresView& s)
+      : w(SLICES ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : 0),
+        S(SLICES ? blockDim.x >> 6 : 1),
+        K(s.K) {}
+  static __device__ __forceinline__ int64_t row(int64_t block) {
+    return SLICES ? block * 64 + (threadIdx.x & 63) : block * 256 + threadIdx.x;
+  }
+  __device__ __forceinline__ bool first_lane() const { return w == 0; }
+  __device__ __forceinline__ int32_t cls(int j) const { return w + j * S; }
+
+  struct Regs {
+    T c[N];
+  };
+  __device__ __forceinline__ void load(Regs& r, const ScoresView& s, int64_t i) const {
+    const T* p = (const T*)s.data + i * s.rs;
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      const int32_t k = cls(j) < K ? cls(j) : K - 1;
+      r.c[j] = p[k * s.ks];
+    }
+  }
+  __device__ __forceinline__ void trim(Regs& r) const {
+#pragma unroll
+    for (int j = 0; j < N; ++j) r.c[j] = cls(j) < K ? r.c[j] : (T)(-__builtin_inff());
+  }
+  static __device__ __forceinline__ float value(const Regs& r, int j) { return to_f32(r.c[j]); }
+
+  template <typename Op>
+  __device__ __forceinline__ float reduce(float x, Op op, float* buf) const {
+    if (!SLICES) return x;
+    const int lane = threadIdx.x & 63;
+    buf[w * 64 + lane] = x;
+    __syncthreads();
+    x = buf[lane];
+    for (int v = 1; v < S; ++v) x = op(x, buf[v * 64 + lane]);
+    return x;
+  }
+  // (the lanes of a workgroup's waves share rows: all go, or none)
+  __device__ __forceinline__ bool any(bool x) const { return SLICES ? __syncthreads_or(x) : x; }
+  __device__ __forceinline__ double wide_sum(const ScoresView& s, int64_t i, float m,
+                                             double* buf) const {
+    const T* p = (const T*)s.data + i * s.rs;
+    double z = 0.0;
+    for (int32_t k = w; k < K; k += S) z += exp((double)to_f32(p[k * s.ks]) - (double)m);
+    if (!SLICES) return z;
+    const int lane = threadIdx.x & 63;
+    buf[w * 64 + lane] = z;
+    __syncthreads();
+    z = 0.0;
+    for (int v = 0; v < S; ++v) z += buf[v * 64 + lane];
+    return z;
+  }
+  template <typename F>
+  __device__ __forceinline__ void store(const ScoresView& o, int64_t i, bool accumulate, F f) const {
+    T* p = (T*)o.data + i * o.rs;
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      if (cls(j) < K) {
+        T* q = p + cls(j) * o.ks;
+        const float x = f(j);
+        *q = from_f32<T>(accumulate ? x + to_f32(*q) : x);
+      }
+    }
+  }
+  __device__ __forceinline__ void store_zero(const ScoresView& o, int64_t i) const {
+    store(o, i, false, [](int) { return 0.0f; });
+  }
+};
+
+}  // namespace wgbm

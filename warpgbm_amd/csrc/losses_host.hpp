@@ -34,6 +34,17 @@ int class_log_probs(const ScoresView& s, const int32_t* label, const uint8_t* ma
 int class_log_probs_grad(const ScoresView& s, const int32_t* label, const float* norm,
                          const float* grad, const ScoresView& out, hipStream_t st);
 
+// rows that fit a thread group's registers, one launch (losses_rows_*.hip);
+// *done = false where they do not
+#define LOSS_ROWS(t)                                                                             \
+  int log_probs_rows_##t(const ScoresView& s, const int32_t* label, float* log_prob, float* norm, \
+                         hipStream_t st, bool* done);                                            \
+  int policy_rows_##t(const ScoresView& s, const ScoresView& ref, const PolicyRows& g,           \
+                      const ScoresView& out, bool accumulate, hipStream_t st, bool* done)
+LOSS_ROWS(f32);
+LOSS_ROWS(bf16);
+LOSS_ROWS(f16);
+
 size_t policy_workspace(int64_t n, int32_t K, bool cm);
 int policy_loss(const ScoresView& s, const ScoresView& ref, const PolicyRows& g,
                 const ScoresView& out, bool accumulate, void* ws, hipStream_t st);

@@ -1,0 +1,219 @@
+// Log-probabilities and the policy loss of rows held in registers: one launch
+// that reads the scores once and writes the gradient (losses_rows_*.hip).
+#pragma once
+#include "losses_frames.hpp"
+#include "losses_host.hpp"
+
+namespace wgbm {
+
+// a row's statistics from its registers (the label's score sa apart); buf:
+// five reductions' words
+template <typename F, bool REF>
+__device__ __forceinline__ RowStats frame_stats(const F& f, const typename F::Regs& s,
+                                                const typename F::Regs& r, int32_t label, float sa,
+                                                float (*buf)[F::kBuf]) {
+  RowStats a = empty_stats();
+#pragma unroll
+  for (int j = 0; j < F::N; ++j) a.m = fmaxf(a.m, F::value(s, j));
+  a.m = f.reduce(a.m, MaxF(), buf[0]);
+  const float ms = safe_max(a.m);
+  float mrs = 0.0f;
+  if (REF) {
+#pragma unroll
+    for (int j = 0; j < F::N; ++j) a.mr = fmaxf(a.mr, F::value(r, j));
+    a.mr = f.reduce(a.mr, MaxF(), buf[1]);
+    mrs = safe_max(a.mr);
+  }
+  // four sums a thread: shorter chains of additions, and fewer roundings
+  float z[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+  for (int j = 0; j < F::N; ++j) {
+    const float d = F::value(s, j) - ms, e = loss_expf(d);
+    z[j % 4] += f.cls(j) == label ? 0.0f : e;
+    if (REF) {
+      const float dr = F::value(r, j) - mrs;
+      a.zr += loss_expf(dr);
+      a.u += e == 0.0f ? 0.0f : e * (d - dr);
+    }
+  }
+  a.z = f.reduce((z[0] + z[1]) + (z[2] + z[3]), AddF(), buf[2]);
+  if (REF) {
+    a.zr = f.reduce(a.zr, AddF(), buf[3]);
+    a.u = f.reduce(a.u, AddF(), buf[4]);
+  }
+  a.za = label >= 0 ? loss_expf(sa - ms) : 0.0f;
+  return a;
+}
+
+template <typename T>
+__device__ __forceinline__ float score_at(const ScoresView& s, int64_t i, int32_t k) {
+  return to_f32(((const T*)s.data)[i * s.rs + k * s.ks]);
+}
+
+template <typename F>
+__global__ __launch_bounds__(F::kMax) void log_probs_frame_kernel(
+    ScoresView s, const int32_t* __restrict__ label, float* __restrict__ log_prob,
+    float2* __restrict__ norm) {
+  __shared__ float buf[3][F::kBuf];
+  const F f(s);
+  const int64_t row = F::row(blockIdx.x);
+  const bool in = row < s.n;
+  if (!F::kBarrier && !in) return;
+  const int64_t i = in ? row : s.n - 1;
+  typename F::Regs v;
+  f.load(v, s, i);
+  const int32_t lab = row_label(label, i, s.K);
+  const float sa = lab >= 0 ? score_at<typename F::T>(s, i, lab) : 0.0f;
+  f.trim(v);
+  const RowStats a = frame_stats<F, false>(f, v, v, lab, sa, buf);
+  if (!in || !f.first_lane()) return;
+  const LogProb lp = row_log_prob(a, sa);
+  log_prob[i] = lp.live && lab >= 0 ? (float)lp.logp : 0.0f;
+  norm[i] = lp.live ? make_float2(lp.m, (float)lp.l) : make_float2(-__builtin_inff(), 0.0f);
+}
+
+template <typename F, bool REF>
+__global__ __launch_bounds__(F::kMax) void policy_frame_kernel(ScoresView s, ScoresView ref,
+                                                               PolicyRows g, ScoresView out,
+                                                               bool accumulate) {
+  using T = typename F::T;
+  __shared__ float buf[5][F::kBuf];
+  __shared__ double wide[F::kBuf];
+  const F f(s);
+  const int64_t row = F::row(blockIdx.x);
+  const bool in = row < s.n;
+  if (!F::kBarrier && !in) return;
+  const int64_t i = in ? row : s.n - 1;
+  const float w = !in ? 0.0f : g.weight ? g.weight[i] : 1.0f;
+  const int32_t lab = row_label(g.action, i, s.K);
+  const bool live = w != 0.0f && lab >= 0;
+  // (a workgroup whose waves share rows goes on: other lanes' rows may be live)
+  if (!F::kSlices && !live) {
+    if (f.first_lane()) {
+      g.loss[i] = g.log_prob[i] = 0.0f;
+      if (g.kl) g.kl[i] = 0.0f;
+    }
+    if (out.data && !accumulate) f.store_zero(out, i);
+    return;
+  }
+  typename F::Regs v, r;
+  f.load(v, s, i);
+  if (REF) f.load(r, ref, i);
+  const int32_t a = lab >= 0 ? lab : 0;
+  const float sa = score_at<T>(s, i, a);
+  const float ra = REF ? score_at<T>(ref, i, a) : 0.0f;
+  const float A = g.advantage[i], old = g.old_log_prob[i];
+  f.trim(v);
+  if (REF) f.trim(r);
+  const RowStats st = frame_stats<F, REF>(f, v, r, lab, sa, buf);
+  PolicyRow o = policy_row<REF>(st, sa, ra, A, old, w, g, i, lab, nullptr);
+  if (f.any(o.near && live)) {
+    // next to a border: the row's sum again, in float64
+    const double z = f.wide_sum(s, i, o.c.m, wide);
+    const double logp = ((double)sa - (double)o.c.m) - log(z);
+    if (o.near) o = policy_row<REF>(st, sa, ra, A, old, w, g, i, lab, &logp);
+  }
+  if (F::kSlices && !live) {
+    o.loss = o.logp = o.kl = 0.0f;
+    o.c = RowCoef{};
+  }
+  if (in && f.first_lane()) {
+    g.loss[i] = o.loss;
+    g.log_prob[i] = o.logp;
+    if (g.kl) g.kl[i] = o.kl;
+  }
+  if (!in || !out.data) return;
+  if (!o.c.live || !live) {
+    if (!accumulate) f.store_zero(out, i);
+    return;
+  }
+  f.store(out, i, accumulate, [&](int j) {
+    const float x = coef_grad<REF>(o.c, F::value(v, j), REF ? F::value(r, j) : 0.0f);
+    return f.cls(j) == lab ? o.c.gl : x;
+  });
+}
+
+// ---------------------------------------------------------------------------
+// which frame a call takes: f(frame tag, workgroups, threads) for the smallest
+// one that holds the rows, false where none does
+// ---------------------------------------------------------------------------
+template <typename F>
+struct FrameTag {
+  using type = F;
+};
+
+// most 16-byte chunks of one matrix in a thread's registers: 16 (64 registers
+// of 128 that a workgroup of 1024 threads has), 8 with a second matrix
+template <typename T, bool REF, typename Fn>
+static bool pick_row_frame(const ScoresView& s, Fn fn) {
+  constexpr int VE = Chunk<T>::VE;
+  if (s.K < VE) return false;
+  const int64_t chunks = (s.K + VE - 1) / VE;
+  const auto go = [&](auto tag) {
+    using F = typename decltype(tag)::type;
+    fn(tag, (s.n + F::kRows - 1) / F::kRows, F::kThreads);
+    return true;
+  };
+  if (chunks <= 4) return go(FrameTag<RowFrame<T, 4, 1>>());
+  if (chunks <= 16) return go(FrameTag<RowFrame<T, 16, 1>>());
+  if (chunks <= 64) return go(FrameTag<RowFrame<T, 64, 1>>());
+  if (chunks <= 256) return go(FrameTag<RowFrame<T, 64, 4>>());
+  if (chunks <= 1024) return go(FrameTag<RowFrame<T, 256, 4>>());
+  if (chunks <= 2048) return go(FrameTag<RowFrame<T, 256, 8>>());
+  if (chunks <= 4096) return go(FrameTag<RowFrame<T, 1024, 4>>());
+  if (chunks <= 8192) return go(FrameTag<RowFrame<T, 1024, 8>>());
+  if (!REF && chunks <= 16384) return go(FrameTag<RowFrame<T, 1024, 16>>());
+  return false;
+}
+
+template <typename T, bool REF, typename Fn>
+static bool pick_class_frame(const ScoresView& s, Fn fn) {
+  const int64_t blocks = (s.n + 255) / 256;
+  if (s.K <= 4) return fn(FrameTag<ClassFrame<T, 4, false>>(), blocks, 256), true;
+  if (s.K <= 8) return fn(FrameTag<ClassFrame<T, 8, false>>(), blocks, 256), true;
+  if (s.K <= 12) return fn(FrameTag<ClassFrame<T, 12, false>>(), blocks, 256), true;
+  if (s.K <= 16) return fn(FrameTag<ClassFrame<T, 16, false>>(), blocks, 256), true;
+  // row-major rows come here only when they are short
+  const int64_t tiles = (s.n + 63) / 64;
+  if (s.K <= 256)
+    return fn(FrameTag<ClassFrame<T, 16, true>>(), tiles, 64 * (int)((s.K + 15) / 16)), true;
+  if (s.K <= 512)
+    return fn(FrameTag<ClassFrame<T, 32, true>>(), tiles, 64 * (int)((s.K + 31) / 32)), true;
+  return false;
+}
+
+// short rows next to each other are read by a thread each
+template <typename T>
+static bool by_class_frame(const ScoresView& s) {
+  return s.class_major() || s.K < Chunk<T>::VE;
+}
+
+template <typename T>
+static int log_probs_frames(const ScoresView& s, const int32_t* label, float* log_prob,
+                            float* norm, hipStream_t st, bool* done) {
+  const auto launch = [&](auto tag, int64_t blocks, int threads) {
+    using F = typename decltype(tag)::type;
+    hipLaunchKernelGGL((log_probs_frame_kernel<F>), dim3((unsigned)blocks), dim3(threads), 0, st, s,
+                       label, log_prob, (float2*)norm);
+  };
+  *done = by_class_frame<T>(s) ? pick_class_frame<T, false>(s, launch)
+                               : pick_row_frame<T, false>(s, launch);
+  if (*done) WGBM_LAUNCH_CHECK();
+  return 0;
+}
+
+template <typename T, bool REF>
+static int policy_frames(const ScoresView& s, const ScoresView& ref, const PolicyRows& g,
+                         const ScoresView& out, bool accumulate, hipStream_t st, bool* done) {
+  const auto launch = [&](auto tag, int64_t blocks, int threads) {
+    using F = typename decltype(tag)::type;
+    hipLaunchKernelGGL((policy_frame_kernel<F, REF>), dim3((unsigned)blocks), dim3(threads), 0, st,
+                       s, ref, g, out, accumulate);
+  };
+  *done = by_class_frame<T>(s) ? pick_class_frame<T, REF>(s, launch)
+                               : pick_row_frame<T, REF>(s, launch);
+  if (*done) WGBM_LAUNCH_CHECK();
+  return 0;
+}
+
+}  // namespace wgbm

@@ -1,0 +1,17 @@
+// Log-probabilities and the policy loss of rows in registers, _Float16 scores.
+#include "losses_rows.hpp"
+
+namespace wgbm {
+
+int log_probs_rows_f16(const ScoresView& s, const int32_t* label, float* log_prob, float* norm,
+                      hipStream_t st, bool* done) {
+  return log_probs_frames<_Float16>(s, label, log_prob, norm, st, done);
+}
+
+int policy_rows_f16(const ScoresView& s, const ScoresView& ref, const PolicyRows& g,
+                   const ScoresView& out, bool accumulate, hipStream_t st, bool* done) {
+  return ref.data ? policy_frames<_Float16, true>(s, ref, g, out, accumulate, st, done)
+                  : policy_frames<_Float16, false>(s, ref, g, out, accumulate, st, done);
+}
+
+}  // namespace wgbm
