@@ -136,7 +136,7 @@ int wgbm_policy_loss(const wgbm_scores* scores, const wgbm_policy_args* a, float
 int64_t wgbm_balance_loss_workspace(const wgbm_scores* scores) {
   ScoresView s;
   if (view_of(scores, "scores", &s)) return -1;
-  return (int64_t)balance_workspace(s.n, s.K, s.class_major());
+  return (int64_t)balance_workspace(s);
 }
 
 int wgbm_balance_loss(const wgbm_scores* scores, const uint8_t* mask, int32_t top_k, float coef,
@@ -154,7 +154,7 @@ int wgbm_balance_loss(const wgbm_scores* scores, const uint8_t* mask, int32_t to
                "balance_loss: top_k must be in [1, min(%d, n_classes)], got %d", kMaxTopK, top_k);
   WGBM_REQUIRE(std::isfinite(coef), "balance_loss: coef must be finite");
   WGBM_REQUIRE(loss && counts && prob && workspace, "balance_loss: null pointer");
-  WGBM_REQUIRE(workspace_bytes >= (int64_t)balance_workspace(s.n, s.K, s.class_major()),
+  WGBM_REQUIRE(workspace_bytes >= (int64_t)balance_workspace(s),
                "balance_loss: workspace too small");
   return balance_loss(s, mask, top_k, coef, BalanceOut{loss, counts, prob}, g, accumulate != 0,
                       workspace, S(stream));

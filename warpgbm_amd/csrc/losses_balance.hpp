@@ -1,0 +1,202 @@
+// The balance loss: how evenly rows fall on classes.
+//   c_k = rows with class k among their top_k, f_k = c_k / (n' top_k),
+//   P_k = mean of p_ik over the n' rows that count,
+//   L = coef K sum_k f_k P_k,   dL/ds_ik = coef K / n' p_ik (f_k - sum_j f_j p_ij)
+// (the counts are held constant).  The gradient needs every row's counts
+// first, so the scores are read twice: rows in registers (losses_frames.hpp)
+// give the counts, the sums of p and each row's norm; a finishing launch the
+// shares; rows in registers again the gradient.  Workgroups take rows in turn
+// and leave one partial sum a class, which the finishing launch joins in
+// float64 in workgroup order: results do not depend on the order of execution.
+#pragma once
+#include <algorithm>
+
+#include "losses_frames.hpp"
+#include "losses_host.hpp"
+
+namespace wgbm {
+
+struct MinF {
+  __device__ __forceinline__ float operator()(float a, float b) const { return fminf(a, b); }
+};
+
+// part, count: [workgroups][K] (count: [workgroups][K + 1], the last the rows
+// that count); norm: a row's maximum and 1 / sum of e^(s - max) (0: left out)
+template <typename F>
+__global__ __launch_bounds__(F::kMax) void balance_stats_kernel(
+    ScoresView s, const uint8_t* __restrict__ mask, int32_t top_k, int64_t blocks,
+    float* __restrict__ part, int32_t* __restrict__ count, float2* __restrict__ norm,
+    uint32_t* __restrict__ ticket) {
+  extern __shared__ int32_t s_count[];  // [K + 1], then [K] floats
+  __shared__ float buf[4][F::kBuf];
+  const int32_t K = s.K;
+  float* s_part = (float*)(s_count + K + 1);
+  if (blockIdx.x == 0 && threadIdx.x == 0) *ticket = 0;
+  for (int32_t k = threadIdx.x; k <= K; k += blockDim.x) s_count[k] = 0;
+  __syncthreads();
+  const F f(s);
+  float acc[F::N];
+#pragma unroll
+  for (int j = 0; j < F::N; ++j) acc[j] = 0.0f;
+  for (int64_t b = blockIdx.x; b < blocks; b += gridDim.x) {
+    const int64_t row = F::row(b);
+    const bool in = row < s.n;
+    const int64_t i = in ? row : s.n - 1;
+    const bool want = in && (!mask || mask[i]);
+    typename F::Regs v;
+    f.load(v, s, i);
+    f.trim(v);
+    float m = -__builtin_inff();
+#pragma unroll
+    for (int j = 0; j < F::N; ++j) m = fmaxf(m, F::value(v, j));
+    m = f.reduce(m, MaxF(), buf[0]);
+    const float ms = safe_max(m);
+    float e[F::N], z = 0.0f;
+#pragma unroll
+    for (int j = 0; j < F::N; ++j) {
+      e[j] = loss_expf(F::value(v, j) - ms);
+      z += e[j];
+    }
+    z = f.reduce(z, AddF(), buf[1]);
+    const bool live = want && !(z == 0.0f);
+    const float iz = live ? 1.0f / z : 0.0f;
+#pragma unroll
+    for (int j = 0; j < F::N; ++j) acc[j] += live ? e[j] * iz : 0.0f;
+    if (in && f.first_lane()) norm[i] = make_float2(ms, iz);
+    // the best classes one after the other: the largest score after the last
+    // one taken, then the lowest class that has it.  (class numbers are exact
+    // in float32; a NaN is not after anything)
+    float v0 = __builtin_inff(), c0 = -1.0f;
+    for (int32_t t = 0; t < top_k; ++t) {
+      float best = m;
+      if (t > 0) {
+        best = -__builtin_inff();
+#pragma unroll
+        for (int j = 0; j < F::N; ++j) {
+          const float x = F::value(v, j);
+          if (x < v0 || (x == v0 && (float)f.cls(j) > c0)) best = fmaxf(best, x);
+        }
+        best = f.reduce(best, MaxF(), buf[2]);
+      }
+      float c = 1e9f;
+#pragma unroll
+      for (int j = 0; j < F::N; ++j) {
+        const float k = (float)f.cls(j);
+        if (F::value(v, j) == best && (best < v0 || k > c0)) c = fminf(c, k);
+      }
+      c = f.reduce(c, MinF(), buf[3]);
+      const bool took = live && best > -__builtin_inff() && c < 1e9f;
+      if (took && f.first_lane()) atomicAdd(&s_count[(int32_t)c], 1);
+      v0 = best;
+      c0 = c;
+    }
+    if (live && f.first_lane()) atomicAdd(&s_count[K], 1);
+  }
+  f.sum_rows(acc, s_part);
+  __syncthreads();
+  for (int32_t k = threadIdx.x; k <= K; k += blockDim.x) {
+    if (k < K) part[(int64_t)blockIdx.x * K + k] = s_part[k];
+    count[(int64_t)blockIdx.x * (K + 1) + k] = s_count[k];
+  }
+}
+
+// the shares as a thread's classes need them
+template <typename F>
+__global__ __launch_bounds__(F::kMax) void balance_grad_kernel(
+    ScoresView s, const float2* __restrict__ norm, const float* __restrict__ share,
+    const float* __restrict__ scale, int64_t blocks, bool accumulate, ScoresView out) {
+  __shared__ float buf[2][F::kBuf];
+  const F f(s);
+  float fk[F::N];
+#pragma unroll
+  for (int j = 0; j < F::N; ++j) fk[j] = share[f.cls(j) < s.K ? f.cls(j) : s.K - 1];
+  const float c = *scale;
+  int turn = 0;
+  for (int64_t b = blockIdx.x; b < blocks; b += gridDim.x, turn ^= 1) {
+    const int64_t row = F::row(b);
+    const bool in = row < s.n;
+    const int64_t i = in ? row : s.n - 1;
+    const float2 nm = norm[i];
+    typename F::Regs v;
+    f.load(v, s, i);
+    f.trim(v);
+    const bool live = in && nm.y != 0.0f;  // (NaN is live)
+    float q = 0.0f;
+#pragma unroll
+    for (int j = 0; j < F::N; ++j)
+      q = fmaf(fk[j], loss_expf(F::value(v, j) - nm.x), q);
+    // (two turns' words: a wave may be one reduction ahead of the others)
+    q = f.reduce(q, AddF(), buf[turn]) * nm.y;
+    if (!in) continue;
+    if (!live) {
+      if (!accumulate) f.store_zero(out, i);
+      continue;
+    }
+    const float cz = c * nm.y;
+    f.store(out, i, accumulate, [&](int j) {
+      return cz * loss_expf(F::value(v, j) - nm.x) * (fk[j] - q);
+    });
+  }
+}
+
+// the frames of up to 4096 classes: f(frame tag, blocks of rows, threads)
+template <typename T, typename Fn>
+static void balance_frame(const ScoresView& s, Fn fn) {
+  if (s.class_major() || s.K < Chunk<T>::VE) {
+    const int64_t rows = (s.n + 255) / 256, tiles = (s.n + 63) / 64;
+    if (s.K <= 4) return fn(FrameTag<ClassFrame<T, 4, false>>(), rows, 256);
+    if (s.K <= 8) return fn(FrameTag<ClassFrame<T, 8, false>>(), rows, 256);
+    if (s.K <= 12) return fn(FrameTag<ClassFrame<T, 12, false>>(), rows, 256);
+    if (s.K <= 16) return fn(FrameTag<ClassFrame<T, 16, false>>(), rows, 256);
+    if (s.K <= 256)
+      return fn(FrameTag<ClassFrame<T, 16, true>>(), tiles, 64 * (int)((s.K + 15) / 16));
+    return fn(FrameTag<ClassFrame<T, 32, true>>(), tiles, 64 * (int)((s.K + 31) / 32));
+  }
+  const int64_t chunks = (s.K + Chunk<T>::VE - 1) / Chunk<T>::VE;
+  const auto go = [&](auto tag) {
+    using F = typename decltype(tag)::type;
+    fn(tag, (s.n + F::kRows - 1) / F::kRows, F::kThreads);
+  };
+  if (chunks <= 4) return go(FrameTag<RowFrame<T, 4, 1>>());
+  if (chunks <= 16) return go(FrameTag<RowFrame<T, 16, 1>>());
+  if (chunks <= 64) return go(FrameTag<RowFrame<T, 64, 1>>());
+  if (chunks <= 256) return go(FrameTag<RowFrame<T, 64, 4>>());
+  return go(FrameTag<RowFrame<T, 256, 4>>());
+}
+
+// workgroups of the two passes: 16 waves a CU, and fewer partial sums where
+// there are many classes
+static inline int64_t balance_groups(int64_t blocks, int threads, int32_t K) {
+  const int64_t fill = kLossWaves * 64 / threads;
+  const int64_t few = std::max<int64_t>(512, (int64_t(1) << 20) / K);
+  return std::min(blocks, std::min(fill, few));
+}
+
+template <typename T>
+int balance_stats(const ScoresView& s, const uint8_t* mask, int32_t top_k, const BalanceWs& w,
+                  int32_t* groups, hipStream_t st) {
+  balance_frame<T>(s, [&](auto tag, int64_t blocks, int threads) {
+    using F = typename decltype(tag)::type;
+    *groups = (int32_t)balance_groups(blocks, threads, s.K);
+    hipLaunchKernelGGL((balance_stats_kernel<F>), dim3((unsigned)*groups), dim3(threads),
+                       (2 * (size_t)s.K + 1) * 4, st, s, mask, top_k, blocks, w.part, w.count,
+                       w.norm, w.ticket);
+  });
+  WGBM_LAUNCH_CHECK();
+  return 0;
+}
+
+template <typename T>
+int balance_grad(const ScoresView& s, const BalanceWs& w, const ScoresView& out, bool accumulate,
+                 hipStream_t st) {
+  balance_frame<T>(s, [&](auto tag, int64_t blocks, int threads) {
+    using F = typename decltype(tag)::type;
+    const int64_t groups = std::min<int64_t>(blocks, kLossWaves * 64 / threads);
+    hipLaunchKernelGGL((balance_grad_kernel<F>), dim3((unsigned)groups), dim3(threads), 0, st, s,
+                       w.norm, w.share, w.scale, blocks, accumulate, out);
+  });
+  WGBM_LAUNCH_CHECK();
+  return 0;
+}
+
+}  // namespace wgbm

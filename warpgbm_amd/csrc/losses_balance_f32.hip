@@ -1,0 +1,16 @@
+// The balance loss's passes over the rows, float scores.
+#include "losses_balance.hpp"
+
+namespace wgbm {
+
+int balance_stats_f32(const ScoresView& s, const uint8_t* mask, int32_t top_k, const BalanceWs& w,
+                     int32_t* groups, hipStream_t st) {
+  return balance_stats<float>(s, mask, top_k, w, groups, st);
+}
+
+int balance_grad_f32(const ScoresView& s, const BalanceWs& w, const ScoresView& out,
+                    bool accumulate, hipStream_t st) {
+  return balance_grad<float>(s, w, out, accumulate, st);
+}
+
+}  // namespace wgbm

@@ -71,6 +71,12 @@ __device__ __forceinline__ float waves_reduce(float x, Op op, float* buf) {
   return x;
 }
 
+// a frame as a value, for the functions that pick one
+template <typename F>
+struct FrameTag {
+  using type = F;
+};
+
 // ---------------------------------------------------------------------------
 // RowFrame: classes next to each other.  G threads share a row; thread t holds
 // the chunks t, t + G, ... (NC of them): classes (c * G + t) * VE .. + VE.
@@ -134,6 +140,25 @@ struct RowFrame {
     return waves_reduce<(G > 64 ? G / 64 : 1)>(x, op, buf);
   }
 
+  // sum[k] = the workgroup's sum of acc over its rows, for every class.  Lanes
+  // at the same place in their groups first, then the waves one after the
+  // other: the same order every time.
+  __device__ __forceinline__ void sum_rows(float (&acc)[N], float* sum) const {
+    if (G < 64) {
+#pragma unroll
+      for (int j = 0; j < N; ++j)
+        for (int o = G; o < 64; o <<= 1) acc[j] += __shfl_xor(acc[j], o);
+    }
+    constexpr int kTurns = G <= 64 ? kThreads / 64 : 1;  // waves that hold the same classes
+    for (int w = 0; w < kTurns; ++w) {
+      if (G > 64 || ((int)(threadIdx.x >> 6) == w && (threadIdx.x & 63) < (G < 64 ? G : 64))) {
+#pragma unroll
+        for (int j = 0; j < N; ++j)
+          if (j % VE >= skip(j / VE)) sum[cls(j)] = w ? sum[cls(j)] + acc[j] : acc[j];
+      }
+      __syncthreads();
+    }
+  }
   // (one row a group: its lanes agree)
   __device__ __forceinline__ bool any(bool x) const { return x; }
   // sum of e^(s - m) over the row in float64, from memory; buf: kBuf words
@@ -237,6 +262,20 @@ struct ClassFrame {
     x = buf[lane];
     for (int v = 1; v < S; ++v) x = op(x, buf[v * 64 + lane]);
     return x;
+  }
+  // sum[k] = the workgroup's sum of acc over its rows, for every class
+  __device__ __forceinline__ void sum_rows(float (&acc)[N], float* sum) const {
+#pragma unroll
+    for (int j = 0; j < N; ++j) acc[j] = lanes_reduce<64>(acc[j], AddF());
+    const int kTurns = SLICES ? 1 : 4;
+    for (int u = 0; u < kTurns; ++u) {
+      if ((SLICES || (int)(threadIdx.x >> 6) == u) && (threadIdx.x & 63) == 0) {
+#pragma unroll
+        for (int j = 0; j < N; ++j)
+          if (cls(j) < K) sum[cls(j)] = u ? sum[cls(j)] + acc[j] : acc[j];
+      }
+      __syncthreads();
+    }
   }
   // (the lanes of a workgroup's waves share rows: all go, or none)
   __device__ __forceinline__ bool any(bool x) const { return SLICES ? __syncthreads_or(x) : x; }

@@ -54,7 +54,27 @@ struct BalanceOut {
   int64_t* counts;
   float* prob;
 };
-size_t balance_workspace(int64_t n, int32_t K, bool cm);
+// working memory of a balance loss
+struct BalanceWs {
+  uint32_t* ticket;
+  float* scale;
+  float* share;       // [K]
+  double* loss_part;  // [K / 16 + 1]
+  float2* norm;       // [n]
+  float* part;        // [workgroups][K]
+  int32_t* count;     // [workgroups][K + 1]
+  void* rows;         // a row-major copy of the scores, where one is needed
+  size_t bytes;
+};
+#define LOSS_BALANCE(t)                                                                          \
+  int balance_stats_##t(const ScoresView& s, const uint8_t* mask, int32_t top_k,                 \
+                        const BalanceWs& w, int32_t* groups, hipStream_t st);                    \
+  int balance_grad_##t(const ScoresView& s, const BalanceWs& w, const ScoresView& out,           \
+                       bool accumulate, hipStream_t st)
+LOSS_BALANCE(f32);
+LOSS_BALANCE(bf16);
+LOSS_BALANCE(f16);
+size_t balance_workspace(const ScoresView& s);
 int balance_loss(const ScoresView& s, const uint8_t* mask, int32_t top_k, float coef,
                  const BalanceOut& o, const ScoresView& out, bool accumulate, void* ws,
                  hipStream_t st);

@@ -137,11 +137,6 @@ __global__ __launch_bounds__(F::kMax) void policy_frame_kernel(ScoresView s, Sco
 // which frame a call takes: f(frame tag, workgroups, threads) for the smallest
 // one that holds the rows, false where none does
 // ---------------------------------------------------------------------------
-template <typename F>
-struct FrameTag {
-  using type = F;
-};
-
 // most 16-byte chunks of one matrix in a thread's registers: 16 (64 registers
 // of 128 that a workgroup of 1024 threads has), 8 with a second matrix
 template <typename T, bool REF, typename Fn>
