@@ -358,8 +358,8 @@ typedef struct wgbm_engine_config {
   int32_t num_bins;           /* 2..127 */
   int32_t num_eras;
   int32_t max_depth;
-  int32_t n_trees;            /* 1 (regression) or K (softmax) */
-  int32_t objective;          /* 0 regression, 1 softmax */
+  int32_t n_trees;            /* 1 (regression), K (softmax), any (gradients) */
+  int32_t objective;          /* 0 regression, 1 softmax, 2 gradients given */
   float min_child_weight;
   float min_split_gain;
   float l2_reg;
@@ -392,10 +392,11 @@ typedef struct wgbm_tree_record {
 
 int wgbm_engine_create(wgbm_engine** out, const wgbm_engine_config* cfg);
 /* One boosting round.  target: float32 y [n_rows] (regression) or int32
- * labels [n_rows] (softmax); pred: float32 [n_rows] (regression) or
- * class-major [K, n_rows] (softmax: the scores of class k are row k, so each
- * class tree's leaf updates stay inside one row), updated in place;
- * feat_sel: int32 [n_sel] features of this round's trees (colsample_bytree
+ * labels [n_rows] (softmax) or float32 gradients [n_trees, n_rows] of a loss,
+ * to whose negative the trees are fitted (objective 2); pred: float32 [n_rows]
+ * (regression) or class-major [n_trees, n_rows] (softmax, gradients: the
+ * scores of class k are row k, so each class tree's leaf updates stay inside
+ * one row), updated in place; feat_sel: int32 [n_sel] features of this round's trees (colsample_bytree
  * subset, local order). */
 int wgbm_engine_round(wgbm_engine* eng, const void* target, float* pred, const int32_t* feat_sel,
                       int32_t n_sel, const wgbm_tree_record* rec, void* stream);

@@ -14,6 +14,13 @@ sequence, with no host synchronisation inside a round, instead of the
 reference's recursive per-node Python loop.  The trees are the same: the
 residual is fixed per tree (core.py:719), each node's decision depends only
 on its own rows, and histogram sums are exact (see include/warpgbm_amd.h).
+
+Three objectives have no counterpart in the reference; their rounds fit the
+trees to the negative gradient of a loss of ``warpgbm_amd.losses``:
+``"preference"`` (a scorer from pairs of rows or of sequences of rows),
+``"policy"`` (class probabilities from logged decisions and their advantages:
+the clipped policy loss with a KL and a balance term) and
+``"policy_preference"`` (class probabilities from pairs of decision sequences).
 """
 from __future__ import annotations
 
@@ -28,8 +35,17 @@ import os
 import time
 
 from . import device as D
+from . import losses as L
 from . import node_kernel
 from .metrics import accuracy_torch, log_loss_torch, rmsle_torch, softmax
+
+# objectives whose rounds fit one tree to one score a row, and those that fit a
+# tree a class
+_SCORE_OBJECTIVES = ("regression", "preference")
+_CLASS_OBJECTIVES = ("multiclass", "binary", "policy", "policy_preference")
+# objectives whose gradients come from warpgbm_amd.losses
+_LOSS_OBJECTIVES = ("preference", "policy", "policy_preference")
+_LOSS_PARAMS = ("beta", "label_smoothing", "clip", "kl_coef", "balance_coef", "balance_top_k")
 
 _TIMING = os.environ.get("WGBM_TIMING", "") not in ("", "0")
 # predict inputs from this many rows on read only the forest's split columns
@@ -232,6 +248,12 @@ class WarpGBM(BaseEstimator, RegressorMixin):
         colsample_bytree=1.0,
         random_state=None,
         warm_start=False,
+        beta=1.0,
+        label_smoothing=0.0,
+        clip=(0.2, 0.2),
+        kl_coef=0.0,
+        balance_coef=0.0,
+        balance_top_k=1,
     ):
         self._validate_hyperparams(
             objective=objective,
@@ -246,6 +268,8 @@ class WarpGBM(BaseEstimator, RegressorMixin):
             L2_reg=L2_reg,
             colsample_bytree=colsample_bytree,
         )
+        self._validate_loss_params(beta, label_smoothing, clip, kl_coef, balance_coef,
+                                   balance_top_k)
         self.objective = objective
         self.num_bins = num_bins
         self.max_depth = max_depth
@@ -262,6 +286,14 @@ class WarpGBM(BaseEstimator, RegressorMixin):
         self.colsample_bytree = colsample_bytree
         self.random_state = random_state
         self.warm_start = warm_start
+        # of the objectives "preference" and "policy_preference"
+        self.beta = beta
+        self.label_smoothing = label_smoothing
+        # of the objective "policy"
+        self.clip = clip
+        self.kl_coef = kl_coef
+        self.balance_coef = balance_coef
+        self.balance_top_k = balance_top_k
         self.forest = [{} for _ in range(self.n_estimators)]
         self.bin_edges = None
         self.base_prediction = None
@@ -281,9 +313,10 @@ class WarpGBM(BaseEstimator, RegressorMixin):
     # ------------------------------------------------------------------ validation
     def _validate_hyperparams(self, **kwargs):
         """Same checks and messages as warpgbm/core.py:83-143."""
-        if kwargs["objective"] not in ["regression", "multiclass", "binary"]:
+        if kwargs["objective"] not in _SCORE_OBJECTIVES + _CLASS_OBJECTIVES:
             raise ValueError(
-                f"objective must be 'regression', 'binary', or 'multiclass', got {kwargs['objective']}."
+                "objective must be 'regression', 'binary', 'multiclass', 'preference', 'policy', or "
+                f"'policy_preference', got {kwargs['objective']}."
             )
         int_params = ["num_bins", "max_depth", "n_estimators", "min_child_weight",
                       "threads_per_block", "rows_per_thread"]
@@ -316,6 +349,28 @@ class WarpGBM(BaseEstimator, RegressorMixin):
             raise ValueError(
                 f"Invalid colsample_bytree: {kwargs['colsample_bytree']}. Must be a float value > 0 and <= 1."
             )
+
+    @staticmethod
+    def _validate_loss_params(beta, label_smoothing, clip, kl_coef, balance_coef, balance_top_k):
+        for name, v in (("beta", beta), ("label_smoothing", label_smoothing),
+                        ("kl_coef", kl_coef), ("balance_coef", balance_coef)):
+            if not isinstance(v, (float, int)):
+                raise TypeError(f"{name} must be a float, got {type(v)}.")
+        if not (isinstance(clip, (tuple, list)) and len(clip) == 2
+                and all(isinstance(c, (float, int)) for c in clip)):
+            raise TypeError(f"clip must be a pair of floats, got {clip!r}.")
+        if not isinstance(balance_top_k, int):
+            raise TypeError(f"balance_top_k must be an integer, got {type(balance_top_k)}.")
+        if not (0 < beta < float("inf")):
+            raise ValueError("beta must be positive and finite.")
+        if not (0 <= label_smoothing <= 0.5):
+            raise ValueError("label_smoothing must be in [0, 0.5].")
+        if not (0 <= clip[0] <= 1 and 0 <= clip[1] < float("inf")):
+            raise ValueError("clip must be (low in [0, 1], high non-negative and finite).")
+        if not (0 <= kl_coef < float("inf")) or not (0 <= balance_coef < float("inf")):
+            raise ValueError("kl_coef and balance_coef must be non-negative and finite.")
+        if not (1 <= balance_top_k <= 8):
+            raise ValueError("balance_top_k must be between 1 and 8 inclusive.")
 
     def validate_fit_params(self, X, y, era_id, X_eval, y_eval, eval_every_n_trees,
                             early_stopping_rounds, eval_metric):
@@ -367,9 +422,36 @@ class WarpGBM(BaseEstimator, RegressorMixin):
 
     # ------------------------------------------------------------------ fit
     def fit(self, X, y, era_id=None, X_eval=None, y_eval=None, eval_every_n_trees=None,
-            early_stopping_rounds=None, eval_metric="mse"):
+            early_stopping_rounds=None, eval_metric="mse", *, pairs=None, segments=None,
+            pair_weight=None, advantage=None, behavior_log_prob=None, reference=None,
+            sample_weight=None):
+        """Train.  The arguments after ``eval_metric`` belong to the objectives
+        without a counterpart in the reference:
+
+        ``"preference"``: y holds the rows' reference scores (zeros where there
+        are none); ``pairs`` [P, 2] integers (preferred, other) are rows, or
+        sequences of rows with ``segments`` (offsets [S + 1]); ``pair_weight``
+        [P].  Scores start at 0 and ``predict`` returns them.
+
+        ``"policy"``: y holds the decisions taken, ``advantage`` [n] how much
+        better each was than expected, ``behavior_log_prob`` [n] its
+        log-probability when it was taken (None: uniform), ``reference`` the
+        policy not to leave too far (log-probabilities [n] of the decisions, or
+        scores [n, K] of all classes, which count by ``kl_coef``),
+        ``sample_weight`` [n] (0: left out).  ``balance_coef`` adds the balance
+        loss over the ``balance_top_k`` best classes of a row.
+
+        ``"policy_preference"``: y holds the decisions, ``pairs`` / ``segments``
+        / ``pair_weight`` as above, ``reference`` [n] the decisions' reference
+        log-probabilities.  Policies start uniform.
+
+        ``training_loss`` then has each round's mean loss before its trees."""
         early_stopping_rounds = self.validate_fit_params(
             X, y, era_id, X_eval, y_eval, eval_every_n_trees, early_stopping_rounds, eval_metric)
+        given = dict(pairs=pairs, segments=segments, pair_weight=pair_weight, advantage=advantage,
+                     behavior_log_prob=behavior_log_prob, reference=reference,
+                     sample_weight=sample_weight)
+        self._validate_loss_inputs(X.shape[0], given, X_eval)
         # random_state seeds the global RNGs as the reference does
         # (warpgbm/core.py:308-314); colsample_bytree subsets are then drawn
         # with torch.randperm on the device (core.py:722, 778)
@@ -395,6 +477,11 @@ class WarpGBM(BaseEstimator, RegressorMixin):
         self._subsets_dev = []
         self._phases = _Phases()
         try:
+            if self.objective in _LOSS_OBJECTIVES:
+                if self.objective in _CLASS_OBJECTIVES:
+                    y = self._encode_labels(y, refit=fresh)
+                    self._check_class_count()
+                return self._fit_losses(X, y, era_id, given)
             if self.objective in ("multiclass", "binary"):
                 y_encoded = self._encode_labels(y, refit=fresh)
                 self._check_class_count()
@@ -413,7 +500,8 @@ class WarpGBM(BaseEstimator, RegressorMixin):
         """A fresh fit: no trees, no loss history (warpgbm/core.py:317-324)."""
         self._is_fitted = False
         self._trees_trained = 0
-        self.forest = [{} for _ in range(self.n_estimators)] if self.objective == "regression" else []
+        self.forest = ([{} for _ in range(self.n_estimators)]
+                       if self.objective in _SCORE_OBJECTIVES else [])
         self.training_loss = []
         self.eval_loss = []
 
@@ -430,8 +518,8 @@ class WarpGBM(BaseEstimator, RegressorMixin):
         K = self.num_classes
         if self.objective == "binary" and K != 2:
             raise ValueError(f"binary objective requires exactly 2 classes, got {K}")
-        if self.objective == "multiclass" and K < 2:
-            raise ValueError(f"multiclass objective requires at least 2 classes, got {K}")
+        if self.objective != "binary" and K < 2:
+            raise ValueError(f"{self.objective} objective requires at least 2 classes, got {K}")
 
     def preprocess_gpu_data(self, X_np, Y_np, era_id_np):
         """Codes, era layout and targets on the device (warpgbm/core.py:487-541)."""
@@ -685,6 +773,174 @@ class WarpGBM(BaseEstimator, RegressorMixin):
         del codes
         return self
 
+    # ------------------------------------------------------------------ losses with gradients
+    def _validate_loss_inputs(self, n, given, X_eval):
+        """The arguments of the objectives of warpgbm_amd.losses (host arrays)."""
+        takes = {"preference": ("pairs", "segments", "pair_weight"),
+                 "policy": ("advantage", "behavior_log_prob", "reference", "sample_weight"),
+                 "policy_preference": ("pairs", "segments", "pair_weight", "reference"),
+                 }.get(self.objective, ())
+        needs = {"preference": "pairs", "policy": "advantage", "policy_preference": "pairs"}
+        for name, a in given.items():
+            if a is not None and name not in takes:
+                raise ValueError(f"{name} is not an argument of the objective '{self.objective}'.")
+            if a is not None and not isinstance(a, np.ndarray):
+                raise TypeError(f"{name} must be a numpy array.")
+        if self.objective not in _LOSS_OBJECTIVES:
+            return
+        if given[needs[self.objective]] is None:
+            raise ValueError(f"objective '{self.objective}' needs {needs[self.objective]}.")
+        if X_eval is not None:
+            raise ValueError(f"objective '{self.objective}' takes no eval set.")
+        for name in ("advantage", "behavior_log_prob", "sample_weight"):
+            if given[name] is not None and given[name].shape != (n,):
+                raise ValueError(f"{name} must have shape ({n},), got {given[name].shape}.")
+        ref = given["reference"]
+        if ref is not None and ref.shape != (n,) and not (
+                self.objective == "policy" and ref.ndim == 2 and ref.shape[0] == n):
+            raise ValueError(f"reference must have one entry per row ({n}), got {ref.shape}.")
+        pairs, seg, w = given["pairs"], given["segments"], given["pair_weight"]
+        if pairs is not None:
+            if pairs.ndim != 2 or pairs.shape[1] != 2 or pairs.shape[0] < 1:
+                raise ValueError(f"pairs must have shape (P, 2) with P >= 1, got {pairs.shape}.")
+            if not np.issubdtype(pairs.dtype, np.integer):
+                raise TypeError(f"pairs must be integers, got {pairs.dtype}.")
+            S = n
+            if seg is not None:
+                if seg.ndim != 1 or len(seg) < 1 or not np.issubdtype(seg.dtype, np.integer):
+                    raise ValueError("segments must be integer offsets [S + 1].")
+                if seg[0] != 0 or seg[-1] > n or np.any(seg[1:] < seg[:-1]):
+                    raise ValueError(f"segments must ascend from 0 to at most {n}.")
+                S = len(seg) - 1
+            if pairs.min() < 0 or pairs.max() >= S:
+                raise ValueError(f"pairs must hold numbers in [0, {S}).")
+            if w is not None and w.shape != (pairs.shape[0],):
+                raise ValueError(f"pair_weight must have shape ({pairs.shape[0]},), got {w.shape}.")
+
+    def _round_losses(self, given, y, scores, dev):
+        """A function of no arguments that computes one round's gradient at the
+        current scores ([n], or class-major [K, n] for class objectives) and the
+        losses' sum (a 0-dim device tensor), and the weight that makes it a
+        mean."""
+        def rows(a):
+            return None if a is None else torch.from_numpy(
+                np.ascontiguousarray(a, dtype=np.float32)).to(dev)
+
+        n, K = self.num_samples, self.num_classes
+        if self.objective == "policy":
+            actions = torch.from_numpy(np.asarray(y).astype(np.int32)).to(dev)
+            adv, w = rows(given["advantage"]), rows(given["sample_weight"])
+            old = rows(given["behavior_log_prob"])
+            if old is None:
+                old = torch.full((n,), -np.log(K), dtype=torch.float32, device=dev)
+            ref = given["reference"]
+            if ref is not None and ref.ndim == 2 and ref.shape[1] != K:
+                raise ValueError(f"reference must have a column per class ({K}), got {ref.shape}.")
+            ref_lp = rows(ref) if ref is not None and ref.ndim == 1 else None
+            ref_s = rows(ref.T).t() if ref is not None and ref.ndim == 2 else None
+            live = None if w is None else w != 0
+            count = n if w is None else int(live.sum())
+            total = float(n) if w is None else float(w.double().sum())
+            view = scores.t()
+
+            def step():
+                r = L.policy_loss(view, actions, old, adv, weight=w, ref_log_prob=ref_lp,
+                                  ref_scores=ref_s, clip=self.clip, kl_coef=self.kl_coef)
+                loss = r.loss.sum()
+                if self.balance_coef:
+                    e = L.balance_loss(view, top_k=min(self.balance_top_k, K), mask=live,
+                                       coef=self.balance_coef * count, grad=r.grad)
+                    loss = loss + e.loss
+                return r.grad, loss
+
+            return step, total
+        plan = L.PreferencePlan(given["pairs"].astype(np.int64), n, device=dev,
+                                segments=None if given["segments"] is None
+                                else given["segments"].astype(np.int64))
+        w = rows(given["pair_weight"])
+        total = float(plan.n_pairs) if w is None else float(w.double().sum())
+        how = dict(weight=w, beta=self.beta, label_smoothing=self.label_smoothing)
+        if self.objective == "preference":
+            ref = rows(y)
+
+            def step():
+                r = L.preference_loss(scores, plan, ref_log_prob=ref, **how)
+                return r.grad, r.loss.sum()
+
+            return step, total
+        actions = torch.from_numpy(np.asarray(y).astype(np.int32)).to(dev)
+        ref, view = rows(given["reference"]), scores.t()
+
+        def step():
+            f = L.class_log_probs(view, actions)
+            r = L.preference_loss(f.log_prob, plan, ref_log_prob=ref, **how)
+            return L.class_log_probs_grad(view, actions, f.norm, r.grad), r.loss.sum()
+
+        return step, total
+
+    def _fit_losses(self, X, y, era_id, given):
+        """Rounds of the objectives of warpgbm_amd.losses: the gradient at the
+        current scores, then a tree a score column fitted to its negative (the
+        engine's objective 2)."""
+        dev = torch.device(self.device)
+        classes = self.objective in _CLASS_OBJECTIVES
+        codes, root_order, era_start, self.bin_edges, _ = self.preprocess_gpu_data(X, y, era_id)
+        self.base_prediction = 0.0
+        start_iter = self._trees_trained if (self.warm_start and self._is_fitted) else 0
+        n = self.num_samples
+        if classes:
+            K = self.num_classes
+            if start_iter > 0:
+                rows = D.rows_of(self._uniform_prior_logits(), n, dev)
+                self._predict_codes_into(codes, rows, self.forest[:start_iter])
+                scores = rows.t().contiguous()
+                del rows
+            else:
+                scores = D.cols_of(self._uniform_prior_logits(), n, dev)
+        else:
+            K = 1
+            scores = torch.zeros(n, dtype=torch.float32, device=dev)
+            if start_iter > 0:
+                self._predict_codes_into(codes, scores.view(-1, 1), self.forest[:start_iter])
+            if len(self.forest) < self.n_estimators:
+                self.forest.extend([{} for _ in range(self.n_estimators - len(self.forest))])
+        step, total = self._round_losses(given, y, scores, dev)
+        if start_iter == 0:
+            self.per_era_feature_importance_ = np.zeros((self.num_eras, self.num_features),
+                                                        dtype=np.float32)
+        self._eval = None
+        eng = self._new_engine(codes, root_order, era_start, K, 2)
+        n_new = self.n_estimators - start_iter
+        rec = self._alloc_records(n_new, K, dev)
+        sums = torch.zeros(n_new, dtype=torch.float32, device=dev)
+        self._phases.mark("engine")
+        done = 0
+        stream = _RecordStream(rec)
+        try:
+            with torch.no_grad():
+                for j in range(n_new):
+                    feat_sel = self._feature_subset(dev)
+                    grad, loss = step()
+                    sums[j] = loss
+                    eng.round(grad, scores, feat_sel, {k: v[j] for k, v in rec.items()})
+                    done = j + 1
+                    stream.round_done(j, n_new)
+            stream.finish(done)
+        finally:
+            stream.close()
+        self._phases.mark("rounds")
+        eng.close()
+        self._absorb_records(rec, stream, done, start_iter, classification=classes)
+        self._phases.mark("records")
+        self._phases.report()
+        self.training_loss.extend((sums.double() / max(total, 1e-30)).tolist())
+        self.feature_importance_ = self.per_era_feature_importance_.sum(axis=0)
+        self._is_fitted = True
+        self._heap = self._records_heap(rec, done) if start_iter == 0 else None
+        print(f"Finished training {self.objective} forest. Total rounds: {self._trees_trained}")
+        del codes
+        return self
+
     # ------------------------------------------------------------------ priors
     def _class_prior_logits(self, y_encoded):
         """log(prior_k + 1e-10) with prior_k the class frequency in float32
@@ -840,10 +1096,11 @@ class WarpGBM(BaseEstimator, RegressorMixin):
         lists of K tree dicts); empty trees are skipped like the reference's
         ``if tree`` filters."""
         H = (1 << (self.max_depth + 1)) - 1
-        K = 1 if self.objective == "regression" else self.num_classes
+        one = self.objective in _SCORE_OBJECTIVES
+        K = 1 if one else self.num_classes
         rows = []
         for r in rounds:
-            trees = [r] if self.objective == "regression" else list(r)
+            trees = [r] if one else list(r)
             if not trees or not all(trees):
                 continue
             rows.append([_dict_to_heap(t, H) for t in trees])
@@ -957,8 +1214,9 @@ class WarpGBM(BaseEstimator, RegressorMixin):
         return self._predict_scores(codes, self._cached_heap())
 
     def predict(self, X_np):
-        """Regression values, or class labels for classification (warpgbm/core.py:957-974)."""
-        if self.objective in ("multiclass", "binary"):
+        """Regression values or preference scores, or class labels for the objectives
+        with classes (warpgbm/core.py:957-974)."""
+        if self.objective in _CLASS_OBJECTIVES:
             probs = self.predict_proba(X_np)
             return self.label_encoder.inverse_transform(np.argmax(probs, axis=1))
         ph = _Phases()
@@ -971,11 +1229,24 @@ class WarpGBM(BaseEstimator, RegressorMixin):
 
     def predict_proba(self, X_np):
         """Class probabilities (warpgbm/core.py:976-989)."""
-        if self.objective not in ["multiclass", "binary"]:
+        if self.objective not in _CLASS_OBJECTIVES:
             raise ValueError("predict_proba only available for classification objectives")
         scores = self._infer(X_np, self.num_classes)
         D.softmax_rows(scores)
         return D.to_host(scores)
+
+    def log_prob(self, X_np, y):
+        """Log-probability [n] (float32) of the label y[i] (one of ``classes_``) in
+        row i: what the next policy fit takes as ``behavior_log_prob``, and a
+        preference fit as ``reference``."""
+        if self.objective not in _CLASS_OBJECTIVES:
+            raise ValueError("log_prob only available for objectives with classes")
+        labels = self.label_encoder.transform(np.asarray(y)).astype(np.int32)
+        if labels.shape[0] != np.asarray(X_np).shape[0]:
+            raise ValueError("X and y must have the same number of rows.")
+        scores = self._infer(X_np, self.num_classes)
+        r = L.class_log_probs(scores, torch.from_numpy(labels).to(scores.device))
+        return D.to_host(r.log_prob)
 
     # ------------------------------------------------------------------ importance
     @staticmethod
@@ -1033,6 +1304,7 @@ class WarpGBM(BaseEstimator, RegressorMixin):
             "_trees_trained": self._trees_trained,
             "training_loss": getattr(self, "training_loss", []),
             "eval_loss": getattr(self, "eval_loss", []),
+            "loss_params": {k: getattr(self, k) for k in _LOSS_PARAMS},
         }
         with open(path, "wb") as f:
             pickle.dump(state, f)
@@ -1052,6 +1324,8 @@ class WarpGBM(BaseEstimator, RegressorMixin):
             setattr(self, k, state[k])
         self.training_loss = state.get("training_loss", [])
         self.eval_loss = state.get("eval_loss", [])
+        for k, v in state.get("loss_params", {}).items():
+            setattr(self, k, v)
         if self.per_era_feature_importance_ is not None:
             self.num_eras = self.per_era_feature_importance_.shape[0]
         self._heap = None

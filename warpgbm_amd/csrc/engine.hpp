@@ -27,7 +27,7 @@ struct EngineConfig {
   int32_t num_eras;
   int32_t max_depth;
   int32_t n_trees;         // trees grown together per round (1 or K)
-  int32_t objective;       // 0 regression, 1 softmax
+  int32_t objective;       // 0 regression, 1 softmax, 2 gradients given
   float min_child_weight;
   float min_split_gain;
   float l2_reg;
@@ -42,8 +42,8 @@ struct EngineConfig {
 struct Engine;
 int engine_create(Engine** out, const EngineConfig& cfg);
 void engine_destroy(Engine* e);
-// One boosting round.  target: float y [n] (regression) or int32 labels
-// (softmax).  pred: [n] or [n, K] row-major, updated in place.
+// One boosting round.  target: float y [n] (regression), int32 labels (softmax)
+// or float gradients [T, n].  pred: [n] or class-major [T, n], updated in place.
 int engine_round(Engine* e, const void* target, float* pred, const int32_t* feat_sel,
                  int32_t n_sel, const TreeRecord& rec, hipStream_t st);
 int engine_set_tuning(Engine* e, int key, int64_t value);
@@ -51,6 +51,7 @@ int engine_set_tuning(Engine* e, int key, int64_t value);
 // kernels (engine_kernels.hip)
 __global__ void residual_regression_kernel(const float* y, const float* pred, int64_t n,
                                            float* r, uint32_t* partial);
+__global__ void residual_gradient_kernel(const float* g, int64_t n, float* r, uint32_t* partial);
 __global__ void residual_softmax_kernel(const float* logits, const int32_t* label, int64_t n,
                                         int32_t K, float* r, uint32_t* partial);
 __global__ void root_setup_kernel(const int32_t* root_order, int64_t n, int32_t T,

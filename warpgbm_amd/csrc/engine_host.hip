@@ -197,8 +197,8 @@ int engine_create(Engine** out, const EngineConfig& cfg) {
                "engine: n_trees * 2^max_depth * num_eras = %lld segments exceeds the int32 "
                "segment numbering; reduce max_depth",
                (long long)(((int64_t)cfg.n_trees << cfg.max_depth) * cfg.num_eras));
-  WGBM_REQUIRE(cfg.objective == 0 || cfg.objective == 1, "engine: bad objective");
-  WGBM_REQUIRE(cfg.objective == 1 || cfg.n_trees == 1, "engine: regression grows one tree per round");
+  WGBM_REQUIRE(cfg.objective >= 0 && cfg.objective <= 2, "engine: bad objective");
+  WGBM_REQUIRE(cfg.objective != 0 || cfg.n_trees == 1, "engine: regression grows one tree per round");
   WGBM_REQUIRE(cfg.codes_rm && cfg.codes_cm && cfg.root_order && cfg.era_start,
                "engine: null input pointer");
   Engine* e = new Engine();
@@ -661,6 +661,22 @@ static HistLaunch level_hist(const Engine* e, int cur, int64_t k0) {
   return a;
 }
 
+// residuals of the objectives whose residual is a launch of its own (all but
+// regression's small rounds): r and the workgroups' maxima
+static void launch_residuals(Engine* e, const void* target, const float* pred, int nres,
+                             hipStream_t st) {
+  const EngineConfig& c = e->c;
+  if (c.objective == 0)
+    hipLaunchKernelGGL(residual_regression_kernel, dim3(nres), dim3(256), 0, st,
+                       (const float*)target, pred, c.n_rows, e->resid, e->abs_part);
+  else if (c.objective == 1)
+    hipLaunchKernelGGL(residual_softmax_kernel, dim3(nres), dim3(256), 0, st, pred,
+                       (const int32_t*)target, c.n_rows, c.n_trees, e->resid, e->abs_part);
+  else
+    hipLaunchKernelGGL(residual_gradient_kernel, dim3(nres, (unsigned)c.n_trees), dim3(256), 0, st,
+                       (const float*)target, c.n_rows, e->resid, e->abs_part);
+}
+
 static inline unsigned blocks_for(int64_t n, int bs) { return (unsigned)((n + bs - 1) / bs); }
 
 // a one-era round of few rows: residuals (regression: in the root level's
@@ -694,10 +710,9 @@ static int small_round(Engine* e, const void* target, float* pred, const int32_t
   a.tot_ql = e->sr.tot_ql;
   a.tot_c = e->sr.tot_c;
   a.rec = rec;
-  if (c.objective == 1) {
+  if (c.objective != 0) {
     const int nres = (int)std::min<int64_t>(blocks_for(c.n_rows, 256), kResidBlocks);
-    hipLaunchKernelGGL(residual_softmax_kernel, dim3(nres), dim3(256), 0, st, pred,
-                       (const int32_t*)target, c.n_rows, T, e->resid, e->abs_part);
+    launch_residuals(e, target, pred, nres, st);
     WGBM_LAUNCH_CHECK();
     a.abs_part = e->abs_part;
     a.n_part = nres;
@@ -733,13 +748,7 @@ int engine_round(Engine* e, const void* target, float* pred, const int32_t* feat
   // residuals and quantisation shifts (per-workgroup maxima, then one
   // workgroup per tree reduces them)
   const int nres = (int)std::max<int64_t>(1, std::min<int64_t>(blocks_for(N, 256), kResidBlocks));
-  if (c.objective == 0) {
-    hipLaunchKernelGGL(residual_regression_kernel, dim3(nres), dim3(256), 0, st,
-                       (const float*)target, pred, N, e->resid, e->abs_part);
-  } else {
-    hipLaunchKernelGGL(residual_softmax_kernel, dim3(nres), dim3(256), 0, st, pred,
-                       (const int32_t*)target, N, T, e->resid, e->abs_part);
-  }
+  launch_residuals(e, target, pred, nres, st);
   WGBM_LAUNCH_CHECK();
   // one era, fused root: the root totals words are cleared here for the
   // root's atomic sums

@@ -35,6 +35,24 @@ __global__ void residual_regression_kernel(const float* __restrict__ y,
   if (threadIdx.x == 0) partial[blockIdx.x] = m;
 }
 
+// gradients given: r = -g, a grid row per tree; partial[tree * gridDim.x +
+// block] = max |r|
+__global__ void residual_gradient_kernel(const float* __restrict__ g /* [T][n] */, int64_t n,
+                                         float* __restrict__ r /* [T][n] */,
+                                         uint32_t* __restrict__ partial) {
+  const int64_t at = (int64_t)blockIdx.y * n;
+  uint32_t m = 0;
+  for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < n;
+       i += (int64_t)gridDim.x * blockDim.x) {
+    const float v = -g[at + i];
+    r[at + i] = v;
+    const uint32_t b = wgbm_abs_bits(v);
+    m = b > m ? b : m;
+  }
+  m = wgbm_block_max_u32(m);
+  if (threadIdx.x == 0) partial[(int64_t)blockIdx.y * gridDim.x + blockIdx.x] = m;
+}
+
 // softmax: p = softmax(F[i, :]); residual_k = -(p_k - onehot_k)
 // (warpgbm/core.py:186-214 and :782; metrics.py:12-15).
 // partial[k * gridDim.x + block] = max_i |residual_k|
