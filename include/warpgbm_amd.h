@@ -320,12 +320,29 @@ int wgbm_balance_loss(const wgbm_scores* scores, const uint8_t* mask, int32_t to
  *   loss[p] = weight[p] * ((1 - e) log(1 + exp(-beta margin)) + e log(1 + exp(beta margin))),
  * e = label_smoothing, and grad[i] = sum over the pairs that hold i's sequence.
  * Rows behind the last sequence have gradient 0.  Without sequence_start every
- * row is a sequence.  pairs [n_pairs][2]: sequence numbers, which the call
- * takes as valid (0 .. n_sequences - 1), as it does the offsets (from 0, not
- * descending, at most n_rows); incidence [2 n_pairs]: the numbers
- * 2 * pair + side (0 preferred, 1 other) grouped by sequence,
- * incidence_start [n_sequences + 1] their offsets.  A pair of weight 0 is not
- * read.  grad NULL: no gradient (incidence may be NULL then). */
+ * row is a sequence.  A pair of weight 0 is not read.  grad NULL: no gradient.
+ *
+ * The tables (device memory) lay the pairs and sequences out for the kernels;
+ * warpgbm_amd.losses.PreferencePlan builds them, once for all calls, and the
+ * call takes them as valid:
+ *  pairs [n_pairs][2]: sequence numbers 0 .. n_sequences - 1;
+ *  incidence [2 n_pairs]: the numbers 2 * pair + side (0 preferred, 1 other)
+ *    grouped by sequence, the sequences in very many pairs (`long`) last;
+ *  incidence_start [n_sequences + 1]: each sequence's range of them, empty for
+ *    the long ones;
+ *  share [n_shares + 1]: sequence numbers that cut the sequences into runs with
+ *    at most 1024 sequences and 1280 of the incidences of incidence_start;
+ *  is_long [n_sequences]: 1 for the long ones (NULL: none);
+ *  piece [n_pieces][3]: (sequence, or -1 where it has several pieces; first and
+ *    end incidence) of the long sequences; multi [n_multi][3]: (sequence, first
+ *    and end piece) of those with several;
+ *  task [n_tasks][3], with sequence_start only: (sequence; first and end row),
+ *    every row of every sequence in one task, in sequence order, at least one a
+ *    sequence, then the rows behind the last one with sequence -1; task_start
+ *    [n_sequences + 1]: each sequence's tasks, NULL where each has one;
+ *  disjoint != 0: each sequence has one task and at most one pair (none of the
+ *    tables above is read but pairs); idle [n_idle][2] then holds the row ranges
+ *    that no pair covers. */
 typedef struct wgbm_preference_args {
   const float* log_prob;            /* [n_rows] */
   const float* ref_log_prob;        /* [n_rows] or NULL (0) */
@@ -336,6 +353,19 @@ typedef struct wgbm_preference_args {
   int64_t n_pairs;
   const int32_t* incidence;
   const int64_t* incidence_start;
+  const int64_t* share;
+  int64_t n_shares;
+  const uint8_t* is_long;
+  const int64_t* task;
+  int64_t n_tasks;
+  const int64_t* task_start;
+  const int64_t* piece;
+  int64_t n_pieces;
+  const int64_t* multi;
+  int64_t n_multi;
+  const int64_t* idle;
+  int64_t n_idle;
+  int32_t disjoint;
   const float* weight;              /* [n_pairs] or NULL (1) */
   float beta;
   float label_smoothing;            /* [0, 0.5] */

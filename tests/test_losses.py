@@ -433,7 +433,15 @@ def test_balance_ties_and_nothing_left(gpu, order):
 # --------------------------------------------------------------------- preferences
 def pref_case(kind, seed):
     g = torch.Generator().manual_seed(seed)
-    if kind == "items":
+    if kind == "hub":
+        # one item in more pairs than a piece holds, some in a few hundred
+        n = S = 3000
+        seg = None
+        pairs = torch.randint(0, n, (40_000, 2), generator=g)
+        pairs[::2, 0] = 5
+        pairs[1::100, 1] = 2999
+        pairs[:, 1] = torch.where(torch.arange(40_000) % 50 == 0, 700, pairs[:, 1])
+    elif kind == "items":
         n = S = 1000
         seg = None
         pairs = torch.randint(0, n, (3000, 2), generator=g)
@@ -444,17 +452,20 @@ def pref_case(kind, seed):
         n = S = 2
         seg, pairs = None, torch.tensor([[1, 0]])
     else:
-        S = {"sequences": 400, "disjoint": 400, "long": 5, "empty": 6}[kind]
-        top = {"sequences": 60, "disjoint": 60, "long": 30_000, "empty": 1}[kind]
+        S = {"sequences": 400, "disjoint": 400, "long": 5, "empty": 6, "tail": 50}[kind]
+        top = {"sequences": 60, "disjoint": 60, "long": 30_000, "empty": 1, "tail": 4}[kind]
         length = torch.randint(0, top, (S,), generator=g)
+        if kind == "tail":
+            length[:] = 3
         length[S // 2] = 0
         if kind == "long":
             length[1] = 1
         seg = torch.zeros(S + 1, dtype=torch.int64)
         seg[1:] = length.cumsum(0)
-        n = int(seg[-1]) + 11
-        if kind == "disjoint":
-            pairs = torch.randperm(S, generator=g).reshape(-1, 2)
+        n = int(seg[-1]) + (11 if kind != "tail" else 9000)
+        if kind in ("disjoint", "tail"):
+            # (some sequences in no pair)
+            pairs = torch.randperm(S, generator=g).reshape(-1, 2)[3:]
         else:
             pairs = torch.randint(0, S, (700, 2), generator=g)
     P = pairs.shape[0]
@@ -468,7 +479,8 @@ def pref_case(kind, seed):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("how", ["plain", "reference", "weights"])
-@pytest.mark.parametrize("kind", ["items", "two", "sequences", "disjoint", "long", "empty"])
+@pytest.mark.parametrize("kind", ["items", "hub", "two", "sequences", "disjoint", "tail", "long",
+                                  "empty"])
 def test_preference_loss(gpu, kind, how):
     from warpgbm_amd import losses
 
@@ -768,12 +780,49 @@ def test_refusals_without_a_gpu():
 
 
 def test_plan_layout():
-    """Incidences grouped by sequence, in pair order (on the CPU)."""
+    """The tables of a plan (on the CPU): incidences grouped by sequence in pair
+    order, tasks that cover every row once, in order, sequences in many pairs in
+    pieces."""
     from warpgbm_amd import losses
 
     p = losses.PreferencePlan(np.asarray([[2, 0], [0, 1], [0, 0]]), 3, device="cpu")
     assert p.incidence.tolist() == [1, 2, 4, 5, 3, 0]
     assert p.incidence_start.tolist() == [0, 4, 5, 6]
+    assert p.task is None and p.piece is None and not p.disjoint
+    seg = np.asarray([0, 5, 5, 4106, 14000, 14002])
+    p = losses.PreferencePlan(np.asarray([[0, 1], [0, 2], [3, 4]]), 18100, segments=seg,
+                              device="cpu")
+    rows = p.task.tolist()
+    assert [r[0] for r in rows] == [0, 1, 2, 2, 3, 3, 3, 4, -1, -1]
+    assert p.task_start.tolist() == [0, 1, 2, 4, 7, 8]
+    assert rows[1] == [1, 5, 5] and rows[3] == [2, 4101, 4106]
+    assert rows[0][1] == 0 and rows[-1][2] == 18100
+    assert all(a[2] == b[1] and a[2] - a[1] <= 4096 for a, b in zip(rows, rows[1:]))
+    p = losses.PreferencePlan(np.asarray([[3, 1]]), 9, segments=np.asarray([0, 2, 3, 3, 5, 8]),
+                              device="cpu")
+    assert p.disjoint and p.idle.tolist() == [[0, 2], [5, 8], [8, 9]]
+    # a sequence of 17,000 incidences, one of 300, others of few
+    pairs = np.asarray([[7, k % 5] if k < 17_000 else [8, 7 - k % 3] for k in range(17_300)])
+    p = losses.PreferencePlan(pairs, 10, device="cpu")
+    inc, start = p.incidence.numpy(), p.incidence_start.tolist()
+    assert sorted(inc.tolist()) == list(range(2 * len(pairs)))
+    ends = pairs.reshape(-1)[inc]
+    for s in range(10):
+        assert (ends[start[s]:start[s + 1]] == s).all()
+    share = p.share.tolist()
+    assert share[0] == 0 and share[-1] == 10 and share == sorted(share)
+    assert p.is_long.tolist() == [int(start[s] == start[s + 1] and s != 9) for s in range(10)]
+    covered = start[-1]
+    whole = {s: f for s, f, e in p.multi.tolist() for s in [s]}
+    assert 7 in whole
+    owner = {}
+    for s, f, e in p.multi.tolist():
+        owner.update({q: s for q in range(f, e)})
+    for q, (s, f, e) in enumerate(p.piece.tolist()):
+        assert f == covered and 0 < e - f <= 8192
+        covered = e
+        assert (ends[f:e] == (s if s >= 0 else owner[q])).all()
+    assert covered == 2 * len(pairs)
 
 
 def test_c_entries_refuse_before_any_launch():
@@ -843,8 +892,10 @@ def test_c_entries_refuse_before_any_launch():
 
     def pref(**kw):
         f = dict(log_prob=one, ref_log_prob=None, n_rows=4, sequence_start=None, n_sequences=4,
-                 pairs=one, n_pairs=2, incidence=one, incidence_start=one, weight=None, beta=1.0,
-                 label_smoothing=0.0)
+                 pairs=one, n_pairs=2, incidence=one, incidence_start=one, share=one, n_shares=1,
+                 is_long=None, task=None, n_tasks=0,
+                 task_start=None, piece=None, n_pieces=0, multi=None, n_multi=0, idle=None,
+                 n_idle=0, disjoint=0, weight=None, beta=1.0, label_smoothing=0.0)
         f.update(kw)
         args = _lib.PreferenceArgs(*f.values())
         return lib.wgbm_preference_loss(C.byref(args), one, one, one, one, 1 << 30, None)
@@ -855,6 +906,12 @@ def test_c_entries_refuse_before_any_launch():
     refused(pref(n_sequences=3), "every row is a sequence")
     refused(pref(n_pairs=1 << 30), "n_pairs")
     refused(pref(incidence=None), "gradient needs")
+    refused(pref(sequence_start=one), "tasks")
+    refused(pref(share=None), "gradient needs")
+    refused(pref(n_pieces=1), "gradient needs")
+    refused(pref(n_pieces=1, is_long=one), "null table")
+    refused(pref(n_multi=-1), "table sizes")
+    refused(pref(disjoint=1), "every row is a sequence")
 
 
 @pytest.mark.gpu

@@ -136,6 +136,19 @@ class PreferenceArgs(C.Structure):
         ("n_pairs", _i64),
         ("incidence", _p),
         ("incidence_start", _p),
+        ("share", _p),
+        ("n_shares", _i64),
+        ("is_long", _p),
+        ("task", _p),
+        ("n_tasks", _i64),
+        ("task_start", _p),
+        ("piece", _p),
+        ("n_pieces", _i64),
+        ("multi", _p),
+        ("n_multi", _i64),
+        ("idle", _p),
+        ("n_idle", _i64),
+        ("disjoint", _i32),
         ("weight", _p),
         ("beta", _f32),
         ("label_smoothing", _f32),

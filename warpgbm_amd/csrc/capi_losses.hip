@@ -160,34 +160,7 @@ int wgbm_balance_loss(const wgbm_scores* scores, const uint8_t* mask, int32_t to
                       workspace, S(stream));
 }
 
-int64_t wgbm_preference_loss_workspace(const wgbm_preference_args* a) {
-  if (!a || a->n_sequences < 0 || a->n_pairs < 0) {
-    wgbm_set_error("preference_loss: bad sizes");
-    return -1;
-  }
-  return (int64_t)preference_workspace(a->n_sequences, a->n_pairs, a->sequence_start != nullptr);
-}
-
-int wgbm_preference_loss(const wgbm_preference_args* a, float* loss, float* margin, float* grad,
-                         void* workspace, int64_t workspace_bytes, void* stream) {
-  WGBM_REQUIRE(a, "preference_loss: null arguments");
-  WGBM_REQUIRE(a->n_rows >= 0 && a->n_rows < (int64_t(1) << 40), "preference_loss: bad n_rows");
-  WGBM_REQUIRE(a->n_sequences >= 0 && a->n_sequences < (int64_t(1) << 31),
-               "preference_loss: bad n_sequences");
-  WGBM_REQUIRE(a->n_pairs >= 0 && a->n_pairs < (int64_t(1) << 30), "preference_loss: bad n_pairs");
-  WGBM_REQUIRE(a->sequence_start || a->n_sequences == a->n_rows,
-               "preference_loss: without sequence_start every row is a sequence");
-  WGBM_REQUIRE(std::isfinite(a->beta) && a->beta > 0.0f,
-               "preference_loss: beta must be positive and finite");
-  WGBM_REQUIRE(a->label_smoothing >= 0.0f && a->label_smoothing <= 0.5f,
-               "preference_loss: label_smoothing must be in [0, 0.5]");
-  WGBM_REQUIRE(a->n_rows == 0 || a->log_prob, "preference_loss: null pointer");
-  WGBM_REQUIRE(a->n_pairs == 0 || (a->pairs && loss && margin && workspace),
-               "preference_loss: null pointer");
-  WGBM_REQUIRE(!grad || (a->incidence_start && (a->n_pairs == 0 || a->incidence)),
-               "preference_loss: the gradient needs the pairs of each sequence");
-  WGBM_REQUIRE(workspace_bytes >= wgbm_preference_loss_workspace(a),
-               "preference_loss: workspace too small");
+static PreferenceArgs preference_args(const wgbm_preference_args* a) {
   PreferenceArgs p{};
   p.log_prob = a->log_prob;
   p.ref = a->ref_log_prob;
@@ -198,12 +171,71 @@ int wgbm_preference_loss(const wgbm_preference_args* a, float* loss, float* marg
   p.n_pairs = a->n_pairs;
   p.inc = a->incidence;
   p.inc_start = a->incidence_start;
+  p.share = a->share;
+  p.n_shares = a->n_shares;
+  p.is_long = a->is_long;
+  p.task = a->task;
+  p.n_tasks = a->n_tasks;
+  p.task_start = a->task_start;
+  p.piece = a->piece;
+  p.n_pieces = a->n_pieces;
+  p.multi = a->multi;
+  p.n_multi = a->n_multi;
+  p.idle = a->idle;
+  p.n_idle = a->n_idle;
+  p.disjoint = a->disjoint != 0;
   p.weight = a->weight;
   p.beta = a->beta;
   p.smooth = a->label_smoothing;
+  return p;
+}
+
+static int check_preference(const wgbm_preference_args* a) {
+  WGBM_REQUIRE(a, "preference_loss: null arguments");
+  WGBM_REQUIRE(a->n_rows >= 0 && a->n_rows < (int64_t(1) << 40), "preference_loss: bad n_rows");
+  WGBM_REQUIRE(a->n_sequences >= 0 && a->n_sequences < (int64_t(1) << 30),
+               "preference_loss: bad n_sequences");
+  WGBM_REQUIRE(a->n_pairs >= 0 && a->n_pairs < (int64_t(1) << 30), "preference_loss: bad n_pairs");
+  WGBM_REQUIRE(a->n_shares >= 0 && a->n_shares < (int64_t(1) << 31) && a->n_tasks >= 0 && a->n_tasks < (int64_t(1) << 31) && a->n_pieces >= 0 &&
+                   a->n_pieces < (int64_t(1) << 31) && a->n_multi >= 0 &&
+                   a->n_multi < (int64_t(1) << 31) && a->n_idle >= 0 &&
+                   a->n_idle < (int64_t(1) << 31),
+               "preference_loss: bad table sizes");
+  WGBM_REQUIRE(a->sequence_start || (a->n_sequences == a->n_rows && !a->disjoint),
+               "preference_loss: without sequence_start every row is a sequence");
+  WGBM_REQUIRE(std::isfinite(a->beta) && a->beta > 0.0f,
+               "preference_loss: beta must be positive and finite");
+  WGBM_REQUIRE(a->label_smoothing >= 0.0f && a->label_smoothing <= 0.5f,
+               "preference_loss: label_smoothing must be in [0, 0.5]");
+  return 0;
+}
+
+int64_t wgbm_preference_loss_workspace(const wgbm_preference_args* a) {
+  if (check_preference(a)) return -1;
+  return (int64_t)preference_workspace(preference_args(a));
+}
+
+int wgbm_preference_loss(const wgbm_preference_args* a, float* loss, float* margin, float* grad,
+                         void* workspace, int64_t workspace_bytes, void* stream) {
+  TRY(check_preference(a));
+  PreferenceArgs p = preference_args(a);
   p.loss = loss;
   p.margin = margin;
   p.grad = grad;
+  WGBM_REQUIRE(a->n_rows == 0 || a->log_prob, "preference_loss: null pointer");
+  WGBM_REQUIRE(a->n_pairs == 0 || (a->pairs && loss && margin), "preference_loss: null pointer");
+  WGBM_REQUIRE(a->disjoint || !a->sequence_start || a->n_rows == 0 || a->task,
+               "preference_loss: sequences need their tasks");
+  WGBM_REQUIRE(a->disjoint || !grad || a->n_sequences == 0 ||
+                   (a->incidence_start && a->share && a->n_shares > 0 &&
+                    (a->n_pairs == 0 || a->incidence) && (a->n_pieces == 0 || a->is_long)),
+               "preference_loss: the gradient needs the pairs of each sequence");
+  WGBM_REQUIRE((a->n_pieces == 0 || a->piece) && (a->n_multi == 0 || a->multi) &&
+                   (a->n_idle == 0 || a->idle) && (a->n_tasks == 0 || a->task),
+               "preference_loss: null table");
+  const int64_t need = (int64_t)preference_workspace(p);
+  WGBM_REQUIRE(workspace_bytes >= need && (need == 0 || workspace),
+               "preference_loss: workspace too small");
   return preference_loss(p, workspace, S(stream));
 }
 

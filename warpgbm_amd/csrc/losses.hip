@@ -176,44 +176,14 @@ __global__ __launch_bounds__(256) void policy_rows_kernel(ScoresView s, ScoresVi
 // ---------------------------------------------------------------------------
 // gradients, elementwise
 // ---------------------------------------------------------------------------
-// p * (1[k = a] - softmax) of the log-probability's gradient
-struct LogProbGrad {
-  const int32_t* label;
-  const float2* norm;
-  const float* grad;
-  static constexpr bool kRef = false;
-  __device__ __forceinline__ RowCoef row(int64_t i, int32_t K) const {
-    RowCoef c{};
-    const int32_t a = row_label(label, i, K);
-    const float g = grad[i];
-    if (a < 0 || g == 0.0f) return c;
-    const float2 v = norm[i];
-    if (v.x == -__builtin_inff()) return c;
-    c.m = v.x;
-    c.iz = v.y;  // (the sum's logarithm)
-    c.c0 = -g;
-    c.label = a;
-    c.live = 1;
-    return c;
-  }
-  __device__ __forceinline__ float at(const RowCoef& c, float s, float) const {
-    return c.c0 * loss_expf((s - c.m) - c.iz);
-  }
-  // the label's from its own logarithm: 1 - p without a difference
-  __device__ __forceinline__ float at_label(const RowCoef& c, float s) const {
-    return c.c0 * expm1f((s - c.m) - c.iz);
-  }
-};
-
 template <bool REF>
 struct PolicyGrad {
   const RowCoef* coef;
   static constexpr bool kRef = REF;
-  __device__ __forceinline__ RowCoef row(int64_t i, int32_t) const { return coef[i]; }
+  __device__ __forceinline__ RowCoef row(const ScoresView&, int64_t i) const { return coef[i]; }
   __device__ __forceinline__ float at(const RowCoef& c, float s, float r) const {
     return coef_grad<REF>(c, s, r);
   }
-  __device__ __forceinline__ float at_label(const RowCoef& c, float) const { return c.gl; }
 };
 
 template <typename T, bool CM, typename G>
@@ -224,7 +194,7 @@ __global__ __launch_bounds__(256) void score_grad_kernel(ScoresView s, ScoresVie
   if (CM) {
     const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
     if (i >= s.n) return;
-    const RowCoef c = g.row(i, s.K);
+    const RowCoef c = g.row(s, i);
     const int32_t k0 = blockIdx.y * span, k1 = s.K - k0 > span ? k0 + span : s.K;
     const T* p = (const T*)s.data + i;
     const T* q = G::kRef ? (const T*)ref.data + i : nullptr;
@@ -238,7 +208,7 @@ __global__ __launch_bounds__(256) void score_grad_kernel(ScoresView s, ScoresVie
     for (int32_t k = k0; k < k1; ++k) {
       const float v = to_f32(p[k * s.ks]);
       const float r = G::kRef ? to_f32(q[k * ref.ks]) : 0.0f;
-      float x = k == c.label ? g.at_label(c, v) : g.at(c, v, r);
+      float x = k == c.label ? c.gl : g.at(c, v, r);
       if (accumulate) x += to_f32(o[k * out.ks]);
       o[k * out.ks] = from_f32<T>(x);
     }
@@ -247,7 +217,7 @@ __global__ __launch_bounds__(256) void score_grad_kernel(ScoresView s, ScoresVie
   // 64 lanes along a row, 4 rows a workgroup
   const int64_t i = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
   if (i >= s.n) return;
-  const RowCoef c = g.row(i, s.K);
+  const RowCoef c = g.row(s, i);
   const int32_t k0 = blockIdx.y * span, k1 = s.K - k0 > span ? k0 + span : s.K;
   const T* p = (const T*)s.data + i * s.rs;
   const T* q = G::kRef ? (const T*)ref.data + i * ref.rs : nullptr;
@@ -275,7 +245,7 @@ __global__ __launch_bounds__(256) void score_grad_kernel(ScoresView s, ScoresVie
       for (int j = 0; j < VE; ++j) {
         const float sv = to_f32(v.v[j]);
         const float rv = G::kRef ? to_f32(r.v[j]) : 0.0f;
-        float x = k + j == c.label ? g.at_label(c, sv) : g.at(c, sv, rv);
+        float x = k + j == c.label ? c.gl : g.at(c, sv, rv);
         if (accumulate) x += to_f32(old.v[j]);
         v.v[j] = from_f32<T>(x);
       }
@@ -369,8 +339,16 @@ int class_log_probs(const ScoresView& s, const int32_t* label, const uint8_t* ma
 
 int class_log_probs_grad(const ScoresView& s, const int32_t* label, const float* norm,
                          const float* grad, const ScoresView& out, hipStream_t st) {
-  const LogProbGrad g{label, (const float2*)norm, grad};
-  LOSS_TYPES(s.dtype, return grad_of<T>(s, ScoresView{}, g, false, out, st));
+  bool done = false;
+  const auto rows = s.dtype == kF32    ? log_probs_grad_rows_f32
+                    : s.dtype == kBF16 ? log_probs_grad_rows_bf16
+                                       : log_probs_grad_rows_f16;
+  const int r = rows(s, label, norm, grad, out, st, &done);
+  if (r || done) return r;
+  LOSS_TYPES(s.dtype, {
+    const LogProbGrad<T> g{label, (const float2*)norm, grad};
+    return grad_of<T>(s, ScoresView{}, g, false, out, st);
+  });
 }
 
 template <typename T, bool REF>

@@ -62,18 +62,14 @@ __device__ __forceinline__ T from_f32(float v) {
   return (T)v;
 }
 
-// e^x for x <= 0 (and NaN), within 2 ulp: v_exp_f32 of the rounded product
-// x * log2(e), whose rounding error is taken along to first order (alone it
-// would cost |x| / 2 ulp).  0 below e^-104; -inf gives 0.
+// e^x for x <= 0 (-inf gives 0, NaN stays): v_exp_f32 of x log2(e).  The
+// product's rounding costs |x| 2^-24 of the value, that is at most 2^-25 of the
+// row's largest exponential (|x| e^x has its maximum 1/e): what a softmax's sums
+// and gradients are rounded by anyway.  Taking the rounding error along would
+// cost six instructions more, as much again as the exponential (the balance
+// loss's first pass over 1M x 100 classes is bound by instructions then).
 __device__ __forceinline__ float loss_expf(float x) {
-  const float log2e = 1.44269502162933349609f;       // log2(e) rounded to float32
-  const float log2e_lo = 1.92596299112661746887e-8f;  // log2(e) - log2e
-  const float ln2 = 0.693147180559945309417f;
-  x = x < -150.0f ? -150.0f : x;  // (keeps NaN; e^-150 is 0 in float32)
-  const float h = x * log2e;
-  const float lo = fmaf(x, log2e_lo, fmaf(x, log2e, -h));
-  const float e = __builtin_amdgcn_exp2f(h);
-  return fmaf(e, lo * ln2, e);
+  return __builtin_amdgcn_exp2f(x * 1.44269504088896340736f);
 }
 
 // running maximum and sums of a set of a row's classes, all in float32:

@@ -4,68 +4,62 @@
 
 namespace wgbm {
 
-// classes of a workgroup of the finishing launch, and its threads along the
-// partial sums
-constexpr int kFinClasses = 16, kFinLanes = 64;
+// classes of a workgroup of the finishing launch: a wave each, its lanes along
+// the workgroups' partial sums
+constexpr int kFinClasses = 4;
 
 // shares f_k, means P_k, counts, the loss and the gradient's scale.  The
 // workgroups' shares of the loss are joined by the last one to arrive, in
 // workgroup order.
-__global__ __launch_bounds__(1024) void balance_finish_kernel(BalanceWs w, int32_t groups,
-                                                              int32_t K, int32_t top_k, float coef,
-                                                              BalanceOut o) {
-  __shared__ int64_t s_live;
-  __shared__ double s_sum[kFinLanes][kFinClasses + 1];
-  __shared__ int64_t s_cnt[kFinLanes][kFinClasses + 1];
+__global__ __launch_bounds__(256) void balance_finish_kernel(BalanceWs w, int32_t groups,
+                                                             int32_t K, int32_t top_k, float coef,
+                                                             BalanceOut o) {
+  __shared__ double s_loss[kFinClasses];
   __shared__ bool s_last;
-  if (threadIdx.x < 64) {
-    int64_t live = 0;
-    for (int32_t g = threadIdx.x; g < groups; g += 64) live += w.count[(int64_t)g * (K + 1) + K];
-    for (int d = 32; d; d >>= 1) live += __shfl_xor(live, d);
-    if (threadIdx.x == 0) s_live = live;
-  }
-  const int c = threadIdx.x % kFinClasses, lane = threadIdx.x / kFinClasses;
+  const int lane = threadIdx.x & 63, c = threadIdx.x >> 6;
   const int32_t k = blockIdx.x * kFinClasses + c;
+  const bool in = k < K;
+  const float* part = w.part + (int64_t)(in ? k : 0) * groups;
+  const int32_t* count = w.count + (int64_t)(in ? k : 0) * groups;
+  const int32_t* rows = w.count + (int64_t)K * groups;
   double a = 0.0;
-  int64_t n = 0;
-  if (k < K)
-    for (int32_t g = lane; g < groups; g += kFinLanes) {
-      a += (double)w.part[(int64_t)g * K + k];
-      n += w.count[(int64_t)g * (K + 1) + k];
-    }
-  s_sum[lane][c] = a;
-  s_cnt[lane][c] = n;
-  __syncthreads();
-  const double inv = s_live > 0 ? 1.0 / (double)s_live : 0.0;
-  if (threadIdx.x < kFinClasses) {
-    a = 0.0;
-    n = 0;
-    for (int l = 0; l < kFinLanes; ++l) {
-      a += s_sum[l][c];
-      n += s_cnt[l][c];
-    }
-    const double f = (double)n * inv / top_k, p = a * inv;
-    if (k < K) {
+  int64_t n = 0, live = 0;
+#pragma unroll 4
+  for (int32_t g = lane; g < groups; g += 64) {
+    a += (double)part[g];
+    n += count[g];
+    live += rows[g];
+  }
+  for (int d = 32; d; d >>= 1) {
+    a += __shfl_xor(a, d);
+    n += __shfl_xor(n, d);
+    live += __shfl_xor(live, d);
+  }
+  const double inv = live > 0 ? 1.0 / (double)live : 0.0;
+  const double f = (double)n * inv / top_k, p = a * inv;
+  if (lane == 0) {
+    if (in) {
       w.share[k] = (float)f;
       o.prob[k] = (float)p;
       o.counts[k] = n;
     }
-    double l = k < K ? f * p : 0.0;
-    for (int d = kFinClasses / 2; d; d >>= 1) l += __shfl_xor(l, d);
-    if (threadIdx.x == 0) {
-      if (blockIdx.x == 0) *w.scale = (float)((double)coef * K * inv);
-      __hip_atomic_store(&w.loss_part[blockIdx.x], l, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-      s_last = __hip_atomic_fetch_add(w.ticket, 1u, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT) ==
-               gridDim.x - 1;
-    }
+    s_loss[c] = in ? f * p : 0.0;
   }
   __syncthreads();
-  if (s_last && threadIdx.x == 0) {
-    double t = 0.0;
-    for (unsigned g = 0; g < gridDim.x; ++g)
-      t += __hip_atomic_load(&w.loss_part[g], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    *o.loss = (float)((double)coef * K * t);
+  if (threadIdx.x == 0) {
+    if (blockIdx.x == 0) *w.scale = (float)((double)coef * K * inv);
+    const double l = (s_loss[0] + s_loss[1]) + (s_loss[2] + s_loss[3]);
+    __hip_atomic_store(&w.loss_part[blockIdx.x], l, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    s_last = __hip_atomic_fetch_add(w.ticket, 1u, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT) ==
+             gridDim.x - 1;
   }
+  __syncthreads();
+  if (!s_last || c > 0) return;
+  double t = 0.0;
+  for (unsigned g = lane; g < gridDim.x; g += 64)
+    t += __hip_atomic_load(&w.loss_part[g], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  for (int d = 32; d; d >>= 1) t += __shfl_xor(t, d);
+  if (lane == 0) *o.loss = (float)((double)coef * K * t);
 }
 
 // no rows: everything is 0
@@ -172,7 +166,7 @@ int balance_loss(const ScoresView& s, const uint8_t* mask, int32_t top_k, float 
   int r = stats(v, mask, top_k, w, &groups, st);
   if (r) return r;
   hipLaunchKernelGGL(balance_finish_kernel,
-                     dim3((unsigned)((s.K + kFinClasses - 1) / kFinClasses)), dim3(1024), 0, st, w,
+                     dim3((unsigned)((s.K + kFinClasses - 1) / kFinClasses)), dim3(256), 0, st, w,
                      groups, s.K, top_k, coef, o);
   WGBM_LAUNCH_CHECK();
   if (!out.data) return 0;

@@ -20,8 +20,13 @@ struct MinF {
   __device__ __forceinline__ float operator()(float a, float b) const { return fminf(a, b); }
 };
 
-// part, count: [workgroups][K] (count: [workgroups][K + 1], the last the rows
-// that count); norm: a row's maximum and 1 / sum of e^(s - max) (0: left out)
+// whether a thread's registers also hold the next rows: two sets of scores, the
+// exponentials and the sums within what 16 waves of a workgroup can have
+template <typename F>
+constexpr bool kAhead = 2 * F::kWords + 2 * F::N <= 104;
+
+// part [K][workgroups], count [K + 1][workgroups] (the last: rows that count);
+// norm: a row's maximum and 1 / sum of e^(s - max) (0: left out)
 template <typename F>
 __global__ __launch_bounds__(F::kMax) void balance_stats_kernel(
     ScoresView s, const uint8_t* __restrict__ mask, int32_t top_k, int64_t blocks,
@@ -38,38 +43,54 @@ __global__ __launch_bounds__(F::kMax) void balance_stats_kernel(
   float acc[F::N];
 #pragma unroll
   for (int j = 0; j < F::N; ++j) acc[j] = 0.0f;
+  // the next rows' loads are in flight while these rows are summed
+  typename F::Regs next;
+  uint8_t next_want = 1;
+  const auto fetch = [&](int64_t b) {
+    const int64_t row = F::row(b), i = row < s.n ? row : s.n - 1;
+    if (mask) next_want = mask[i];
+    f.load(next, s, i);
+  };
+  if (kAhead<F>) fetch(blockIdx.x);
   for (int64_t b = blockIdx.x; b < blocks; b += gridDim.x) {
     const int64_t row = F::row(b);
     const bool in = row < s.n;
     const int64_t i = in ? row : s.n - 1;
-    const bool want = in && (!mask || mask[i]);
-    typename F::Regs v;
-    f.load(v, s, i);
+    if (!kAhead<F>) fetch(b);
+    typename F::Regs v = next;
+    const bool want = in && next_want;
+    if (kAhead<F> && b + gridDim.x < blocks) fetch(b + gridDim.x);
     f.trim(v);
+    if (!want) f.drop(v);
     float m = -__builtin_inff();
 #pragma unroll
     for (int j = 0; j < F::N; ++j) m = fmaxf(m, F::value(v, j));
     m = f.reduce(m, MaxF(), buf[0]);
     const float ms = safe_max(m);
-    float e[F::N], z = 0.0f;
+    float e[F::N], z[2] = {0.0f, 0.0f};
 #pragma unroll
     for (int j = 0; j < F::N; ++j) {
       e[j] = loss_expf(F::value(v, j) - ms);
-      z += e[j];
+      z[j % 2] += e[j];
     }
-    z = f.reduce(z, AddF(), buf[1]);
-    const bool live = want && !(z == 0.0f);
-    const float iz = live ? 1.0f / z : 0.0f;
+    z[0] = f.reduce(z[0] + z[1], AddF(), buf[1]);
+    const bool live = !(z[0] == 0.0f);  // (NaN is live)
+    const float iz = live ? 1.0f / z[0] : 0.0f;
 #pragma unroll
-    for (int j = 0; j < F::N; ++j) acc[j] += live ? e[j] * iz : 0.0f;
+    for (int j = 0; j < F::N; ++j) acc[j] = fmaf(e[j], iz, acc[j]);
     if (in && f.first_lane()) norm[i] = make_float2(ms, iz);
     // the best classes one after the other: the largest score after the last
-    // one taken, then the lowest class that has it.  (class numbers are exact
-    // in float32; a NaN is not after anything)
+    // one taken, then the lowest class that has it (a thread's classes ascend).
+    // Class numbers are exact in float32; a NaN is not after anything.
+    constexpr float kNone = 1e9f;
     float v0 = __builtin_inff(), c0 = -1.0f;
     for (int32_t t = 0; t < top_k; ++t) {
-      float best = m;
-      if (t > 0) {
+      float best = m, c = kNone;
+      if (t == 0) {
+#pragma unroll
+        for (int j = F::N - 1; j >= 0; --j)
+          c = F::value(v, j) == best ? (float)f.cls(j) : c;
+      } else {
         best = -__builtin_inff();
 #pragma unroll
         for (int j = 0; j < F::N; ++j) {
@@ -77,16 +98,15 @@ __global__ __launch_bounds__(F::kMax) void balance_stats_kernel(
           if (x < v0 || (x == v0 && (float)f.cls(j) > c0)) best = fmaxf(best, x);
         }
         best = f.reduce(best, MaxF(), buf[2]);
-      }
-      float c = 1e9f;
 #pragma unroll
-      for (int j = 0; j < F::N; ++j) {
-        const float k = (float)f.cls(j);
-        if (F::value(v, j) == best && (best < v0 || k > c0)) c = fminf(c, k);
+        for (int j = F::N - 1; j >= 0; --j) {
+          const float k = (float)f.cls(j);
+          if (F::value(v, j) == best && (best < v0 || k > c0)) c = k;
+        }
       }
       c = f.reduce(c, MinF(), buf[3]);
-      const bool took = live && best > -__builtin_inff() && c < 1e9f;
-      if (took && f.first_lane()) atomicAdd(&s_count[(int32_t)c], 1);
+      if (best > -__builtin_inff() && c < kNone && f.first_lane())
+        atomicAdd(&s_count[(int32_t)c], 1);
       v0 = best;
       c0 = c;
     }
@@ -95,12 +115,11 @@ __global__ __launch_bounds__(F::kMax) void balance_stats_kernel(
   f.sum_rows(acc, s_part);
   __syncthreads();
   for (int32_t k = threadIdx.x; k <= K; k += blockDim.x) {
-    if (k < K) part[(int64_t)blockIdx.x * K + k] = s_part[k];
-    count[(int64_t)blockIdx.x * (K + 1) + k] = s_count[k];
+    if (k < K) part[(int64_t)k * gridDim.x + blockIdx.x] = s_part[k];
+    count[(int64_t)k * gridDim.x + blockIdx.x] = s_count[k];
   }
 }
 
-// the shares as a thread's classes need them
 template <typename F>
 __global__ __launch_bounds__(F::kMax) void balance_grad_kernel(
     ScoresView s, const float2* __restrict__ norm, const float* __restrict__ share,
@@ -112,19 +131,30 @@ __global__ __launch_bounds__(F::kMax) void balance_grad_kernel(
   for (int j = 0; j < F::N; ++j) fk[j] = share[f.cls(j) < s.K ? f.cls(j) : s.K - 1];
   const float c = *scale;
   int turn = 0;
+  typename F::Regs next;
+  float2 next_norm;
+  const auto fetch = [&](int64_t b) {
+    const int64_t row = F::row(b), i = row < s.n ? row : s.n - 1;
+    next_norm = norm[i];
+    f.load(next, s, i);
+  };
+  if (kAhead<F>) fetch(blockIdx.x);
   for (int64_t b = blockIdx.x; b < blocks; b += gridDim.x, turn ^= 1) {
     const int64_t row = F::row(b);
     const bool in = row < s.n;
     const int64_t i = in ? row : s.n - 1;
-    const float2 nm = norm[i];
-    typename F::Regs v;
-    f.load(v, s, i);
+    if (!kAhead<F>) fetch(b);
+    typename F::Regs v = next;
+    const float2 nm = next_norm;
+    if (kAhead<F> && b + gridDim.x < blocks) fetch(b + gridDim.x);
     f.trim(v);
     const bool live = in && nm.y != 0.0f;  // (NaN is live)
-    float q = 0.0f;
+    float e[F::N], q = 0.0f;
 #pragma unroll
-    for (int j = 0; j < F::N; ++j)
-      q = fmaf(fk[j], loss_expf(F::value(v, j) - nm.x), q);
+    for (int j = 0; j < F::N; ++j) {
+      e[j] = loss_expf(F::value(v, j) - nm.x);
+      q = fmaf(fk[j], e[j], q);
+    }
     // (two turns' words: a wave may be one reduction ahead of the others)
     q = f.reduce(q, AddF(), buf[turn]) * nm.y;
     if (!in) continue;
@@ -133,9 +163,7 @@ __global__ __launch_bounds__(F::kMax) void balance_grad_kernel(
       continue;
     }
     const float cz = c * nm.y;
-    f.store(out, i, accumulate, [&](int j) {
-      return cz * loss_expf(F::value(v, j) - nm.x) * (fk[j] - q);
-    });
+    f.store(out, i, accumulate, [&](int j) { return cz * e[j] * (fk[j] - q); });
   }
 }
 

@@ -32,6 +32,39 @@ __device__ __forceinline__ int32_t row_label(const int32_t* label, int64_t i, in
   return a >= 0 && a < K ? a : -1;
 }
 
+template <typename T>
+__device__ __forceinline__ float score_at(const ScoresView& s, int64_t i, int32_t k) {
+  return to_f32(((const T*)s.data)[i * s.rs + k * s.ks]);
+}
+
+// g (1[k = a] - softmax), the log-probability's gradient, from the row's norm
+// (c.iz is the logarithm of its sum)
+template <typename T>
+struct LogProbGrad {
+  const int32_t* label;
+  const float2* norm;
+  const float* grad;
+  static constexpr bool kRef = false;
+  __device__ __forceinline__ RowCoef row(const ScoresView& s, int64_t i) const {
+    RowCoef c{};
+    const int32_t a = row_label(label, i, s.K);
+    const float g = grad[i];
+    const float2 v = norm[i];
+    if (a < 0 || g == 0.0f || v.x == -__builtin_inff()) return c;
+    c.m = v.x;
+    c.iz = v.y;
+    c.c0 = -g;
+    // the label's from its own logarithm: 1 - p without a difference
+    c.gl = c.c0 * expm1f((score_at<T>(s, i, a) - v.x) - v.y);
+    c.label = a;
+    c.live = 1;
+    return c;
+  }
+  __device__ __forceinline__ float at(const RowCoef& c, float s, float) const {
+    return c.c0 * loss_expf((s - c.m) - c.iz);
+  }
+};
+
 // ---------------------------------------------------------------------------
 // reductions over a group of G lanes (a power of two up to 64, aligned); every
 // lane gets the same bits (each step combines two values that commute)
@@ -91,6 +124,7 @@ template <typename T_, int G_, int NC_>
 struct RowFrame {
   using T = T_;
   static constexpr int G = G_, NC = NC_, VE = Chunk<T>::VE, N = NC * VE;
+  static constexpr int kWords = 4 * NC;  // registers of a thread's scores
   static constexpr int kThreads = G <= 256 ? 256 : G, kMax = kThreads;
   static constexpr bool kBarrier = G > 64, kSlices = false;
   static constexpr int kRows = kThreads / G;  // rows of a workgroup
@@ -127,6 +161,13 @@ struct RowFrame {
           r.c[c].v[e] = e < sk ? (T)(-__builtin_inff()) : r.c[c].v[e];
       }
     }
+  }
+  // a row that is left out has no class
+  __device__ __forceinline__ void drop(Regs& r) const {
+#pragma unroll
+    for (int c = 0; c < NC; ++c)
+#pragma unroll
+      for (int e = 0; e < VE; ++e) r.c[c].v[e] = (T)(-__builtin_inff());
   }
   static __device__ __forceinline__ float value(const Regs& r, int j) {
     return to_f32(r.c[j / VE].v[j % VE]);
@@ -220,7 +261,7 @@ struct RowFrame {
 template <typename T_, int N_, bool SLICES>
 struct ClassFrame {
   using T = T_;
-  static constexpr int N = N_;
+  static constexpr int N = N_, kWords = N_;
   static constexpr int kMax = SLICES ? 1024 : 256;
   static constexpr bool kBarrier = SLICES, kSlices = SLICES;
   static constexpr int kBuf = SLICES ? 16 * 64 : 1;
@@ -250,6 +291,10 @@ struct ClassFrame {
   __device__ __forceinline__ void trim(Regs& r) const {
 #pragma unroll
     for (int j = 0; j < N; ++j) r.c[j] = cls(j) < K ? r.c[j] : (T)(-__builtin_inff());
+  }
+  __device__ __forceinline__ void drop(Regs& r) const {
+#pragma unroll
+    for (int j = 0; j < N; ++j) r.c[j] = (T)(-__builtin_inff());
   }
   static __device__ __forceinline__ float value(const Regs& r, int j) { return to_f32(r.c[j]); }
 

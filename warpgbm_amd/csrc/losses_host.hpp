@@ -37,6 +37,9 @@ int class_log_probs_grad(const ScoresView& s, const int32_t* label, const float*
 // rows that fit a thread group's registers, one launch (losses_rows_*.hip);
 // *done = false where they do not
 #define LOSS_ROWS(t)                                                                             \
+  int log_probs_grad_rows_##t(const ScoresView& s, const int32_t* label, const float* norm,      \
+                              const float* grad, const ScoresView& out, hipStream_t st,          \
+                              bool* done);                                                       \
   int log_probs_rows_##t(const ScoresView& s, const int32_t* label, float* log_prob, float* norm, \
                          hipStream_t st, bool* done);                                            \
   int policy_rows_##t(const ScoresView& s, const ScoresView& ref, const PolicyRows& g,           \
@@ -59,10 +62,10 @@ struct BalanceWs {
   uint32_t* ticket;
   float* scale;
   float* share;       // [K]
-  double* loss_part;  // [K / 16 + 1]
+  double* loss_part;  // [K / 4 + 1]
   float2* norm;       // [n]
-  float* part;        // [workgroups][K]
-  int32_t* count;     // [workgroups][K + 1]
+  float* part;        // [K][workgroups]
+  int32_t* count;     // [K + 1][workgroups]
   void* rows;         // a row-major copy of the scores, where one is needed
   size_t bytes;
 };
@@ -79,23 +82,37 @@ int balance_loss(const ScoresView& s, const uint8_t* mask, int32_t top_k, float 
                  const BalanceOut& o, const ScoresView& out, bool accumulate, void* ws,
                  hipStream_t st);
 
+// (the tables as in wgbm_preference_args)
 struct PreferenceArgs {
   const float* log_prob;
   const float* ref;
   int64_t n_rows;
   const int64_t* seg_start;  // null: every row is a sequence of its own
   int64_t n_seg;
-  const int32_t* pairs;      // [n_pairs][2]: preferred, other
+  const int32_t* pairs;
   int64_t n_pairs;
-  const int32_t* inc;        // [2 n_pairs]: 2 * pair + side, grouped by sequence
-  const int64_t* inc_start;  // [n_seg + 1]
+  const int32_t* inc;
+  const int64_t* inc_start;
+  const int64_t* share;
+  int64_t n_shares;
+  const uint8_t* is_long;
+  const int64_t* task;
+  int64_t n_tasks;
+  const int64_t* task_start;  // null: task t < n_seg is sequence t
+  const int64_t* piece;
+  int64_t n_pieces;
+  const int64_t* multi;
+  int64_t n_multi;
+  const int64_t* idle;
+  int64_t n_idle;
+  bool disjoint;
   const float* weight;
   float beta, smooth;
   float* loss;
   float* margin;
   float* grad;
 };
-size_t preference_workspace(int64_t n_seg, int64_t n_pairs, bool segments);
+size_t preference_workspace(const PreferenceArgs& a);
 int preference_loss(const PreferenceArgs& a, void* ws, hipStream_t st);
 
 }  // namespace wgbm

@@ -45,11 +45,6 @@ __device__ __forceinline__ RowStats frame_stats(const F& f, const typename F::Re
   return a;
 }
 
-template <typename T>
-__device__ __forceinline__ float score_at(const ScoresView& s, int64_t i, int32_t k) {
-  return to_f32(((const T*)s.data)[i * s.rs + k * s.ks]);
-}
-
 template <typename F>
 __global__ __launch_bounds__(F::kMax) void log_probs_frame_kernel(
     ScoresView s, const int32_t* __restrict__ label, float* __restrict__ log_prob,
@@ -70,6 +65,22 @@ __global__ __launch_bounds__(F::kMax) void log_probs_frame_kernel(
   const LogProb lp = row_log_prob(a, sa);
   log_prob[i] = lp.live && lab >= 0 ? (float)lp.logp : 0.0f;
   norm[i] = lp.live ? make_float2(lp.m, (float)lp.l) : make_float2(-__builtin_inff(), 0.0f);
+}
+
+// (no reduction: the norm is given)
+template <typename F>
+__global__ __launch_bounds__(F::kMax) void log_probs_grad_frame_kernel(
+    ScoresView s, LogProbGrad<typename F::T> g, ScoresView out) {
+  const F f(s);
+  const int64_t i = F::row(blockIdx.x);
+  if (i >= s.n) return;
+  typename F::Regs v;
+  f.load(v, s, i);
+  const RowCoef c = g.row(s, i);
+  f.store(out, i, false, [&](int j) {
+    const float x = g.at(c, F::value(v, j), 0.0f);
+    return !c.live ? 0.0f : f.cls(j) == c.label ? c.gl : x;
+  });
 }
 
 template <typename F, bool REF>
@@ -190,6 +201,22 @@ static int log_probs_frames(const ScoresView& s, const int32_t* label, float* lo
     using F = typename decltype(tag)::type;
     hipLaunchKernelGGL((log_probs_frame_kernel<F>), dim3((unsigned)blocks), dim3(threads), 0, st, s,
                        label, log_prob, (float2*)norm);
+  };
+  *done = by_class_frame<T>(s) ? pick_class_frame<T, false>(s, launch)
+                               : pick_row_frame<T, false>(s, launch);
+  if (*done) WGBM_LAUNCH_CHECK();
+  return 0;
+}
+
+template <typename T>
+static int log_probs_grad_frames(const ScoresView& s, const int32_t* label, const float* norm,
+                                 const float* grad, const ScoresView& out, hipStream_t st,
+                                 bool* done) {
+  const LogProbGrad<T> g{label, (const float2*)norm, grad};
+  const auto launch = [&](auto tag, int64_t blocks, int threads) {
+    using F = typename decltype(tag)::type;
+    hipLaunchKernelGGL((log_probs_grad_frame_kernel<F>), dim3((unsigned)blocks), dim3(threads), 0,
+                       st, s, g, out);
   };
   *done = by_class_frame<T>(s) ? pick_class_frame<T, false>(s, launch)
                                : pick_row_frame<T, false>(s, launch);

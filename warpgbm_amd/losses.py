@@ -286,30 +286,111 @@ class PreferencePlan:
         if P >= 1 << 30:
             raise RuntimeError("at most 2^30 - 1 pairs")
         self.n_pairs = P
-        self.sequence_start = None
+        seg = None
         S = self.n_rows
         if segments is not None:
             seg = self._whole_numbers(segments, "segments").to(device=device, dtype=torch.int64)
             if seg.dim() != 1 or seg.shape[0] < 1:
                 raise RuntimeError("segments must be the offsets [S + 1] of S sequences")
             S = seg.shape[0] - 1
-            if int(seg[0]) != 0 or int(seg[-1]) > self.n_rows or bool((seg[1:] < seg[:-1]).any()):
-                raise RuntimeError(f"segments must ascend from 0 to at most n_rows={self.n_rows}")
-            self.sequence_start = seg.clone()
-        if S >= 1 << 31:
-            raise RuntimeError("too many sequences")
+            seg = seg.clone()
+        if S >= 1 << 30:
+            raise RuntimeError("at most 2^30 - 1 sequences")
         self.n_sequences = S
+        self.sequence_start = seg
         pairs = pairs.to(device=device, dtype=torch.int64)
-        if P and (int(pairs.min()) < 0 or int(pairs.max()) >= S):
-            raise RuntimeError(f"pairs must hold sequence numbers in [0, {S})")
+        # (each .tolist() waits for the GPU)
+        if seg is not None:
+            length = seg.diff()
+            first, last, least, longest = torch.stack(
+                [seg[0], seg[-1], length.min() if S else seg[0], length.max() if S else seg[0]]
+            ).tolist()
+            if first != 0 or last > self.n_rows or (S and least < 0):
+                raise RuntimeError(f"segments must ascend from 0 to at most n_rows={self.n_rows}")
+        if P:
+            least, most = torch.stack(list(pairs.aminmax())).tolist()
+            if least < 0 or most >= S:
+                raise RuntimeError(f"pairs must hold sequence numbers in [0, {S})")
         self.pairs = pairs.to(torch.int32).contiguous().clone()
-        # the numbers 2 * pair + side grouped by sequence (a stable sort: in
-        # pair order), and each sequence's range of them
+        self.task = self.task_start = self.piece = self.multi = self.idle = None
+        self.disjoint = False
+        degree = self._incidences(device)
+        if seg is not None:
+            self._tasks(seg, length, last, longest, degree, device)
+
+    # rows of a wave's task; pairs of a sequence from which on it is summed by
+    # workgroups of its own, and the pairs of one of these
+    _TASK, _LONG, _PIECE = 4096, 256, 8192
+    # sequences and pairs' sides, together, of a workgroup that sums the others
+    _SHARE = 1024
+
+    @staticmethod
+    def _cut(first, end, size):
+        """The ranges [first, end) cut into pieces of size (at least one each):
+        (number of the range, first, end) of every piece, and the ranges' offsets
+        in that list."""
+        n = ((end - first + size - 1) // size).clamp(min=1)
+        start = torch.zeros(n.shape[0] + 1, dtype=torch.int64, device=n.device)
+        torch.cumsum(n, 0, out=start[1:])
+        of = torch.repeat_interleave(torch.arange(n.shape[0], device=n.device), n)
+        at = first[of] + (torch.arange(of.shape[0], device=n.device) - start[of]) * size
+        return torch.stack([of, at, torch.minimum(at + size, end[of])], 1), start
+
+    def _incidences(self, device):
+        """The numbers 2 * pair + side grouped by sequence, in pair order (a
+        stable sort), the sequences in very many pairs last.  Returns the largest
+        number of pairs of a sequence."""
+        S = self.n_sequences
         ends = self.pairs.reshape(-1)
-        order = torch.sort(ends, stable=True)
-        self.incidence = order.indices.to(torch.int32)
-        self.incidence_start = torch.searchsorted(
-            order.values, torch.arange(S + 1, dtype=torch.int32, device=device))
+        degree = torch.bincount(ends, minlength=S) if S else ends.long()
+        most = int(degree.max()) if S else 0
+        key = ends
+        if most > self._LONG:
+            long = degree > self._LONG
+            key = torch.where(long[ends.long()], ends.long() + S, ends.long())
+        self.incidence = torch.sort(key, stable=True).indices.to(torch.int32)
+        short = degree if most <= self._LONG else degree.masked_fill(long, 0)
+        self.incidence_start = torch.zeros(S + 1, dtype=torch.int64, device=device)
+        torch.cumsum(short, 0, out=self.incidence_start[1:])
+        # a run's first sequence: the first whose number and incidences before it
+        # reach the run's start
+        before = self.incidence_start + torch.arange(S + 1, device=device)
+        runs = (S + (2 * self.n_pairs if most <= self._LONG else int(before[-1]) - S)
+                + self._SHARE - 1) // self._SHARE
+        cuts = torch.arange(runs + 1, device=device) * self._SHARE
+        self.share = torch.searchsorted(before, cuts).clamp(max=S)
+        self.is_long = None
+        if most > self._LONG:
+            self.is_long = long.to(torch.uint8)
+            who = long.nonzero()[:, 0]
+            end = self.incidence_start[-1] + degree[who].cumsum(0)
+            self.piece, start = self._cut(end - degree[who], end, self._PIECE)
+            several = start.diff() > 1
+            of = self.piece[:, 0]
+            self.piece[:, 0] = torch.where(several[of], torch.full_like(of, -1), who[of])
+            self.multi = torch.stack([who, start[:-1], start[1:]], 1)[several].contiguous()
+        return most
+
+    def _tasks(self, seg, length, last, longest, most, device):
+        """The rows of every sequence, and those behind the last one, in tasks of
+        a wave."""
+        S, n = self.n_sequences, self.n_rows
+        tail = None
+        if last < n:
+            tail = self._cut(seg[-1:], torch.full_like(seg[-1:], n), self._TASK)[0]
+            tail[:, 0] = -1
+        if longest > self._TASK:
+            task, self.task_start = self._cut(seg[:-1], seg[1:], self._TASK)
+        else:
+            task = torch.stack([torch.arange(S, device=device), seg[:-1], seg[1:]], 1)
+        if most <= 1 and self.task_start is None:
+            self.disjoint = True
+            free = torch.diff(self.incidence_start) == 0
+            free &= length > 0
+            task = task[free]
+        self.task = (task if tail is None else torch.cat([task, tail])).contiguous()
+        if self.disjoint:
+            self.idle, self.task = self.task[:, 1:].contiguous(), None
 
     @staticmethod
     def _whole_numbers(a, name):
@@ -317,6 +398,10 @@ class PreferencePlan:
         if t.dtype not in (torch.int32, torch.int64):
             raise RuntimeError(f"{name} must be int32 or int64, got {t.dtype}")
         return t
+
+
+def _table(t):
+    return (None, 0) if t is None else (t.data_ptr(), t.shape[0])
 
 
 def preference_loss(log_prob, plan, *, ref_log_prob=None, weight=None, beta=1.0,
@@ -341,7 +426,11 @@ def preference_loss(log_prob, plan, *, ref_log_prob=None, weight=None, beta=1.0,
     seg = plan.sequence_start
     args = _lib.PreferenceArgs(
         lp, rp, n, seg.data_ptr() if seg is not None else None, plan.n_sequences,
-        plan.pairs.data_ptr(), P, plan.incidence.data_ptr(), plan.incidence_start.data_ptr(), w,
+        plan.pairs.data_ptr(), P, plan.incidence.data_ptr(), plan.incidence_start.data_ptr(),
+        plan.share.data_ptr(), plan.share.shape[0] - 1,
+        plan.is_long.data_ptr() if plan.is_long is not None else None,
+        *_table(plan.task), plan.task_start.data_ptr() if plan.task_start is not None else None,
+        *_table(plan.piece), *_table(plan.multi), *_table(plan.idle), int(plan.disjoint), w,
         float(beta), float(label_smoothing))
     lib = _lib.load()
     with _on(dev):
