@@ -33,10 +33,10 @@ __device__ __forceinline__ RowStats scan_classes(const T* s, const T* r, int64_t
       mr = fmaxf(mr, w[j]);
     }
     rebase_stats<REF>(a, m, mr);
-    const float ms = safe_max(m), mrs = safe_max(mr);
+    const Base b = base_of(safe_max(m)), br = base_of(safe_max(mr));
 #pragma unroll
     for (int j = 0; j < U; ++j)
-      add_class<REF>(a, v[j] - ms, w[j] - mrs, k + j * step == label);
+      add_class<REF>(a, power_of(v[j], b), power_of(w[j], br), k + j * step == label);
   }
   return a;
 }
@@ -108,9 +108,7 @@ __global__ __launch_bounds__(256) void log_prob_rows_kernel(ScoresView s,
   if (wave && (threadIdx.x & 63)) return;
   const int32_t lab = row_label(label, i, s.K);
   const float sa = lab >= 0 ? to_f32(((const T*)s.data)[i * s.rs + lab * s.ks]) : 0.0f;
-  const LogProb lp = row_log_prob(a, sa);
-  if (log_prob) log_prob[i] = lp.live && lab >= 0 ? (float)lp.logp : 0.0f;
-  norm[i] = lp.live ? make_float2(lp.m, (float)lp.l) : make_float2(-__builtin_inff(), 0.0f);
+  write_log_prob(a, sa, lab, i, log_prob, norm);
 }
 
 // log p of the label in float64, by the 64 lanes of a wave
@@ -137,10 +135,7 @@ __global__ __launch_bounds__(256) void policy_rows_kernel(ScoresView s, ScoresVi
   const float w = !in ? 0.0f : g.weight ? g.weight[i] : 1.0f;
   const int32_t lab = in ? row_label(g.action, i, s.K) : -1;
   const bool live = w != 0.0f && lab >= 0;
-  PolicyRow o;
-  o.near = false;
-  o.loss = o.logp = o.kl = 0.0f;
-  o.c = RowCoef{};
+  PolicyRow o{};
   RowStats a = empty_stats();
   float sa = 0.0f, ra = 0.0f, A = 0.0f, old = 0.0f;
   if (live) {
@@ -158,7 +153,7 @@ __global__ __launch_bounds__(256) void policy_rows_kernel(ScoresView s, ScoresVi
     todo &= todo - 1;
     const int64_t row = wave ? i : (t & ~63ll) + src;
     const double e = wave_exact_logp((const T*)s.data + row * s.rs, s.ks, s.K,
-                                     __shfl(lab, src), __shfl(o.c.m, src));
+                                     __shfl(lab, src), __shfl(a.m, src));
     if ((threadIdx.x & 63) == src || wave)
       o = policy_row<REF>(a, sa, ra, A, old, w, g, i, lab, &e);
   }
@@ -223,38 +218,32 @@ __global__ __launch_bounds__(256) void score_grad_kernel(ScoresView s, ScoresVie
   const T* q = G::kRef ? (const T*)ref.data + i * ref.rs : nullptr;
   T* o = (T*)out.data + i * out.rs;
   for (int32_t k = k0 + (int)(threadIdx.x & 63) * VE; k < k1; k += 64 * VE) {
-    Chunk<T> v, r, old;
     const int m = k1 - k < VE ? k1 - k : VE;
-    if (!c.live) {
-      if (accumulate) continue;
-      for (int j = 0; j < VE; ++j) v.v[j] = from_f32<T>(0.0f);
-    } else {
-      if (m == VE) {
-        v = load_chunk<T>(p + k);
-        if (G::kRef) r = load_chunk<T>(q + k);
-        if (accumulate) old = load_chunk<T>(o + k);
-      } else {
-        for (int j = 0; j < VE; ++j) {
-          const int kk = k + (j < m ? j : 0);
-          v.v[j] = p[kk];
-          if (G::kRef) r.v[j] = q[kk];
-          if (accumulate) old.v[j] = o[kk];
+    if (m < VE || !c.live) {
+      for (int j = 0; j < m; ++j) {
+        float x = 0.0f;
+        if (c.live) {
+          const float sv = to_f32(p[k + j]), rv = G::kRef ? to_f32(q[k + j]) : 0.0f;
+          x = k + j == c.label ? c.gl : g.at(c, sv, rv);
+        } else if (accumulate) {
+          break;
         }
+        if (accumulate) x += to_f32(o[k + j]);
+        o[k + j] = from_f32<T>(x);
       }
+      continue;
+    }
+    Chunk<T> v = load_chunk<T>(p + k), r, old;
+    if (G::kRef) r = load_chunk<T>(q + k);
+    if (accumulate) old = load_chunk<T>(o + k);
+    float x[VE];
 #pragma unroll
-      for (int j = 0; j < VE; ++j) {
-        const float sv = to_f32(v.v[j]);
-        const float rv = G::kRef ? to_f32(r.v[j]) : 0.0f;
-        float x = k + j == c.label ? c.gl : g.at(c, sv, rv);
-        if (accumulate) x += to_f32(old.v[j]);
-        v.v[j] = from_f32<T>(x);
-      }
+    for (int j = 0; j < VE; ++j) {
+      x[j] = k + j == c.label ? c.gl : g.at(c, v.get(j), G::kRef ? r.get(j) : 0.0f);
+      if (accumulate) x[j] += old.get(j);
     }
-    if (m == VE) {
-      store_chunk<T>(o + k, v);
-    } else {
-      for (int j = 0; j < m; ++j) o[k + j] = v.v[j];
-    }
+    v.set(x);
+    store_chunk<T>(o + k, v);
   }
 }
 

@@ -40,11 +40,18 @@ struct PolicyRows {
   float* kl;
 };
 
-// what a row's gradient is made of: with d = s - m, p_k = exp(d_k) * iz,
-//   g_k = p_k * (c1 * (d_k - (r_k - mr)) + c0),  and at the label g_a = gl
-// (c1 and mr only with reference scores).  live = 0: the row's gradient is 0.
+// a row's maximum as the exponentials take it: 2^(s lg - m2) = e^(s - m)
+struct Base {
+  float m2, lg;
+};
+
+// what a row's gradient is made of: with h = s lg - m2 of the scores' base and
+// hr of the reference's, 2^h = e^(s - max) and
+//   g_k = 2^h (c1 (h - hr) + c0),  and at the label g_a = gl
+// (c1 and br only with reference scores).  live = 0: the row's gradient is 0.
 struct RowCoef {
-  float m, iz, c0, c1, mr, gl;
+  Base b, br;
+  float c0, c1, gl;
   int32_t label;
   int32_t live;
 };
@@ -62,21 +69,32 @@ __device__ __forceinline__ T from_f32(float v) {
   return (T)v;
 }
 
-// e^x for x <= 0 (-inf gives 0, NaN stays): v_exp_f32 of x log2(e).  The
-// product's rounding costs |x| 2^-24 of the value, that is at most 2^-25 of the
-// row's largest exponential (|x| e^x has its maximum 1/e): what a softmax's sums
-// and gradients are rounded by anyway.  Taking the rounding error along would
-// cost six instructions more, as much again as the exponential (the balance
-// loss's first pass over 1M x 100 classes is bound by instructions then).
-__device__ __forceinline__ float loss_expf(float x) {
-  return __builtin_amdgcn_exp2f(x * 1.44269504088896340736f);
+// Exponentials: e^(s - m) = 2^(s lg - m2), lg = log2(e), m2 = m lg rounded: one
+// fused multiply-add and v_exp_f32.  The fused result's rounding costs |h| 2^-24
+// of the value, that is at most 2^-25 of the row's largest exponential (|x| e^-x
+// has its maximum 1/e): what a softmax's sums and gradients are rounded by
+// anyway.  The rounding of m2 is a factor that all classes of the row share and
+// that every quotient loses; row_log_prob takes it out of the sum's logarithm.
+// The losses are bound by instructions as much as by memory (a 16-bit score and
+// its gradient are 4 bytes, about 30 instructions at this GPU's rates).
+constexpr float kLog2e = 1.44269504088896340736f;
+constexpr double kLn2 = 0.693147180559945309417;
+// (m: finite.  A maximum near the type's ends, a row whose classes are all
+// masked by the type's lowest value, would overflow; scores that far out differ
+// by 10^30 or not at all, so that any factor will do: 1.)
+__device__ __forceinline__ Base base_of(float m) {
+  const float lg = fabsf(m) > 1e38f ? 1.0f : kLog2e;
+  return {m * lg, lg};
 }
+__device__ __forceinline__ float power_of(float s, const Base& b) {
+  return fmaf(s, b.lg, -b.m2);
+}
+__device__ __forceinline__ float exp2_f32(float h) { return __builtin_amdgcn_exp2f(h); }
 
 // running maximum and sums of a set of a row's classes, all in float32:
-//   m = max s_k, z = sum of e^(s_k - m) over the classes but the label,
-//   za = the label's e^(s_a - m) (0 when it is in another set); with
-//   reference scores r: mr = max r_k, zr = sum of e^(r_k - mr),
-//   u = sum of e^(s_k - m) ((s_k - m) - (r_k - mr))
+//   m = max s_k, z = sum of 2^h_k over the classes but the label (h as above),
+//   za = the label's 2^h_a (0 when it is in another set); with reference scores
+//   r: mr = max r_k, zr = sum of 2^hr_k, u = sum of 2^h_k (h_k - hr_k)
 // The label is summed apart so that 1 - p_a = z / (z + za) keeps its digits
 // for a row that is sure of its label.
 struct RowStats {
@@ -94,12 +112,14 @@ __device__ __forceinline__ float safe_max(float m) { return m == -__builtin_inff
 // the same statistics relative to the larger maxima m and mr
 template <bool REF>
 __device__ __forceinline__ void rebase_stats(RowStats& a, float m, float mr) {
-  const float ms = safe_max(m), f = loss_expf(a.m - ms);  // 0 for an empty set
+  // (differences of the rounded scaled maxima, as the classes' own powers have)
+  const float b = base_of(safe_max(m)).m2 - base_of(safe_max(a.m)).m2;
+  const float f = a.m == -__builtin_inff() ? 0.0f : exp2_f32(-b);  // 0 for an empty set
   if (REF) {
-    const float mrs = safe_max(mr), t = a.z + a.za;
-    // an empty set has no difference to move (its maxima are -inf)
-    if (t != 0.0f) a.u = f * (a.u + ((a.m - ms) - (safe_max(a.mr) - mrs)) * t);
-    a.zr *= loss_expf(a.mr - mrs);
+    const float br = base_of(safe_max(mr)).m2 - base_of(safe_max(a.mr)).m2, t = a.z + a.za;
+    // a set that counts for nothing has no difference to move
+    a.u = t != 0.0f && f != 0.0f ? f * (a.u + (br - b) * t) : 0.0f;
+    a.zr *= a.mr == -__builtin_inff() ? 0.0f : exp2_f32(-br);
     a.mr = mr;
   }
   a.z *= f;
@@ -107,19 +127,19 @@ __device__ __forceinline__ void rebase_stats(RowStats& a, float m, float mr) {
   a.m = m;
 }
 
-// one more class: e is e^(s - m), d = s - m, dr = r - mr, er = e^(r - mr)
+// one more class of powers h and hr
 template <bool REF>
-__device__ __forceinline__ void add_class(RowStats& a, float d, float dr, bool is_label) {
-  const float e = loss_expf(d);
+__device__ __forceinline__ void add_class(RowStats& a, float h, float hr, bool is_label) {
+  const float e = exp2_f32(h);
   if (is_label)
     a.za += e;
   else
     a.z += e;
   if (REF) {
-    a.zr += loss_expf(dr);
+    a.zr += exp2_f32(hr);
     // a class of probability 0 takes no part in the divergence, whatever the
     // reference says of it (both are -inf at classes that a row may not take)
-    a.u += e == 0.0f ? 0.0f : e * (d - dr);
+    a.u += e == 0.0f ? 0.0f : e * (h - hr);
   }
 }
 
@@ -140,24 +160,60 @@ __device__ __forceinline__ RowStats join_stats(RowStats a, RowStats b) {
 // ---------------------------------------------------------------------------
 // what follows from a row's statistics
 // ---------------------------------------------------------------------------
-// (float64 from the row's sum on: the logarithm of many classes' sum, some
-// ten, would lose a digit in float32 that the ratio and the divergence of a
-// policy near its reference need)
-struct LogProb {
-  double logp, l;  // l = log of the sum of e^(s - m)
-  float m;
-  bool live;  // the row has a class
+// Logarithms of float32 sums to some 10^-8, with the exponent's part in float64:
+// log2(z) = k + log2(f), f in [0.7, 1.41), where a float32 logarithm's absolute
+// error is 2^-25.  (A float32 logarithm of many classes' sum, some ten, would
+// lose a digit that the ratio and the divergence of a policy near its reference
+// need; a float64 one costs as much as ten classes.)
+struct Split {
+  float k, f;
 };
-
-// sa: the label's score
-__device__ __forceinline__ LogProb row_log_prob(const RowStats& a, float sa) {
-  const float z = a.z + a.za;
-  LogProb o;
-  o.live = !(z == 0.0f);  // (NaN is live: it shows in the results)
-  o.m = safe_max(a.m);
-  o.l = log((double)z);
-  o.logp = ((double)sa - (double)o.m) - o.l;
+__device__ __forceinline__ Split split_f32(float z) {
+  Split o{(float)__builtin_amdgcn_frexp_expf(z), __builtin_amdgcn_frexp_mantf(z)};
+  if (o.f < 0.70710678f) {
+    o.f *= 2.0f;
+    o.k -= 1.0f;
+  }
   return o;
+}
+// (v_log_f32: the logarithm to base 2 of a normal number)
+__device__ __forceinline__ float log2_f32(float f) { return __builtin_amdgcn_logf(f); }
+__device__ __forceinline__ double log_of(float z) {
+  const Split s = split_f32(z);
+  return ((double)s.k + (double)log2_f32(s.f)) * kLn2;
+}
+// log2(a / b)
+__device__ __forceinline__ double log2_ratio(float a, float b) {
+  const Split x = split_f32(a), y = split_f32(b);
+  return (double)(x.k - y.k) + (double)(log2_f32(x.f) - log2_f32(y.f));
+}
+// log(1 + q) for q in [0, 1]: the logarithm of the rounded sum, and what the
+// rounding left out
+__device__ __forceinline__ float log1p_of(float q) {
+  const float w = 1.0f + q;
+  return fmaf(log2_f32(w), (float)kLn2, (q - (w - 1.0f)) * __builtin_amdgcn_rcpf(w));
+}
+// e^x within 2 ulp: the product's rounding taken along
+__device__ __forceinline__ float exp_of(float x) {
+  const float h = x * kLog2e, lo = fmaf(x, kLog2e, -h), e = exp2_f32(h);
+  return fabsf(h) < 200.0f ? fmaf(e, lo * (float)kLn2, e) : e;  // (no inf * 0)
+}
+
+// logarithm of a sum of 2^(s lg - m2), the rounding of m2 taken out
+__device__ __forceinline__ double sum_log(float z, float m) {
+  const Base b = base_of(m);
+  return log_of(z) + kLn2 * ((double)b.m2 - (double)m * (double)b.lg);
+}
+__device__ __forceinline__ bool row_live(const RowStats& a) {
+  return !(a.z + a.za == 0.0f);  // the row has a class (NaN: it shows in the results)
+}
+// log-probability of the label, whose score is sa.  A label of at least half:
+// from the others' share, which keeps the digits of a row that is sure of its
+// label (and the sign).
+__device__ __forceinline__ double row_log_prob(const RowStats& a, float sa) {
+  const float m = safe_max(a.m);
+  if (a.za >= a.z) return -(double)log1p_of(a.z / a.za);
+  return ((double)sa - (double)m) - sum_log(a.z + a.za, m);
 }
 
 // The policy loss of one row and its gradient's coefficients.
@@ -179,21 +235,21 @@ __device__ __forceinline__ PolicyRow policy_row(const RowStats& st, float sa, fl
                                                 float old, float w, const PolicyRows& g, int64_t i,
                                                 int32_t label, const double* exact_logp) {
   PolicyRow o;
-  const LogProb lp = row_log_prob(st, sa);
-  const float z = st.z + st.za;
-  o.c.m = lp.m;
-  o.c.iz = 1.0f / z;
+  const float z = st.z + st.za, iz = __builtin_amdgcn_rcpf(z);
+  o.c.b = base_of(safe_max(st.m));
+  o.c.br = REF ? base_of(safe_max(st.mr)) : o.c.b;
   o.c.label = label;
-  o.c.live = lp.live;
+  o.c.live = row_live(st);
   o.near = false;
-  if (!lp.live) {
+  if (!o.c.live) {
     o.loss = o.logp = o.kl = 0.0f;
-    o.c.c0 = o.c.c1 = o.c.mr = o.c.gl = o.c.iz = 0.0f;
+    o.c.c0 = o.c.c1 = o.c.gl = 0.0f;
     return o;
   }
-  o.logp = (float)lp.logp;
-  const float x = (float)(lp.logp - (double)old);
-  const float ratio = expf(x);
+  const double logp = row_log_prob(st, sa);
+  o.logp = (float)logp;
+  const float x = (float)(logp - (double)old);
+  const float ratio = exp_of(x);
   // positive advantages stop above the upper border, negative ones below the
   // lower
   const bool up = A > 0.0f;
@@ -216,14 +272,16 @@ __device__ __forceinline__ PolicyRow policy_row(const RowStats& st, float sa, fl
   o.kl = 0.0f;
   float wk = 0.0f, base = 0.0f;
   if (REF) {
-    const double lr = log((double)st.zr) - lp.l;
-    const double kl = (double)st.u / (double)z + lr;
-    o.kl = (float)kl;
-    base = (float)(lr - kl);  // log p_k - log q_k - KL = (d_k - dr_k) + base
+    // in powers of two: log2 p_k - log2 q_k = (h_k - hr_k) + lr, lr = log2 of
+    // the sums' quotient (the maxima's roundings are in both h and the sums)
+    const double lr = log2_ratio(st.zr, z);
+    const double kl = (double)(st.u / z) + lr;
+    o.kl = (float)(kLn2 * kl);
+    base = (float)(lr - kl);  // (log2 p_k - log2 q_k - KL2) - (h_k - hr_k)
     value += g.kl_coef * o.kl;
     wk = w * g.kl_coef;
   } else if (g.ref_log_prob) {
-    const float d = (float)((double)g.ref_log_prob[i] - lp.logp);
+    const float d = (float)((double)g.ref_log_prob[i] - logp);
     const float e = expm1f(d);
     o.kl = e - d;
     // near 0 the difference loses what the series keeps
@@ -234,22 +292,21 @@ __device__ __forceinline__ PolicyRow policy_row(const RowStats& st, float sa, fl
   }
   c *= w;
   o.loss = w * value;
-  const float pa = st.za / z;
-  o.c.c0 = wk * base - c;
-  o.c.c1 = wk;
-  o.c.mr = REF ? safe_max(st.mr) : 0.0f;
-  o.c.gl = c * (st.z / z);
-  if (REF && pa != 0.0f) o.c.gl += pa * wk * (((sa - lp.m) - (ra - o.c.mr)) + base);
+  const float wn = wk * (float)kLn2;
+  o.c.c0 = (wn * base - c) * iz;
+  o.c.c1 = wn * iz;
+  o.c.gl = c * (st.z * iz);
+  if (REF && st.za != 0.0f)
+    o.c.gl += st.za * iz * wn * ((power_of(sa, o.c.b) - power_of(ra, o.c.br)) + base);
   return o;
 }
 
 // gradient at a class that is not the label
 template <bool REF>
 __device__ __forceinline__ float coef_grad(const RowCoef& c, float s, float r) {
-  const float d = s - c.m, e = loss_expf(d);
-  float t = c.c0;
-  if (REF) t = e == 0.0f ? 0.0f : fmaf(c.c1, d - (r - c.mr), t);
-  return e * c.iz * t;
+  const float h = power_of(s, c.b), e = exp2_f32(h);
+  if (!REF) return e * c.c0;
+  return e == 0.0f ? 0.0f : e * fmaf(c.c1, h - power_of(r, c.br), c.c0);
 }
 
 }  // namespace wgbm

@@ -116,9 +116,8 @@ static BalanceWs balance_ws(int64_t n, int32_t K, bool cm, void* base) {
     at = (at + b + 255) & ~(size_t)255;
     return (void*)((unsigned char*)base + o);
   };
-  const size_t groups = (size_t)std::min<int64_t>(n, kLossWaves);
-  const size_t few = std::max<size_t>(512, (size_t(1) << 20) / K);
-  const size_t g = std::min(groups, few);
+  // (at least the workgroups of the first pass: of 64 threads or more, a row each)
+  const size_t g = (size_t)std::min(n, std::min(4 * kLossWaves, balance_few(K)));
   w.ticket = (uint32_t*)take(4);
   w.scale = (float*)take(4);
   w.share = (float*)take(4 * (size_t)K);

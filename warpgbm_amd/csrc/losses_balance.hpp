@@ -26,7 +26,7 @@ template <typename F>
 constexpr bool kAhead = 2 * F::kWords + 2 * F::N <= 104;
 
 // part [K][workgroups], count [K + 1][workgroups] (the last: rows that count);
-// norm: a row's maximum and 1 / sum of e^(s - max) (0: left out)
+// norm: a row's maximum and 1 / sum of 2^h (0: left out)
 template <typename F>
 __global__ __launch_bounds__(F::kMax) void balance_stats_kernel(
     ScoresView s, const uint8_t* __restrict__ mask, int32_t top_k, int64_t blocks,
@@ -47,9 +47,9 @@ __global__ __launch_bounds__(F::kMax) void balance_stats_kernel(
   typename F::Regs next;
   uint8_t next_want = 1;
   const auto fetch = [&](int64_t b) {
-    const int64_t row = F::row(b), i = row < s.n ? row : s.n - 1;
-    if (mask) next_want = mask[i];
-    f.load(next, s, i);
+    const int64_t row = F::row(b);
+    if (mask) next_want = mask[row < s.n ? row : s.n - 1];
+    f.load(next, s, b);
   };
   if (kAhead<F>) fetch(blockIdx.x);
   for (int64_t b = blockIdx.x; b < blocks; b += gridDim.x) {
@@ -64,51 +64,68 @@ __global__ __launch_bounds__(F::kMax) void balance_stats_kernel(
     if (!want) f.drop(v);
     float m = -__builtin_inff();
 #pragma unroll
-    for (int j = 0; j < F::N; ++j) m = fmaxf(m, F::value(v, j));
+    for (int j = 0; j < F::N; ++j) {
+      m = fmaxf(m, F::value(v, j));
+    }
     m = f.reduce(m, MaxF(), buf[0]);
     const float ms = safe_max(m);
-    float e[F::N], z[2] = {0.0f, 0.0f};
+    const Base base = base_of(ms);
+    // the exponentials of up to 16 classes stay in registers; more are worked
+    // out again for the sums
+    constexpr bool kKeep = F::N <= 16;
+    float e[kKeep ? F::N : 1], z[2] = {0.0f, 0.0f};
 #pragma unroll
     for (int j = 0; j < F::N; ++j) {
-      e[j] = loss_expf(F::value(v, j) - ms);
-      z[j % 2] += e[j];
+      const float x = exp2_f32(power_of(F::value(v, j), base));
+      z[j % 2] += x;
+      if constexpr (kKeep) e[j] = x;
     }
     z[0] = f.reduce(z[0] + z[1], AddF(), buf[1]);
     const bool live = !(z[0] == 0.0f);  // (NaN is live)
     const float iz = live ? 1.0f / z[0] : 0.0f;
 #pragma unroll
-    for (int j = 0; j < F::N; ++j) acc[j] = fmaf(e[j], iz, acc[j]);
+    for (int j = 0; j < F::N; ++j) {
+      float x;
+      if constexpr (kKeep)
+        x = e[j];
+      else
+        x = exp2_f32(power_of(F::value(v, j), base));
+      acc[j] = fmaf(x, iz, acc[j]);
+    }
     if (in && f.first_lane()) norm[i] = make_float2(ms, iz);
     // the best classes one after the other: the largest score after the last
-    // one taken, then the lowest class that has it (a thread's classes ascend).
+    // one taken, then the lowest class that has it.  A thread's classes ascend
+    // with its slots, so it looks for its lowest slot (slot numbers are
+    // constants of the instructions, class numbers would each take a register).
     // Class numbers are exact in float32; a NaN is not after anything.
     constexpr float kNone = 1e9f;
-    float v0 = __builtin_inff(), c0 = -1.0f;
+    float v0 = __builtin_inff();
+    int32_t c0 = -1;
     for (int32_t t = 0; t < top_k; ++t) {
-      float best = m, c = kNone;
+      float best = m;
+      int slot = F::N;
       if (t == 0) {
 #pragma unroll
-        for (int j = F::N - 1; j >= 0; --j)
-          c = F::value(v, j) == best ? (float)f.cls(j) : c;
+        for (int j = F::N - 1; j >= 0; --j) slot = F::value(v, j) == best ? j : slot;
       } else {
+        const int taken = f.last_slot(c0);  // of the scores equal to v0
         best = -__builtin_inff();
 #pragma unroll
         for (int j = 0; j < F::N; ++j) {
           const float x = F::value(v, j);
-          if (x < v0 || (x == v0 && (float)f.cls(j) > c0)) best = fmaxf(best, x);
+          if (x < v0 || (x == v0 && j > taken)) best = fmaxf(best, x);
         }
         best = f.reduce(best, MaxF(), buf[2]);
+        const int from = best < v0 ? -1 : taken;
 #pragma unroll
-        for (int j = F::N - 1; j >= 0; --j) {
-          const float k = (float)f.cls(j);
-          if (F::value(v, j) == best && (best < v0 || k > c0)) c = k;
-        }
+        for (int j = F::N - 1; j >= 0; --j)
+          slot = F::value(v, j) == best && j > from ? j : slot;
       }
-      c = f.reduce(c, MinF(), buf[3]);
+      const float c = f.reduce(slot < F::N ? (float)f.cls(slot) : kNone, MinF(), buf[3]);
       if (best > -__builtin_inff() && c < kNone && f.first_lane())
         atomicAdd(&s_count[(int32_t)c], 1);
       v0 = best;
-      c0 = c;
+      c0 = (int32_t)c;
     }
     if (live && f.first_lane()) atomicAdd(&s_count[K], 1);
   }
@@ -134,9 +151,9 @@ __global__ __launch_bounds__(F::kMax) void balance_grad_kernel(
   typename F::Regs next;
   float2 next_norm;
   const auto fetch = [&](int64_t b) {
-    const int64_t row = F::row(b), i = row < s.n ? row : s.n - 1;
-    next_norm = norm[i];
-    f.load(next, s, i);
+    const int64_t row = F::row(b);
+    next_norm = norm[row < s.n ? row : s.n - 1];
+    f.load(next, s, b);
   };
   if (kAhead<F>) fetch(blockIdx.x);
   for (int64_t b = blockIdx.x; b < blocks; b += gridDim.x, turn ^= 1) {
@@ -149,36 +166,41 @@ __global__ __launch_bounds__(F::kMax) void balance_grad_kernel(
     if (kAhead<F> && b + gridDim.x < blocks) fetch(b + gridDim.x);
     f.trim(v);
     const bool live = in && nm.y != 0.0f;  // (NaN is live)
+    const Base base = base_of(nm.x);
     float e[F::N], q = 0.0f;
 #pragma unroll
     for (int j = 0; j < F::N; ++j) {
-      e[j] = loss_expf(F::value(v, j) - nm.x);
+      e[j] = exp2_f32(power_of(F::value(v, j), base));
       q = fmaf(fk[j], e[j], q);
     }
     // (two turns' words: a wave may be one reduction ahead of the others)
     q = f.reduce(q, AddF(), buf[turn]) * nm.y;
     if (!in) continue;
     if (!live) {
-      if (!accumulate) f.store_zero(out, i);
+      if (!accumulate) f.store_zero(out, b);
       continue;
     }
     const float cz = c * nm.y;
-    f.store(out, i, accumulate, [&](int j) { return cz * e[j] * (fk[j] - q); });
+    f.store(out, b, accumulate, [&](int j) { return cz * e[j] * (fk[j] - q); });
   }
 }
 
 // the frames of up to 4096 classes: f(frame tag, blocks of rows, threads)
 template <typename T, typename Fn>
 static void balance_frame(const ScoresView& s, Fn fn) {
-  if (s.class_major() || s.K < Chunk<T>::VE) {
-    const int64_t rows = (s.n + 255) / 256, tiles = (s.n + 63) / 64;
-    if (s.K <= 4) return fn(FrameTag<ClassFrame<T, 4, false>>(), rows, 256);
-    if (s.K <= 8) return fn(FrameTag<ClassFrame<T, 8, false>>(), rows, 256);
-    if (s.K <= 12) return fn(FrameTag<ClassFrame<T, 12, false>>(), rows, 256);
-    if (s.K <= 16) return fn(FrameTag<ClassFrame<T, 16, false>>(), rows, 256);
+  const int64_t rows = (s.n + 255) / 256, tiles = (s.n + 63) / 64;
+  if (!s.class_major() && s.K < Chunk<T>::VE) {
+    if (s.K <= 4) return fn(FrameTag<ClassFrame<T, 4, false, false>>(), rows, 256);
+    return fn(FrameTag<ClassFrame<T, 8, false, false>>(), rows, 256);
+  }
+  if (s.class_major()) {
+    if (s.K <= 4) return fn(FrameTag<ClassFrame<T, 4, false, true>>(), rows, 256);
+    if (s.K <= 8) return fn(FrameTag<ClassFrame<T, 8, false, true>>(), rows, 256);
+    if (s.K <= 12) return fn(FrameTag<ClassFrame<T, 12, false, true>>(), rows, 256);
+    if (s.K <= 16) return fn(FrameTag<ClassFrame<T, 16, false, true>>(), rows, 256);
     if (s.K <= 256)
-      return fn(FrameTag<ClassFrame<T, 16, true>>(), tiles, 64 * (int)((s.K + 15) / 16));
-    return fn(FrameTag<ClassFrame<T, 32, true>>(), tiles, 64 * (int)((s.K + 31) / 32));
+      return fn(FrameTag<ClassFrame<T, 16, true, true>>(), tiles, 64 * (int)((s.K + 15) / 16));
+    return fn(FrameTag<ClassFrame<T, 32, true, true>>(), tiles, 64 * (int)((s.K + 31) / 32));
   }
   const int64_t chunks = (s.K + Chunk<T>::VE - 1) / Chunk<T>::VE;
   const auto go = [&](auto tag) {
@@ -192,12 +214,17 @@ static void balance_frame(const ScoresView& s, Fn fn) {
   return go(FrameTag<RowFrame<T, 256, 4>>());
 }
 
-// workgroups of the two passes: 16 waves a CU, and fewer partial sums where
-// there are many classes
-static inline int64_t balance_groups(int64_t blocks, int threads, int32_t K) {
-  const int64_t fill = kLossWaves * 64 / threads;
-  const int64_t few = std::max<int64_t>(512, (int64_t(1) << 20) / K);
-  return std::min(blocks, std::min(fill, few));
+// workgroups of the two passes: 16 waves a CU (with 64, the class-major 1M x 10
+// takes 45 us instead of 37 and a gate's 65536 x 64 32 instead of 26: more
+// partial sums), but 64 where the waves of a workgroup wait for one another
+// (1M x 100 class-major 359 us with 16, 331 with 64; 200000 x 400 721, 603); and
+// fewer partial sums where there are many classes
+template <typename F>
+static int64_t balance_fill(int threads) {
+  return (F::kSlices ? 4 : 1) * kLossWaves * 64 / threads;
+}
+static inline int64_t balance_few(int32_t K) {
+  return std::max<int64_t>(512, (int64_t(1) << 20) / K);
 }
 
 template <typename T>
@@ -205,7 +232,7 @@ int balance_stats(const ScoresView& s, const uint8_t* mask, int32_t top_k, const
                   int32_t* groups, hipStream_t st) {
   balance_frame<T>(s, [&](auto tag, int64_t blocks, int threads) {
     using F = typename decltype(tag)::type;
-    *groups = (int32_t)balance_groups(blocks, threads, s.K);
+    *groups = (int32_t)std::min(blocks, std::min(balance_fill<F>(threads), balance_few(s.K)));
     hipLaunchKernelGGL((balance_stats_kernel<F>), dim3((unsigned)*groups), dim3(threads),
                        (2 * (size_t)s.K + 1) * 4, st, s, mask, top_k, blocks, w.part, w.count,
                        w.norm, w.ticket);
@@ -219,7 +246,7 @@ int balance_grad(const ScoresView& s, const BalanceWs& w, const ScoresView& out,
                  hipStream_t st) {
   balance_frame<T>(s, [&](auto tag, int64_t blocks, int threads) {
     using F = typename decltype(tag)::type;
-    const int64_t groups = std::min<int64_t>(blocks, kLossWaves * 64 / threads);
+    const int64_t groups = std::min(blocks, balance_fill<F>(threads));
     hipLaunchKernelGGL((balance_grad_kernel<F>), dim3((unsigned)groups), dim3(threads), 0, st, s,
                        w.norm, w.share, w.scale, blocks, accumulate, out);
   });

@@ -12,17 +12,67 @@ namespace wgbm {
 template <typename T>
 struct Chunk {
   static constexpr int VE = 16 / (int)sizeof(T);
-  T v[VE];
+  // (kept as words: an array of 16-bit elements would take a register each)
+  uint32_t w[4];
+  __device__ __forceinline__ float get(int e) const;  // element e as float32
+  __device__ __forceinline__ T element(int e) const {
+    if constexpr (sizeof(T) == 4)
+      return __builtin_bit_cast(T, w[e]);
+    else
+      return __builtin_bit_cast(T, (uint16_t)(w[e / 2] >> (16 * (e % 2))));
+  }
+  __device__ __forceinline__ void set(const float* x);  // all elements, each rounded once
 };
+template <>
+__device__ __forceinline__ float Chunk<float>::get(int e) const {
+  return __builtin_bit_cast(float, w[e]);
+}
+template <>
+__device__ __forceinline__ float Chunk<__bf16>::get(int e) const {
+  return __builtin_bit_cast(float, e % 2 ? w[e / 2] & 0xffff0000u : w[e / 2] << 16);
+}
+template <>
+__device__ __forceinline__ float Chunk<_Float16>::get(int e) const {
+  return (float)element(e);
+}
+template <>
+__device__ __forceinline__ void Chunk<float>::set(const float* x) {
+#pragma unroll
+  for (int e = 0; e < 4; ++e) w[e] = __builtin_bit_cast(uint32_t, x[e]);
+}
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+template <>
+__device__ __forceinline__ void Chunk<__bf16>::set(const float* x) {
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    w[e] = __builtin_bit_cast(
+        uint32_t, __builtin_convertvector((f32x2){x[2 * e], x[2 * e + 1]}, bf16x2));
+}
+template <>
+__device__ __forceinline__ void Chunk<_Float16>::set(const float* x) {
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    w[e] = __builtin_bit_cast(
+        uint32_t, __builtin_convertvector((f32x2){x[2 * e], x[2 * e + 1]}, f16x2));
+}
 template <typename T>
 __device__ __forceinline__ Chunk<T> load_chunk(const T* p) {
   Chunk<T> c;
-  __builtin_memcpy(&c, p, 16);
+  __builtin_memcpy(c.w, p, 16);
   return c;
 }
 template <typename T>
 __device__ __forceinline__ void store_chunk(T* p, const Chunk<T>& c) {
-  __builtin_memcpy(p, &c, 16);
+  __builtin_memcpy(p, c.w, 16);
+}
+// The compiler keeps what one pass over the registers worked out (converted
+// scores, exponentials) for the next one, in registers of their own; after
+// hidden() the next pass starts from the scores again.
+template <typename T>
+__device__ __forceinline__ void hidden(Chunk<T>& c) {
+  asm volatile("" : "+v"(c.w[0]), "+v"(c.w[1]), "+v"(c.w[2]), "+v"(c.w[3]));
 }
 
 // label of row i, -1 where it has none
@@ -37,8 +87,17 @@ __device__ __forceinline__ float score_at(const ScoresView& s, int64_t i, int32_
   return to_f32(((const T*)s.data)[i * s.rs + k * s.ks]);
 }
 
+// results of class_log_probs for one row
+__device__ __forceinline__ void write_log_prob(const RowStats& a, float sa, int32_t label,
+                                               int64_t i, float* log_prob, float2* norm) {
+  const bool live = row_live(a);
+  const float m = safe_max(a.m);
+  log_prob[i] = live && label >= 0 ? (float)row_log_prob(a, sa) : 0.0f;
+  norm[i] = live ? make_float2(m, (float)sum_log(a.z + a.za, m))
+                 : make_float2(-__builtin_inff(), 0.0f);
+}
+
 // g (1[k = a] - softmax), the log-probability's gradient, from the row's norm
-// (c.iz is the logarithm of its sum)
 template <typename T>
 struct LogProbGrad {
   const int32_t* label;
@@ -51,17 +110,16 @@ struct LogProbGrad {
     const float g = grad[i];
     const float2 v = norm[i];
     if (a < 0 || g == 0.0f || v.x == -__builtin_inff()) return c;
-    c.m = v.x;
-    c.iz = v.y;
-    c.c0 = -g;
+    c.b = base_of(v.x);
+    c.c0 = -g * expf(-v.y);
     // the label's from its own logarithm: 1 - p without a difference
-    c.gl = c.c0 * expm1f((score_at<T>(s, i, a) - v.x) - v.y);
+    c.gl = -g * expm1f((score_at<T>(s, i, a) - v.x) - v.y);
     c.label = a;
     c.live = 1;
     return c;
   }
   __device__ __forceinline__ float at(const RowCoef& c, float s, float) const {
-    return c.c0 * loss_expf((s - c.m) - c.iz);
+    return coef_grad<false>(c, s, 0.0f);
   }
 };
 
@@ -127,6 +185,7 @@ struct RowFrame {
   static constexpr int kWords = 4 * NC;  // registers of a thread's scores
   static constexpr int kThreads = G <= 256 ? 256 : G, kMax = kThreads;
   static constexpr bool kBarrier = G > 64, kSlices = false;
+  static constexpr int kShared = 1;  // rows that the waves of a workgroup share
   static constexpr int kRows = kThreads / G;  // rows of a workgroup
   static constexpr int kBuf = G > 64 ? G / 64 : 1;
   int32_t t, K;  // this thread's place in its group
@@ -146,33 +205,70 @@ struct RowFrame {
   struct Regs {
     Chunk<T> c[NC];
   };
-  __device__ __forceinline__ void load(Regs& r, const ScoresView& s, int64_t i) const {
-    const T* p = (const T*)s.data + i * s.rs;
+  // the row's first element (rows of a whole wave: an address in scalar
+  // registers, the classes a 32-bit offset)
+  __device__ __forceinline__ T* at(const ScoresView& s, int64_t b) const {
+    int64_t i;
+    if (G >= 64)
+      i = b * kRows + (kRows > 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x / G) : 0);
+    else
+      i = row(b);
+    return (T*)s.data + (i < s.n ? i : s.n - 1) * s.rs;
+  }
+  __device__ __forceinline__ void load(Regs& r, const ScoresView& s, int64_t b) const {
+    const T* p = at(s, b);
 #pragma unroll
-    for (int c = 0; c < NC; ++c) r.c[c] = load_chunk<T>(p + first(c));
+    for (int c = 0; c < NC; ++c) r.c[c] = load_chunk<T>(p + (uint32_t)first(c));
   }
   __device__ __forceinline__ void trim(Regs& r) const {
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
       const int32_t sk = skip(c);
       if (__any(sk > 0)) {
+        uint32_t(&w)[4] = r.c[c].w;
 #pragma unroll
-        for (int e = 0; e < VE; ++e)
-          r.c[c].v[e] = e < sk ? (T)(-__builtin_inff()) : r.c[c].v[e];
+        for (int e = 0; e < 4; ++e) {
+          if (VE == 4) {
+            w[e] = e < sk ? kNegInf : w[e];
+          } else {
+            const uint32_t one = (w[e] & 0xffff0000u) | (kNegInf & 0xffffu);
+            w[e] = sk >= 2 * e + 2 ? kNegInf : sk == 2 * e + 1 ? one : w[e];
+          }
+        }
       }
     }
   }
+  // -inf, or two of them
+  static constexpr uint32_t kNegInf = sizeof(T) == 4                  ? 0xff800000u
+                                      : __is_same(T, _Float16) ? 0xfc00fc00u
+                                                               : 0xff80ff80u;
+  // whether each pass starts from the scores again (8191 x 16001 bfloat16, 64
+  // classes a thread: 121 us without, 115 with, five waves instead of three)
+  static constexpr bool kHide = N >= 64;
+  __device__ __forceinline__ void hide(Regs& r) const {
+#pragma unroll
+    for (int c = 0; c < NC; ++c) hidden(r.c[c]);
+  }
+  // whether class k (-1: none) is one of this thread's
+  __device__ __forceinline__ bool has(int32_t k) const { return k >= 0 && (k / VE) % G == t; }
   // a row that is left out has no class
   __device__ __forceinline__ void drop(Regs& r) const {
 #pragma unroll
     for (int c = 0; c < NC; ++c)
 #pragma unroll
-      for (int e = 0; e < VE; ++e) r.c[c].v[e] = (T)(-__builtin_inff());
+      for (int e = 0; e < 4; ++e) r.c[c].w[e] = kNegInf;
   }
   static __device__ __forceinline__ float value(const Regs& r, int j) {
-    return to_f32(r.c[j / VE].v[j % VE]);
+    return r.c[j / VE].get(j % VE);
   }
   __device__ __forceinline__ int32_t cls(int j) const { return first(j / VE) + j % VE; }
+  // this thread's last slot with a class up to k (-1: none)
+  __device__ __forceinline__ int last_slot(int32_t k) const {
+    const int32_t q = k / VE;
+    if (q < t) return -1;
+    const int c = (q - t) / G;
+    return c * VE + (c * G + t == q ? k - first(c) : VE - 1);
+  }
 
   // reductions over the row; buf as for waves_reduce (kBuf words each)
   template <typename Op>
@@ -200,8 +296,6 @@ struct RowFrame {
       __syncthreads();
     }
   }
-  // (one row a group: its lanes agree)
-  __device__ __forceinline__ bool any(bool x) const { return x; }
   // sum of e^(s - m) over the row in float64, from memory; buf: kBuf words
   __device__ __forceinline__ double wide_sum(const ScoresView& s, int64_t i, float m,
                                              double* buf) const {
@@ -219,34 +313,52 @@ struct RowFrame {
 
   // out[cls(j)] (+)= f(j) for this thread's classes
   template <typename F>
-  __device__ __forceinline__ void store(const ScoresView& o, int64_t i, bool accumulate, F f) const {
-    T* p = (T*)o.data + i * o.rs;
-#pragma unroll
-    for (int c = 0; c < NC; ++c) {
-      const int32_t k = want(c), sk = skip(c), at = first(c);
-      if (sk >= VE) continue;
+  __device__ __forceinline__ void store(const ScoresView& o, int64_t b, bool accumulate, F f) const {
+    T* p = at(o, b);
+    const auto values = [&](int c, T* q) {
       float x[VE];
 #pragma unroll
       for (int e = 0; e < VE; ++e) x[e] = f(c * VE + e);
-      if (sk == 0) {
-        Chunk<T> v;
-        if (accumulate) {
-          const Chunk<T> old = load_chunk<T>(p + k);
+      if (accumulate) {
+        const Chunk<T> old = load_chunk<T>(q);
 #pragma unroll
-          for (int e = 0; e < VE; ++e) x[e] += to_f32(old.v[e]);
-        }
+        for (int e = 0; e < VE; ++e) x[e] += old.get(e);
+      }
+      Chunk<T> v;
+      v.set(x);
+      return v;
+    };
 #pragma unroll
-        for (int e = 0; e < VE; ++e) v.v[e] = from_f32<T>(x[e]);
-        store_chunk<T>(p + k, v);
-      } else {
+    for (int c = 0; c < NC; ++c) {
+      T* q = p + (uint32_t)first(c);
+      if (skip(c) == 0) store_chunk<T>(q, values(c, q));
+    }
+    // a part of a chunk at the row's end, one thread's
+    const int32_t part = K % VE;
+    if (part && __any((K / VE) % G == t)) {
 #pragma unroll
-        for (int e = 0; e < VE; ++e)
-          if (e >= sk) p[at + e] = from_f32<T>(accumulate ? x[e] + to_f32(p[at + e]) : x[e]);
+      for (int c = 0; c < NC; ++c) {
+        if (c * G + t != K / VE) continue;
+        T* q = p + (uint32_t)first(c);
+        const Chunk<T> v = values(c, q);
+#pragma unroll
+        for (int e = 1; e < VE; ++e)
+          if (e >= VE - part) q[e] = v.element(e);
       }
     }
   }
-  __device__ __forceinline__ void store_zero(const ScoresView& o, int64_t i) const {
-    store(o, i, false, [](int) { return 0.0f; });
+  // the same, and gl for class `label`: its thread writes it after its chunk
+  template <typename F>
+  __device__ __forceinline__ void store_row(const ScoresView& o, int64_t b, bool accumulate,
+                                            int32_t label, float gl, F f) const {
+    const bool mine = has(label);
+    T* q = at(o, b) + (mine ? label : 0);
+    if (mine && accumulate) gl += to_f32(*q);
+    store(o, b, accumulate, f);
+    if (mine) *q = from_f32<T>(gl);
+  }
+  __device__ __forceinline__ void store_zero(const ScoresView& o, int64_t b) const {
+    store(o, b, false, [](int) { return 0.0f; });
   }
 };
 
@@ -255,15 +367,17 @@ struct RowFrame {
 // next to each other (one load instruction reads 64 rows of a class).  The
 // slices w = 0 .. S-1 are the waves of a workgroup; slice w holds the classes
 // w, w + S, ... (N of them).  With S = 1 a workgroup's waves hold rows of
-// their own; rows may then also be short and next to each other (any strides).
-// Classes past the last are read as the last one and set to -inf.
+// their own; short rows may then also have their classes next to each other
+// (ADJ false: any strides).  Classes past the last are read as the last one and
+// set to -inf.
 // ---------------------------------------------------------------------------
-template <typename T_, int N_, bool SLICES>
+template <typename T_, int N_, bool SLICES, bool ADJ>
 struct ClassFrame {
   using T = T_;
   static constexpr int N = N_, kWords = N_;
   static constexpr int kMax = SLICES ? 1024 : 256;
   static constexpr bool kBarrier = SLICES, kSlices = SLICES;
+  static constexpr int kShared = SLICES ? 64 : 1;
   static constexpr int kBuf = SLICES ? 16 * 64 : 1;
   int32_t w, S, K;
 
@@ -276,22 +390,46 @@ struct ClassFrame {
   }
   __device__ __forceinline__ bool first_lane() const { return w == 0; }
   __device__ __forceinline__ int32_t cls(int j) const { return w + j * S; }
+  // this thread's last slot with a class up to k (-1: none)
+  __device__ __forceinline__ int last_slot(int32_t k) const { return k < w ? -1 : (k - w) / S; }
 
   struct Regs {
     T c[N];
   };
-  __device__ __forceinline__ void load(Regs& r, const ScoresView& s, int64_t i) const {
-    const T* p = (const T*)s.data + i * s.rs;
+  // the first row of this wave's 64, and this lane's offset from it (the last
+  // row for lanes past the end): class addresses stay in scalar registers
+  __device__ __forceinline__ T* at(const ScoresView& s, int64_t b) const {
+    return (T*)s.data + first_row(s, b) * s.rs;
+  }
+  // (a wave wholly past the end: the last row of the matrix)
+  static __device__ __forceinline__ int64_t first_row(const ScoresView& s, int64_t b) {
+    if (SLICES) return b * 64;
+    const int64_t i = b * 256 + 64 * __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+    return i < s.n ? i : s.n - 1;
+  }
+  static __device__ __forceinline__ auto offset(const ScoresView& s, int64_t b) {
+    const int64_t left = s.n - 1 - first_row(s, b);
+    const uint32_t lane = threadIdx.x & 63, l = lane < left ? lane : (uint32_t)left;
+    if constexpr (ADJ)
+      return l;
+    else
+      return (int64_t)l * s.rs;
+  }
+  __device__ __forceinline__ void load(Regs& r, const ScoresView& s, int64_t b) const {
+    const T* p = at(s, b);
+    const auto o = offset(s, b);
 #pragma unroll
     for (int j = 0; j < N; ++j) {
       const int32_t k = cls(j) < K ? cls(j) : K - 1;
-      r.c[j] = p[k * s.ks];
+      r.c[j] = (p + k * s.ks)[o];
     }
   }
   __device__ __forceinline__ void trim(Regs& r) const {
 #pragma unroll
     for (int j = 0; j < N; ++j) r.c[j] = cls(j) < K ? r.c[j] : (T)(-__builtin_inff());
   }
+  static constexpr bool kHide = false;
+  __device__ __forceinline__ void hide(Regs&) const {}
   __device__ __forceinline__ void drop(Regs& r) const {
 #pragma unroll
     for (int j = 0; j < N; ++j) r.c[j] = (T)(-__builtin_inff());
@@ -311,7 +449,10 @@ struct ClassFrame {
   // sum[k] = the workgroup's sum of acc over its rows, for every class
   __device__ __forceinline__ void sum_rows(float (&acc)[N], float* sum) const {
 #pragma unroll
-    for (int j = 0; j < N; ++j) acc[j] = lanes_reduce<64>(acc[j], AddF());
+    for (int j = 0; j < N; ++j) {
+      acc[j] = lanes_reduce<64>(acc[j], AddF());
+      __builtin_amdgcn_sched_barrier(0);  // (N at once would take the registers of two waves)
+    }
     const int kTurns = SLICES ? 1 : 4;
     for (int u = 0; u < kTurns; ++u) {
       if ((SLICES || (int)(threadIdx.x >> 6) == u) && (threadIdx.x & 63) == 0) {
@@ -322,8 +463,6 @@ struct ClassFrame {
       __syncthreads();
     }
   }
-  // (the lanes of a workgroup's waves share rows: all go, or none)
-  __device__ __forceinline__ bool any(bool x) const { return SLICES ? __syncthreads_or(x) : x; }
   __device__ __forceinline__ double wide_sum(const ScoresView& s, int64_t i, float m,
                                              double* buf) const {
     const T* p = (const T*)s.data + i * s.rs;
@@ -338,19 +477,25 @@ struct ClassFrame {
     return z;
   }
   template <typename F>
-  __device__ __forceinline__ void store(const ScoresView& o, int64_t i, bool accumulate, F f) const {
-    T* p = (T*)o.data + i * o.rs;
+  __device__ __forceinline__ void store(const ScoresView& o, int64_t b, bool accumulate, F f) const {
+    store_row(o, b, accumulate, -1, 0.0f, f);
+  }
+  template <typename F>
+  __device__ __forceinline__ void store_row(const ScoresView& o, int64_t b, bool accumulate,
+                                            int32_t label, float gl, F f) const {
+    T* p = at(o, b);
+    const auto l = offset(o, b);
 #pragma unroll
     for (int j = 0; j < N; ++j) {
       if (cls(j) < K) {
-        T* q = p + cls(j) * o.ks;
-        const float x = f(j);
+        T* q = p + cls(j) * o.ks + l;
+        const float y = f(j), x = cls(j) == label ? gl : y;
         *q = from_f32<T>(accumulate ? x + to_f32(*q) : x);
       }
     }
   }
-  __device__ __forceinline__ void store_zero(const ScoresView& o, int64_t i) const {
-    store(o, i, false, [](int) { return 0.0f; });
+  __device__ __forceinline__ void store_zero(const ScoresView& o, int64_t b) const {
+    store(o, b, false, [](int) { return 0.0f; });
   }
 };
 

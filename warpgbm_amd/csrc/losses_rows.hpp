@@ -9,39 +9,43 @@ namespace wgbm {
 // a row's statistics from its registers (the label's score sa apart); buf:
 // five reductions' words
 template <typename F, bool REF>
-__device__ __forceinline__ RowStats frame_stats(const F& f, const typename F::Regs& s,
-                                                const typename F::Regs& r, int32_t label, float sa,
+__device__ __forceinline__ RowStats frame_stats(const F& f, typename F::Regs& s,
+                                                typename F::Regs& r, int32_t label, float sa,
                                                 float (*buf)[F::kBuf]) {
   RowStats a = empty_stats();
 #pragma unroll
   for (int j = 0; j < F::N; ++j) a.m = fmaxf(a.m, F::value(s, j));
   a.m = f.reduce(a.m, MaxF(), buf[0]);
-  const float ms = safe_max(a.m);
-  float mrs = 0.0f;
+  const Base b = base_of(safe_max(a.m));
+  Base br = b;
   if (REF) {
 #pragma unroll
     for (int j = 0; j < F::N; ++j) a.mr = fmaxf(a.mr, F::value(r, j));
     a.mr = f.reduce(a.mr, MaxF(), buf[1]);
-    mrs = safe_max(a.mr);
+    br = base_of(safe_max(a.mr));
   }
+  if (F::kHide) f.hide(s);
+  if (REF && F::kHide) f.hide(r);
   // four sums a thread: shorter chains of additions, and fewer roundings
   float z[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
   for (int j = 0; j < F::N; ++j) {
-    const float d = F::value(s, j) - ms, e = loss_expf(d);
+    const float h = power_of(F::value(s, j), b), e = exp2_f32(h);
     z[j % 4] += f.cls(j) == label ? 0.0f : e;
     if (REF) {
-      const float dr = F::value(r, j) - mrs;
-      a.zr += loss_expf(dr);
-      a.u += e == 0.0f ? 0.0f : e * (d - dr);
+      const float hr = power_of(F::value(r, j), br);
+      a.zr += exp2_f32(hr);
+      a.u += e == 0.0f ? 0.0f : e * (h - hr);
     }
   }
+  if (F::kHide) f.hide(s);
+  if (REF && F::kHide) f.hide(r);
   a.z = f.reduce((z[0] + z[1]) + (z[2] + z[3]), AddF(), buf[2]);
   if (REF) {
     a.zr = f.reduce(a.zr, AddF(), buf[3]);
     a.u = f.reduce(a.u, AddF(), buf[4]);
   }
-  a.za = label >= 0 ? loss_expf(sa - ms) : 0.0f;
+  if (label >= 0) a.za = exp2_f32(power_of(sa, b));
   return a;
 }
 
@@ -56,15 +60,13 @@ __global__ __launch_bounds__(F::kMax) void log_probs_frame_kernel(
   if (!F::kBarrier && !in) return;
   const int64_t i = in ? row : s.n - 1;
   typename F::Regs v;
-  f.load(v, s, i);
+  f.load(v, s, blockIdx.x);
   const int32_t lab = row_label(label, i, s.K);
   const float sa = lab >= 0 ? score_at<typename F::T>(s, i, lab) : 0.0f;
   f.trim(v);
   const RowStats a = frame_stats<F, false>(f, v, v, lab, sa, buf);
   if (!in || !f.first_lane()) return;
-  const LogProb lp = row_log_prob(a, sa);
-  log_prob[i] = lp.live && lab >= 0 ? (float)lp.logp : 0.0f;
-  norm[i] = lp.live ? make_float2(lp.m, (float)lp.l) : make_float2(-__builtin_inff(), 0.0f);
+  write_log_prob(a, sa, lab, i, log_prob, norm);
 }
 
 // (no reduction: the norm is given)
@@ -75,12 +77,11 @@ __global__ __launch_bounds__(F::kMax) void log_probs_grad_frame_kernel(
   const int64_t i = F::row(blockIdx.x);
   if (i >= s.n) return;
   typename F::Regs v;
-  f.load(v, s, i);
+  f.load(v, s, blockIdx.x);
   const RowCoef c = g.row(s, i);
-  f.store(out, i, false, [&](int j) {
-    const float x = g.at(c, F::value(v, j), 0.0f);
-    return !c.live ? 0.0f : f.cls(j) == c.label ? c.gl : x;
-  });
+  if (!c.live) return f.store_zero(out, blockIdx.x);
+  f.store_row(out, blockIdx.x, false, c.label, c.gl,
+              [&](int j) { return g.at(c, F::value(v, j), 0.0f); });
 }
 
 template <typename F, bool REF>
@@ -90,6 +91,8 @@ __global__ __launch_bounds__(F::kMax) void policy_frame_kernel(ScoresView s, Sco
   using T = typename F::T;
   __shared__ float buf[5][F::kBuf];
   __shared__ double wide[F::kBuf];
+  __shared__ RowCoef share[F::kShared];
+  __shared__ int share_near;
   const F f(s);
   const int64_t row = F::row(blockIdx.x);
   const bool in = row < s.n;
@@ -104,12 +107,12 @@ __global__ __launch_bounds__(F::kMax) void policy_frame_kernel(ScoresView s, Sco
       g.loss[i] = g.log_prob[i] = 0.0f;
       if (g.kl) g.kl[i] = 0.0f;
     }
-    if (out.data && !accumulate) f.store_zero(out, i);
+    if (out.data && !accumulate) f.store_zero(out, blockIdx.x);
     return;
   }
   typename F::Regs v, r;
-  f.load(v, s, i);
-  if (REF) f.load(r, ref, i);
+  f.load(v, s, blockIdx.x);
+  if (REF) f.load(r, ref, blockIdx.x);
   const int32_t a = lab >= 0 ? lab : 0;
   const float sa = score_at<T>(s, i, a);
   const float ra = REF ? score_at<T>(ref, i, a) : 0.0f;
@@ -117,30 +120,44 @@ __global__ __launch_bounds__(F::kMax) void policy_frame_kernel(ScoresView s, Sco
   f.trim(v);
   if (REF) f.trim(r);
   const RowStats st = frame_stats<F, REF>(f, v, r, lab, sa, buf);
-  PolicyRow o = policy_row<REF>(st, sa, ra, A, old, w, g, i, lab, nullptr);
-  if (f.any(o.near && live)) {
+  // what follows from the row as a whole costs as much as some ten classes:
+  // where waves share rows, the first one works it out for all
+  const bool owner = !F::kBarrier || threadIdx.x < 64;
+  const int slot = F::kSlices ? threadIdx.x & 63 : 0;
+  PolicyRow o{};
+  if (owner) o = policy_row<REF>(st, sa, ra, A, old, w, g, i, lab, nullptr);
+  bool near = o.near && live;
+  if (F::kBarrier) {
+    const bool any = __any(near);
+    if (threadIdx.x == 0) share_near = any;
+    __syncthreads();
+    near = share_near;
+  }
+  if (near) {
     // next to a border: the row's sum again, in float64
-    const double z = f.wide_sum(s, i, o.c.m, wide);
-    const double logp = ((double)sa - (double)o.c.m) - log(z);
+    const float m = safe_max(st.m);
+    const double z = f.wide_sum(s, i, m, wide);
+    const double logp = ((double)sa - (double)m) - log(z);
     if (o.near) o = policy_row<REF>(st, sa, ra, A, old, w, g, i, lab, &logp);
   }
-  if (F::kSlices && !live) {
-    o.loss = o.logp = o.kl = 0.0f;
-    o.c = RowCoef{};
-  }
-  if (in && f.first_lane()) {
+  if (F::kSlices && !live) o = PolicyRow{};
+  if (in && owner && f.first_lane()) {
     g.loss[i] = o.loss;
     g.log_prob[i] = o.logp;
     if (g.kl) g.kl[i] = o.kl;
   }
+  if (F::kBarrier) {
+    if (owner && (F::kSlices || threadIdx.x == 0)) share[slot] = o.c;
+    __syncthreads();
+    o.c = share[slot];
+  }
   if (!in || !out.data) return;
-  if (!o.c.live || !live) {
-    if (!accumulate) f.store_zero(out, i);
+  if (!o.c.live) {
+    if (!accumulate) f.store_zero(out, blockIdx.x);
     return;
   }
-  f.store(out, i, accumulate, [&](int j) {
-    const float x = coef_grad<REF>(o.c, F::value(v, j), REF ? F::value(r, j) : 0.0f);
-    return f.cls(j) == lab ? o.c.gl : x;
+  f.store_row(out, blockIdx.x, accumulate, lab, o.c.gl, [&](int j) {
+    return coef_grad<REF>(o.c, F::value(v, j), REF ? F::value(r, j) : 0.0f);
   });
 }
 
@@ -149,7 +166,9 @@ __global__ __launch_bounds__(F::kMax) void policy_frame_kernel(ScoresView s, Sco
 // one that holds the rows, false where none does
 // ---------------------------------------------------------------------------
 // most 16-byte chunks of one matrix in a thread's registers: 16 (64 registers
-// of 128 that a workgroup of 1024 threads has), 8 with a second matrix
+// of 128 that a workgroup of 1024 threads has), 4 with a second matrix (with 8
+// the registers no longer hold the passes: 2000 x 50000 bfloat16 677 us, the
+// ranged path 415)
 template <typename T, bool REF, typename Fn>
 static bool pick_row_frame(const ScoresView& s, Fn fn) {
   constexpr int VE = Chunk<T>::VE;
@@ -167,24 +186,28 @@ static bool pick_row_frame(const ScoresView& s, Fn fn) {
   if (chunks <= 1024) return go(FrameTag<RowFrame<T, 256, 4>>());
   if (chunks <= 2048) return go(FrameTag<RowFrame<T, 256, 8>>());
   if (chunks <= 4096) return go(FrameTag<RowFrame<T, 1024, 4>>());
-  if (chunks <= 8192) return go(FrameTag<RowFrame<T, 1024, 8>>());
-  if (!REF && chunks <= 16384) return go(FrameTag<RowFrame<T, 1024, 16>>());
+  if constexpr (!REF) {
+    if (chunks <= 8192) return go(FrameTag<RowFrame<T, 1024, 8>>());
+    if (chunks <= 16384) return go(FrameTag<RowFrame<T, 1024, 16>>());
+  }
   return false;
 }
 
 template <typename T, bool REF, typename Fn>
 static bool pick_class_frame(const ScoresView& s, Fn fn) {
-  const int64_t blocks = (s.n + 255) / 256;
-  if (s.K <= 4) return fn(FrameTag<ClassFrame<T, 4, false>>(), blocks, 256), true;
-  if (s.K <= 8) return fn(FrameTag<ClassFrame<T, 8, false>>(), blocks, 256), true;
-  if (s.K <= 12) return fn(FrameTag<ClassFrame<T, 12, false>>(), blocks, 256), true;
-  if (s.K <= 16) return fn(FrameTag<ClassFrame<T, 16, false>>(), blocks, 256), true;
-  // row-major rows come here only when they are short
-  const int64_t tiles = (s.n + 63) / 64;
+  const int64_t blocks = (s.n + 255) / 256, tiles = (s.n + 63) / 64;
+  if (!s.class_major()) {  // short rows
+    if (s.K <= 4) return fn(FrameTag<ClassFrame<T, 4, false, false>>(), blocks, 256), true;
+    return fn(FrameTag<ClassFrame<T, 8, false, false>>(), blocks, 256), true;
+  }
+  if (s.K <= 4) return fn(FrameTag<ClassFrame<T, 4, false, true>>(), blocks, 256), true;
+  if (s.K <= 8) return fn(FrameTag<ClassFrame<T, 8, false, true>>(), blocks, 256), true;
+  if (s.K <= 12) return fn(FrameTag<ClassFrame<T, 12, false, true>>(), blocks, 256), true;
+  if (s.K <= 16) return fn(FrameTag<ClassFrame<T, 16, false, true>>(), blocks, 256), true;
   if (s.K <= 256)
-    return fn(FrameTag<ClassFrame<T, 16, true>>(), tiles, 64 * (int)((s.K + 15) / 16)), true;
+    return fn(FrameTag<ClassFrame<T, 16, true, true>>(), tiles, 64 * (int)((s.K + 15) / 16)), true;
   if (s.K <= 512)
-    return fn(FrameTag<ClassFrame<T, 32, true>>(), tiles, 64 * (int)((s.K + 31) / 32)), true;
+    return fn(FrameTag<ClassFrame<T, 32, true, true>>(), tiles, 64 * (int)((s.K + 31) / 32)), true;
   return false;
 }
 
