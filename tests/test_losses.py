@@ -853,7 +853,8 @@ def test_c_entries_refuse_before_any_launch():
     refused(lp(scores(row_stride=16, class_stride=2)), "strides")
     refused(lp(scores(data=18)), "aligned")
     refused(lp(scores(data=None)), "null data")
-    refused(lp(scores(), ws=8), "workspace too small")
+    # (rows of 100,000 classes go through the workspace)
+    refused(lp(scores(n_classes=100_000, row_stride=100_000), ws=8), "workspace too small")
     empty = scores(n_rows=0)
     for fn in (lib.wgbm_class_log_probs_workspace, lib.wgbm_policy_loss_workspace,
                lib.wgbm_balance_loss_workspace):

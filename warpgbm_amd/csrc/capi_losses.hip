@@ -48,6 +48,12 @@ static int same_kind(const ScoresView& a, const ScoresView& b, const char* what)
   return 0;
 }
 
+static int balance_classes(const ScoresView& s) {
+  WGBM_REQUIRE(s.K <= kMaxBalanceClasses, "balance_loss: at most %d classes, got %d",
+               kMaxBalanceClasses, s.K);
+  return 0;
+}
+
 #define TRY(expr)         \
   do {                    \
     const int _r = (expr); \
@@ -59,7 +65,7 @@ extern "C" {
 int64_t wgbm_class_log_probs_workspace(const wgbm_scores* scores) {
   ScoresView s;
   if (view_of(scores, "scores", &s)) return -1;
-  return (int64_t)log_probs_workspace(s.n, s.K, s.class_major());
+  return (int64_t)log_probs_workspace(s);
 }
 
 int wgbm_class_log_probs(const wgbm_scores* scores, const int32_t* labels, float* log_prob,
@@ -67,10 +73,11 @@ int wgbm_class_log_probs(const wgbm_scores* scores, const int32_t* labels, float
   ScoresView s;
   TRY(view_of(scores, "scores", &s));
   if (s.n == 0) return 0;
-  WGBM_REQUIRE(labels && log_prob && norm && workspace, "class_log_probs: null pointer");
-  WGBM_REQUIRE(workspace_bytes >= (int64_t)log_probs_workspace(s.n, s.K, s.class_major()),
+  WGBM_REQUIRE(labels && log_prob && norm, "class_log_probs: null pointer");
+  const int64_t need = (int64_t)log_probs_workspace(s);
+  WGBM_REQUIRE(need == 0 || (workspace && workspace_bytes >= need),
                "class_log_probs: workspace too small");
-  return class_log_probs(s, labels, nullptr, log_prob, norm, workspace, S(stream));
+  return class_log_probs(s, labels, log_prob, norm, workspace, S(stream));
 }
 
 int wgbm_class_log_probs_grad(const wgbm_scores* scores, const int32_t* labels, const float* norm,
@@ -87,7 +94,7 @@ int wgbm_class_log_probs_grad(const wgbm_scores* scores, const int32_t* labels, 
 int64_t wgbm_policy_loss_workspace(const wgbm_scores* scores) {
   ScoresView s;
   if (view_of(scores, "scores", &s)) return -1;
-  return (int64_t)policy_workspace(s.n, s.K, s.class_major());
+  return (int64_t)policy_workspace(s);
 }
 
 int wgbm_policy_loss(const wgbm_scores* scores, const wgbm_policy_args* a, float* loss,
@@ -112,9 +119,10 @@ int wgbm_policy_loss(const wgbm_scores* scores, const wgbm_policy_args* a, float
   WGBM_REQUIRE(std::isfinite(a->kl_coef) && a->kl_coef >= 0.0f,
                "policy_loss: kl_coef must be non-negative and finite");
   if (s.n == 0) return 0;
-  WGBM_REQUIRE(a->actions && a->old_log_prob && a->advantage && loss && log_prob && workspace,
+  WGBM_REQUIRE(a->actions && a->old_log_prob && a->advantage && loss && log_prob,
                "policy_loss: null pointer");
-  WGBM_REQUIRE(workspace_bytes >= (int64_t)policy_workspace(s.n, s.K, s.class_major()),
+  const int64_t need = (int64_t)policy_workspace(s);
+  WGBM_REQUIRE(need == 0 || (workspace && workspace_bytes >= need),
                "policy_loss: workspace too small");
   PolicyRows p{};
   p.action = a->actions;
@@ -135,7 +143,7 @@ int wgbm_policy_loss(const wgbm_scores* scores, const wgbm_policy_args* a, float
 
 int64_t wgbm_balance_loss_workspace(const wgbm_scores* scores) {
   ScoresView s;
-  if (view_of(scores, "scores", &s)) return -1;
+  if (view_of(scores, "scores", &s) || balance_classes(s)) return -1;
   return (int64_t)balance_workspace(s);
 }
 
@@ -148,8 +156,7 @@ int wgbm_balance_loss(const wgbm_scores* scores, const uint8_t* mask, int32_t to
     TRY(view_of(grad, "grad", &g));
     TRY(same_kind(s, g, "grad"));
   }
-  WGBM_REQUIRE(s.K <= kMaxBalanceClasses, "balance_loss: at most %d classes, got %d",
-               kMaxBalanceClasses, s.K);
+  TRY(balance_classes(s));
   WGBM_REQUIRE(top_k >= 1 && top_k <= kMaxTopK && top_k <= s.K,
                "balance_loss: top_k must be in [1, min(%d, n_classes)], got %d", kMaxTopK, top_k);
   WGBM_REQUIRE(std::isfinite(coef), "balance_loss: coef must be finite");

@@ -1,9 +1,11 @@
 // Losses of class scores: log-probabilities, the clipped policy loss and the
 // balance loss, each with its gradient with respect to the scores.
 //
-// Any size, both layouts: a row's classes are cut into `splits` ranges whose
-// statistics (running maximum and sums) are kept in the workspace, joined per
-// row, and the gradient is written by an elementwise pass over the scores.
+// Rows that fit the registers of the threads that share them take one launch
+// (losses_rows.hpp).  Here: longer rows, both layouts.  A row's classes are cut
+// into `splits` ranges whose statistics (running maximum and sums) are kept in
+// the workspace, joined per row, and the gradient is written by an elementwise
+// pass that reads the scores again.
 #include <algorithm>
 
 #include "losses_frames.hpp"
@@ -57,23 +59,20 @@ __device__ __forceinline__ RowStats shfl_xor_stats(const RowStats& a, int o) {
 template <typename T, bool CM, bool REF>
 __global__ __launch_bounds__(256) void row_stats_kernel(ScoresView s, ScoresView ref,
                                                         const int32_t* __restrict__ label,
-                                                        const uint8_t* __restrict__ mask,
                                                         int32_t span, RowStats* __restrict__ part) {
   const int64_t i = CM ? (int64_t)blockIdx.x * 256 + threadIdx.x
                        : (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
   if (i >= s.n) return;
   const int32_t k0 = blockIdx.y * span, k1 = s.K - k0 > span ? k0 + span : s.K;
-  RowStats a = empty_stats();
-  if (!mask || mask[i]) {
-    const T* p = (const T*)s.data + i * s.rs;
-    const T* q = REF ? (const T*)ref.data + i * ref.rs : nullptr;
-    const int32_t lab = row_label(label, i, s.K);
-    if (CM) {
-      a = scan_classes<T, REF>(p, q, s.ks, ref.ks, k0, k1, 1, lab);
-    } else {
-      a = scan_classes<T, REF>(p, q, s.ks, ref.ks, k0 + (int)(threadIdx.x & 63), k1, 64, lab);
-      for (int o = 32; o; o >>= 1) a = join_stats<REF>(a, shfl_xor_stats(a, o));
-    }
+  const T* p = (const T*)s.data + i * s.rs;
+  const T* q = REF ? (const T*)ref.data + i * ref.rs : nullptr;
+  const int32_t lab = row_label(label, i, s.K);
+  RowStats a;
+  if (CM) {
+    a = scan_classes<T, REF>(p, q, s.ks, ref.ks, k0, k1, 1, lab);
+  } else {
+    a = scan_classes<T, REF>(p, q, s.ks, ref.ks, k0 + (int)(threadIdx.x & 63), k1, 64, lab);
+    for (int o = 32; o; o >>= 1) a = join_stats<REF>(a, shfl_xor_stats(a, o));
   }
   if (CM || (threadIdx.x & 63) == 0) part[(int64_t)blockIdx.y * s.n + i] = a;
 }
@@ -252,7 +251,7 @@ __global__ __launch_bounds__(256) void score_grad_kernel(ScoresView s, ScoresVie
 // ---------------------------------------------------------------------------
 // a row's classes in ranges: one range where the rows alone fill the GPU, else
 // ranges of at least 256 classes (row-major: 1024, a wave's 16 loads each)
-int32_t loss_splits(int64_t n, int32_t K, bool cm) {
+static int32_t loss_splits(int64_t n, int32_t K, bool cm) {
   const int64_t waves = std::max<int64_t>(1, cm ? (n + 63) / 64 : n);
   const int64_t want = (kLossWaves + waves - 1) / waves;
   const int64_t most = (K + (cm ? 255 : 1023)) / (cm ? 256 : 1024);
@@ -265,16 +264,16 @@ static dim3 rows_grid(const ScoresView& s, int32_t splits) {
 
 template <typename T, bool REF>
 static int stats_of(const ScoresView& s, const ScoresView& ref, const int32_t* label,
-                    const uint8_t* mask, RowStats* part, hipStream_t st) {
+                    RowStats* part, hipStream_t st) {
   const int32_t splits = loss_splits(s.n, s.K, s.class_major());
   const int32_t span = (s.K + splits - 1) / splits;
   const dim3 grid = rows_grid(s, splits);
   if (s.class_major())
     hipLaunchKernelGGL((row_stats_kernel<T, true, REF>), grid, dim3(256), 0, st, s, ref, label,
-                       mask, span, part);
+                       span, part);
   else
     hipLaunchKernelGGL((row_stats_kernel<T, false, REF>), grid, dim3(256), 0, st, s, ref, label,
-                       mask, span, part);
+                       span, part);
   WGBM_LAUNCH_CHECK();
   return 0;
 }
@@ -301,11 +300,11 @@ static unsigned row_blocks(int64_t n, int32_t splits) {
 }
 
 template <typename T>
-static int log_probs_t(const ScoresView& s, const int32_t* label, const uint8_t* mask,
-                       float* log_prob, float* norm, void* ws, hipStream_t st) {
+static int log_probs_t(const ScoresView& s, const int32_t* label, float* log_prob, float* norm,
+                       void* ws, hipStream_t st) {
   RowStats* part = (RowStats*)ws;
   const int32_t splits = loss_splits(s.n, s.K, s.class_major());
-  const int r = stats_of<T, false>(s, ScoresView{}, label, mask, part, st);
+  const int r = stats_of<T, false>(s, ScoresView{}, label, part, st);
   if (r) return r;
   hipLaunchKernelGGL((log_prob_rows_kernel<T>), dim3(row_blocks(s.n, splits)), dim3(256), 0, st, s,
                      label, part, splits, log_prob, (float2*)norm);
@@ -313,27 +312,25 @@ static int log_probs_t(const ScoresView& s, const int32_t* label, const uint8_t*
   return 0;
 }
 
-int class_log_probs(const ScoresView& s, const int32_t* label, const uint8_t* mask,
-                    float* log_prob, float* norm, void* ws, hipStream_t st) {
-  if (log_prob) {
-    bool done = false;
+int class_log_probs(const ScoresView& s, const int32_t* label, float* log_prob, float* norm,
+                    void* ws, hipStream_t st) {
+  if (rows_fit(s, false)) {
     const auto rows = s.dtype == kF32    ? log_probs_rows_f32
                       : s.dtype == kBF16 ? log_probs_rows_bf16
                                          : log_probs_rows_f16;
-    const int r = rows(s, label, log_prob, norm, st, &done);
-    if (r || done) return r;
+    return rows(s, label, log_prob, norm, st);
   }
-  LOSS_TYPES(s.dtype, return log_probs_t<T>(s, label, mask, log_prob, norm, ws, st));
+  LOSS_TYPES(s.dtype, return log_probs_t<T>(s, label, log_prob, norm, ws, st));
 }
 
 int class_log_probs_grad(const ScoresView& s, const int32_t* label, const float* norm,
                          const float* grad, const ScoresView& out, hipStream_t st) {
-  bool done = false;
-  const auto rows = s.dtype == kF32    ? log_probs_grad_rows_f32
-                    : s.dtype == kBF16 ? log_probs_grad_rows_bf16
-                                       : log_probs_grad_rows_f16;
-  const int r = rows(s, label, norm, grad, out, st, &done);
-  if (r || done) return r;
+  if (rows_fit(s, false)) {
+    const auto rows = s.dtype == kF32    ? log_probs_grad_rows_f32
+                      : s.dtype == kBF16 ? log_probs_grad_rows_bf16
+                                         : log_probs_grad_rows_f16;
+    return rows(s, label, norm, grad, out, st);
+  }
   LOSS_TYPES(s.dtype, {
     const LogProbGrad<T> g{label, (const float2*)norm, grad};
     return grad_of<T>(s, ScoresView{}, g, false, out, st);
@@ -346,7 +343,7 @@ static int policy_t(const ScoresView& s, const ScoresView& ref, const PolicyRows
   const int32_t splits = loss_splits(s.n, s.K, s.class_major());
   RowCoef* coef = (RowCoef*)ws;
   RowStats* part = (RowStats*)(coef + s.n);
-  int r = stats_of<T, REF>(s, ref, g.action, nullptr, part, st);
+  int r = stats_of<T, REF>(s, ref, g.action, part, st);
   if (r) return r;
   hipLaunchKernelGGL((policy_rows_kernel<T, REF>), dim3(row_blocks(s.n, splits)), dim3(256), 0, st,
                      s, ref, g, part, splits, out.data ? coef : nullptr);
@@ -357,21 +354,24 @@ static int policy_t(const ScoresView& s, const ScoresView& ref, const PolicyRows
 
 int policy_loss(const ScoresView& s, const ScoresView& ref, const PolicyRows& g,
                 const ScoresView& out, bool accumulate, void* ws, hipStream_t st) {
-  bool done = false;
-  const auto rows = s.dtype == kF32    ? policy_rows_f32
-                    : s.dtype == kBF16 ? policy_rows_bf16
-                                       : policy_rows_f16;
-  const int r = rows(s, ref, g, out, accumulate, st, &done);
-  if (r || done) return r;
+  if (rows_fit(s, ref.data != nullptr)) {
+    const auto rows = s.dtype == kF32    ? policy_rows_f32
+                      : s.dtype == kBF16 ? policy_rows_bf16
+                                         : policy_rows_f16;
+    return rows(s, ref, g, out, accumulate, st);
+  }
   if (ref.data) LOSS_TYPES(s.dtype, return (policy_t<T, true>(s, ref, g, out, accumulate, ws, st)));
   LOSS_TYPES(s.dtype, return (policy_t<T, false>(s, ref, g, out, accumulate, ws, st)));
 }
 
-size_t log_probs_workspace(int64_t n, int32_t K, bool cm) {
-  return sizeof(RowStats) * (size_t)n * loss_splits(n, K, cm);
+static size_t ranges_bytes(const ScoresView& s) {
+  return sizeof(RowStats) * (size_t)s.n * loss_splits(s.n, s.K, s.class_major());
 }
-size_t policy_workspace(int64_t n, int32_t K, bool cm) {
-  return sizeof(RowCoef) * (size_t)n + log_probs_workspace(n, K, cm);
+size_t log_probs_workspace(const ScoresView& s) {
+  return rows_fit(s, false) ? 0 : ranges_bytes(s);
+}
+size_t policy_workspace(const ScoresView& s) {
+  return rows_fit(s, true) ? 0 : sizeof(RowCoef) * (size_t)s.n + ranges_bytes(s);
 }
 
 }  // namespace wgbm

@@ -26,29 +26,35 @@ constexpr int64_t kLossWaves = 4096;
     }                                 \
   } while (0)
 
-int32_t loss_splits(int64_t n, int32_t K, bool cm);
-
-size_t log_probs_workspace(int64_t n, int32_t K, bool cm);
-int class_log_probs(const ScoresView& s, const int32_t* label, const uint8_t* mask,
-                    float* log_prob, float* norm, void* ws, hipStream_t st);
+size_t log_probs_workspace(const ScoresView& s);
+int class_log_probs(const ScoresView& s, const int32_t* label, float* log_prob, float* norm,
+                    void* ws, hipStream_t st);
 int class_log_probs_grad(const ScoresView& s, const int32_t* label, const float* norm,
                          const float* grad, const ScoresView& out, hipStream_t st);
 
-// rows that fit a thread group's registers, one launch (losses_rows_*.hip);
-// *done = false where they do not
+// Whether rows fit the registers of the threads that share them (one launch,
+// losses_rows.hpp).  Class-major: 16 waves' slices of 32 classes.  Row-major:
+// 1024 threads of 16 chunks of 16 bytes (64 of the 128 registers that a thread
+// has), of 4 with a second matrix: with 8 the registers no longer hold the
+// passes (2000 x 50000 bfloat16 against a reference 882 us, the ranged path 420).
+// Shorter rows than a chunk: a thread each.
+inline bool rows_fit(const ScoresView& s, bool ref) {
+  const int32_t VE = s.dtype == kF32 ? 4 : 8;
+  if (s.class_major()) return s.K <= 512;
+  return s.K < VE || (s.K + VE - 1) / VE <= (ref ? 4096 : 16384);
+}
 #define LOSS_ROWS(t)                                                                             \
   int log_probs_grad_rows_##t(const ScoresView& s, const int32_t* label, const float* norm,      \
-                              const float* grad, const ScoresView& out, hipStream_t st,          \
-                              bool* done);                                                       \
+                              const float* grad, const ScoresView& out, hipStream_t st);         \
   int log_probs_rows_##t(const ScoresView& s, const int32_t* label, float* log_prob, float* norm, \
-                         hipStream_t st, bool* done);                                            \
+                         hipStream_t st);                                                        \
   int policy_rows_##t(const ScoresView& s, const ScoresView& ref, const PolicyRows& g,           \
-                      const ScoresView& out, bool accumulate, hipStream_t st, bool* done)
+                      const ScoresView& out, bool accumulate, hipStream_t st)
 LOSS_ROWS(f32);
 LOSS_ROWS(bf16);
 LOSS_ROWS(f16);
 
-size_t policy_workspace(int64_t n, int32_t K, bool cm);
+size_t policy_workspace(const ScoresView& s);
 int policy_loss(const ScoresView& s, const ScoresView& ref, const PolicyRows& g,
                 const ScoresView& out, bool accumulate, void* ws, hipStream_t st);
 

@@ -162,22 +162,16 @@ __global__ __launch_bounds__(F::kMax) void policy_frame_kernel(ScoresView s, Sco
 }
 
 // ---------------------------------------------------------------------------
-// which frame a call takes: f(frame tag, workgroups, threads) for the smallest
-// one that holds the rows, false where none does
+// which frame a call takes: fn(frame tag, workgroups, threads) for the smallest
+// one that holds the rows (rows_fit)
 // ---------------------------------------------------------------------------
-// most 16-byte chunks of one matrix in a thread's registers: 16 (64 registers
-// of 128 that a workgroup of 1024 threads has), 4 with a second matrix (with 8
-// the registers no longer hold the passes: 2000 x 50000 bfloat16 677 us, the
-// ranged path 415)
 template <typename T, bool REF, typename Fn>
-static bool pick_row_frame(const ScoresView& s, Fn fn) {
+static void pick_row_frame(const ScoresView& s, Fn fn) {
   constexpr int VE = Chunk<T>::VE;
-  if (s.K < VE) return false;
   const int64_t chunks = (s.K + VE - 1) / VE;
   const auto go = [&](auto tag) {
     using F = typename decltype(tag)::type;
     fn(tag, (s.n + F::kRows - 1) / F::kRows, F::kThreads);
-    return true;
   };
   if (chunks <= 4) return go(FrameTag<RowFrame<T, 4, 1>>());
   if (chunks <= 16) return go(FrameTag<RowFrame<T, 16, 1>>());
@@ -185,79 +179,71 @@ static bool pick_row_frame(const ScoresView& s, Fn fn) {
   if (chunks <= 256) return go(FrameTag<RowFrame<T, 64, 4>>());
   if (chunks <= 1024) return go(FrameTag<RowFrame<T, 256, 4>>());
   if (chunks <= 2048) return go(FrameTag<RowFrame<T, 256, 8>>());
-  if (chunks <= 4096) return go(FrameTag<RowFrame<T, 1024, 4>>());
+  if (REF || chunks <= 4096) return go(FrameTag<RowFrame<T, 1024, 4>>());
   if constexpr (!REF) {
     if (chunks <= 8192) return go(FrameTag<RowFrame<T, 1024, 8>>());
-    if (chunks <= 16384) return go(FrameTag<RowFrame<T, 1024, 16>>());
+    go(FrameTag<RowFrame<T, 1024, 16>>());
   }
-  return false;
+}
+
+template <typename T, typename Fn>
+static void pick_class_frame(const ScoresView& s, Fn fn) {
+  const int64_t blocks = (s.n + 255) / 256, tiles = (s.n + 63) / 64;
+  if (!s.class_major()) {  // rows shorter than a chunk
+    if (s.K <= 4) return fn(FrameTag<ClassFrame<T, 4, false, false>>(), blocks, 256);
+    return fn(FrameTag<ClassFrame<T, 8, false, false>>(), blocks, 256);
+  }
+  if (s.K <= 4) return fn(FrameTag<ClassFrame<T, 4, false, true>>(), blocks, 256);
+  if (s.K <= 8) return fn(FrameTag<ClassFrame<T, 8, false, true>>(), blocks, 256);
+  if (s.K <= 12) return fn(FrameTag<ClassFrame<T, 12, false, true>>(), blocks, 256);
+  if (s.K <= 16) return fn(FrameTag<ClassFrame<T, 16, false, true>>(), blocks, 256);
+  if (s.K <= 256)
+    return fn(FrameTag<ClassFrame<T, 16, true, true>>(), tiles, 64 * (int)((s.K + 15) / 16));
+  fn(FrameTag<ClassFrame<T, 32, true, true>>(), tiles, 64 * (int)((s.K + 31) / 32));
 }
 
 template <typename T, bool REF, typename Fn>
-static bool pick_class_frame(const ScoresView& s, Fn fn) {
-  const int64_t blocks = (s.n + 255) / 256, tiles = (s.n + 63) / 64;
-  if (!s.class_major()) {  // short rows
-    if (s.K <= 4) return fn(FrameTag<ClassFrame<T, 4, false, false>>(), blocks, 256), true;
-    return fn(FrameTag<ClassFrame<T, 8, false, false>>(), blocks, 256), true;
-  }
-  if (s.K <= 4) return fn(FrameTag<ClassFrame<T, 4, false, true>>(), blocks, 256), true;
-  if (s.K <= 8) return fn(FrameTag<ClassFrame<T, 8, false, true>>(), blocks, 256), true;
-  if (s.K <= 12) return fn(FrameTag<ClassFrame<T, 12, false, true>>(), blocks, 256), true;
-  if (s.K <= 16) return fn(FrameTag<ClassFrame<T, 16, false, true>>(), blocks, 256), true;
-  if (s.K <= 256)
-    return fn(FrameTag<ClassFrame<T, 16, true, true>>(), tiles, 64 * (int)((s.K + 15) / 16)), true;
-  if (s.K <= 512)
-    return fn(FrameTag<ClassFrame<T, 32, true, true>>(), tiles, 64 * (int)((s.K + 31) / 32)), true;
-  return false;
-}
-
-// short rows next to each other are read by a thread each
-template <typename T>
-static bool by_class_frame(const ScoresView& s) {
-  return s.class_major() || s.K < Chunk<T>::VE;
+static void pick_frame(const ScoresView& s, Fn fn) {
+  if (s.class_major() || s.K < Chunk<T>::VE)
+    pick_class_frame<T>(s, fn);
+  else
+    pick_row_frame<T, REF>(s, fn);
 }
 
 template <typename T>
 static int log_probs_frames(const ScoresView& s, const int32_t* label, float* log_prob,
-                            float* norm, hipStream_t st, bool* done) {
-  const auto launch = [&](auto tag, int64_t blocks, int threads) {
+                            float* norm, hipStream_t st) {
+  pick_frame<T, false>(s, [&](auto tag, int64_t blocks, int threads) {
     using F = typename decltype(tag)::type;
     hipLaunchKernelGGL((log_probs_frame_kernel<F>), dim3((unsigned)blocks), dim3(threads), 0, st, s,
                        label, log_prob, (float2*)norm);
-  };
-  *done = by_class_frame<T>(s) ? pick_class_frame<T, false>(s, launch)
-                               : pick_row_frame<T, false>(s, launch);
-  if (*done) WGBM_LAUNCH_CHECK();
+  });
+  WGBM_LAUNCH_CHECK();
   return 0;
 }
 
 template <typename T>
 static int log_probs_grad_frames(const ScoresView& s, const int32_t* label, const float* norm,
-                                 const float* grad, const ScoresView& out, hipStream_t st,
-                                 bool* done) {
+                                 const float* grad, const ScoresView& out, hipStream_t st) {
   const LogProbGrad<T> g{label, (const float2*)norm, grad};
-  const auto launch = [&](auto tag, int64_t blocks, int threads) {
+  pick_frame<T, false>(s, [&](auto tag, int64_t blocks, int threads) {
     using F = typename decltype(tag)::type;
     hipLaunchKernelGGL((log_probs_grad_frame_kernel<F>), dim3((unsigned)blocks), dim3(threads), 0,
                        st, s, g, out);
-  };
-  *done = by_class_frame<T>(s) ? pick_class_frame<T, false>(s, launch)
-                               : pick_row_frame<T, false>(s, launch);
-  if (*done) WGBM_LAUNCH_CHECK();
+  });
+  WGBM_LAUNCH_CHECK();
   return 0;
 }
 
 template <typename T, bool REF>
 static int policy_frames(const ScoresView& s, const ScoresView& ref, const PolicyRows& g,
-                         const ScoresView& out, bool accumulate, hipStream_t st, bool* done) {
-  const auto launch = [&](auto tag, int64_t blocks, int threads) {
+                         const ScoresView& out, bool accumulate, hipStream_t st) {
+  pick_frame<T, REF>(s, [&](auto tag, int64_t blocks, int threads) {
     using F = typename decltype(tag)::type;
     hipLaunchKernelGGL((policy_frame_kernel<F, REF>), dim3((unsigned)blocks), dim3(threads), 0, st,
                        s, ref, g, out, accumulate);
-  };
-  *done = by_class_frame<T>(s) ? pick_class_frame<T, REF>(s, launch)
-                               : pick_row_frame<T, REF>(s, launch);
-  if (*done) WGBM_LAUNCH_CHECK();
+  });
+  WGBM_LAUNCH_CHECK();
   return 0;
 }
 

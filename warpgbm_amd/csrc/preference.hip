@@ -19,65 +19,71 @@
 
 namespace wgbm {
 
-// sum of u over the rows [b, e), by a wave (every lane gets it)
-__device__ __forceinline__ double wave_rows_sum(const PreferenceArgs& a, int64_t b, int64_t e) {
+// Rows are read and written four to a lane, 16 bytes wherever they begin (this
+// GPU takes such addresses): a wave has 256 rows a load.  A lane whose four would
+// pass the end reads the last four instead (no branch: all loads are in flight
+// together) and leaves out those that are another lane's.
+struct Rows4 {
+  float v[4];
+};
+__device__ __forceinline__ Rows4 load_rows(const float* p) {
+  Rows4 r;
+  __builtin_memcpy(&r, p, 16);
+  return r;
+}
+
+// sum of u over the rows [b, b + n), by the lanes of a wave (each its own part)
+template <int U>
+__device__ __forceinline__ double lane_rows_sum(const PreferenceArgs& a, int64_t b, int n) {
   const int lane = threadIdx.x & 63;
-  double x[4] = {0.0, 0.0, 0.0, 0.0};
-  int64_t i = b + lane;
-  // four rows a lane in flight
-  for (; i + 192 < e; i += 256) {
-    float l[4], r[4];
+  const float* lp = a.log_prob + b;
+  const float* ref = a.ref ? a.ref + b : nullptr;
+  if (n < 4) {
+    if (lane >= n) return 0.0;
+    return (double)lp[lane] - (ref ? (double)ref[lane] : 0.0);
+  }
+  double x[U];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      l[j] = a.log_prob[i + 64 * j];
-      r[j] = a.ref ? a.ref[i + 64 * j] : 0.0f;
+  for (int j = 0; j < U; ++j) x[j] = 0.0;
+  for (int k0 = 4 * lane; k0 < n; k0 += 256 * U) {
+    Rows4 l[U], r[U];
+#pragma unroll
+    for (int j = 0; j < U; ++j) {
+      const int k = k0 + 256 * j, at = k < n - 4 ? k : n - 4;
+      l[j] = load_rows(lp + at);
+      if (ref) r[j] = load_rows(ref + at);
     }
 #pragma unroll
-    for (int j = 0; j < 4; ++j) x[j] += (double)l[j] - (double)r[j];
-  }
-  float l[3], r[3];
+    for (int j = 0; j < U; ++j) {
+      const int k = k0 + 256 * j, skip = k < n - 4 ? 0 : k - (n - 4);
 #pragma unroll
-  for (int j = 0; j < 3; ++j) {
-    const bool in = i + 64 * j < e;
-    l[j] = in ? a.log_prob[i + 64 * j] : 0.0f;
-    r[j] = in && a.ref ? a.ref[i + 64 * j] : 0.0f;
+      for (int e = 0; e < 4; ++e) {
+        const double u = (double)l[j].v[e] - (ref ? (double)r[j].v[e] : 0.0);
+        if (e >= skip) x[j] += u;
+      }
+    }
   }
+  double s = x[0];
 #pragma unroll
-  for (int j = 0; j < 3; ++j) x[j] += (double)l[j] - (double)r[j];
-  double s = (x[0] + x[1]) + (x[2] + x[3]);
+  for (int j = 1; j < U; ++j) s += x[j];
+  return s;
+}
+__device__ __forceinline__ double wave_sum(double s) {
   for (int o = 32; o; o >>= 1) s += __shfl_xor(s, o);
   return s;
 }
 
-// sum of u over the rows [b0, b0 + n0) less that over [b1, b1 + n1), by a wave:
-// one list of rows, eight a lane in flight
-__device__ __forceinline__ double wave_difference(const PreferenceArgs& a, int64_t b0, int n0,
-                                                  int64_t b1, int n1) {
-  constexpr int U = 8;
-  double x[2] = {0.0, 0.0};
-  for (int i = threadIdx.x & 63; i < n0 + n1; i += 64 * U) {
-    float l[U], r[U];
-#pragma unroll
-    for (int j = 0; j < U; ++j) {
-      const int k = i + 64 * j;
-      const int64_t at = k < n0 ? b0 + k : b1 + (k - n0);
-      l[j] = k < n0 + n1 ? a.log_prob[at] : 0.0f;
-      r[j] = a.ref && k < n0 + n1 ? a.ref[at] : 0.0f;
-    }
-#pragma unroll
-    for (int j = 0; j < U; ++j) {
-      const double u = (double)l[j] - (double)r[j];
-      x[j % 2] += i + 64 * j < n0 ? u : -u;
+// grad = g for the rows [b, b + n), by a wave
+__device__ __forceinline__ void wave_rows_fill(float* grad, int64_t b, int n, float g) {
+  float* p = grad + b;
+  const Rows4 v = {{g, g, g, g}};
+  for (int k = 4 * (threadIdx.x & 63); k < n; k += 256) {
+    if (n - k >= 4) {
+      __builtin_memcpy(p + k, &v, 16);
+    } else {
+      for (int j = k; j < n; ++j) p[j] = g;
     }
   }
-  double s = x[0] + x[1];
-  for (int o = 32; o; o >>= 1) s += __shfl_xor(s, o);
-  return s;
-}
-
-// grad = g for the rows [b, e), by a wave
-__device__ __forceinline__ void wave_rows_fill(float* grad, int64_t b, int64_t e, float g) {
-  for (int64_t i = b + (threadIdx.x & 63); i < e; i += 64) grad[i] = g;
 }
 
 struct PairLoss {
@@ -107,24 +113,26 @@ __global__ __launch_bounds__(256) void preference_fused_kernel(PreferenceArgs a)
     const int64_t k = t - a.n_pairs;
     if (a.grad && k < a.n_idle) {
       const int64_t b = a.idle[2 * k], e = a.idle[2 * k + 1];
-      wave_rows_fill(a.grad, b, e, 0.0f);
+      wave_rows_fill(a.grad, b, (int)(e - b), 0.0f);
     }
     return;
   }
   const int32_t s0 = a.pairs[2 * t], s1 = a.pairs[2 * t + 1];
-  const int64_t b0 = a.seg_start[s0], e0 = a.seg_start[s0 + 1];
-  const int64_t b1 = a.seg_start[s1], e1 = a.seg_start[s1 + 1];
+  const int64_t b0 = a.seg_start[s0], b1 = a.seg_start[s1];
+  const int n0 = (int)(a.seg_start[s0 + 1] - b0), n1 = (int)(a.seg_start[s1 + 1] - b1);
   const float w = a.weight ? a.weight[t] : 1.0f;
   PairLoss o{0.0f, 0.0f, 0.0f};
-  if (w != 0.0f)
-    o = pair_loss(a, wave_difference(a, b0, (int)(e0 - b0), b1, (int)(e1 - b1)), w);
+  if (w != 0.0f) {
+    const double x = lane_rows_sum<2>(a, b0, n0), y = lane_rows_sum<2>(a, b1, n1);
+    o = pair_loss(a, wave_sum(x - y), w);
+  }
   if (lane == 0) {
     a.loss[t] = o.loss;
     a.margin[t] = o.margin;
   }
   if (!a.grad) return;
-  wave_rows_fill(a.grad, b0, e0, o.slope);
-  wave_rows_fill(a.grad, b1, e1, -o.slope);
+  wave_rows_fill(a.grad, b0, n0, o.slope);
+  wave_rows_fill(a.grad, b1, n1, -o.slope);
 }
 
 // ---------------------------------------------------------------------------
@@ -134,7 +142,8 @@ __global__ __launch_bounds__(256) void preference_fused_kernel(PreferenceArgs a)
 __global__ __launch_bounds__(256) void task_sums_kernel(PreferenceArgs a, double* __restrict__ part) {
   const int64_t t = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
   if (t >= a.n_tasks || a.task[3 * t] < 0) return;
-  const double x = wave_rows_sum(a, a.task[3 * t + 1], a.task[3 * t + 2]);
+  const int64_t b = a.task[3 * t + 1];
+  const double x = wave_sum(lane_rows_sum<4>(a, b, (int)(a.task[3 * t + 2] - b)));
   if ((threadIdx.x & 63) == 0) part[t] = x;
 }
 
@@ -250,7 +259,8 @@ __global__ __launch_bounds__(256) void task_rows_kernel(PreferenceArgs a,
   const int64_t t = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
   if (t >= a.n_tasks) return;
   const int64_t s = a.task[3 * t];
-  wave_rows_fill(a.grad, a.task[3 * t + 1], a.task[3 * t + 2], s >= 0 ? seq[s] : 0.0f);
+  const int64_t b = a.task[3 * t + 1];
+  wave_rows_fill(a.grad, b, (int)(a.task[3 * t + 2] - b), s >= 0 ? seq[s] : 0.0f);
 }
 
 // ---------------------------------------------------------------------------

@@ -23,6 +23,7 @@ HIP graph.  Wrong types, shapes, devices or layouts raise ``RuntimeError``.
 from __future__ import annotations
 
 import ctypes as C
+import functools
 from collections import namedtuple
 
 import numpy as np
@@ -124,10 +125,24 @@ class _on:
             torch.cuda.set_device(self.back)
 
 
-def _workspace(nbytes, device, what):
+@functools.lru_cache(maxsize=4096)
+def _bytes_of(entry, dtype, n, K, class_major):
+    """What a _workspace entry returns for scores of a shape and order (a call
+    into the library costs more than the small losses' launches)."""
+    v = _lib.Scores(16, dtype, n, K, 1 if class_major else K, max(n, 2) if class_major else 1)
+    return getattr(_lib.load(), entry)(C.byref(v))
+
+
+def _workspace(entry, v, device):
+    """Working memory of a call: (tensor or None, address, bytes)."""
+    nbytes = _bytes_of(entry, v.dtype, v.n_rows, v.n_classes,
+                       v.row_stride == 1 and v.class_stride != 1)
     if nbytes < 0:
-        _lib.check(1000, what)
-    return torch.empty(max(int(nbytes), 16), dtype=torch.uint8, device=device)
+        _lib.check(1000, entry)
+    if nbytes == 0:
+        return None, None, 0
+    t = torch.empty(nbytes, dtype=torch.uint8, device=device)
+    return t, t.data_ptr(), nbytes
 
 
 def class_log_probs(scores, labels) -> ClassLogProbs:
@@ -142,9 +157,9 @@ def class_log_probs(scores, labels) -> ClassLogProbs:
     with _on(dev):
         log_prob = torch.empty(n, dtype=torch.float32, device=dev)
         norm = torch.empty((n, 2), dtype=torch.float32, device=dev)
-        ws = _workspace(lib.wgbm_class_log_probs_workspace(C.byref(v)), dev, "class_log_probs")
-        rc = lib.wgbm_class_log_probs(C.byref(v), lab, log_prob.data_ptr(), norm.data_ptr(),
-                                      ws.data_ptr(), ws.numel(), _lib.current_stream_ptr(dev))
+        ws, at, size = _workspace("wgbm_class_log_probs_workspace", v, dev)
+        rc = lib.wgbm_class_log_probs(C.byref(v), lab, log_prob.data_ptr(), norm.data_ptr(), at,
+                                      size, _lib.current_stream_ptr(dev))
     _lib.check(rc, "class_log_probs")
     return ClassLogProbs(log_prob, norm)
 
@@ -216,12 +231,12 @@ def policy_loss(scores, actions, old_log_prob, advantage, *, weight=None, ref_lo
         kl = None
         if ref_scores is not None or ref_log_prob is not None:
             kl = torch.empty(n, dtype=f32, device=dev)
-        ws = _workspace(lib.wgbm_policy_loss_workspace(C.byref(v)), dev, "policy_loss")
+        ws, at, size = _workspace("wgbm_policy_loss_workspace", v, dev)
         rc = lib.wgbm_policy_loss(
             C.byref(v), C.byref(args), loss.data_ptr(), log_prob.data_ptr(),
             kl.data_ptr() if kl is not None else None,
-            C.byref(gv) if gv is not None else None, int(grad is not None), ws.data_ptr(),
-            ws.numel(), _lib.current_stream_ptr(dev))
+            C.byref(gv) if gv is not None else None, int(grad is not None), at, size,
+            _lib.current_stream_ptr(dev))
     _lib.check(rc, "policy_loss")
     return PolicyLoss(loss, log_prob, kl, out)
 
@@ -248,11 +263,11 @@ def balance_loss(scores, *, top_k=1, mask=None, coef=1.0, grad=None,
         loss = torch.empty((), dtype=torch.float32, device=dev)
         counts = torch.empty(K, dtype=torch.int64, device=dev)
         prob = torch.empty(K, dtype=torch.float32, device=dev)
-        ws = _workspace(lib.wgbm_balance_loss_workspace(C.byref(v)), dev, "balance_loss")
+        ws, at, size = _workspace("wgbm_balance_loss_workspace", v, dev)
         rc = lib.wgbm_balance_loss(
             C.byref(v), mask, int(top_k), float(coef), loss.data_ptr(), counts.data_ptr(),
             prob.data_ptr(), C.byref(gv) if gv is not None else None, int(grad is not None),
-            ws.data_ptr(), ws.numel(), _lib.current_stream_ptr(dev))
+            at, size, _lib.current_stream_ptr(dev))
     _lib.check(rc, "balance_loss")
     return BalanceLoss(loss, counts, prob, out)
 
@@ -314,6 +329,7 @@ class PreferencePlan:
         self.pairs = pairs.to(torch.int32).contiguous().clone()
         self.task = self.task_start = self.piece = self.multi = self.idle = None
         self.disjoint = False
+        self.workspace_bytes = None
         degree = self._incidences(device)
         if seg is not None:
             self._tasks(seg, length, last, longest, degree, device)
@@ -437,9 +453,16 @@ def preference_loss(log_prob, plan, *, ref_log_prob=None, weight=None, beta=1.0,
         loss = torch.empty(P, dtype=f32, device=dev)
         margin = torch.empty(P, dtype=f32, device=dev)
         grad = torch.empty(n, dtype=f32, device=dev) if with_grad else None
-        ws = _workspace(lib.wgbm_preference_loss_workspace(C.byref(args)), dev, "preference_loss")
+        size = plan.workspace_bytes  # (of the plan alone)
+        if size is None:
+            size = lib.wgbm_preference_loss_workspace(C.byref(args))
+            if size < 0:
+                _lib.check(1000, "preference_loss")
+            plan.workspace_bytes = size
+        ws = torch.empty(size, dtype=torch.uint8, device=dev) if size else None
         rc = lib.wgbm_preference_loss(C.byref(args), loss.data_ptr(), margin.data_ptr(),
                                       grad.data_ptr() if grad is not None else None,
-                                      ws.data_ptr(), ws.numel(), _lib.current_stream_ptr(dev))
+                                      ws.data_ptr() if ws is not None else None, size,
+                                      _lib.current_stream_ptr(dev))
     _lib.check(rc, "preference_loss")
     return PreferenceLoss(loss, margin, grad)
