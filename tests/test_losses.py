@@ -130,6 +130,10 @@ def check(got, want, tol, what):
 SHAPES = [(1, 1), (5, 1), (1, 2), (1, 3), (3, 2), (64, 10), (65, 7), (257, 10), (1000, 3),
           (63, 31), (130, 32), (70, 33), (33, 64), (9, 65), (300, 100), (21, 257), (50, 513),
           (7, 1000), (3, 4097), (2, 20001)]
+# rows enough for a workgroup to take several a thread group, a part of a
+# workgroup left over
+MANY_ROWS = [(262_147, 10), (131_075, 33), (66_000, 65), (33_001, 130), (17_003, 257),
+             (8_300, 700)]
 ORDERS = ["row", "class", "row+", "class+"]
 
 
@@ -182,6 +186,45 @@ def test_log_probs_and_gradient(gpu, dtype, order):
         grad[odd] = -P[odd] * up.to(F64)[odd, None]
         grad[odd, a[odd].long()] += up.to(F64)[odd]
         check(got, grad, grad_tol(grad, up.abs().to(F64), dtype), "gradient")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", list(DTYPES))
+def test_many_rows(gpu, dtype):
+    """The first, some middle and the last rows of large matrices against the
+    same rows alone, which float64 forms check above (a row's results may differ
+    by the order of its sums)."""
+    from warpgbm_amd import losses
+
+    for n, K in MANY_ROWS:
+        print_case("many rows", dtype, n, K)
+        g = torch.Generator(device="cuda").manual_seed(K)
+        s = (2 * torch.randn((n, K), generator=g, device="cuda")).to(DTYPES[dtype])
+        a = torch.randint(-1, K, (n,), generator=g, device="cuda", dtype=torch.int32)
+        old = -2 - torch.rand(n, generator=g, device="cuda")
+        adv = torch.randn(n, generator=g, device="cuda")
+        w = (torch.rand(n, generator=g, device="cuda") < 0.9).float()
+        f = losses.class_log_probs(s, a)
+        p = losses.policy_loss(s, a, old, adv, weight=w, ref_log_prob=old, kl_coef=0.1)
+        one = torch.ones(n, device="cuda")
+        b = losses.class_log_probs_grad(s, a, f.norm, one)
+        for at in (0, n // 2 + 1, n - 301):
+            r = slice(at, at + 301)
+            f1 = losses.class_log_probs(s[r], a[r])
+            p1 = losses.policy_loss(s[r], a[r], old[r], adv[r], weight=w[r], ref_log_prob=old[r],
+                                    kl_coef=0.1)
+            # log-probabilities down to some -20: 2 STEPS of rounding
+            assert torch.allclose(f.log_prob[r], f1.log_prob, rtol=0, atol=2 * STEPS * U)
+            assert torch.allclose(p.log_prob[r], p1.log_prob, rtol=0, atol=2 * STEPS * U)
+            size = (1 + adv[r].abs()) * (1 + torch.exp(p1.log_prob - old[r]))
+            assert ((p.loss[r] - p1.loss).abs() <= 60 * STEPS * U * size).all()
+            fin = torch.finfo(s.dtype)
+            step = (0.0 if dtype == "f32" else fin.eps) + 1e-30
+            tol = 60 * STEPS * U * size[:, None] + step * p1.grad[:].float().abs() + 2.0 ** -24
+            assert ((p.grad[r].float() - p1.grad.float()).abs() <= tol).all()
+            b1 = losses.class_log_probs_grad(s[r], a[r], f1.norm, one[r])
+            tol = STEPS * U + step * b1.float().abs() + 2.0 ** -24
+            assert ((b[r].float() - b1.float()).abs() <= tol).all()
 
 
 # --------------------------------------------------------------------- policy

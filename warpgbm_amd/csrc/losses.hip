@@ -110,17 +110,6 @@ __global__ __launch_bounds__(256) void log_prob_rows_kernel(ScoresView s,
   write_log_prob(a, sa, lab, i, log_prob, norm);
 }
 
-// log p of the label in float64, by the 64 lanes of a wave
-template <typename T>
-__device__ __attribute__((noinline)) double wave_exact_logp(const T* p, int64_t ks, int32_t K,
-                                                            int32_t label, float m) {
-  double z = 0.0;
-  for (int32_t k = threadIdx.x & 63; k < K; k += 64)
-    z += exp((double)to_f32(p[(int64_t)k * ks]) - (double)m);
-  for (int o = 32; o; o >>= 1) z += __shfl_xor(z, o);
-  return (double)to_f32(p[(int64_t)label * ks]) - (double)m - log(z);
-}
-
 template <typename T, bool REF>
 __global__ __launch_bounds__(256) void policy_rows_kernel(ScoresView s, ScoresView ref,
                                                           PolicyRows g,

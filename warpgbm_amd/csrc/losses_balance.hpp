@@ -208,9 +208,13 @@ static void balance_frame(const ScoresView& s, Fn fn) {
     fn(tag, (s.n + F::kRows - 1) / F::kRows, F::kThreads);
   };
   if (chunks <= 4) return go(FrameTag<RowFrame<T, 4, 1>>());
+  if (chunks <= 8) return go(FrameTag<RowFrame<T, 8, 1>>());
   if (chunks <= 16) return go(FrameTag<RowFrame<T, 16, 1>>());
+  if (chunks <= 32) return go(FrameTag<RowFrame<T, 32, 1>>());
   if (chunks <= 64) return go(FrameTag<RowFrame<T, 64, 1>>());
+  if (chunks <= 128) return go(FrameTag<RowFrame<T, 64, 2>>());
   if (chunks <= 256) return go(FrameTag<RowFrame<T, 64, 4>>());
+  if (chunks <= 512) return go(FrameTag<RowFrame<T, 256, 2>>());
   return go(FrameTag<RowFrame<T, 256, 4>>());
 }
 

@@ -123,6 +123,17 @@ struct LogProbGrad {
   }
 };
 
+// log p of the label in float64, by the 64 lanes of a wave
+template <typename T>
+__device__ __forceinline__ double wave_exact_logp(const T* p, int64_t ks, int32_t K,
+                                                            int32_t label, float m) {
+  double z = 0.0;
+  for (int32_t k = threadIdx.x & 63; k < K; k += 64)
+    z += exp((double)to_f32(p[(int64_t)k * ks]) - (double)m);
+  for (int o = 32; o; o >>= 1) z += __shfl_xor(z, o);
+  return (double)to_f32(p[(int64_t)label * ks]) - (double)m - log(z);
+}
+
 // ---------------------------------------------------------------------------
 // reductions over a group of G lanes (a power of two up to 64, aligned); every
 // lane gets the same bits (each step combines two values that commute)
@@ -184,7 +195,7 @@ struct RowFrame {
   static constexpr int G = G_, NC = NC_, VE = Chunk<T>::VE, N = NC * VE;
   static constexpr int kWords = 4 * NC;  // registers of a thread's scores
   static constexpr int kThreads = G <= 256 ? 256 : G, kMax = kThreads;
-  static constexpr bool kBarrier = G > 64, kSlices = false;
+  static constexpr bool kBarrier = G > 64, kSlices = false, kLaneRows = false;
   static constexpr int kShared = 1;  // rows that the waves of a workgroup share
   static constexpr int kRows = kThreads / G;  // rows of a workgroup
   static constexpr int kBuf = G > 64 ? G / 64 : 1;
@@ -273,6 +284,7 @@ struct RowFrame {
   // reductions over the row; buf as for waves_reduce (kBuf words each)
   template <typename Op>
   __device__ __forceinline__ float reduce(float x, Op op, float* buf) const {
+    // (buf is null where rows are one wave's)
     if (G <= 64) return lanes_reduce<(G < 64 ? G : 64)>(x, op);
     return waves_reduce<(G > 64 ? G / 64 : 1)>(x, op, buf);
   }
@@ -376,7 +388,7 @@ struct ClassFrame {
   using T = T_;
   static constexpr int N = N_, kWords = N_;
   static constexpr int kMax = SLICES ? 1024 : 256;
-  static constexpr bool kBarrier = SLICES, kSlices = SLICES;
+  static constexpr bool kBarrier = SLICES, kSlices = SLICES, kLaneRows = true;
   static constexpr int kShared = SLICES ? 64 : 1;
   static constexpr int kBuf = SLICES ? 16 * 64 : 1;
   int32_t w, S, K;

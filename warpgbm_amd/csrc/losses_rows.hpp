@@ -6,11 +6,11 @@
 
 namespace wgbm {
 
-// a row's statistics from its registers (the label's score sa apart); buf:
-// five reductions' words
+// a row's statistics from its registers, all but the label's own term za; buf:
+// five reductions' words (null where a row is one wave's)
 template <typename F, bool REF>
 __device__ __forceinline__ RowStats frame_stats(const F& f, typename F::Regs& s,
-                                                typename F::Regs& r, int32_t label, float sa,
+                                                typename F::Regs& r, int32_t label,
                                                 float (*buf)[F::kBuf]) {
   RowStats a = empty_stats();
 #pragma unroll
@@ -45,7 +45,6 @@ __device__ __forceinline__ RowStats frame_stats(const F& f, typename F::Regs& s,
     a.zr = f.reduce(a.zr, AddF(), buf[3]);
     a.u = f.reduce(a.u, AddF(), buf[4]);
   }
-  if (label >= 0) a.za = exp2_f32(power_of(sa, b));
   return a;
 }
 
@@ -64,7 +63,8 @@ __global__ __launch_bounds__(F::kMax) void log_probs_frame_kernel(
   const int32_t lab = row_label(label, i, s.K);
   const float sa = lab >= 0 ? score_at<typename F::T>(s, i, lab) : 0.0f;
   f.trim(v);
-  const RowStats a = frame_stats<F, false>(f, v, v, lab, sa, buf);
+  RowStats a = frame_stats<F, false>(f, v, v, lab, buf);
+  if (lab >= 0) a.za = exp2_f32(power_of(sa, base_of(safe_max(a.m))));
   if (!in || !f.first_lane()) return;
   write_log_prob(a, sa, lab, i, log_prob, norm);
 }
@@ -119,7 +119,8 @@ __global__ __launch_bounds__(F::kMax) void policy_frame_kernel(ScoresView s, Sco
   const float A = g.advantage[i], old = g.old_log_prob[i];
   f.trim(v);
   if (REF) f.trim(r);
-  const RowStats st = frame_stats<F, REF>(f, v, r, lab, sa, buf);
+  RowStats st = frame_stats<F, REF>(f, v, r, lab, buf);
+  if (lab >= 0) st.za = exp2_f32(power_of(sa, base_of(safe_max(st.m))));
   // what follows from the row as a whole costs as much as some ten classes:
   // where waves share rows, the first one works it out for all
   const bool owner = !F::kBarrier || threadIdx.x < 64;
@@ -162,6 +163,146 @@ __global__ __launch_bounds__(F::kMax) void policy_frame_kernel(ScoresView s, Sco
 }
 
 // ---------------------------------------------------------------------------
+// Many rows of up to 64 threads each: a workgroup takes B rows a thread group,
+// all loads in flight at once, and a thread a row works out what follows from
+// the row as a whole, which otherwise every wave spends on its one to sixteen
+// rows (the policy loss some 250 instructions, a row's own passes 20 a class and
+// thread).  A row at a time and four: log-probabilities of 300000 x 100 float32
+// 46 and 24 us, 100000 x 500 bfloat16 38 and 26, 1M x 10 float32 18 and 12; the
+// policy loss of 300000 x 100 float32 78 and 60, 1M x 10 38 and 35, but 60000 x
+// 1000 bfloat16 45 and 48 and 100000 x 200 float32 against a reference 64 and 78
+// (their rows hold more registers): those take a row at a time.
+// ---------------------------------------------------------------------------
+template <typename F, int B>
+__global__ __launch_bounds__(256) void log_probs_batch_kernel(ScoresView s,
+                                                              const int32_t* __restrict__ label,
+                                                              float* __restrict__ log_prob,
+                                                              float2* __restrict__ norm) {
+  constexpr int R = F::kRows * B;
+  static_assert(R <= 256, "a thread a row");
+  __shared__ int32_t s_label[R];
+  __shared__ RowStats s_stats[R];
+  const F f(s);
+  const int64_t i = (int64_t)blockIdx.x * R + threadIdx.x;
+  const bool mine = (int)threadIdx.x < R && i < s.n;
+  typename F::Regs v[B];
+#pragma unroll
+  for (int b = 0; b < B; ++b) f.load(v[b], s, (int64_t)blockIdx.x * B + b);
+  const int32_t lab = mine ? row_label(label, i, s.K) : -1;
+  const float sa = lab >= 0 ? score_at<typename F::T>(s, i, lab) : 0.0f;
+  if ((int)threadIdx.x < R) s_label[threadIdx.x] = lab;
+  __syncthreads();
+#pragma unroll
+  for (int b = 0; b < B; ++b) {
+    const int r = b * F::kRows + threadIdx.x / F::G;
+    f.trim(v[b]);
+    const RowStats a = frame_stats<F, false>(f, v[b], v[b], s_label[r], nullptr);
+    if (f.first_lane()) s_stats[r] = a;
+  }
+  __syncthreads();
+  if (!mine) return;
+  RowStats a = s_stats[threadIdx.x];
+  if (lab >= 0) a.za = exp2_f32(power_of(sa, base_of(safe_max(a.m))));
+  write_log_prob(a, sa, lab, i, log_prob, norm);
+}
+
+template <typename F, int B>
+__global__ __launch_bounds__(256) void policy_batch_kernel(ScoresView s, PolicyRows g,
+                                                           ScoresView out, bool accumulate) {
+  using T = typename F::T;
+  constexpr int R = F::kRows * B;
+  static_assert(R <= 256, "a thread a row");
+  __shared__ int32_t s_label[R];
+  __shared__ RowStats s_stats[R];
+  __shared__ RowCoef s_coef[R];
+  const F f(s);
+  const int64_t i = (int64_t)blockIdx.x * R + threadIdx.x;
+  const bool mine = (int)threadIdx.x < R && i < s.n;
+  typename F::Regs v[B];
+#pragma unroll
+  for (int b = 0; b < B; ++b) f.load(v[b], s, (int64_t)blockIdx.x * B + b);
+  const float w = !mine ? 0.0f : g.weight ? g.weight[i] : 1.0f;
+  const int32_t lab = mine ? row_label(g.action, i, s.K) : -1;
+  const bool live = w != 0.0f && lab >= 0;
+  float sa = 0.0f, A = 0.0f, old = 0.0f;
+  if (live) {
+    sa = score_at<T>(s, i, lab);
+    A = g.advantage[i];
+    old = g.old_log_prob[i];
+  }
+  if ((int)threadIdx.x < R) s_label[threadIdx.x] = lab;
+  __syncthreads();
+#pragma unroll
+  for (int b = 0; b < B; ++b) {
+    const int q = b * F::kRows + threadIdx.x / F::G;
+    f.trim(v[b]);
+    const RowStats a = frame_stats<F, false>(f, v[b], v[b], s_label[q], nullptr);
+    if (f.first_lane()) s_stats[q] = a;
+    f.hide(v[b]);
+  }
+  __syncthreads();
+  if ((int)(threadIdx.x & ~63u) < R) {  // (whole waves)
+    PolicyRow o{};
+    RowStats a = empty_stats();
+    if (live) {
+      a = s_stats[threadIdx.x];
+      a.za = exp2_f32(power_of(sa, base_of(safe_max(a.m))));
+      o = policy_row<false>(a, sa, 0.0f, A, old, w, g, i, lab, nullptr);
+    }
+    // rows next to a border, one after the other, each by the whole wave
+    unsigned long long todo = __ballot(o.near);
+    while (todo) {
+      const int src = __ffsll((unsigned long long)todo) - 1;
+      todo &= todo - 1;
+      const int64_t row = i - (int)(threadIdx.x & 63) + src;
+      const double e = wave_exact_logp((const T*)s.data + row * s.rs, s.ks, s.K,
+                                       __shfl(lab, src), __shfl(a.m, src));
+      if ((int)(threadIdx.x & 63) == src)
+        o = policy_row<false>(a, sa, 0.0f, A, old, w, g, i, lab, &e);
+    }
+    if (mine) {
+      g.loss[i] = o.loss;
+      g.log_prob[i] = o.logp;
+      if (g.kl) g.kl[i] = o.kl;
+    }
+    if ((int)threadIdx.x < R) s_coef[threadIdx.x] = o.c;
+  }
+  if (!out.data) return;
+  __syncthreads();
+#pragma unroll
+  for (int b = 0; b < B; ++b) {
+    const int q = b * F::kRows + threadIdx.x / F::G;
+    if ((int64_t)blockIdx.x * R + q >= s.n) continue;
+    const int64_t block = (int64_t)blockIdx.x * B + b;
+    const RowCoef c = s_coef[q];
+    if (!c.live) {
+      if (!accumulate) f.store_zero(out, block);
+      continue;
+    }
+    f.store_row(out, block, accumulate, c.label, c.gl,
+                [&](int j) { return coef_grad<false>(c, F::value(v[b], j), 0.0f); });
+  }
+}
+
+// rows of a thread group in the kernels above (1: a row at a time): four chunks
+// of a thread's registers
+template <typename F, bool POLICY, bool REF>
+constexpr int batch_rows() {
+  if constexpr (F::kLaneRows || REF) {
+    return 1;
+  } else {
+    if (F::G > 64 || (POLICY && (F::NC > 1 || sizeof(typename F::T) != 4))) return 1;
+    return 4 / F::NC < F::G ? 4 / F::NC : F::G;
+  }
+}
+// from 4 workgroups a CU on; with fewer the rows of a group would wait for one
+// another while CUs are idle
+template <typename F, int B>
+static bool batch_pays(const ScoresView& s) {
+  return s.n >= (int64_t)1024 * F::kRows * B;
+}
+
+// ---------------------------------------------------------------------------
 // which frame a call takes: fn(frame tag, workgroups, threads) for the smallest
 // one that holds the rows (rows_fit)
 // ---------------------------------------------------------------------------
@@ -174,9 +315,13 @@ static void pick_row_frame(const ScoresView& s, Fn fn) {
     fn(tag, (s.n + F::kRows - 1) / F::kRows, F::kThreads);
   };
   if (chunks <= 4) return go(FrameTag<RowFrame<T, 4, 1>>());
+  if (chunks <= 8) return go(FrameTag<RowFrame<T, 8, 1>>());
   if (chunks <= 16) return go(FrameTag<RowFrame<T, 16, 1>>());
+  if (chunks <= 32) return go(FrameTag<RowFrame<T, 32, 1>>());
   if (chunks <= 64) return go(FrameTag<RowFrame<T, 64, 1>>());
+  if (chunks <= 128) return go(FrameTag<RowFrame<T, 64, 2>>());
   if (chunks <= 256) return go(FrameTag<RowFrame<T, 64, 4>>());
+  if (chunks <= 512) return go(FrameTag<RowFrame<T, 256, 2>>());
   if (chunks <= 1024) return go(FrameTag<RowFrame<T, 256, 4>>());
   if (chunks <= 2048) return go(FrameTag<RowFrame<T, 256, 8>>());
   if (REF || chunks <= 4096) return go(FrameTag<RowFrame<T, 1024, 4>>());
@@ -215,6 +360,14 @@ static int log_probs_frames(const ScoresView& s, const int32_t* label, float* lo
                             float* norm, hipStream_t st) {
   pick_frame<T, false>(s, [&](auto tag, int64_t blocks, int threads) {
     using F = typename decltype(tag)::type;
+    constexpr int B = batch_rows<F, false, false>();
+    if constexpr (B > 1) {
+      if (batch_pays<F, B>(s)) {
+        hipLaunchKernelGGL((log_probs_batch_kernel<F, B>), dim3((unsigned)((blocks + B - 1) / B)),
+                           dim3(threads), 0, st, s, label, log_prob, (float2*)norm);
+        return;
+      }
+    }
     hipLaunchKernelGGL((log_probs_frame_kernel<F>), dim3((unsigned)blocks), dim3(threads), 0, st, s,
                        label, log_prob, (float2*)norm);
   });
@@ -240,6 +393,14 @@ static int policy_frames(const ScoresView& s, const ScoresView& ref, const Polic
                          const ScoresView& out, bool accumulate, hipStream_t st) {
   pick_frame<T, REF>(s, [&](auto tag, int64_t blocks, int threads) {
     using F = typename decltype(tag)::type;
+    constexpr int B = batch_rows<F, true, REF>();
+    if constexpr (B > 1) {
+      if (batch_pays<F, B>(s)) {
+        hipLaunchKernelGGL((policy_batch_kernel<F, B>), dim3((unsigned)((blocks + B - 1) / B)),
+                           dim3(threads), 0, st, s, g, out, accumulate);
+        return;
+      }
+    }
     hipLaunchKernelGGL((policy_frame_kernel<F, REF>), dim3((unsigned)blocks), dim3(threads), 0, st,
                        s, ref, g, out, accumulate);
   });
