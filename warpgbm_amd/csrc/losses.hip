@@ -187,13 +187,23 @@ __global__ __launch_bounds__(256) void score_grad_kernel(ScoresView s, ScoresVie
         for (int32_t k = k0; k < k1; ++k) o[k * out.ks] = from_f32<T>(0.0f);
       return;
     }
-#pragma unroll 4
-    for (int32_t k = k0; k < k1; ++k) {
-      const float v = to_f32(p[k * s.ks]);
-      const float r = G::kRef ? to_f32(q[k * ref.ks]) : 0.0f;
-      float x = k == c.label ? c.gl : g.at(c, v, r);
-      if (accumulate) x += to_f32(o[k * out.ks]);
-      o[k * out.ks] = from_f32<T>(x);
+    // eight classes' loads in flight (the stores might be to the same memory as
+    // far as the compiler knows)
+    constexpr int U = 8;
+    for (int32_t k = k0; k < k1; k += U) {
+      float v[U], r[U], x[U];
+#pragma unroll
+      for (int j = 0; j < U; ++j) {
+        const int64_t at = k + j < k1 ? k + j : k1 - 1;
+        v[j] = to_f32(p[at * s.ks]);
+        r[j] = G::kRef ? to_f32(q[at * ref.ks]) : 0.0f;
+        x[j] = accumulate ? to_f32(o[at * out.ks]) : 0.0f;
+      }
+#pragma unroll
+      for (int j = 0; j < U; ++j) {
+        x[j] += k + j == c.label ? c.gl : g.at(c, v[j], r[j]);
+        if (k + j < k1) o[(int64_t)(k + j) * out.ks] = from_f32<T>(x[j]);
+      }
     }
     return;
   }
@@ -239,11 +249,11 @@ __global__ __launch_bounds__(256) void score_grad_kernel(ScoresView s, ScoresVie
 // host
 // ---------------------------------------------------------------------------
 // a row's classes in ranges: one range where the rows alone fill the GPU, else
-// ranges of at least 256 classes (row-major: 1024, a wave's 16 loads each)
+// ranges of at least 32 classes (row-major: 1024, a wave's 16 loads each)
 static int32_t loss_splits(int64_t n, int32_t K, bool cm) {
   const int64_t waves = std::max<int64_t>(1, cm ? (n + 63) / 64 : n);
   const int64_t want = (kLossWaves + waves - 1) / waves;
-  const int64_t most = (K + (cm ? 255 : 1023)) / (cm ? 256 : 1024);
+  const int64_t most = (K + (cm ? 31 : 1023)) / (cm ? 32 : 1024);
   return (int32_t)std::max<int64_t>(1, std::min(want, most));
 }
 

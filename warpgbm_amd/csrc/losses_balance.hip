@@ -1,5 +1,7 @@
 // The balance loss: its finishing launch, the transposes of wide class-major
 // scores, and the host side (the passes over rows: losses_balance.hpp).
+#include <type_traits>
+
 #include "losses_balance.hpp"
 
 namespace wgbm {
@@ -73,7 +75,7 @@ __global__ void balance_empty_kernel(int32_t K, BalanceOut o) {
 }
 
 // b(i, k) (+)= a(i, k) between class-major scores (or gradient) and a row-major
-// float32 copy, by tiles of 64 x 64 through LDS
+// copy, by tiles of 64 x 64 through LDS
 template <typename A, typename B, bool TO_ROWS>
 __global__ __launch_bounds__(256) void transpose_kernel(ScoresView a, ScoresView b,
                                                         bool accumulate) {
@@ -103,8 +105,9 @@ __global__ __launch_bounds__(256) void transpose_kernel(ScoresView a, ScoresView
   }
 }
 
-// class-major scores of more classes than a workgroup's slices hold go
-// through a row-major copy, in float32 so that the gradient is rounded once
+// class-major scores of more classes than a workgroup's slices hold go through
+// a row-major copy: of their type, or of float32 where the gradient is added to
+// another (so that it is rounded once)
 constexpr int32_t kClassFrameMax = 512;
 static bool through_rows(int32_t K, bool cm) { return cm && K > kClassFrameMax; }
 
@@ -133,8 +136,20 @@ size_t balance_workspace(const ScoresView& s) {
   return balance_ws(s.n, s.K, s.class_major(), nullptr).bytes;
 }
 
-static dim3 transpose_grid(const ScoresView& s) {
-  return dim3((unsigned)((s.n + 63) / 64), (unsigned)((s.K + 63) / 64));
+// T: the class-major side's type; the row-major side has it too, or float32
+template <typename T, bool TO_ROWS>
+static void transpose(const ScoresView& a, const ScoresView& b, bool accumulate, hipStream_t st) {
+  const dim3 grid((unsigned)((a.n + 63) / 64), (unsigned)((a.K + 63) / 64));
+  const auto go = [&](auto rows) {
+    using R = decltype(rows);
+    using A = std::conditional_t<TO_ROWS, T, R>;
+    using B = std::conditional_t<TO_ROWS, R, T>;
+    hipLaunchKernelGGL((transpose_kernel<A, B, TO_ROWS>), grid, dim3(256), 0, st, a, b, accumulate);
+  };
+  if ((TO_ROWS ? b : a).dtype == kF32)
+    go(float());
+  else
+    go(T());
 }
 
 int balance_loss(const ScoresView& s, const uint8_t* mask, int32_t top_k, float coef,
@@ -151,11 +166,10 @@ int balance_loss(const ScoresView& s, const uint8_t* mask, int32_t top_k, float 
   ScoresView v = s;
   if (turn) {
     v.data = w.rows;
-    v.dtype = kF32;
+    if (accumulate) v.dtype = kF32;
     v.rs = s.K;
     v.ks = 1;
-    LOSS_TYPES(s.dtype, hipLaunchKernelGGL((transpose_kernel<T, float, true>), transpose_grid(s),
-                                           dim3(256), 0, st, s, v, false));
+    LOSS_TYPES(s.dtype, (transpose<T, true>(s, v, false, st)));
     WGBM_LAUNCH_CHECK();
   }
   int32_t groups = 0;
@@ -175,8 +189,7 @@ int balance_loss(const ScoresView& s, const uint8_t* mask, int32_t top_k, float 
   // (in place in the row-major copy: a thread writes what it alone has read)
   r = grad(v, w, turn ? v : out, turn ? false : accumulate, st);
   if (r || !turn) return r;
-  LOSS_TYPES(s.dtype, hipLaunchKernelGGL((transpose_kernel<float, T, false>), transpose_grid(s),
-                                         dim3(256), 0, st, v, out, accumulate));
+  LOSS_TYPES(s.dtype, (transpose<T, false>(v, out, accumulate, st)));
   WGBM_LAUNCH_CHECK();
   return 0;
 }
