@@ -381,6 +381,52 @@ def test_policy_extreme_rows(gpu):
         assert loss[6] == 0 and lp[6] == 0 and (g[6] == 0).all()
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("K", [3, 40, 700, 6000])
+def test_policy_against_a_reference_that_excludes_a_class(gpu, K):
+    """The divergence is infinite then; it does no harm where it does not count,
+    nor does a class of probability 0 that the reference allows."""
+    from warpgbm_amd import losses
+
+    g = torch.Generator().manual_seed(K)
+    for order in ("row", "class"):
+        s = torch.randn((4, K), generator=g)
+        r = s + 0.1
+        r[0, 1] = -math.inf
+        s[1, 2] = -math.inf
+        a = torch.zeros(4, dtype=torch.int32)
+        old, adv = torch.full((4,), -2.0), torch.ones(4)
+        put = (lambda t: t.cuda()) if order == "row" else (lambda t: t.t().contiguous().cuda().t())
+        plain = losses.policy_loss(put(s), a.cuda(), old.cuda(), adv.cuda())
+        zero = losses.policy_loss(put(s), a.cuda(), old.cuda(), adv.cuda(), ref_scores=put(r))
+        assert torch.equal(zero.loss, plain.loss)
+        assert torch.allclose(zero.grad, plain.grad, rtol=1e-5, atol=1e-7)
+        assert zero.kl[0] == math.inf and torch.isfinite(zero.kl[1:]).all()
+        some = losses.policy_loss(put(s), a.cuda(), old.cuda(), adv.cuda(), ref_scores=put(r),
+                                  kl_coef=0.5)
+        assert some.loss[0] == math.inf
+        assert torch.isfinite(some.loss[1:]).all() and torch.isfinite(some.grad[1:]).all()
+        far = losses.policy_loss(put(s), a.cuda(), old.cuda(), adv.cuda(), kl_coef=0.0,
+                                 ref_log_prob=torch.full((4,), math.inf).cuda())
+        assert torch.equal(far.loss, plain.loss) and (far.kl == math.inf).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("order", ["row", "class"])
+def test_very_long_rows(gpu, order):
+    """Rows past every frame: ranges, joined."""
+    for dtype, n, K in (("f32", 3, 300_001), ("bf16", 2, 140_003), ("f16", 70, 131_080)):
+        for kl in ("sampled", "exact"):
+            print_case("long rows", order, dtype, n, K, kl)
+            d = policy_inputs(n, K, dtype, order, 61)
+            loss, lp, k, grad, live = policy_want(d, kl, (0.2, 0.2), 0.1)
+            scale = policy_scales(d, kl, 0.1, k, live)
+            r = run_policy(d, kl, (0.2, 0.2), 0.1)
+            check(r.log_prob, lp, norm_tol(lp), "log_prob")
+            check(r.loss, loss, STEPS * U * (scale + d["w"].to(F64)), "loss")
+            check(r.grad, grad, grad_tol(grad, scale, dtype), "gradient")
+
+
 # --------------------------------------------------------------------- balance
 def balance_want(s, mask, k, coef):
     live = live_rows(s)
@@ -585,6 +631,17 @@ def test_preference_left_out_and_extreme(gpu):
     assert g[3] == 0 and g[1] == 1.0 and g[2] == -1.0
     p = 1 / (1 + math.exp(1e-3))
     assert g[4].item() == pytest.approx(-p, rel=1e-6) and g[0].item() == pytest.approx(p, rel=1e-6)
+    # sequences that cannot be (log-probability -inf)
+    lp = torch.tensor([0.0, -math.inf, -1.0, -2.0])
+    for seg in (None, np.asarray([0, 1, 2, 3, 4])):
+        plan = losses.PreferencePlan(np.asarray([[0, 1], [2, 3]]), 4, segments=seg, device="cuda")
+        r = losses.preference_loss(lp.cuda(), plan)
+        assert r.margin.tolist() == [math.inf, 1.0] and r.loss[0] == 0.0
+        assert r.grad.tolist()[:2] == [0.0, 0.0] and r.grad[2] < 0
+        plan = losses.PreferencePlan(np.asarray([[1, 0], [2, 3]]), 4, segments=seg, device="cuda")
+        r = losses.preference_loss(lp.cuda(), plan)
+        assert r.loss[0] == math.inf and r.grad.tolist()[:2] == [1.0, -1.0]
+        assert r.margin[1] == 1.0
     for P, n, seg in ((0, 4, None), (0, 4, [0, 2, 4]), (0, 0, [0])):
         plan = losses.PreferencePlan(np.zeros((P, 2), np.int32), n, device="cuda",
                                      segments=np.asarray(seg) if seg is not None else None)

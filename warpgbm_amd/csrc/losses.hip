@@ -36,9 +36,17 @@ __device__ __forceinline__ RowStats scan_classes(const T* s, const T* r, int64_t
     }
     rebase_stats<REF>(a, m, mr);
     const Base b = base_of(safe_max(m)), br = base_of(safe_max(mr));
+    // (the eight's sums first: a shorter chain of additions, fewer roundings)
+    RowStats e = empty_stats();
 #pragma unroll
     for (int j = 0; j < U; ++j)
-      add_class<REF>(a, power_of(v[j], b), power_of(w[j], br), k + j * step == label);
+      add_class<REF>(e, power_of(v[j], b), power_of(w[j], br), k + j * step == label);
+    a.z += e.z;
+    a.za += e.za;
+    if (REF) {
+      a.zr += e.zr;
+      a.u += e.u;
+    }
   }
   return a;
 }
@@ -249,12 +257,14 @@ __global__ __launch_bounds__(256) void score_grad_kernel(ScoresView s, ScoresVie
 // host
 // ---------------------------------------------------------------------------
 // a row's classes in ranges: one range where the rows alone fill the GPU, else
-// ranges of at least 32 classes (row-major: 1024, a wave's 16 loads each)
+// ranges of at least 32 classes (row-major: 1024, a wave's 16 loads each); at
+// most 2048 classes a thread, which bounds the sums' rounding
 static int32_t loss_splits(int64_t n, int32_t K, bool cm) {
   const int64_t waves = std::max<int64_t>(1, cm ? (n + 63) / 64 : n);
   const int64_t want = (kLossWaves + waves - 1) / waves;
   const int64_t most = (K + (cm ? 31 : 1023)) / (cm ? 32 : 1024);
-  return (int32_t)std::max<int64_t>(1, std::min(want, most));
+  const int64_t least = cm ? (K + 2047) / 2048 : (K + 131071) / 131072;
+  return (int32_t)std::max<int64_t>(least, std::min(want, most));
 }
 
 static dim3 rows_grid(const ScoresView& s, int32_t splits) {

@@ -278,17 +278,23 @@ __device__ __forceinline__ PolicyRow policy_row(const RowStats& st, float sa, fl
     const double kl = (double)(st.u / z) + lr;
     o.kl = (float)(kLn2 * kl);
     base = (float)(lr - kl);  // (log2 p_k - log2 q_k - KL2) - (h_k - hr_k)
-    value += g.kl_coef * o.kl;
+    // (a divergence that does not count may be infinite)
+    if (g.kl_coef != 0.0f)
+      value += g.kl_coef * o.kl;
+    else
+      base = 0.0f;
     wk = w * g.kl_coef;
   } else if (g.ref_log_prob) {
     const float d = (float)((double)g.ref_log_prob[i] - logp);
     const float e = expm1f(d);
-    o.kl = e - d;
+    o.kl = d > 88.0f ? e : e - d;  // (no inf - inf)
     // near 0 the difference loses what the series keeps
     if (fabsf(d) < 0.03125f)
       o.kl = d * d * fmaf(d, fmaf(d, fmaf(d, 1.0f / 120.0f, 1.0f / 24.0f), 1.0f / 6.0f), 0.5f);
-    value += g.kl_coef * o.kl;
-    c -= g.kl_coef * e;
+    if (g.kl_coef != 0.0f) {
+      value += g.kl_coef * o.kl;
+      c -= g.kl_coef * e;
+    }
   }
   c *= w;
   o.loss = w * value;
@@ -296,7 +302,7 @@ __device__ __forceinline__ PolicyRow policy_row(const RowStats& st, float sa, fl
   o.c.c0 = (wn * base - c) * iz;
   o.c.c1 = wn * iz;
   o.c.gl = c * (st.z * iz);
-  if (REF && st.za != 0.0f)
+  if (REF && wn != 0.0f && st.za != 0.0f)
     o.c.gl += st.za * iz * wn * ((power_of(sa, o.c.b) - power_of(ra, o.c.br)) + base);
   return o;
 }
@@ -305,7 +311,7 @@ __device__ __forceinline__ PolicyRow policy_row(const RowStats& st, float sa, fl
 template <bool REF>
 __device__ __forceinline__ float coef_grad(const RowCoef& c, float s, float r) {
   const float h = power_of(s, c.b), e = exp2_f32(h);
-  if (!REF) return e * c.c0;
+  if (!REF || c.c1 == 0.0f) return e * c.c0;
   return e == 0.0f ? 0.0f : e * fmaf(c.c1, h - power_of(r, c.br), c.c0);
 }
 

@@ -97,7 +97,10 @@ __device__ __forceinline__ PairLoss pair_loss(const PreferenceArgs& a, double m,
   // difference of nearly equal numbers
   const float e = expf(-fabsf(z)), l = log1pf(e), inv = 1.0f / (1.0f + e);
   const float up = z >= 0.0f ? inv : e * inv, down = z >= 0.0f ? e * inv : inv;
-  o.loss = w * ((1.0f - a.smooth) * (l + fmaxf(-z, 0.0f)) + a.smooth * (l + fmaxf(z, 0.0f)));
+  o.loss = (1.0f - a.smooth) * (l + fmaxf(-z, 0.0f));
+  // (no 0 * inf where the preferred sequence alone is possible)
+  if (a.smooth != 0.0f) o.loss += a.smooth * (l + fmaxf(z, 0.0f));
+  o.loss *= w;
   o.slope = w * a.beta * (a.smooth * up - (1.0f - a.smooth) * down);
   return o;
 }
