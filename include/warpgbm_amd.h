@@ -236,8 +236,9 @@ int wgbm_importance_add(float* acc, int32_t n_feats, int32_t num_eras, const flo
  * only: results are the same in every run.  Gradients are rounded to the
  * scores' type once.  The calls allocate nothing and may be captured into a
  * HIP graph; `workspace` (device memory, 16-byte aligned, of the bytes that the
- * matching _workspace call returns, -1 for arguments it refuses) is written
- * before it is read and must not be shared by calls that may overlap.
+ * matching _workspace call returns: 0, none, for most, -1 for arguments it
+ * refuses) is written before it is read and must not be shared by calls that may
+ * overlap.
  * ------------------------------------------------------------------------ */
 #define WGBM_F32 0
 #define WGBM_BF16 1
