@@ -879,6 +879,31 @@ def test_refusals_without_a_gpu():
         losses.preference_loss(s[0], None)
 
 
+def test_strides_of_single_rows_and_classes():
+    """The strides of [n, K] scores: that of a dimension of one element does not
+    count, a repeated row or class is refused (the library would read past its
+    end)."""
+    from warpgbm_amd.losses import _strides
+
+    assert _strides(0, 4, 0, 0, "s") == (4, 1)
+    assert _strides(1, 1, 0, 7, "s") == (1, 1)
+    assert _strides(5, 1, 1, 9, "s") == (1, 1) and _strides(5, 1, 8, 0, "s") == (8, 1)
+    assert _strides(1, 4, 0, 1, "s") == (4, 1) and _strides(1, 4, 0, 3, "s") == (1, 3)
+    assert _strides(5, 4, 6, 1, "s") == (6, 1) and _strides(5, 4, 1, 5, "s") == (1, 5)
+    for n, K, rs, ks in ((5, 1, 0, 1), (5, 1, 0, 0), (1, 4, 4, 0), (5, 4, 3, 1), (5, 4, 1, 4),
+                         (5, 4, 0, 1), (5, 4, 1, 0), (5, 4, 8, 2)):
+        with pytest.raises(RuntimeError, match="next to each other"):
+            _strides(n, K, rs, ks, "s")
+
+
+def test_plan_without_a_gpu_is_not_evaluated():
+    from warpgbm_amd import losses
+
+    plan = losses.PreferencePlan(np.asarray([[0, 1]]), 2, device="cpu")
+    with pytest.raises(RuntimeError, match="on a GPU"):
+        losses.preference_loss(torch.zeros(2), plan)
+
+
 def test_plan_layout():
     """The tables of a plan (on the CPU): incidences grouped by sequence in pair
     order, tasks that cover every row once, in order, sequences in many pairs in
@@ -1034,6 +1059,7 @@ def test_refusals_on_the_gpu(gpu):
     no("next to each other", losses.class_log_probs, s.repeat(2, 2)[::2, ::2], a)
     no("next to each other", losses.class_log_probs, s[:, :1].expand(6, 4), a)
     no("next to each other", losses.class_log_probs, s[:1].expand(6, 4), a)
+    no("next to each other", losses.class_log_probs, s[:1, :1].expand(6, 1), a)
     no("at least one class", losses.class_log_probs, s[:, :0], a)
     no("2-D", losses.class_log_probs, s[0], a)
     no("norm", losses.class_log_probs_grad, s, a, f, f)

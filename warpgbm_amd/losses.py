@@ -18,7 +18,9 @@ results and gradients are 0, whatever their scores hold.
 Launches go on torch's current stream of the scores' device; nothing
 synchronises except the construction of a :class:`PreferencePlan`.  Outputs and
 working memory come from torch's allocator, so calls may be captured into a
-HIP graph.  Wrong types, shapes, devices or layouts raise ``RuntimeError``.
+HIP graph.  Nothing is recorded for autograd.  A gradient that is given to be
+added to must not share memory with an input.  Wrong types, shapes, devices or
+layouts raise ``RuntimeError``.
 """
 from __future__ import annotations
 
@@ -54,6 +56,24 @@ def _vector(t, name, dtype, n, device):
     return t.data_ptr()
 
 
+def _strides(n, K, rs, ks, name):
+    """The strides of [n, K] scores as the library takes them: that of a
+    dimension of one element says nothing and is replaced."""
+    given = (rs, ks)
+    if n == 0:
+        return K, 1
+    if K == 1:
+        ks = 1
+        if n == 1:
+            rs = 1
+    elif n == 1:
+        rs = K if ks == 1 else 1
+    if not ((ks == 1 and rs >= K) or (rs == 1 and ks >= n)):
+        raise RuntimeError(f"{name} must have the classes of a row or the rows of a class next to "
+                           f"each other (no overlap), got strides {given}")
+    return rs, ks
+
+
 def _matrix(t, name):
     """The C view of a [n, K] tensor of scores."""
     if not isinstance(t, torch.Tensor):
@@ -68,15 +88,7 @@ def _matrix(t, name):
     n, K = t.shape
     if K < 1:
         raise RuntimeError(f"{name} must have at least one class")
-    rs, ks = t.stride()
-    # the stride of a dimension of one element says nothing
-    if K == 1 or n == 0:
-        rs, ks = max(rs, K), 1
-    elif n == 1:
-        rs = K if ks == 1 else 1
-    if not ((ks == 1 and rs >= K) or (rs == 1 and ks >= n)):
-        raise RuntimeError(f"{name} must have the classes of a row or the rows of a class next to "
-                           f"each other (no overlap), got strides {tuple(t.stride())}")
+    rs, ks = _strides(n, K, *t.stride(), name)
     return _lib.Scores(t.data_ptr(), code, n, K, rs, ks)
 
 
@@ -255,6 +267,8 @@ def balance_loss(scores, *, top_k=1, mask=None, coef=1.0, grad=None,
     v = _matrix(scores, "scores")
     n, dev = scores.shape[0], scores.device
     K = scores.shape[1]
+    if not 1 <= top_k <= min(8, K):
+        raise RuntimeError(f"top_k must be in [1, min(8, n_classes)], got {top_k}")
     if mask is not None:
         mask = _vector(mask, "mask", torch.bool, n, dev)
     lib = _lib.load()
@@ -333,6 +347,8 @@ class PreferencePlan:
         degree = self._incidences(device)
         if seg is not None:
             self._tasks(seg, length, last, longest, degree, device)
+        if device.type == "cuda":  # the tables are whole for every stream that reads them
+            torch.cuda.current_stream(device).synchronize()
 
     # rows of a wave's task; pairs of a sequence from which on it is summed by
     # workgroups of its own, and the pairs of one of these
@@ -433,6 +449,8 @@ def preference_loss(log_prob, plan, *, ref_log_prob=None, weight=None, beta=1.0,
     weight: float32 [P], pairs of weight 0 are left out (margin 0)."""
     if not isinstance(plan, PreferencePlan):
         raise RuntimeError("plan must be a PreferencePlan")
+    if plan.device.type != "cuda":
+        raise RuntimeError(f"the plan must be on a GPU, got device {plan.device}")
     n, dev = plan.n_rows, plan.device
     f32 = torch.float32
     lp = _vector(log_prob, "log_prob", f32, n, dev)
