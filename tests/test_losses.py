@@ -1086,3 +1086,64 @@ def test_refusals_on_the_gpu(gpu):
     b = losses.balance_loss(s[:0])
     assert b.loss.item() == 0 and not b.counts.any() and not b.prob.any()
     assert losses.class_log_probs(s[:0], a[:0]).norm.shape == (0, 2)
+
+
+@pytest.mark.gpu
+def test_more_threads_than_a_grid_counts(gpu):
+    """Rows of 64 threads each whose launch would have some 2^32 threads: the
+    last rows as in a call of their own, the first ones too."""
+    from warpgbm_amd import losses
+
+    n, K, m = 16_900_000, 257, 3000
+    s = torch.zeros((n, K), dtype=torch.bfloat16, device="cuda")
+    gen = torch.Generator(device="cuda").manual_seed(3)
+    parts = [slice(0, m), slice(n - 500_000, n - 500_000 + m), slice(n - m, n)]
+    for p in parts:
+        s[p] = torch.randn((m, K), generator=gen, device="cuda").to(torch.bfloat16)
+    a = torch.randint(0, K, (n,), generator=gen, device="cuda", dtype=torch.int32)
+    old = torch.full((n,), -5.5, device="cuda")
+    adv = torch.randn(n, generator=gen, device="cuda")
+    f = losses.class_log_probs(s, a)
+    g = losses.class_log_probs_grad(s, a, f.norm, adv)
+    want = []
+    for p in parts:
+        x = losses.class_log_probs(s[p], a[p])
+        assert torch.equal(f.log_prob[p], x.log_prob) and torch.equal(f.norm[p], x.norm)
+        assert torch.equal(g[p], losses.class_log_probs_grad(s[p], a[p], x.norm, adv[p]))
+        want.append(losses.policy_loss(s[p], a[p], old[p], adv[p], weight=adv[p].abs(),
+                                       ref_log_prob=old[p], kl_coef=0.1))
+    del f, g
+    r = losses.policy_loss(s, a, old, adv, weight=adv.abs(), ref_log_prob=old, kl_coef=0.1)
+    for p, x in zip(parts, want):
+        assert torch.equal(r.loss[p], x.loss) and torch.equal(r.log_prob[p], x.log_prob)
+        assert torch.equal(r.kl[p], x.kl) and torch.equal(r.grad[p], x.grad)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("twice", [False, True])
+def test_more_sequences_than_a_grid_counts(gpu, twice):
+    """A wave a sequence, more than 2^26 of them; with a pair's sequence in
+    another pair, the steps apart."""
+    from warpgbm_amd import losses
+
+    n = (1 << 26) + 5000
+    pairs = [[0, n - 2], [n - 1, 5]] + ([[0, n - 1]] if twice else [])
+    plan = losses.PreferencePlan(np.asarray(pairs), n,
+                                 segments=torch.arange(n + 1, device="cuda"))
+    assert plan.disjoint != twice
+    lp = torch.zeros(n, device="cuda")
+    lp[n - 1], lp[0], lp[n - 2] = 1.5, -0.5, 2.0
+    r = losses.preference_loss(lp, plan)
+    margin = [-2.5, 1.5] + ([-2.0] if twice else [])
+    assert r.margin.tolist() == margin
+    # -sigmoid(-margin), float32's expf, sum, reciprocal and product: 6 roundings
+    slope = [-1 / (1 + np.exp(v)) for v in margin]
+    want = {0: slope[0], n - 2: -slope[0], n - 1: slope[1], 5: -slope[1]}
+    if twice:
+        want[0] += slope[2]
+        want[n - 1] -= slope[2]
+    at = sorted(want)
+    got = r.grad[torch.tensor(at, device="cuda")].cpu().double().numpy()
+    assert np.abs(got - [want[i] for i in at]).max() <= 8 * 2.0 ** -24
+    r.grad[torch.tensor(at, device="cuda")] = 0
+    assert not r.grad.any()

@@ -36,7 +36,7 @@ __global__ void residual_regression_kernel(const float* __restrict__ y,
 }
 
 // gradients given: r = -g, a grid row per tree; partial[tree * gridDim.x +
-// block] = max |r|
+// block] = max |r|.  Bound by memory (8 bytes an element).
 __global__ void residual_gradient_kernel(const float* __restrict__ g /* [T][n] */, int64_t n,
                                          float* __restrict__ r /* [T][n] */,
                                          uint32_t* __restrict__ partial) {

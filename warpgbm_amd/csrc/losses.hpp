@@ -75,8 +75,8 @@ __device__ __forceinline__ T from_f32(float v) {
 // has its maximum 1/e): what a softmax's sums and gradients are rounded by
 // anyway.  The rounding of m2 is a factor that all classes of the row share and
 // that every quotient loses; row_log_prob takes it out of the sum's logarithm.
-// The losses are bound by instructions as much as by memory (a 16-bit score and
-// its gradient are 4 bytes, about 30 instructions at this GPU's rates).
+// (The losses of 16-bit scores are bound by instructions as much as by memory: the
+// 4 bytes of a score and its gradient pass while a lane issues some 30.)
 constexpr float kLog2e = 1.44269504088896340736f;
 constexpr double kLn2 = 0.693147180559945309417;
 // (m: finite.  A maximum near the type's ends, a row whose classes are all

