@@ -370,6 +370,9 @@ typedef struct wgbm_preference_args {
   const float* weight;              /* [n_pairs] or NULL (1) */
   float beta;
   float label_smoothing;            /* [0, 0.5] */
+  int32_t lanes;                    /* threads of a task, or of a pair where disjoint:
+                                       4, 8, 16, 32 or 64 (0: 64); results may differ in the
+                                       last bits of the float64 sums */
 } wgbm_preference_args;
 int64_t wgbm_preference_loss_workspace(const wgbm_preference_args* args);
 int wgbm_preference_loss(const wgbm_preference_args* args, float* loss, float* margin, float* grad,

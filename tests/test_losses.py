@@ -1031,6 +1031,8 @@ def test_c_entries_refuse_before_any_launch():
     refused(pref(label_smoothing=0.6), "label_smoothing")
     refused(pref(n_sequences=3), "every row is a sequence")
     refused(pref(n_pairs=1 << 30), "n_pairs")
+    refused(pref(lanes=5), "lanes")
+    refused(pref(lanes=128), "lanes")
     refused(pref(incidence=None), "gradient needs")
     refused(pref(sequence_start=one), "tasks")
     refused(pref(share=None), "gradient needs")

@@ -152,6 +152,7 @@ class PreferenceArgs(C.Structure):
         ("weight", _p),
         ("beta", _f32),
         ("label_smoothing", _f32),
+        ("lanes", _i32),
     ]
 
 

@@ -194,6 +194,7 @@ static PreferenceArgs preference_args(const wgbm_preference_args* a) {
   p.weight = a->weight;
   p.beta = a->beta;
   p.smooth = a->label_smoothing;
+  p.lanes = a->lanes ? a->lanes : 64;
   return p;
 }
 
@@ -203,17 +204,17 @@ static int check_preference(const wgbm_preference_args* a) {
   WGBM_REQUIRE(a->n_sequences >= 0 && a->n_sequences < (int64_t(1) << 30),
                "preference_loss: bad n_sequences");
   WGBM_REQUIRE(a->n_pairs >= 0 && a->n_pairs < (int64_t(1) << 30), "preference_loss: bad n_pairs");
-  WGBM_REQUIRE(a->n_shares >= 0 && a->n_shares < (int64_t(1) << 31) && a->n_tasks >= 0 && a->n_tasks < (int64_t(1) << 31) && a->n_pieces >= 0 &&
-                   a->n_pieces < (int64_t(1) << 31) && a->n_multi >= 0 &&
-                   a->n_multi < (int64_t(1) << 31) && a->n_idle >= 0 &&
-                   a->n_idle < (int64_t(1) << 31),
-               "preference_loss: bad table sizes");
+  for (const int64_t size : {a->n_shares, a->n_tasks, a->n_pieces, a->n_multi, a->n_idle})
+    WGBM_REQUIRE(size >= 0 && size < (int64_t(1) << 31), "preference_loss: bad table sizes");
   WGBM_REQUIRE(a->sequence_start || (a->n_sequences == a->n_rows && !a->disjoint),
                "preference_loss: without sequence_start every row is a sequence");
   WGBM_REQUIRE(std::isfinite(a->beta) && a->beta > 0.0f,
                "preference_loss: beta must be positive and finite");
   WGBM_REQUIRE(a->label_smoothing >= 0.0f && a->label_smoothing <= 0.5f,
                "preference_loss: label_smoothing must be in [0, 0.5]");
+  WGBM_REQUIRE(a->lanes == 0 || a->lanes == 4 || a->lanes == 8 || a->lanes == 16 ||
+                   a->lanes == 32 || a->lanes == 64,
+               "preference_loss: lanes must be 4, 8, 16, 32 or 64 (or 0)");
   return 0;
 }
 

@@ -114,6 +114,7 @@ struct PreferenceArgs {
   bool disjoint;
   const float* weight;
   float beta, smooth;
+  int32_t lanes;  // 4 .. 64
   float* loss;
   float* margin;
   float* grad;

@@ -173,15 +173,13 @@ __global__ __launch_bounds__(F::kMax) void policy_frame_kernel(ScoresView s, Sco
 }
 
 // ---------------------------------------------------------------------------
-// Many rows of up to 64 threads each: a workgroup takes B rows a thread group,
-// all loads in flight at once, and a thread a row works out what follows from
-// the row as a whole, which otherwise every wave spends on its one to sixteen
-// rows (the policy loss some 250 instructions, a row's own passes 20 a class and
-// thread).  A row at a time and four: log-probabilities of 300000 x 100 float32
-// 46 and 24 us, 100000 x 500 bfloat16 38 and 26, 1M x 10 float32 18 and 12; the
-// policy loss of 300000 x 100 float32 78 and 60, 1M x 10 38 and 35, but 60000 x
-// 1000 bfloat16 45 and 48 and 100000 x 200 float32 against a reference 64 and 78
-// (their rows hold more registers): those take a row at a time.
+// Log-probabilities of many rows of up to 64 threads each: a workgroup takes B
+// rows a thread group, all loads in flight at once, and a thread a row works out
+// what follows from the row as a whole.  A row at a time and several: 300000 x
+// 100 float32 30 and 22 us, 100000 x 500 bfloat16 28 and 24, 60000 x 1000 28 and
+// 25, 1M x 10 float32 19 and 13.  (The policy loss, whose registers hold the row
+// until its gradient is written, gains nothing: 300000 x 100 float32 44 either
+// way, x 30 21 a row at a time and 23.)
 // ---------------------------------------------------------------------------
 template <typename F, int B>
 __global__ __launch_bounds__(256) void log_probs_batch_kernel(ScoresView s,
@@ -216,93 +214,15 @@ __global__ __launch_bounds__(256) void log_probs_batch_kernel(ScoresView s,
   write_log_prob(a, sa, lab, i, log_prob, norm);
 }
 
-template <typename F, int B>
-__global__ __launch_bounds__(256) void policy_batch_kernel(ScoresView s, PolicyRows g,
-                                                           ScoresView out, bool accumulate) {
-  using T = typename F::T;
-  constexpr int R = F::kRows * B;
-  static_assert(R <= 256, "a thread a row");
-  __shared__ int32_t s_label[R];
-  __shared__ RowStats s_stats[R];
-  __shared__ RowCoef s_coef[R];
-  const F f(s);
-  const int64_t i = (int64_t)blockIdx.x * R + threadIdx.x;
-  const bool mine = (int)threadIdx.x < R && i < s.n;
-  typename F::Regs v[B];
-#pragma unroll
-  for (int b = 0; b < B; ++b) f.load(v[b], s, (int64_t)blockIdx.x * B + b);
-  const float w = !mine ? 0.0f : g.weight ? g.weight[i] : 1.0f;
-  const int32_t lab = mine ? row_label(g.action, i, s.K) : -1;
-  const bool live = w != 0.0f && lab >= 0;
-  float sa = 0.0f, A = 0.0f, old = 0.0f;
-  if (live) {
-    sa = score_at<T>(s, i, lab);
-    A = g.advantage[i];
-    old = g.old_log_prob[i];
-  }
-  if ((int)threadIdx.x < R) s_label[threadIdx.x] = lab;
-  __syncthreads();
-#pragma unroll
-  for (int b = 0; b < B; ++b) {
-    const int q = b * F::kRows + threadIdx.x / F::G;
-    f.trim(v[b]);
-    const RowStats a = frame_stats<F, false>(f, v[b], v[b], s_label[q], nullptr);
-    if (f.first_lane()) s_stats[q] = a;
-    f.hide(v[b]);
-  }
-  __syncthreads();
-  if ((int)(threadIdx.x & ~63u) < R) {  // (whole waves)
-    PolicyRow o{};
-    RowStats a = empty_stats();
-    if (live) {
-      a = s_stats[threadIdx.x];
-      a.za = exp2_f32(power_of(sa, base_of(safe_max(a.m))));
-      o = policy_row<false>(a, sa, 0.0f, A, old, w, g, i, lab, nullptr);
-    }
-    // rows next to a border, one after the other, each by the whole wave
-    unsigned long long todo = __ballot(o.near);
-    while (todo) {
-      const int src = __ffsll((unsigned long long)todo) - 1;
-      todo &= todo - 1;
-      const int64_t row = i - (int)(threadIdx.x & 63) + src;
-      const double e = wave_exact_logp((const T*)s.data + row * s.rs, s.ks, s.K,
-                                       __shfl(lab, src), __shfl(a.m, src));
-      if ((int)(threadIdx.x & 63) == src)
-        o = policy_row<false>(a, sa, 0.0f, A, old, w, g, i, lab, &e);
-    }
-    if (mine) {
-      g.loss[i] = o.loss;
-      g.log_prob[i] = o.logp;
-      if (g.kl) g.kl[i] = o.kl;
-    }
-    if ((int)threadIdx.x < R) s_coef[threadIdx.x] = o.c;
-  }
-  if (!out.data) return;
-  __syncthreads();
-#pragma unroll
-  for (int b = 0; b < B; ++b) {
-    const int q = b * F::kRows + threadIdx.x / F::G;
-    if ((int64_t)blockIdx.x * R + q >= s.n) continue;
-    const int64_t block = (int64_t)blockIdx.x * B + b;
-    const RowCoef c = s_coef[q];
-    if (!c.live) {
-      if (!accumulate) f.store_zero(out, block);
-      continue;
-    }
-    f.store_row(out, block, accumulate, c.label, c.gl,
-                [&](int j) { return coef_grad<false>(c, F::value(v[b], j), 0.0f); });
-  }
-}
-
-// rows of a thread group in the kernels above (1: a row at a time): four chunks
-// of a thread's registers
-template <typename F, bool POLICY, bool REF>
+// rows of a thread group in the kernel above (1: a row at a time): four chunks of
+// a thread's registers, or two rows of four
+template <typename F>
 constexpr int batch_rows() {
-  if constexpr (F::kLaneRows || REF) {
+  if constexpr (F::kLaneRows) {
     return 1;
   } else {
-    if (F::G > 64 || (POLICY && (F::NC > 1 || sizeof(typename F::T) != 4))) return 1;
-    return 4 / F::NC < F::G ? 4 / F::NC : F::G;
+    if (F::G > 64 || F::NC > 4) return 1;
+    return F::NC == 4 ? 2 : 4 / F::NC;
   }
 }
 // from 4 workgroups a CU on; with fewer the rows of a group would wait for one
@@ -314,9 +234,17 @@ static bool batch_pays(const ScoresView& s) {
 
 // ---------------------------------------------------------------------------
 // which frame a call takes: fn(frame tag, workgroups, threads) for the smallest
-// one that holds the rows (rows_fit)
+// one that holds the rows (rows_fit).  Row-major rows take two to eight chunks a
+// thread rather than one, so that a wave has more loads in flight and spends
+// what a row costs as a whole on more rows: with one chunk a thread the policy
+// loss of 300000 x 100 float32 takes 57 us instead of 43, of 100000 x 500
+// bfloat16 57 and 40, the log-probabilities' gradient 59 and 44, 47 and 38; 30000 x
+// 3000 bfloat16, eight chunks of a wave's threads instead of two of a
+// workgroup's, whose waves wait for one another: 95 and 65 (not the gradient
+// without sums: 66 and 68).  Up to eight chunks a thread each: log-probabilities'
+// gradient of 300000 x 30 float32 19 us, 20 with two.
 // ---------------------------------------------------------------------------
-template <typename T, bool REF, typename Fn>
+template <typename T, bool REF, bool SUMS, typename Fn>
 static void pick_row_frame(const ScoresView& s, Fn fn) {
   constexpr int VE = Chunk<T>::VE;
   const int64_t chunks = (s.K + VE - 1) / VE;
@@ -326,12 +254,15 @@ static void pick_row_frame(const ScoresView& s, Fn fn) {
   };
   if (chunks <= 4) return go(FrameTag<RowFrame<T, 4, 1>>());
   if (chunks <= 8) return go(FrameTag<RowFrame<T, 8, 1>>());
-  if (chunks <= 16) return go(FrameTag<RowFrame<T, 16, 1>>());
-  if (chunks <= 32) return go(FrameTag<RowFrame<T, 32, 1>>());
-  if (chunks <= 64) return go(FrameTag<RowFrame<T, 64, 1>>());
-  if (chunks <= 128) return go(FrameTag<RowFrame<T, 64, 2>>());
-  if (chunks <= 256) return go(FrameTag<RowFrame<T, 64, 4>>());
-  if (chunks <= 512) return go(FrameTag<RowFrame<T, 256, 2>>());
+  if (chunks <= 16) return go(FrameTag<RowFrame<T, 8, 2>>());
+  if (chunks <= 32) return go(FrameTag<RowFrame<T, 16, 2>>());
+  if (chunks <= 64) return go(FrameTag<RowFrame<T, 32, 2>>());
+  if (chunks <= 128) return go(FrameTag<RowFrame<T, 32, 4>>());
+  if (chunks <= 256) return go(FrameTag<RowFrame<T, 32, 8>>());
+  if constexpr (!SUMS) {
+    if (chunks <= 512) return go(FrameTag<RowFrame<T, 256, 2>>());
+  }
+  if (chunks <= 512) return go(FrameTag<RowFrame<T, 64, 8>>());
   if (chunks <= 1024) return go(FrameTag<RowFrame<T, 256, 4>>());
   if (chunks <= 2048) return go(FrameTag<RowFrame<T, 256, 8>>());
   if (REF || chunks <= 4096) return go(FrameTag<RowFrame<T, 1024, 4>>());
@@ -357,20 +288,20 @@ static void pick_class_frame(const ScoresView& s, Fn fn) {
   fn(FrameTag<ClassFrame<T, 32, true, true>>(), tiles, 64 * (int)((s.K + 31) / 32));
 }
 
-template <typename T, bool REF, typename Fn>
+template <typename T, bool REF, bool SUMS, typename Fn>
 static void pick_frame(const ScoresView& s, Fn fn) {
   if (s.class_major() || s.K < Chunk<T>::VE)
     pick_class_frame<T>(s, fn);
   else
-    pick_row_frame<T, REF>(s, fn);
+    pick_row_frame<T, REF, SUMS>(s, fn);
 }
 
 template <typename T>
 static int log_probs_frames(const ScoresView& s, const int32_t* label, float* log_prob,
                             float* norm, hipStream_t st) {
-  pick_frame<T, false>(s, [&](auto tag, int64_t blocks, int threads) {
+  pick_frame<T, false, true>(s, [&](auto tag, int64_t blocks, int threads) {
     using F = typename decltype(tag)::type;
-    constexpr int B = batch_rows<F, false, false>();
+    constexpr int B = batch_rows<F>();
     if constexpr (B > 1) {
       if (batch_pays<F, B>(s)) {
         hipLaunchKernelGGL((log_probs_batch_kernel<F, B>), dim3((unsigned)((blocks + B - 1) / B)),
@@ -389,7 +320,7 @@ template <typename T>
 static int log_probs_grad_frames(const ScoresView& s, const int32_t* label, const float* norm,
                                  const float* grad, const ScoresView& out, hipStream_t st) {
   const LogProbGrad<T> g{label, (const float2*)norm, grad};
-  pick_frame<T, false>(s, [&](auto tag, int64_t blocks, int threads) {
+  pick_frame<T, false, false>(s, [&](auto tag, int64_t blocks, int threads) {
     using F = typename decltype(tag)::type;
     hipLaunchKernelGGL((log_probs_grad_frame_kernel<F>), dim3((unsigned)blocks), dim3(threads), 0,
                        st, s, g, out);
@@ -401,16 +332,8 @@ static int log_probs_grad_frames(const ScoresView& s, const int32_t* label, cons
 template <typename T, bool REF>
 static int policy_frames(const ScoresView& s, const ScoresView& ref, const PolicyRows& g,
                          const ScoresView& out, bool accumulate, hipStream_t st) {
-  pick_frame<T, REF>(s, [&](auto tag, int64_t blocks, int threads) {
+  pick_frame<T, REF, true>(s, [&](auto tag, int64_t blocks, int threads) {
     using F = typename decltype(tag)::type;
-    constexpr int B = batch_rows<F, true, REF>();
-    if constexpr (B > 1) {
-      if (batch_pays<F, B>(s)) {
-        hipLaunchKernelGGL((policy_batch_kernel<F, B>), dim3((unsigned)((blocks + B - 1) / B)),
-                           dim3(threads), 0, st, s, g, out, accumulate);
-        return;
-      }
-    }
     hipLaunchKernelGGL((policy_frame_kernel<F, REF>), dim3((unsigned)blocks), dim3(threads), 0, st,
                        s, ref, g, out, accumulate);
   });

@@ -9,10 +9,10 @@
 // in the order of execution).
 //
 // Bound by memory: every row is read and written once.  The plan cuts sequences
-// into tasks of at most 4096 rows, a wave each.  Where every sequence is one
-// task and in at most one pair, one launch does everything: a wave sums a pair's
-// two sequences, and writes their gradients.  Otherwise: tasks' sums, (tasks
-// joined,) pairs, sequences' slopes, rows.
+// into tasks of at most 4096 rows, 4 to 64 lanes each (the plan's choice).  Where
+// every sequence is one task and in at most one pair, one launch does everything:
+// the lanes of a pair sum its two sequences, and write their gradients.
+// Otherwise: tasks' sums, (tasks joined,) pairs, sequences' slopes, rows.
 #include <algorithm>
 
 #include "losses_host.hpp"
@@ -32,10 +32,10 @@ __device__ __forceinline__ Rows4 load_rows(const float* p) {
   return r;
 }
 
-// sum of u over the rows [b, b + n), by the lanes of a wave (each its own part)
-template <int U>
+// sum of u over the rows [b, b + n), by L lanes (each its own part)
+template <int U, int L>
 __device__ __forceinline__ double lane_rows_sum(const PreferenceArgs& a, int64_t b, int n) {
-  const int lane = threadIdx.x & 63;
+  const int lane = threadIdx.x & (L - 1);
   const float* lp = a.log_prob + b;
   const float* ref = a.ref ? a.ref + b : nullptr;
   if (n < 4) {
@@ -45,17 +45,17 @@ __device__ __forceinline__ double lane_rows_sum(const PreferenceArgs& a, int64_t
   double x[U];
 #pragma unroll
   for (int j = 0; j < U; ++j) x[j] = 0.0;
-  for (int k0 = 4 * lane; k0 < n; k0 += 256 * U) {
+  for (int k0 = 4 * lane; k0 < n; k0 += 4 * L * U) {
     Rows4 l[U], r[U];
 #pragma unroll
     for (int j = 0; j < U; ++j) {
-      const int k = k0 + 256 * j, at = k < n - 4 ? k : n - 4;
+      const int k = k0 + 4 * L * j, at = k < n - 4 ? k : n - 4;
       l[j] = load_rows(lp + at);
       if (ref) r[j] = load_rows(ref + at);
     }
 #pragma unroll
     for (int j = 0; j < U; ++j) {
-      const int k = k0 + 256 * j, skip = k < n - 4 ? 0 : k - (n - 4);
+      const int k = k0 + 4 * L * j, skip = k < n - 4 ? 0 : k - (n - 4);
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const double u = (double)l[j].v[e] - (ref ? (double)r[j].v[e] : 0.0);
@@ -68,21 +68,24 @@ __device__ __forceinline__ double lane_rows_sum(const PreferenceArgs& a, int64_t
   for (int j = 1; j < U; ++j) s += x[j];
   return s;
 }
-// the number of a wave in a grid of 256-thread workgroups (a grid's threads are
-// counted in 32 bits along x: wave_blocks folds longer ones)
-__device__ __forceinline__ int64_t wave_number() {
-  return ((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * 4 + (threadIdx.x >> 6);
+// the number of a group of L lanes in a grid of 256-thread workgroups (a grid's
+// threads are counted in 32 bits along x: group_blocks folds longer ones)
+template <int L>
+__device__ __forceinline__ int64_t group_number() {
+  return ((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * (256 / L) + threadIdx.x / L;
 }
-__device__ __forceinline__ double wave_sum(double s) {
-  for (int o = 32; o; o >>= 1) s += __shfl_xor(s, o);
+template <int L>
+__device__ __forceinline__ double lanes_sum(double s) {
+  for (int o = L / 2; o; o >>= 1) s += __shfl_xor(s, o);
   return s;
 }
 
-// grad = g for the rows [b, b + n), by a wave
-__device__ __forceinline__ void wave_rows_fill(float* grad, int64_t b, int n, float g) {
+// grad = g for the rows [b, b + n), by L lanes
+template <int L>
+__device__ __forceinline__ void rows_fill(float* grad, int64_t b, int n, float g) {
   float* p = grad + b;
   const Rows4 v = {{g, g, g, g}};
-  for (int k = 4 * (threadIdx.x & 63); k < n; k += 256) {
+  for (int k = 4 * (threadIdx.x & (L - 1)); k < n; k += 4 * L) {
     if (n - k >= 4) {
       __builtin_memcpy(p + k, &v, 16);
     } else {
@@ -111,19 +114,19 @@ __device__ __forceinline__ PairLoss pair_loss(const PreferenceArgs& a, double m,
 }
 
 // ---------------------------------------------------------------------------
-// everything in one launch: a wave per pair, then a wave per idle task (rows
-// of sequences without a pair, and rows behind the last sequence).  50000 pairs
-// of sequences of 200 rows on average, all with reference: 55 us, 4.4 TB/s (a
+// everything in one launch: L lanes a pair, then as many an idle task (rows of
+// sequences without a pair, and rows behind the last sequence).  50000 pairs
+// of sequences of 200 rows on average, all with reference: 53 us, 4.5 TB/s (a
 // copy of as many bytes 47); with a row a lane and load instead of four 63.
 // ---------------------------------------------------------------------------
+template <int L>
 __global__ __launch_bounds__(256) void preference_fused_kernel(PreferenceArgs a) {
-  const int64_t t = wave_number();
-  const int lane = threadIdx.x & 63;
+  const int64_t t = group_number<L>();
   if (t >= a.n_pairs) {
     const int64_t k = t - a.n_pairs;
     if (a.grad && k < a.n_idle) {
       const int64_t b = a.idle[2 * k], e = a.idle[2 * k + 1];
-      wave_rows_fill(a.grad, b, (int)(e - b), 0.0f);
+      rows_fill<L>(a.grad, b, (int)(e - b), 0.0f);
     }
     return;
   }
@@ -133,37 +136,40 @@ __global__ __launch_bounds__(256) void preference_fused_kernel(PreferenceArgs a)
   const float w = a.weight ? a.weight[t] : 1.0f;
   PairLoss o{0.0f, 0.0f, 0.0f};
   if (w != 0.0f) {
-    const double x = lane_rows_sum<2>(a, b0, n0), y = lane_rows_sum<2>(a, b1, n1);
-    o = pair_loss(a, wave_sum(x - y), w);
+    const double x = lane_rows_sum<2, L>(a, b0, n0), y = lane_rows_sum<2, L>(a, b1, n1);
+    o = pair_loss(a, lanes_sum<L>(x - y), w);
   }
-  if (lane == 0) {
+  if ((threadIdx.x & (L - 1)) == 0) {
     a.loss[t] = o.loss;
     a.margin[t] = o.margin;
   }
   if (!a.grad) return;
-  wave_rows_fill(a.grad, b0, n0, o.slope);
-  wave_rows_fill(a.grad, b1, n1, -o.slope);
+  rows_fill<L>(a.grad, b0, n0, o.slope);
+  rows_fill<L>(a.grad, b1, n1, -o.slope);
 }
 
 // ---------------------------------------------------------------------------
 // the steps apart
 // ---------------------------------------------------------------------------
 // part[t]: a task's sum (tasks of rows behind the last sequence: none).  20001
-// sequences of 25 rows 12 us: short ones are bound by the latency of their table,
-// then their rows; 100 sequences of 200000 rows with reference 4 TB/s.
+// sequences of 25 rows 5 us (12 with a wave each): short ones are bound by the
+// latency of their table, then their rows; 100 sequences of 200000 rows with
+// reference 4 TB/s.
+template <int L>
 __global__ __launch_bounds__(256) void task_sums_kernel(PreferenceArgs a, double* __restrict__ part) {
-  const int64_t t = wave_number();
-  if (t >= a.n_tasks || a.task[3 * t] < 0) return;
-  const int64_t b = a.task[3 * t + 1];
-  const double x = wave_sum(lane_rows_sum<4>(a, b, (int)(a.task[3 * t + 2] - b)));
-  if ((threadIdx.x & 63) == 0) part[t] = x;
+  const int64_t t = group_number<L>();
+  if (t >= a.n_tasks) return;
+  const int64_t s = a.task[3 * t], b = a.task[3 * t + 1], e = a.task[3 * t + 2];
+  if (s < 0) return;
+  const double x = lanes_sum<L>(lane_rows_sum<L < 64 ? 2 : 4, L>(a, b, (int)(e - b)));
+  if ((threadIdx.x & (L - 1)) == 0) part[t] = x;
 }
 
 // U[s]: a sequence's tasks joined, a wave each
 __global__ __launch_bounds__(256) void join_tasks_kernel(PreferenceArgs a,
                                                          const double* __restrict__ part,
                                                          double* __restrict__ U) {
-  const int64_t s = wave_number();
+  const int64_t s = group_number<64>();
   if (s >= a.n_seg) return;
   double x = 0.0;
   const int64_t t1 = a.task_start[s + 1];
@@ -268,14 +274,14 @@ __global__ __launch_bounds__(64) void seq_pieces_kernel(PreferenceArgs a,
   if (threadIdx.x == 0) out[a.multi[3 * k]] = (float)x;
 }
 
-// rows take their sequence's slope, a wave a task
+// rows take their sequence's slope, L lanes a task
+template <int L>
 __global__ __launch_bounds__(256) void task_rows_kernel(PreferenceArgs a,
                                                         const float* __restrict__ seq) {
-  const int64_t t = wave_number();
+  const int64_t t = group_number<L>();
   if (t >= a.n_tasks) return;
-  const int64_t s = a.task[3 * t];
-  const int64_t b = a.task[3 * t + 1];
-  wave_rows_fill(a.grad, b, (int)(a.task[3 * t + 2] - b), s >= 0 ? seq[s] : 0.0f);
+  const int64_t s = a.task[3 * t], b = a.task[3 * t + 1], e = a.task[3 * t + 2];
+  rows_fill<L>(a.grad, b, (int)(e - b), s >= 0 ? seq[s] : 0.0f);
 }
 
 // ---------------------------------------------------------------------------
@@ -310,26 +316,30 @@ static PrefWs pref_ws(const PreferenceArgs& a, void* base) {
 }
 size_t preference_workspace(const PreferenceArgs& a) { return pref_ws(a, nullptr).bytes; }
 
-static dim3 wave_blocks(int64_t waves) {
-  const int64_t n = (waves + 3) / 4, x = std::min(n, int64_t(1) << 23);
-  return dim3((unsigned)x, (unsigned)((n + x - 1) / x));
+// workgroups of n groups of L lanes
+template <int L>
+static dim3 group_blocks(int64_t n) {
+  const int64_t b = (n + 256 / L - 1) / (256 / L), x = std::min(b, int64_t(1) << 23);
+  return dim3((unsigned)x, (unsigned)((b + x - 1) / x));
 }
 
-int preference_loss(const PreferenceArgs& a, void* base, hipStream_t st) {
+// L: lanes of a task or pair
+template <int L>
+static int preference_lanes(const PreferenceArgs& a, void* base, hipStream_t st) {
   const dim3 wg(256);
   if (a.disjoint) {
-    const int64_t waves = a.n_pairs + (a.grad ? a.n_idle : 0);
-    if (!waves) return 0;
-    hipLaunchKernelGGL(preference_fused_kernel, wave_blocks(waves), wg, 0, st, a);
+    const int64_t n = a.n_pairs + (a.grad ? a.n_idle : 0);
+    if (!n) return 0;
+    hipLaunchKernelGGL(preference_fused_kernel<L>, group_blocks<L>(n), wg, 0, st, a);
     WGBM_LAUNCH_CHECK();
     return 0;
   }
   const PrefWs w = pref_ws(a, base);
   if (a.seg_start && a.n_pairs) {
-    hipLaunchKernelGGL(task_sums_kernel, wave_blocks(a.n_tasks), wg, 0, st, a, w.part);
+    hipLaunchKernelGGL(task_sums_kernel<L>, group_blocks<L>(a.n_tasks), wg, 0, st, a, w.part);
     WGBM_LAUNCH_CHECK();
     if (a.task_start) {
-      hipLaunchKernelGGL(join_tasks_kernel, wave_blocks(a.n_seg), wg, 0, st, a, w.part, w.U);
+      hipLaunchKernelGGL(join_tasks_kernel, group_blocks<64>(a.n_seg), wg, 0, st, a, w.part, w.U);
       WGBM_LAUNCH_CHECK();
     }
   }
@@ -351,10 +361,20 @@ int preference_loss(const PreferenceArgs& a, void* base, hipStream_t st) {
     WGBM_LAUNCH_CHECK();
   }
   if (a.seg_start && a.n_tasks) {
-    hipLaunchKernelGGL(task_rows_kernel, wave_blocks(a.n_tasks), wg, 0, st, a, seq);
+    hipLaunchKernelGGL(task_rows_kernel<L>, group_blocks<L>(a.n_tasks), wg, 0, st, a, seq);
     WGBM_LAUNCH_CHECK();
   }
   return 0;
+}
+
+int preference_loss(const PreferenceArgs& a, void* base, hipStream_t st) {
+  switch (a.lanes) {
+    case 4: return preference_lanes<4>(a, base, st);
+    case 8: return preference_lanes<8>(a, base, st);
+    case 16: return preference_lanes<16>(a, base, st);
+    case 32: return preference_lanes<32>(a, base, st);
+    default: return preference_lanes<64>(a, base, st);
+  }
 }
 
 }  // namespace wgbm

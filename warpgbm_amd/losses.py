@@ -344,6 +344,7 @@ class PreferencePlan:
         self.task = self.task_start = self.piece = self.multi = self.idle = None
         self.disjoint = False
         self.workspace_bytes = None
+        self.lanes = 0
         degree = self._incidences(device)
         if seg is not None:
             self._tasks(seg, length, last, longest, degree, device)
@@ -407,9 +408,12 @@ class PreferencePlan:
         """The rows of every sequence, and those behind the last one, in tasks of
         a wave."""
         S, n = self.n_sequences, self.n_rows
+        self.lanes = self._lanes(last / max(S, 1), min(longest, self._TASK))
         tail = None
         if last < n:
-            tail = self._cut(seg[-1:], torch.full_like(seg[-1:], n), self._TASK)[0]
+            # (no longer than the sequences' tasks: they have as many threads)
+            size = min(self._TASK, max(longest, 64))
+            tail = self._cut(seg[-1:], torch.full_like(seg[-1:], n), size)[0]
             tail[:, 0] = -1
         if longest > self._TASK:
             task, self.task_start = self._cut(seg[:-1], seg[1:], self._TASK)
@@ -423,6 +427,22 @@ class PreferencePlan:
         self.task = (task if tail is None else torch.cat([task, tail])).contiguous()
         if self.disjoint:
             self.idle, self.task = self.task[:, 1:].contiguous(), None
+
+    @staticmethod
+    def _lanes(mean, longest):
+        """Threads of a task or pair: a row is read by four to a thread, and a wave
+        of 64 for sequences of 20 rows leaves most of it idle.  Measured, us, with
+        64, 32, 16, 8 and 4 threads: 50000 pairs of 200 rows 55, 54, 63, 80; of 100
+        rows 44, 34, 36, 46; of 50 rows, 100000 pairs, 74, 47, 39, 44; of 20 rows,
+        250000 pairs, 159, 96, 63, 59, 65; 1M sequences of 5 rows in 1M pairs 503, 278,
+        174, 115, 86.
+        A sequence much longer than the mean must not keep its threads busy alone
+        for more than some 16 turns."""
+        lanes = 4 if mean <= 10 else 8 if mean <= 32 else 16 if mean <= 64 else \
+            32 if mean <= 256 else 64
+        while lanes < 64 and longest > 128 * lanes:
+            lanes *= 2
+        return lanes
 
     @staticmethod
     def _whole_numbers(a, name):
@@ -465,7 +485,7 @@ def preference_loss(log_prob, plan, *, ref_log_prob=None, weight=None, beta=1.0,
         plan.is_long.data_ptr() if plan.is_long is not None else None,
         *_table(plan.task), plan.task_start.data_ptr() if plan.task_start is not None else None,
         *_table(plan.piece), *_table(plan.multi), *_table(plan.idle), int(plan.disjoint), w,
-        float(beta), float(label_smoothing))
+        float(beta), float(label_smoothing), plan.lanes)
     lib = _lib.load()
     with _on(dev):
         loss = torch.empty(P, dtype=f32, device=dev)
