@@ -332,7 +332,7 @@ int wgbm_balance_loss(const wgbm_scores* scores, const uint8_t* mask, int32_t to
  *  incidence_start [n_sequences + 1]: each sequence's range of them, empty for
  *    the long ones;
  *  share [n_shares + 1]: sequence numbers that cut the sequences into runs with
- *    at most 1024 sequences and 1280 of the incidences of incidence_start;
+ *    at most 256 sequences and 512 of the incidences of incidence_start;
  *  is_long [n_sequences]: 1 for the long ones (NULL: none);
  *  piece [n_pieces][3]: (sequence, or -1 where it has several pieces; first and
  *    end incidence) of the long sequences; multi [n_multi][3]: (sequence, first

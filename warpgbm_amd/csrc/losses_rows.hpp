@@ -75,8 +75,8 @@ __global__ __launch_bounds__(F::kMax) void log_probs_frame_kernel(
 }
 
 // its gradient, g (1[k = a] - p_k): no reduction, the norm is given.  4099 x 32000
-// bfloat16 95 us (525 MB, 5.5 TB/s); 20047 x 257 float16 10.5, bound by latency:
-// rows are short and wait for their label and norm; 500000 x 32 float32 33.
+// bfloat16 95 us (525 MB, 5.5 TB/s); 20047 x 257 float16 8, bound by latency: rows
+// are short and wait for their label and norm; 500000 x 32 float32 class-major 33.
 template <typename F>
 __global__ __launch_bounds__(F::kMax) void log_probs_grad_frame_kernel(
     ScoresView s, LogProbGrad<typename F::T> g, ScoresView out) {

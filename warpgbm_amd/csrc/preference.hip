@@ -213,7 +213,7 @@ __device__ __forceinline__ float signed_slope(const PreferenceArgs& a, const flo
 // one are consecutive, fit LDS, and are gathered with all lanes busy, however
 // few or many a sequence has.  1M sequences, 2M pairs: 45 us, 4M gathers of a
 // slope from another line each.
-constexpr int kIncTile = 1536;  // 1024 + the pairs of one sequence (256)
+constexpr int kIncTile = 512;  // 256 + the pairs of one sequence (256)
 __global__ __launch_bounds__(256) void seq_slopes_kernel(PreferenceArgs a,
                                                          const float* __restrict__ slope,
                                                          double* __restrict__ piece_sum,
@@ -253,13 +253,12 @@ __global__ __launch_bounds__(256) void seq_slopes_kernel(PreferenceArgs a,
 #pragma unroll
   for (int k = 0; k < kIncTile / 256; ++k) tile[threadIdx.x + 256 * k] = d[k];
   __syncthreads();
-  for (int64_t s = s0 + threadIdx.x; s < s1; s += 256) {
-    if (a.is_long && a.is_long[s]) continue;
-    const int lo = (int)(a.inc_start[s] - r0), hi = (int)(a.inc_start[s + 1] - r0);
-    double x = 0.0;
-    for (int j = lo; j < hi; ++j) x += (double)tile[j];
-    out[s] = (float)x;
-  }
+  const int64_t s = s0 + threadIdx.x;
+  if (s >= s1 || (a.is_long && a.is_long[s])) return;
+  const int lo = (int)(a.inc_start[s] - r0), hi = (int)(a.inc_start[s + 1] - r0);
+  double x = 0.0;
+  for (int j = lo; j < hi; ++j) x += (double)tile[j];
+  out[s] = (float)x;
 }
 
 // the sequences of several pieces, a wave each

@@ -351,11 +351,11 @@ class PreferencePlan:
         if device.type == "cuda":  # the tables are whole for every stream that reads them
             torch.cuda.current_stream(device).synchronize()
 
-    # rows of a wave's task; pairs of a sequence from which on it is summed by
+    # most rows of a task; pairs of a sequence from which on it is summed by
     # workgroups of its own, and the pairs of one of these
     _TASK, _LONG, _PIECE = 4096, 256, 8192
     # sequences and pairs' sides, together, of a workgroup that sums the others
-    _SHARE = 1024
+    _SHARE = 256
 
     @staticmethod
     def _cut(first, end, size):
@@ -405,8 +405,8 @@ class PreferencePlan:
         return most
 
     def _tasks(self, seg, length, last, longest, most, device):
-        """The rows of every sequence, and those behind the last one, in tasks of
-        a wave."""
+        """The rows of every sequence, and those behind the last one, in tasks
+        of :meth:`_lanes` threads."""
         S, n = self.n_sequences, self.n_rows
         self.lanes = self._lanes(last / max(S, 1), min(longest, self._TASK))
         tail = None
@@ -439,7 +439,7 @@ class PreferencePlan:
         A sequence much longer than the mean must not keep its threads busy alone
         for more than some 16 turns."""
         lanes = 4 if mean <= 10 else 8 if mean <= 32 else 16 if mean <= 64 else \
-            32 if mean <= 256 else 64
+            32 if mean <= 128 else 64
         while lanes < 64 and longest > 128 * lanes:
             lanes *= 2
         return lanes
