@@ -11,7 +11,7 @@ namespace wgbm {
 constexpr int kFinClasses = 4;
 
 // shares f_k, means P_k, counts, the loss and the gradient's scale (some 1000
-// partial sums a class: 8 us for 100 classes, a launch's latency for few).  The
+// partial sums a class: 7 us for 100 classes, a launch's latency for few).  The
 // workgroups' shares of the loss are joined by the last one to arrive, in
 // workgroup order.
 __global__ __launch_bounds__(256) void balance_finish_kernel(BalanceWs w, int32_t groups,

@@ -9,9 +9,9 @@
 // and leave one partial sum a class, which the finishing launch joins in
 // float64 in workgroup order: results do not depend on the order of execution.
 //
-// 1M x 100 float32 class-major: the first pass 140 us (3 TB/s; the seven waves
-// that share 64 rows wait for one another at three reductions, and for one more
-// where a row's best class is counted), the finish 8, the gradient 183 (4.4 TB/s).
+// 1M x 100 float32 class-major: the first pass 131 us (3.1 TB/s; the eight waves
+// that share 64 rows wait for one another at three reductions), the finish 7, the
+// gradient 182 (4.4 TB/s).
 // 65536 x 64 bfloat16, two choices: 10, 5 and 5.
 #pragma once
 #include <algorithm>
@@ -196,7 +196,7 @@ __global__ __launch_bounds__(F::kMax) void balance_grad_kernel(
 // x 256 bfloat16 27 with one, 30 with two.
 template <typename T, typename Fn>
 static void balance_frame(const ScoresView& s, Fn fn) {
-  const int64_t rows = (s.n + 255) / 256, tiles = (s.n + 63) / 64;
+  const int64_t rows = (s.n + 255) / 256;
   if (!s.class_major() && s.K < Chunk<T>::VE) {
     if (s.K <= 4) return fn(FrameTag<ClassFrame<T, 4, false, false>>(), rows, 256);
     return fn(FrameTag<ClassFrame<T, 8, false, false>>(), rows, 256);
@@ -206,9 +206,7 @@ static void balance_frame(const ScoresView& s, Fn fn) {
     if (s.K <= 8) return fn(FrameTag<ClassFrame<T, 8, false, true>>(), rows, 256);
     if (s.K <= 12) return fn(FrameTag<ClassFrame<T, 12, false, true>>(), rows, 256);
     if (s.K <= 16) return fn(FrameTag<ClassFrame<T, 16, false, true>>(), rows, 256);
-    if (s.K <= 256)
-      return fn(FrameTag<ClassFrame<T, 16, true, true>>(), tiles, 64 * (int)((s.K + 15) / 16));
-    return fn(FrameTag<ClassFrame<T, 32, true, true>>(), tiles, 64 * (int)((s.K + 31) / 32));
+    return pick_slices<T>(s, fn);
   }
   const int64_t chunks = (s.K + Chunk<T>::VE - 1) / Chunk<T>::VE;
   const auto go = [&](auto tag) {
@@ -234,7 +232,7 @@ static void balance_frame(const ScoresView& s, Fn fn) {
 // workgroups of the two passes: 16 waves a CU (with 64, the class-major 1M x 10
 // takes 45 us instead of 37 and a gate's 65536 x 64 32 instead of 26: more
 // partial sums), but 64 where the waves of a workgroup wait for one another
-// (1M x 100 class-major 359 us with 16, 331 with 64; 200000 x 400 721, 603); and
+// (200000 x 400 class-major 721 us with 16, 603 with 64); and
 // fewer partial sums where there are many classes
 template <typename F>
 static int64_t balance_fill(int threads) {

@@ -511,4 +511,22 @@ struct ClassFrame {
   }
 };
 
+// which slices class-major rows of 17 to 512 classes take: fn(frame tag,
+// workgroups, threads).  4, 8, 12 or 16 waves, which fill the SIMDs evenly, of as
+// few classes each as hold the row.  1M x 100 float32, 8 waves of 13 classes, 10 of 10,
+// 7 of 16, 13 of 8: balance loss 319, 325, 330, 349 us; policy loss of 500000 x 100
+// 94, 125, 108, 158; of 1M x 30, 4 waves of 8, 3 of 10, 3 of 13, 2 of 16: 65, 66,
+// 70, 75; of 160000 x 150, 12 of 13, 16 of 10, 10 of 16: 58, 68, 61.
+template <typename T, typename Fn>
+static void pick_slices(const ScoresView& s, Fn fn) {
+  const int64_t tiles = (s.n + 63) / 64;
+  if (s.K > 256)
+    return fn(FrameTag<ClassFrame<T, 32, true, true>>(), tiles, 64 * (int)((s.K + 31) / 32));
+  const int S = s.K <= 64 ? 4 : s.K <= 128 ? 8 : s.K <= 192 ? 12 : 16;
+  if (s.K <= 8 * S) return fn(FrameTag<ClassFrame<T, 8, true, true>>(), tiles, 64 * S);
+  if (s.K <= 10 * S) return fn(FrameTag<ClassFrame<T, 10, true, true>>(), tiles, 64 * S);
+  if (s.K <= 13 * S) return fn(FrameTag<ClassFrame<T, 13, true, true>>(), tiles, 64 * S);
+  fn(FrameTag<ClassFrame<T, 16, true, true>>(), tiles, 64 * S);
+}
+
 }  // namespace wgbm

@@ -76,7 +76,7 @@ __global__ __launch_bounds__(F::kMax) void log_probs_frame_kernel(
 
 // its gradient, g (1[k = a] - p_k): no reduction, the norm is given.  4099 x 32000
 // bfloat16 95 us (525 MB, 5.5 TB/s); 20047 x 257 float16 8, bound by latency: rows
-// are short and wait for their label and norm; 500000 x 32 float32 class-major 33.
+// are short and wait for their label and norm; 500000 x 32 float32 class-major 32.
 template <typename F>
 __global__ __launch_bounds__(F::kMax) void log_probs_grad_frame_kernel(
     ScoresView s, LogProbGrad<typename F::T> g, ScoresView out) {
@@ -274,7 +274,7 @@ static void pick_row_frame(const ScoresView& s, Fn fn) {
 
 template <typename T, typename Fn>
 static void pick_class_frame(const ScoresView& s, Fn fn) {
-  const int64_t blocks = (s.n + 255) / 256, tiles = (s.n + 63) / 64;
+  const int64_t blocks = (s.n + 255) / 256;
   if (!s.class_major()) {  // rows shorter than a chunk
     if (s.K <= 4) return fn(FrameTag<ClassFrame<T, 4, false, false>>(), blocks, 256);
     return fn(FrameTag<ClassFrame<T, 8, false, false>>(), blocks, 256);
@@ -283,9 +283,7 @@ static void pick_class_frame(const ScoresView& s, Fn fn) {
   if (s.K <= 8) return fn(FrameTag<ClassFrame<T, 8, false, true>>(), blocks, 256);
   if (s.K <= 12) return fn(FrameTag<ClassFrame<T, 12, false, true>>(), blocks, 256);
   if (s.K <= 16) return fn(FrameTag<ClassFrame<T, 16, false, true>>(), blocks, 256);
-  if (s.K <= 256)
-    return fn(FrameTag<ClassFrame<T, 16, true, true>>(), tiles, 64 * (int)((s.K + 15) / 16));
-  fn(FrameTag<ClassFrame<T, 32, true, true>>(), tiles, 64 * (int)((s.K + 31) / 32));
+  pick_slices<T>(s, fn);
 }
 
 template <typename T, bool REF, bool SUMS, typename Fn>
