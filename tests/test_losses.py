@@ -1149,3 +1149,42 @@ def test_more_sequences_than_a_grid_counts(gpu, twice):
     assert np.abs(got - [want[i] for i in at]).max() <= 8 * 2.0 ** -24
     r.grad[torch.tensor(at, device="cuda")] = 0
     assert not r.grad.any()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["pairs", "mixed"])
+@pytest.mark.parametrize("lanes", [0, 4, 8, 16, 32, 64])
+def test_threads_of_a_sequence(gpu, kind, lanes):
+    """Sequences of 0 to 700 rows and rows behind the last one, by as many threads
+    as a plan may choose; one pair a sequence, or several."""
+    from warpgbm_amd import losses
+
+    g = torch.Generator().manual_seed(31)
+    S = 120
+    length = torch.randint(0, 12, (S,), generator=g)
+    length[7], length[50], length[119] = 700, 257, 64
+    seg = torch.cat([torch.zeros(1, dtype=torch.int64), length.cumsum(0)])
+    n = int(seg[-1]) + 333
+    if kind == "pairs":
+        pairs = torch.randperm(S, generator=g)[:80].reshape(-1, 2)
+    else:
+        pairs = torch.randint(0, S, (200, 2), generator=g)
+    lp, ref = -torch.rand(n, generator=g), -torch.rand(n, generator=g)
+    plan = losses.PreferencePlan(pairs, n, segments=seg, device="cuda")
+    assert plan.disjoint == (kind == "pairs")
+    plan.lanes = lanes
+    r = losses.preference_loss(lp.cuda(), plan, ref_log_prob=ref.cuda(), beta=0.5,
+                               label_smoothing=0.1)
+    x = lp.to(F64).requires_grad_()
+    loss, margin = preference64(x, pairs, S, seg, ref, None, 0.5, 0.1)
+    loss.sum().backward()
+    # sums in float64; the margin, its product with beta, and the few operations
+    # of a loss or slope round to float32: 2^-24 of each, eight at most
+    # relative to 1 + |margin|; a gradient adds its pairs' slopes (at most 0.5)
+    scale = 1 + margin.detach().abs()
+    assert ((r.margin.cpu() - margin.detach()).abs() <= 2 ** -24 * scale).all()
+    assert ((r.loss.cpu() - loss.detach()).abs() <= 8 * 2 ** -24 * scale).all()
+    many = torch.bincount(pairs.reshape(-1), minlength=S).max()
+    tol = float(many) * 0.5 * 8 * 2 ** -24 * float(scale.max())
+    assert (r.grad.cpu() - x.grad).abs().max() <= tol
+    assert not r.grad[int(seg[-1]):].any()
