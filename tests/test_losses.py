@@ -6,6 +6,7 @@ of each float32 step, half a step of the gradient's type (torch.finfo(t).eps /
 2 of the value, and half of float16's smallest subnormal number).
 """
 import math
+import sys
 
 import numpy as np
 import pytest
@@ -1188,3 +1189,32 @@ def test_threads_of_a_sequence(gpu, kind, lanes):
     tol = float(many) * 0.5 * 8 * 2 ** -24 * float(scale.max())
     assert (r.grad.cpu() - x.grad).abs().max() <= tol
     assert not r.grad[int(seg[-1]):].any()
+
+
+# classes at which rows take another number of threads, chunks or slices
+EDGES = [(70, K) for K in (16, 17, 32, 33, 36, 40, 41, 52, 53, 64, 65, 80, 81, 104, 105, 128, 129,
+                           156, 157, 192, 193, 208, 209, 256, 257)] + \
+        [(11, K) for K in (511, 512, 513, 1024, 1025, 2047, 2048, 2049, 4095, 4096, 4097)]
+# rows enough for the balance loss to take two chunks a thread
+BALANCE_ROWS = [(44_000, 49), (42_003, 99), (21_001, 201), (11_000, 403), (1_500, 2500)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("order", ["row", "class"])
+@pytest.mark.parametrize("dtype", list(DTYPES))
+def test_edges_of_frames(gpu, monkeypatch, dtype, order):
+    here = sys.modules[__name__]
+    monkeypatch.setattr(here, "SHAPES", EDGES)
+    test_log_probs_and_gradient(gpu, dtype, order)
+    for kl in ("none", "sampled", "exact"):
+        test_policy_loss(gpu, dtype, order, kl)
+    monkeypatch.setattr(here, "BALANCE_SHAPES", [e for e in EDGES if e[1] <= 4096])
+    test_balance_loss(gpu, dtype, order)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("order", ["row", "row+"])
+@pytest.mark.parametrize("dtype", list(DTYPES))
+def test_balance_loss_of_many_rows(gpu, monkeypatch, dtype, order):
+    monkeypatch.setattr(sys.modules[__name__], "BALANCE_SHAPES", BALANCE_ROWS)
+    test_balance_loss(gpu, dtype, order)
