@@ -1,0 +1,181 @@
+"""The losses at scores of any finite size: rows far from zero, classes masked
+by finite numbers, whole ranges of them, and sums of very many rows, against
+float64 forms."""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from conftest import print_case
+from test_losses import (DTYPES, F64, STEPS, U, balance_want, check, grad_tol, log_softmax64,
+                         norm_tol, policy_scales, policy_want, run_policy, to_gpu)
+
+# every frame, and rows in ranges: class-major of more than 512 classes, row-major
+# of more than 65536 float32 or 131072 16-bit classes
+SHAPES = [(40, 3), (70, 10), (65, 40), (33, 100), (24, 257), (18, 700), (9, 5000), (9, 70_001)]
+LONG = {"f32": (9, 70_001), "bf16": (9, 140_003), "f16": (9, 140_003)}
+OFFSETS = [0.0, 1e3, -1e3, 1e5, -1e6, 1e10, -1e10, 1e30, -3e38]
+OFFSETS_F16 = [0.0, 1e3, -1e3, 3e4, -6e4, 6e4]
+MASKS = [-1e4, -1e9, -1e10, -1e30, float(torch.finfo(torch.float32).min)]
+MASKS_F16 = [-1e4, -6e4, float(torch.finfo(torch.float16).min)]
+
+
+def place(v, order):
+    return v if order == "row" else v.t().contiguous().t()
+
+
+def far_rows(n, K, dtype, order, seed, roll=0):
+    """Rows of a few units' spread about offsets of many sizes."""
+    g = torch.Generator().manual_seed(seed)
+    off = OFFSETS_F16 if dtype == "f16" else OFFSETS
+    at = torch.tensor([off[(i + roll) % len(off)] for i in range(n)], dtype=F64)
+    v = at[:, None] + 2 * torch.randn((n, K), generator=g, dtype=F64)
+    return place(v.to(DTYPES[dtype]), order)
+
+
+def masked_rows(n, K, dtype, order, seed):
+    """Rows with blocks of classes masked by finite numbers: the first half, the
+    second, all but one class, every other class; the open classes."""
+    g = torch.Generator().manual_seed(seed)
+    low = MASKS_F16 if dtype == "f16" else MASKS
+    v = 2 * torch.randn((n, K), generator=g)
+    shut = torch.zeros((n, K), dtype=torch.bool)
+    for i in range(n):
+        one = int(torch.randint(0, K, (1,), generator=g))
+        way = i % 4
+        if way == 0:
+            shut[i, :K // 2] = True
+        elif way == 1:
+            shut[i, (K + 1) // 2:] = True
+        elif way == 2:
+            shut[i] = True
+            shut[i, one] = False
+        else:
+            shut[i, ::2] = True
+        v[i, shut[i]] = max(low[(i // 4) % len(low)], float(torch.finfo(DTYPES[dtype]).min))
+    return place(v.to(DTYPES[dtype]), order), ~shut
+
+
+def labels_of(s, allowed, seed):
+    g = torch.Generator().manual_seed(seed)
+    p = torch.softmax(s.to(F64), 1) if allowed is None else allowed.to(F64)
+    return torch.multinomial(p, 1, generator=g)[:, 0].to(torch.int32)
+
+
+def check_log_probs(s, a, dtype):
+    """class_log_probs and its gradient (finite scores only)."""
+    from warpgbm_amd import losses
+
+    n = s.shape[0]
+    up = torch.randn(n, generator=torch.Generator().manual_seed(n))
+    sd = to_gpu(s)
+    r = losses.class_log_probs(sd, a.cuda())
+    L = log_softmax64(s)
+    lp = L.gather(1, a.long()[:, None])[:, 0]
+    check(r.log_prob, lp, norm_tol(lp), "log_prob")
+    top = s.to(F64).max(1).values
+    check(r.norm[:, 0], top, 0.0, "maximum")
+    spread = torch.exp(s.to(F64) - top[:, None]).sum(1).log()
+    check(r.norm[:, 1], spread, norm_tol(spread), "log of the sum")
+    got = losses.class_log_probs_grad(sd, a.cuda(), r.norm, up.cuda())
+    grad = -L.exp() * up.to(F64)[:, None]
+    at = torch.arange(n)
+    grad[at, a.long()] = -torch.expm1(lp) * up.to(F64)
+    check(got, grad, grad_tol(grad, up.abs().to(F64), dtype), "gradient")
+
+
+def policy_dict(s, rs, a, seed):
+    n = s.shape[0]
+    g = torch.Generator().manual_seed(seed)
+    lp = log_softmax64(s).gather(1, a.long()[:, None])[:, 0].float()
+    return dict(s=s, ref_s=rs, a=a, old=lp + 0.3 * torch.randn(n, generator=g),
+                adv=torch.randn(n, generator=g), w=0.5 + torch.rand(n, generator=g),
+                ref=lp + 0.4 * torch.randn(n, generator=g))
+
+
+def check_policy(d, dtype):
+    clip, c = (0.2, 0.3), 0.25
+    for kl in ("none", "sampled", "exact"):
+        loss, lp, k, grad, live = policy_want(d, kl, clip, c)
+        scale = policy_scales(d, kl, c, k, live)
+        r = run_policy(d, kl, clip, c)
+        check(r.log_prob, lp, norm_tol(lp), "log_prob")
+        check(r.loss, loss, STEPS * U * (scale + d["w"].to(F64)), "loss")
+        if kl != "none":
+            check(r.kl, k, STEPS * U * (scale / d["w"].to(F64) / c + 1), "kl")
+        check(r.grad, grad, grad_tol(grad, scale, dtype), "gradient")
+
+
+def check_balance(s, dtype, top_k):
+    from warpgbm_amd import losses
+
+    n, K = s.shape
+    coef = 3.0 * n
+    loss, counts, prob, grad, live = balance_want(s, None, top_k, coef)
+    r = losses.balance_loss(to_gpu(s), top_k=top_k, coef=coef)
+    assert torch.equal(r.counts.cpu(), counts)
+    check(r.prob, prob, 2 * STEPS * U * prob + 1e-12, "prob")
+    check(r.loss, loss, 2 * STEPS * U * loss.abs() + 1e-12, "loss")
+    f = counts.to(F64) / (n * top_k)
+    P = torch.softmax(s.to(F64), 1)
+    tol = STEPS * U * (coef * K / n * (P * (f + (P @ f)[:, None]))).amax(1) + 1e-12
+    check(r.grad, grad, grad_tol(grad, torch.zeros(n, dtype=F64), dtype) + tol[:, None], "grad")
+
+
+def shapes_of(dtype):
+    return SHAPES + ([LONG[dtype]] if LONG[dtype] not in SHAPES else [])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("order", ["row", "class"])
+@pytest.mark.parametrize("dtype", list(DTYPES))
+def test_rows_far_from_zero(gpu, dtype, order):
+    """A row's offset, however large, changes nothing but the scores' own
+    rounding."""
+    for j, (n, K) in enumerate(shapes_of(dtype)):
+        print_case("far rows", dtype, order, n, K)
+        s = far_rows(n, K, dtype, order, 400 + j)
+        a = labels_of(s, None, j)
+        check_log_probs(s, a, dtype)
+        rs = far_rows(n, K, dtype, order, 500 + j, roll=2)
+        check_policy(policy_dict(s, rs, a, 600 + j), dtype)
+        if K <= 4096:
+            check_balance(s, dtype, min(K, 1 + j % 3))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("order", ["row", "class"])
+@pytest.mark.parametrize("dtype", list(DTYPES))
+def test_classes_masked_by_finite_numbers(gpu, dtype, order):
+    """Blocks of -1e4 to the type's lowest value count as far less likely classes,
+    also where a range or a thread's part of a row holds nothing else."""
+    for j, (n, K) in enumerate(shapes_of(dtype)):
+        print_case("finite masks", dtype, order, n, K)
+        n = max(n, 20)
+        s, allowed = masked_rows(n, K, dtype, order, 700 + j)
+        any_label = torch.randint(0, K, (n,), generator=torch.Generator().manual_seed(j),
+                                  dtype=torch.int32)
+        check_log_probs(s, any_label, dtype)
+        a = labels_of(s, allowed, j)
+        g = torch.Generator().manual_seed(800 + j)
+        noise = torch.where(allowed, 0.5 * torch.randn((n, K), generator=g), torch.zeros(()))
+        rs = place((s.float() + noise).to(s.dtype), order)
+        check_policy(policy_dict(s, rs, a, 900 + j), dtype)
+        if K <= 4096:
+            check_balance(s, dtype, min(K, 1 + j % 3))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("order", ["row", "class"])
+def test_divergence_from_a_reference_masked_by_finite_numbers(gpu, order):
+    """Classes that only the reference masks: the divergence is as large as the
+    mask times their probability, and finite."""
+    for j, (n, K) in enumerate(SHAPES):
+        print_case("reference masked", order, n, K)
+        n = max(n, 20)
+        rs, allowed = masked_rows(n, K, "f32", order, 1000 + j)
+        rs.clamp_(min=-1e30)
+        g = torch.Generator().manual_seed(j)
+        s = place(2 * torch.randn((n, K), generator=g), order)
+        check_policy(policy_dict(s, rs, labels_of(s, None, j), 1100 + j), "f32")

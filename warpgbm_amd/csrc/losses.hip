@@ -38,12 +38,12 @@ __device__ __forceinline__ RowStats scan_classes(const T* s, const T* r, int64_t
       mr = fmaxf(mr, w[j]);
     }
     rebase_stats<REF>(a, m, mr);
-    const Base b = base_of(safe_max(m)), br = base_of(safe_max(mr));
+    const float ms = safe_max(m), mrs = safe_max(mr);
     // (the eight's sums first: a shorter chain of additions, fewer roundings)
     RowStats e = empty_stats();
 #pragma unroll
     for (int j = 0; j < U; ++j)
-      add_class<REF>(e, power_of(v[j], b), power_of(w[j], br), k + j * step == label);
+      add_class<REF>(e, v[j] - ms, w[j] - mrs, k + j * step == label);
     a.z += e.z;
     a.za += e.za;
     if (REF) {

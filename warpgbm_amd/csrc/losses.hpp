@@ -40,17 +40,12 @@ struct PolicyRows {
   float* kl;
 };
 
-// a row's maximum as the exponentials take it: 2^(s lg - m2) = e^(s - m)
-struct Base {
-  float m2, lg;
-};
-
-// what a row's gradient is made of: with h = s lg - m2 of the scores' base and
-// hr of the reference's, 2^h = e^(s - max) and
-//   g_k = 2^h (c1 (h - hr) + c0),  and at the label g_a = gl
-// (c1 and br only with reference scores).  live = 0: the row's gradient is 0.
+// what a row's gradient is made of: with x = s - m of the scores and y = r - mr
+// of the reference's (m, mr: the maxima)
+//   g_k = e^x (c1 (x - y) + c0),  and at the label g_a = gl
+// (c1 and mr only with reference scores).  live = 0: the row's gradient is 0.
 struct RowCoef {
-  Base b, br;
+  float m, mr;
   float c0, c1, gl;
   int32_t label;
   int32_t live;
@@ -69,32 +64,25 @@ __device__ __forceinline__ T from_f32(float v) {
   return (T)v;
 }
 
-// Exponentials: e^(s - m) = 2^(s lg - m2), lg = log2(e), m2 = m lg rounded: one
-// fused multiply-add and v_exp_f32.  The fused result's rounding costs |h| 2^-24
-// of the value, that is at most 2^-25 of the row's largest exponential (|x| e^-x
-// has its maximum 1/e): what a softmax's sums and gradients are rounded by
-// anyway.  The rounding of m2 is a factor that all classes of the row share and
-// that every quotient loses; row_log_prob takes it out of the sum's logarithm.
-// (The losses of 16-bit scores are bound by instructions as much as by memory: the
-// 4 bytes of a score and its gradient pass while a lane issues some 30.)
+// Exponentials: e^x, x = s - m, by v_exp_f32 of x log2(e).  The difference comes
+// first: it is exact for the scores that count (s within a factor of two of m, or
+// both small), 0 at the maximum whatever its size, and -inf at worst.  (One fused
+// multiply-add, s log2(e) - fl(m log2(e)), would save an instruction a class but
+// leaves m log2(e)'s rounding in the power: 10^-3 at a maximum of 10^5, a factor
+// of 2^440 at 10^10; both forms take the same time, 8191 x 16001 bfloat16 110 us, 1M x
+// 10 float32 against a reference 37.)  The difference's, the product's and log2(e)'s roundings
+// cost 2.3 |x| log2(e) 2^-24 ln(2) of the value, that is less than 2^-24 of the
+// row's largest exponential (|x| e^-|x| has its maximum 1/e): what a softmax's sums
+// and gradients are rounded by anyway.
 constexpr float kLog2e = 1.44269504088896340736f;
 constexpr double kLn2 = 0.693147180559945309417;
-// (m: finite.  A maximum near the type's ends, a row whose classes are all
-// masked by the type's lowest value, would overflow; scores that far out differ
-// by 10^30 or not at all, so that any factor will do: 1.)
-__device__ __forceinline__ Base base_of(float m) {
-  const float lg = fabsf(m) > 1e38f ? 1.0f : kLog2e;
-  return {m * lg, lg};
-}
-__device__ __forceinline__ float power_of(float s, const Base& b) {
-  return fmaf(s, b.lg, -b.m2);
-}
 __device__ __forceinline__ float exp2_f32(float h) { return __builtin_amdgcn_exp2f(h); }
+__device__ __forceinline__ float exp_diff(float x) { return exp2_f32(x * kLog2e); }
 
 // running maximum and sums of a set of a row's classes, all in float32:
-//   m = max s_k, z = sum of 2^h_k over the classes but the label (h as above),
-//   za = the label's 2^h_a (0 when it is in another set); with reference scores
-//   r: mr = max r_k, zr = sum of 2^hr_k, u = sum of 2^h_k (h_k - hr_k)
+//   m = max s_k, z = sum of e^x_k over the classes but the label (x = s - m),
+//   za = the label's e^x_a (0 when it is in another set); with reference scores
+//   r: mr = max r_k, zr = sum of e^y_k (y = r - mr), u = sum of e^x_k (x_k - y_k)
 // The label is summed apart so that 1 - p_a = z / (z + za) keeps its digits
 // for a row that is sure of its label.
 struct RowStats {
@@ -112,14 +100,13 @@ __device__ __forceinline__ float safe_max(float m) { return m == -__builtin_inff
 // the same statistics relative to the larger maxima m and mr
 template <bool REF>
 __device__ __forceinline__ void rebase_stats(RowStats& a, float m, float mr) {
-  // (differences of the rounded scaled maxima, as the classes' own powers have)
-  const float b = base_of(safe_max(m)).m2 - base_of(safe_max(a.m)).m2;
-  const float f = a.m == -__builtin_inff() ? 0.0f : exp2_f32(-b);  // 0 for an empty set
+  const float b = safe_max(m) - safe_max(a.m);
+  const float f = a.m == -__builtin_inff() ? 0.0f : exp_diff(-b);  // 0 for an empty set
   if (REF) {
-    const float br = base_of(safe_max(mr)).m2 - base_of(safe_max(a.mr)).m2, t = a.z + a.za;
+    const float br = safe_max(mr) - safe_max(a.mr), t = a.z + a.za;
     // a set that counts for nothing has no difference to move
     a.u = t != 0.0f && f != 0.0f ? f * (a.u + (br - b) * t) : 0.0f;
-    a.zr *= a.mr == -__builtin_inff() ? 0.0f : exp2_f32(-br);
+    a.zr *= a.mr == -__builtin_inff() ? 0.0f : exp_diff(-br);
     a.mr = mr;
   }
   a.z *= f;
@@ -127,19 +114,19 @@ __device__ __forceinline__ void rebase_stats(RowStats& a, float m, float mr) {
   a.m = m;
 }
 
-// one more class of powers h and hr
+// one more class of differences x and y
 template <bool REF>
-__device__ __forceinline__ void add_class(RowStats& a, float h, float hr, bool is_label) {
-  const float e = exp2_f32(h);
+__device__ __forceinline__ void add_class(RowStats& a, float x, float y, bool is_label) {
+  const float e = exp_diff(x);
   if (is_label)
     a.za += e;
   else
     a.z += e;
   if (REF) {
-    a.zr += exp2_f32(hr);
+    a.zr += exp_diff(y);
     // a class of probability 0 takes no part in the divergence, whatever the
     // reference says of it (both are -inf at classes that a row may not take)
-    a.u += e == 0.0f ? 0.0f : e * (h - hr);
+    a.u += e == 0.0f ? 0.0f : e * (x - y);
   }
 }
 
@@ -182,10 +169,10 @@ __device__ __forceinline__ double log_of(float z) {
   const Split s = split_f32(z);
   return ((double)s.k + (double)log2_f32(s.f)) * kLn2;
 }
-// log2(a / b)
-__device__ __forceinline__ double log2_ratio(float a, float b) {
+// log(a / b)
+__device__ __forceinline__ double log_ratio(float a, float b) {
   const Split x = split_f32(a), y = split_f32(b);
-  return (double)(x.k - y.k) + (double)(log2_f32(x.f) - log2_f32(y.f));
+  return ((double)(x.k - y.k) + (double)(log2_f32(x.f) - log2_f32(y.f))) * kLn2;
 }
 // log(1 + q) for q in [0, 1]: the logarithm of the rounded sum, and what the
 // rounding left out
@@ -199,11 +186,6 @@ __device__ __forceinline__ float exp_of(float x) {
   return fabsf(h) < 200.0f ? fmaf(e, lo * (float)kLn2, e) : e;  // (no inf * 0)
 }
 
-// logarithm of a sum of 2^(s lg - m2), the rounding of m2 taken out
-__device__ __forceinline__ double sum_log(float z, float m) {
-  const Base b = base_of(m);
-  return log_of(z) + kLn2 * ((double)b.m2 - (double)m * (double)b.lg);
-}
 __device__ __forceinline__ bool row_live(const RowStats& a) {
   return !(a.z + a.za == 0.0f);  // the row has a class (NaN: it shows in the results)
 }
@@ -211,9 +193,8 @@ __device__ __forceinline__ bool row_live(const RowStats& a) {
 // from the others' share, which keeps the digits of a row that is sure of its
 // label (and the sign).
 __device__ __forceinline__ double row_log_prob(const RowStats& a, float sa) {
-  const float m = safe_max(a.m);
   if (a.za >= a.z) return -(double)log1p_of(a.z / a.za);
-  return ((double)sa - (double)m) - sum_log(a.z + a.za, m);
+  return ((double)sa - (double)safe_max(a.m)) - log_of(a.z + a.za);
 }
 
 // The policy loss of one row and its gradient's coefficients.
@@ -236,8 +217,8 @@ __device__ __forceinline__ PolicyRow policy_row(const RowStats& st, float sa, fl
                                                 int32_t label, const double* exact_logp) {
   PolicyRow o;
   const float z = st.z + st.za, iz = __builtin_amdgcn_rcpf(z);
-  o.c.b = base_of(safe_max(st.m));
-  o.c.br = REF ? base_of(safe_max(st.mr)) : o.c.b;
+  o.c.m = safe_max(st.m);
+  o.c.mr = REF ? safe_max(st.mr) : 0.0f;
   o.c.label = label;
   o.c.live = row_live(st);
   o.near = false;
@@ -272,12 +253,11 @@ __device__ __forceinline__ PolicyRow policy_row(const RowStats& st, float sa, fl
   o.kl = 0.0f;
   float wk = 0.0f, base = 0.0f;
   if (REF) {
-    // in powers of two: log2 p_k - log2 q_k = (h_k - hr_k) + lr, lr = log2 of
-    // the sums' quotient (the maxima's roundings are in both h and the sums)
-    const double lr = log2_ratio(st.zr, z);
+    // log p_k - log q_k = (x_k - y_k) + lr, lr = log of the sums' quotient
+    const double lr = log_ratio(st.zr, z);
     const double kl = (double)(st.u / z) + lr;
-    o.kl = (float)(kLn2 * kl);
-    base = (float)(lr - kl);  // (log2 p_k - log2 q_k - KL2) - (h_k - hr_k)
+    o.kl = (float)kl;
+    base = (float)(lr - kl);  // (log p_k - log q_k - KL) - (x_k - y_k)
     // (a divergence that does not count may be infinite)
     if (g.kl_coef != 0.0f)
       value += g.kl_coef * o.kl;
@@ -298,21 +278,20 @@ __device__ __forceinline__ PolicyRow policy_row(const RowStats& st, float sa, fl
   }
   c *= w;
   o.loss = w * value;
-  const float wn = wk * (float)kLn2;
-  o.c.c0 = (wn * base - c) * iz;
-  o.c.c1 = wn * iz;
+  o.c.c0 = (wk * base - c) * iz;
+  o.c.c1 = wk * iz;
   o.c.gl = c * (st.z * iz);
-  if (REF && wn != 0.0f && st.za != 0.0f)
-    o.c.gl += st.za * iz * wn * ((power_of(sa, o.c.b) - power_of(ra, o.c.br)) + base);
+  if (REF && wk != 0.0f && st.za != 0.0f)
+    o.c.gl += st.za * iz * wk * (((sa - o.c.m) - (ra - o.c.mr)) + base);
   return o;
 }
 
 // gradient at a class that is not the label
 template <bool REF>
 __device__ __forceinline__ float coef_grad(const RowCoef& c, float s, float r) {
-  const float h = power_of(s, c.b), e = exp2_f32(h);
+  const float x = s - c.m, e = exp_diff(x);
   if (!REF || c.c1 == 0.0f) return e * c.c0;
-  return e == 0.0f ? 0.0f : e * fmaf(c.c1, h - power_of(r, c.br), c.c0);
+  return e == 0.0f ? 0.0f : e * fmaf(c.c1, x - (r - c.mr), c.c0);
 }
 
 }  // namespace wgbm

@@ -31,7 +31,7 @@ template <typename F>
 constexpr bool kAhead = 2 * F::kWords + 2 * F::N <= 104;
 
 // part [K][workgroups], count [K + 1][workgroups] (the last: rows that count);
-// norm: a row's maximum and 1 / sum of 2^h (0: left out)
+// norm: a row's maximum and 1 / sum of e^(s - m) (0: left out)
 template <typename F>
 __global__ __launch_bounds__(F::kMax) void balance_stats_kernel(
     ScoresView s, const uint8_t* __restrict__ mask, int32_t top_k, int64_t blocks,
@@ -74,14 +74,13 @@ __global__ __launch_bounds__(F::kMax) void balance_stats_kernel(
     }
     m = f.reduce(m, MaxF(), buf[0]);
     const float ms = safe_max(m);
-    const Base base = base_of(ms);
     // the exponentials of up to 16 classes stay in registers; more are worked
     // out again for the sums
     constexpr bool kKeep = F::N <= 16;
     float e[kKeep ? F::N : 1], z[2] = {0.0f, 0.0f};
 #pragma unroll
     for (int j = 0; j < F::N; ++j) {
-      const float x = exp2_f32(power_of(F::value(v, j), base));
+      const float x = exp_diff(F::value(v, j) - ms);
       z[j % 2] += x;
       if constexpr (kKeep) e[j] = x;
     }
@@ -94,7 +93,7 @@ __global__ __launch_bounds__(F::kMax) void balance_stats_kernel(
       if constexpr (kKeep)
         x = e[j];
       else
-        x = exp2_f32(power_of(F::value(v, j), base));
+        x = exp_diff(F::value(v, j) - ms);
       acc[j] = fmaf(x, iz, acc[j]);
     }
     if (in && f.first_lane()) norm[i] = make_float2(ms, iz);
@@ -171,11 +170,10 @@ __global__ __launch_bounds__(F::kMax) void balance_grad_kernel(
     if (kAhead<F> && b + gridDim.x < blocks) fetch(b + gridDim.x);
     f.trim(v);
     const bool live = in && nm.y != 0.0f;  // (NaN is live)
-    const Base base = base_of(nm.x);
     float e[F::N], q = 0.0f;
 #pragma unroll
     for (int j = 0; j < F::N; ++j) {
-      e[j] = exp2_f32(power_of(F::value(v, j), base));
+      e[j] = exp_diff(F::value(v, j) - nm.x);
       q = fmaf(fk[j], e[j], q);
     }
     // (two turns' words: a wave may be one reduction ahead of the others)

@@ -93,7 +93,7 @@ __device__ __forceinline__ void write_log_prob(const RowStats& a, float sa, int3
   const bool live = row_live(a);
   const float m = safe_max(a.m);
   log_prob[i] = live && label >= 0 ? (float)row_log_prob(a, sa) : 0.0f;
-  norm[i] = live ? make_float2(m, (float)sum_log(a.z + a.za, m))
+  norm[i] = live ? make_float2(m, (float)log_of(a.z + a.za))
                  : make_float2(-__builtin_inff(), 0.0f);
 }
 
@@ -110,7 +110,7 @@ struct LogProbGrad {
     const float g = grad[i];
     const float2 v = norm[i];
     if (a < 0 || g == 0.0f || v.x == -__builtin_inff()) return c;
-    c.b = base_of(v.x);
+    c.m = v.x;
     c.c0 = -g * expf(-v.y);
     // the label's from its own logarithm: 1 - p without a difference
     c.gl = -g * expm1f((score_at<T>(s, i, a) - v.x) - v.y);

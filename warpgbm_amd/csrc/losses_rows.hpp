@@ -18,13 +18,13 @@ __device__ __forceinline__ RowStats frame_stats(const F& f, typename F::Regs& s,
 #pragma unroll
   for (int j = 0; j < F::N; ++j) a.m = fmaxf(a.m, F::value(s, j));
   a.m = f.reduce(a.m, MaxF(), buf[0]);
-  const Base b = base_of(safe_max(a.m));
-  Base br = b;
+  const float m = safe_max(a.m);
+  float mr = m;
   if (REF) {
 #pragma unroll
     for (int j = 0; j < F::N; ++j) a.mr = fmaxf(a.mr, F::value(r, j));
     a.mr = f.reduce(a.mr, MaxF(), buf[1]);
-    br = base_of(safe_max(a.mr));
+    mr = safe_max(a.mr);
   }
   if (F::kHide) f.hide(s);
   if (REF && F::kHide) f.hide(r);
@@ -32,12 +32,12 @@ __device__ __forceinline__ RowStats frame_stats(const F& f, typename F::Regs& s,
   float z[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
   for (int j = 0; j < F::N; ++j) {
-    const float h = power_of(F::value(s, j), b), e = exp2_f32(h);
+    const float x = F::value(s, j) - m, e = exp_diff(x);
     z[j % 4] += f.cls(j) == label ? 0.0f : e;
     if (REF) {
-      const float hr = power_of(F::value(r, j), br);
-      a.zr += exp2_f32(hr);
-      a.u += e == 0.0f ? 0.0f : e * (h - hr);
+      const float y = F::value(r, j) - mr;
+      a.zr += exp_diff(y);
+      a.u += e == 0.0f ? 0.0f : e * (x - y);
     }
   }
   if (F::kHide) f.hide(s);
@@ -69,7 +69,7 @@ __global__ __launch_bounds__(F::kMax) void log_probs_frame_kernel(
   const float sa = lab >= 0 ? score_at<typename F::T>(s, i, lab) : 0.0f;
   f.trim(v);
   RowStats a = frame_stats<F, false>(f, v, v, lab, buf);
-  if (lab >= 0) a.za = exp2_f32(power_of(sa, base_of(safe_max(a.m))));
+  if (lab >= 0) a.za = exp_diff(sa - safe_max(a.m));
   if (!in || !f.first_lane()) return;
   write_log_prob(a, sa, lab, i, log_prob, norm);
 }
@@ -130,7 +130,7 @@ __global__ __launch_bounds__(F::kMax) void policy_frame_kernel(ScoresView s, Sco
   f.trim(v);
   if (REF) f.trim(r);
   RowStats st = frame_stats<F, REF>(f, v, r, lab, buf);
-  if (lab >= 0) st.za = exp2_f32(power_of(sa, base_of(safe_max(st.m))));
+  if (lab >= 0) st.za = exp_diff(sa - safe_max(st.m));
   // what follows from the row as a whole costs as much as some ten classes:
   // where waves share rows, the first one works it out for all
   const bool owner = !F::kBarrier || threadIdx.x < 64;
@@ -210,7 +210,7 @@ __global__ __launch_bounds__(256) void log_probs_batch_kernel(ScoresView s,
   __syncthreads();
   if (!mine) return;
   RowStats a = s_stats[threadIdx.x];
-  if (lab >= 0) a.za = exp2_f32(power_of(sa, base_of(safe_max(a.m))));
+  if (lab >= 0) a.za = exp_diff(sa - safe_max(a.m));
   write_log_prob(a, sa, lab, i, log_prob, norm);
 }
 
