@@ -231,8 +231,9 @@ int wgbm_importance_add(float* acc, int32_t n_feats, int32_t num_eras, const flo
  * counterpart in the reference, whose losses are squared error and softmax
  * cross entropy): what a boosting round with the engine's objective 2 fits.
  *
- * All sums are float32 (sums over the rows of a sequence, over the pairs of a
- * sequence and over all rows: float64), in an order that depends on the sizes
+ * All sums are float32 (sums over the rows of a sequence and over the pairs of a
+ * sequence: float64; the balance loss's over all rows: float32 for at most 256
+ * rows one after the other, float64 from there), in an order that depends on the sizes
  * only: results are the same in every run.  Gradients are rounded to the
  * scores' type once.  The calls allocate nothing and may be captured into a
  * HIP graph; `workspace` (device memory, 16-byte aligned, of the bytes that the

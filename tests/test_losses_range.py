@@ -179,3 +179,43 @@ def test_divergence_from_a_reference_masked_by_finite_numbers(gpu, order):
         g = torch.Generator().manual_seed(j)
         s = place(2 * torch.randn((n, K), generator=g), order)
         check_policy(policy_dict(s, rs, labels_of(s, None, j), 1100 + j), "f32")
+
+
+# (type, order, rows, classes): some 4096, 2048 and 1950 rows for each thread of the
+# first pass
+CHAINS = [("f32", "row", (1 << 30) - 5, 2), ("bf16", "class", (1 << 30) + 77, 2),
+          ("bf16", "class", (1 << 29) + 77, 17), ("f32", "row", 1_000_003, 4096)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,order,n,K", CHAINS)
+def test_balance_of_very_many_equal_rows(gpu, dtype, order, n, K):
+    """Equal rows: one after the other in float32 their probabilities would round
+    the same way each time, thousands of times."""
+    from warpgbm_amd import losses
+
+    print_case("very many rows", dtype, order, n, K)
+    torch.cuda.empty_cache()
+    row = torch.randn(K, generator=torch.Generator().manual_seed(K)).to(DTYPES[dtype])
+    if K == 2:
+        row = torch.tensor([0.0, 1.3]).to(DTYPES[dtype])
+    if order == "row":
+        s = torch.empty((n, K), dtype=row.dtype, device="cuda")
+        s[:] = row.cuda()
+    else:
+        s = torch.empty((K, n), dtype=row.dtype, device="cuda").t()
+        for k in range(K):
+            s[:, k] = float(row[k])
+    r = losses.balance_loss(s, with_grad=False)
+    del s
+    prob = torch.softmax(row.to(F64), 0)
+    counts = torch.zeros(K, dtype=torch.int64)
+    counts[row.argmax()] = n
+    assert torch.equal(r.counts.cpu(), counts)
+    # 256 additions one after the other, ten more in a workgroup; 70 roundings of a
+    # row's exponentials (their powers: 2.3 * 8 * 1.44 ln 2, at most 19), of its sum and
+    # of the quotient
+    check(r.prob, prob, (256 + 10 + 70) * U * prob, "prob")
+    want = K * prob[row.argmax()]
+    check(r.loss, want, (256 + 10 + 70 + 1) * U * want, "loss")
+    torch.cuda.empty_cache()

@@ -6,8 +6,9 @@
 // first, so the scores are read twice: rows in registers (losses_frames.hpp)
 // give the counts, the sums of p and each row's norm; a finishing launch the
 // shares; rows in registers again the gradient.  Workgroups take rows in turn
-// and leave one partial sum a class, which the finishing launch joins in
-// float64 in workgroup order: results do not depend on the order of execution.
+// and leave one partial sum a class for each kChain rows of a thread, which the
+// finishing launch joins in float64 in workgroup order: results do not depend on
+// the order of execution, and float32 sums stay short however many rows there are.
 //
 // 1M x 100 float32 class-major: the first pass 131 us (3.1 TB/s; the eight waves
 // that share 64 rows wait for one another at three reductions), the finish 7, the
@@ -30,12 +31,16 @@ struct MinF {
 template <typename F>
 constexpr bool kAhead = 2 * F::kWords + 2 * F::N <= 104;
 
-// part [K][workgroups], count [K + 1][workgroups] (the last: rows that count);
+// most rows that a thread adds up in float32: their roundings come to 256 * 2^-24 of
+// the sum at worst (float64 sums would take the registers of two)
+constexpr int32_t kChain = 256;
+
+// part [K][parts][workgroups], count [K + 1][workgroups] (the last: rows that count);
 // norm: a row's maximum and 1 / sum of e^(s - m) (0: left out)
 template <typename F>
 __global__ __launch_bounds__(F::kMax) void balance_stats_kernel(
     ScoresView s, const uint8_t* __restrict__ mask, int32_t top_k, int64_t blocks,
-    float* __restrict__ part, int32_t* __restrict__ count, float2* __restrict__ norm,
+    int32_t parts, float* __restrict__ part, int32_t* __restrict__ count, float2* __restrict__ norm,
     uint32_t* __restrict__ ticket) {
   extern __shared__ int32_t s_count[];  // [K + 1], then [K] floats
   __shared__ float buf[4][F::kBuf];
@@ -45,9 +50,6 @@ __global__ __launch_bounds__(F::kMax) void balance_stats_kernel(
   for (int32_t k = threadIdx.x; k <= K; k += blockDim.x) s_count[k] = 0;
   __syncthreads();
   const F f(s);
-  float acc[F::N];
-#pragma unroll
-  for (int j = 0; j < F::N; ++j) acc[j] = 0.0f;
   // the next rows' loads are in flight while these rows are summed
   typename F::Regs next;
   uint8_t next_want = 1;
@@ -57,88 +59,98 @@ __global__ __launch_bounds__(F::kMax) void balance_stats_kernel(
     f.load(next, s, b);
   };
   if (kAhead<F>) fetch(blockIdx.x);
-  for (int64_t b = blockIdx.x; b < blocks; b += gridDim.x) {
-    const int64_t row = F::row(b);
-    const bool in = row < s.n;
-    const int64_t i = in ? row : s.n - 1;
-    if (!kAhead<F>) fetch(b);
-    typename F::Regs v = next;
-    const bool want = in && next_want;
-    if (kAhead<F> && b + gridDim.x < blocks) fetch(b + gridDim.x);
-    f.trim(v);
-    if (!want) f.drop(v);
-    float m = -__builtin_inff();
+  // a thread adds at most kChain rows in float32; then the workgroup's sums are
+  // written and started again
+  int64_t b = blockIdx.x;
+  for (int32_t part_no = 0; part_no < parts; ++part_no) {
+    float acc[F::N];
 #pragma unroll
-    for (int j = 0; j < F::N; ++j) {
-      m = fmaxf(m, F::value(v, j));
-    }
-    m = f.reduce(m, MaxF(), buf[0]);
-    const float ms = safe_max(m);
-    // the exponentials of up to 16 classes stay in registers; more are worked
-    // out again for the sums
-    constexpr bool kKeep = F::N <= 16;
-    float e[kKeep ? F::N : 1], z[2] = {0.0f, 0.0f};
+    for (int j = 0; j < F::N; ++j) acc[j] = 0.0f;
+    const int64_t stop = b + (int64_t)kChain * gridDim.x, end = stop < blocks ? stop : blocks;
+    for (; b < end; b += gridDim.x) {
+      const int64_t row = F::row(b);
+      const bool in = row < s.n;
+      const int64_t i = in ? row : s.n - 1;
+      if (!kAhead<F>) fetch(b);
+      typename F::Regs v = next;
+      const bool want = in && next_want;
+      if (kAhead<F> && b + gridDim.x < blocks) fetch(b + gridDim.x);
+      f.trim(v);
+      if (!want) f.drop(v);
+      float m = -__builtin_inff();
 #pragma unroll
-    for (int j = 0; j < F::N; ++j) {
-      const float x = exp_diff(F::value(v, j) - ms);
-      z[j % 2] += x;
-      if constexpr (kKeep) e[j] = x;
-    }
-    z[0] = f.reduce(z[0] + z[1], AddF(), buf[1]);
-    const bool live = !(z[0] == 0.0f);  // (NaN is live)
-    const float iz = live ? 1.0f / z[0] : 0.0f;
-#pragma unroll
-    for (int j = 0; j < F::N; ++j) {
-      float x;
-      if constexpr (kKeep)
-        x = e[j];
-      else
-        x = exp_diff(F::value(v, j) - ms);
-      acc[j] = fmaf(x, iz, acc[j]);
-    }
-    if (in && f.first_lane()) norm[i] = make_float2(ms, iz);
-    // the best classes one after the other: the largest score after the last
-    // one taken, then the lowest class that has it.  A thread's classes ascend
-    // with its slots, so it looks for its lowest slot (slot numbers are
-    // constants of the instructions, class numbers would each take a register).
-    // Class numbers are exact in float32; a NaN is not after anything.
-    constexpr float kNone = 1e9f;
-    float v0 = __builtin_inff();
-    int32_t c0 = -1;
-    for (int32_t t = 0; t < top_k; ++t) {
-      float best = m;
-      int slot = F::N;
-      if (t == 0) {
-#pragma unroll
-        for (int j = F::N - 1; j >= 0; --j) slot = F::value(v, j) == best ? j : slot;
-      } else {
-        const int taken = f.last_slot(c0);  // of the scores equal to v0
-        best = -__builtin_inff();
-#pragma unroll
-        for (int j = 0; j < F::N; ++j) {
-          const float x = F::value(v, j);
-          if (x < v0 || (x == v0 && j > taken)) best = fmaxf(best, x);
-        }
-        best = f.reduce(best, MaxF(), buf[2]);
-        const int from = best < v0 ? -1 : taken;
-#pragma unroll
-        for (int j = F::N - 1; j >= 0; --j)
-          slot = F::value(v, j) == best && j > from ? j : slot;
+      for (int j = 0; j < F::N; ++j) {
+        m = fmaxf(m, F::value(v, j));
       }
-      const float c = f.reduce(slot < F::N ? (float)f.cls(slot) : kNone, MinF(), buf[3]);
-      if (best > -__builtin_inff() && c < kNone && f.first_lane())
-        atomicAdd(&s_count[(int32_t)c], 1);
-      v0 = best;
-      c0 = (int32_t)c;
+      m = f.reduce(m, MaxF(), buf[0]);
+      const float ms = safe_max(m);
+      // the exponentials of up to 16 classes stay in registers; more are worked
+      // out again for the sums
+      constexpr bool kKeep = F::N <= 16;
+      float e[kKeep ? F::N : 1], z[2] = {0.0f, 0.0f};
+#pragma unroll
+      for (int j = 0; j < F::N; ++j) {
+        const float x = exp_diff(F::value(v, j) - ms);
+        z[j % 2] += x;
+        if constexpr (kKeep) e[j] = x;
+      }
+      z[0] = f.reduce(z[0] + z[1], AddF(), buf[1]);
+      const bool live = !(z[0] == 0.0f);  // (NaN is live)
+      const float iz = live ? 1.0f / z[0] : 0.0f;
+#pragma unroll
+      for (int j = 0; j < F::N; ++j) {
+        float x;
+        if constexpr (kKeep)
+          x = e[j];
+        else
+          x = exp_diff(F::value(v, j) - ms);
+        acc[j] = fmaf(x, iz, acc[j]);
+      }
+      if (in && f.first_lane()) norm[i] = make_float2(ms, iz);
+      // the best classes one after the other: the largest score after the last
+      // one taken, then the lowest class that has it.  A thread's classes ascend
+      // with its slots, so it looks for its lowest slot (slot numbers are
+      // constants of the instructions, class numbers would each take a register).
+      // Class numbers are exact in float32; a NaN is not after anything.
+      constexpr float kNone = 1e9f;
+      float v0 = __builtin_inff();
+      int32_t c0 = -1;
+      for (int32_t t = 0; t < top_k; ++t) {
+        float best = m;
+        int slot = F::N;
+        if (t == 0) {
+#pragma unroll
+          for (int j = F::N - 1; j >= 0; --j) slot = F::value(v, j) == best ? j : slot;
+        } else {
+          const int taken = f.last_slot(c0);  // of the scores equal to v0
+          best = -__builtin_inff();
+#pragma unroll
+          for (int j = 0; j < F::N; ++j) {
+            const float x = F::value(v, j);
+            if (x < v0 || (x == v0 && j > taken)) best = fmaxf(best, x);
+          }
+          best = f.reduce(best, MaxF(), buf[2]);
+          const int from = best < v0 ? -1 : taken;
+#pragma unroll
+          for (int j = F::N - 1; j >= 0; --j)
+            slot = F::value(v, j) == best && j > from ? j : slot;
+        }
+        const float c = f.reduce(slot < F::N ? (float)f.cls(slot) : kNone, MinF(), buf[3]);
+        if (best > -__builtin_inff() && c < kNone && f.first_lane())
+          atomicAdd(&s_count[(int32_t)c], 1);
+        v0 = best;
+        c0 = (int32_t)c;
+      }
+      if (live && f.first_lane()) atomicAdd(&s_count[K], 1);
     }
-    if (live && f.first_lane()) atomicAdd(&s_count[K], 1);
+    f.sum_rows(acc, s_part);
+    __syncthreads();
+    for (int32_t k = threadIdx.x; k < K; k += blockDim.x)
+      part[((int64_t)k * parts + part_no) * gridDim.x + blockIdx.x] = s_part[k];
+    if (part_no + 1 < parts) __syncthreads();  // (s_part is written again)
   }
-  f.sum_rows(acc, s_part);
-  __syncthreads();
-  for (int32_t k = threadIdx.x; k <= K; k += blockDim.x) {
-    if (k < K) part[(int64_t)k * gridDim.x + blockIdx.x] = s_part[k];
+  for (int32_t k = threadIdx.x; k <= K; k += blockDim.x)
     count[(int64_t)k * gridDim.x + blockIdx.x] = s_count[k];
-  }
 }
 
 template <typename F>
@@ -242,12 +254,14 @@ static inline int64_t balance_few(int32_t K) {
 
 template <typename T>
 int balance_stats(const ScoresView& s, const uint8_t* mask, int32_t top_k, const BalanceWs& w,
-                  int32_t* groups, hipStream_t st) {
+                  int32_t* groups, int32_t* parts, hipStream_t st) {
   balance_frame<T>(s, [&](auto tag, int64_t blocks, int threads) {
     using F = typename decltype(tag)::type;
     *groups = (int32_t)std::min(blocks, std::min(balance_fill<F>(threads), balance_few(s.K)));
+    const int64_t turns = (blocks + *groups - 1) / *groups;
+    *parts = (int32_t)((turns + kChain - 1) / kChain);
     hipLaunchKernelGGL((balance_stats_kernel<F>), dim3((unsigned)*groups), dim3(threads),
-                       (2 * (size_t)s.K + 1) * 4, st, s, mask, top_k, blocks, w.part, w.count,
+                       (2 * (size_t)s.K + 1) * 4, st, s, mask, top_k, blocks, *parts, w.part, w.count,
                        w.norm, w.ticket);
   });
   WGBM_LAUNCH_CHECK();
