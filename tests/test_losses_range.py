@@ -219,3 +219,22 @@ def test_balance_of_very_many_equal_rows(gpu, dtype, order, n, K):
     want = K * prob[row.argmax()]
     check(r.loss, want, (256 + 10 + 70 + 1) * U * want, "loss")
     torch.cuda.empty_cache()
+
+
+@pytest.mark.gpu
+def test_large_and_small_ratios(gpu):
+    """Ratios from e^-80 to e^85 that no border holds, of rows of one class, whose
+    log-probability is 0: the loss is the ratio."""
+    from warpgbm_amd import losses
+
+    n = 200_000
+    g = torch.Generator().manual_seed(12)
+    old = 80 - 165 * torch.rand(n, generator=g)
+    s = torch.randn((n, 1), generator=g)
+    r = losses.policy_loss(s.cuda(), torch.zeros(n, dtype=torch.int32, device="cuda"), old.cuda(),
+                           -torch.ones(n, device="cuda"), clip=(1.0, 0.2))
+    assert not r.log_prob.any()
+    want = torch.exp(-old.to(F64))
+    # v_exp_f32: one ulp (2 * 2^-24 of the value at most); the correction's product and
+    # sum round once more
+    check(r.loss, want, 4 * U * want, "loss")
