@@ -238,3 +238,14 @@ def test_large_and_small_ratios(gpu):
     # v_exp_f32: one ulp (2 * 2^-24 of the value at most); the correction's product and
     # sum round once more
     check(r.loss, want, 4 * U * want, "loss")
+
+
+def test_refused_sizes_keep_their_message():
+    """A refusal says why each time, whatever was refused in between."""
+    from warpgbm_amd import losses
+
+    for _ in range(2):
+        with pytest.raises(RuntimeError, match="at most 4096 classes"):
+            losses._bytes_of("wgbm_balance_loss_workspace", 0, 6, 5000, False)
+        with pytest.raises(RuntimeError, match="n_classes must be in"):
+            losses._bytes_of("wgbm_class_log_probs_workspace", 0, 6, (1 << 24) + 1, False)

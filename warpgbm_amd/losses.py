@@ -140,17 +140,19 @@ class _on:
 @functools.lru_cache(maxsize=4096)
 def _bytes_of(entry, dtype, n, K, class_major):
     """What a _workspace entry returns for scores of a shape and order (a call
-    into the library costs more than the small losses' launches)."""
+    into the library costs more than the small losses' launches).  A refusal is
+    raised, and so not kept: its message is the library's last one now."""
     v = _lib.Scores(16, dtype, n, K, 1 if class_major else K, max(n, 2) if class_major else 1)
-    return getattr(_lib.load(), entry)(C.byref(v))
+    nbytes = getattr(_lib.load(), entry)(C.byref(v))
+    if nbytes < 0:
+        _lib.check(1000, entry)
+    return nbytes
 
 
 def _workspace(entry, v, device):
     """Working memory of a call: (tensor or None, address, bytes)."""
     nbytes = _bytes_of(entry, v.dtype, v.n_rows, v.n_classes,
                        v.row_stride == 1 and v.class_stride != 1)
-    if nbytes < 0:
-        _lib.check(1000, entry)
     if nbytes == 0:
         return None, None, 0
     t = torch.empty(nbytes, dtype=torch.uint8, device=device)
