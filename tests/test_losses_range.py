@@ -249,3 +249,55 @@ def test_refused_sizes_keep_their_message():
             losses._bytes_of("wgbm_balance_loss_workspace", 0, 6, 5000, False)
         with pytest.raises(RuntimeError, match="n_classes must be in"):
             losses._bytes_of("wgbm_class_log_probs_workspace", 0, 6, (1 << 24) + 1, False)
+
+
+def test_shared_memory_is_found():
+    """Views of one buffer: whether they share an element, for rows between rows,
+    columns, single rows and vectors."""
+    from warpgbm_amd import losses
+
+    rng = np.random.default_rng(5)
+    buf = torch.arange(400, dtype=torch.int16)
+
+    def view():
+        at, way = int(rng.integers(0, 120)), int(rng.integers(0, 4))
+        n, K, gap = (int(x) for x in rng.integers(1, 6, 3))
+        if way == 0:
+            return torch.as_strided(buf, (n * K,), (1,), at)
+        if way == 1:
+            return torch.as_strided(buf, (n, K), (K + gap * 5, 1), at)
+        if way == 2:
+            return torch.as_strided(buf, (n, K), (1, n + gap * 5), at)
+        # (a stride that two views often have in common)
+        return torch.as_strided(buf, (n, K), (20, 1), at)
+
+    seen = [0, 0]
+    for _ in range(4000):
+        a, b = view(), view()
+        share = bool(set(a.reshape(-1).tolist()) & set(b.reshape(-1).tolist()))
+        assert losses._meet(a, b) == share, (a, b)
+        seen[share] += 1
+    assert min(seen) > 500
+    assert not losses._meet(buf[:0], buf) and not losses._meet(buf[:0].view(0, 3), buf)
+
+
+@pytest.mark.gpu
+def test_a_gradient_that_shares_memory_is_refused(gpu):
+    from warpgbm_amd import losses
+
+    both = torch.zeros((6, 9), device="cuda")
+    s, a = both[:, :4], torch.zeros(6, dtype=torch.int32, device="cuda")
+    f = torch.zeros(6, device="cuda")
+    for grad in (both[:, 1:5], both[:, 3:7], both[:, :4]):
+        with pytest.raises(RuntimeError, match="scores' memory"):
+            losses.balance_loss(s, grad=grad)
+        with pytest.raises(RuntimeError, match="share memory with an input"):
+            losses.policy_loss(torch.zeros((6, 4), device="cuda"), a, f, f, ref_scores=s,
+                               grad=grad)
+    flat = torch.zeros(48, device="cuda")
+    with pytest.raises(RuntimeError, match="share memory with an input"):
+        losses.policy_loss(s.clone(), a, flat[20:26], f, grad=flat[:24].view(6, 4))
+    # rows between the scores' rows are not the scores'
+    want = losses.balance_loss(s.clone())
+    got = losses.balance_loss(s, grad=both[:, 5:])
+    assert torch.equal(got.grad, want.grad) and not both[:, :5].any()

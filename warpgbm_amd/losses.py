@@ -19,8 +19,8 @@ Launches go on torch's current stream of the scores' device; nothing
 synchronises except the construction of a :class:`PreferencePlan`.  Outputs and
 working memory come from torch's allocator, so calls may be captured into a
 HIP graph.  Nothing is recorded for autograd.  A gradient that is given to be
-added to must not share memory with an input.  Wrong types, shapes, devices or
-layouts raise ``RuntimeError``.
+added to must not share memory with an input.  Shared memory, wrong types,
+shapes, devices or layouts raise ``RuntimeError``.
 """
 from __future__ import annotations
 
@@ -102,8 +102,39 @@ def _like(v, scores):
     return t, _lib.Scores(t.data_ptr(), v.dtype, n, K, K, 1)
 
 
-def _grad(grad, v, scores, with_grad):
-    """The gradient's matrix: a given one (added to), a new one, or none."""
+def _lines(t):
+    """A tensor's memory as (address, bytes of a line, lines, bytes from line to
+    line): its rows, or the columns where those are contiguous; one line where
+    it is contiguous as a whole."""
+    es = t.element_size()
+    if t.dim() != 2 or t.is_contiguous():
+        return t.data_ptr(), t.numel() * es, 1, t.numel() * es
+    (n, K), (rs, ks) = t.shape, t.stride()
+    if K > 1 and ks != 1:
+        n, K, rs = K, n, ks
+    return t.data_ptr(), K * es, n, rs * es
+
+
+def _meet(a, b):
+    """Whether two tensors share memory (rows of one between rows of another do
+    not)."""
+    p, w, m, s = _lines(a)
+    q, x, k, t = _lines(b)
+    if not (w and m and x and k) or p + (m - 1) * s + w <= q or q + (k - 1) * t + x <= p:
+        return False
+    if m == 1 or k == 1 or s == t:
+        # r: the last line of b, counted from a's i-th, that begins before that one ends
+        step = t if m == 1 else s
+        r = min(max((w - 1 - (q - p)) // step, 1 - m), k - 1)
+        return q - p + r * step < w and q - p + r * step + x > 0
+    at = p + np.arange(m) * s
+    j = np.clip((at + w - 1 - q) // t, 0, k - 1) * t + q
+    return bool(np.any((j < at + w) & (j + x > at)))
+
+
+def _grad(grad, v, scores, with_grad, *inputs):
+    """The gradient's matrix: a given one (added to), a new one, or none.  inputs:
+    what else the call reads."""
     if grad is None:
         return _like(v, scores) if with_grad else (None, None)
     if not with_grad:
@@ -113,8 +144,19 @@ def _grad(grad, v, scores, with_grad):
         raise RuntimeError("grad must have the shape, dtype and device of scores")
     if (g.row_stride == 1 and g.class_stride != 1) != (v.row_stride == 1 and v.class_stride != 1):
         raise RuntimeError("grad must have its rows or classes next to each other as scores has")
-    if grad.data_ptr() == scores.data_ptr() and scores.numel():
-        raise RuntimeError("grad must not be the scores' memory")
+    # (tensors of other allocations, which most are, cost a tenth of _meet)
+    whole = grad.untyped_storage()
+    lo = whole.data_ptr()
+    hi = lo + whole.nbytes()
+    for t in (scores, *inputs):
+        if t is None:
+            continue
+        at = t.data_ptr()
+        if at >= hi or (at < lo and at + t.untyped_storage().nbytes() <= lo):
+            continue
+        if _meet(grad, t):
+            raise RuntimeError("grad must not share the scores' memory" if t is scores
+                               else "grad must not share memory with an input")
     return grad, g
 
 
@@ -239,7 +281,8 @@ def policy_loss(scores, actions, old_log_prob, advantage, *, weight=None, ref_lo
         C.pointer(rv) if rv is not None else None, low, high, float(kl_coef))
     lib = _lib.load()
     with _on(dev):
-        out, gv = _grad(grad, v, scores, with_grad)
+        out, gv = _grad(grad, v, scores, with_grad, actions, old_log_prob, advantage, weight,
+                        ref_log_prob, ref_scores)
         loss = torch.empty(n, dtype=f32, device=dev)
         log_prob = torch.empty(n, dtype=f32, device=dev)
         kl = None
@@ -271,17 +314,16 @@ def balance_loss(scores, *, top_k=1, mask=None, coef=1.0, grad=None,
     K = scores.shape[1]
     if not 1 <= top_k <= min(8, K):
         raise RuntimeError(f"top_k must be in [1, min(8, n_classes)], got {top_k}")
-    if mask is not None:
-        mask = _vector(mask, "mask", torch.bool, n, dev)
+    at_mask = _vector(mask, "mask", torch.bool, n, dev) if mask is not None else None
     lib = _lib.load()
     with _on(dev):
-        out, gv = _grad(grad, v, scores, with_grad)
+        out, gv = _grad(grad, v, scores, with_grad, mask)
         loss = torch.empty((), dtype=torch.float32, device=dev)
         counts = torch.empty(K, dtype=torch.int64, device=dev)
         prob = torch.empty(K, dtype=torch.float32, device=dev)
         ws, at, size = _workspace("wgbm_balance_loss_workspace", v, dev)
         rc = lib.wgbm_balance_loss(
-            C.byref(v), mask, int(top_k), float(coef), loss.data_ptr(), counts.data_ptr(),
+            C.byref(v), at_mask, int(top_k), float(coef), loss.data_ptr(), counts.data_ptr(),
             prob.data_ptr(), C.byref(gv) if gv is not None else None, int(grad is not None),
             at, size, _lib.current_stream_ptr(dev))
     _lib.check(rc, "balance_loss")
