@@ -298,6 +298,8 @@ typedef struct wgbm_policy_args {
   double clip_high;                /* [0, inf) */
   float kl_coef;
 } wgbm_policy_args;
+/* (what a call with ref_scores takes; without them a call takes none where
+ * wgbm_class_log_probs_workspace returns 0) */
 int64_t wgbm_policy_loss_workspace(const wgbm_scores* scores);
 int wgbm_policy_loss(const wgbm_scores* scores, const wgbm_policy_args* args, float* loss,
                      float* log_prob, float* kl, const wgbm_scores* grad, int32_t accumulate,

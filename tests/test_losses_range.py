@@ -301,3 +301,46 @@ def test_a_gradient_that_shares_memory_is_refused(gpu):
     want = losses.balance_loss(s.clone())
     got = losses.balance_loss(s, grad=both[:, 5:])
     assert torch.equal(got.grad, want.grad) and not both[:, :5].any()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("K", [40_001, 131_072, 131_081])
+def test_policy_workspace_without_a_reference(gpu, K):
+    """Rows that fit registers without a reference's take no working memory then,
+    by torch or by the C entry."""
+    import ctypes as C
+
+    from warpgbm_amd import _lib, losses
+
+    n = 6
+    s = far_rows(n, K, "bf16", "row", 3).cuda()
+    a = torch.zeros(n, dtype=torch.int32, device="cuda")
+    f = torch.ones(n, device="cuda")
+    old = -12 * f
+
+    def allocations(**kw):
+        before = torch.cuda.memory_stats()["allocation.all.allocated"]
+        r = losses.policy_loss(s, a, old, f, **kw)
+        return torch.cuda.memory_stats()["allocation.all.allocated"] - before, r
+
+    long = K > 131_072
+    count, r = allocations()
+    assert count == 3 + long  # the gradient, the loss, the log-probabilities
+    count, with_ref = allocations(ref_scores=s)
+    assert count == 5  # the divergence and the working memory too
+    assert torch.allclose(r.log_prob, with_ref.log_prob, rtol=1e-5, atol=1e-5)
+    if long:
+        return
+    v = losses._matrix(s, "scores")
+    assert gpu.wgbm_policy_loss_workspace(C.byref(v)) > 0
+    args = _lib.PolicyArgs(a.data_ptr(), old.data_ptr(), f.data_ptr(), None, None, None, 0.2, 0.2,
+                           0.0)
+    loss, lp = torch.empty(n, device="cuda"), torch.empty(n, device="cuda")
+    rc = gpu.wgbm_policy_loss(C.byref(v), C.byref(args), loss.data_ptr(), lp.data_ptr(), None, None,
+                              0, None, 0, _lib.current_stream_ptr())
+    assert rc == 0 and torch.equal(loss, r.loss) and torch.equal(lp, r.log_prob)
+    rv = losses._matrix(s, "scores")
+    args.ref_scores = C.pointer(rv)
+    rc = gpu.wgbm_policy_loss(C.byref(v), C.byref(args), loss.data_ptr(), lp.data_ptr(), None, None,
+                              0, None, 0, _lib.current_stream_ptr())
+    assert rc == 1000 and "workspace too small" in gpu.wgbm_last_error().decode()

@@ -94,7 +94,7 @@ int wgbm_class_log_probs_grad(const wgbm_scores* scores, const int32_t* labels, 
 int64_t wgbm_policy_loss_workspace(const wgbm_scores* scores) {
   ScoresView s;
   if (view_of(scores, "scores", &s)) return -1;
-  return (int64_t)policy_workspace(s);
+  return (int64_t)policy_workspace(s, true);
 }
 
 int wgbm_policy_loss(const wgbm_scores* scores, const wgbm_policy_args* a, float* loss,
@@ -121,7 +121,7 @@ int wgbm_policy_loss(const wgbm_scores* scores, const wgbm_policy_args* a, float
   if (s.n == 0) return 0;
   WGBM_REQUIRE(a->actions && a->old_log_prob && a->advantage && loss && log_prob,
                "policy_loss: null pointer");
-  const int64_t need = (int64_t)policy_workspace(s);
+  const int64_t need = (int64_t)policy_workspace(s, a->ref_scores != nullptr);
   WGBM_REQUIRE(need == 0 || (workspace && workspace_bytes >= need),
                "policy_loss: workspace too small");
   PolicyRows p{};

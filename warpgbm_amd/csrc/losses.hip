@@ -418,8 +418,8 @@ static size_t ranges_bytes(const ScoresView& s) {
 size_t log_probs_workspace(const ScoresView& s) {
   return rows_fit(s, false) ? 0 : ranges_bytes(s);
 }
-size_t policy_workspace(const ScoresView& s) {
-  return rows_fit(s, true) ? 0 : sizeof(RowCoef) * (size_t)s.n + ranges_bytes(s);
+size_t policy_workspace(const ScoresView& s, bool ref) {
+  return rows_fit(s, ref) ? 0 : sizeof(RowCoef) * (size_t)s.n + ranges_bytes(s);
 }
 
 }  // namespace wgbm

@@ -54,7 +54,7 @@ LOSS_ROWS(f32);
 LOSS_ROWS(bf16);
 LOSS_ROWS(f16);
 
-size_t policy_workspace(const ScoresView& s);
+size_t policy_workspace(const ScoresView& s, bool ref);
 int policy_loss(const ScoresView& s, const ScoresView& ref, const PolicyRows& g,
                 const ScoresView& out, bool accumulate, void* ws, hipStream_t st);
 

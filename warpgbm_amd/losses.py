@@ -191,10 +191,14 @@ def _bytes_of(entry, dtype, n, K, class_major):
     return nbytes
 
 
+def _bytes(entry, v):
+    return _bytes_of(entry, v.dtype, v.n_rows, v.n_classes,
+                     v.row_stride == 1 and v.class_stride != 1)
+
+
 def _workspace(entry, v, device):
     """Working memory of a call: (tensor or None, address, bytes)."""
-    nbytes = _bytes_of(entry, v.dtype, v.n_rows, v.n_classes,
-                       v.row_stride == 1 and v.class_stride != 1)
+    nbytes = _bytes(entry, v)
     if nbytes == 0:
         return None, None, 0
     t = torch.empty(nbytes, dtype=torch.uint8, device=device)
@@ -288,7 +292,10 @@ def policy_loss(scores, actions, old_log_prob, advantage, *, weight=None, ref_lo
         kl = None
         if ref_scores is not None or ref_log_prob is not None:
             kl = torch.empty(n, dtype=f32, device=dev)
-        ws, at, size = _workspace("wgbm_policy_loss_workspace", v, dev)
+        # (rows whose log-probabilities need none take none without reference scores)
+        ws, at, size = None, None, 0
+        if ref_scores is not None or _bytes("wgbm_class_log_probs_workspace", v):
+            ws, at, size = _workspace("wgbm_policy_loss_workspace", v, dev)
         rc = lib.wgbm_policy_loss(
             C.byref(v), C.byref(args), loss.data_ptr(), log_prob.data_ptr(),
             kl.data_ptr() if kl is not None else None,
