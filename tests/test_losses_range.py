@@ -344,3 +344,29 @@ def test_policy_workspace_without_a_reference(gpu, K):
     rc = gpu.wgbm_policy_loss(C.byref(v), C.byref(args), loss.data_ptr(), lp.data_ptr(), None, None,
                               0, None, 0, _lib.current_stream_ptr())
     assert rc == 1000 and "workspace too small" in gpu.wgbm_last_error().decode()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("order", ["row", "class"])
+@pytest.mark.parametrize("K", [3, 40, 700, 70_001])
+def test_divergence_from_a_reference_without_a_class(gpu, K, order):
+    """It excludes every class: the divergence is infinite, and does no harm where
+    it does not count."""
+    from warpgbm_amd import losses
+
+    n = 5
+    g = torch.Generator().manual_seed(K)
+    s = place(torch.randn((n, K), generator=g), order)
+    rs = place(s.clone(memory_format=torch.contiguous_format) + 0.1, order)
+    rs[2] = -math.inf
+    a, old = torch.zeros(n, dtype=torch.int32).cuda(), torch.full((n,), -2.0).cuda()
+    adv = torch.ones(n).cuda()
+    r = losses.policy_loss(to_gpu(s), a, old, adv, ref_scores=to_gpu(rs), kl_coef=0.5)
+    rest = [0, 1, 3, 4]
+    assert r.kl[2] == math.inf and r.loss[2] == math.inf
+    assert torch.isfinite(r.kl[rest]).all() and torch.isfinite(r.grad[rest]).all()
+    zero = losses.policy_loss(to_gpu(s), a, old, adv, ref_scores=to_gpu(rs))
+    plain = losses.policy_loss(to_gpu(s), a, old, adv)
+    assert zero.kl[2] == math.inf and torch.isfinite(zero.grad).all()
+    # (the frames may differ: the classes are added in another order)
+    assert torch.allclose(zero.loss, plain.loss, rtol=1e-5)

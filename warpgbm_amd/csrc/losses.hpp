@@ -256,7 +256,8 @@ __device__ __forceinline__ PolicyRow policy_row(const RowStats& st, float sa, fl
   float wk = 0.0f, base = 0.0f;
   if (REF) {
     // log p_k - log q_k = (x_k - y_k) + lr, lr = log of the sums' quotient
-    const double lr = log_ratio(st.zr, z);
+    // (a reference without a class: u is infinite, and so is the divergence)
+    const double lr = st.zr == 0.0f ? 0.0 : log_ratio(st.zr, z);
     const double kl = (double)(st.u / z) + lr;
     o.kl = (float)kl;
     base = (float)(lr - kl);  // (log p_k - log q_k - KL) - (x_k - y_k)
