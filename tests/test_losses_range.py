@@ -370,3 +370,55 @@ def test_divergence_from_a_reference_without_a_class(gpu, K, order):
     assert zero.kl[2] == math.inf and torch.isfinite(zero.grad).all()
     # (the frames may differ: the classes are added in another order)
     assert torch.allclose(zero.loss, plain.loss, rtol=1e-5)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("K", [2056, 4104])
+def test_launches_of_more_than_2_to_the_32_threads(gpu, K):
+    """Rows of 256 threads each, more than 2^24 of them: the gradient's of 257 to 512
+    chunks of 16 bytes, the log-probabilities' of 513 to 1024."""
+    from warpgbm_amd import losses
+
+    n, m = (1 << 24) + 9000, 60
+    matrices = 1 if K > 4096 else 2
+    print_case("threads", n, K)
+    torch.cuda.empty_cache()
+    if torch.cuda.mem_get_info()[0] < matrices * 2 * n * K + (4 << 30):
+        pytest.skip("the card's memory is in use")
+    s = torch.zeros((n, K), dtype=torch.bfloat16, device="cuda")
+    gen = torch.Generator(device="cuda").manual_seed(3)
+    # the ends, and rows by where 2^32 threads are and by where parts of 4095 * 1024
+    # rows end
+    at = [0, 4095 * 1024 - m // 2, 4 * 4095 * 1024 - m // 2, (1 << 24) - m // 2, n - m]
+    for i in at:
+        s[i:i + m] = 2 * torch.randn((m, K), generator=gen, device="cuda")
+    a = torch.randint(0, K, (n,), generator=gen, device="cuda", dtype=torch.int32)
+    up = torch.randn(n, generator=gen, device="cuda")
+    f = losses.class_log_probs(s, a)
+    even = torch.ones(n, dtype=torch.bool, device="cuda")
+    for i in at:
+        even[i:i + m] = False
+    flat = f.log_prob[even]
+    assert ((flat + math.log(K)).abs() <= norm_tol(torch.tensor(math.log(K))).item()).all()
+    grad = losses.class_log_probs_grad(s, a, f.norm, up) if matrices == 2 else None
+    for i in at:
+        x, b = s[i:i + m].cpu(), a[i:i + m].cpu().long()
+        L = log_softmax64(x)
+        lp = L.gather(1, b[:, None])[:, 0]
+        check(f.log_prob[i:i + m], lp, norm_tol(lp), "log_prob")
+        if grad is None:
+            continue
+        u = up[i:i + m].cpu().to(F64)
+        want = -L.exp() * u[:, None]
+        want[torch.arange(m), b] = -torch.expm1(lp) * u
+        check(grad[i:i + m], want, grad_tol(want, u.abs(), "bf16"), "gradient")
+    if grad is not None:
+        # (a row of equal scores; every 1009th, so that a part left out shows)
+        some = torch.arange(0, n, 1009, device="cuda")
+        some = some[even[some]]
+        want = -up[some] / K
+        other = (a[some] + 1) % K
+        got = grad[some, other.long()].float()
+        assert ((got - want).abs() <= (2.0 ** -8 + STEPS * U) * want.abs()).all()
+    del s, grad
+    torch.cuda.empty_cache()
