@@ -15,15 +15,14 @@ constexpr int kFinClasses = 4;
 // workgroups' shares of the loss are joined by the last one to arrive, in
 // workgroup order.
 __global__ __launch_bounds__(256) void balance_finish_kernel(BalanceWs w, int32_t groups,
-                                                             int32_t parts, int32_t K, int32_t top_k, float coef,
+                                                             int32_t K, int32_t top_k, float coef,
                                                              BalanceOut o) {
   __shared__ double s_loss[kFinClasses];
   __shared__ bool s_last;
   const int lane = threadIdx.x & 63, c = threadIdx.x >> 6;
   const int32_t k = blockIdx.x * kFinClasses + c;
   const bool in = k < K;
-  const int32_t sums = groups * parts;
-  const float* part = w.part + (int64_t)(in ? k : 0) * sums;
+  const float* part = w.part + (int64_t)(in ? k : 0) * groups;
   const int32_t* count = w.count + (int64_t)(in ? k : 0) * groups;
   const int32_t* rows = w.count + (int64_t)K * groups;
   double a = 0.0;
@@ -34,9 +33,6 @@ __global__ __launch_bounds__(256) void balance_finish_kernel(BalanceWs w, int32_
     n += count[g];
     live += rows[g];
   }
-  // (apart, so that the loads above depend on nothing: 7 us, 15 with a condition)
-#pragma unroll 4
-  for (int32_t g = groups + lane; g < sums; g += 64) a += (double)part[g];
   for (int d = 32; d; d >>= 1) {
     a += __shfl_xor(a, d);
     n += __shfl_xor(n, d);
@@ -125,17 +121,14 @@ static BalanceWs balance_ws(int64_t n, int32_t K, bool cm, void* base) {
     at = (at + b + 255) & ~(size_t)255;
     return (void*)((unsigned char*)base + o);
   };
-  // (at least the workgroups of the first pass: of 64 threads or more, a row each.
-  // Only 512 workgroups or more have several turns: blocks / workgroups + 1, which
-  // is some n / (256 workgroups) + 1 parts of the sums for each.)
+  // (at least the workgroups of the first pass: of 64 threads or more, a row each)
   const size_t g = (size_t)std::min(n, std::min(4 * kLossWaves, balance_few(K)));
-  const size_t sums = g + (n > 512 * (int64_t)kChain ? ((size_t)n + g) / kChain + 1 : 0);
   w.ticket = (uint32_t*)take(4);
   w.scale = (float*)take(4);
   w.share = (float*)take(4 * (size_t)K);
   w.loss_part = (double*)take(8 * ((size_t)K / kFinClasses + 1));
   w.norm = (float2*)take(8 * (size_t)n);
-  w.part = (float*)take(4 * sums * K);
+  w.part = (float*)take(4 * g * K);
   w.count = (int32_t*)take(4 * g * (K + 1));
   if (through_rows(K, cm)) w.rows = take(4 * (size_t)n * K);
   w.bytes = at;
@@ -181,15 +174,15 @@ int balance_loss(const ScoresView& s, const uint8_t* mask, int32_t top_k, float 
     LOSS_TYPES(s.dtype, (transpose<T, true>(s, v, false, st)));
     WGBM_LAUNCH_CHECK();
   }
-  int32_t groups = 0, parts = 0;
+  int32_t groups = 0;
   const auto stats = v.dtype == kF32    ? balance_stats_f32
                      : v.dtype == kBF16 ? balance_stats_bf16
                                         : balance_stats_f16;
-  int r = stats(v, mask, top_k, w, &groups, &parts, st);
+  int r = stats(v, mask, top_k, w, &groups, st);
   if (r) return r;
   hipLaunchKernelGGL(balance_finish_kernel,
                      dim3((unsigned)((s.K + kFinClasses - 1) / kFinClasses)), dim3(256), 0, st, w,
-                     groups, parts, s.K, top_k, coef, o);
+                     groups, s.K, top_k, coef, o);
   WGBM_LAUNCH_CHECK();
   if (!out.data) return 0;
   const auto grad = v.dtype == kF32    ? balance_grad_f32
