@@ -14,7 +14,7 @@ constexpr int kFinClasses = 4;
 // partial sums a class: 7 us for 100 classes, a launch's latency for few).  The
 // workgroups' shares of the loss are joined by the last one to arrive, in
 // workgroup order.
-__global__ __launch_bounds__(256) void balance_finish_kernel(BalanceWs w, int32_t groups,
+__global__ __launch_bounds__(256) void balance_finish_kernel(BalanceWs w, int32_t slots,
                                                              int32_t K, int32_t top_k, float coef,
                                                              BalanceOut o) {
   __shared__ double s_loss[kFinClasses];
@@ -22,13 +22,13 @@ __global__ __launch_bounds__(256) void balance_finish_kernel(BalanceWs w, int32_
   const int lane = threadIdx.x & 63, c = threadIdx.x >> 6;
   const int32_t k = blockIdx.x * kFinClasses + c;
   const bool in = k < K;
-  const float* part = w.part + (int64_t)(in ? k : 0) * groups;
-  const int32_t* count = w.count + (int64_t)(in ? k : 0) * groups;
-  const int32_t* rows = w.count + (int64_t)K * groups;
+  const float* part = w.part + (int64_t)(in ? k : 0) * slots;
+  const int32_t* count = w.count + (int64_t)(in ? k : 0) * slots;
+  const int32_t* rows = w.count + (int64_t)K * slots;
   double a = 0.0;
   int64_t n = 0, live = 0;
 #pragma unroll 4
-  for (int32_t g = lane; g < groups; g += 64) {
+  for (int32_t g = lane; g < slots; g += 64) {
     a += (double)part[g];
     n += count[g];
     live += rows[g];
@@ -121,8 +121,10 @@ static BalanceWs balance_ws(int64_t n, int32_t K, bool cm, void* base) {
     at = (at + b + 255) & ~(size_t)255;
     return (void*)((unsigned char*)base + o);
   };
-  // (at least the workgroups of the first pass: of 64 threads or more, a row each)
-  const size_t g = (size_t)std::min(n, std::min(4 * kLossWaves, balance_few(K)));
+  // (at least the workgroups of the first pass: of 64 threads or more, a row each; of
+  // further launches, which follow 512 workgroups or more, one for kChain rows)
+  const size_t g = (size_t)std::min(n, std::min(4 * kLossWaves, balance_few(K))) +
+                   (n > 512 * (int64_t)kChain ? (size_t)n / kChain : 0);
   w.ticket = (uint32_t*)take(4);
   w.scale = (float*)take(4);
   w.share = (float*)take(4 * (size_t)K);
@@ -174,15 +176,15 @@ int balance_loss(const ScoresView& s, const uint8_t* mask, int32_t top_k, float 
     LOSS_TYPES(s.dtype, (transpose<T, true>(s, v, false, st)));
     WGBM_LAUNCH_CHECK();
   }
-  int32_t groups = 0;
+  int32_t slots = 0;
   const auto stats = v.dtype == kF32    ? balance_stats_f32
                      : v.dtype == kBF16 ? balance_stats_bf16
                                         : balance_stats_f16;
-  int r = stats(v, mask, top_k, w, &groups, st);
+  int r = stats(v, mask, top_k, w, &slots, st);
   if (r) return r;
   hipLaunchKernelGGL(balance_finish_kernel,
                      dim3((unsigned)((s.K + kFinClasses - 1) / kFinClasses)), dim3(256), 0, st, w,
-                     groups, s.K, top_k, coef, o);
+                     slots, s.K, top_k, coef, o);
   WGBM_LAUNCH_CHECK();
   if (!out.data) return 0;
   const auto grad = v.dtype == kF32    ? balance_grad_f32

@@ -6,9 +6,10 @@
 // first, so the scores are read twice: rows in registers (losses_frames.hpp)
 // give the counts, the sums of p and each row's norm; a finishing launch the
 // shares; rows in registers again the gradient.  Workgroups take rows in turn
-// and leave one partial sum a class for each kChain rows of a thread, which the
-// finishing launch joins in float64 in workgroup order: results do not depend on
-// the order of execution, and float32 sums stay short however many rows there are.
+// and leave one partial sum a class, which the finishing launch joins in
+// float64 in workgroup order: results do not depend on the order of execution.
+// Rows that would take a workgroup more than kChain turns are further launches of
+// the first pass, so that float32 sums stay short however many rows there are.
 //
 // 1M x 100 float32 class-major: the first pass 131 us (3.1 TB/s; the eight waves
 // that share 64 rows wait for one another at three reductions), the finish 7, the
@@ -32,15 +33,17 @@ template <typename F>
 constexpr bool kAhead = 2 * F::kWords + 2 * F::N <= 104;
 
 // most rows that a thread adds up in float32: their roundings come to 256 * 2^-24 of
-// the sum at worst (float64 sums would take the registers of two)
+// the sum at worst (float64 sums would take the registers of two, and a loop around
+// the rows' loop, in one launch, costs 500000 x 64 class-major 113 us instead of 105)
 constexpr int32_t kChain = 256;
 
-// part [K][parts][workgroups], count [K + 1][workgroups] (the last: rows that count);
+// The blocks of rows first .. end, to part [K][slots] and count [K + 1][slots] (the
+// last: rows that count), a slot a workgroup from slot0 on;
 // norm: a row's maximum and 1 / sum of e^(s - m) (0: left out)
 template <typename F>
 __global__ __launch_bounds__(F::kMax) void balance_stats_kernel(
-    ScoresView s, const uint8_t* __restrict__ mask, int32_t top_k, int64_t blocks,
-    int32_t parts, float* __restrict__ part, int32_t* __restrict__ count, float2* __restrict__ norm,
+    ScoresView s, const uint8_t* __restrict__ mask, int32_t top_k, int64_t first,
+    int64_t end, int32_t slot0, int32_t slots, float* __restrict__ part, int32_t* __restrict__ count, float2* __restrict__ norm,
     uint32_t* __restrict__ ticket) {
   extern __shared__ int32_t s_count[];  // [K + 1], then [K] floats
   __shared__ float buf[4][F::kBuf];
@@ -50,6 +53,9 @@ __global__ __launch_bounds__(F::kMax) void balance_stats_kernel(
   for (int32_t k = threadIdx.x; k <= K; k += blockDim.x) s_count[k] = 0;
   __syncthreads();
   const F f(s);
+  float acc[F::N];
+#pragma unroll
+  for (int j = 0; j < F::N; ++j) acc[j] = 0.0f;
   // the next rows' loads are in flight while these rows are summed
   typename F::Regs next;
   uint8_t next_want = 1;
@@ -58,99 +64,94 @@ __global__ __launch_bounds__(F::kMax) void balance_stats_kernel(
     if (mask) next_want = mask[row < s.n ? row : s.n - 1];
     f.load(next, s, b);
   };
-  if (kAhead<F>) fetch(blockIdx.x);
-  // a thread adds at most kChain rows in float32; then the workgroup's sums are
-  // written and started again
-  int64_t b = blockIdx.x;
-  for (int32_t part_no = 0; part_no < parts; ++part_no) {
-    float acc[F::N];
+  if (kAhead<F>) fetch(first + blockIdx.x);
+  for (int64_t b = first + blockIdx.x; b < end; b += gridDim.x) {
+    const int64_t row = F::row(b);
+    const bool in = row < s.n;
+    const int64_t i = in ? row : s.n - 1;
+    if (!kAhead<F>) fetch(b);
+    typename F::Regs v = next;
+    const bool want = in && next_want;
+    if (kAhead<F> && b + gridDim.x < end) fetch(b + gridDim.x);
+    f.trim(v);
+    if (!want) f.drop(v);
+    float m = -__builtin_inff();
 #pragma unroll
-    for (int j = 0; j < F::N; ++j) acc[j] = 0.0f;
-    const int64_t stop = b + (int64_t)kChain * gridDim.x, end = stop < blocks ? stop : blocks;
-    for (; b < end; b += gridDim.x) {
-      const int64_t row = F::row(b);
-      const bool in = row < s.n;
-      const int64_t i = in ? row : s.n - 1;
-      if (!kAhead<F>) fetch(b);
-      typename F::Regs v = next;
-      const bool want = in && next_want;
-      if (kAhead<F> && b + gridDim.x < blocks) fetch(b + gridDim.x);
-      f.trim(v);
-      if (!want) f.drop(v);
-      float m = -__builtin_inff();
-#pragma unroll
-      for (int j = 0; j < F::N; ++j) {
-        m = fmaxf(m, F::value(v, j));
-      }
-      m = f.reduce(m, MaxF(), buf[0]);
-      const float ms = safe_max(m);
-      // the exponentials of up to 16 classes stay in registers; more are worked
-      // out again for the sums
-      constexpr bool kKeep = F::N <= 16;
-      float e[kKeep ? F::N : 1], z[2] = {0.0f, 0.0f};
-#pragma unroll
-      for (int j = 0; j < F::N; ++j) {
-        const float x = exp_diff(F::value(v, j) - ms);
-        z[j % 2] += x;
-        if constexpr (kKeep) e[j] = x;
-      }
-      z[0] = f.reduce(z[0] + z[1], AddF(), buf[1]);
-      const bool live = !(z[0] == 0.0f);  // (NaN is live)
-      const float iz = live ? 1.0f / z[0] : 0.0f;
-#pragma unroll
-      for (int j = 0; j < F::N; ++j) {
-        float x;
-        if constexpr (kKeep)
-          x = e[j];
-        else
-          x = exp_diff(F::value(v, j) - ms);
-        acc[j] = fmaf(x, iz, acc[j]);
-      }
-      if (in && f.first_lane()) norm[i] = make_float2(ms, iz);
-      // the best classes one after the other: the largest score after the last
-      // one taken, then the lowest class that has it.  A thread's classes ascend
-      // with its slots, so it looks for its lowest slot (slot numbers are
-      // constants of the instructions, class numbers would each take a register).
-      // Class numbers are exact in float32; a NaN is not after anything.
-      constexpr float kNone = 1e9f;
-      float v0 = __builtin_inff();
-      int32_t c0 = -1;
-      for (int32_t t = 0; t < top_k; ++t) {
-        float best = m;
-        int slot = F::N;
-        if (t == 0) {
-#pragma unroll
-          for (int j = F::N - 1; j >= 0; --j) slot = F::value(v, j) == best ? j : slot;
-        } else {
-          const int taken = f.last_slot(c0);  // of the scores equal to v0
-          best = -__builtin_inff();
-#pragma unroll
-          for (int j = 0; j < F::N; ++j) {
-            const float x = F::value(v, j);
-            if (x < v0 || (x == v0 && j > taken)) best = fmaxf(best, x);
-          }
-          best = f.reduce(best, MaxF(), buf[2]);
-          const int from = best < v0 ? -1 : taken;
-#pragma unroll
-          for (int j = F::N - 1; j >= 0; --j)
-            slot = F::value(v, j) == best && j > from ? j : slot;
-        }
-        const float c = f.reduce(slot < F::N ? (float)f.cls(slot) : kNone, MinF(), buf[3]);
-        if (best > -__builtin_inff() && c < kNone && f.first_lane())
-          atomicAdd(&s_count[(int32_t)c], 1);
-        v0 = best;
-        c0 = (int32_t)c;
-      }
-      if (live && f.first_lane()) atomicAdd(&s_count[K], 1);
+    for (int j = 0; j < F::N; ++j) {
+      m = fmaxf(m, F::value(v, j));
     }
-    f.sum_rows(acc, s_part);
-    __syncthreads();
-    for (int32_t k = threadIdx.x; k < K; k += blockDim.x)
-      part[((int64_t)k * parts + part_no) * gridDim.x + blockIdx.x] = s_part[k];
-    if (part_no + 1 < parts) __syncthreads();  // (s_part is written again)
+    m = f.reduce(m, MaxF(), buf[0]);
+    const float ms = safe_max(m);
+    // the exponentials of up to 16 classes stay in registers; more are worked
+    // out again for the sums
+    constexpr bool kKeep = F::N <= 16;
+    float e[kKeep ? F::N : 1], z[2] = {0.0f, 0.0f};
+#pragma unroll
+    for (int j = 0; j < F::N; ++j) {
+      const float x = exp_diff(F::value(v, j) - ms);
+      z[j % 2] += x;
+      if constexpr (kKeep) e[j] = x;
+    }
+    z[0] = f.reduce(z[0] + z[1], AddF(), buf[1]);
+    const bool live = !(z[0] == 0.0f);  // (NaN is live)
+    const float iz = live ? 1.0f / z[0] : 0.0f;
+    // (slices of 32 classes have 128 registers: unknown to be ms, so that the compiler
+    // works the exponentials out again.  200000 x 400 class-major 483 us, 523 without.)
+    float m2 = ms;
+    if constexpr (!kKeep && F::kSlices) asm volatile("" : "+v"(m2));
+#pragma unroll
+    for (int j = 0; j < F::N; ++j) {
+      float x;
+      if constexpr (kKeep)
+        x = e[j];
+      else
+        x = exp_diff(F::value(v, j) - m2);
+      acc[j] = fmaf(x, iz, acc[j]);
+    }
+    if (in && f.first_lane()) norm[i] = make_float2(ms, iz);
+    // the best classes one after the other: the largest score after the last
+    // one taken, then the lowest class that has it.  A thread's classes ascend
+    // with its slots, so it looks for its lowest slot (slot numbers are
+    // constants of the instructions, class numbers would each take a register).
+    // Class numbers are exact in float32; a NaN is not after anything.
+    constexpr float kNone = 1e9f;
+    float v0 = __builtin_inff();
+    int32_t c0 = -1;
+    for (int32_t t = 0; t < top_k; ++t) {
+      float best = m;
+      int slot = F::N;
+      if (t == 0) {
+#pragma unroll
+        for (int j = F::N - 1; j >= 0; --j) slot = F::value(v, j) == best ? j : slot;
+      } else {
+        const int taken = f.last_slot(c0);  // of the scores equal to v0
+        best = -__builtin_inff();
+#pragma unroll
+        for (int j = 0; j < F::N; ++j) {
+          const float x = F::value(v, j);
+          if (x < v0 || (x == v0 && j > taken)) best = fmaxf(best, x);
+        }
+        best = f.reduce(best, MaxF(), buf[2]);
+        const int from = best < v0 ? -1 : taken;
+#pragma unroll
+        for (int j = F::N - 1; j >= 0; --j)
+          slot = F::value(v, j) == best && j > from ? j : slot;
+      }
+      const float c = f.reduce(slot < F::N ? (float)f.cls(slot) : kNone, MinF(), buf[3]);
+      if (best > -__builtin_inff() && c < kNone && f.first_lane())
+        atomicAdd(&s_count[(int32_t)c], 1);
+      v0 = best;
+      c0 = (int32_t)c;
+    }
+    if (live && f.first_lane()) atomicAdd(&s_count[K], 1);
   }
-  for (int32_t k = threadIdx.x; k <= K; k += blockDim.x)
-    count[(int64_t)k * gridDim.x + blockIdx.x] = s_count[k];
+  f.sum_rows(acc, s_part);
+  __syncthreads();
+  for (int32_t k = threadIdx.x; k <= K; k += blockDim.x) {
+    const int64_t at = (int64_t)k * slots + slot0 + blockIdx.x;
+    if (k < K) part[at] = s_part[k];
+    count[at] = s_count[k];
+  }
 }
 
 template <typename F>
@@ -254,15 +255,18 @@ static inline int64_t balance_few(int32_t K) {
 
 template <typename T>
 int balance_stats(const ScoresView& s, const uint8_t* mask, int32_t top_k, const BalanceWs& w,
-                  int32_t* groups, int32_t* parts, hipStream_t st) {
+                  int32_t* slots, hipStream_t st) {
   balance_frame<T>(s, [&](auto tag, int64_t blocks, int threads) {
     using F = typename decltype(tag)::type;
-    *groups = (int32_t)std::min(blocks, std::min(balance_fill<F>(threads), balance_few(s.K)));
-    const int64_t turns = (blocks + *groups - 1) / *groups;
-    *parts = (int32_t)((turns + kChain - 1) / kChain);
-    hipLaunchKernelGGL((balance_stats_kernel<F>), dim3((unsigned)*groups), dim3(threads),
-                       (2 * (size_t)s.K + 1) * 4, st, s, mask, top_k, blocks, *parts, w.part, w.count,
-                       w.norm, w.ticket);
+    const int64_t groups = std::min(blocks, std::min(balance_fill<F>(threads), balance_few(s.K)));
+    const int64_t each = groups * kChain, last = (blocks - 1) / each;
+    *slots = (int32_t)(last * groups + std::min(groups, blocks - last * each));
+    for (int64_t p = 0; p <= last; ++p) {
+      const int64_t first = p * each, end = std::min(blocks, first + each);
+      hipLaunchKernelGGL((balance_stats_kernel<F>), dim3((unsigned)std::min(groups, end - first)),
+                         dim3(threads), (2 * (size_t)s.K + 1) * 4, st, s, mask, top_k, first, end,
+                         (int32_t)(p * groups), *slots, w.part, w.count, w.norm, w.ticket);
+    }
   });
   WGBM_LAUNCH_CHECK();
   return 0;

@@ -4,8 +4,8 @@
 namespace wgbm {
 
 int balance_stats_f32(const ScoresView& s, const uint8_t* mask, int32_t top_k, const BalanceWs& w,
-                     int32_t* groups, hipStream_t st) {
-  return balance_stats<float>(s, mask, top_k, w, groups, st);
+                     int32_t* slots, hipStream_t st) {
+  return balance_stats<float>(s, mask, top_k, w, slots, st);
 }
 
 int balance_grad_f32(const ScoresView& s, const BalanceWs& w, const ScoresView& out,

@@ -70,14 +70,14 @@ struct BalanceWs {
   float* share;       // [K]
   double* loss_part;  // [K / 4 + 1]
   float2* norm;       // [n]
-  float* part;        // [K][parts][workgroups]
-  int32_t* count;     // [K + 1][workgroups]
+  float* part;        // [K][slots]
+  int32_t* count;     // [K + 1][slots]
   void* rows;         // a row-major copy of the scores, where one is needed
   size_t bytes;
 };
 #define LOSS_BALANCE(t)                                                                          \
   int balance_stats_##t(const ScoresView& s, const uint8_t* mask, int32_t top_k,                 \
-                        const BalanceWs& w, int32_t* groups, int32_t* parts, hipStream_t st);    \
+                        const BalanceWs& w, int32_t* slots, hipStream_t st);                     \
   int balance_grad_##t(const ScoresView& s, const BalanceWs& w, const ScoresView& out,           \
                        bool accumulate, hipStream_t st)
 LOSS_BALANCE(f32);
