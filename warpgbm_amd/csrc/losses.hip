@@ -6,9 +6,9 @@
 // into `splits` ranges whose statistics (running maximum and sums) are kept in
 // the workspace, joined per row, and the gradient is written by an elementwise
 // pass that reads the scores again.  The policy loss of 30000 x 3300 bfloat16
-// class-major takes 391 us (a lane reads two bytes: 128 a wave and load), of 20000
-// x 2000 float32 class-major against a reference 279 (2.9 TB/s of two reads of
-// both and the gradient), of 2000 x 50000 bfloat16 row-major against one 420.
+// class-major takes 392 us (a lane reads two bytes: 128 a wave and load), of 20000
+// x 2000 float32 class-major against a reference 276 (2.9 TB/s of two reads of
+// both and the gradient), of 2000 x 50000 bfloat16 row-major against one 422.
 #include <algorithm>
 
 #include "losses_frames.hpp"

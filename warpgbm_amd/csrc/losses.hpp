@@ -231,6 +231,8 @@ __device__ __forceinline__ PolicyRow policy_row(const RowStats& st, float sa, fl
   }
   const double logp = row_log_prob(st, sa);
   o.logp = (float)logp;
+  // (the ratio's and the divergence's terms are float32, of a float64 difference: its
+  // rounding costs 2^-24 |x| of the ratio, beside the sums' roundings)
   const float x = (float)(logp - (double)old);
   const float ratio = exp_of(x);
   // positive advantages stop above the upper border, negative ones below the

@@ -96,7 +96,7 @@ __global__ __launch_bounds__(F::kMax) void balance_stats_kernel(
     const bool live = !(z[0] == 0.0f);  // (NaN is live)
     const float iz = live ? 1.0f / z[0] : 0.0f;
     // (slices of 32 classes have 128 registers: unknown to be ms, so that the compiler
-    // works the exponentials out again.  200000 x 400 class-major 483 us, 523 without.)
+    // works the exponentials out again.  200000 x 400 class-major 440 us, 523 without.)
     float m2 = ms;
     if constexpr (!kKeep && F::kSlices) asm volatile("" : "+v"(m2));
 #pragma unroll
@@ -243,7 +243,8 @@ static void balance_frame(const ScoresView& s, Fn fn) {
 // workgroups of the two passes: 16 waves a CU (with 64, the class-major 1M x 10
 // takes 45 us instead of 37 and a gate's 65536 x 64 32 instead of 26: more
 // partial sums), but 64 where the waves of a workgroup wait for one another
-// (200000 x 400 class-major 721 us with 16, 603 with 64); and
+// (200000 x 400 class-major, 13 waves each, 505 us with 16, 421 with 64; 1M x 100,
+// eight waves, 288 and 318: one rule for both is a compromise); and
 // fewer partial sums where there are many classes
 template <typename F>
 static int64_t balance_fill(int threads) {

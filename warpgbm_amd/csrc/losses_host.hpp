@@ -35,8 +35,9 @@ int class_log_probs_grad(const ScoresView& s, const int32_t* label, const float*
 // Whether rows fit the registers of the threads that share them (one launch,
 // losses_rows.hpp).  Class-major: 16 waves' slices of 32 classes.  Row-major:
 // 1024 threads of 16 chunks of 16 bytes (64 of the 128 registers that a thread
-// has), of 4 with a second matrix: with 8 the registers no longer hold the
-// passes (2000 x 50000 bfloat16 against a reference 882 us, the ranged path 420).
+// has), of 4 with a second matrix.  (8 with a second matrix would fit now that the
+// sums against a reference are pinned: 2000 x 50000 bfloat16 220 us, the ranged path,
+// which takes them, 422.)
 // Shorter rows than a chunk: a thread each.
 inline bool rows_fit(const ScoresView& s, bool ref) {
   const int32_t VE = s.dtype == kF32 ? 4 : 8;

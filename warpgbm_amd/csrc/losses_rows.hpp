@@ -56,7 +56,7 @@ __device__ __forceinline__ RowStats frame_stats(const F& f, typename F::Regs& s,
 }
 
 // log p_a = s_a - log sum_k e^(s_k), and the row's norm.  1M x 10 float32
-// class-major 12 us (56 MB, 4.8 TB/s); one row of 50001 float32 6.7 us, a
+// class-major 12 us (56 MB, 4.8 TB/s); one row of 50001 float32 6.8 us, a
 // workgroup's latency (two reductions between 1024 threads).
 template <typename F>
 __global__ __launch_bounds__(F::kMax) void log_probs_frame_kernel(
@@ -97,7 +97,7 @@ __global__ __launch_bounds__(F::kMax) void log_probs_grad_frame_kernel(
 }
 
 // the clipped policy loss and its gradient (policy_row).  8191 x 16001 bfloat16
-// 110 us (524 MB, 4.75 TB/s, vector instructions in 69% of the cycles); 1M x 10
+// 110 us (524 MB, 4.75 TB/s, vector instructions in 75% of the cycles); 1M x 10
 // float32 class-major against a reference's scores 37 (4 TB/s).
 template <typename F, bool REF>
 __global__ __launch_bounds__(F::kMax) void policy_frame_kernel(ScoresView s, ScoresView ref,
