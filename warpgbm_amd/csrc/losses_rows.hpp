@@ -30,9 +30,16 @@ __device__ __forceinline__ RowStats frame_stats(const F& f, typename F::Regs& s,
   if (REF && F::kHide) f.hide(r);
   // four sums a thread: shorter chains of additions, and fewer roundings
   float z[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+  // Float16 scores that are converted anew for this pass: s log2(e) - m2 takes them as
+  // they are (v_fma_mix_f32).  m2 is m log2(e) rounded, off by 2^-8 at most, as m is at
+  // most 65504; the sum, 2^(m log2(e) - m2) times too large, is set right below.
+  // Log-probabilities of 30000 x 3300 43 us, 47 with the difference first.
+  constexpr bool kScaled = !REF && F::kHide && __is_same(typename F::T, _Float16);
+  const float m2 = m * kLog2e;
 #pragma unroll
   for (int j = 0; j < F::N; ++j) {
-    const float x = F::value(s, j) - m, e = exp_diff(x);
+    const float x = F::value(s, j) - m;
+    const float e = kScaled ? exp2_f32(fmaf(F::value(s, j), kLog2e, -m2)) : exp_diff(x);
     z[j % 4] += f.cls(j) == label ? 0.0f : e;
     if (REF) {
       const float y = F::value(r, j) - mr;
@@ -48,6 +55,7 @@ __device__ __forceinline__ RowStats frame_stats(const F& f, typename F::Regs& s,
   if (F::kHide) f.hide(s);
   if (REF && F::kHide) f.hide(r);
   a.z = f.reduce((z[0] + z[1]) + (z[2] + z[3]), AddF(), buf[2]);
+  if (kScaled) a.z *= exp2_f32(-fmaf(m, kLog2e, -m2));
   if (REF) {
     a.zr = f.reduce(a.zr, AddF(), buf[3]);
     a.u = f.reduce(a.u, AddF(), buf[4]);
