@@ -284,9 +284,9 @@ int wgbm_class_log_probs_grad(const wgbm_scores* scores, const int32_t* labels, 
  * [0, n_classes) is not read: loss, log_prob, kl and gradient 0.  A class of
  * probability 0 takes no part in the exact KL; one that only the reference
  * excludes makes it infinite, as do finite scores of a reference so low that the
- * sum of e^(s_k - max s) (log p_k - log q_k) passes float32's range.  kl may be NULL; grad NULL: no gradient;
- * accumulate != 0 adds to grad instead of overwriting it.  grad must not
- * overlap an input. */
+ * sum of e^(s_k - max s) (log p_k - log q_k) passes float32's range.  kl may be
+ * NULL; grad NULL: no gradient; accumulate != 0 adds to grad instead of
+ * overwriting it.  grad must not overlap an input. */
 typedef struct wgbm_policy_args {
   const int32_t* actions;          /* [n_rows] */
   const float* old_log_prob;       /* [n_rows] */

@@ -69,11 +69,12 @@ __device__ __forceinline__ T from_f32(float v) {
 // both small), 0 at the maximum whatever its size, and -inf at worst.  (One fused
 // multiply-add, s log2(e) - fl(m log2(e)), would save an instruction a class but
 // leaves m log2(e)'s rounding in the power: 10^-3 at a maximum of 10^5, a factor
-// of 2^440 at 10^10; both forms take the same time, 8191 x 16001 bfloat16 110 us, 1M x
-// 10 float32 against a reference 37.)  The difference's, the product's and log2(e)'s roundings
-// cost 2.3 |x| log2(e) 2^-24 ln(2) of the value, that is less than 2^-24 of the
-// row's largest exponential (|x| e^-|x| has its maximum 1/e): what a softmax's sums
-// and gradients are rounded by anyway.
+// of 2^440 at 10^10.  Both forms take the same time where memory bounds them, 8191 x
+// 16001 bfloat16 110 us, 1M x 10 float32 against a reference 37; long rows against a
+// reference lose 3 to 7%.)  The difference's, the product's and log2(e)'s roundings
+// cost 2.3 |x| 2^-24 of the value, that is less than 2^-24 of the row's largest
+// exponential (|x| e^-|x| has its maximum 1/e): what a softmax's sums and gradients are
+// rounded by anyway.
 constexpr float kLog2e = 1.44269504088896340736f;
 constexpr double kLn2 = 0.693147180559945309417;
 __device__ __forceinline__ float exp2_f32(float h) { return __builtin_amdgcn_exp2f(h); }

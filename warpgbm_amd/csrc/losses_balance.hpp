@@ -38,13 +38,13 @@ constexpr bool kAhead = 2 * F::kWords + 2 * F::N <= 104;
 constexpr int32_t kChain = 256;
 
 // The blocks of rows first .. end, to part [K][slots] and count [K + 1][slots] (the
-// last: rows that count), a slot a workgroup from slot0 on;
-// norm: a row's maximum and 1 / sum of e^(s - m) (0: left out)
+// last: rows that count), a slot a workgroup from slot0 on; norm: a row's maximum
+// and 1 / sum of e^(s - m) (0: left out)
 template <typename F>
 __global__ __launch_bounds__(F::kMax) void balance_stats_kernel(
-    ScoresView s, const uint8_t* __restrict__ mask, int32_t top_k, int64_t first,
-    int64_t end, int32_t slot0, int32_t slots, float* __restrict__ part, int32_t* __restrict__ count, float2* __restrict__ norm,
-    uint32_t* __restrict__ ticket) {
+    ScoresView s, const uint8_t* __restrict__ mask, int32_t top_k, int64_t first, int64_t end,
+    int32_t slot0, int32_t slots, float* __restrict__ part, int32_t* __restrict__ count,
+    float2* __restrict__ norm, uint32_t* __restrict__ ticket) {
   extern __shared__ int32_t s_count[];  // [K + 1], then [K] floats
   __shared__ float buf[4][F::kBuf];
   const int32_t K = s.K;
