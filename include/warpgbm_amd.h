@@ -318,6 +318,82 @@ int wgbm_balance_loss(const wgbm_scores* scores, const uint8_t* mask, int32_t to
                       float* loss, int64_t* counts, float* prob, const wgbm_scores* grad,
                       int32_t accumulate, void* workspace, int64_t workspace_bytes, void* stream);
 
+/* Lists of a row's classes: at most WGBM_MAX_LIST of them.  Temperatures are in [1e-6,
+ * 1e6] and divide the scores. */
+#define WGBM_MAX_LIST 64
+
+/* With p = softmax(scores[i] / temperature): the top_k classes of largest score, in
+ * descending order, the lower class first among equal scores, with log p of each
+ * (classes, log_prob [n_rows][top_k]; -1 and -inf where the row has fewer classes;
+ * NaN is never taken); the entropy of p; log p of the row's label (labels NULL: not
+ * written; 0 for a label outside [0, n_classes)); and norm [n_rows][3]: the row's
+ * largest score m, log(sum exp((s - m) / temperature)) and sum p (m - s) /
+ * temperature.  top_k in [0, min(WGBM_MAX_LIST, n_classes)]; with 0 classes and
+ * log_prob are not written.  A row without a class has entropy 0, label log-probability
+ * 0 and norm (-inf, 0, 0). */
+int64_t wgbm_class_alternatives_workspace(const wgbm_scores* scores);
+int wgbm_class_alternatives(const wgbm_scores* scores, const int32_t* labels, int32_t top_k,
+                            float temperature, int32_t* classes, float* log_prob, float* entropy,
+                            float* label_log_prob, float* norm, void* workspace,
+                            int64_t workspace_bytes, void* stream);
+
+/* Gradient with respect to the scores of
+ *   grad_label_log_prob[i] log p[label] + sum_j grad_log_prob[i][j] log p[classes[i][j]]
+ *     + grad_entropy[i] entropy
+ * (each term absent where its pointers are NULL or list_length is 0), from the norm
+ * that wgbm_class_alternatives wrote at the same temperature.  Entries outside [0,
+ * n_classes) do not count; a class that is listed twice counts twice.  Rows without a
+ * class, and rows whose upstream gradients are all 0, have gradient 0 (with accumulate
+ * they keep what they hold).  grad as for the policy loss. */
+typedef struct wgbm_alternatives_grad_args {
+  const float* norm;                  /* [n_rows][3] */
+  const int32_t* labels;              /* [n_rows] or NULL */
+  const float* grad_label_log_prob;   /* [n_rows], with labels */
+  const int32_t* classes;             /* [n_rows][list_length], rows classes_stride apart */
+  int64_t classes_stride;
+  const float* grad_log_prob;         /* the same, rows grad_stride apart */
+  int64_t grad_stride;
+  int32_t list_length;                /* [0, WGBM_MAX_LIST] */
+  const float* grad_entropy;          /* [n_rows] or NULL */
+  float temperature;
+} wgbm_alternatives_grad_args;
+int64_t wgbm_class_alternatives_grad_workspace(const wgbm_scores* scores);
+int wgbm_class_alternatives_grad(const wgbm_scores* scores,
+                                 const wgbm_alternatives_grad_args* args, const wgbm_scores* grad,
+                                 int32_t accumulate, void* workspace, int64_t workspace_bytes,
+                                 void* stream);
+
+/* Divergence of p = softmax(scores[i] / T), T = temperature, from a teacher's listed
+ * classes c_j with logits l_j, per row, and its gradient:
+ *   loss = weight T^2 (sum_j q_j log(q_j / p_cj) + Q log(Q / P))
+ * with q_j = exp(l_j / T - log_norm[i]), Q = 1 - sum_j q_j the teacher's share of all
+ * other classes and P the scores' (rest != 0), or q = softmax(l / T) over the list and
+ * Q = 0 (rest == 0).  log_norm[i] is log(sum over all the teacher's classes of
+ * exp(l / T)); log_norm NULL: log_norm_all for every row (0: the logits are T times
+ * log-probabilities).  A Q below 2^-20 is taken as rounding, and as 0.
+ * Entries outside [0, n_classes) are unused; a class that is listed again counts the
+ * first time only.  Listed classes of score -inf do not count, nor does Q where no
+ * other class has a score above -inf: what is left of q and Q is scaled to sum 1.
+ * A row of weight 0 (weight NULL: 1) is not read; one without a class or of whose
+ * list nothing counts is left out: loss and gradient 0.  grad as for the policy loss
+ * (NULL: none). */
+typedef struct wgbm_distill_args {
+  const int32_t* classes;  /* [n_rows][list_length], rows classes_stride apart */
+  int64_t classes_stride;
+  const float* logits;     /* the same, rows logits_stride apart */
+  int64_t logits_stride;
+  int32_t list_length;     /* [1, WGBM_MAX_LIST] */
+  int32_t rest;
+  const float* log_norm;   /* [n_rows] or NULL */
+  float log_norm_all;
+  const float* weight;     /* [n_rows] or NULL */
+  float temperature;
+} wgbm_distill_args;
+int64_t wgbm_distill_loss_workspace(const wgbm_scores* scores);
+int wgbm_distill_loss(const wgbm_scores* scores, const wgbm_distill_args* args, float* loss,
+                      const wgbm_scores* grad, int32_t accumulate, void* workspace,
+                      int64_t workspace_bytes, void* stream);
+
 /* Preference loss of pairs of sequences of rows (paired log ratios): with
  * u_i = log_prob[i] - ref_log_prob[i] and U_s the sum of u over the rows
  * sequence_start[s] .. sequence_start[s + 1] of sequence s (none: U_s = 0),

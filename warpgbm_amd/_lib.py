@@ -52,6 +52,12 @@ SIGNATURES = {
     "wgbm_policy_loss": (C.c_int, [_p, _p, _p, _p, _p, _p, _i32, _p, _i64, _p]),
     "wgbm_balance_loss_workspace": (_i64, [_p]),
     "wgbm_balance_loss": (C.c_int, [_p, _p, _i32, _f32, _p, _p, _p, _p, _i32, _p, _i64, _p]),
+    "wgbm_class_alternatives_workspace": (_i64, [_p]),
+    "wgbm_class_alternatives": (C.c_int, [_p, _p, _i32, _f32, _p, _p, _p, _p, _p, _p, _i64, _p]),
+    "wgbm_class_alternatives_grad_workspace": (_i64, [_p]),
+    "wgbm_class_alternatives_grad": (C.c_int, [_p, _p, _p, _i32, _p, _i64, _p]),
+    "wgbm_distill_loss_workspace": (_i64, [_p]),
+    "wgbm_distill_loss": (C.c_int, [_p, _p, _p, _p, _i32, _p, _i64, _p]),
     "wgbm_preference_loss_workspace": (_i64, [_p]),
     "wgbm_preference_loss": (C.c_int, [_p, _p, _p, _p, _p, _i64, _p]),
     "wgbm_engine_create": (C.c_int, [C.POINTER(_p), _p]),
@@ -122,6 +128,36 @@ class PolicyArgs(C.Structure):
         ("clip_low", C.c_double),
         ("clip_high", C.c_double),
         ("kl_coef", _f32),
+    ]
+
+
+class AlternativesGradArgs(C.Structure):
+    _fields_ = [
+        ("norm", _p),
+        ("labels", _p),
+        ("grad_label_log_prob", _p),
+        ("classes", _p),
+        ("classes_stride", _i64),
+        ("grad_log_prob", _p),
+        ("grad_stride", _i64),
+        ("list_length", _i32),
+        ("grad_entropy", _p),
+        ("temperature", _f32),
+    ]
+
+
+class DistillArgs(C.Structure):
+    _fields_ = [
+        ("classes", _p),
+        ("classes_stride", _i64),
+        ("logits", _p),
+        ("logits_stride", _i64),
+        ("list_length", _i32),
+        ("rest", _i32),
+        ("log_norm", _p),
+        ("log_norm_all", _f32),
+        ("weight", _p),
+        ("temperature", _f32),
     ]
 
 

@@ -1,0 +1,454 @@
+// Alternatives of a row's scores: with x = (s - m) / tau, m = max s,
+//   lse = log sum e^x,  down = sum p (-x),  p = e^(x - lse)
+//   entropy = lse + down, log-probability of class c = x_c - lse
+// for the row's label and its k best classes (the lower class first among equal
+// scores).  Both terms of the entropy are sums of numbers >= 0, and lse is
+// log1p of the sum without the largest term, 1: nothing cancels, for a row sure
+// of its class as for an even one.  Rows are read once into registers
+// (losses_frames.hpp).
+#pragma once
+#include "losses_lists.hpp"
+
+namespace wgbm {
+
+// a row's sums: of e^x over the scores below the maximum; of e^x h, h = x log2(e);
+// and how many scores equal the maximum
+struct AltSums {
+  float z, u, ties;
+};
+__device__ __forceinline__ void add_score(AltSums& a, float v, float m, float ms, float c) {
+  const float h = (v - ms) * c, e = exp2_f32(h);
+  a.z += v == m ? 0.0f : e;
+  a.ties += v == m ? 1.0f : 0.0f;
+  a.u = fmaf(e, fmaxf(h, kLowPower), a.u);
+}
+
+struct AltRow {
+  float m;      // the maximum, 0 for a row without a class
+  double lse;
+  float down;
+  bool live;    // (a row of NaN is live: it shows in the results)
+};
+__device__ __forceinline__ AltRow alt_row(const AltSums& a, float m) {
+  AltRow o;
+  o.live = m > -__builtin_inff() || a.z != a.z;
+  o.m = safe_max(m);
+  const float rest = a.z + (a.ties - 1.0f);
+  o.lse = log_1p(rest);
+  o.down = -a.u * (float)kLn2 / (1.0f + rest);
+  return o;
+}
+__device__ __forceinline__ float alt_log_prob(const AltRow& r, const AltRows& g, float v) {
+  return (float)(((double)v - (double)r.m) * g.inv_tau - r.lse);
+}
+// the row's results but for its alternatives, by one thread
+__device__ __forceinline__ void write_alt_row(const AltRow& r, const AltRows& g, int64_t i,
+                                              int32_t label, float sa) {
+  g.entropy[i] = r.live ? (float)(r.lse + (double)r.down) : 0.0f;
+  g.norm[3 * i] = r.live ? r.m : -__builtin_inff();
+  g.norm[3 * i + 1] = r.live ? (float)r.lse : 0.0f;
+  g.norm[3 * i + 2] = r.live ? r.down : 0.0f;
+  if (g.label) g.label_log_prob[i] = r.live && label >= 0 ? alt_log_prob(r, g, sa) : 0.0f;
+}
+__device__ __forceinline__ void write_alternative(const AltRow& r, const AltRows& g, int64_t i,
+                                                  int t, int32_t cls, float v) {
+  const int64_t at = i * g.k + t;
+  g.classes[at] = cls;
+  g.log_prob[at] = cls >= 0 ? alt_log_prob(r, g, v) : -__builtin_inff();
+}
+
+// ---------------------------------------------------------------------------
+// Few classes a row, or few alternatives: the best classes one after the other.
+// A thread's classes ascend with its slots, so it looks for its lowest slot
+// (as in the balance loss); each turn costs some eight instructions a slot and
+// two reductions.
+// ---------------------------------------------------------------------------
+template <typename F>
+__global__ __launch_bounds__(F::kMax) void alternatives_turns_kernel(ScoresView s, AltRows g) {
+  __shared__ float buf[4][F::kBuf];
+  const F f(s);
+  const int64_t row = F::row(blockIdx.x);
+  const bool in = row < s.n;
+  if (!F::kBarrier && !in) return;
+  const int64_t i = in ? row : s.n - 1;
+  typename F::Regs v;
+  f.load(v, s, blockIdx.x);
+  const int32_t lab = row_label(g.label, i, s.K);
+  const float sa = lab >= 0 ? score_at<typename F::T>(s, i, lab) : 0.0f;
+  f.trim(v);
+  float m = -__builtin_inff();
+#pragma unroll
+  for (int j = 0; j < F::N; ++j) m = fmaxf(m, F::value(v, j));
+  m = f.reduce(m, MaxF(), buf[0]);
+  const float ms = safe_max(m);
+  AltSums a{0.0f, 0.0f, 0.0f};
+#pragma unroll
+  for (int j = 0; j < F::N; ++j) add_score(a, F::value(v, j), m, ms, g.scale);
+  a.z = f.reduce(a.z, AddF(), buf[1]);
+  a.u = f.reduce(a.u, AddF(), buf[2]);
+  a.ties = f.reduce(a.ties, AddF(), buf[3]);
+  const AltRow r = alt_row(a, m);
+  const bool write = in && f.first_lane();
+  if (write) write_alt_row(r, g, i, lab, sa);
+  constexpr float kNone = 1e9f;  // (class numbers are exact in float32)
+  float v0 = __builtin_inff();
+  int32_t c0 = -1;
+  for (int32_t t = 0; t < g.k; ++t) {
+    float best = m;
+    int slot = F::N;
+    if (t == 0) {
+#pragma unroll
+      for (int j = F::N - 1; j >= 0; --j) slot = F::value(v, j) == best ? j : slot;
+    } else {
+      const int taken = f.last_slot(c0);  // of the scores equal to v0
+      best = -__builtin_inff();
+#pragma unroll
+      for (int j = 0; j < F::N; ++j) {
+        const float x = F::value(v, j);
+        if (x < v0 || (x == v0 && j > taken)) best = fmaxf(best, x);
+      }
+      best = f.reduce(best, MaxF(), buf[1]);
+      const int from = best < v0 ? -1 : taken;
+#pragma unroll
+      for (int j = F::N - 1; j >= 0; --j) slot = F::value(v, j) == best && j > from ? j : slot;
+    }
+    const float c = f.reduce(slot < F::N ? (float)f.cls(slot) : kNone, [](float x, float y) {
+      return fminf(x, y);
+    }, buf[0]);
+    const bool found = best > -__builtin_inff() && c < kNone;
+    if (write) write_alternative(r, g, i, t, found ? (int32_t)c : -1, best);
+    v0 = best;
+    c0 = found ? (int32_t)c : s.K - 1;
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Longer rows: candidates.  The k-th largest of the maxima of 128 or more parts of
+// the row is no larger than the k-th largest score, so the classes from there on
+// (some more than k in rows without an order) are copied to LDS, and a
+// candidate's place is the number of candidates with a larger key.  Rows with
+// more candidates than the copy holds (many equal scores) take their best
+// classes in turns.
+// ---------------------------------------------------------------------------
+// a number no larger than the k-th largest of the wave's M keys a lane (its upper
+// 16 bits: 2^-7 of the value), as a score
+template <int M>
+__device__ __forceinline__ float kth_at_least(const uint32_t (&key)[M], int32_t k) {
+  uint32_t t = 0;
+  for (int b = 31; b >= 16; --b) {
+    const uint32_t next = t | 1u << b;
+    int n = 0;
+#pragma unroll
+    for (int j = 0; j < M; ++j) n += __popcll(__ballot(key[j] >= next));
+    if (n >= k) t = next;
+  }
+  // (fewer than k parts with a class: every class is a candidate)
+  return t <= kOrderNegInf ? -__FLT_MAX__ : score_of(t);
+}
+
+__device__ __forceinline__ uint64_t wave_max_key(uint64_t key) {
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const uint64_t other = (uint64_t)__shfl_xor((unsigned long long)key, o);
+    key = other > key ? other : key;
+  }
+  return key;
+}
+
+// the places of n candidates, by the thread group's threads t, t + step, ...
+__device__ __forceinline__ void rank_candidates(const uint64_t* cand, int n, int t, int step,
+                                                const AltRow& r, const AltRows& g, int64_t i) {
+  for (int q = t; q < n || q < g.k; q += step) {
+    if (q >= n) {  // (the row has fewer classes)
+      write_alternative(r, g, i, q, -1, 0.0f);
+      continue;
+    }
+    const uint64_t mine = cand[q];
+    int place = 0;
+    for (int o = 0; o < n; ++o) place += cand[o] > mine;
+    if (place < g.k)
+      write_alternative(r, g, i, place, class_of(mine), score_of((uint32_t)(mine >> 32)));
+  }
+}
+
+// workgroup's or wave's largest key below `below` (0: none), best(below) being a
+// thread's
+template <int NW, typename Fn>
+__device__ __forceinline__ uint64_t next_key(uint64_t below, uint64_t* buf, Fn best) {
+  uint64_t key = wave_max_key(best(below));
+  if (NW == 1) return key;
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) buf[threadIdx.x >> 6] = key;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < NW; ++w) key = buf[w] > key ? buf[w] : key;
+  return key;
+}
+
+template <typename F>
+__global__ __launch_bounds__(F::kMax) void alternatives_candidates_kernel(ScoresView s,
+                                                                          AltRows g) {
+  constexpr int NW = F::G / 64, R = F::kRows, kHold = NW == 1 ? 256 : 512;
+  static_assert(F::G >= 64, "a row is a wave's or a workgroup's");
+  __shared__ uint64_t cand[R][kHold];
+  __shared__ uint32_t part[NW == 1 ? 1 : 256];
+  __shared__ uint64_t key_buf[NW];
+  __shared__ float buf[3 * F::kBuf], most[F::kBuf];
+  __shared__ int count;
+  __shared__ float from_share;
+  const F f(s);
+  const int64_t row = F::row(blockIdx.x);
+  if (row >= s.n) return;  // (a whole wave or workgroup)
+  const int64_t i = row;
+  typename F::Regs v;
+  f.load(v, s, blockIdx.x);
+  const int32_t lab = row_label(g.label, i, s.K);
+  const float sa = lab >= 0 ? score_at<typename F::T>(s, i, lab) : 0.0f;
+  if (NW > 1 && threadIdx.x == 0) count = 0;
+  f.trim(v);
+  float half[2] = {-__builtin_inff(), -__builtin_inff()};
+#pragma unroll
+  for (int j = 0; j < F::N; ++j) half[j >= F::N / 2] = fmaxf(half[j >= F::N / 2], F::value(v, j));
+  float m = fmaxf(half[0], half[1]);
+  float from = 0.0f;
+  if constexpr (NW == 1) {
+    if (g.k > 0) {
+      const uint32_t key[2] = {order_of(half[0]), order_of(half[1])};
+      from = kth_at_least<2>(key, g.k);
+    }
+  } else {
+    // 256 parts: a thread's classes, or those of four threads
+    const float four = NW > 4 ? lanes_reduce<4>(m, MaxF()) : m;
+    if (NW <= 4 || (threadIdx.x & 3) == 0)
+      part[NW > 4 ? threadIdx.x >> 2 : threadIdx.x] = order_of(four);
+  }
+  m = f.reduce(m, MaxF(), most);
+  const float ms = safe_max(m);
+  if (NW > 1 && threadIdx.x < 64 && g.k > 0) {
+    const uint32_t key[4] = {part[threadIdx.x], part[threadIdx.x + 64], part[threadIdx.x + 128],
+                             part[threadIdx.x + 192]};
+    const float t = kth_at_least<4>(key, g.k);
+    if (threadIdx.x == 0) from_share = t;
+  }
+  if (F::kHide) f.hide(v);
+  AltSums a[2] = {};
+#pragma unroll
+  for (int j = 0; j < F::N; ++j) add_score(a[j % 2], F::value(v, j), m, ms, g.scale);
+  float sum[3] = {a[0].z + a[1].z, a[0].u + a[1].u, a[0].ties + a[1].ties};
+  f.template reduce_all<3>(sum, AddF(), buf);
+  const AltRow r = alt_row(AltSums{sum[0], sum[1], sum[2]}, m);
+  if (f.first_lane()) write_alt_row(r, g, i, lab, sa);
+  if (g.k == 0) return;
+  if (F::kHide) f.hide(v);
+  uint64_t* const list = cand[threadIdx.x / F::G];
+  int n = 0;
+  if constexpr (NW == 1) {
+#pragma unroll
+    for (int j = 0; j < F::N; ++j) {
+      const float x = F::value(v, j);
+      const uint64_t who = __ballot(x >= from);
+      if (who == 0) continue;
+      const int at = n + __popcll(who & ((1ull << (threadIdx.x & 63)) - 1));
+      if (x >= from && at < kHold) list[at] = key_of(x, f.cls(j));
+      n += __popcll(who);
+    }
+  } else {
+    from = from_share;
+    if (half[0] >= from || half[1] >= from) {
+#pragma unroll
+      for (int j = 0; j < F::N; ++j) {
+        const float x = F::value(v, j);
+        if (x >= from) {
+          const int at = atomicAdd(&count, 1);
+          if (at < kHold) list[at] = key_of(x, f.cls(j));
+        }
+      }
+    }
+    __syncthreads();
+    n = count;
+  }
+  if (n <= kHold) {
+    // (a wave's own list: its writes are done before it reads)
+    if (NW == 1) __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");
+    rank_candidates(list, n, threadIdx.x % F::G, F::G, r, g, i);
+    return;
+  }
+  uint64_t below = ~0ull;
+  for (int32_t t = 0; t < g.k; ++t) {
+    below = next_key<NW>(below, key_buf, [&](uint64_t under) {
+      uint64_t best = 0;
+#pragma unroll
+      for (int j = 0; j < F::N; ++j) {
+        const float x = F::value(v, j);
+        const uint64_t key = key_of(x, f.cls(j));
+        if (x > -__builtin_inff() && key < under && key > best) best = key;
+      }
+      return best;
+    });
+    if (f.first_lane())
+      write_alternative(r, g, i, t, below ? class_of(below) : -1,
+                        score_of((uint32_t)(below >> 32)));
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Rows longer than a workgroup's registers: a workgroup a row, tile after tile,
+// twice (the maximum and where candidates begin; then sums and candidates)
+// ---------------------------------------------------------------------------
+template <typename T>
+using AltTile = RowFrame<T, 1024, 4>;
+
+template <typename T>
+__global__ __launch_bounds__(1024) void alternatives_long_kernel(ScoresView s, AltRows g,
+                                                                 int32_t span, int32_t tiles) {
+  using F = AltTile<T>;
+  constexpr int NW = 16, kHold = 1024;
+  __shared__ uint64_t list[kHold];
+  __shared__ uint32_t part[256];
+  __shared__ uint64_t key_buf[NW];
+  __shared__ float buf[3 * F::kBuf], most[F::kBuf];
+  __shared__ int count;
+  __shared__ float from_share;
+  const int64_t i = blockIdx.x;
+  const int32_t lab = row_label(g.label, i, s.K);
+  const float sa = lab >= 0 ? score_at<T>(s, i, lab) : 0.0f;
+  if (threadIdx.x == 0) count = 0;
+  float m = -__builtin_inff();
+  for (int32_t t = 0; t < tiles; ++t) {
+    const ScoresView p = tile_of(s, span, t);
+    const F f(p);
+    typename F::Regs v;
+    f.load(v, p, i);
+    f.trim(v);  // (a class counts in one part only)
+#pragma unroll
+    for (int j = 0; j < F::N; ++j) m = fmaxf(m, F::value(v, j));
+  }
+  const float own = m;
+  const float four = lanes_reduce<4>(m, MaxF());
+  if ((threadIdx.x & 3) == 0) part[threadIdx.x >> 2] = order_of(four);
+  const F whole(s);
+  m = whole.reduce(m, MaxF(), most);
+  const float ms = safe_max(m);
+  if (threadIdx.x < 64 && g.k > 0) {
+    const uint32_t key[4] = {part[threadIdx.x], part[threadIdx.x + 64], part[threadIdx.x + 128],
+                             part[threadIdx.x + 192]};
+    const float t = kth_at_least<4>(key, g.k);
+    if (threadIdx.x == 0) from_share = t;
+  }
+  __syncthreads();
+  const float from = g.k > 0 ? from_share : __builtin_inff();
+  const bool some = g.k > 0 && own >= from;
+  // (the tiles' sums are joined in float64: a row may have 2^24 classes)
+  double z = 0.0, u = 0.0;
+  float ties = 0.0f;
+  for (int32_t t = 0; t < tiles; ++t) {
+    const ScoresView p = tile_of(s, span, t);
+    const F f(p);
+    typename F::Regs v;
+    f.load(v, p, i);
+    f.trim(v);
+    AltSums a[2] = {};
+#pragma unroll
+    for (int j = 0; j < F::N; ++j) add_score(a[j % 2], F::value(v, j), m, ms, g.scale);
+    z += (double)(a[0].z + a[1].z);
+    u += (double)(a[0].u + a[1].u);
+    ties += a[0].ties + a[1].ties;
+    if (some) {
+#pragma unroll
+      for (int j = 0; j < F::N; ++j) {
+        const float x = F::value(v, j);
+        if (x >= from) {
+          const int at = atomicAdd(&count, 1);
+          if (at < kHold) list[at] = key_of(x, t * span + f.cls(j));
+        }
+      }
+    }
+  }
+  float sum[3] = {(float)z, (float)u, ties};
+  whole.template reduce_all<3>(sum, AddF(), buf);
+  const AltRow r = alt_row(AltSums{sum[0], sum[1], sum[2]}, m);
+  if (threadIdx.x == 0) write_alt_row(r, g, i, lab, sa);
+  if (g.k == 0) return;
+  const int n = count;
+  if (n <= kHold) {
+    rank_candidates(list, n, threadIdx.x, 1024, r, g, i);
+    return;
+  }
+  uint64_t below = ~0ull;
+  for (int32_t t = 0; t < g.k; ++t) {
+    below = next_key<NW>(below, key_buf, [&](uint64_t under) {
+      uint64_t best = 0;
+      for (int32_t k = threadIdx.x; k < s.K; k += 1024) {
+        const float x = score_at<T>(s, i, k);
+        const uint64_t key = key_of(x, k);
+        if (x > -__builtin_inff() && key < under && key > best) best = key;
+      }
+      return best;
+    });
+    if (threadIdx.x == 0)
+      write_alternative(r, g, i, t, below ? class_of(below) : -1,
+                        score_of((uint32_t)(below >> 32)));
+  }
+}
+
+// ---------------------------------------------------------------------------
+// which kernel a call takes
+// ---------------------------------------------------------------------------
+template <typename T>
+static int alternatives_frames(const ScoresView& s, const AltRows& g, hipStream_t st) {
+  constexpr int VE = Chunk<T>::VE;
+  const auto turns = [&](auto tag, int64_t blocks, int threads) {
+    using F = typename decltype(tag)::type;
+    hipLaunchKernelGGL((alternatives_turns_kernel<F>), dim3((unsigned)blocks), dim3(threads), 0,
+                       st, s, g);
+  };
+  const auto candidates = [&](auto tag) {
+    using F = typename decltype(tag)::type;
+    hipLaunchKernelGGL((alternatives_candidates_kernel<F>),
+                       dim3((unsigned)((s.n + F::kRows - 1) / F::kRows)), dim3(F::kThreads), 0, st,
+                       s, g);
+  };
+  const auto row_turns = [&](auto tag) {
+    using F = typename decltype(tag)::type;
+    turns(tag, (s.n + F::kRows - 1) / F::kRows, F::kThreads);
+  };
+  const int64_t chunks = (s.K + VE - 1) / VE;
+  if (s.class_major() || s.K < VE) {
+    pick_class_frame<T>(s, turns);
+  } else if (chunks <= 4) {
+    row_turns(FrameTag<RowFrame<T, 4, 1>>());
+  } else if (chunks <= 8) {
+    row_turns(FrameTag<RowFrame<T, 8, 1>>());
+  } else if (chunks <= 16) {
+    row_turns(FrameTag<RowFrame<T, 8, 2>>());
+  } else if (chunks <= 32) {
+    row_turns(FrameTag<RowFrame<T, 16, 2>>());
+  } else if (chunks <= 64) {
+    candidates(FrameTag<RowFrame<T, 64, 1>>());
+  } else if (chunks <= 128) {
+    candidates(FrameTag<RowFrame<T, 64, 2>>());
+  } else if (chunks <= 256) {
+    candidates(FrameTag<RowFrame<T, 64, 4>>());
+  } else if (chunks <= 512) {
+    candidates(FrameTag<RowFrame<T, 64, 8>>());
+  } else if (chunks <= 1024) {
+    candidates(FrameTag<RowFrame<T, 256, 4>>());
+  } else if (chunks <= 2048) {
+    candidates(FrameTag<RowFrame<T, 256, 8>>());
+  } else if (chunks <= 4096) {
+    candidates(FrameTag<RowFrame<T, 1024, 4>>());
+  } else if (chunks <= 8192) {
+    candidates(FrameTag<RowFrame<T, 1024, 8>>());
+  } else if (chunks <= 16384) {
+    candidates(FrameTag<RowFrame<T, 1024, 16>>());
+  } else {
+    int32_t span, tiles;
+    cut_tiles(s.K, AltTile<T>::N * 1024, &span, &tiles);
+    hipLaunchKernelGGL((alternatives_long_kernel<T>), dim3((unsigned)s.n), dim3(1024), 0, st, s, g,
+                       span, tiles);
+  }
+  WGBM_LAUNCH_CHECK();
+  return 0;
+}
+
+}  // namespace wgbm

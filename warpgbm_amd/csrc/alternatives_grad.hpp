@@ -1,0 +1,262 @@
+// Gradient of what a training step makes of a row's label, alternatives and
+// entropy: with upstream gradients g_j of the log-probabilities of the classes c_j
+// (the label's among them), g_H of the entropy and G = sum g_j,
+//   ds_k = (1 / tau) (sum of g_j with c_j = k  -  p_k (G + g_H (x_k + down)))
+// x, down and p = e^(x - lse) from the row's norm (alternatives.hpp).  No sums over
+// classes: rows are read once and the gradient written once.  At a class with a
+// g of its own: g (1 - p) - p ((G - g) + g_H (x + down)), 1 - p from log p, so that
+// a row sure of that class keeps its digits.
+#pragma once
+#include "losses_lists.hpp"
+
+namespace wgbm {
+
+// e^x (c0 + c1 h), h = x log2(e): a class without a g of its own
+struct AltGradRow {
+  float m, c0, c1;
+  float lse, down, g_all, g_entropy;
+  bool live;
+};
+__device__ __forceinline__ AltGradRow alt_grad_row(const AltGradRows& g, int64_t i, float g_all,
+                                                   bool any) {
+  AltGradRow o;
+  o.m = g.norm[3 * i];
+  o.lse = g.norm[3 * i + 1];
+  o.down = g.norm[3 * i + 2];
+  o.g_entropy = g.grad_entropy ? g.grad_entropy[i] : 0.0f;
+  o.g_all = g_all;
+  o.live = o.m != -__builtin_inff() && (any || o.g_entropy != 0.0f);
+  const float f = -exp_of(-o.lse) * (float)g.inv_tau;
+  o.c0 = f * fmaf(o.g_entropy, o.down, g_all);
+  o.c1 = f * o.g_entropy * (float)kLn2;
+  return o;
+}
+__device__ __forceinline__ float alt_grad_at(const AltGradRow& r, const AltGradRows& g, float v) {
+  const float h = (v - r.m) * g.scale;
+  return exp2_f32(h) * fmaf(r.c1, fmaxf(h, kLowPower), r.c0);
+}
+__device__ __forceinline__ float alt_grad_listed(const AltGradRow& r, const AltGradRows& g, float v,
+                                                 float own) {
+  const float x = (v - r.m) * (float)g.inv_tau, lp = x - r.lse;
+  const float rest = fmaf(r.g_entropy, fmaxf(x, kLowPower) + r.down, r.g_all - own);
+  return (float)g.inv_tau * fmaf(own, one_less_exp(lp), -exp_of(lp) * rest);
+}
+
+// no list: only the label has a g of its own.  tile: of a long row (span 0: the rows
+// are whole)
+template <typename F>
+__global__ __launch_bounds__(F::kMax) void alternatives_grad_plain_kernel(ScoresView whole,
+                                                                          AltGradRows g,
+                                                                          ScoresView out_whole,
+                                                                          bool accumulate,
+                                                                          int32_t span) {
+  const ScoresView s = span ? tile_of(whole, span, blockIdx.y) : whole;
+  const ScoresView out = span ? tile_of(out_whole, span, blockIdx.y) : out_whole;
+  const F f(s);
+  const int64_t i = F::row(blockIdx.x);
+  if (i >= s.n) return;
+  typename F::Regs v;
+  f.load(v, s, blockIdx.x);
+  int32_t lab = row_label(g.label, i, whole.K);
+  const float own = lab >= 0 ? g.grad_label[i] : 0.0f;
+  const float sa = lab >= 0 ? score_at<typename F::T>(whole, i, lab) : 0.0f;
+  const AltGradRow r = alt_grad_row(g, i, own, own != 0.0f);
+  if (!r.live) {
+    if (!accumulate) f.store_zero(out, blockIdx.x);
+    return;
+  }
+  lab -= blockIdx.y * span;
+  f.store_row(out, blockIdx.x, accumulate, lab >= 0 && lab < s.K ? lab : -1,
+              alt_grad_listed(r, g, sa, own),
+              [&](int j) { return alt_grad_at(r, g, F::value(v, j)); });
+}
+
+// a thread a row: the list's g are added up in registers
+template <typename F>
+__global__ __launch_bounds__(F::kMax) void alternatives_grad_lane_kernel(ScoresView s,
+                                                                         AltGradRows g,
+                                                                         ScoresView out,
+                                                                         bool accumulate) {
+  const F f(s);
+  const int64_t i = F::row(blockIdx.x);
+  if (i >= s.n) return;
+  typename F::Regs v;
+  f.load(v, s, blockIdx.x);
+  float own[F::N], all = 0.0f;
+  bool any = false;
+#pragma unroll
+  for (int j = 0; j < F::N; ++j) own[j] = 0.0f;
+  const auto add = [&](int32_t c, float x) {
+    if (c < 0 || c >= s.K) return;
+    all += x;
+    any |= x != 0.0f;
+#pragma unroll
+    for (int j = 0; j < F::N; ++j) own[j] += f.cls(j) == c ? x : 0.0f;
+  };
+  if (g.label) add(g.label[i], g.grad_label[i]);
+  for (int32_t e = 0; e < g.k; ++e)
+    add(g.classes[i * g.class_stride + e], g.grad_list[i * g.grad_stride + e]);
+  const AltGradRow r = alt_grad_row(g, i, all, any);
+  if (!r.live) {
+    if (!accumulate) f.store_zero(out, blockIdx.x);
+    return;
+  }
+  f.store(out, blockIdx.x, accumulate, [&](int j) {
+    const float x = F::value(v, j);
+    return own[j] != 0.0f ? alt_grad_listed(r, g, x, own[j]) : alt_grad_at(r, g, x);
+  });
+}
+
+// Rows that threads share.  The listed classes are taken out of the rows (a bit a
+// slot, set through LDS, found again by the thread that has the class), which
+// leaves their places 0 or as they were, and their gradients are written to
+// memory after the others': each is rounded once.
+template <typename F>
+__global__ __launch_bounds__(F::kMax) void alternatives_grad_list_kernel(ScoresView whole,
+                                                                         AltGradRows g,
+                                                                         ScoresView out_whole,
+                                                                         bool accumulate,
+                                                                         int32_t span) {
+  using T = typename F::T;
+  extern __shared__ uint32_t lds[];  // classes, gradients, scores of the lists; bits of the slots
+  __shared__ float buf[2 * F::kBuf];
+  const int k = g.k;
+  int32_t* const l_cls = (int32_t*)lds;
+  float* const l_own = (float*)(l_cls + F::kListRows * k);
+  float* const l_score = l_own + F::kListRows * k;
+  uint32_t* const bits = (uint32_t*)(l_score + F::kListRows * k);
+  const int32_t k0 = span ? (int32_t)blockIdx.y * span : 0;
+  const ScoresView s = span ? tile_of(whole, span, blockIdx.y) : whole;
+  const ScoresView out = span ? tile_of(out_whole, span, blockIdx.y) : out_whole;
+  const F f(s);
+  const int64_t row = F::row(blockIdx.x);
+  const bool in = row < s.n;
+  const int64_t i = in ? row : s.n - 1;
+  typename F::Regs v;
+  f.load(v, s, blockIdx.x);
+#pragma unroll
+  for (int b = 0; b < F::kMaskWords; ++b) bits[b * blockDim.x + threadIdx.x] = 0;
+  const int32_t lab = row_label(g.label, i, whole.K);
+  const float g_label = lab >= 0 ? g.grad_label[i] : 0.0f;
+  const float sa = lab >= 0 ? score_at<T>(whole, i, lab) : 0.0f;
+  __syncthreads();
+  float sum[2] = {0.0f, 0.0f};  // of the g, and how many are not 0
+  bool twice = false;
+  int word;
+  uint32_t bit;
+  for (int j = f.entry(); j < k; j += f.entry_step()) {
+    int32_t c = g.classes[i * g.class_stride + j];
+    float own = 0.0f, sc = 0.0f;
+    if (c < 0 || c >= whole.K) c = -1;
+    if (c >= 0) {
+      own = g.grad_list[i * g.grad_stride + j];
+      sum[0] += own;
+      sum[1] += own != 0.0f ? 1.0f : 0.0f;
+      if (c >= k0 && c - k0 < s.K) {
+        f.locate(c - k0, word, bit);
+        twice |= (atomicOr(&bits[word], bit) & bit) != 0;
+        sc = score_at<T>(whole, i, c);
+      } else {
+        c = -1;  // another tile's
+      }
+    }
+    l_cls[f.entry_at(j, k)] = c;
+    l_own[f.entry_at(j, k)] = own;
+    l_score[f.entry_at(j, k)] = sc;
+  }
+  if (__syncthreads_or(twice)) {
+    // a class that is listed again: the first entry takes all its g
+    uint32_t again = 0;
+    int n = 0;
+    for (int j = f.entry(); j < k; j += f.entry_step(), ++n) {
+      const int32_t c = l_cls[f.entry_at(j, k)];
+      if (c >= 0 && listed_before(f, l_cls, j, k, c)) again |= 1u << n;
+    }
+    __syncthreads();
+    n = 0;
+    for (int j = f.entry(); j < k; j += f.entry_step(), ++n) {
+      const int32_t c = l_cls[f.entry_at(j, k)];
+      if (c < 0 || again >> n & 1) continue;
+      // (later entries' own numbers: only first entries' are changed)
+      float more = 0.0f;
+      for (int o = j + 1; o < k; ++o)
+        if (l_cls[f.entry_at(o, k)] == c) more += l_own[f.entry_at(o, k)];
+      l_own[f.entry_at(j, k)] += more;
+    }
+    __syncthreads();
+    n = 0;
+    for (int j = f.entry(); j < k; j += f.entry_step(), ++n)
+      if (again >> n & 1) l_cls[f.entry_at(j, k)] = -1;
+  }
+  // the label: an entry of its own unless the list has it
+  bool mine = false;
+  const bool label_here = lab >= k0 && lab - k0 < s.K && lab >= 0;
+  if (f.entry() == 0 && label_here) {
+    f.locate(lab - k0, word, bit);
+    mine = (bits[word] & bit) == 0;
+    if (mine) atomicOr(&bits[word], bit);
+  }
+  f.reduce_all(sum, AddF(), buf);
+  __syncthreads();
+  uint32_t out_bits[F::kMaskWords];
+#pragma unroll
+  for (int b = 0; b < F::kMaskWords; ++b) out_bits[b] = bits[b * blockDim.x + threadIdx.x];
+  const AltGradRow r = alt_grad_row(g, i, sum[0] + g_label, sum[1] != 0.0f || g_label != 0.0f);
+  f.take_out(v, out_bits);
+  if (in) {
+    if (r.live)
+      f.store(out, blockIdx.x, accumulate,
+              [&](int j) { return alt_grad_at(r, g, F::value(v, j)); });
+    else if (!accumulate)
+      f.store_zero(out, blockIdx.x);
+  }
+  __syncthreads();
+  if (!in || !r.live) return;
+  // (the scores were read before: the gradient may be written over them)
+  const auto write = [&](int32_t c, float sc, float own) {
+    float x = alt_grad_listed(r, g, sc, own);
+    T* q = (T*)out.data + i * out.rs + (c - k0) * out.ks;
+    if (accumulate) x += to_f32(*q);
+    *q = from_f32<T>(x);
+  };
+  for (int j = f.entry(); j < k; j += f.entry_step()) {
+    const int at = f.entry_at(j, k);
+    const int32_t c = l_cls[at];
+    if (c >= 0) write(c, l_score[at], l_own[at] + (c == lab ? g_label : 0.0f));
+  }
+  if (mine) write(lab, sa, g_label);
+}
+
+template <typename T>
+static int alternatives_grad_frames(const ScoresView& s, const AltGradRows& g,
+                                    const ScoresView& out, bool accumulate, hipStream_t st) {
+  const auto launch = [&](auto tag, int64_t blocks, int threads, int32_t span, int32_t tiles) {
+    using F = typename decltype(tag)::type;
+    const dim3 grid((unsigned)blocks, (unsigned)tiles);
+    if (g.k == 0) {
+      hipLaunchKernelGGL((alternatives_grad_plain_kernel<F>), grid, dim3(threads), 0, st, s, g, out,
+                         accumulate, span);
+    } else if constexpr (F::kLaneRows && !F::kSlices) {
+      hipLaunchKernelGGL((alternatives_grad_lane_kernel<F>), grid, dim3(threads), 0, st, s, g, out,
+                         accumulate);
+    } else {
+      const size_t lds = (size_t)F::kListRows * g.k * 12 + (size_t)F::kMaskWords * threads * 4;
+      hipLaunchKernelGGL((alternatives_grad_list_kernel<F>), grid, dim3(threads), lds, st, s, g,
+                         out, accumulate, span);
+    }
+  };
+  if (rows_fit(s, false)) {
+    pick_frame<T, false, false>(s, [&](auto tag, int64_t blocks, int threads) {
+      launch(tag, blocks, threads, 0, 1);
+    });
+  } else {
+    using Tile = RowFrame<T, 1024, 4>;
+    int32_t span, tiles;
+    cut_tiles(s.K, Tile::N * 1024, &span, &tiles);
+    launch(FrameTag<Tile>(), s.n, 1024, span, tiles);
+  }
+  WGBM_LAUNCH_CHECK();
+  return 0;
+}
+
+}  // namespace wgbm

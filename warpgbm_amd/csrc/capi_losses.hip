@@ -6,6 +6,7 @@
 
 using namespace wgbm;
 
+static_assert(WGBM_MAX_LIST == kMaxList, "list length");
 static_assert(WGBM_F32 == kF32 && WGBM_BF16 == kBF16 && WGBM_F16 == kF16, "type codes");
 
 // most classes of a row, and of the balance loss
@@ -165,6 +166,142 @@ int wgbm_balance_loss(const wgbm_scores* scores, const uint8_t* mask, int32_t to
                "balance_loss: workspace too small");
   return balance_loss(s, mask, top_k, coef, BalanceOut{loss, counts, prob}, g, accumulate != 0,
                       workspace, S(stream));
+}
+
+// log2(e) / tau and 1 / tau of a temperature
+static int tempered(float temperature, const char* what, float* scale, double* inv) {
+  WGBM_REQUIRE(temperature >= 1e-6f && temperature <= 1e6f,
+               "%s: temperature must be in [1e-6, 1e6]", what);
+  *inv = 1.0 / (double)temperature;
+  *scale = (float)(1.44269504088896340736 / (double)temperature);
+  return 0;
+}
+static int list_length(int32_t k, int32_t least, const char* what) {
+  WGBM_REQUIRE(k >= least && k <= kMaxList, "%s: the lists' length must be in [%d, %d], got %d",
+               what, least, kMaxList, k);
+  return 0;
+}
+static int list_stride(int64_t stride, int32_t k, const char* what) {
+  WGBM_REQUIRE(stride >= k && stride < (int64_t(1) << 40), "%s: a list's stride is out of range",
+               what);
+  return 0;
+}
+
+int64_t wgbm_class_alternatives_workspace(const wgbm_scores* scores) {
+  ScoresView s;
+  if (view_of(scores, "scores", &s)) return -1;
+  return (int64_t)lists_workspace(s, false);
+}
+
+int wgbm_class_alternatives(const wgbm_scores* scores, const int32_t* labels, int32_t top_k,
+                            float temperature, int32_t* classes, float* log_prob, float* entropy,
+                            float* label_log_prob, float* norm, void* workspace,
+                            int64_t workspace_bytes, void* stream) {
+  ScoresView s;
+  TRY(view_of(scores, "scores", &s));
+  TRY(list_length(top_k, 0, "class_alternatives"));
+  WGBM_REQUIRE(top_k <= s.K, "class_alternatives: top_k must be at most n_classes (%d), got %d", s.K,
+               top_k);
+  AltRows g{};
+  TRY(tempered(temperature, "class_alternatives", &g.scale, &g.inv_tau));
+  if (s.n == 0) return 0;
+  WGBM_REQUIRE(entropy && norm && (top_k == 0 || (classes && log_prob)) &&
+                   (!labels || label_log_prob),
+               "class_alternatives: null pointer");
+  const int64_t need = (int64_t)lists_workspace(s, false);
+  WGBM_REQUIRE(need == 0 || (workspace && workspace_bytes >= need),
+               "class_alternatives: workspace too small");
+  g.label = labels;
+  g.k = top_k;
+  g.classes = classes;
+  g.log_prob = log_prob;
+  g.entropy = entropy;
+  g.label_log_prob = label_log_prob;
+  g.norm = norm;
+  return class_alternatives(s, g, workspace, S(stream));
+}
+
+int64_t wgbm_class_alternatives_grad_workspace(const wgbm_scores* scores) {
+  ScoresView s;
+  if (view_of(scores, "scores", &s)) return -1;
+  return (int64_t)lists_workspace(s, true);
+}
+
+int wgbm_class_alternatives_grad(const wgbm_scores* scores,
+                                 const wgbm_alternatives_grad_args* a, const wgbm_scores* grad,
+                                 int32_t accumulate, void* workspace, int64_t workspace_bytes,
+                                 void* stream) {
+  ScoresView s, o;
+  TRY(view_of(scores, "scores", &s));
+  TRY(view_of(grad, "grad", &o));
+  TRY(same_kind(s, o, "grad"));
+  WGBM_REQUIRE(a, "class_alternatives_grad: null arguments");
+  TRY(list_length(a->list_length, 0, "class_alternatives_grad"));
+  AltGradRows g{};
+  TRY(tempered(a->temperature, "class_alternatives_grad", &g.scale, &g.inv_tau));
+  if (a->list_length) {
+    TRY(list_stride(a->classes_stride, a->list_length, "class_alternatives_grad"));
+    TRY(list_stride(a->grad_stride, a->list_length, "class_alternatives_grad"));
+  }
+  if (s.n == 0) return 0;
+  WGBM_REQUIRE(a->norm && (!a->labels || a->grad_label_log_prob) &&
+                   (a->list_length == 0 || (a->classes && a->grad_log_prob)),
+               "class_alternatives_grad: null pointer");
+  const int64_t need = (int64_t)lists_workspace(s, true);
+  WGBM_REQUIRE(need == 0 || (workspace && workspace_bytes >= need),
+               "class_alternatives_grad: workspace too small");
+  g.norm = a->norm;
+  g.label = a->labels;
+  g.grad_label = a->grad_label_log_prob;
+  g.classes = a->classes;
+  g.class_stride = a->classes_stride;
+  g.grad_list = a->grad_log_prob;
+  g.grad_stride = a->grad_stride;
+  g.k = a->list_length;
+  g.grad_entropy = a->grad_entropy;
+  return class_alternatives_grad(s, g, o, accumulate != 0, workspace, S(stream));
+}
+
+int64_t wgbm_distill_loss_workspace(const wgbm_scores* scores) {
+  ScoresView s;
+  if (view_of(scores, "scores", &s)) return -1;
+  return (int64_t)lists_workspace(s, true);
+}
+
+int wgbm_distill_loss(const wgbm_scores* scores, const wgbm_distill_args* a, float* loss,
+                      const wgbm_scores* grad, int32_t accumulate, void* workspace,
+                      int64_t workspace_bytes, void* stream) {
+  ScoresView s, o{};
+  TRY(view_of(scores, "scores", &s));
+  if (grad) {
+    TRY(view_of(grad, "grad", &o));
+    TRY(same_kind(s, o, "grad"));
+  }
+  WGBM_REQUIRE(a, "distill_loss: null arguments");
+  TRY(list_length(a->list_length, 1, "distill_loss"));
+  TRY(list_stride(a->classes_stride, a->list_length, "distill_loss"));
+  TRY(list_stride(a->logits_stride, a->list_length, "distill_loss"));
+  DistillRows g{};
+  TRY(tempered(a->temperature, "distill_loss", &g.scale, &g.inv_tau));
+  WGBM_REQUIRE(a->log_norm || !a->rest || std::isfinite(a->log_norm_all),
+               "distill_loss: log_norm must be finite");
+  if (s.n == 0) return 0;
+  WGBM_REQUIRE(a->classes && a->logits && loss, "distill_loss: null pointer");
+  const int64_t need = (int64_t)lists_workspace(s, true);
+  WGBM_REQUIRE(need == 0 || (workspace && workspace_bytes >= need),
+               "distill_loss: workspace too small");
+  g.classes = a->classes;
+  g.class_stride = a->classes_stride;
+  g.logits = a->logits;
+  g.logit_stride = a->logits_stride;
+  g.k = a->list_length;
+  g.rest = a->rest != 0;
+  g.log_norm = a->rest ? a->log_norm : nullptr;
+  g.log_norm_all = a->log_norm_all;
+  g.weight = a->weight;
+  g.tau = a->temperature;
+  g.loss = loss;
+  return distill_loss(s, g, o, accumulate != 0, workspace, S(stream));
 }
 
 static PreferenceArgs preference_args(const wgbm_preference_args* a) {

@@ -1,0 +1,519 @@
+// Divergence of a row's scores from a teacher's listed classes, and its gradient.
+// With x = s / tau, p = softmax(x), the teacher's shares q_j of the listed classes
+// and Q of all the others together (P: the scores' own), scaled to sum 1 over
+// those that the row may take,
+//   loss = w tau^2 (sum q_j log(q_j / p_j) + Q log(Q / P))
+//   ds_k = w tau (p_k - q_k) at a listed class, w tau p_k (1 - Q / P) at others
+// q_j = e^(l_j / tau - log norm), Q = 1 - sum q_j; without log norms q = softmax(l /
+// tau) over the list and Q = 0.
+//
+// As both sides sum to 1 the loss is also a sum of terms >= 0,
+//   p - q - q x = q (e^x - 1 - x) with x = log(p / q),
+// in which the rounding of log sum e^x, common to all, cancels to first order;
+// the gradient is q (e^x - 1).  Logarithms are differences in float64 of
+// float32-exact sums; the sums leave out their largest term, 1.
+//
+// The listed classes are taken out of the rows as they sit in registers (a bit a
+// slot): what is left is the others' maximum and sum, and their gradient
+// needs one exponential a class.  The list's own terms are worked out an entry a
+// thread.
+#pragma once
+#include "losses_lists.hpp"
+
+namespace wgbm {
+
+// a rest smaller than this is the rounding of the list's numbers: 0
+constexpr float kLeastRest = 9.5367431640625e-07f;  // 2^-20
+
+// sums over a row, relative to maxima: m of all its scores, mr of those not
+// listed, lm of the listed classes' logits that count
+struct DistillSums {
+  float zr;                // others: sum of e^(s - mr)
+  float zl, zl_ties;       // listed: of e^(s - m) below m, and scores equal to m
+  float q, q_ties;         // counting: of e^(l - lm) below lm, and logits equal to lm
+  float out;               // not counting: of their shares (with log norms)
+};
+
+struct DistillRow {
+  bool live;
+  float m, mr;
+  double lse, shift;  // log p = (s - m) / tau - lse, log q = l / tau - shift
+  float others;       // gradient of another class: others * e^(s - mr)
+  float rest_term;    // the others' term of the loss
+  float scale, value; // w tau, w tau^2
+};
+
+// a bucket's term and what its gradient is made of, from its logarithms
+struct Bucket {
+  float term, slope;
+};
+__device__ __forceinline__ Bucket bucket(double log_p, double log_q) {
+  const float p = exp_of((float)log_p), q = exp_of((float)log_q);
+  if (q == 0.0f) return {p, p};
+  const float x = (float)(log_p - log_q);
+  if (fabsf(x) <= 1.0f) {
+    const float f = phi_small(x);
+    return {q * f, q * (x + f)};
+  }
+  return {p - q - q * x, p - q};
+}
+
+__device__ __forceinline__ float logit_power(const DistillRows& g, float l, float lm) {
+  return exp_of((float)(((double)l - (double)lm) * g.inv_tau));
+}
+
+__device__ __forceinline__ DistillRow distill_row(const DistillSums& a, const DistillRows& g,
+                                                  int64_t i, float m, float mr, float lm, float w) {
+  DistillRow o{};
+  o.m = safe_max(m);
+  o.mr = safe_max(mr);
+  o.scale = w * g.tau;
+  o.value = o.scale * g.tau;
+  const bool has_rest = mr > -__builtin_inff() || a.zr != a.zr;
+  // scores: listed A, others B, relative to m
+  const double drop = has_rest ? ((double)mr - (double)o.m) * g.inv_tau : 0.0;
+  const float B = has_rest ? exp_of((float)drop) * a.zr : 0.0f;
+  const float A = a.zl + a.zl_ties;
+  o.live = w != 0.0f && !(A + B == 0.0f);
+  // (the largest term, 1, is among the listed or among the others)
+  const float over = a.zl_ties > 0.0f ? a.zl + (a.zl_ties - 1.0f) + B : -1.0f;
+  o.lse = over >= 0.0f ? log_1p(over) : log_of(A + B);
+  // shares: `one` of the largest logit, C of the other counting ones
+  const bool counts = lm > -__builtin_inff() || a.q != a.q;
+  const double norm = g.rest ? (double)(g.log_norm ? g.log_norm[i] : g.log_norm_all) : 0.0;
+  const float more = a.q + (a.q_ties - 1.0f);  // relative to the largest
+  float Q = 0.0f;
+  double log_mass = 0.0;
+  if (!g.rest) {
+    o.live = o.live && counts;
+    o.shift = (double)lm * g.inv_tau + (counts ? log_1p(more) : 0.0);
+  } else {
+    const float top = (float)((double)lm * g.inv_tau - norm);  // its logarithm
+    const float one = counts ? exp_of(top) : 0.0f, C = counts ? more * one : 0.0f;
+    const float left = counts ? one_less_exp(top) - C - a.out : 1.0f - a.out;
+    const bool rest = left >= kLeastRest && has_rest;
+    Q = rest ? left : 0.0f;
+    // what is left out of sum 1
+    const float lost = a.out + (rest ? 0.0f : left);
+    if (lost != 0.0f) log_mass = lost < 0.5f ? log1p(-(double)lost) : log((double)(one + C + Q));
+    o.live = o.live && (counts || rest) && !(one + C + Q == 0.0f);
+    o.shift = norm + log_mass;
+  }
+  // the others
+  if (has_rest) {
+    const double log_P = B >= A ? -(double)log1p_of(A / B) : drop + log_of(a.zr) - o.lse;
+    const Bucket b = Q > 0.0f ? bucket(log_P, log_of(Q) - log_mass)
+                              : bucket(log_P, -(double)__builtin_inff());
+    o.rest_term = b.term;
+    o.others = o.scale * b.slope / a.zr;
+  }
+  return o;
+}
+// a listed class that counts (score above -infinity)
+__device__ __forceinline__ Bucket distill_entry(const DistillRow& r, const DistillRows& g, float s,
+                                                float l) {
+  return bucket(((double)s - (double)r.m) * g.inv_tau - r.lse, (double)l * g.inv_tau - r.shift);
+}
+// a listed class that does not count: the row may not take it
+__device__ __forceinline__ bool closed(float s) { return s == -__builtin_inff(); }
+
+// ---------------------------------------------------------------------------
+// a thread a row: the list as numbers beside the row's classes
+// ---------------------------------------------------------------------------
+template <typename F>
+__global__ __launch_bounds__(F::kMax) void distill_lane_kernel(ScoresView s, DistillRows g,
+                                                               ScoresView out, bool accumulate) {
+  constexpr int N = F::N;
+  const F f(s);
+  const int64_t i = F::row(blockIdx.x);
+  if (i >= s.n) return;
+  const float w = g.weight ? g.weight[i] : 1.0f;
+  if (w == 0.0f) {
+    g.loss[i] = 0.0f;
+    if (out.data && !accumulate) f.store_zero(out, blockIdx.x);
+    return;
+  }
+  typename F::Regs v;
+  f.load(v, s, blockIdx.x);
+  f.trim(v);
+  float l[N];
+  uint32_t listed = 0;
+#pragma unroll
+  for (int j = 0; j < N; ++j) l[j] = 0.0f;
+  for (int32_t e = 0; e < g.k; ++e) {
+    const int32_t c = g.classes[i * g.class_stride + e];
+    const float x = g.logits[i * g.logit_stride + e];
+    if (c < 0 || c >= s.K || (listed >> c & 1)) continue;  // (the first of equal classes counts)
+    listed |= 1u << c;
+#pragma unroll
+    for (int j = 0; j < N; ++j) l[j] = j == c ? x : l[j];
+  }
+  float m = -__builtin_inff(), mr = m, lm = m;
+#pragma unroll
+  for (int j = 0; j < N; ++j) {
+    const float x = F::value(v, j);
+    m = fmaxf(m, x);
+    if (listed >> j & 1)
+      lm = closed(x) ? lm : fmaxf(lm, l[j]);
+    else
+      mr = fmaxf(mr, x);
+  }
+  const float ms = safe_max(m), mrs = safe_max(mr);
+  DistillSums a{};
+  const float norm = g.rest ? (g.log_norm ? g.log_norm[i] : g.log_norm_all) : 0.0f;
+  // exponentials of the others, kept for the gradient
+  float e[N];
+#pragma unroll
+  for (int j = 0; j < N; ++j) {
+    const float x = F::value(v, j);
+    const bool in = listed >> j & 1;
+    e[j] = exp2_f32((x - (in ? ms : mrs)) * g.scale);
+    a.zr += in ? 0.0f : e[j];
+    a.zl += in && x != m ? e[j] : 0.0f;
+    a.zl_ties += in && x == m && !closed(x) ? 1.0f : 0.0f;
+    if (!in) continue;
+    if (!closed(x)) {
+      if (l[j] == lm)
+        a.q_ties += 1.0f;
+      else
+        a.q += logit_power(g, l[j], lm);
+    } else if (g.rest) {
+      a.out += exp_of((float)((double)l[j] * g.inv_tau - (double)norm));
+    }
+  }
+  const DistillRow r = distill_row(a, g, i, m, mr, lm, w);
+  float loss = r.rest_term;
+  float grad[N];
+#pragma unroll
+  for (int j = 0; j < N; ++j) {
+    const float x = F::value(v, j);
+    grad[j] = r.others * e[j];
+    if (listed >> j & 1) {
+      grad[j] = 0.0f;
+      if (!closed(x)) {
+        const Bucket b = distill_entry(r, g, x, l[j]);
+        loss += b.term;
+        grad[j] = r.scale * b.slope;
+      }
+    }
+  }
+  g.loss[i] = r.live ? r.value * loss : 0.0f;
+  if (!out.data) return;
+  if (!r.live) {
+    if (!accumulate) f.store_zero(out, blockIdx.x);
+    return;
+  }
+  f.store(out, blockIdx.x, accumulate, [&](int j) { return grad[j]; });
+}
+
+// ---------------------------------------------------------------------------
+// rows that threads share
+// ---------------------------------------------------------------------------
+// a workgroup's lists in LDS: classes (-1: not used), logits, scores of these
+struct ListTable {
+  int32_t* cls;
+  float* logit;
+  float* score;
+  uint32_t* bits;  // of the threads' slots
+};
+template <typename F>
+__device__ __forceinline__ ListTable list_table(uint32_t* lds, int k) {
+  ListTable t;
+  t.cls = (int32_t*)lds;
+  t.logit = (float*)(t.cls + F::kListRows * k);
+  t.score = t.logit + F::kListRows * k;
+  t.bits = (uint32_t*)(t.score + F::kListRows * k);
+  return t;
+}
+
+// entries that name a class again no longer count
+template <typename F>
+__device__ __forceinline__ void drop_repeated(const F& f, const ListTable& t, int k) {
+  uint32_t again = 0;
+  int n = 0;
+  for (int j = f.entry(); j < k; j += f.entry_step(), ++n) {
+    const int32_t c = t.cls[f.entry_at(j, k)];
+    if (c >= 0 && listed_before(f, t.cls, j, k, c)) again |= 1u << n;
+  }
+  __syncthreads();
+  n = 0;
+  for (int j = f.entry(); j < k; j += f.entry_step(), ++n)
+    if (again >> n & 1) t.cls[f.entry_at(j, k)] = -1;
+}
+
+// the list's part of the maxima: x[1] of listed scores, x[2] of counting logits
+template <typename F>
+__device__ __forceinline__ void list_maxima(const F& f, const ListTable& t, int k, float (&x)[3]) {
+  x[1] = x[2] = -__builtin_inff();
+  for (int j = f.entry(); j < k; j += f.entry_step()) {
+    const int at = f.entry_at(j, k);
+    if (t.cls[at] < 0) continue;
+    const float sc = t.score[at];
+    x[1] = fmaxf(x[1], sc);
+    if (!closed(sc)) x[2] = fmaxf(x[2], t.logit[at]);
+  }
+}
+// the list's part of the sums: x[1] .. x[5]
+template <typename F>
+__device__ __forceinline__ void list_sums(const F& f, const ListTable& t, const DistillRows& g,
+                                          int64_t i, float m, float lm, float (&x)[6]) {
+  const int k = g.k;
+  const float ms = safe_max(m);
+  const double norm = g.rest ? (double)(g.log_norm ? g.log_norm[i] : g.log_norm_all) : 0.0;
+  x[1] = x[2] = x[3] = x[4] = x[5] = 0.0f;
+  for (int j = f.entry(); j < k; j += f.entry_step()) {
+    const int at = f.entry_at(j, k);
+    if (t.cls[at] < 0) continue;
+    const float sc = t.score[at], l = t.logit[at];
+    if (closed(sc)) {
+      if (g.rest) x[5] += exp_of((float)((double)l * g.inv_tau - norm));
+      continue;
+    }
+    if (sc == m)
+      x[2] += 1.0f;
+    else
+      x[1] += exp2_f32((sc - ms) * g.scale);
+    if (l == lm)
+      x[4] += 1.0f;
+    else
+      x[3] += logit_power(g, l, lm);
+  }
+}
+
+template <typename F>
+__global__ __launch_bounds__(F::kMax) void distill_frame_kernel(ScoresView s, DistillRows g,
+                                                                ScoresView out, bool accumulate) {
+  using T = typename F::T;
+  extern __shared__ uint32_t lds[];
+  __shared__ float buf[6 * F::kBuf];
+  const int k = g.k;
+  const ListTable tab = list_table<F>(lds, k);
+  const F f(s);
+  const int64_t row = F::row(blockIdx.x);
+  const bool in = row < s.n;
+  const int64_t i = in ? row : s.n - 1;
+  typename F::Regs v;
+  f.load(v, s, blockIdx.x);
+  const float w = !in ? 0.0f : g.weight ? g.weight[i] : 1.0f;
+#pragma unroll
+  for (int b = 0; b < F::kMaskWords; ++b) tab.bits[b * blockDim.x + threadIdx.x] = 0;
+  __syncthreads();
+  bool twice = false;
+  for (int j = f.entry(); j < k; j += f.entry_step()) {
+    int32_t c = w != 0.0f ? g.classes[i * g.class_stride + j] : -1;
+    if (c >= s.K) c = -1;
+    float l = 0.0f, sc = 0.0f;
+    if (c >= 0) {
+      int word;
+      uint32_t bit;
+      f.locate(c, word, bit);
+      twice |= (atomicOr(&tab.bits[word], bit) & bit) != 0;
+      l = g.logits[i * g.logit_stride + j];
+      sc = score_at<T>(s, i, c);
+    }
+    const int at = f.entry_at(j, k);
+    tab.cls[at] = c < 0 ? -1 : c;
+    tab.logit[at] = l;
+    tab.score[at] = sc;
+  }
+  if (__syncthreads_or(twice)) drop_repeated(f, tab, k);
+  f.trim(v);
+  uint32_t mine[F::kMaskWords];
+#pragma unroll
+  for (int b = 0; b < F::kMaskWords; ++b) mine[b] = tab.bits[b * blockDim.x + threadIdx.x];
+  f.take_out(v, mine);
+  if (w == 0.0f) f.drop(v);
+  float x[3];
+  x[0] = -__builtin_inff();
+#pragma unroll
+  for (int j = 0; j < F::N; ++j) x[0] = fmaxf(x[0], F::value(v, j));
+  list_maxima(f, tab, k, x);
+  f.reduce_all(x, MaxF(), buf);
+  const float mr = x[0], m = fmaxf(x[0], x[1]), lm = x[2], mrs = safe_max(mr);
+  if (F::kHide) f.hide(v);
+  float z[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+  for (int j = 0; j < F::N; ++j) z[j % 4] += exp2_f32((F::value(v, j) - mrs) * g.scale);
+  float y[6];
+  y[0] = (z[0] + z[1]) + (z[2] + z[3]);
+  list_sums(f, tab, g, i, m, lm, y);
+  if (F::kBarrier) __syncthreads();  // the maxima have been read
+  f.reduce_all(y, AddF(), buf);
+  const DistillRow r = distill_row(DistillSums{y[0], y[1], y[2], y[3], y[4], y[5]}, g, i, m, mr, lm, w);
+  if (F::kHide) f.hide(v);
+  if (in && out.data) {
+    if (r.live)
+      f.store(out, blockIdx.x, accumulate, [&](int j) {
+        return r.others * exp2_f32((F::value(v, j) - mrs) * g.scale);
+      });
+    else if (!accumulate)
+      f.store_zero(out, blockIdx.x);
+  }
+  // (also: the others' gradients are written before the list's, the sums read)
+  __syncthreads();
+  float loss[1] = {0.0f};
+  for (int j = f.entry(); j < k; j += f.entry_step()) {
+    const int at = f.entry_at(j, k);
+    const int32_t c = tab.cls[at];
+    const float sc = tab.score[at];
+    if (c < 0 || closed(sc)) continue;
+    const Bucket b = distill_entry(r, g, sc, tab.logit[at]);
+    loss[0] += b.term;
+    if (in && r.live && out.data) {
+      float d = r.scale * b.slope;
+      T* q = (T*)out.data + i * out.rs + c * out.ks;
+      if (accumulate) d += to_f32(*q);
+      *q = from_f32<T>(d);
+    }
+  }
+  f.reduce_all(loss, AddF(), buf);
+  if (in && f.first_lane()) g.loss[i] = r.live ? r.value * (loss[0] + r.rest_term) : 0.0f;
+}
+
+// ---------------------------------------------------------------------------
+// rows longer than a workgroup's registers: a workgroup a row, its tiles one after
+// the other, twice (maximum and sum of each thread's classes as they come, then the
+// gradient)
+// ---------------------------------------------------------------------------
+template <typename T>
+__global__ __launch_bounds__(1024) void distill_long_kernel(ScoresView s, DistillRows g,
+                                                            ScoresView out, bool accumulate,
+                                                            int32_t span, int32_t tiles) {
+  using F = RowFrame<T, 1024, 4>;
+  extern __shared__ uint32_t lds[];
+  __shared__ float buf[6 * F::kBuf];
+  const int k = g.k;
+  const ListTable tab = list_table<F>(lds, k);
+  const F whole(s);
+  const int64_t i = blockIdx.x;
+  const float w = g.weight ? g.weight[i] : 1.0f;
+  // the list: an entry a thread; repeated classes by comparison (a tile's bits say
+  // nothing of the others)
+  for (int j = threadIdx.x; j < k; j += 1024) {
+    int32_t c = w != 0.0f ? g.classes[i * g.class_stride + j] : -1;
+    if (c < 0 || c >= s.K) c = -1;
+    tab.cls[j] = c;
+    tab.logit[j] = c >= 0 ? g.logits[i * g.logit_stride + j] : 0.0f;
+    tab.score[j] = c >= 0 ? score_at<T>(s, i, c) : 0.0f;
+  }
+  __syncthreads();
+  drop_repeated(whole, tab, k);
+  __syncthreads();
+  // this thread's bits of tile t
+  const auto bits_of = [&](const F& f, int32_t t, uint32_t (&b)[F::kMaskWords]) {
+    tab.bits[threadIdx.x] = 0;
+    __syncthreads();
+    if ((int)threadIdx.x < k) {
+      const int32_t c = tab.cls[threadIdx.x] - t * span;
+      if (tab.cls[threadIdx.x] >= 0 && c >= 0 && c < f.K) {
+        int word;
+        uint32_t bit;
+        f.locate(c, word, bit);
+        atomicOr(&tab.bits[word], bit);
+      }
+    }
+    __syncthreads();
+    b[0] = tab.bits[threadIdx.x];
+  };
+  static_assert(F::kMaskWords == 1, "a word a thread");
+  float most = -__builtin_inff();
+  double sum = 0.0;
+  if (w != 0.0f) {
+    for (int32_t t = 0; t < tiles; ++t) {
+      const ScoresView p = tile_of(s, span, t);
+      const F f(p);
+      typename F::Regs v;
+      f.load(v, p, i);
+      uint32_t b[F::kMaskWords];
+      bits_of(f, t, b);
+      f.trim(v);
+      f.take_out(v, b);
+      float m = most;
+#pragma unroll
+      for (int j = 0; j < F::N; ++j) m = fmaxf(m, F::value(v, j));
+      const float ms = safe_max(m);
+      float z[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int j = 0; j < F::N; ++j) z[j % 4] += exp2_f32((F::value(v, j) - ms) * g.scale);
+      if (most > -__builtin_inff()) sum *= (double)exp2_f32((most - ms) * g.scale);
+      sum += (double)((z[0] + z[1]) + (z[2] + z[3]));
+      most = m;
+    }
+  }
+  float x[3] = {most, 0.0f, 0.0f};
+  list_maxima(whole, tab, k, x);
+  whole.reduce_all(x, MaxF(), buf);
+  const float mr = x[0], m = fmaxf(x[0], x[1]), lm = x[2], mrs = safe_max(mr);
+  float y[6];
+  // (a thread without a class has sum 0, or NaN)
+  y[0] = (float)sum * (most > -__builtin_inff() ? exp2_f32((most - mrs) * g.scale) : 1.0f);
+  list_sums(whole, tab, g, i, m, lm, y);
+  __syncthreads();
+  whole.reduce_all(y, AddF(), buf);
+  const DistillRow r = distill_row(DistillSums{y[0], y[1], y[2], y[3], y[4], y[5]}, g, i, m, mr, lm, w);
+  if (out.data && (r.live || !accumulate)) {
+    for (int32_t t = 0; t < tiles; ++t) {
+      const ScoresView p = tile_of(s, span, t), o = tile_of(out, span, t);
+      const F f(p);
+      if (!r.live) {
+        f.store_zero(o, i);
+        continue;
+      }
+      typename F::Regs v;
+      f.load(v, p, i);
+      uint32_t b[F::kMaskWords];
+      bits_of(f, t, b);
+      f.trim(v);
+      f.take_out(v, b);
+      f.store(o, i, accumulate, [&](int j) {
+        return r.others * exp2_f32((F::value(v, j) - mrs) * g.scale);
+      });
+    }
+  }
+  __syncthreads();
+  float loss[1] = {0.0f};
+  for (int j = threadIdx.x; j < k; j += 1024) {
+    const int32_t c = tab.cls[j];
+    const float sc = tab.score[j];
+    if (c < 0 || closed(sc)) continue;
+    const Bucket b = distill_entry(r, g, sc, tab.logit[j]);
+    loss[0] += b.term;
+    if (r.live && out.data) {
+      float d = r.scale * b.slope;
+      T* q = (T*)out.data + i * out.rs + c;
+      if (accumulate) d += to_f32(*q);
+      *q = from_f32<T>(d);
+    }
+  }
+  whole.reduce_all(loss, AddF(), buf);
+  if (threadIdx.x == 0) g.loss[i] = r.live ? r.value * (loss[0] + r.rest_term) : 0.0f;
+}
+
+template <typename T>
+static int distill_frames(const ScoresView& s, const DistillRows& g, const ScoresView& out,
+                          bool accumulate, hipStream_t st) {
+  if (!rows_fit(s, false)) {
+    using F = RowFrame<T, 1024, 4>;
+    int32_t span, tiles;
+    cut_tiles(s.K, F::N * 1024, &span, &tiles);
+    hipLaunchKernelGGL((distill_long_kernel<T>), dim3((unsigned)s.n), dim3(1024),
+                       (size_t)g.k * 12 + 1024 * 4, st, s, g, out, accumulate, span, tiles);
+    WGBM_LAUNCH_CHECK();
+    return 0;
+  }
+  pick_frame<T, false, true>(s, [&](auto tag, int64_t blocks, int threads) {
+    using F = typename decltype(tag)::type;
+    if constexpr (F::kLaneRows && !F::kSlices) {
+      hipLaunchKernelGGL((distill_lane_kernel<F>), dim3((unsigned)blocks), dim3(threads), 0, st, s,
+                         g, out, accumulate);
+    } else {
+      const size_t lds = (size_t)F::kListRows * g.k * 12 + (size_t)F::kMaskWords * threads * 4;
+      hipLaunchKernelGGL((distill_frame_kernel<F>), dim3((unsigned)blocks), dim3(threads), lds, st,
+                         s, g, out, accumulate);
+    }
+  });
+  WGBM_LAUNCH_CHECK();
+  return 0;
+}
+
+}  // namespace wgbm

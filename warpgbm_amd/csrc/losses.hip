@@ -324,27 +324,6 @@ static int log_probs_t(const ScoresView& s, const int32_t* label, float* log_pro
   return 0;
 }
 
-// A grid's threads are counted in 32 bits: rows in registers are launched in
-// parts of fewer (no frame gives a row more than 1024 threads, nor more than its
-// classes and 3).  fn(first row, rows) for each part.
-template <typename Fn>
-static int row_parts(const ScoresView& s, Fn fn) {
-  const int64_t threads = std::min<int64_t>(1024, (int64_t)s.K + 3);
-  const int64_t most = ((int64_t(1) << 32) - 1) / threads / 1024 * 1024;
-  for (int64_t i = 0; i < s.n; i += most) {
-    const int r = fn(i, std::min(most, s.n - i));
-    if (r) return r;
-  }
-  return 0;
-}
-static ScoresView rows_of(const ScoresView& s, int64_t i, int64_t n) {
-  ScoresView v = s;
-  if (!s.data) return v;
-  v.data = (unsigned char*)s.data + i * s.rs * (s.dtype == kF32 ? 4 : 2);
-  v.n = n;
-  return v;
-}
-
 int class_log_probs(const ScoresView& s, const int32_t* label, float* log_prob, float* norm,
                     void* ws, hipStream_t st) {
   if (rows_fit(s, false)) {

@@ -1,7 +1,5 @@
-// The balance loss: its finishing launch, the transposes of wide class-major
-// scores, and the host side (the passes over rows: losses_balance.hpp).
-#include <type_traits>
-
+// The balance loss: its finishing launch and the host side (the passes over rows:
+// losses_balance.hpp).
 #include "losses_balance.hpp"
 
 namespace wgbm {
@@ -75,38 +73,6 @@ __global__ void balance_empty_kernel(int32_t K, BalanceOut o) {
   }
 }
 
-// b(i, k) (+)= a(i, k) between class-major scores (or gradient) and a row-major
-// copy, by tiles of 64 x 64 through LDS (60000 x 2000 bfloat16: the balance loss
-// takes 598 us with its two transposes, 204 of row-major scores)
-template <typename A, typename B, bool TO_ROWS>
-__global__ __launch_bounds__(256) void transpose_kernel(ScoresView a, ScoresView b,
-                                                        bool accumulate) {
-  __shared__ float tile[64][65];
-  const int64_t i0 = (int64_t)blockIdx.x * 64;
-  const int32_t k0 = blockIdx.y * 64;
-  const int x = threadIdx.x & 63, y = threadIdx.x >> 6;
-  const A* p = (const A*)a.data;
-  B* q = (B*)b.data;
-#pragma unroll 4
-  for (int r = y; r < 64; r += 4) {
-    // x along the dimension that is contiguous in a
-    const int64_t i = i0 + (TO_ROWS ? x : r);
-    const int32_t k = k0 + (TO_ROWS ? r : x);
-    if (i < a.n && k < a.K) tile[r][x] = to_f32(p[i * a.rs + k * a.ks]);
-  }
-  __syncthreads();
-#pragma unroll 4
-  for (int r = y; r < 64; r += 4) {
-    const int64_t i = i0 + (TO_ROWS ? r : x);
-    const int32_t k = k0 + (TO_ROWS ? x : r);
-    if (i < a.n && k < a.K) {
-      B* o = q + i * b.rs + k * b.ks;
-      const float v = tile[x][r];
-      *o = from_f32<B>(accumulate ? v + to_f32(*o) : v);
-    }
-  }
-}
-
 // class-major scores of more classes than a workgroup's slices hold go through
 // a row-major copy: of their type, or of float32 where the gradient is added to
 // another (so that it is rounded once)
@@ -140,22 +106,6 @@ size_t balance_workspace(const ScoresView& s) {
   return balance_ws(s.n, s.K, s.class_major(), nullptr).bytes;
 }
 
-// T: the class-major side's type; the row-major side has it too, or float32
-template <typename T, bool TO_ROWS>
-static void transpose(const ScoresView& a, const ScoresView& b, bool accumulate, hipStream_t st) {
-  const dim3 grid((unsigned)((a.n + 63) / 64), (unsigned)((a.K + 63) / 64));
-  const auto go = [&](auto rows) {
-    using R = decltype(rows);
-    using A = std::conditional_t<TO_ROWS, T, R>;
-    using B = std::conditional_t<TO_ROWS, R, T>;
-    hipLaunchKernelGGL((transpose_kernel<A, B, TO_ROWS>), grid, dim3(256), 0, st, a, b, accumulate);
-  };
-  if ((TO_ROWS ? b : a).dtype == kF32)
-    go(float());
-  else
-    go(T());
-}
-
 int balance_loss(const ScoresView& s, const uint8_t* mask, int32_t top_k, float coef,
                  const BalanceOut& o, const ScoresView& out, bool accumulate, void* base,
                  hipStream_t st) {
@@ -173,8 +123,8 @@ int balance_loss(const ScoresView& s, const uint8_t* mask, int32_t top_k, float 
     if (accumulate) v.dtype = kF32;
     v.rs = s.K;
     v.ks = 1;
-    LOSS_TYPES(s.dtype, (transpose<T, true>(s, v, false, st)));
-    WGBM_LAUNCH_CHECK();
+    const int r = scores_to_rows(s, v, st);
+    if (r) return r;
   }
   int32_t slots = 0;
   const auto stats = v.dtype == kF32    ? balance_stats_f32
@@ -193,9 +143,7 @@ int balance_loss(const ScoresView& s, const uint8_t* mask, int32_t top_k, float 
   // (in place in the row-major copy: a thread writes what it alone has read)
   r = grad(v, w, turn ? v : out, turn ? false : accumulate, st);
   if (r || !turn) return r;
-  LOSS_TYPES(s.dtype, (transpose<T, false>(v, out, accumulate, st)));
-  WGBM_LAUNCH_CHECK();
-  return 0;
+  return rows_to_scores(v, out, accumulate, st);
 }
 
 }  // namespace wgbm

@@ -288,6 +288,60 @@ struct RowFrame {
     if (G <= 64) return lanes_reduce<(G < 64 ? G : 64)>(x, op);
     return waves_reduce<(G > 64 ? G / 64 : 1)>(x, op, buf);
   }
+  // NV of them at once; buf: NV * kBuf words, free again after one more barrier
+  template <int NV, typename Op>
+  __device__ __forceinline__ void reduce_all(float (&x)[NV], Op op, float* buf) const {
+#pragma unroll
+    for (int v = 0; v < NV; ++v) x[v] = lanes_reduce<(G < 64 ? G : 64)>(x[v], op);
+    if (G <= 64) return;
+    if ((threadIdx.x & 63) == 0)
+#pragma unroll
+      for (int v = 0; v < NV; ++v) buf[v * kBuf + (threadIdx.x >> 6)] = x[v];
+    __syncthreads();
+#pragma unroll
+    for (int v = 0; v < NV; ++v) {
+      x[v] = buf[v * kBuf];
+#pragma unroll
+      for (int w = 1; w < kBuf; ++w) x[v] = op(x[v], buf[v * kBuf + w]);
+    }
+  }
+
+  // Lists of a row's classes (losses_lists.hpp): its entries j = t, t + G, ... are
+  // this thread's.
+  static constexpr int kListRows = kRows;
+  __device__ __forceinline__ int entry() const { return t; }
+  __device__ __forceinline__ int entry_step() const { return G; }
+  // place of entry j in a table of the workgroup's lists of k
+  __device__ __forceinline__ int entry_at(int j, int k) const { return threadIdx.x / G * k + j; }
+  // a bit for each of a thread's slots; class k's is bit `bit` of word `word` among the
+  // workgroup's (kMaskWords a thread, those of a number next to each other)
+  static constexpr int kMaskWords = (N + 31) / 32;
+  __device__ __forceinline__ void locate(int32_t k, int& word, uint32_t& bit) const {
+    const int32_t q = k / VE, w = q * VE, from = w < K - VE ? w : K - VE;
+    const int slot = q / G * VE + (k - from);
+    word = (slot >> 5) * kThreads + threadIdx.x / G * G + q % G;
+    bit = 1u << (slot & 31);
+  }
+  // classes whose bits are set are no longer this row's
+  __device__ __forceinline__ void take_out(Regs& r, const uint32_t (&m)[kMaskWords]) const {
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+      const uint32_t b = (m[c * VE / 32] >> (c * VE % 32)) & ((1u << VE) - 1);
+      if (__any(b != 0)) {
+        uint32_t(&w)[4] = r.c[c].w;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          if (VE == 4) {
+            w[e] = b >> e & 1 ? kNegInf : w[e];
+          } else {
+            const uint32_t keep = (b >> (2 * e) & 1 ? 0u : 0xffffu) |
+                                  (b >> (2 * e + 1) & 1 ? 0u : 0xffff0000u);
+            w[e] = (w[e] & keep) | (kNegInf & ~keep);
+          }
+        }
+      }
+    }
+  }
 
   // sum[k] = the workgroup's sum of acc over its rows, for every class.  Lanes
   // at the same place in their groups first, then the waves one after the
@@ -458,6 +512,35 @@ struct ClassFrame {
     for (int v = 1; v < S; ++v) x = op(x, buf[v * 64 + lane]);
     return x;
   }
+  template <int NV, typename Op>
+  __device__ __forceinline__ void reduce_all(float (&x)[NV], Op op, float* buf) const {
+    if (!SLICES) return;
+    const int lane = threadIdx.x & 63;
+#pragma unroll
+    for (int v = 0; v < NV; ++v) buf[v * kBuf + w * 64 + lane] = x[v];
+    __syncthreads();
+#pragma unroll
+    for (int v = 0; v < NV; ++v) {
+      x[v] = buf[v * kBuf + lane];
+      for (int u = 1; u < S; ++u) x[v] = op(x[v], buf[v * kBuf + u * 64 + lane]);
+    }
+  }
+  // lists as in RowFrame, of slices: a row's entries are spread over the waves
+  static constexpr int kListRows = 64;
+  __device__ __forceinline__ int entry() const { return w; }
+  __device__ __forceinline__ int entry_step() const { return S; }
+  __device__ __forceinline__ int entry_at(int j, int) const {
+    return j * 64 + (threadIdx.x & 63);
+  }
+  static constexpr int kMaskWords = 1;
+  __device__ __forceinline__ void locate(int32_t k, int& word, uint32_t& bit) const {
+    word = k % S * 64 + (threadIdx.x & 63);
+    bit = 1u << (k / S);
+  }
+  __device__ __forceinline__ void take_out(Regs& r, const uint32_t (&m)[1]) const {
+#pragma unroll
+    for (int j = 0; j < N; ++j) r.c[j] = m[0] >> j & 1 ? (T)(-__builtin_inff()) : r.c[j];
+  }
   // sum[k] = the workgroup's sum of acc over its rows, for every class
   __device__ __forceinline__ void sum_rows(float (&acc)[N], float* sum) const {
 #pragma unroll
@@ -527,6 +610,68 @@ static void pick_slices(const ScoresView& s, Fn fn) {
   if (s.K <= 10 * S) return fn(FrameTag<ClassFrame<T, 10, true, true>>(), tiles, 64 * S);
   if (s.K <= 13 * S) return fn(FrameTag<ClassFrame<T, 13, true, true>>(), tiles, 64 * S);
   fn(FrameTag<ClassFrame<T, 16, true, true>>(), tiles, 64 * S);
+}
+
+// ---------------------------------------------------------------------------
+// which frame a call takes: fn(frame tag, workgroups, threads) for the smallest
+// one that holds the rows (rows_fit).  Row-major rows take two to eight chunks a
+// thread rather than one, so that a wave has more loads in flight and spends
+// what a row costs as a whole on more rows: with one chunk a thread the policy
+// loss of 300000 x 100 float32 takes 57 us instead of 43, of 100000 x 500
+// bfloat16 57 and 40, the log-probabilities' gradient 59 and 44, 47 and 38; 30000 x
+// 3000 bfloat16, eight chunks of a wave's threads instead of two of a
+// workgroup's, whose waves wait for one another: 95 and 65 (not the gradient
+// without sums: 66 and 68).  Up to eight chunks a thread each: log-probabilities'
+// gradient of 300000 x 30 float32 19 us, 20 with two.
+// ---------------------------------------------------------------------------
+template <typename T, bool REF, bool SUMS, typename Fn>
+static void pick_row_frame(const ScoresView& s, Fn fn) {
+  constexpr int VE = Chunk<T>::VE;
+  const int64_t chunks = (s.K + VE - 1) / VE;
+  const auto go = [&](auto tag) {
+    using F = typename decltype(tag)::type;
+    fn(tag, (s.n + F::kRows - 1) / F::kRows, F::kThreads);
+  };
+  if (chunks <= 4) return go(FrameTag<RowFrame<T, 4, 1>>());
+  if (chunks <= 8) return go(FrameTag<RowFrame<T, 8, 1>>());
+  if (chunks <= 16) return go(FrameTag<RowFrame<T, 8, 2>>());
+  if (chunks <= 32) return go(FrameTag<RowFrame<T, 16, 2>>());
+  if (chunks <= 64) return go(FrameTag<RowFrame<T, 32, 2>>());
+  if (chunks <= 128) return go(FrameTag<RowFrame<T, 32, 4>>());
+  if (chunks <= 256) return go(FrameTag<RowFrame<T, 32, 8>>());
+  if constexpr (!SUMS) {
+    if (chunks <= 512) return go(FrameTag<RowFrame<T, 256, 2>>());
+  }
+  if (chunks <= 512) return go(FrameTag<RowFrame<T, 64, 8>>());
+  if (chunks <= 1024) return go(FrameTag<RowFrame<T, 256, 4>>());
+  if (chunks <= 2048) return go(FrameTag<RowFrame<T, 256, 8>>());
+  if (REF || chunks <= 4096) return go(FrameTag<RowFrame<T, 1024, 4>>());
+  if constexpr (!REF) {
+    if (chunks <= 8192) return go(FrameTag<RowFrame<T, 1024, 8>>());
+    go(FrameTag<RowFrame<T, 1024, 16>>());
+  }
+}
+
+template <typename T, typename Fn>
+static void pick_class_frame(const ScoresView& s, Fn fn) {
+  const int64_t blocks = (s.n + 255) / 256;
+  if (!s.class_major()) {  // rows shorter than a chunk
+    if (s.K <= 4) return fn(FrameTag<ClassFrame<T, 4, false, false>>(), blocks, 256);
+    return fn(FrameTag<ClassFrame<T, 8, false, false>>(), blocks, 256);
+  }
+  if (s.K <= 4) return fn(FrameTag<ClassFrame<T, 4, false, true>>(), blocks, 256);
+  if (s.K <= 8) return fn(FrameTag<ClassFrame<T, 8, false, true>>(), blocks, 256);
+  if (s.K <= 12) return fn(FrameTag<ClassFrame<T, 12, false, true>>(), blocks, 256);
+  if (s.K <= 16) return fn(FrameTag<ClassFrame<T, 16, false, true>>(), blocks, 256);
+  pick_slices<T>(s, fn);
+}
+
+template <typename T, bool REF, bool SUMS, typename Fn>
+static void pick_frame(const ScoresView& s, Fn fn) {
+  if (s.class_major() || s.K < Chunk<T>::VE)
+    pick_class_frame<T>(s, fn);
+  else
+    pick_row_frame<T, REF, SUMS>(s, fn);
 }
 
 }  // namespace wgbm

@@ -4,6 +4,8 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <algorithm>
+
 #include "losses.hpp"
 
 namespace wgbm {
@@ -54,6 +56,97 @@ inline bool rows_fit(const ScoresView& s, bool ref) {
 LOSS_ROWS(f32);
 LOSS_ROWS(bf16);
 LOSS_ROWS(f16);
+
+// Lists of a row's classes: at most kMaxList entries.  scale = log2(e) / tau.
+constexpr int32_t kMaxList = 64;
+struct AltRows {
+  const int32_t* label;  // null: none
+  int32_t k;
+  float scale;
+  double inv_tau;
+  int32_t* classes;  // [n][k]
+  float* log_prob;   // [n][k]
+  float* entropy;
+  float* label_log_prob;
+  float* norm;  // [n][3]
+};
+struct AltGradRows {
+  const float* norm;
+  const int32_t* label;  // null: none
+  const float* grad_label;
+  const int32_t* classes;  // row i's entries at classes + i * class_stride
+  int64_t class_stride;
+  const float* grad_list;
+  int64_t grad_stride;
+  int32_t k;
+  const float* grad_entropy;  // null: 0
+  float scale;
+  double inv_tau;
+};
+struct DistillRows {
+  const int32_t* classes;
+  int64_t class_stride;
+  const float* logits;
+  int64_t logit_stride;
+  int32_t k;
+  bool rest;              // the classes that are not listed count
+  const float* log_norm;  // null: log_norm_all for every row
+  float log_norm_all;
+  const float* weight;  // null: 1
+  float scale;
+  double inv_tau;
+  float tau;
+  float* loss;
+};
+#define LOSS_LISTS(t)                                                                          \
+  int alternatives_##t(const ScoresView& s, const AltRows& g, hipStream_t st);                 \
+  int alternatives_grad_##t(const ScoresView& s, const AltGradRows& g, const ScoresView& out,  \
+                            bool accumulate, hipStream_t st);                                  \
+  int distill_##t(const ScoresView& s, const DistillRows& g, const ScoresView& out,            \
+                  bool accumulate, hipStream_t st)
+LOSS_LISTS(f32);
+LOSS_LISTS(bf16);
+LOSS_LISTS(f16);
+// (class-major rows of more classes than slices hold go through a row-major copy)
+size_t lists_workspace(const ScoresView& s, bool grad);
+int class_alternatives(const ScoresView& s, const AltRows& g, void* ws, hipStream_t st);
+int class_alternatives_grad(const ScoresView& s, const AltGradRows& g, const ScoresView& out,
+                            bool accumulate, void* ws, hipStream_t st);
+int distill_loss(const ScoresView& s, const DistillRows& g, const ScoresView& out, bool accumulate,
+                 void* ws, hipStream_t st);
+// a row of more classes than registers hold in tiles of at most `most` classes, at
+// least 8 each, of whole chunks
+inline void cut_tiles(int32_t K, int32_t most, int32_t* span, int32_t* tiles) {
+  const int32_t n = (K + most - 1) / most;
+  *span = ((K + n - 1) / n + 7) / 8 * 8;
+  *tiles = (K + *span - 1) / *span;
+}
+
+// A grid's threads are counted in 32 bits: rows in registers are launched in
+// parts of fewer (no frame gives a row more than 1024 threads, nor more than its
+// classes and 3).  fn(first row, rows) for each part.
+template <typename Fn>
+static int row_parts(const ScoresView& s, Fn fn) {
+  const int64_t threads = std::min<int64_t>(1024, (int64_t)s.K + 3);
+  const int64_t most = ((int64_t(1) << 32) - 1) / threads / 1024 * 1024;
+  for (int64_t i = 0; i < s.n; i += most) {
+    const int r = fn(i, std::min(most, s.n - i));
+    if (r) return r;
+  }
+  return 0;
+}
+inline ScoresView rows_of(const ScoresView& s, int64_t i, int64_t n) {
+  ScoresView v = s;
+  if (!s.data) return v;
+  v.data = (unsigned char*)s.data + i * s.rs * (s.dtype == kF32 ? 4 : 2);
+  v.n = n;
+  return v;
+}
+
+// class-major scores to a row-major copy of their type or of float32, and a
+// row-major gradient back (added to b where accumulate)
+int scores_to_rows(const ScoresView& a, const ScoresView& b, hipStream_t st);
+int rows_to_scores(const ScoresView& a, const ScoresView& b, bool accumulate, hipStream_t st);
 
 size_t policy_workspace(const ScoresView& s, bool ref);
 int policy_loss(const ScoresView& s, const ScoresView& ref, const PolicyRows& g,

@@ -1,0 +1,80 @@
+// Lists of a row's classes: its best alternatives, and a teacher's.  Arguments
+// and arithmetic shared by alternatives*.hpp and distill.hpp.
+//
+// Scores are divided by a temperature: with m = max s, x = (s - m) / tau and
+// e^x = 2^h, h = (s - m) c, c = log2(e) / tau (the difference first, as
+// in exp_diff).
+#pragma once
+#include "losses_frames.hpp"
+#include "losses_host.hpp"
+
+namespace wgbm {
+
+// below this power an exponential is 0 in float32; products with it take the
+// power no lower (0 * infinity would be NaN)
+constexpr float kLowPower = -1000.0f;
+
+// log(1 + z) of a float32 sum z >= 0 with all its digits
+__device__ __forceinline__ double log_1p(float z) {
+  return z <= 1.0f ? (double)log1p_of(z) : log_of(1.0f + z);
+}
+
+// phi(x) = e^x - 1 - x for |x| <= 1
+__device__ __forceinline__ float phi_small(float x) {
+  float p = 1.0f / 39916800.0f;
+  p = fmaf(p, x, 1.0f / 3628800.0f);
+  p = fmaf(p, x, 1.0f / 362880.0f);
+  p = fmaf(p, x, 1.0f / 40320.0f);
+  p = fmaf(p, x, 1.0f / 5040.0f);
+  p = fmaf(p, x, 1.0f / 720.0f);
+  p = fmaf(p, x, 1.0f / 120.0f);
+  p = fmaf(p, x, 1.0f / 24.0f);
+  p = fmaf(p, x, 1.0f / 6.0f);
+  p = fmaf(p, x, 0.5f);
+  return p * x * x;
+}
+// 1 - e^x
+__device__ __forceinline__ float one_less_exp(float x) {
+  return fabsf(x) <= 1.0f ? -(x + phi_small(x)) : 1.0f - exp_of(x);
+}
+
+// ---------------------------------------------------------------------------
+// ordered keys: a larger score has a larger one, and among equal scores the
+// lower class; -0 and 0 are equal
+// ---------------------------------------------------------------------------
+__device__ __forceinline__ uint32_t order_of(float v) {
+  const uint32_t b = __builtin_bit_cast(uint32_t, v + 0.0f);
+  return b ^ ((uint32_t)((int32_t)b >> 31) | 0x80000000u);
+}
+__device__ __forceinline__ float score_of(uint32_t o) {
+  return __builtin_bit_cast(float, o & 0x80000000u ? o ^ 0x80000000u : ~o);
+}
+constexpr uint32_t kOrderNegInf = 0x007fffffu;  // of -infinity; what lies below are NaNs'
+__device__ __forceinline__ uint64_t key_of(float v, int32_t k) {
+  return (uint64_t)order_of(v) << 32 | (0xffffffffu - (uint32_t)k);
+}
+__device__ __forceinline__ int32_t class_of(uint64_t key) {
+  return (int32_t)(0xffffffffu - (uint32_t)key);
+}
+
+// classes that a row lists twice: whether entry j's class c is that of an
+// earlier one
+template <typename F>
+__device__ __forceinline__ bool listed_before(const F& f, const int32_t* cls, int j, int k,
+                                              int32_t c) {
+  for (int o = 0; o < j; ++o)
+    if (cls[f.entry_at(o, k)] == c) return true;
+  return false;
+}
+
+// a part of a row's classes as a matrix of its own: tile t of tiles, at least 8
+// classes each
+__device__ __forceinline__ ScoresView tile_of(const ScoresView& s, int32_t span, int32_t t) {
+  ScoresView v = s;
+  const int32_t k0 = t * span;
+  v.data = (unsigned char*)s.data + (int64_t)k0 * (s.dtype == kF32 ? 4 : 2);
+  v.K = s.K - k0 < span ? s.K - k0 : span;
+  return v;
+}
+
+}  // namespace wgbm

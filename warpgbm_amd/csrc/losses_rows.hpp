@@ -245,68 +245,6 @@ static bool batch_pays(const ScoresView& s) {
   return s.n >= (int64_t)1024 * F::kRows * B;
 }
 
-// ---------------------------------------------------------------------------
-// which frame a call takes: fn(frame tag, workgroups, threads) for the smallest
-// one that holds the rows (rows_fit).  Row-major rows take two to eight chunks a
-// thread rather than one, so that a wave has more loads in flight and spends
-// what a row costs as a whole on more rows: with one chunk a thread the policy
-// loss of 300000 x 100 float32 takes 57 us instead of 43, of 100000 x 500
-// bfloat16 57 and 40, the log-probabilities' gradient 59 and 44, 47 and 38; 30000 x
-// 3000 bfloat16, eight chunks of a wave's threads instead of two of a
-// workgroup's, whose waves wait for one another: 95 and 65 (not the gradient
-// without sums: 66 and 68).  Up to eight chunks a thread each: log-probabilities'
-// gradient of 300000 x 30 float32 19 us, 20 with two.
-// ---------------------------------------------------------------------------
-template <typename T, bool REF, bool SUMS, typename Fn>
-static void pick_row_frame(const ScoresView& s, Fn fn) {
-  constexpr int VE = Chunk<T>::VE;
-  const int64_t chunks = (s.K + VE - 1) / VE;
-  const auto go = [&](auto tag) {
-    using F = typename decltype(tag)::type;
-    fn(tag, (s.n + F::kRows - 1) / F::kRows, F::kThreads);
-  };
-  if (chunks <= 4) return go(FrameTag<RowFrame<T, 4, 1>>());
-  if (chunks <= 8) return go(FrameTag<RowFrame<T, 8, 1>>());
-  if (chunks <= 16) return go(FrameTag<RowFrame<T, 8, 2>>());
-  if (chunks <= 32) return go(FrameTag<RowFrame<T, 16, 2>>());
-  if (chunks <= 64) return go(FrameTag<RowFrame<T, 32, 2>>());
-  if (chunks <= 128) return go(FrameTag<RowFrame<T, 32, 4>>());
-  if (chunks <= 256) return go(FrameTag<RowFrame<T, 32, 8>>());
-  if constexpr (!SUMS) {
-    if (chunks <= 512) return go(FrameTag<RowFrame<T, 256, 2>>());
-  }
-  if (chunks <= 512) return go(FrameTag<RowFrame<T, 64, 8>>());
-  if (chunks <= 1024) return go(FrameTag<RowFrame<T, 256, 4>>());
-  if (chunks <= 2048) return go(FrameTag<RowFrame<T, 256, 8>>());
-  if (REF || chunks <= 4096) return go(FrameTag<RowFrame<T, 1024, 4>>());
-  if constexpr (!REF) {
-    if (chunks <= 8192) return go(FrameTag<RowFrame<T, 1024, 8>>());
-    go(FrameTag<RowFrame<T, 1024, 16>>());
-  }
-}
-
-template <typename T, typename Fn>
-static void pick_class_frame(const ScoresView& s, Fn fn) {
-  const int64_t blocks = (s.n + 255) / 256;
-  if (!s.class_major()) {  // rows shorter than a chunk
-    if (s.K <= 4) return fn(FrameTag<ClassFrame<T, 4, false, false>>(), blocks, 256);
-    return fn(FrameTag<ClassFrame<T, 8, false, false>>(), blocks, 256);
-  }
-  if (s.K <= 4) return fn(FrameTag<ClassFrame<T, 4, false, true>>(), blocks, 256);
-  if (s.K <= 8) return fn(FrameTag<ClassFrame<T, 8, false, true>>(), blocks, 256);
-  if (s.K <= 12) return fn(FrameTag<ClassFrame<T, 12, false, true>>(), blocks, 256);
-  if (s.K <= 16) return fn(FrameTag<ClassFrame<T, 16, false, true>>(), blocks, 256);
-  pick_slices<T>(s, fn);
-}
-
-template <typename T, bool REF, bool SUMS, typename Fn>
-static void pick_frame(const ScoresView& s, Fn fn) {
-  if (s.class_major() || s.K < Chunk<T>::VE)
-    pick_class_frame<T>(s, fn);
-  else
-    pick_row_frame<T, REF, SUMS>(s, fn);
-}
-
 template <typename T>
 static int log_probs_frames(const ScoresView& s, const int32_t* label, float* log_prob,
                             float* norm, hipStream_t st) {

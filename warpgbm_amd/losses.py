@@ -37,6 +37,11 @@ ClassLogProbs = namedtuple("ClassLogProbs", ["log_prob", "norm"])
 PolicyLoss = namedtuple("PolicyLoss", ["loss", "log_prob", "kl", "grad"])
 BalanceLoss = namedtuple("BalanceLoss", ["loss", "counts", "prob", "grad"])
 PreferenceLoss = namedtuple("PreferenceLoss", ["loss", "margin", "grad"])
+ClassAlternatives = namedtuple("ClassAlternatives",
+                               ["classes", "log_prob", "entropy", "label_log_prob", "norm"])
+DistillLoss = namedtuple("DistillLoss", ["loss", "grad"])
+
+MAX_LIST = 64  # entries of a row's list of classes
 
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 
@@ -205,6 +210,39 @@ def _workspace(entry, v, device):
     return t, t.data_ptr(), nbytes
 
 
+def _list(t, name, dtype, n, k, device):
+    """A [n, k] tensor of dtype on device whose rows are contiguous (any stride from
+    row to row); its address and stride."""
+    if not isinstance(t, torch.Tensor):
+        raise RuntimeError(f"{name} must be a torch.Tensor")
+    if t.dtype != dtype:
+        raise RuntimeError(f"{name} must have dtype {dtype}, got {t.dtype}")
+    if t.device != device:
+        raise RuntimeError(f"{name} must be on {device}, got {t.device}")
+    if t.dim() != 2 or tuple(t.shape) != (n, k):
+        raise RuntimeError(f"{name} must have shape ({n}, {k}), got {tuple(t.shape)}")
+    rs, ks = t.stride()
+    if n <= 1 or k == 0:
+        rs = k
+    if (k > 1 and ks != 1) or rs < k:
+        raise RuntimeError(f"{name} must have the entries of a row next to each other (no overlap), "
+                           f"got strides {t.stride()}")
+    return t.data_ptr(), rs
+
+
+def _length(t, name):
+    if not isinstance(t, torch.Tensor) or t.dim() != 2:
+        raise RuntimeError(f"{name} must be a 2-D torch.Tensor")
+    return t.shape[1]
+
+
+def _temperature(temperature):
+    t = float(temperature)
+    if not 1e-6 <= t <= 1e6:
+        raise RuntimeError(f"temperature must be in [1e-6, 1e6], got {temperature}")
+    return t
+
+
 def class_log_probs(scores, labels) -> ClassLogProbs:
     """Log-probability of each row's label under softmax(scores), and the norm
     [n, 2] of every row (its maximum m and log(sum exp(s - m))), which
@@ -335,6 +373,147 @@ def balance_loss(scores, *, top_k=1, mask=None, coef=1.0, grad=None,
             at, size, _lib.current_stream_ptr(dev))
     _lib.check(rc, "balance_loss")
     return BalanceLoss(loss, counts, prob, out)
+
+
+def class_alternatives(scores, top_k, *, labels=None, temperature=1.0) -> ClassAlternatives:
+    """What a row's scores say under p = softmax(scores / temperature): its best classes,
+    how sure it is, and how likely its label.
+
+    ``classes`` (int32 [n, top_k]) are the top_k classes of largest score, the best
+    first and the lower class first among equal scores, ``log_prob`` (float32 [n,
+    top_k]) their log-probabilities; -1 and -inf where a row has fewer classes.
+    ``entropy`` [n] is that of p, ``label_log_prob`` [n] the log-probability of labels
+    (int32 [n]; None without them; 0 for a label outside [0, K)), and ``norm`` [n, 3]
+    what :func:`class_alternatives_grad` takes: the largest score m,
+    log(sum exp((s - m) / temperature)) and the mean of (m - s) / temperature.
+    A row without a class has entropy 0 and norm (-inf, 0, 0).
+
+    top_k: 0 (no alternatives) to min(64, K)."""
+    v = _matrix(scores, "scores")
+    (n, K), dev = scores.shape, scores.device
+    if isinstance(top_k, bool) or not isinstance(top_k, int) or not 0 <= top_k <= min(MAX_LIST, K):
+        raise RuntimeError(f"top_k must be an integer in [0, min({MAX_LIST}, n_classes)], got {top_k}")
+    tau = _temperature(temperature)
+    lab = _vector(labels, "labels", torch.int32, n, dev) if labels is not None else None
+    f32 = torch.float32
+    lib = _lib.load()
+    with _on(dev):
+        classes = torch.empty((n, top_k), dtype=torch.int32, device=dev)
+        log_prob = torch.empty((n, top_k), dtype=f32, device=dev)
+        entropy = torch.empty(n, dtype=f32, device=dev)
+        norm = torch.empty((n, 3), dtype=f32, device=dev)
+        label = torch.empty(n, dtype=f32, device=dev) if labels is not None else None
+        ws, at, size = _workspace("wgbm_class_alternatives_workspace", v, dev)
+        rc = lib.wgbm_class_alternatives(
+            C.byref(v), lab, top_k, tau, classes.data_ptr(), log_prob.data_ptr(),
+            entropy.data_ptr(), label.data_ptr() if label is not None else None, norm.data_ptr(),
+            at, size, _lib.current_stream_ptr(dev))
+    _lib.check(rc, "class_alternatives")
+    return ClassAlternatives(classes, log_prob, entropy, label, norm)
+
+
+def class_alternatives_grad(scores, norm, *, labels=None, grad_label_log_prob=None, classes=None,
+                            grad_log_prob=None, grad_entropy=None, temperature=1.0,
+                            grad=None) -> torch.Tensor:
+    """Gradient with respect to the scores of
+
+    ``sum_i grad_label_log_prob[i] * label_log_prob[i] + grad_entropy[i] * entropy[i]
+    + sum_j grad_log_prob[i, j] * log p[i, classes[i, j]]``
+
+    (each term where its arguments are given), added to a given ``grad``.  norm and
+    temperature: of :func:`class_alternatives` for the same scores; classes: int32
+    [n, k], its own or any (k at most 64; entries outside [0, K) do not count, one
+    that comes twice counts twice); gradients float32.  Rows whose upstream gradients
+    are all 0 have gradient 0."""
+    v = _matrix(scores, "scores")
+    n, dev = scores.shape[0], scores.device
+    f32 = torch.float32
+    tau = _temperature(temperature)
+    if (labels is None) != (grad_label_log_prob is None):
+        raise RuntimeError("labels and grad_label_log_prob come together")
+    if (classes is None) != (grad_log_prob is None):
+        raise RuntimeError("classes and grad_log_prob come together")
+    if not isinstance(norm, torch.Tensor) or tuple(norm.shape) != (n, 3):
+        raise RuntimeError(f"norm must be a ({n}, 3) tensor")
+    args = _lib.AlternativesGradArgs(temperature=tau)
+    args.norm = _vector(norm.view(-1) if norm.is_contiguous() else norm, "norm", f32, 3 * n, dev)
+    if labels is not None:
+        args.labels = _vector(labels, "labels", torch.int32, n, dev)
+        args.grad_label_log_prob = _vector(grad_label_log_prob, "grad_label_log_prob", f32, n, dev)
+    if classes is not None:
+        k = _length(classes, "classes")
+        if k > MAX_LIST:
+            raise RuntimeError(f"classes must have at most {MAX_LIST} entries a row, got {k}")
+        args.classes, args.classes_stride = _list(classes, "classes", torch.int32, n, k, dev)
+        args.grad_log_prob, args.grad_stride = _list(grad_log_prob, "grad_log_prob", f32, n, k, dev)
+        args.list_length = k
+    if grad_entropy is not None:
+        args.grad_entropy = _vector(grad_entropy, "grad_entropy", f32, n, dev)
+    lib = _lib.load()
+    with _on(dev):
+        out, gv = _grad(grad, v, scores, True, norm, labels, grad_label_log_prob, classes,
+                        grad_log_prob, grad_entropy)
+        ws, at, size = _workspace("wgbm_class_alternatives_grad_workspace", v, dev)
+        rc = lib.wgbm_class_alternatives_grad(C.byref(v), C.byref(args), C.byref(gv),
+                                              int(grad is not None), at, size,
+                                              _lib.current_stream_ptr(dev))
+    _lib.check(rc, "class_alternatives_grad")
+    return out
+
+
+def distill_loss(scores, classes, logits, *, log_norm=None, weight=None, temperature=1.0, grad=None,
+                 with_grad=True) -> DistillLoss:
+    """Divergence of the scores from a teacher of whom each row's best classes are known,
+    and its gradient.
+
+    classes (int32 [n, k], k at most 64; entries outside [0, K) are unused, a class that
+    a row lists again counts the first time only) and logits (float32 [n, k]) are the
+    teacher's list.  With T = temperature and p = softmax(scores / T),
+    ``loss = weight * T^2 * (sum_j q_j log(q_j / p_j) + Q log(Q / P))``, where
+
+    * with ``log_norm`` (float32 [n], or a number for all rows) q_j = exp(logits_j / T -
+      log_norm), and the classes that are not listed count together: Q = 1 - sum q_j is
+      the teacher's share of them, P the scores'.  log_norm is the logarithm of the sum
+      of exp(logit / T) over all the teacher's classes; log-probabilities (of
+      :func:`class_alternatives`, at temperature T, times T) have log_norm 0.  A Q below
+      2^-20 is taken as rounding, and as 0;
+    * without it q is softmax(logits / T) over the list, and Q = 0.
+
+    Listed classes of score -inf do not count, nor does Q where every other class has
+    score -inf; what is left of q and Q is scaled to sum 1.  Rows of weight 0
+    (weight: float32 [n]), without a class, or of whose list nothing counts are left out.
+
+    ``loss`` is float32 [n], ``grad`` the gradient of the losses' sum, added to a given
+    ``grad``, None with ``with_grad=False``."""
+    v = _matrix(scores, "scores")
+    n, dev = scores.shape[0], scores.device
+    f32 = torch.float32
+    k = _length(classes, "classes")
+    if not 1 <= k <= MAX_LIST:
+        raise RuntimeError(f"classes must have 1 to {MAX_LIST} entries a row, got {k}")
+    args = _lib.DistillArgs(list_length=k, temperature=_temperature(temperature))
+    args.classes, args.classes_stride = _list(classes, "classes", torch.int32, n, k, dev)
+    args.logits, args.logits_stride = _list(logits, "logits", f32, n, k, dev)
+    norms = None
+    if log_norm is not None:
+        args.rest = 1
+        if isinstance(log_norm, torch.Tensor):
+            norms = log_norm
+            args.log_norm = _vector(log_norm, "log_norm", f32, n, dev)
+        else:
+            args.log_norm_all = float(log_norm)
+    if weight is not None:
+        args.weight = _vector(weight, "weight", f32, n, dev)
+    lib = _lib.load()
+    with _on(dev):
+        out, gv = _grad(grad, v, scores, with_grad, classes, logits, norms, weight)
+        loss = torch.empty(n, dtype=f32, device=dev)
+        ws, at, size = _workspace("wgbm_distill_loss_workspace", v, dev)
+        rc = lib.wgbm_distill_loss(C.byref(v), C.byref(args), loss.data_ptr(),
+                                   C.byref(gv) if gv is not None else None, int(grad is not None),
+                                   at, size, _lib.current_stream_ptr(dev))
+    _lib.check(rc, "distill_loss")
+    return DistillLoss(loss, out)
 
 
 class PreferencePlan:
