@@ -461,3 +461,417 @@ def test_distill(gpu, dtype, order, rest):
                                        temperature=tau, with_grad=False)
             assert none.grad is None
             check_distill(none, want, w, tau, dtype)
+
+
+# --------------------------------------------------------------------- distillation, edges
+def place(s, order):
+    return s.t().contiguous().t() if order == "class" else s
+
+
+EDGE_CLASSES = [2, 3, 11, 40, 300, 1500, 9000, 70_001]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rest", [False, True])
+@pytest.mark.parametrize("order", ["row", "class"])
+def test_distill_lists_that_leave_little(gpu, order, rest):
+    """Rows whose list the row may not take, whose other classes it may not take, with
+    one class, without a list; a list of all classes; a teacher sure of a class."""
+    from warpgbm_amd import losses
+
+    for K in EDGE_CLASSES:
+        print_case("edges", order, K, rest)
+        n, k = 9, min(K, 12)
+        g = torch.Generator().manual_seed(K)
+        s = torch.randn((n, K), generator=g)
+        cls = torch.argsort(torch.rand((n, K), generator=g), 1)[:, :k].to(torch.int32).contiguous()
+        t = torch.randn((n, K), generator=g)
+        logits = t.gather(1, cls.long())
+        ln = torch.logsumexp(t.double(), 1).float()
+        rows = torch.arange(k)
+        s[0, cls[0].long()] = -INF                      # nothing of the list
+        keep = s[1, cls[1].long()].clone()
+        s[1] = -INF
+        s[1, cls[1].long()] = keep                      # nothing but the list
+        s[2] = -INF
+        s[2, cls[2, 0].long()] = 0.5                    # one class, listed
+        s[3] = -INF
+        s[3, (set(range(K)) - set(cls[3].tolist()) or {0}).__iter__().__next__()] = 0.5
+        cls[4] = -1                                     # no list
+        logits[5] = logits[5, 0]                        # an even teacher
+        logits[6] = -50.0
+        logits[6, 0] = float(ln[6])                     # a sure one
+        s[7, cls[7, : max(1, k // 2)].long()] = -INF    # a part of the list
+        w = 0.5 + torch.rand(n, generator=g)
+        s = place(s, order)
+        norms = ln if rest else None
+        want = distill64(s, cls, logits, norms, w, 1.0)
+        got = losses.distill_loss(to_gpu(s), cls.cuda(), logits.cuda(), weight=w.cuda(),
+                                  log_norm=norms.cuda() if rest else None)
+        check_distill(got, want, w, 1.0, "f32")
+        assert bool(want["live"][0]) == (rest and k < K)
+        assert bool(want["live"][4]) == rest
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("order", ["row", "class"])
+def test_distill_sure_rows_keep_their_digits(gpu, order):
+    """Student and teacher both sure of a class: the gradient there is a difference
+    of numbers next to 1, the rest a difference of small ones."""
+    from warpgbm_amd import losses
+
+    for K in EDGE_CLASSES[1:]:
+        print_case("sure", order, K)
+        s = torch.zeros((4, K))
+        s[:, 0] = torch.tensor([14.0, 12.0, 9.0, 16.0])
+        s[:, 1] = 1.0
+        cls = torch.tensor([[0, 1]] * 4, dtype=torch.int32)
+        left = torch.tensor([4e-5, 1e-4, 3e-3, 8e-6], dtype=F64)  # of the teacher beside class 0
+        logits = torch.stack([torch.log1p(-left), torch.log(0.4 * left)], 1).float()
+        w = torch.ones(4)
+        sp = place(s, order)
+        got = losses.distill_loss(to_gpu(sp), cls.cuda(), logits.cuda(), log_norm=0.0)
+        # shares and probabilities beside class 0, without differences of numbers near 1
+        x = s.to(F64) - s.to(F64)[:, :1]
+        z = torch.exp(x[:, 1:]).sum(1)
+        dp = z / (1 + z)
+        q = logits.to(F64).exp()
+        dq = -torch.expm1(logits[:, 0].to(F64))
+        Q = dq - q[:, 1]
+        p1 = torch.exp(x[:, 1]) / (1 + z)
+        P = dp - p1
+        tol = U * (STEPS + 64) * (dp + dq)
+        check(got.grad[:, 0], dq - dp, tol, "sure class")
+        check(got.grad[:, 1], p1 - q[:, 1], tol, "listed class")
+        r = torch.exp(x[:, 2]) / torch.exp(x[:, 2:]).sum(1)
+        check(got.grad[:, 2], r * (P - Q), tol * r, "other class")
+        # terms q (e^x - 1 - x), a second-order difference
+        want = (torch.special.xlogy(q[:, 1], q[:, 1] / p1) + torch.special.xlogy(Q, Q / P)
+                + q[:, 0] * (torch.log1p(-dq) - torch.log1p(-dp)))
+        gap = (dp - dq).abs() + (p1 - q[:, 1]).abs() + (P - Q).abs()
+        check(got.loss, want, U * ((STEPS + 64) * gap + 64 * (dp + dq)), "loss")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("order", ["row", "class"])
+def test_distill_far_scores_and_lowest_masks(gpu, order, dtype):
+    """Offsets far from 0, and classes masked by the type's lowest number, which
+    count as scores: masked like -inf where the teacher's rest is none."""
+    from warpgbm_amd import losses
+
+    low = torch.finfo(DTYPES[dtype]).min
+    for K in EDGE_CLASSES[1:]:
+        print_case("far", dtype, order, K)
+        g = torch.Generator().manual_seed(K)
+        n, k = 6, 2
+        s = torch.randn((n, K), generator=g)
+        s[0] += 3e4
+        s[1] -= 3e4
+        s = s.to(DTYPES[dtype])
+        cls = torch.argsort(torch.rand((n, K), generator=g), 1)[:, :k].to(torch.int32).contiguous()
+        t = torch.randn((n, k), generator=g)
+        t = (t - torch.logsumexp(t, 1, keepdim=True)).contiguous()  # a teacher of these alone
+        others = torch.ones((n, K), dtype=torch.bool).scatter_(1, cls.long(), False)
+        others[:2] = False
+        w = torch.ones(n)
+        a = losses.distill_loss(to_gpu(place(s.masked_fill(others, low), order)), cls.cuda(),
+                                t.cuda(), log_norm=0.0)
+        b = distill64(place(s.masked_fill(others, -INF), order), cls, t, 0.0, w, 1.0)
+        check_distill(a, b, w, 1.0, dtype)
+        c = losses.distill_loss(to_gpu(place(s.masked_fill(others, low), order)), cls.cuda(),
+                                t.cuda())
+        check_distill(c, distill64(place(s.masked_fill(others, -INF), order), cls, t, None, w, 1.0),
+                      w, 1.0, dtype)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("order", ["row", "class"])
+def test_lists_with_strides(gpu, order):
+    """The first entries of longer lists, and lists inside of other tensors."""
+    from warpgbm_amd import losses
+
+    for n, K in ((37, 12), (37, 90), (20, 700)):
+        s = make_scores(n, K, "f32", order, 3)
+        cls, logits, ln = lists_for(s, 8, 4, 1.0, spare=False)
+        big = torch.full((n, 19), 77, dtype=torch.int32)
+        big[:, 5:13] = cls
+        far = torch.full((n, 11), float("nan"))
+        far[:, 3:11] = logits
+        sd, w = to_gpu(s), torch.ones(n)
+        a = losses.distill_loss(sd, big.cuda()[:, 5:9], far.cuda()[:, 3:7], log_norm=ln.cuda())
+        check_distill(a, distill64(s, cls[:, :4], logits[:, :4], ln, w, 1.0), w, 1.0, "f32")
+        b = losses.distill_loss(sd, cls[:, :4].contiguous().cuda(), logits[:, :4].contiguous().cuda(),
+                                log_norm=ln.cuda())
+        assert torch.equal(a.loss, b.loss) and torch.equal(a.grad, b.grad)
+        f = losses.class_alternatives(sd, 0)
+        up = torch.randn((n, 30), generator=torch.Generator().manual_seed(1)).cuda()
+        x = losses.class_alternatives_grad(sd, f.norm, classes=big.cuda()[:, 5:9],
+                                           grad_log_prob=up[:, 7:11])
+        y = losses.class_alternatives_grad(sd, f.norm, classes=cls[:, :4].contiguous().cuda(),
+                                           grad_log_prob=up[:, 7:11].contiguous())
+        assert torch.equal(x, y)
+
+
+@pytest.mark.gpu
+def test_distill_against_differences(gpu):
+    """The gradient against central differences of the kernel's own losses."""
+    from warpgbm_amd import losses
+
+    n, h = 64, 2.0 ** -6
+    for K in (6, 50, 600):
+        s = make_scores(n, K, "f32", "row", 9, spread=1.0)
+        cls, logits, ln = lists_for(s, 4, 10, 2.0, spare=False)
+        way = torch.randn((n, K), generator=torch.Generator().manual_seed(3))
+
+        def run(x, grad=False):
+            return losses.distill_loss(x.cuda(), cls.cuda(), logits.cuda(), log_norm=ln.cuda(),
+                                       temperature=2.0, with_grad=grad)
+
+        slope = (run(s + h * way).loss.double() - run(s - h * way).loss.double()).cpu() / (2 * h)
+        along = (run(s, True).grad.cpu().double() * way.double()).sum(1)
+        # third derivatives of a log-sum-exp of scores / T are at most 1 / T^3 of the cube of
+        # the direction; two of them, T^2; the losses' own rounding
+        cube = way.abs().max(1).values.double() ** 3
+        assert ((slope - along).abs() <= 2 * cube * h * h / 6 + 64 * 60 * U / h).all()
+
+
+# --------------------------------------------------------------------- together
+def teach(s, t, a, w, k, tau, coef):
+    """A student's step: the teacher's lists, the divergence, the labels."""
+    from warpgbm_amd import losses
+
+    f = losses.class_alternatives(t, k, temperature=tau)
+    r = losses.distill_loss(s, f.classes, f.log_prob * tau, log_norm=0.0, weight=w, temperature=tau)
+    e = losses.class_alternatives(s, 0, labels=a)
+    up = -coef * w
+    g = losses.class_alternatives_grad(s, e.norm, labels=a, grad_label_log_prob=up, grad=r.grad)
+    return f, r, e, g
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("order", ["row", "class"])
+@pytest.mark.parametrize("dtype", list(DTYPES))
+def test_a_student_learns_from_a_teacher(gpu, dtype, order):
+    for n, K, k in ((200, 12, 4), (100, 90, 8), (50, 700, 20), (9, 20_001, 64)):
+        print_case("teach", dtype, order, n, K, k)
+        tau, coef = 2.0, 0.25
+        s = make_scores(n, K, dtype, order, 21, masked=0.1)
+        t = make_scores(n, K, dtype, order, 22)
+        g = torch.Generator().manual_seed(2)
+        a = torch.randint(0, K, (n,), generator=g, dtype=torch.int32)
+        w = 0.5 + torch.rand(n, generator=g)
+        f, r, e, got = teach(to_gpu(s), to_gpu(t), a.cuda(), w.cuda(), k, tau, coef)
+        check_alternatives(f, alternatives64(t, a, k, tau), k, label=False)
+        want = distill64(s, f.classes.cpu(), f.log_prob.cpu() * tau, 0.0, w, tau)
+        assert got.data_ptr() == r.grad.data_ptr()
+        more, tol = alternatives_grad64(s, a, -coef * w, None, None, None, 1.0)
+        # the divergence's gradient was rounded to the type before the labels' came
+        first = want["grad"]
+        total = first + more
+        scale = (w.to(F64) * tau)[:, None]
+        p, q, rr, P, Q = want["p"], want["q"], want["r"], want["P"][:, None], want["Q"][:, None]
+        tol = tol + scale * U * ((STEPS + 4 * want["far"] + 64) * (p + q + rr * (P + Q))
+                                 + (k + 8) * (q + rr))
+        half = U if dtype == "f32" else torch.finfo(DTYPES[dtype]).eps / 2 * (1 + 1e-3)
+        tol = tol + half * (first.abs() + total.abs()) + (2.0 ** -24 if dtype == "f16" else 1e-37)
+        check(got, total, tol, "gradient")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("order", ["row", "class"])
+@pytest.mark.parametrize("K", [12, 90, 700, 20_001])
+def test_graphs_streams_and_same_bits(gpu, K, order):
+    """Two captured steps replayed in turn with eager work between, each replay
+    against the eager result on the same inputs; another stream."""
+    n, k = 64, 8
+    inputs = [[make_scores(n, K, "f32", order, 30 + 2 * j).cuda() for j in range(2)] for _ in "ab"]
+    a = torch.randint(0, K, (n,), dtype=torch.int32).cuda()
+    w = torch.ones(n).cuda()
+    side = torch.cuda.Stream()
+    graphs, outs = [], []
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for s, t in inputs:
+            teach(s, t, a, w, k, 2.0, 0.5)
+    side.synchronize()
+    for s, t in inputs:
+        gr = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(gr):
+            outs.append(teach(s, t, a, w, k, 2.0, 0.5))
+        graphs.append(gr)
+    for turn in range(4):
+        which = turn % 2
+        s, t = inputs[which]
+        s.copy_(make_scores(n, K, "f32", order, 50 + turn))
+        t.copy_(make_scores(n, K, "f32", order, 60 + turn))
+        graphs[which].replay()
+        torch.cuda.synchronize()
+        f, r, e, g = teach(s, t, a, w, k, 2.0, 0.5)
+        F, R, E, G = outs[which]
+        for x, y in ((f.classes, F.classes), (f.log_prob, F.log_prob), (f.norm, F.norm),
+                     (r.loss, R.loss), (e.entropy, E.entropy), (g, G)):
+            assert torch.equal(x, y)
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            other = teach(s, t, a, w, k, 2.0, 0.5)
+        side.synchronize()
+        assert torch.equal(other[3], g) and torch.equal(other[1].loss, r.loss)
+
+
+# --------------------------------------------------------------------- refusals
+def test_float64_forms_against_differences():
+    s = make_scores(9, 7, "f32", "row", 1, masked=0.2).to(F64)
+    cls, logits, ln = lists_for(s, 3, 2, 1.5, spare=False)
+    w, h = torch.ones(9), 1e-5
+    way = torch.randn((9, 7), generator=torch.Generator().manual_seed(1), dtype=F64)
+    for norm in (None, ln):
+        d = distill64(s, cls, logits, norm, w, 1.5)
+        up = distill64(s + h * way, cls, logits, norm, w, 1.5)["loss"]
+        down = distill64(s - h * way, cls, logits, norm, w, 1.5)["loss"]
+        finite = torch.where(s > -INF, way, torch.zeros((), dtype=F64))
+        assert torch.allclose((up - down) / (2 * h), (d["grad"] * finite).sum(1), atol=1e-7)
+
+
+def test_refusals_without_a_gpu():
+    from warpgbm_amd import losses
+
+    s = torch.zeros((4, 8))
+    c, x = torch.zeros((4, 2), dtype=torch.int32), torch.zeros((4, 2))
+    for call in (lambda: losses.class_alternatives(s, 2),
+                 lambda: losses.class_alternatives_grad(s, torch.zeros((4, 3))),
+                 lambda: losses.distill_loss(s, c, x)):
+        with pytest.raises(RuntimeError, match="GPU tensor"):
+            call()
+    cpu = torch.device("cpu")
+    with pytest.raises(RuntimeError, match="dtype"):
+        losses._list(c.long(), "classes", torch.int32, 4, 2, cpu)
+    with pytest.raises(RuntimeError, match="shape"):
+        losses._list(c, "classes", torch.int32, 4, 3, cpu)
+    with pytest.raises(RuntimeError, match="next to each other"):
+        losses._list(c.t().contiguous().t(), "classes", torch.int32, 4, 2, cpu)
+    with pytest.raises(RuntimeError, match="next to each other"):
+        losses._list(c[:1].expand(4, 2), "classes", torch.int32, 4, 2, cpu)
+    assert losses._list(c[:1], "classes", torch.int32, 1, 2, cpu)[1] == 2
+    assert losses._list(torch.zeros((4, 9), dtype=torch.int32)[:, :1], "c", torch.int32, 4, 1,
+                        cpu)[1] == 9
+    for t in (0.0, -1.0, INF, float("nan")):
+        with pytest.raises(RuntimeError, match="temperature"):
+            losses._temperature(t)
+
+
+def test_c_entries_refuse_before_any_launch():
+    from warpgbm_amd import _lib
+
+    lib = _lib.load()
+    one = 16  # never dereferenced
+
+    def scores(**kw):
+        f = dict(data=one, dtype=0, n_rows=4, n_classes=8, row_stride=8, class_stride=1)
+        f.update(kw)
+        return _lib.Scores(*f.values())
+
+    def refused(rc, text):
+        msg = lib.wgbm_last_error().decode()
+        assert rc == 1000 and text in msg, (rc, msg)
+
+    def alternatives(s=None, k=2, tau=1.0, labels=None, label=one, out=one, ws=0):
+        return lib.wgbm_class_alternatives(C.byref(s or scores()), labels, k, tau, out, out, one,
+                                           label, one, None if ws == 0 else one, ws, None)
+
+    refused(alternatives(k=-1), "length")
+    refused(alternatives(k=65, s=scores(n_classes=100, row_stride=100)), "length")
+    refused(alternatives(k=9), "top_k")
+    refused(alternatives(tau=0.0), "temperature")
+    refused(alternatives(tau=float("nan")), "temperature")
+    refused(alternatives(labels=one, label=None), "null pointer")
+    refused(alternatives(out=None), "null pointer")
+    refused(alternatives(s=scores(dtype=9)), "type code")
+    wide = dict(n_classes=600, row_stride=1, class_stride=4)
+    refused(alternatives(s=scores(**wide)), "workspace too small")
+    refused(alternatives(s=scores(**wide), ws=4 * 600 * 4 - 1), "workspace too small")
+    assert lib.wgbm_class_alternatives_workspace(C.byref(scores(**wide))) == 4 * 600 * 4
+    assert lib.wgbm_class_alternatives_workspace(C.byref(scores(**wide, dtype=1))) == 4 * 600 * 2
+    assert lib.wgbm_distill_loss_workspace(C.byref(scores(**wide, dtype=1))) == 4 * 600 * 4
+    assert lib.wgbm_class_alternatives_grad_workspace(C.byref(scores())) == 0
+    assert lib.wgbm_distill_loss_workspace(C.byref(scores(dtype=7))) == -1
+    assert alternatives(s=scores(n_rows=0)) == 0
+
+    def grad(out=None, **kw):
+        f = dict(norm=one, labels=None, grad_label_log_prob=None, classes=one, classes_stride=2,
+                 grad_log_prob=one, grad_stride=2, list_length=2, grad_entropy=None,
+                 temperature=1.0)
+        f.update(kw)
+        args = _lib.AlternativesGradArgs(*f.values())
+        return lib.wgbm_class_alternatives_grad(C.byref(scores()), C.byref(args),
+                                                C.byref(out or scores()), 0, None, 0, None)
+
+    refused(grad(list_length=65, classes_stride=65, grad_stride=65), "length")
+    refused(grad(classes_stride=1), "stride")
+    refused(grad(grad_stride=1), "stride")
+    refused(grad(temperature=-1.0), "temperature")
+    refused(grad(norm=None), "null pointer")
+    refused(grad(labels=one), "null pointer")
+    refused(grad(classes=None), "null pointer")
+    refused(grad(out=scores(dtype=1)), "shape and type")
+    refused(grad(out=scores(row_stride=1, class_stride=8)), "order")
+
+    def distill(out=None, **kw):
+        f = dict(classes=one, classes_stride=2, logits=one, logits_stride=2, list_length=2, rest=0,
+                 log_norm=None, log_norm_all=0.0, weight=None, temperature=1.0)
+        f.update(kw)
+        args = _lib.DistillArgs(*f.values())
+        return lib.wgbm_distill_loss(C.byref(scores()), C.byref(args), one,
+                                     C.byref(out) if out else None, 0, None, 0, None)
+
+    refused(distill(list_length=0), "length")
+    refused(distill(list_length=65), "length")
+    refused(distill(classes_stride=1), "stride")
+    refused(distill(logits_stride=1 << 41), "stride")
+    refused(distill(temperature=0.0), "temperature")
+    refused(distill(rest=1, log_norm_all=INF), "log_norm")
+    refused(distill(classes=None), "null pointer")
+    refused(distill(logits=None), "null pointer")
+    refused(distill(out=scores(n_classes=7)), "shape and type")
+
+
+@pytest.mark.gpu
+def test_refusals_on_the_gpu(gpu):
+    from warpgbm_amd import losses
+
+    s = torch.zeros((4, 8)).cuda()
+    c, x = torch.zeros((4, 2), dtype=torch.int32).cuda(), torch.zeros((4, 2)).cuda()
+    v = torch.zeros(4).cuda()
+    f = losses.class_alternatives(s, 2)
+
+    def no(text, call):
+        with pytest.raises(RuntimeError, match=text):
+            call()
+
+    for k in (-1, 9, 2.0, True, None):
+        no("top_k", lambda: losses.class_alternatives(s, k))
+    no("labels must have dtype", lambda: losses.class_alternatives(s, 2, labels=v))
+    no("come together", lambda: losses.class_alternatives_grad(s, f.norm, labels=c[:, 0]))
+    no("come together", lambda: losses.class_alternatives_grad(s, f.norm, classes=c))
+    no("norm must be", lambda: losses.class_alternatives_grad(s, f.norm[:, :2], grad_entropy=v))
+    no("must have shape", lambda: losses.class_alternatives_grad(
+        s, f.norm, classes=c, grad_log_prob=x[:, :1]))
+    no("at most 64", lambda: losses.class_alternatives_grad(
+        s, f.norm, classes=torch.zeros((4, 65), dtype=torch.int32).cuda(),
+        grad_log_prob=torch.zeros((4, 65)).cuda()))
+    no("share", lambda: losses.class_alternatives_grad(s, f.norm, grad_entropy=v, grad=s))
+    whole = torch.zeros(64).cuda()
+    no("share", lambda: losses.class_alternatives_grad(
+        s, whole[:12].view(4, 3), grad_entropy=v, grad=whole[:32].view(4, 8)))
+    no("share", lambda: losses.distill_loss(s, c, whole[10:18].view(4, 2),
+                                            grad=whole[:32].view(4, 8)))
+    no("1 to 64", lambda: losses.distill_loss(s, c[:, :0], x[:, :0]))
+    no("must have dtype", lambda: losses.distill_loss(s, c.long(), x))
+    no("must have dtype", lambda: losses.distill_loss(s, c, x.double()))
+    no("must be on", lambda: losses.distill_loss(s, c.cpu(), x))
+    no("must have shape", lambda: losses.distill_loss(s, c, x[:3]))
+    no("must have shape", lambda: losses.distill_loss(s, c, x, weight=v[:3]))
+    no("must have shape", lambda: losses.distill_loss(s, c, x, log_norm=v[:3]))
+    no("log_norm", lambda: losses.distill_loss(s, c, x, log_norm=INF))
+    no("with_grad", lambda: losses.distill_loss(s, c, x, grad=torch.zeros_like(s), with_grad=False))
+    no("temperature", lambda: losses.distill_loss(s, c, x, temperature=0))

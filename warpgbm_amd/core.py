@@ -15,12 +15,13 @@ reference's recursive per-node Python loop.  The trees are the same: the
 residual is fixed per tree (core.py:719), each node's decision depends only
 on its own rows, and histogram sums are exact (see include/warpgbm_amd.h).
 
-Three objectives have no counterpart in the reference; their rounds fit the
+Four objectives have no counterpart in the reference; their rounds fit the
 trees to the negative gradient of a loss of ``warpgbm_amd.losses``:
 ``"preference"`` (a scorer from pairs of rows or of sequences of rows),
 ``"policy"`` (class probabilities from logged decisions and their advantages:
-the clipped policy loss with a KL and a balance term) and
-``"policy_preference"`` (class probabilities from pairs of decision sequences).
+the clipped policy loss with KL, balance and entropy terms),
+``"policy_preference"`` (class probabilities from pairs of decision sequences) and
+``"distill"`` (class probabilities from a teacher's best classes of each row).
 """
 from __future__ import annotations
 
@@ -42,10 +43,11 @@ from .metrics import accuracy_torch, log_loss_torch, rmsle_torch, softmax
 # objectives whose rounds fit one tree to one score a row, and those that fit a
 # tree a class
 _SCORE_OBJECTIVES = ("regression", "preference")
-_CLASS_OBJECTIVES = ("multiclass", "binary", "policy", "policy_preference")
+_CLASS_OBJECTIVES = ("multiclass", "binary", "policy", "policy_preference", "distill")
 # objectives whose gradients come from warpgbm_amd.losses
-_LOSS_OBJECTIVES = ("preference", "policy", "policy_preference")
-_LOSS_PARAMS = ("beta", "label_smoothing", "clip", "kl_coef", "balance_coef", "balance_top_k")
+_LOSS_OBJECTIVES = ("preference", "policy", "policy_preference", "distill")
+_LOSS_PARAMS = ("beta", "label_smoothing", "clip", "kl_coef", "balance_coef", "balance_top_k",
+                "entropy_coef", "temperature", "label_coef")
 
 _TIMING = os.environ.get("WGBM_TIMING", "") not in ("", "0")
 # predict inputs from this many rows on read only the forest's split columns
@@ -254,6 +256,9 @@ class WarpGBM(BaseEstimator, RegressorMixin):
         kl_coef=0.0,
         balance_coef=0.0,
         balance_top_k=1,
+        entropy_coef=0.0,
+        temperature=1.0,
+        label_coef=0.0,
     ):
         self._validate_hyperparams(
             objective=objective,
@@ -269,7 +274,7 @@ class WarpGBM(BaseEstimator, RegressorMixin):
             colsample_bytree=colsample_bytree,
         )
         self._validate_loss_params(beta, label_smoothing, clip, kl_coef, balance_coef,
-                                   balance_top_k)
+                                   balance_top_k, entropy_coef, temperature, label_coef)
         self.objective = objective
         self.num_bins = num_bins
         self.max_depth = max_depth
@@ -294,6 +299,10 @@ class WarpGBM(BaseEstimator, RegressorMixin):
         self.kl_coef = kl_coef
         self.balance_coef = balance_coef
         self.balance_top_k = balance_top_k
+        self.entropy_coef = entropy_coef
+        # of the objective "distill"
+        self.temperature = temperature
+        self.label_coef = label_coef
         self.forest = [{} for _ in range(self.n_estimators)]
         self.bin_edges = None
         self.base_prediction = None
@@ -315,8 +324,8 @@ class WarpGBM(BaseEstimator, RegressorMixin):
         """Same checks and messages as warpgbm/core.py:83-143."""
         if kwargs["objective"] not in _SCORE_OBJECTIVES + _CLASS_OBJECTIVES:
             raise ValueError(
-                "objective must be 'regression', 'binary', 'multiclass', 'preference', 'policy', or "
-                f"'policy_preference', got {kwargs['objective']}."
+                "objective must be 'regression', 'binary', 'multiclass', 'preference', 'policy', "
+                f"'policy_preference', or 'distill', got {kwargs['objective']}."
             )
         int_params = ["num_bins", "max_depth", "n_estimators", "min_child_weight",
                       "threads_per_block", "rows_per_thread"]
@@ -351,9 +360,12 @@ class WarpGBM(BaseEstimator, RegressorMixin):
             )
 
     @staticmethod
-    def _validate_loss_params(beta, label_smoothing, clip, kl_coef, balance_coef, balance_top_k):
+    def _validate_loss_params(beta, label_smoothing, clip, kl_coef, balance_coef, balance_top_k,
+                              entropy_coef, temperature, label_coef):
         for name, v in (("beta", beta), ("label_smoothing", label_smoothing),
-                        ("kl_coef", kl_coef), ("balance_coef", balance_coef)):
+                        ("kl_coef", kl_coef), ("balance_coef", balance_coef),
+                        ("entropy_coef", entropy_coef), ("temperature", temperature),
+                        ("label_coef", label_coef)):
             if not isinstance(v, (float, int)):
                 raise TypeError(f"{name} must be a float, got {type(v)}.")
         if not (isinstance(clip, (tuple, list)) and len(clip) == 2
@@ -371,6 +383,12 @@ class WarpGBM(BaseEstimator, RegressorMixin):
             raise ValueError("kl_coef and balance_coef must be non-negative and finite.")
         if not (1 <= balance_top_k <= 8):
             raise ValueError("balance_top_k must be between 1 and 8 inclusive.")
+        if not (0 <= entropy_coef < float("inf")):
+            raise ValueError("entropy_coef must be non-negative and finite.")
+        if not (1e-6 <= temperature <= 1e6):
+            raise ValueError("temperature must be in [1e-6, 1e6].")
+        if not (0 <= label_coef <= 1):
+            raise ValueError("label_coef must be in [0, 1].")
 
     def validate_fit_params(self, X, y, era_id, X_eval, y_eval, eval_every_n_trees,
                             early_stopping_rounds, eval_metric):
@@ -424,7 +442,7 @@ class WarpGBM(BaseEstimator, RegressorMixin):
     def fit(self, X, y, era_id=None, X_eval=None, y_eval=None, eval_every_n_trees=None,
             early_stopping_rounds=None, eval_metric="mse", *, pairs=None, segments=None,
             pair_weight=None, advantage=None, behavior_log_prob=None, reference=None,
-            sample_weight=None):
+            sample_weight=None, teacher_classes=None, teacher_logits=None, teacher_log_norm=None):
         """Train.  The arguments after ``eval_metric`` belong to the objectives
         without a counterpart in the reference:
 
@@ -439,18 +457,28 @@ class WarpGBM(BaseEstimator, RegressorMixin):
         policy not to leave too far (log-probabilities [n] of the decisions, or
         scores [n, K] of all classes, which count by ``kl_coef``),
         ``sample_weight`` [n] (0: left out).  ``balance_coef`` adds the balance
-        loss over the ``balance_top_k`` best classes of a row.
+        loss over the ``balance_top_k`` best classes of a row, ``entropy_coef`` takes
+        that much of the policy's entropy from each row's loss.
 
         ``"policy_preference"``: y holds the decisions, ``pairs`` / ``segments``
         / ``pair_weight`` as above, ``reference`` [n] the decisions' reference
         log-probabilities.  Policies start uniform.
+
+        ``"distill"``: y holds the labels, ``teacher_classes`` [n, k] (k at most 64) a
+        teacher's best classes of each row as columns of ``classes_`` (-1: none) and
+        ``teacher_logits`` [n, k] its scores of them: the loss is their divergence at
+        ``temperature`` (``warpgbm_amd.losses.distill_loss``), which counts the classes
+        that are not listed as one with ``teacher_log_norm`` [n] (the logarithm of the
+        sum of exp(logit / temperature) over all classes).  ``label_coef`` of the loss
+        is the labels' cross entropy instead; ``sample_weight`` [n].
 
         ``training_loss`` then has each round's mean loss before its trees."""
         early_stopping_rounds = self.validate_fit_params(
             X, y, era_id, X_eval, y_eval, eval_every_n_trees, early_stopping_rounds, eval_metric)
         given = dict(pairs=pairs, segments=segments, pair_weight=pair_weight, advantage=advantage,
                      behavior_log_prob=behavior_log_prob, reference=reference,
-                     sample_weight=sample_weight)
+                     sample_weight=sample_weight, teacher_classes=teacher_classes,
+                     teacher_logits=teacher_logits, teacher_log_norm=teacher_log_norm)
         self._validate_loss_inputs(X.shape[0], given, X_eval)
         # random_state seeds the global RNGs as the reference does
         # (warpgbm/core.py:308-314); colsample_bytree subsets are then drawn
@@ -779,8 +807,11 @@ class WarpGBM(BaseEstimator, RegressorMixin):
         takes = {"preference": ("pairs", "segments", "pair_weight"),
                  "policy": ("advantage", "behavior_log_prob", "reference", "sample_weight"),
                  "policy_preference": ("pairs", "segments", "pair_weight", "reference"),
+                 "distill": ("teacher_classes", "teacher_logits", "teacher_log_norm",
+                             "sample_weight"),
                  }.get(self.objective, ())
-        needs = {"preference": "pairs", "policy": "advantage", "policy_preference": "pairs"}
+        needs = {"preference": ("pairs",), "policy": ("advantage",),
+                 "policy_preference": ("pairs",), "distill": ("teacher_classes", "teacher_logits")}
         for name, a in given.items():
             if a is not None and name not in takes:
                 raise ValueError(f"{name} is not an argument of the objective '{self.objective}'.")
@@ -788,17 +819,27 @@ class WarpGBM(BaseEstimator, RegressorMixin):
                 raise TypeError(f"{name} must be a numpy array.")
         if self.objective not in _LOSS_OBJECTIVES:
             return
-        if given[needs[self.objective]] is None:
-            raise ValueError(f"objective '{self.objective}' needs {needs[self.objective]}.")
+        for name in needs[self.objective]:
+            if given[name] is None:
+                raise ValueError(f"objective '{self.objective}' needs {name}.")
         if X_eval is not None:
             raise ValueError(f"objective '{self.objective}' takes no eval set.")
-        for name in ("advantage", "behavior_log_prob", "sample_weight"):
+        for name in ("advantage", "behavior_log_prob", "sample_weight", "teacher_log_norm"):
             if given[name] is not None and given[name].shape != (n,):
                 raise ValueError(f"{name} must have shape ({n},), got {given[name].shape}.")
         ref = given["reference"]
         if ref is not None and ref.shape != (n,) and not (
                 self.objective == "policy" and ref.ndim == 2 and ref.shape[0] == n):
             raise ValueError(f"reference must have one entry per row ({n}), got {ref.shape}.")
+        tc, tl = given["teacher_classes"], given["teacher_logits"]
+        if tc is not None:
+            if tc.ndim != 2 or tc.shape[0] != n or not 1 <= tc.shape[1] <= L.MAX_LIST:
+                raise ValueError(f"teacher_classes must have shape ({n}, k) with k in "
+                                 f"[1, {L.MAX_LIST}], got {tc.shape}.")
+            if not np.issubdtype(tc.dtype, np.integer):
+                raise TypeError(f"teacher_classes must be integers, got {tc.dtype}.")
+            if tl.shape != tc.shape:
+                raise ValueError(f"teacher_logits must have shape {tc.shape}, got {tl.shape}.")
         pairs, seg, w = given["pairs"], given["segments"], given["pair_weight"]
         if pairs is not None:
             if pairs.ndim != 2 or pairs.shape[1] != 2 or pairs.shape[0] < 1:
@@ -842,6 +883,10 @@ class WarpGBM(BaseEstimator, RegressorMixin):
             count = n if w is None else int(live.sum())
             total = float(n) if w is None else float(w.double().sum())
             view = scores.t()
+            bonus = None
+            if self.entropy_coef:
+                bonus = torch.full((n,), -self.entropy_coef, dtype=torch.float32, device=dev)
+                bonus = bonus if w is None else bonus * w
 
             def step():
                 r = L.policy_loss(view, actions, old, adv, weight=w, ref_log_prob=ref_lp,
@@ -851,6 +896,37 @@ class WarpGBM(BaseEstimator, RegressorMixin):
                     e = L.balance_loss(view, top_k=min(self.balance_top_k, K), mask=live,
                                        coef=self.balance_coef * count, grad=r.grad)
                     loss = loss + e.loss
+                if bonus is not None:
+                    f = L.class_alternatives(view, 0)
+                    L.class_alternatives_grad(view, f.norm, grad_entropy=bonus, grad=r.grad)
+                    loss = loss + (bonus * f.entropy).sum()
+                return r.grad, loss
+
+            return step, total
+        if self.objective == "distill":
+            labels = torch.from_numpy(np.asarray(y).astype(np.int32)).to(dev)
+            tc = given["teacher_classes"]
+            # (numbers outside the classes, -1 among them, are unused entries)
+            classes = torch.from_numpy(np.where((tc >= 0) & (tc < K), tc, -1).astype(np.int32)).to(dev)
+            logits, log_norm = rows(given["teacher_logits"]), rows(given["teacher_log_norm"])
+            w = rows(given["sample_weight"])
+            total = float(n) if w is None else float(w.double().sum())
+            part = w
+            by_label = None
+            if self.label_coef:
+                whole = torch.ones(n, dtype=torch.float32, device=dev) if w is None else w
+                part, by_label = whole * (1.0 - self.label_coef), whole * -self.label_coef
+            view = scores.t()
+
+            def step():
+                r = L.distill_loss(view, classes, logits, log_norm=log_norm, weight=part,
+                                   temperature=self.temperature)
+                loss = r.loss.sum()
+                if by_label is not None:
+                    f = L.class_alternatives(view, 0, labels=labels)
+                    L.class_alternatives_grad(view, f.norm, labels=labels,
+                                              grad_label_log_prob=by_label, grad=r.grad)
+                    loss = loss + (by_label * f.label_log_prob).sum()
                 return r.grad, loss
 
             return step, total
@@ -1247,6 +1323,28 @@ class WarpGBM(BaseEstimator, RegressorMixin):
         scores = self._infer(X_np, self.num_classes)
         r = L.class_log_probs(scores, torch.from_numpy(labels).to(scores.device))
         return D.to_host(r.log_prob)
+
+    def alternatives(self, X_np, top_k=5, y=None, temperature=1.0):
+        """Each row's best classes and how sure the forest is of them: a
+        ``losses.ClassAlternatives`` of host arrays, ``classes`` [n, k] (columns of
+        ``classes_``, the best first; k = min(top_k, number of classes)), their
+        ``log_prob`` [n, k], the ``entropy`` [n] and, with labels y,
+        ``label_log_prob`` [n], of softmax(scores / temperature).  ``classes`` with
+        ``log_prob * temperature`` and a log norm of 0 is a teacher's list for the
+        objective "distill" at that temperature."""
+        if self.objective not in _CLASS_OBJECTIVES:
+            raise ValueError("alternatives only available for objectives with classes")
+        labels = None
+        if y is not None:
+            labels = self.label_encoder.transform(np.asarray(y)).astype(np.int32)
+            if labels.shape[0] != np.asarray(X_np).shape[0]:
+                raise ValueError("X and y must have the same number of rows.")
+        scores = self._infer(X_np, self.num_classes)
+        if labels is not None:
+            labels = torch.from_numpy(labels).to(scores.device)
+        r = L.class_alternatives(scores, min(top_k, self.num_classes), labels=labels,
+                                 temperature=temperature)
+        return L.ClassAlternatives(*(None if t is None else D.to_host(t) for t in r))
 
     # ------------------------------------------------------------------ importance
     @staticmethod
