@@ -185,16 +185,38 @@ __device__ __forceinline__ uint64_t next_key(uint64_t below, uint64_t* buf, Fn b
   return key;
 }
 
+// the row's best classes in turns, read from memory again
+template <typename T, int NW>
+__device__ __forceinline__ void take_turns(const ScoresView& s, const AltRow& r, const AltRows& g,
+                                           int64_t i, int t, uint64_t* buf) {
+  uint64_t below = ~0ull;
+  for (int32_t e = 0; e < g.k; ++e) {
+    below = next_key<NW>(below, buf, [&](uint64_t under) {
+      uint64_t best = 0;
+      for (int32_t k = t; k < s.K; k += 64 * NW) {
+        const float x = score_at<T>(s, i, k);
+        const uint64_t key = key_of(x, k);
+        if (x > -__builtin_inff() && key < under && key > best) best = key;
+      }
+      return best;
+    });
+    if (t == 0)
+      write_alternative(r, g, i, e, below ? class_of(below) : -1,
+                        score_of((uint32_t)(below >> 32)));
+  }
+}
+
 template <typename F>
 __global__ __launch_bounds__(F::kMax) void alternatives_candidates_kernel(ScoresView s,
                                                                           AltRows g) {
-  constexpr int NW = F::G / 64, R = F::kRows, kHold = NW == 1 ? 256 : 512;
+  using T = typename F::T;
+  constexpr int NW = F::G / 64, R = F::kRows, VE = F::VE, kHold = NW == 1 ? 256 : 512;
   static_assert(F::G >= 64, "a row is a wave's or a workgroup's");
   __shared__ uint64_t cand[R][kHold];
   __shared__ uint32_t part[NW == 1 ? 1 : 256];
   __shared__ uint64_t key_buf[NW];
-  __shared__ float buf[3 * F::kBuf], most[F::kBuf];
-  __shared__ int count;
+  __shared__ float buf[2][2 * F::kBuf], most[F::kBuf];
+  __shared__ int counts[R];
   __shared__ float from_share;
   const F f(s);
   const int64_t row = F::row(blockIdx.x);
@@ -203,17 +225,34 @@ __global__ __launch_bounds__(F::kMax) void alternatives_candidates_kernel(Scores
   typename F::Regs v;
   f.load(v, s, blockIdx.x);
   const int32_t lab = row_label(g.label, i, s.K);
-  const float sa = lab >= 0 ? score_at<typename F::T>(s, i, lab) : 0.0f;
-  if (NW > 1 && threadIdx.x == 0) count = 0;
+  const float sa = lab >= 0 ? score_at<T>(s, i, lab) : 0.0f;
+  int* const count = &counts[threadIdx.x / F::G];
+  if (f.first_lane()) *count = 0;
   f.trim(v);
-  float half[2] = {-__builtin_inff(), -__builtin_inff()};
+  // the chunks' maxima: a candidate is looked for in a chunk that has one
+  float top[F::NC];
+  float m = -__builtin_inff(), half = m;
 #pragma unroll
-  for (int j = 0; j < F::N; ++j) half[j >= F::N / 2] = fmaxf(half[j >= F::N / 2], F::value(v, j));
-  float m = fmaxf(half[0], half[1]);
+  for (int c = 0; c < F::NC; ++c) {
+    top[c] = F::value(v, c * VE);
+#pragma unroll
+    for (int e = 1; e < VE; ++e) {
+      top[c] = fmaxf(top[c], F::value(v, c * VE + e));
+      if (F::NC == 1 && e == VE / 2 - 1) half = top[0];
+    }
+    m = fmaxf(m, top[c]);
+    if (F::NC > 1 && c == F::NC / 2 - 1) half = m;
+  }
+  const float own = m;
   float from = 0.0f;
   if constexpr (NW == 1) {
     if (g.k > 0) {
-      const uint32_t key[2] = {order_of(half[0]), order_of(half[1])};
+      // 128 parts: the halves of a lane's classes (the second one's maximum is m, or
+      // another one that is no larger)
+      float other = -__builtin_inff();
+#pragma unroll
+      for (int j = F::N / 2; j < F::N; ++j) other = fmaxf(other, F::value(v, j));
+      const uint32_t key[2] = {order_of(half), order_of(other)};
       from = kth_at_least<2>(key, g.k);
     }
   } else {
@@ -230,65 +269,65 @@ __global__ __launch_bounds__(F::kMax) void alternatives_candidates_kernel(Scores
     const float t = kth_at_least<4>(key, g.k);
     if (threadIdx.x == 0) from_share = t;
   }
-  if (F::kHide) f.hide(v);
-  AltSums a[2] = {};
+  if (F::N >= 32) f.hide(v);
+  float z[2] = {0.0f, 0.0f}, u[2] = {0.0f, 0.0f};
 #pragma unroll
-  for (int j = 0; j < F::N; ++j) add_score(a[j % 2], F::value(v, j), m, ms, g.scale);
-  float sum[3] = {a[0].z + a[1].z, a[0].u + a[1].u, a[0].ties + a[1].ties};
-  f.template reduce_all<3>(sum, AddF(), buf);
-  const AltRow r = alt_row(AltSums{sum[0], sum[1], sum[2]}, m);
-  if (f.first_lane()) write_alt_row(r, g, i, lab, sa);
-  if (g.k == 0) return;
-  if (F::kHide) f.hide(v);
-  uint64_t* const list = cand[threadIdx.x / F::G];
-  int n = 0;
-  if constexpr (NW == 1) {
+  for (int j = 0; j < F::N; ++j) {
+    const float h = (F::value(v, j) - ms) * g.scale, e = exp2_f32(h);
+    z[j % 2] += e;
+    u[j % 2] = fmaf(e, fmaxf(h, kLowPower), u[j % 2]);
+  }
+  float sum[2] = {z[0] + z[1], u[0] + u[1]};
+  f.template reduce_all<2>(sum, AddF(), buf[0]);
+  // the sum without its largest term: where it is small next to that, once more
+  // from the scores below the maximum (a row without a class: 0 or NaN)
+  AltSums a{sum[0] - 1.0f, sum[1], 1.0f};
+  if (!(a.z >= 0.125f)) {
+    f.hide(v);  // (or the compiler would keep the first pass's numbers for this one)
+    float again[2] = {0.0f, 0.0f};
 #pragma unroll
     for (int j = 0; j < F::N; ++j) {
       const float x = F::value(v, j);
-      const uint64_t who = __ballot(x >= from);
-      if (who == 0) continue;
-      const int at = n + __popcll(who & ((1ull << (threadIdx.x & 63)) - 1));
-      if (x >= from && at < kHold) list[at] = key_of(x, f.cls(j));
-      n += __popcll(who);
+      again[0] += x == m ? 0.0f : exp2_f32((x - ms) * g.scale);
+      again[1] += x == m ? 1.0f : 0.0f;
     }
-  } else {
-    from = from_share;
-    if (half[0] >= from || half[1] >= from) {
+    f.template reduce_all<2>(again, AddF(), buf[1]);
+    a.z = again[0];
+    a.ties = again[1];
+  }
+  const AltRow r = alt_row(a, m);
+  if (f.first_lane()) write_alt_row(r, g, i, lab, sa);
+  if (g.k == 0) return;
+  if (NW > 1) from = from_share;
+  uint64_t* const list = cand[threadIdx.x / F::G];
+  if (own >= from) {
+    uint32_t has = 0;
 #pragma unroll
-      for (int j = 0; j < F::N; ++j) {
-        const float x = F::value(v, j);
-        if (x >= from) {
-          const int at = atomicAdd(&count, 1);
-          if (at < kHold) list[at] = key_of(x, f.cls(j));
+    for (int c = 0; c < F::NC; ++c) has |= top[c] >= from ? 1u << c : 0u;
+    const T* p = (const T*)s.data + i * s.rs;
+    for (; has; has &= has - 1) {
+      const int c = __ffs(has) - 1;
+      const int32_t k = f.first(c), skip = f.skip(c);
+      const Chunk<T> x = load_chunk<T>(p + (uint32_t)k);
+#pragma unroll
+      for (int e = 0; e < VE; ++e) {
+        const float y = x.get(e);
+        if (y >= from && e >= skip) {
+          const int at = atomicAdd(count, 1);
+          if (at < kHold) list[at] = key_of(y, k + e);
         }
       }
     }
+  }
+  if (NW > 1)
     __syncthreads();
-    n = count;
-  }
-  if (n <= kHold) {
-    // (a wave's own list: its writes are done before it reads)
-    if (NW == 1) __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");
+  else
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");  // (a wave's own list)
+  const int n = *(volatile int*)count;
+  if (n <= kHold)
     rank_candidates(list, n, threadIdx.x % F::G, F::G, r, g, i);
-    return;
-  }
-  uint64_t below = ~0ull;
-  for (int32_t t = 0; t < g.k; ++t) {
-    below = next_key<NW>(below, key_buf, [&](uint64_t under) {
-      uint64_t best = 0;
-#pragma unroll
-      for (int j = 0; j < F::N; ++j) {
-        const float x = F::value(v, j);
-        const uint64_t key = key_of(x, f.cls(j));
-        if (x > -__builtin_inff() && key < under && key > best) best = key;
-      }
-      return best;
-    });
-    if (f.first_lane())
-      write_alternative(r, g, i, t, below ? class_of(below) : -1,
-                        score_of((uint32_t)(below >> 32)));
-  }
+  else
+    take_turns<T, NW>(s, r, g, i, threadIdx.x % F::G, key_buf);
 }
 
 // ---------------------------------------------------------------------------
@@ -374,21 +413,7 @@ __global__ __launch_bounds__(1024) void alternatives_long_kernel(ScoresView s, A
     rank_candidates(list, n, threadIdx.x, 1024, r, g, i);
     return;
   }
-  uint64_t below = ~0ull;
-  for (int32_t t = 0; t < g.k; ++t) {
-    below = next_key<NW>(below, key_buf, [&](uint64_t under) {
-      uint64_t best = 0;
-      for (int32_t k = threadIdx.x; k < s.K; k += 1024) {
-        const float x = score_at<T>(s, i, k);
-        const uint64_t key = key_of(x, k);
-        if (x > -__builtin_inff() && key < under && key > best) best = key;
-      }
-      return best;
-    });
-    if (threadIdx.x == 0)
-      write_alternative(r, g, i, t, below ? class_of(below) : -1,
-                        score_of((uint32_t)(below >> 32)));
-  }
+  take_turns<T, NW>(s, r, g, i, threadIdx.x, key_buf);
 }
 
 // ---------------------------------------------------------------------------

@@ -286,6 +286,7 @@ __global__ __launch_bounds__(F::kMax) void distill_frame_kernel(ScoresView s, Di
   using T = typename F::T;
   extern __shared__ uint32_t lds[];
   __shared__ float buf[6 * F::kBuf];
+  __shared__ DistillRow share[F::kBarrier ? F::kShared : 1];
   const int k = g.k;
   const ListTable tab = list_table<F>(lds, k);
   const F f(s);
@@ -330,7 +331,7 @@ __global__ __launch_bounds__(F::kMax) void distill_frame_kernel(ScoresView s, Di
   list_maxima(f, tab, k, x);
   f.reduce_all(x, MaxF(), buf);
   const float mr = x[0], m = fmaxf(x[0], x[1]), lm = x[2], mrs = safe_max(mr);
-  if (F::kHide) f.hide(v);
+  if (F::N >= 32) f.hide(v);
   float z[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
   for (int j = 0; j < F::N; ++j) z[j % 4] += exp2_f32((F::value(v, j) - mrs) * g.scale);
@@ -338,9 +339,23 @@ __global__ __launch_bounds__(F::kMax) void distill_frame_kernel(ScoresView s, Di
   y[0] = (z[0] + z[1]) + (z[2] + z[3]);
   list_sums(f, tab, g, i, m, lm, y);
   if (F::kBarrier) __syncthreads();  // the maxima have been read
-  f.reduce_all(y, AddF(), buf);
-  const DistillRow r = distill_row(DistillSums{y[0], y[1], y[2], y[3], y[4], y[5]}, g, i, m, mr, lm, w);
-  if (F::kHide) f.hide(v);
+  f.put_all(y, AddF(), buf);
+  // what follows from the row as a whole costs as much as some 20 classes: where waves
+  // share rows, the first one works it out for all
+  const bool owner = !F::kBarrier || threadIdx.x < 64;
+  const int slot = F::kSlices ? threadIdx.x & 63 : 0;
+  if (F::kBarrier) __syncthreads();
+  DistillRow r;
+  if (owner) {
+    f.join_all(y, AddF(), buf);
+    r = distill_row(DistillSums{y[0], y[1], y[2], y[3], y[4], y[5]}, g, i, m, mr, lm, w);
+    if (F::kBarrier && (F::kSlices || threadIdx.x == 0)) share[slot] = r;
+  }
+  if (F::kBarrier) {
+    __syncthreads();
+    if (!owner) r = share[slot];
+  }
+  if (F::N >= 32) f.hide(v);
   if (in && out.data) {
     if (r.live)
       f.store(out, blockIdx.x, accumulate, [&](int j) {
@@ -349,8 +364,7 @@ __global__ __launch_bounds__(F::kMax) void distill_frame_kernel(ScoresView s, Di
     else if (!accumulate)
       f.store_zero(out, blockIdx.x);
   }
-  // (also: the others' gradients are written before the list's, the sums read)
-  __syncthreads();
+  __syncthreads();  // the others' gradients are written before the list's
   float loss[1] = {0.0f};
   for (int j = f.entry(); j < k; j += f.entry_step()) {
     const int at = f.entry_at(j, k);
@@ -366,7 +380,14 @@ __global__ __launch_bounds__(F::kMax) void distill_frame_kernel(ScoresView s, Di
       *q = from_f32<T>(d);
     }
   }
-  f.reduce_all(loss, AddF(), buf);
+  // (rows of several waves have their list in the first one)
+  if (F::kSlices) {
+    f.put_all(loss, AddF(), buf);
+    __syncthreads();
+    if (owner) f.join_all(loss, AddF(), buf);
+  } else if (owner) {
+    loss[0] = lanes_reduce<(F::kListLanes)>(loss[0], AddF());
+  }
   if (in && f.first_lane()) g.loss[i] = r.live ? r.value * (loss[0] + r.rest_term) : 0.0f;
 }
 

@@ -288,16 +288,19 @@ struct RowFrame {
     if (G <= 64) return lanes_reduce<(G < 64 ? G : 64)>(x, op);
     return waves_reduce<(G > 64 ? G / 64 : 1)>(x, op, buf);
   }
-  // NV of them at once; buf: NV * kBuf words, free again after one more barrier
+  // NV of them at once, in two steps with a barrier between where kBarrier; buf: NV *
+  // kBuf words, free again after one more barrier
   template <int NV, typename Op>
-  __device__ __forceinline__ void reduce_all(float (&x)[NV], Op op, float* buf) const {
+  __device__ __forceinline__ void put_all(float (&x)[NV], Op op, float* buf) const {
 #pragma unroll
     for (int v = 0; v < NV; ++v) x[v] = lanes_reduce<(G < 64 ? G : 64)>(x[v], op);
-    if (G <= 64) return;
-    if ((threadIdx.x & 63) == 0)
+    if (G > 64 && (threadIdx.x & 63) == 0)
 #pragma unroll
       for (int v = 0; v < NV; ++v) buf[v * kBuf + (threadIdx.x >> 6)] = x[v];
-    __syncthreads();
+  }
+  template <int NV, typename Op>
+  __device__ __forceinline__ void join_all(float (&x)[NV], Op op, const float* buf) const {
+    if (G <= 64) return;
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
       x[v] = buf[v * kBuf];
@@ -305,10 +308,16 @@ struct RowFrame {
       for (int w = 1; w < kBuf; ++w) x[v] = op(x[v], buf[v * kBuf + w]);
     }
   }
+  template <int NV, typename Op>
+  __device__ __forceinline__ void reduce_all(float (&x)[NV], Op op, float* buf) const {
+    put_all(x, op, buf);
+    if (G > 64) __syncthreads();
+    join_all(x, op, buf);
+  }
 
   // Lists of a row's classes (losses_lists.hpp): its entries j = t, t + G, ... are
   // this thread's.
-  static constexpr int kListRows = kRows;
+  static constexpr int kListRows = kRows, kListLanes = G < 64 ? G : 64;
   __device__ __forceinline__ int entry() const { return t; }
   __device__ __forceinline__ int entry_step() const { return G; }
   // place of entry j in a table of the workgroup's lists of k
@@ -513,20 +522,29 @@ struct ClassFrame {
     return x;
   }
   template <int NV, typename Op>
-  __device__ __forceinline__ void reduce_all(float (&x)[NV], Op op, float* buf) const {
+  __device__ __forceinline__ void put_all(float (&x)[NV], Op, float* buf) const {
+    if (!SLICES) return;
+#pragma unroll
+    for (int v = 0; v < NV; ++v) buf[v * kBuf + threadIdx.x] = x[v];
+  }
+  template <int NV, typename Op>
+  __device__ __forceinline__ void join_all(float (&x)[NV], Op op, const float* buf) const {
     if (!SLICES) return;
     const int lane = threadIdx.x & 63;
-#pragma unroll
-    for (int v = 0; v < NV; ++v) buf[v * kBuf + w * 64 + lane] = x[v];
-    __syncthreads();
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
       x[v] = buf[v * kBuf + lane];
       for (int u = 1; u < S; ++u) x[v] = op(x[v], buf[v * kBuf + u * 64 + lane]);
     }
   }
+  template <int NV, typename Op>
+  __device__ __forceinline__ void reduce_all(float (&x)[NV], Op op, float* buf) const {
+    put_all(x, op, buf);
+    if (SLICES) __syncthreads();
+    join_all(x, op, buf);
+  }
   // lists as in RowFrame, of slices: a row's entries are spread over the waves
-  static constexpr int kListRows = 64;
+  static constexpr int kListRows = 64, kListLanes = 64;
   __device__ __forceinline__ int entry() const { return w; }
   __device__ __forceinline__ int entry_step() const { return S; }
   __device__ __forceinline__ int entry_at(int j, int) const {
