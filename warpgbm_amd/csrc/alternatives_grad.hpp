@@ -61,14 +61,14 @@ __global__ __launch_bounds__(F::kMax) void alternatives_grad_plain_kernel(Scores
   const float own = lab >= 0 ? g.grad_label[i] : 0.0f;
   const float sa = lab >= 0 ? score_at<typename F::T>(whole, i, lab) : 0.0f;
   const AltGradRow r = alt_grad_row(g, i, own, own != 0.0f);
-  if (!r.live) {
-    if (!accumulate) f.store_zero(out, blockIdx.x);
-    return;
-  }
+  if (!r.live && accumulate) return;
   lab -= blockIdx.y * span;
+  // (one store for rows that count and rows left out: lanes of a wave may hold both)
   f.store_row(out, blockIdx.x, accumulate, lab >= 0 && lab < s.K ? lab : -1,
-              alt_grad_listed(r, g, sa, own),
-              [&](int j) { return alt_grad_at(r, g, F::value(v, j)); });
+              r.live ? alt_grad_listed(r, g, sa, own) : 0.0f, [&](int j) {
+                const float x = alt_grad_at(r, g, F::value(v, j));
+                return r.live ? x : 0.0f;
+              });
 }
 
 // a thread a row: the list's g are added up in registers
@@ -97,13 +97,11 @@ __global__ __launch_bounds__(F::kMax) void alternatives_grad_lane_kernel(ScoresV
   for (int32_t e = 0; e < g.k; ++e)
     add(g.classes[i * g.class_stride + e], g.grad_list[i * g.grad_stride + e]);
   const AltGradRow r = alt_grad_row(g, i, all, any);
-  if (!r.live) {
-    if (!accumulate) f.store_zero(out, blockIdx.x);
-    return;
-  }
+  if (!r.live && accumulate) return;
   f.store(out, blockIdx.x, accumulate, [&](int j) {
     const float x = F::value(v, j);
-    return own[j] != 0.0f ? alt_grad_listed(r, g, x, own[j]) : alt_grad_at(r, g, x);
+    const float y = own[j] != 0.0f ? alt_grad_listed(r, g, x, own[j]) : alt_grad_at(r, g, x);
+    return r.live ? y : 0.0f;
   });
 }
 
@@ -203,13 +201,11 @@ __global__ __launch_bounds__(F::kMax) void alternatives_grad_list_kernel(ScoresV
   for (int b = 0; b < F::kMaskWords; ++b) out_bits[b] = bits[b * blockDim.x + threadIdx.x];
   const AltGradRow r = alt_grad_row(g, i, sum[0] + g_label, sum[1] != 0.0f || g_label != 0.0f);
   f.take_out(v, out_bits);
-  if (in) {
-    if (r.live)
-      f.store(out, blockIdx.x, accumulate,
-              [&](int j) { return alt_grad_at(r, g, F::value(v, j)); });
-    else if (!accumulate)
-      f.store_zero(out, blockIdx.x);
-  }
+  // (one store for rows that count and rows left out: lanes of a wave may hold both)
+  if (in && (r.live || !accumulate))
+    f.store(out, blockIdx.x, accumulate, [&](int j) {
+      return r.live ? alt_grad_at(r, g, F::value(v, j)) : 0.0f;
+    });
   __syncthreads();
   if (!in || !r.live) return;
   // (the scores were read before: the gradient may be written over them)
@@ -225,6 +221,27 @@ __global__ __launch_bounds__(F::kMax) void alternatives_grad_list_kernel(ScoresV
     if (c >= 0) write(c, l_score[at], l_own[at] + (c == lab ? g_label : 0.0f));
   }
   if (mine) write(lab, sa, g_label);
+}
+
+// frames of class-major rows and of row-major ones up to 1024 chunks
+template <typename T, typename Fn>
+static void pick_short_frame(const ScoresView& s, Fn fn) {
+  constexpr int VE = Chunk<T>::VE;
+  if (s.class_major() || s.K < VE) return pick_class_frame<T>(s, fn);
+  const int64_t chunks = (s.K + VE - 1) / VE;
+  const auto go = [&](auto tag) {
+    using F = typename decltype(tag)::type;
+    fn(tag, (s.n + F::kRows - 1) / F::kRows, F::kThreads);
+  };
+  if (chunks <= 4) return go(FrameTag<RowFrame<T, 4, 1>>());
+  if (chunks <= 8) return go(FrameTag<RowFrame<T, 8, 1>>());
+  if (chunks <= 16) return go(FrameTag<RowFrame<T, 8, 2>>());
+  if (chunks <= 32) return go(FrameTag<RowFrame<T, 16, 2>>());
+  if (chunks <= 64) return go(FrameTag<RowFrame<T, 32, 2>>());
+  if (chunks <= 128) return go(FrameTag<RowFrame<T, 32, 4>>());
+  if (chunks <= 256) return go(FrameTag<RowFrame<T, 32, 8>>());
+  if (chunks <= 512) return go(FrameTag<RowFrame<T, 256, 2>>());
+  go(FrameTag<RowFrame<T, 256, 4>>());
 }
 
 template <typename T>
@@ -245,15 +262,16 @@ static int alternatives_grad_frames(const ScoresView& s, const AltGradRows& g,
                          out, accumulate, span);
     }
   };
-  if (rows_fit(s, false)) {
-    pick_frame<T, false, false>(s, [&](auto tag, int64_t blocks, int threads) {
+  // (nothing is summed over a row: long rows go in parts)
+  using Tile = RowFrame<T, 256, 4>;
+  if (s.class_major() || s.K <= Tile::N * 256) {
+    pick_short_frame<T>(s, [&](auto tag, int64_t blocks, int threads) {
       launch(tag, blocks, threads, 0, 1);
     });
   } else {
-    using Tile = RowFrame<T, 1024, 4>;
     int32_t span, tiles;
-    cut_tiles(s.K, Tile::N * 1024, &span, &tiles);
-    launch(FrameTag<Tile>(), s.n, 1024, span, tiles);
+    cut_tiles(s.K, Tile::N * 256, &span, &tiles);
+    launch(FrameTag<Tile>(), s.n, 256, span, tiles);
   }
   WGBM_LAUNCH_CHECK();
   return 0;

@@ -36,37 +36,36 @@ struct DistillSums {
 
 struct DistillRow {
   bool live;
-  float m, mr;
-  double lse, shift;  // log p = (s - m) / tau - lse, log q = l / tau - shift
-  float others;       // gradient of another class: others * e^(s - mr)
-  float rest_term;    // the others' term of the loss
-  float scale, value; // w tau, w tau^2
+  float m, lm;         // (0 where there is none)
+  float to_p, to_q;    // p = to_p e^(s - m), q = to_q e^(l - lm)
+  double apart;        // log(p / q) = (s - l) / tau - apart
+  float others;        // gradient of another class: others * e^(s - mr)
+  float rest_term;     // the others' term of the loss
+  float scale, value;  // w tau, w tau^2
 };
 
-// a bucket's term and what its gradient is made of, from its logarithms
+// a bucket's term and what its gradient is made of, x = log(p / q)
 struct Bucket {
   float term, slope;
 };
-__device__ __forceinline__ Bucket bucket(double log_p, double log_q) {
-  const float p = exp_of((float)log_p), q = exp_of((float)log_q);
-  if (q == 0.0f) return {p, p};
-  const float x = (float)(log_p - log_q);
+__device__ __forceinline__ Bucket bucket(float p, float q, float x) {
   if (fabsf(x) <= 1.0f) {
     const float f = phi_small(x);
     return {q * f, q * (x + f)};
   }
+  if (q == 0.0f) return {p, p};
   return {p - q - q * x, p - q};
 }
 
-__device__ __forceinline__ float logit_power(const DistillRows& g, float l, float lm) {
-  return exp_of((float)(((double)l - (double)lm) * g.inv_tau));
+__device__ __forceinline__ float power_of(float v, float from, const DistillRows& g) {
+  return exp2_f32((v - from) * g.scale);
 }
 
 __device__ __forceinline__ DistillRow distill_row(const DistillSums& a, const DistillRows& g,
                                                   int64_t i, float m, float mr, float lm, float w) {
   DistillRow o{};
   o.m = safe_max(m);
-  o.mr = safe_max(mr);
+  o.lm = safe_max(lm);
   o.scale = w * g.tau;
   o.value = o.scale * g.tau;
   const bool has_rest = mr > -__builtin_inff() || a.zr != a.zr;
@@ -77,16 +76,16 @@ __device__ __forceinline__ DistillRow distill_row(const DistillSums& a, const Di
   o.live = w != 0.0f && !(A + B == 0.0f);
   // (the largest term, 1, is among the listed or among the others)
   const float over = a.zl_ties > 0.0f ? a.zl + (a.zl_ties - 1.0f) + B : -1.0f;
-  o.lse = over >= 0.0f ? log_1p(over) : log_of(A + B);
+  const double lse = over >= 0.0f ? log_1p(over) : log_of(A + B);
   // shares: `one` of the largest logit, C of the other counting ones
   const bool counts = lm > -__builtin_inff() || a.q != a.q;
   const double norm = g.rest ? (double)(g.log_norm ? g.log_norm[i] : g.log_norm_all) : 0.0;
   const float more = a.q + (a.q_ties - 1.0f);  // relative to the largest
   float Q = 0.0f;
-  double log_mass = 0.0;
+  double log_mass = 0.0, shift;  // log q = l / tau - shift
   if (!g.rest) {
     o.live = o.live && counts;
-    o.shift = (double)lm * g.inv_tau + (counts ? log_1p(more) : 0.0);
+    shift = (double)o.lm * g.inv_tau + (counts ? log_1p(more) : 0.0);
   } else {
     const float top = (float)((double)lm * g.inv_tau - norm);  // its logarithm
     const float one = counts ? exp_of(top) : 0.0f, C = counts ? more * one : 0.0f;
@@ -97,13 +96,20 @@ __device__ __forceinline__ DistillRow distill_row(const DistillSums& a, const Di
     const float lost = a.out + (rest ? 0.0f : left);
     if (lost != 0.0f) log_mass = lost < 0.5f ? log1p(-(double)lost) : log((double)(one + C + Q));
     o.live = o.live && (counts || rest) && !(one + C + Q == 0.0f);
-    o.shift = norm + log_mass;
+    shift = norm + log_mass;
   }
+  o.to_p = exp_of((float)-lse);
+  o.to_q = exp_of((float)((double)o.lm * g.inv_tau - shift));
+  o.apart = (double)o.m * g.inv_tau + lse - shift;
   // the others
   if (has_rest) {
-    const double log_P = B >= A ? -(double)log1p_of(A / B) : drop + log_of(a.zr) - o.lse;
-    const Bucket b = Q > 0.0f ? bucket(log_P, log_of(Q) - log_mass)
-                              : bucket(log_P, -(double)__builtin_inff());
+    const double log_P = B >= A ? -(double)log1p_of(A / B) : drop + log_of(a.zr) - lse;
+    const float P = exp_of((float)log_P);
+    Bucket b{P, P};
+    if (Q > 0.0f) {
+      const double log_Q = log_of(Q) - log_mass;
+      b = bucket(P, exp_of((float)log_Q), (float)(log_P - log_Q));
+    }
     o.rest_term = b.term;
     o.others = o.scale * b.slope / a.zr;
   }
@@ -112,7 +118,8 @@ __device__ __forceinline__ DistillRow distill_row(const DistillSums& a, const Di
 // a listed class that counts (score above -infinity)
 __device__ __forceinline__ Bucket distill_entry(const DistillRow& r, const DistillRows& g, float s,
                                                 float l) {
-  return bucket(((double)s - (double)r.m) * g.inv_tau - r.lse, (double)l * g.inv_tau - r.shift);
+  return bucket(r.to_p * power_of(s, r.m, g), r.to_q * power_of(l, r.lm, g),
+                (float)(((double)s - (double)l) * g.inv_tau - r.apart));
 }
 // a listed class that does not count: the row may not take it
 __device__ __forceinline__ bool closed(float s) { return s == -__builtin_inff(); }
@@ -128,19 +135,16 @@ __global__ __launch_bounds__(F::kMax) void distill_lane_kernel(ScoresView s, Dis
   const int64_t i = F::row(blockIdx.x);
   if (i >= s.n) return;
   const float w = g.weight ? g.weight[i] : 1.0f;
-  if (w == 0.0f) {
-    g.loss[i] = 0.0f;
-    if (out.data && !accumulate) f.store_zero(out, blockIdx.x);
-    return;
-  }
   typename F::Regs v;
   f.load(v, s, blockIdx.x);
   f.trim(v);
+  // (left out: no class; rows that count and rows that do not go the same way)
+  if (w == 0.0f) f.drop(v);
   float l[N];
   uint32_t listed = 0;
 #pragma unroll
   for (int j = 0; j < N; ++j) l[j] = 0.0f;
-  for (int32_t e = 0; e < g.k; ++e) {
+  for (int32_t e = 0; e < (w != 0.0f ? g.k : 0); ++e) {
     const int32_t c = g.classes[i * g.class_stride + e];
     const float x = g.logits[i * g.logit_stride + e];
     if (c < 0 || c >= s.K || (listed >> c & 1)) continue;  // (the first of equal classes counts)
@@ -158,7 +162,7 @@ __global__ __launch_bounds__(F::kMax) void distill_lane_kernel(ScoresView s, Dis
     else
       mr = fmaxf(mr, x);
   }
-  const float ms = safe_max(m), mrs = safe_max(mr);
+  const float ms = safe_max(m), mrs = safe_max(mr), lms = safe_max(lm);
   DistillSums a{};
   const float norm = g.rest ? (g.log_norm ? g.log_norm[i] : g.log_norm_all) : 0.0f;
   // exponentials of the others, kept for the gradient
@@ -176,7 +180,7 @@ __global__ __launch_bounds__(F::kMax) void distill_lane_kernel(ScoresView s, Dis
       if (l[j] == lm)
         a.q_ties += 1.0f;
       else
-        a.q += logit_power(g, l[j], lm);
+        a.q += power_of(l[j], lms, g);
     } else if (g.rest) {
       a.out += exp_of((float)((double)l[j] * g.inv_tau - (double)norm));
     }
@@ -198,12 +202,8 @@ __global__ __launch_bounds__(F::kMax) void distill_lane_kernel(ScoresView s, Dis
     }
   }
   g.loss[i] = r.live ? r.value * loss : 0.0f;
-  if (!out.data) return;
-  if (!r.live) {
-    if (!accumulate) f.store_zero(out, blockIdx.x);
-    return;
-  }
-  f.store(out, blockIdx.x, accumulate, [&](int j) { return grad[j]; });
+  if (!out.data || (!r.live && accumulate)) return;
+  f.store(out, blockIdx.x, accumulate, [&](int j) { return r.live ? grad[j] : 0.0f; });
 }
 
 // ---------------------------------------------------------------------------
@@ -215,6 +215,7 @@ struct ListTable {
   float* logit;
   float* score;
   uint32_t* bits;  // of the threads' slots
+  float* buf;      // of the reductions, six values at most
 };
 template <typename F>
 __device__ __forceinline__ ListTable list_table(uint32_t* lds, int k) {
@@ -223,8 +224,11 @@ __device__ __forceinline__ ListTable list_table(uint32_t* lds, int k) {
   t.logit = (float*)(t.cls + F::kListRows * k);
   t.score = t.logit + F::kListRows * k;
   t.bits = (uint32_t*)(t.score + F::kListRows * k);
+  t.buf = (float*)(t.bits + F::kMaskWords * blockDim.x);
   return t;
 }
+
+// entries that are not used have class -1 and score -infinity
 
 // entries that name a class again no longer count
 template <typename F>
@@ -238,7 +242,10 @@ __device__ __forceinline__ void drop_repeated(const F& f, const ListTable& t, in
   __syncthreads();
   n = 0;
   for (int j = f.entry(); j < k; j += f.entry_step(), ++n)
-    if (again >> n & 1) t.cls[f.entry_at(j, k)] = -1;
+    if (again >> n & 1) {
+      t.cls[f.entry_at(j, k)] = -1;
+      t.score[f.entry_at(j, k)] = -__builtin_inff();
+    }
 }
 
 // the list's part of the maxima: x[1] of listed scores, x[2] of counting logits
@@ -247,10 +254,9 @@ __device__ __forceinline__ void list_maxima(const F& f, const ListTable& t, int 
   x[1] = x[2] = -__builtin_inff();
   for (int j = f.entry(); j < k; j += f.entry_step()) {
     const int at = f.entry_at(j, k);
-    if (t.cls[at] < 0) continue;
-    const float sc = t.score[at];
+    const float sc = t.score[at], l = t.logit[at];
     x[1] = fmaxf(x[1], sc);
-    if (!closed(sc)) x[2] = fmaxf(x[2], t.logit[at]);
+    x[2] = closed(sc) ? x[2] : fmaxf(x[2], l);
   }
 }
 // the list's part of the sums: x[1] .. x[5]
@@ -258,25 +264,21 @@ template <typename F>
 __device__ __forceinline__ void list_sums(const F& f, const ListTable& t, const DistillRows& g,
                                           int64_t i, float m, float lm, float (&x)[6]) {
   const int k = g.k;
-  const float ms = safe_max(m);
+  const float ms = safe_max(m), lms = safe_max(lm);
   const double norm = g.rest ? (double)(g.log_norm ? g.log_norm[i] : g.log_norm_all) : 0.0;
   x[1] = x[2] = x[3] = x[4] = x[5] = 0.0f;
   for (int j = f.entry(); j < k; j += f.entry_step()) {
     const int at = f.entry_at(j, k);
-    if (t.cls[at] < 0) continue;
     const float sc = t.score[at], l = t.logit[at];
     if (closed(sc)) {
-      if (g.rest) x[5] += exp_of((float)((double)l * g.inv_tau - norm));
+      if (g.rest && t.cls[at] >= 0) x[5] += exp_of((float)((double)l * g.inv_tau - norm));
       continue;
     }
-    if (sc == m)
-      x[2] += 1.0f;
-    else
-      x[1] += exp2_f32((sc - ms) * g.scale);
-    if (l == lm)
-      x[4] += 1.0f;
-    else
-      x[3] += logit_power(g, l, lm);
+    const float es = power_of(sc, ms, g), el = power_of(l, lms, g);
+    x[1] += sc == m ? 0.0f : es;
+    x[2] += sc == m ? 1.0f : 0.0f;
+    x[3] += l == lm ? 0.0f : el;
+    x[4] += l == lm ? 1.0f : 0.0f;
   }
 }
 
@@ -285,7 +287,6 @@ __global__ __launch_bounds__(F::kMax) void distill_frame_kernel(ScoresView s, Di
                                                                 ScoresView out, bool accumulate) {
   using T = typename F::T;
   extern __shared__ uint32_t lds[];
-  __shared__ float buf[6 * F::kBuf];
   __shared__ DistillRow share[F::kBarrier ? F::kShared : 1];
   const int k = g.k;
   const ListTable tab = list_table<F>(lds, k);
@@ -300,20 +301,22 @@ __global__ __launch_bounds__(F::kMax) void distill_frame_kernel(ScoresView s, Di
   for (int b = 0; b < F::kMaskWords; ++b) tab.bits[b * blockDim.x + threadIdx.x] = 0;
   __syncthreads();
   bool twice = false;
+  const int32_t* const classes = g.classes + i * g.class_stride;
+  const float* const logits = g.logits + i * g.logit_stride;
+  const T* const scores = (const T*)s.data + i * s.rs;
   for (int j = f.entry(); j < k; j += f.entry_step()) {
-    int32_t c = w != 0.0f ? g.classes[i * g.class_stride + j] : -1;
-    if (c >= s.K) c = -1;
-    float l = 0.0f, sc = 0.0f;
+    int32_t c = w != 0.0f ? classes[j] : -1;
+    float l = logits[j], sc = -__builtin_inff();
+    if (c < 0 || c >= s.K) c = -1;
     if (c >= 0) {
       int word;
       uint32_t bit;
       f.locate(c, word, bit);
       twice |= (atomicOr(&tab.bits[word], bit) & bit) != 0;
-      l = g.logits[i * g.logit_stride + j];
-      sc = score_at<T>(s, i, c);
+      sc = to_f32(scores[c * s.ks]);
     }
     const int at = f.entry_at(j, k);
-    tab.cls[at] = c < 0 ? -1 : c;
+    tab.cls[at] = c;
     tab.logit[at] = l;
     tab.score[at] = sc;
   }
@@ -329,7 +332,7 @@ __global__ __launch_bounds__(F::kMax) void distill_frame_kernel(ScoresView s, Di
 #pragma unroll
   for (int j = 0; j < F::N; ++j) x[0] = fmaxf(x[0], F::value(v, j));
   list_maxima(f, tab, k, x);
-  f.reduce_all(x, MaxF(), buf);
+  f.reduce_all(x, MaxF(), tab.buf);
   const float mr = x[0], m = fmaxf(x[0], x[1]), lm = x[2], mrs = safe_max(mr);
   if (F::N >= 32) f.hide(v);
   float z[4] = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -339,7 +342,7 @@ __global__ __launch_bounds__(F::kMax) void distill_frame_kernel(ScoresView s, Di
   y[0] = (z[0] + z[1]) + (z[2] + z[3]);
   list_sums(f, tab, g, i, m, lm, y);
   if (F::kBarrier) __syncthreads();  // the maxima have been read
-  f.put_all(y, AddF(), buf);
+  f.put_all(y, AddF(), tab.buf);
   // what follows from the row as a whole costs as much as some 20 classes: where waves
   // share rows, the first one works it out for all
   const bool owner = !F::kBarrier || threadIdx.x < 64;
@@ -347,7 +350,7 @@ __global__ __launch_bounds__(F::kMax) void distill_frame_kernel(ScoresView s, Di
   if (F::kBarrier) __syncthreads();
   DistillRow r;
   if (owner) {
-    f.join_all(y, AddF(), buf);
+    f.join_all(y, AddF(), tab.buf);
     r = distill_row(DistillSums{y[0], y[1], y[2], y[3], y[4], y[5]}, g, i, m, mr, lm, w);
     if (F::kBarrier && (F::kSlices || threadIdx.x == 0)) share[slot] = r;
   }
@@ -356,35 +359,33 @@ __global__ __launch_bounds__(F::kMax) void distill_frame_kernel(ScoresView s, Di
     if (!owner) r = share[slot];
   }
   if (F::N >= 32) f.hide(v);
-  if (in && out.data) {
-    if (r.live)
-      f.store(out, blockIdx.x, accumulate, [&](int j) {
-        return r.others * exp2_f32((F::value(v, j) - mrs) * g.scale);
-      });
-    else if (!accumulate)
-      f.store_zero(out, blockIdx.x);
-  }
+  // (one store for rows that count and rows left out: lanes of a wave may hold both)
+  if (in && out.data && (r.live || !accumulate))
+    f.store(out, blockIdx.x, accumulate, [&](int j) {
+      const float e = exp2_f32((F::value(v, j) - mrs) * g.scale);
+      return r.live ? r.others * e : 0.0f;
+    });
   __syncthreads();  // the others' gradients are written before the list's
+  T* const grads = (T*)out.data + i * out.rs;
   float loss[1] = {0.0f};
   for (int j = f.entry(); j < k; j += f.entry_step()) {
     const int at = f.entry_at(j, k);
-    const int32_t c = tab.cls[at];
     const float sc = tab.score[at];
-    if (c < 0 || closed(sc)) continue;
+    if (closed(sc)) continue;
     const Bucket b = distill_entry(r, g, sc, tab.logit[at]);
     loss[0] += b.term;
     if (in && r.live && out.data) {
       float d = r.scale * b.slope;
-      T* q = (T*)out.data + i * out.rs + c * out.ks;
+      T* q = grads + tab.cls[at] * out.ks;
       if (accumulate) d += to_f32(*q);
       *q = from_f32<T>(d);
     }
   }
   // (rows of several waves have their list in the first one)
   if (F::kSlices) {
-    f.put_all(loss, AddF(), buf);
+    f.put_all(loss, AddF(), tab.buf);
     __syncthreads();
-    if (owner) f.join_all(loss, AddF(), buf);
+    if (owner) f.join_all(loss, AddF(), tab.buf);
   } else if (owner) {
     loss[0] = lanes_reduce<(F::kListLanes)>(loss[0], AddF());
   }
@@ -415,7 +416,7 @@ __global__ __launch_bounds__(1024) void distill_long_kernel(ScoresView s, Distil
     if (c < 0 || c >= s.K) c = -1;
     tab.cls[j] = c;
     tab.logit[j] = c >= 0 ? g.logits[i * g.logit_stride + j] : 0.0f;
-    tab.score[j] = c >= 0 ? score_at<T>(s, i, c) : 0.0f;
+    tab.score[j] = c >= 0 ? score_at<T>(s, i, c) : -__builtin_inff();
   }
   __syncthreads();
   drop_repeated(whole, tab, k);
@@ -494,14 +495,13 @@ __global__ __launch_bounds__(1024) void distill_long_kernel(ScoresView s, Distil
   __syncthreads();
   float loss[1] = {0.0f};
   for (int j = threadIdx.x; j < k; j += 1024) {
-    const int32_t c = tab.cls[j];
     const float sc = tab.score[j];
-    if (c < 0 || closed(sc)) continue;
+    if (closed(sc)) continue;
     const Bucket b = distill_entry(r, g, sc, tab.logit[j]);
     loss[0] += b.term;
     if (r.live && out.data) {
       float d = r.scale * b.slope;
-      T* q = (T*)out.data + i * out.rs + c;
+      T* q = (T*)out.data + i * out.rs + tab.cls[j];
       if (accumulate) d += to_f32(*q);
       *q = from_f32<T>(d);
     }
@@ -528,7 +528,9 @@ static int distill_frames(const ScoresView& s, const DistillRows& g, const Score
       hipLaunchKernelGGL((distill_lane_kernel<F>), dim3((unsigned)blocks), dim3(threads), 0, st, s,
                          g, out, accumulate);
     } else {
-      const size_t lds = (size_t)F::kListRows * g.k * 12 + (size_t)F::kMaskWords * threads * 4;
+      const size_t words = F::kSlices ? threads : F::kBuf;  // of a reduction
+      const size_t lds = (size_t)F::kListRows * g.k * 12 + (size_t)F::kMaskWords * threads * 4 +
+                         6 * words * 4;
       hipLaunchKernelGGL((distill_frame_kernel<F>), dim3((unsigned)blocks), dim3(threads), lds, st,
                          s, g, out, accumulate);
     }

@@ -288,8 +288,8 @@ struct RowFrame {
     if (G <= 64) return lanes_reduce<(G < 64 ? G : 64)>(x, op);
     return waves_reduce<(G > 64 ? G / 64 : 1)>(x, op, buf);
   }
-  // NV of them at once, in two steps with a barrier between where kBarrier; buf: NV *
-  // kBuf words, free again after one more barrier
+  // NV of them at once, in two steps with a barrier between where kBarrier; buf: kBuf
+  // words a value (a workgroup's threads for slices), free again after one more barrier
   template <int NV, typename Op>
   __device__ __forceinline__ void put_all(float (&x)[NV], Op op, float* buf) const {
 #pragma unroll
@@ -525,16 +525,17 @@ struct ClassFrame {
   __device__ __forceinline__ void put_all(float (&x)[NV], Op, float* buf) const {
     if (!SLICES) return;
 #pragma unroll
-    for (int v = 0; v < NV; ++v) buf[v * kBuf + threadIdx.x] = x[v];
+    for (int v = 0; v < NV; ++v) buf[v * blockDim.x + threadIdx.x] = x[v];
   }
   template <int NV, typename Op>
   __device__ __forceinline__ void join_all(float (&x)[NV], Op op, const float* buf) const {
     if (!SLICES) return;
     const int lane = threadIdx.x & 63;
 #pragma unroll
-    for (int v = 0; v < NV; ++v) {
-      x[v] = buf[v * kBuf + lane];
-      for (int u = 1; u < S; ++u) x[v] = op(x[v], buf[v * kBuf + u * 64 + lane]);
+    for (int v = 0; v < NV; ++v) x[v] = buf[v * blockDim.x + lane];
+    for (int u = 1; u < S; ++u) {
+#pragma unroll
+      for (int v = 0; v < NV; ++v) x[v] = op(x[v], buf[v * blockDim.x + u * 64 + lane]);
     }
   }
   template <int NV, typename Op>
@@ -552,8 +553,10 @@ struct ClassFrame {
   }
   static constexpr int kMaskWords = 1;
   __device__ __forceinline__ void locate(int32_t k, int& word, uint32_t& bit) const {
-    word = k % S * 64 + (threadIdx.x & 63);
-    bit = 1u << (k / S);
+    // (k / S of k < 512 by a multiplication)
+    const int32_t slot = (k * ((65535 + S) / S)) >> 16;
+    word = (k - slot * S) * 64 + (threadIdx.x & 63);
+    bit = 1u << slot;
   }
   __device__ __forceinline__ void take_out(Regs& r, const uint32_t (&m)[1]) const {
 #pragma unroll
