@@ -94,7 +94,7 @@ __device__ __forceinline__ DistillRow distill_row(const DistillSums& a, const Di
     Q = rest ? left : 0.0f;
     // what is left out of sum 1
     const float lost = a.out + (rest ? 0.0f : left);
-    if (lost != 0.0f) log_mass = lost < 0.5f ? log1p(-(double)lost) : log((double)(one + C + Q));
+    log_mass = lost < 0.5f ? (double)log1p_of(-lost) : log_of(one + C + Q);
     o.live = o.live && (counts || rest) && !(one + C + Q == 0.0f);
     shift = norm + log_mass;
   }
@@ -111,7 +111,7 @@ __device__ __forceinline__ DistillRow distill_row(const DistillSums& a, const Di
       b = bucket(P, exp_of((float)log_Q), (float)(log_P - log_Q));
     }
     o.rest_term = b.term;
-    o.others = o.scale * b.slope / a.zr;
+    if (o.live) o.others = o.scale * b.slope / a.zr;
   }
   return o;
 }
@@ -125,13 +125,17 @@ __device__ __forceinline__ Bucket distill_entry(const DistillRow& r, const Disti
 __device__ __forceinline__ bool closed(float s) { return s == -__builtin_inff(); }
 
 // ---------------------------------------------------------------------------
-// a thread a row: the list as numbers beside the row's classes
+// a thread a row.  A list names classes by number, and registers have none: the
+// row's scores also lie in LDS, a column a thread, beside the listed classes' logits,
+// and their gradients go back through it.
 // ---------------------------------------------------------------------------
 template <typename F>
 __global__ __launch_bounds__(F::kMax) void distill_lane_kernel(ScoresView s, DistillRows g,
                                                                ScoresView out, bool accumulate) {
   constexpr int N = F::N;
+  __shared__ float score[N][256], logit[N][256];
   const F f(s);
+  const int t = threadIdx.x;
   const int64_t i = F::row(blockIdx.x);
   if (i >= s.n) return;
   const float w = g.weight ? g.weight[i] : 1.0f;
@@ -140,70 +144,68 @@ __global__ __launch_bounds__(F::kMax) void distill_lane_kernel(ScoresView s, Dis
   f.trim(v);
   // (left out: no class; rows that count and rows that do not go the same way)
   if (w == 0.0f) f.drop(v);
-  float l[N];
+#pragma unroll
+  for (int j = 0; j < N; ++j) score[j][t] = F::value(v, j);
   uint32_t listed = 0;
-#pragma unroll
-  for (int j = 0; j < N; ++j) l[j] = 0.0f;
-  for (int32_t e = 0; e < (w != 0.0f ? g.k : 0); ++e) {
-    const int32_t c = g.classes[i * g.class_stride + e];
-    const float x = g.logits[i * g.logit_stride + e];
-    if (c < 0 || c >= s.K || (listed >> c & 1)) continue;  // (the first of equal classes counts)
+  const int32_t* const classes = g.classes + i * g.class_stride;
+  const float* const logits = g.logits + i * g.logit_stride;
+  float m = -__builtin_inff(), lm = m;
+  const int k = w != 0.0f ? g.k : 0;
+  for (int e = 0; e < k; ++e) {
+    const int32_t c = classes[e];
+    const float l = logits[e];
+    if ((uint32_t)c >= (uint32_t)s.K || (listed >> c & 1)) continue;  // (the first one counts)
     listed |= 1u << c;
-#pragma unroll
-    for (int j = 0; j < N; ++j) l[j] = j == c ? x : l[j];
+    logit[c][t] = l;
+    const float sc = score[c][t];
+    m = fmaxf(m, sc);
+    lm = closed(sc) ? lm : fmaxf(lm, l);
   }
-  float m = -__builtin_inff(), mr = m, lm = m;
+  float mr = -__builtin_inff();
 #pragma unroll
-  for (int j = 0; j < N; ++j) {
-    const float x = F::value(v, j);
-    m = fmaxf(m, x);
-    if (listed >> j & 1)
-      lm = closed(x) ? lm : fmaxf(lm, l[j]);
-    else
-      mr = fmaxf(mr, x);
-  }
+  for (int j = 0; j < N; ++j) mr = listed >> j & 1 ? mr : fmaxf(mr, F::value(v, j));
+  m = fmaxf(m, mr);
   const float ms = safe_max(m), mrs = safe_max(mr), lms = safe_max(lm);
   DistillSums a{};
-  const float norm = g.rest ? (g.log_norm ? g.log_norm[i] : g.log_norm_all) : 0.0f;
-  // exponentials of the others, kept for the gradient
-  float e[N];
+  float e[N];  // exponentials of the others
 #pragma unroll
   for (int j = 0; j < N; ++j) {
-    const float x = F::value(v, j);
-    const bool in = listed >> j & 1;
-    e[j] = exp2_f32((x - (in ? ms : mrs)) * g.scale);
-    a.zr += in ? 0.0f : e[j];
-    a.zl += in && x != m ? e[j] : 0.0f;
-    a.zl_ties += in && x == m && !closed(x) ? 1.0f : 0.0f;
-    if (!in) continue;
-    if (!closed(x)) {
-      if (l[j] == lm)
-        a.q_ties += 1.0f;
-      else
-        a.q += power_of(l[j], lms, g);
-    } else if (g.rest) {
-      a.out += exp_of((float)((double)l[j] * g.inv_tau - (double)norm));
+    e[j] = listed >> j & 1 ? 0.0f : power_of(F::value(v, j), mrs, g);
+    a.zr += e[j];
+  }
+  const float norm = g.rest ? (g.log_norm ? g.log_norm[i] : g.log_norm_all) : 0.0f;
+  for (uint32_t b = listed; b; b &= b - 1) {
+    const int c = __ffs(b) - 1;
+    const float sc = score[c][t], l = logit[c][t];
+    if (closed(sc)) {
+      if (g.rest) a.out += exp_of((float)((double)l * g.inv_tau - (double)norm));
+      continue;
     }
+    const float es = power_of(sc, ms, g), el = power_of(l, lms, g);
+    a.zl += sc == m ? 0.0f : es;
+    a.zl_ties += sc == m ? 1.0f : 0.0f;
+    a.q += l == lm ? 0.0f : el;
+    a.q_ties += l == lm ? 1.0f : 0.0f;
   }
   const DistillRow r = distill_row(a, g, i, m, mr, lm, w);
   float loss = r.rest_term;
-  float grad[N];
-#pragma unroll
-  for (int j = 0; j < N; ++j) {
-    const float x = F::value(v, j);
-    grad[j] = r.others * e[j];
-    if (listed >> j & 1) {
-      grad[j] = 0.0f;
-      if (!closed(x)) {
-        const Bucket b = distill_entry(r, g, x, l[j]);
-        loss += b.term;
-        grad[j] = r.scale * b.slope;
-      }
+  for (uint32_t b = listed; b; b &= b - 1) {
+    const int c = __ffs(b) - 1;
+    const float sc = score[c][t];
+    float grad = 0.0f;
+    if (!closed(sc)) {
+      const Bucket u = distill_entry(r, g, sc, logit[c][t]);
+      loss += u.term;
+      grad = r.scale * u.slope;
     }
+    score[c][t] = grad;
   }
   g.loss[i] = r.live ? r.value * loss : 0.0f;
   if (!out.data || (!r.live && accumulate)) return;
-  f.store(out, blockIdx.x, accumulate, [&](int j) { return r.live ? grad[j] : 0.0f; });
+  f.store(out, blockIdx.x, accumulate, [&](int j) {
+    const float x = listed >> j & 1 ? score[j][t] : r.others * e[j];
+    return r.live ? x : 0.0f;
+  });
 }
 
 // ---------------------------------------------------------------------------
@@ -359,11 +361,12 @@ __global__ __launch_bounds__(F::kMax) void distill_frame_kernel(ScoresView s, Di
     if (!owner) r = share[slot];
   }
   if (F::N >= 32) f.hide(v);
-  // (one store for rows that count and rows left out: lanes of a wave may hold both)
+  // (one store for rows that count and rows left out, whose others' gradient is 0 times
+  // an exponential of -infinity: lanes of a wave may hold both)
+  if (!r.live) f.drop(v);
   if (in && out.data && (r.live || !accumulate))
     f.store(out, blockIdx.x, accumulate, [&](int j) {
-      const float e = exp2_f32((F::value(v, j) - mrs) * g.scale);
-      return r.live ? r.others * e : 0.0f;
+      return r.others * exp2_f32((F::value(v, j) - mrs) * g.scale);
     });
   __syncthreads();  // the others' gradients are written before the list's
   T* const grads = (T*)out.data + i * out.rs;

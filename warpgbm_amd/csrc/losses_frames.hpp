@@ -301,12 +301,10 @@ struct RowFrame {
   template <int NV, typename Op>
   __device__ __forceinline__ void join_all(float (&x)[NV], Op op, const float* buf) const {
     if (G <= 64) return;
+    // (a wave's value a lane: 16 waves' values in registers would cost the rows' room)
 #pragma unroll
-    for (int v = 0; v < NV; ++v) {
-      x[v] = buf[v * kBuf];
-#pragma unroll
-      for (int w = 1; w < kBuf; ++w) x[v] = op(x[v], buf[v * kBuf + w]);
-    }
+    for (int v = 0; v < NV; ++v)
+      x[v] = lanes_reduce<kBuf>(buf[v * kBuf + (threadIdx.x & (kBuf - 1))], op);
   }
   template <int NV, typename Op>
   __device__ __forceinline__ void reduce_all(float (&x)[NV], Op op, float* buf) const {
