@@ -105,6 +105,91 @@ __global__ __launch_bounds__(F::kMax) void alternatives_grad_lane_kernel(ScoresV
   });
 }
 
+// class-major rows in slices: the list's gradients are worked out by the threads that
+// have the entries, and written by those that have the classes (SliceMap).  A label
+// beside the list is entry k.
+template <typename F>
+static size_t grad_slices_lds(int32_t k, int threads) {
+  return ((size_t)SliceMap<F>::kWords * threads + 2 * 64 * (size_t)(k + 1) + 2 * (size_t)threads) *
+         4;
+}
+
+template <typename F>
+__global__ __launch_bounds__(F::kMax) void alternatives_grad_slices_kernel(ScoresView s,
+                                                                           AltGradRows g,
+                                                                           ScoresView out,
+                                                                           bool accumulate) {
+  using Map = SliceMap<F>;
+  extern __shared__ uint32_t lds[];
+  const int k = g.k, all = k + 1, lane = threadIdx.x & 63;
+  const Map map{lds};
+  // the entries' gradients, and their scores, later the classes' gradients
+  float* const own = (float*)(lds + Map::kWords * blockDim.x) + lane;
+  float* const score = own + 64 * all;
+  float* const buf = (float*)(lds + Map::kWords * blockDim.x) + 128 * all;
+  const F f(s);
+  const int64_t row = F::row(blockIdx.x);
+  const bool in = row < s.n;
+  const int64_t i = in ? row : s.n - 1;
+  typename F::Regs v;
+  f.load(v, s, blockIdx.x);
+  map.clear();
+  __syncthreads();
+  const int32_t* const classes = g.classes + i * g.class_stride;
+  const float* const grads = g.grad_list + i * g.grad_stride;
+  const auto class_of_entry = [&](int j) { return j < k ? classes[j] : g.label ? g.label[i] : -1; };
+  float sum[2] = {0.0f, 0.0f};  // of the g, and how many are not 0
+  bool twice = false;
+  for (int j = f.w; j < all; j += f.S) {
+    const int32_t c = class_of_entry(j);
+    float x = 0.0f;
+    if ((uint32_t)c < (uint32_t)s.K) {
+      x = j < k ? grads[j] : g.grad_label[i];
+      sum[0] += x;
+      sum[1] += x != 0.0f ? 1.0f : 0.0f;
+      twice |= map.put(f, c, j);
+    }
+    own[64 * j] = x;
+    score[64 * j] = 0.0f;
+  }
+  if (__syncthreads_or(twice)) {
+    // the first of the entries that name a class takes its place, and all their g
+    for (int j = f.w; j < all; j += f.S) {
+      const int32_t c = class_of_entry(j);
+      bool first = (uint32_t)c < (uint32_t)s.K;
+      for (int o = 0; o < j; ++o) first &= classes[o] != c;
+      if (!first) continue;
+      map.set(f, c, j);
+      // (later entries' own numbers: only first entries' are changed)
+      float more = 0.0f;
+      for (int o = j + 1; o < all; ++o)
+        if (class_of_entry(o) == c) more += own[64 * o];
+      own[64 * j] += more;
+    }
+    __syncthreads();
+  }
+  uint32_t mine[Map::kWords];
+  map.mine(mine);
+#pragma unroll
+  for (int j = 0; j < F::N; ++j) {
+    const int e = Map::entry(mine, j);
+    if (e) score[64 * (e - 1)] = F::value(v, j);
+  }
+  f.reduce_all(sum, AddF(), buf);
+  const AltGradRow r = alt_grad_row(g, i, sum[0], sum[1] != 0.0f);
+  for (int j = f.w; j < all; j += f.S)
+    score[64 * j] = alt_grad_listed(r, g, score[64 * j], own[64 * j]);
+  __syncthreads();
+  // (one store for rows that count and rows left out: lanes of a wave may hold both)
+  if (!in || (!r.live && accumulate)) return;
+  f.store(out, blockIdx.x, accumulate, [&](int j) {
+    const int e = Map::entry(mine, j);
+    float y = alt_grad_at(r, g, F::value(v, j));
+    if (e) y = score[64 * (e - 1)];
+    return r.live ? y : 0.0f;
+  });
+}
+
 // Rows that threads share.  The listed classes are taken out of the rows (a bit a
 // slot, set through LDS, found again by the thread that has the class), which
 // leaves their places 0 or as they were, and their gradients are written to
@@ -256,6 +341,9 @@ static int alternatives_grad_frames(const ScoresView& s, const AltGradRows& g,
     } else if constexpr (F::kLaneRows && !F::kSlices) {
       hipLaunchKernelGGL((alternatives_grad_lane_kernel<F>), grid, dim3(threads), 0, st, s, g, out,
                          accumulate);
+    } else if constexpr (F::kSlices) {
+      hipLaunchKernelGGL((alternatives_grad_slices_kernel<F>), grid, dim3(threads),
+                         grad_slices_lds<F>(g.k, threads), st, s, g, out, accumulate);
     } else {
       const size_t lds = (size_t)F::kListRows * g.k * 12 + (size_t)F::kMaskWords * threads * 4;
       hipLaunchKernelGGL((alternatives_grad_list_kernel<F>), grid, dim3(threads), lds, st, s, g,

@@ -208,6 +208,142 @@ __global__ __launch_bounds__(F::kMax) void distill_lane_kernel(ScoresView s, Dis
   });
 }
 
+// a listed class's part of the sums x[1] .. x[5]
+__device__ __forceinline__ void add_entry(const DistillRows& g, double norm, bool used, float sc,
+                                          float l, float m, float ms, float lm, float lms,
+                                          float (&x)[6]) {
+  if (closed(sc)) {
+    if (g.rest && used) x[5] += exp_of((float)((double)l * g.inv_tau - norm));
+    return;
+  }
+  const float es = power_of(sc, ms, g), el = power_of(l, lms, g);
+  x[1] += sc == m ? 0.0f : es;
+  x[2] += sc == m ? 1.0f : 0.0f;
+  x[3] += l == lm ? 0.0f : el;
+  x[4] += l == lm ? 1.0f : 0.0f;
+}
+__device__ __forceinline__ double row_norm(const DistillRows& g, int64_t i) {
+  return g.rest ? (double)(g.log_norm ? g.log_norm[i] : g.log_norm_all) : 0.0;
+}
+
+// ---------------------------------------------------------------------------
+// class-major rows in slices (SliceMap)
+// ---------------------------------------------------------------------------
+template <typename F>
+static size_t distill_slices_lds(int32_t k, int threads) {
+  return ((size_t)SliceMap<F>::kWords * threads + 2 * 64 * (size_t)k + 10 * (size_t)threads) * 4;
+}
+
+template <typename F>
+__global__ __launch_bounds__(F::kMax) void distill_slices_kernel(ScoresView s, DistillRows g,
+                                                                 ScoresView out, bool accumulate) {
+  using Map = SliceMap<F>;
+  extern __shared__ uint32_t lds[];
+  __shared__ DistillRow share[64];
+  const int k = g.k, lane = threadIdx.x & 63;
+  const Map map{lds};
+  // logits of the lists, and their scores, later gradients
+  float* const logit = (float*)(lds + Map::kWords * blockDim.x) + lane;
+  float* const score = logit + 64 * k;
+  float* const buf = (float*)(lds + Map::kWords * blockDim.x) + 128 * k;
+  const F f(s);
+  const int64_t row = F::row(blockIdx.x);
+  const bool in = row < s.n;
+  const int64_t i = in ? row : s.n - 1;
+  typename F::Regs v;
+  f.load(v, s, blockIdx.x);
+  const float w = !in ? 0.0f : g.weight ? g.weight[i] : 1.0f;
+  map.clear();
+  __syncthreads();
+  const int32_t* const classes = g.classes + i * g.class_stride;
+  const float* const logits = g.logits + i * g.logit_stride;
+  uint32_t used = 0;  // a bit for each of this thread's entries j = f.w, f.w + f.S, ...
+  bool twice = false;
+  for (int j = f.w, n = 0; j < k; j += f.S, ++n) {
+    const int32_t c = classes[j];
+    logit[64 * j] = logits[j];
+    score[64 * j] = -__builtin_inff();
+    if (w != 0.0f && (uint32_t)c < (uint32_t)s.K) {
+      used |= 1u << n;
+      twice |= map.put(f, c, j);
+    }
+  }
+  if (__syncthreads_or(twice)) {
+    // the first of the entries that name a class takes its place
+    for (int j = f.w, n = 0; j < k; j += f.S, ++n) {
+      const int32_t c = classes[j];
+      for (int o = 0; o < j; ++o)
+        if (classes[o] == c) used &= ~(1u << n);
+      if (used >> n & 1) map.set(f, c, j);
+    }
+    __syncthreads();
+  }
+  uint32_t mine[Map::kWords];
+  map.mine(mine);
+  f.trim(v);
+  if (w == 0.0f) f.drop(v);
+  float x[3];
+  x[0] = -__builtin_inff();
+#pragma unroll
+  for (int j = 0; j < F::N; ++j) {
+    const int e = Map::entry(mine, j);
+    if (e) score[64 * (e - 1)] = F::value(v, j);
+    f.take_out(v, j, e != 0);
+    x[0] = fmaxf(x[0], F::value(v, j));
+  }
+  __syncthreads();
+  x[1] = x[2] = -__builtin_inff();
+  for (int j = f.w; j < k; j += f.S) {
+    const float sc = score[64 * j], l = logit[64 * j];
+    x[1] = fmaxf(x[1], sc);
+    x[2] = closed(sc) ? x[2] : fmaxf(x[2], l);
+  }
+  f.reduce_all(x, MaxF(), buf);
+  const float mr = x[0], m = fmaxf(x[0], x[1]), lm = x[2];
+  const float ms = safe_max(m), mrs = safe_max(mr), lms = safe_max(lm);
+  float z[2] = {0.0f, 0.0f};
+#pragma unroll
+  for (int j = 0; j < F::N; ++j) z[j % 2] += power_of(F::value(v, j), mrs, g);
+  float y[6] = {z[0] + z[1], 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+  const double norm = row_norm(g, i);
+  for (int j = f.w, n = 0; j < k; j += f.S, ++n)
+    add_entry(g, norm, used >> n & 1, score[64 * j], logit[64 * j], m, ms, lm, lms, y);
+  f.put_all(y, AddF(), buf + 3 * blockDim.x);
+  __syncthreads();
+  // what follows from the row as a whole costs as much as some 20 classes: the first wave
+  // works it out for all
+  DistillRow r;
+  if (f.w == 0) {
+    f.join_all(y, AddF(), buf + 3 * blockDim.x);
+    r = distill_row(DistillSums{y[0], y[1], y[2], y[3], y[4], y[5]}, g, i, m, mr, lm, w);
+    share[lane] = r;
+  }
+  __syncthreads();
+  if (f.w != 0) r = share[lane];
+  float loss[1] = {0.0f};
+  for (int j = f.w; j < k; j += f.S) {
+    const float sc = score[64 * j];
+    Bucket b{0.0f, 0.0f};
+    if (!closed(sc)) b = distill_entry(r, g, sc, logit[64 * j]);
+    loss[0] += b.term;
+    score[64 * j] = r.scale * b.slope;
+  }
+  f.put_all(loss, AddF(), buf + 9 * blockDim.x);
+  __syncthreads();
+  if (f.w == 0) {
+    f.join_all(loss, AddF(), buf + 9 * blockDim.x);
+    if (in) g.loss[i] = r.live ? r.value * (loss[0] + r.rest_term) : 0.0f;
+  }
+  // (one store for rows that count and rows left out: lanes of a wave may hold both)
+  if (!in || !out.data || (!r.live && accumulate)) return;
+  f.store(out, blockIdx.x, accumulate, [&](int j) {
+    const int e = Map::entry(mine, j);
+    float y = r.others * power_of(F::value(v, j), mrs, g);
+    if (e) y = score[64 * (e - 1)];
+    return r.live ? y : 0.0f;
+  });
+}
+
 // ---------------------------------------------------------------------------
 // rows that threads share
 // ---------------------------------------------------------------------------
@@ -267,20 +403,11 @@ __device__ __forceinline__ void list_sums(const F& f, const ListTable& t, const 
                                           int64_t i, float m, float lm, float (&x)[6]) {
   const int k = g.k;
   const float ms = safe_max(m), lms = safe_max(lm);
-  const double norm = g.rest ? (double)(g.log_norm ? g.log_norm[i] : g.log_norm_all) : 0.0;
+  const double norm = row_norm(g, i);
   x[1] = x[2] = x[3] = x[4] = x[5] = 0.0f;
   for (int j = f.entry(); j < k; j += f.entry_step()) {
     const int at = f.entry_at(j, k);
-    const float sc = t.score[at], l = t.logit[at];
-    if (closed(sc)) {
-      if (g.rest && t.cls[at] >= 0) x[5] += exp_of((float)((double)l * g.inv_tau - norm));
-      continue;
-    }
-    const float es = power_of(sc, ms, g), el = power_of(l, lms, g);
-    x[1] += sc == m ? 0.0f : es;
-    x[2] += sc == m ? 1.0f : 0.0f;
-    x[3] += l == lm ? 0.0f : el;
-    x[4] += l == lm ? 1.0f : 0.0f;
+    add_entry(g, norm, t.cls[at] >= 0, t.score[at], t.logit[at], m, ms, lm, lms, x);
   }
 }
 
@@ -289,7 +416,7 @@ __global__ __launch_bounds__(F::kMax) void distill_frame_kernel(ScoresView s, Di
                                                                 ScoresView out, bool accumulate) {
   using T = typename F::T;
   extern __shared__ uint32_t lds[];
-  __shared__ DistillRow share[F::kBarrier ? F::kShared : 1];
+  __shared__ DistillRow share;
   const int k = g.k;
   const ListTable tab = list_table<F>(lds, k);
   const F f(s);
@@ -348,21 +475,20 @@ __global__ __launch_bounds__(F::kMax) void distill_frame_kernel(ScoresView s, Di
   // what follows from the row as a whole costs as much as some 20 classes: where waves
   // share rows, the first one works it out for all
   const bool owner = !F::kBarrier || threadIdx.x < 64;
-  const int slot = F::kSlices ? threadIdx.x & 63 : 0;
   if (F::kBarrier) __syncthreads();
   DistillRow r;
   if (owner) {
     f.join_all(y, AddF(), tab.buf);
     r = distill_row(DistillSums{y[0], y[1], y[2], y[3], y[4], y[5]}, g, i, m, mr, lm, w);
-    if (F::kBarrier && (F::kSlices || threadIdx.x == 0)) share[slot] = r;
+    if (F::kBarrier && threadIdx.x == 0) share = r;
   }
   if (F::kBarrier) {
     __syncthreads();
-    if (!owner) r = share[slot];
+    if (!owner) r = share;
   }
   if (F::N >= 32) f.hide(v);
   // (one store for rows that count and rows left out, whose others' gradient is 0 times
-  // an exponential of -infinity: lanes of a wave may hold both)
+  // an exponential of -infinity: a wave may hold both)
   if (!r.live) f.drop(v);
   if (in && out.data && (r.live || !accumulate))
     f.store(out, blockIdx.x, accumulate, [&](int j) {
@@ -385,13 +511,7 @@ __global__ __launch_bounds__(F::kMax) void distill_frame_kernel(ScoresView s, Di
     }
   }
   // (rows of several waves have their list in the first one)
-  if (F::kSlices) {
-    f.put_all(loss, AddF(), tab.buf);
-    __syncthreads();
-    if (owner) f.join_all(loss, AddF(), tab.buf);
-  } else if (owner) {
-    loss[0] = lanes_reduce<(F::kListLanes)>(loss[0], AddF());
-  }
+  if (owner) loss[0] = lanes_reduce<(F::kListLanes)>(loss[0], AddF());
   if (in && f.first_lane()) g.loss[i] = r.live ? r.value * (loss[0] + r.rest_term) : 0.0f;
 }
 
@@ -530,10 +650,12 @@ static int distill_frames(const ScoresView& s, const DistillRows& g, const Score
     if constexpr (F::kLaneRows && !F::kSlices) {
       hipLaunchKernelGGL((distill_lane_kernel<F>), dim3((unsigned)blocks), dim3(threads), 0, st, s,
                          g, out, accumulate);
+    } else if constexpr (F::kSlices) {
+      hipLaunchKernelGGL((distill_slices_kernel<F>), dim3((unsigned)blocks), dim3(threads),
+                         distill_slices_lds<F>(g.k, threads), st, s, g, out, accumulate);
     } else {
-      const size_t words = F::kSlices ? threads : F::kBuf;  // of a reduction
       const size_t lds = (size_t)F::kListRows * g.k * 12 + (size_t)F::kMaskWords * threads * 4 +
-                         6 * words * 4;
+                         6 * F::kBuf * 4;
       hipLaunchKernelGGL((distill_frame_kernel<F>), dim3((unsigned)blocks), dim3(threads), lds, st,
                          s, g, out, accumulate);
     }

@@ -543,22 +543,20 @@ struct ClassFrame {
     join_all(x, op, buf);
   }
   // lists as in RowFrame, of slices: a row's entries are spread over the waves
-  static constexpr int kListRows = 64, kListLanes = 64;
+  static constexpr int kListRows = 64;
   __device__ __forceinline__ int entry() const { return w; }
   __device__ __forceinline__ int entry_step() const { return S; }
   __device__ __forceinline__ int entry_at(int j, int) const {
     return j * 64 + (threadIdx.x & 63);
   }
-  static constexpr int kMaskWords = 1;
-  __device__ __forceinline__ void locate(int32_t k, int& word, uint32_t& bit) const {
-    // (k / S of k < 512 by a multiplication)
-    const int32_t slot = (k * ((65535 + S) / S)) >> 16;
-    word = (k - slot * S) * 64 + (threadIdx.x & 63);
-    bit = 1u << slot;
+  // the wave and slot of class k (k / S of k < 512 by a multiplication)
+  __device__ __forceinline__ void locate(int32_t k, int& wave, int& slot) const {
+    slot = (k * ((65535 + S) / S)) >> 16;
+    wave = k - slot * S;
   }
-  __device__ __forceinline__ void take_out(Regs& r, const uint32_t (&m)[1]) const {
-#pragma unroll
-    for (int j = 0; j < N; ++j) r.c[j] = m[0] >> j & 1 ? (T)(-__builtin_inff()) : r.c[j];
+  // slot j is no longer one of this row's classes
+  __device__ __forceinline__ void take_out(Regs& r, int j, bool out) const {
+    r.c[j] = out ? (T)(-__builtin_inff()) : r.c[j];
   }
   // sum[k] = the workgroup's sum of acc over its rows, for every class
   __device__ __forceinline__ void sum_rows(float (&acc)[N], float* sum) const {
