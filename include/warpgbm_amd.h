@@ -318,8 +318,9 @@ int wgbm_balance_loss(const wgbm_scores* scores, const uint8_t* mask, int32_t to
                       float* loss, int64_t* counts, float* prob, const wgbm_scores* grad,
                       int32_t accumulate, void* workspace, int64_t workspace_bytes, void* stream);
 
-/* Lists of a row's classes: at most WGBM_MAX_LIST of them.  Temperatures are in [1e-6,
- * 1e6] and divide the scores. */
+/* Lists of a row's classes: at most WGBM_MAX_LIST of them.  Entry j of row i of an
+ * argument is at i * stride + j * step; either step is 1 (stride >= list_length) or
+ * stride is 1 (step >= n_rows).  Temperatures are in [1e-6, 1e6] and divide the scores. */
 #define WGBM_MAX_LIST 64
 
 /* With p = softmax(scores[i] / temperature): the top_k classes of largest score, in
@@ -349,10 +350,12 @@ typedef struct wgbm_alternatives_grad_args {
   const float* norm;                  /* [n_rows][3] */
   const int32_t* labels;              /* [n_rows] or NULL */
   const float* grad_label_log_prob;   /* [n_rows], with labels */
-  const int32_t* classes;             /* [n_rows][list_length], rows classes_stride apart */
+  const int32_t* classes;             /* [n_rows][list_length] */
   int64_t classes_stride;
-  const float* grad_log_prob;         /* the same, rows grad_stride apart */
+  int64_t classes_step;
+  const float* grad_log_prob;         /* [n_rows][list_length] */
   int64_t grad_stride;
+  int64_t grad_step;
   int32_t list_length;                /* [0, WGBM_MAX_LIST] */
   const float* grad_entropy;          /* [n_rows] or NULL */
   float temperature;
@@ -378,10 +381,12 @@ int wgbm_class_alternatives_grad(const wgbm_scores* scores,
  * list nothing counts is left out: loss and gradient 0.  grad as for the policy loss
  * (NULL: none). */
 typedef struct wgbm_distill_args {
-  const int32_t* classes;  /* [n_rows][list_length], rows classes_stride apart */
+  const int32_t* classes;  /* [n_rows][list_length] */
   int64_t classes_stride;
-  const float* logits;     /* the same, rows logits_stride apart */
+  int64_t classes_step;
+  const float* logits;     /* [n_rows][list_length] */
   int64_t logits_stride;
+  int64_t logits_step;
   int32_t list_length;     /* [1, WGBM_MAX_LIST] */
   int32_t rest;
   const float* log_norm;   /* [n_rows] or NULL */

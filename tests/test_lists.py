@@ -588,7 +588,8 @@ def test_distill_far_scores_and_lowest_masks(gpu, order, dtype):
 @pytest.mark.gpu
 @pytest.mark.parametrize("order", ["row", "class"])
 def test_lists_with_strides(gpu, order):
-    """The first entries of longer lists, and lists inside of other tensors."""
+    """The first entries of longer lists, lists inside of other tensors, and lists whose
+    rows are next to each other."""
     from warpgbm_amd import losses
 
     for n, K in ((37, 12), (37, 90), (20, 700)):
@@ -604,12 +605,19 @@ def test_lists_with_strides(gpu, order):
         b = losses.distill_loss(sd, cls[:, :4].contiguous().cuda(), logits[:, :4].contiguous().cuda(),
                                 log_norm=ln.cuda())
         assert torch.equal(a.loss, b.loss) and torch.equal(a.grad, b.grad)
+        b = losses.distill_loss(sd, cls.cuda().t().contiguous().t()[:, :4],
+                                far.cuda().t().contiguous().t()[:, 3:7], log_norm=ln.cuda())
+        assert torch.equal(a.loss, b.loss) and torch.equal(a.grad, b.grad)
         f = losses.class_alternatives(sd, 0)
         up = torch.randn((n, 30), generator=torch.Generator().manual_seed(1)).cuda()
         x = losses.class_alternatives_grad(sd, f.norm, classes=big.cuda()[:, 5:9],
                                            grad_log_prob=up[:, 7:11])
         y = losses.class_alternatives_grad(sd, f.norm, classes=cls[:, :4].contiguous().cuda(),
                                            grad_log_prob=up[:, 7:11].contiguous())
+        assert torch.equal(x, y)
+        y = losses.class_alternatives_grad(
+            sd, f.norm, classes=cls.cuda().t().contiguous().t()[:, :4],
+            grad_log_prob=up.t().contiguous().t()[:, 7:11])
         assert torch.equal(x, y)
 
 
@@ -748,13 +756,15 @@ def test_refusals_without_a_gpu():
         losses._list(c.long(), "classes", torch.int32, 4, 2, cpu)
     with pytest.raises(RuntimeError, match="shape"):
         losses._list(c, "classes", torch.int32, 4, 3, cpu)
-    with pytest.raises(RuntimeError, match="next to each other"):
-        losses._list(c.t().contiguous().t(), "classes", torch.int32, 4, 2, cpu)
-    with pytest.raises(RuntimeError, match="next to each other"):
-        losses._list(c[:1].expand(4, 2), "classes", torch.int32, 4, 2, cpu)
-    assert losses._list(c[:1], "classes", torch.int32, 1, 2, cpu)[1] == 2
-    assert losses._list(torch.zeros((4, 9), dtype=torch.int32)[:, :1], "c", torch.int32, 4, 1,
-                        cpu)[1] == 9
+    wide = torch.zeros((8, 18), dtype=torch.int32)
+    for bad in (wide[::2, ::9], c[:1].expand(4, 2), c[:, :1].expand(4, 2)):
+        with pytest.raises(RuntimeError, match="next to each other"):
+            losses._list(bad, "classes", torch.int32, 4, 2, cpu)
+    assert losses._list(c.t().contiguous().t(), "classes", torch.int32, 4, 2, cpu)[1:] == (1, 4)
+    assert losses._list(c[:1], "classes", torch.int32, 1, 2, cpu)[1:] == (2, 1)
+    assert losses._list(wide[:4, :1], "c", torch.int32, 4, 1, cpu)[1:] == (18, 1)
+    assert losses._list(wide[:4, 3:5], "c", torch.int32, 4, 2, cpu)[1:] == (18, 1)
+    assert losses._list(wide.t()[:4, :2], "c", torch.int32, 4, 2, cpu)[1:] == (1, 18)
     for t in (0.0, -1.0, INF, float("nan")):
         with pytest.raises(RuntimeError, match="temperature"):
             losses._temperature(t)
@@ -799,7 +809,7 @@ def test_c_entries_refuse_before_any_launch():
 
     def grad(out=None, **kw):
         f = dict(norm=one, labels=None, grad_label_log_prob=None, classes=one, classes_stride=2,
-                 grad_log_prob=one, grad_stride=2, list_length=2, grad_entropy=None,
+                 classes_step=1, grad_log_prob=one, grad_stride=2, grad_step=1, list_length=2, grad_entropy=None,
                  temperature=1.0)
         f.update(kw)
         args = _lib.AlternativesGradArgs(*f.values())
@@ -817,7 +827,8 @@ def test_c_entries_refuse_before_any_launch():
     refused(grad(out=scores(row_stride=1, class_stride=8)), "order")
 
     def distill(out=None, **kw):
-        f = dict(classes=one, classes_stride=2, logits=one, logits_stride=2, list_length=2, rest=0,
+        f = dict(classes=one, classes_stride=2, classes_step=1, logits=one, logits_stride=2,
+                 logits_step=1, list_length=2, rest=0,
                  log_norm=None, log_norm_all=0.0, weight=None, temperature=1.0)
         f.update(kw)
         args = _lib.DistillArgs(*f.values())
@@ -827,6 +838,8 @@ def test_c_entries_refuse_before_any_launch():
     refused(distill(list_length=0), "length")
     refused(distill(list_length=65), "length")
     refused(distill(classes_stride=1), "stride")
+    refused(distill(classes_stride=1, classes_step=3), "stride")
+    refused(distill(classes_stride=4, classes_step=2), "stride")
     refused(distill(logits_stride=1 << 41), "stride")
     refused(distill(temperature=0.0), "temperature")
     refused(distill(rest=1, log_norm_all=INF), "log_norm")

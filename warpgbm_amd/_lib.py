@@ -138,8 +138,10 @@ class AlternativesGradArgs(C.Structure):
         ("grad_label_log_prob", _p),
         ("classes", _p),
         ("classes_stride", _i64),
+        ("classes_step", _i64),
         ("grad_log_prob", _p),
         ("grad_stride", _i64),
+        ("grad_step", _i64),
         ("list_length", _i32),
         ("grad_entropy", _p),
         ("temperature", _f32),
@@ -150,8 +152,10 @@ class DistillArgs(C.Structure):
     _fields_ = [
         ("classes", _p),
         ("classes_stride", _i64),
+        ("classes_step", _i64),
         ("logits", _p),
         ("logits_stride", _i64),
+        ("logits_step", _i64),
         ("list_length", _i32),
         ("rest", _i32),
         ("log_norm", _p),

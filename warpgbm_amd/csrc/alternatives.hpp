@@ -59,13 +59,48 @@ __device__ __forceinline__ void write_alternative(const AltRow& r, const AltRows
 
 // ---------------------------------------------------------------------------
 // Few classes a row, or few alternatives: the best classes one after the other.
-// A thread's classes ascend with its slots, so it looks for its lowest slot
-// (as in the balance loss); each turn costs some eight instructions a slot and
-// two reductions.
+// Each thread knows the best of its classes that are not taken; the best of those is
+// the row's, and the thread that had it looks through its classes again (five
+// instructions a slot).  Classes ascend with slots, so the first of equal scores is
+// the lowest class.
 // ---------------------------------------------------------------------------
 template <typename F>
+struct Turns {
+  static constexpr int kWords = (F::N + 31) / 32;
+  uint32_t taken[kWords];  // a bit a slot
+  float best;
+  int slot;  // -1: none is left
+  __device__ __forceinline__ void look(const typename F::Regs& v) {
+    best = -__builtin_inff();
+    slot = -1;
+#pragma unroll
+    for (int j = 0; j < F::N; ++j) {
+      // (a taken class's score reads as NaN, which is larger than nothing)
+      const int32_t gone = __builtin_amdgcn_sbfe((int32_t)taken[j / 32], j % 32, 1);
+      const float x = __builtin_bit_cast(
+          float, __builtin_bit_cast(int32_t, F::value(v, j)) | gone);
+      const bool more = x > best;
+      best = more ? x : best;
+      slot = more ? j : slot;
+    }
+  }
+  __device__ __forceinline__ void take(const typename F::Regs& v) {
+#pragma unroll
+    for (int q = 0; q < kWords; ++q) taken[q] |= slot / 32 == q ? 1u << (slot % 32) : 0u;
+    look(v);
+  }
+};
+
+// words of LDS: two turns' best scores and classes, three sums, of slices
+template <typename F>
+static size_t turns_lds(int threads) {
+  return F::kSlices ? 7 * 4 * (size_t)threads : 0;
+}
+
+template <typename F>
 __global__ __launch_bounds__(F::kMax) void alternatives_turns_kernel(ScoresView s, AltRows g) {
-  __shared__ float buf[4][F::kBuf];
+  extern __shared__ uint32_t lds[];
+  float* const words = (float*)lds;
   const F f(s);
   const int64_t row = F::row(blockIdx.x);
   const bool in = row < s.n;
@@ -76,49 +111,48 @@ __global__ __launch_bounds__(F::kMax) void alternatives_turns_kernel(ScoresView 
   const int32_t lab = row_label(g.label, i, s.K);
   const float sa = lab >= 0 ? score_at<typename F::T>(s, i, lab) : 0.0f;
   f.trim(v);
-  float m = -__builtin_inff();
-#pragma unroll
-  for (int j = 0; j < F::N; ++j) m = fmaxf(m, F::value(v, j));
-  m = f.reduce(m, MaxF(), buf[0]);
-  const float ms = safe_max(m);
+  Turns<F> turn{};
+  turn.look(v);
+  float* const sums = words + 4 * blockDim.x;
+  const float m = f.reduce(turn.best, MaxF(), words), ms = safe_max(m);
   AltSums a{0.0f, 0.0f, 0.0f};
 #pragma unroll
   for (int j = 0; j < F::N; ++j) add_score(a, F::value(v, j), m, ms, g.scale);
-  a.z = f.reduce(a.z, AddF(), buf[1]);
-  a.u = f.reduce(a.u, AddF(), buf[2]);
-  a.ties = f.reduce(a.ties, AddF(), buf[3]);
-  const AltRow r = alt_row(a, m);
+  float sum[3] = {a.z, a.u, a.ties};
+  f.template reduce_all<3>(sum, AddF(), sums);
+  const AltRow r = alt_row(AltSums{sum[0], sum[1], sum[2]}, m);
   const bool write = in && f.first_lane();
   if (write) write_alt_row(r, g, i, lab, sa);
-  constexpr float kNone = 1e9f;  // (class numbers are exact in float32)
-  float v0 = __builtin_inff();
-  int32_t c0 = -1;
+  constexpr int32_t kNone = 0x7fffffff;
   for (int32_t t = 0; t < g.k; ++t) {
-    float best = m;
-    int slot = F::N;
-    if (t == 0) {
-#pragma unroll
-      for (int j = F::N - 1; j >= 0; --j) slot = F::value(v, j) == best ? j : slot;
-    } else {
-      const int taken = f.last_slot(c0);  // of the scores equal to v0
-      best = -__builtin_inff();
-#pragma unroll
-      for (int j = 0; j < F::N; ++j) {
-        const float x = F::value(v, j);
-        if (x < v0 || (x == v0 && j > taken)) best = fmaxf(best, x);
+    // the row's best, and the lowest class that has it
+    float best = turn.best;
+    const int32_t mine = turn.slot >= 0 ? f.cls(turn.slot) : kNone;
+    int32_t c = mine;
+    if constexpr (F::kSlices) {
+      // (two turns' words: a wave may be one turn ahead of the others)
+      float* const bv = words + t % 2 * 2 * blockDim.x;
+      int32_t* const bc = (int32_t*)(bv + blockDim.x);
+      const int lane = threadIdx.x & 63;
+      bv[threadIdx.x] = best;
+      bc[threadIdx.x] = c;
+      __syncthreads();
+      for (int u = 0; u < f.S; ++u) {
+        const float x = bv[u * 64 + lane];
+        const int32_t k = bc[u * 64 + lane];
+        const bool more = x > best || (x == best && k < c);
+        best = more ? x : best;
+        c = more ? k : c;
       }
-      best = f.reduce(best, MaxF(), buf[1]);
-      const int from = best < v0 ? -1 : taken;
-#pragma unroll
-      for (int j = F::N - 1; j >= 0; --j) slot = F::value(v, j) == best && j > from ? j : slot;
+    } else if constexpr (!F::kLaneRows) {
+      best = lanes_reduce<F::G>(best, MaxF());
+      // (class numbers are exact in float32)
+      c = (int32_t)lanes_reduce<F::G>(turn.slot >= 0 && turn.best == best ? (float)mine : 1e9f,
+                                      [](float x, float y) { return fminf(x, y); });
+      if (c >= s.K) c = kNone;
     }
-    const float c = f.reduce(slot < F::N ? (float)f.cls(slot) : kNone, [](float x, float y) {
-      return fminf(x, y);
-    }, buf[0]);
-    const bool found = best > -__builtin_inff() && c < kNone;
-    if (write) write_alternative(r, g, i, t, found ? (int32_t)c : -1, best);
-    v0 = best;
-    c0 = found ? (int32_t)c : s.K - 1;
+    if (write) write_alternative(r, g, i, t, c != kNone ? c : -1, best);
+    if (c == mine && c != kNone) turn.take(v);
   }
 }
 
@@ -424,8 +458,8 @@ static int alternatives_frames(const ScoresView& s, const AltRows& g, hipStream_
   constexpr int VE = Chunk<T>::VE;
   const auto turns = [&](auto tag, int64_t blocks, int threads) {
     using F = typename decltype(tag)::type;
-    hipLaunchKernelGGL((alternatives_turns_kernel<F>), dim3((unsigned)blocks), dim3(threads), 0,
-                       st, s, g);
+    hipLaunchKernelGGL((alternatives_turns_kernel<F>), dim3((unsigned)blocks), dim3(threads),
+                       turns_lds<F>(threads), st, s, g);
   };
   const auto candidates = [&](auto tag) {
     using F = typename decltype(tag)::type;
@@ -433,21 +467,13 @@ static int alternatives_frames(const ScoresView& s, const AltRows& g, hipStream_
                        dim3((unsigned)((s.n + F::kRows - 1) / F::kRows)), dim3(F::kThreads), 0, st,
                        s, g);
   };
-  const auto row_turns = [&](auto tag) {
-    using F = typename decltype(tag)::type;
-    turns(tag, (s.n + F::kRows - 1) / F::kRows, F::kThreads);
-  };
   const int64_t chunks = (s.K + VE - 1) / VE;
-  if (s.class_major() || s.K < VE) {
-    pick_class_frame<T>(s, turns);
-  } else if (chunks <= 4) {
-    row_turns(FrameTag<RowFrame<T, 4, 1>>());
-  } else if (chunks <= 8) {
-    row_turns(FrameTag<RowFrame<T, 8, 1>>());
-  } else if (chunks <= 16) {
-    row_turns(FrameTag<RowFrame<T, 8, 2>>());
+  if (thread_rows(s)) {
+    pick_thread_rows<T>(s, turns);
+  } else if (s.class_major()) {
+    pick_list_slices<T>(s, turns);
   } else if (chunks <= 32) {
-    row_turns(FrameTag<RowFrame<T, 16, 2>>());
+    pick_few_threads<T>(s, chunks, turns);
   } else if (chunks <= 64) {
     candidates(FrameTag<RowFrame<T, 64, 1>>());
   } else if (chunks <= 128) {

@@ -95,7 +95,7 @@ __global__ __launch_bounds__(F::kMax) void alternatives_grad_lane_kernel(ScoresV
   };
   if (g.label) add(g.label[i], g.grad_label[i]);
   for (int32_t e = 0; e < g.k; ++e)
-    add(g.classes[i * g.class_stride + e], g.grad_list[i * g.grad_stride + e]);
+    add(g.classes[i * g.class_stride + e * g.class_step], g.grad_list[i * g.grad_stride + e * g.grad_step]);
   const AltGradRow r = alt_grad_row(g, i, all, any);
   if (!r.live && accumulate) return;
   f.store(out, blockIdx.x, accumulate, [&](int j) {
@@ -137,14 +137,13 @@ __global__ __launch_bounds__(F::kMax) void alternatives_grad_slices_kernel(Score
   __syncthreads();
   const int32_t* const classes = g.classes + i * g.class_stride;
   const float* const grads = g.grad_list + i * g.grad_stride;
-  const auto class_of_entry = [&](int j) { return j < k ? classes[j] : g.label ? g.label[i] : -1; };
   float sum[2] = {0.0f, 0.0f};  // of the g, and how many are not 0
   bool twice = false;
-  for (int j = f.w; j < all; j += f.S) {
-    const int32_t c = class_of_entry(j);
+  for (int j = f.w; j < k; j += f.S) {
+    const int32_t c = classes[j * g.class_step];
     float x = 0.0f;
     if ((uint32_t)c < (uint32_t)s.K) {
-      x = j < k ? grads[j] : g.grad_label[i];
+      x = grads[j * g.grad_step];
       sum[0] += x;
       sum[1] += x != 0.0f ? 1.0f : 0.0f;
       twice |= map.put(f, c, j);
@@ -154,20 +153,37 @@ __global__ __launch_bounds__(F::kMax) void alternatives_grad_slices_kernel(Score
   }
   if (__syncthreads_or(twice)) {
     // the first of the entries that name a class takes its place, and all their g
-    for (int j = f.w; j < all; j += f.S) {
-      const int32_t c = class_of_entry(j);
+    for (int j = f.w; j < k; j += f.S) {
+      const int32_t c = classes[j * g.class_step];
       bool first = (uint32_t)c < (uint32_t)s.K;
-      for (int o = 0; o < j; ++o) first &= classes[o] != c;
+      for (int o = 0; o < j; ++o) first &= classes[o * g.class_step] != c;
       if (!first) continue;
       map.set(f, c, j);
       // (later entries' own numbers: only first entries' are changed)
       float more = 0.0f;
-      for (int o = j + 1; o < all; ++o)
-        if (class_of_entry(o) == c) more += own[64 * o];
+      for (int o = j + 1; o < k; ++o)
+        if (classes[o * g.class_step] == c) more += own[64 * o];
       own[64 * j] += more;
     }
     __syncthreads();
   }
+  if (f.w == 0) {
+    // the label, an entry of its own unless the list has it
+    const int32_t c = row_label(g.label, i, s.K);
+    const float x = c >= 0 ? g.grad_label[i] : 0.0f;
+    sum[0] += x;
+    sum[1] += x != 0.0f ? 1.0f : 0.0f;
+    own[64 * k] = x;
+    score[64 * k] = 0.0f;
+    if (c >= 0) {
+      const int e = map.get(f, c);
+      if (e)
+        own[64 * (e - 1)] += x;
+      else
+        map.set(f, c, k);
+    }
+  }
+  __syncthreads();
   uint32_t mine[Map::kWords];
   map.mine(mine);
 #pragma unroll
@@ -177,7 +193,7 @@ __global__ __launch_bounds__(F::kMax) void alternatives_grad_slices_kernel(Score
   }
   f.reduce_all(sum, AddF(), buf);
   const AltGradRow r = alt_grad_row(g, i, sum[0], sum[1] != 0.0f);
-  for (int j = f.w; j < all; j += f.S)
+  for (int j = f.w; j <= k; j += f.S)
     score[64 * j] = alt_grad_listed(r, g, score[64 * j], own[64 * j]);
   __syncthreads();
   // (one store for rows that count and rows left out: lanes of a wave may hold both)
@@ -228,11 +244,11 @@ __global__ __launch_bounds__(F::kMax) void alternatives_grad_list_kernel(ScoresV
   int word;
   uint32_t bit;
   for (int j = f.entry(); j < k; j += f.entry_step()) {
-    int32_t c = g.classes[i * g.class_stride + j];
+    int32_t c = g.classes[i * g.class_stride + j * g.class_step];
     float own = 0.0f, sc = 0.0f;
     if (c < 0 || c >= whole.K) c = -1;
     if (c >= 0) {
-      own = g.grad_list[i * g.grad_stride + j];
+      own = g.grad_list[i * g.grad_stride + j * g.grad_step];
       sum[0] += own;
       sum[1] += own != 0.0f ? 1.0f : 0.0f;
       if (c >= k0 && c - k0 < s.K) {
@@ -312,14 +328,15 @@ __global__ __launch_bounds__(F::kMax) void alternatives_grad_list_kernel(ScoresV
 template <typename T, typename Fn>
 static void pick_short_frame(const ScoresView& s, Fn fn) {
   constexpr int VE = Chunk<T>::VE;
-  if (s.class_major() || s.K < VE) return pick_class_frame<T>(s, fn);
+  if (thread_rows(s)) return pick_thread_rows<T>(s, fn);
+  if (s.class_major()) return pick_list_slices<T>(s, fn);
   const int64_t chunks = (s.K + VE - 1) / VE;
   const auto go = [&](auto tag) {
     using F = typename decltype(tag)::type;
     fn(tag, (s.n + F::kRows - 1) / F::kRows, F::kThreads);
   };
   if (chunks <= 4) return go(FrameTag<RowFrame<T, 4, 1>>());
-  if (chunks <= 8) return go(FrameTag<RowFrame<T, 8, 1>>());
+  if (chunks <= 8) return go(FrameTag<RowFrame<T, 4, 2>>());
   if (chunks <= 16) return go(FrameTag<RowFrame<T, 8, 2>>());
   if (chunks <= 32) return go(FrameTag<RowFrame<T, 16, 2>>());
   if (chunks <= 64) return go(FrameTag<RowFrame<T, 32, 2>>());

@@ -181,9 +181,13 @@ static int list_length(int32_t k, int32_t least, const char* what) {
                what, least, kMaxList, k);
   return 0;
 }
-static int list_stride(int64_t stride, int32_t k, const char* what) {
-  WGBM_REQUIRE(stride >= k && stride < (int64_t(1) << 40), "%s: a list's stride is out of range",
-               what);
+static int list_strides(int64_t stride, int64_t step, int64_t n, int32_t k, const char* what) {
+  WGBM_REQUIRE((step == 1 && stride >= k) || (stride == 1 && step >= n),
+               "%s: a list's strides (%lld, %lld) are neither those of rows nor of entries next to "
+               "each other without overlap",
+               what, (long long)stride, (long long)step);
+  WGBM_REQUIRE(stride < (int64_t(1) << 40) && step < (int64_t(1) << 40),
+               "%s: a list's stride is out of range", what);
   return 0;
 }
 
@@ -240,8 +244,10 @@ int wgbm_class_alternatives_grad(const wgbm_scores* scores,
   AltGradRows g{};
   TRY(tempered(a->temperature, "class_alternatives_grad", &g.scale, &g.inv_tau));
   if (a->list_length) {
-    TRY(list_stride(a->classes_stride, a->list_length, "class_alternatives_grad"));
-    TRY(list_stride(a->grad_stride, a->list_length, "class_alternatives_grad"));
+    TRY(list_strides(a->classes_stride, a->classes_step, s.n, a->list_length,
+                     "class_alternatives_grad"));
+    TRY(list_strides(a->grad_stride, a->grad_step, s.n, a->list_length,
+                     "class_alternatives_grad"));
   }
   if (s.n == 0) return 0;
   WGBM_REQUIRE(a->norm && (!a->labels || a->grad_label_log_prob) &&
@@ -255,8 +261,10 @@ int wgbm_class_alternatives_grad(const wgbm_scores* scores,
   g.grad_label = a->grad_label_log_prob;
   g.classes = a->classes;
   g.class_stride = a->classes_stride;
+  g.class_step = a->classes_step;
   g.grad_list = a->grad_log_prob;
   g.grad_stride = a->grad_stride;
+  g.grad_step = a->grad_step;
   g.k = a->list_length;
   g.grad_entropy = a->grad_entropy;
   return class_alternatives_grad(s, g, o, accumulate != 0, workspace, S(stream));
@@ -279,8 +287,8 @@ int wgbm_distill_loss(const wgbm_scores* scores, const wgbm_distill_args* a, flo
   }
   WGBM_REQUIRE(a, "distill_loss: null arguments");
   TRY(list_length(a->list_length, 1, "distill_loss"));
-  TRY(list_stride(a->classes_stride, a->list_length, "distill_loss"));
-  TRY(list_stride(a->logits_stride, a->list_length, "distill_loss"));
+  TRY(list_strides(a->classes_stride, a->classes_step, s.n, a->list_length, "distill_loss"));
+  TRY(list_strides(a->logits_stride, a->logits_step, s.n, a->list_length, "distill_loss"));
   DistillRows g{};
   TRY(tempered(a->temperature, "distill_loss", &g.scale, &g.inv_tau));
   WGBM_REQUIRE(a->log_norm || !a->rest || std::isfinite(a->log_norm_all),
@@ -292,8 +300,10 @@ int wgbm_distill_loss(const wgbm_scores* scores, const wgbm_distill_args* a, flo
                "distill_loss: workspace too small");
   g.classes = a->classes;
   g.class_stride = a->classes_stride;
+  g.class_step = a->classes_step;
   g.logits = a->logits;
   g.logit_stride = a->logits_stride;
+  g.logit_step = a->logits_step;
   g.k = a->list_length;
   g.rest = a->rest != 0;
   g.log_norm = a->rest ? a->log_norm : nullptr;

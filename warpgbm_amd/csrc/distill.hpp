@@ -152,8 +152,8 @@ __global__ __launch_bounds__(F::kMax) void distill_lane_kernel(ScoresView s, Dis
   float m = -__builtin_inff(), lm = m;
   const int k = w != 0.0f ? g.k : 0;
   for (int e = 0; e < k; ++e) {
-    const int32_t c = classes[e];
-    const float l = logits[e];
+    const int32_t c = classes[e * g.class_step];
+    const float l = logits[e * g.logit_step];
     if ((uint32_t)c >= (uint32_t)s.K || (listed >> c & 1)) continue;  // (the first one counts)
     listed |= 1u << c;
     logit[c][t] = l;
@@ -260,8 +260,8 @@ __global__ __launch_bounds__(F::kMax) void distill_slices_kernel(ScoresView s, D
   uint32_t used = 0;  // a bit for each of this thread's entries j = f.w, f.w + f.S, ...
   bool twice = false;
   for (int j = f.w, n = 0; j < k; j += f.S, ++n) {
-    const int32_t c = classes[j];
-    logit[64 * j] = logits[j];
+    const int32_t c = classes[j * g.class_step];
+    logit[64 * j] = logits[j * g.logit_step];
     score[64 * j] = -__builtin_inff();
     if (w != 0.0f && (uint32_t)c < (uint32_t)s.K) {
       used |= 1u << n;
@@ -271,9 +271,9 @@ __global__ __launch_bounds__(F::kMax) void distill_slices_kernel(ScoresView s, D
   if (__syncthreads_or(twice)) {
     // the first of the entries that name a class takes its place
     for (int j = f.w, n = 0; j < k; j += f.S, ++n) {
-      const int32_t c = classes[j];
+      const int32_t c = classes[j * g.class_step];
       for (int o = 0; o < j; ++o)
-        if (classes[o] == c) used &= ~(1u << n);
+        if (classes[o * g.class_step] == c) used &= ~(1u << n);
       if (used >> n & 1) map.set(f, c, j);
     }
     __syncthreads();
@@ -434,8 +434,8 @@ __global__ __launch_bounds__(F::kMax) void distill_frame_kernel(ScoresView s, Di
   const float* const logits = g.logits + i * g.logit_stride;
   const T* const scores = (const T*)s.data + i * s.rs;
   for (int j = f.entry(); j < k; j += f.entry_step()) {
-    int32_t c = w != 0.0f ? classes[j] : -1;
-    float l = logits[j], sc = -__builtin_inff();
+    int32_t c = w != 0.0f ? classes[j * g.class_step] : -1;
+    float l = logits[j * g.logit_step], sc = -__builtin_inff();
     if (c < 0 || c >= s.K) c = -1;
     if (c >= 0) {
       int word;
@@ -535,10 +535,10 @@ __global__ __launch_bounds__(1024) void distill_long_kernel(ScoresView s, Distil
   // the list: an entry a thread; repeated classes by comparison (a tile's bits say
   // nothing of the others)
   for (int j = threadIdx.x; j < k; j += 1024) {
-    int32_t c = w != 0.0f ? g.classes[i * g.class_stride + j] : -1;
+    int32_t c = w != 0.0f ? g.classes[i * g.class_stride + j * g.class_step] : -1;
     if (c < 0 || c >= s.K) c = -1;
     tab.cls[j] = c;
-    tab.logit[j] = c >= 0 ? g.logits[i * g.logit_stride + j] : 0.0f;
+    tab.logit[j] = c >= 0 ? g.logits[i * g.logit_stride + j * g.logit_step] : 0.0f;
     tab.score[j] = c >= 0 ? score_at<T>(s, i, c) : -__builtin_inff();
   }
   __syncthreads();
@@ -645,7 +645,7 @@ static int distill_frames(const ScoresView& s, const DistillRows& g, const Score
     WGBM_LAUNCH_CHECK();
     return 0;
   }
-  pick_frame<T, false, true>(s, [&](auto tag, int64_t blocks, int threads) {
+  const auto launch = [&](auto tag, int64_t blocks, int threads) {
     using F = typename decltype(tag)::type;
     if constexpr (F::kLaneRows && !F::kSlices) {
       hipLaunchKernelGGL((distill_lane_kernel<F>), dim3((unsigned)blocks), dim3(threads), 0, st, s,
@@ -659,7 +659,18 @@ static int distill_frames(const ScoresView& s, const DistillRows& g, const Score
       hipLaunchKernelGGL((distill_frame_kernel<F>), dim3((unsigned)blocks), dim3(threads), lds, st,
                          s, g, out, accumulate);
     }
-  });
+  };
+  const int64_t chunks = (s.K + Chunk<T>::VE - 1) / Chunk<T>::VE;
+  if (thread_rows(s))
+    pick_thread_rows<T>(s, launch);
+  else if (s.class_major())
+    pick_list_slices<T>(s, launch);
+  else if (chunks <= 32)
+    pick_few_threads<T>(s, chunks, launch);
+  else if (chunks <= 64)  // (20047 x 257 float16 15.8 us, with 32 threads of two chunks 18.1)
+    launch(FrameTag<RowFrame<T, 16, 4>>(), (s.n + 15) / 16, 256);
+  else
+    pick_row_frame<T, false, true>(s, launch);
   WGBM_LAUNCH_CHECK();
   return 0;
 }

@@ -74,10 +74,10 @@ struct AltGradRows {
   const float* norm;
   const int32_t* label;  // null: none
   const float* grad_label;
-  const int32_t* classes;  // row i's entries at classes + i * class_stride
-  int64_t class_stride;
+  const int32_t* classes;  // row i's entry j at classes + i * class_stride + j * class_step
+  int64_t class_stride, class_step;
   const float* grad_list;
-  int64_t grad_stride;
+  int64_t grad_stride, grad_step;
   int32_t k;
   const float* grad_entropy;  // null: 0
   float scale;
@@ -85,9 +85,9 @@ struct AltGradRows {
 };
 struct DistillRows {
   const int32_t* classes;
-  int64_t class_stride;
+  int64_t class_stride, class_step;
   const float* logits;
-  int64_t logit_stride;
+  int64_t logit_stride, logit_step;
   int32_t k;
   bool rest;              // the classes that are not listed count
   const float* log_norm;  // null: log_norm_all for every row

@@ -102,6 +102,11 @@ struct SliceMap {
     const int word = at(f, c, shift);
     ((uint8_t*)&words[word])[shift / 8] = (uint8_t)(j + 1);
   }
+  __device__ __forceinline__ int get(const F& f, int32_t c) const {
+    int shift;
+    const int word = at(f, c, shift);
+    return words[word] >> shift & 255;
+  }
   __device__ __forceinline__ void mine(uint32_t (&m)[kWords]) const {
 #pragma unroll
     for (int q = 0; q < kWords; ++q) m[q] = words[q * blockDim.x + threadIdx.x];
@@ -110,6 +115,64 @@ struct SliceMap {
     return m[slot / 4] >> (slot % 4 * 8) & 255;
   }
 };
+
+// Which slices rows with lists take: fn(frame tag, workgroups, threads).  What a row's
+// list costs is shared by its waves, but each wave joins what all have, so fewer waves
+// with more classes each than pick_slices takes: 4, 8, 12 or 16, which fill the SIMDs
+// evenly.  Distillation, us: 1M x 100 float32, 16 listed, 4 waves of 26 242, 8 of 13 280,
+// 2 of 50 310, 5 of 20 297; 300000 x 200 8 waves of 26 134, 16 of 13 214; 150000 x 400
+// 12 of 36 141, 13 of 32 197; 500000 x 64 4 of 16 78, 8 of 8 103.
+template <typename T, typename Fn>
+static void pick_list_slices(const ScoresView& s, Fn fn) {
+  const auto go = [&](auto tag, int S) { fn(tag, (s.n + 63) / 64, 64 * S); };
+  const int S = s.K <= 128 ? 4 : s.K <= 256 ? 8 : s.K <= 432 ? 12 : 16;
+  const int N = (s.K + S - 1) / S;
+  if (N <= 8) return go(FrameTag<ClassFrame<T, 8, true, true>>(), S);
+  if (N <= 10) return go(FrameTag<ClassFrame<T, 10, true, true>>(), S);
+  if (N <= 13) return go(FrameTag<ClassFrame<T, 13, true, true>>(), S);
+  if (N <= 16) return go(FrameTag<ClassFrame<T, 16, true, true>>(), S);
+  if (N <= 20) return go(FrameTag<ClassFrame<T, 20, true, true>>(), S);
+  if (N <= 26) return go(FrameTag<ClassFrame<T, 26, true, true>>(), S);
+  if (N <= 32) return go(FrameTag<ClassFrame<T, 32, true, true>>(), S);
+  go(FrameTag<ClassFrame<T, 36, true, true>>(), S);
+}
+
+// Whether a thread takes a whole row: class-major up to 16 classes, and row-major ones
+// up to 12 (a lane's loads are 48 bytes apart at most), which share what a row costs as
+// a whole with nobody.  1M x 10 row-major, a thread a row and four: best three classes
+// float32 23 and 39 us, bfloat16 21 and 48; distillation 50 and 66, 34 and 71; gradient 44
+// and 45, 30 and 50; but of 1M x 16 float32 38 and 36, 113 and 60, 97 and 42.
+static inline bool thread_rows(const ScoresView& s) {
+  return s.K <= (s.class_major() ? 16 : 12);
+}
+template <typename T, typename Fn>
+static void pick_thread_rows(const ScoresView& s, Fn fn) {
+  if (s.class_major()) return pick_class_frame<T>(s, fn);
+  const int64_t blocks = (s.n + 255) / 256;
+  if (s.K <= 4) return fn(FrameTag<ClassFrame<T, 4, false, false>>(), blocks, 256);
+  if (s.K <= 8) return fn(FrameTag<ClassFrame<T, 8, false, false>>(), blocks, 256);
+  fn(FrameTag<ClassFrame<T, 12, false, false>>(), blocks, 256);
+}
+
+// Row-major rows of up to 32 chunks with work for each row as a whole: few threads a
+// row, so that a wave spends it on more rows, where there are rows enough.  300000 x 30
+// float32, 4 threads of two chunks and 8 of one: best four classes 20 and 27 us,
+// distillation 27 and 38; 200000 x 60, 4 of four and 8 of two: 25 and 30, 30 and 32;
+// 300000 x 100, 8 of four and 16 of two: 55 and 74, 56 and 80.
+template <typename T, typename Fn>
+static void pick_few_threads(const ScoresView& s, int64_t chunks, Fn fn) {
+  const auto go = [&](auto tag) {
+    using F = typename decltype(tag)::type;
+    fn(tag, (s.n + F::kRows - 1) / F::kRows, F::kThreads);
+  };
+  const bool many = s.n * chunks >= kLossWaves * 128;
+  if (chunks <= 4) return go(FrameTag<RowFrame<T, 4, 1>>());
+  if (chunks <= 8)
+    return many ? go(FrameTag<RowFrame<T, 4, 2>>()) : go(FrameTag<RowFrame<T, 8, 1>>());
+  if (chunks <= 16)
+    return many ? go(FrameTag<RowFrame<T, 4, 4>>()) : go(FrameTag<RowFrame<T, 8, 2>>());
+  many ? go(FrameTag<RowFrame<T, 8, 4>>()) : go(FrameTag<RowFrame<T, 16, 2>>());
+}
 
 // a part of a row's classes as a matrix of its own: tile t of tiles, at least 8
 // classes each

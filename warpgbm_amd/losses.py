@@ -10,8 +10,8 @@ squared error and softmax cross entropy, warpgbm/core.py:186-214, 719).
 Scores are [n rows, K classes] in float32, bfloat16 or float16, with either the
 classes of a row next to each other (``scores`` contiguous, or rows with a
 stride) or the rows of a class (``scores_cm.t()`` of the engine's class-major
-[K, n]).  Per-row inputs are contiguous.  A score of -inf is a class that the
-row may not take; a row whose scores are all -inf counts as left out.  Rows
+[K, n]).  Per-row inputs are contiguous; lists [n, k] of a row's classes have
+either order too.  A score of -inf is a class that the row may not take; a row whose scores are all -inf counts as left out.  Rows
 left out (weight 0, mask false, label outside [0, K)) are not read: their
 results and gradients are 0, whatever their scores hold.
 
@@ -211,8 +211,8 @@ def _workspace(entry, v, device):
 
 
 def _list(t, name, dtype, n, k, device):
-    """A [n, k] tensor of dtype on device whose rows are contiguous (any stride from
-    row to row); its address and stride."""
+    """A [n, k] tensor of dtype on device, its rows or its columns contiguous; its
+    address and strides."""
     if not isinstance(t, torch.Tensor):
         raise RuntimeError(f"{name} must be a torch.Tensor")
     if t.dtype != dtype:
@@ -221,13 +221,9 @@ def _list(t, name, dtype, n, k, device):
         raise RuntimeError(f"{name} must be on {device}, got {t.device}")
     if t.dim() != 2 or tuple(t.shape) != (n, k):
         raise RuntimeError(f"{name} must have shape ({n}, {k}), got {tuple(t.shape)}")
-    rs, ks = t.stride()
-    if n <= 1 or k == 0:
-        rs = k
-    if (k > 1 and ks != 1) or rs < k:
-        raise RuntimeError(f"{name} must have the entries of a row next to each other (no overlap), "
-                           f"got strides {t.stride()}")
-    return t.data_ptr(), rs
+    if k == 0:
+        return t.data_ptr(), 1, n
+    return (t.data_ptr(), *_strides(n, k, *t.stride(), name))
 
 
 def _length(t, name):
@@ -444,8 +440,10 @@ def class_alternatives_grad(scores, norm, *, labels=None, grad_label_log_prob=No
         k = _length(classes, "classes")
         if k > MAX_LIST:
             raise RuntimeError(f"classes must have at most {MAX_LIST} entries a row, got {k}")
-        args.classes, args.classes_stride = _list(classes, "classes", torch.int32, n, k, dev)
-        args.grad_log_prob, args.grad_stride = _list(grad_log_prob, "grad_log_prob", f32, n, k, dev)
+        args.classes, args.classes_stride, args.classes_step = _list(
+            classes, "classes", torch.int32, n, k, dev)
+        args.grad_log_prob, args.grad_stride, args.grad_step = _list(
+            grad_log_prob, "grad_log_prob", f32, n, k, dev)
         args.list_length = k
     if grad_entropy is not None:
         args.grad_entropy = _vector(grad_entropy, "grad_entropy", f32, n, dev)
@@ -492,8 +490,9 @@ def distill_loss(scores, classes, logits, *, log_norm=None, weight=None, tempera
     if not 1 <= k <= MAX_LIST:
         raise RuntimeError(f"classes must have 1 to {MAX_LIST} entries a row, got {k}")
     args = _lib.DistillArgs(list_length=k, temperature=_temperature(temperature))
-    args.classes, args.classes_stride = _list(classes, "classes", torch.int32, n, k, dev)
-    args.logits, args.logits_stride = _list(logits, "logits", f32, n, k, dev)
+    args.classes, args.classes_stride, args.classes_step = _list(
+        classes, "classes", torch.int32, n, k, dev)
+    args.logits, args.logits_stride, args.logits_step = _list(logits, "logits", f32, n, k, dev)
     norms = None
     if log_norm is not None:
         args.rest = 1
