@@ -74,9 +74,8 @@ __device__ __forceinline__ DistillRow distill_row(const DistillSums& a, const Di
   const float B = has_rest ? exp_of((float)drop) * a.zr : 0.0f;
   const float A = a.zl + a.zl_ties;
   o.live = w != 0.0f && !(A + B == 0.0f);
-  // (the largest term, 1, is among the listed or among the others)
-  const float over = a.zl_ties > 0.0f ? a.zl + (a.zl_ties - 1.0f) + B : -1.0f;
-  const double lse = over >= 0.0f ? log_1p(over) : log_of(A + B);
+  // without the largest term, 1, which is among the listed or among the others
+  const double lse = log_1p(a.zl_ties > 0.0f ? a.zl + (a.zl_ties - 1.0f) + B : A + (B - 1.0f));
   // shares: `one` of the largest logit, C of the other counting ones
   const bool counts = lm > -__builtin_inff() || a.q != a.q;
   const double norm = g.rest ? (double)(g.log_norm ? g.log_norm[i] : g.log_norm_all) : 0.0;
@@ -94,7 +93,8 @@ __device__ __forceinline__ DistillRow distill_row(const DistillSums& a, const Di
     Q = rest ? left : 0.0f;
     // what is left out of sum 1
     const float lost = a.out + (rest ? 0.0f : left);
-    log_mass = lost < 0.5f ? (double)log1p_of(-lost) : log_of(one + C + Q);
+    log_mass = (double)log1p_of(-lost);
+    if (!(lost < 0.5f)) log_mass = log_of(one + C + Q);
     o.live = o.live && (counts || rest) && !(one + C + Q == 0.0f);
     shift = norm + log_mass;
   }
@@ -103,7 +103,8 @@ __device__ __forceinline__ DistillRow distill_row(const DistillSums& a, const Di
   o.apart = (double)o.m * g.inv_tau + lse - shift;
   // the others
   if (has_rest) {
-    const double log_P = B >= A ? -(double)log1p_of(A / B) : drop + log_of(a.zr) - lse;
+    double log_P = -log_1p(A / B);
+    if (!(B > 1e-30f * A)) log_P = drop + log_of(a.zr) - lse;
     const float P = exp_of((float)log_P);
     Bucket b{P, P};
     if (Q > 0.0f) {

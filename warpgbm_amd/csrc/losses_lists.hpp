@@ -14,9 +14,11 @@ namespace wgbm {
 // power no lower (0 * infinity would be NaN)
 constexpr float kLowPower = -1000.0f;
 
-// log(1 + z) of a float32 sum z >= 0 with all its digits
+// log(1 + z) of a float32 sum z >= 0 with all its digits, large or small: the
+// logarithm of the rounded sum (its exponent apart) and what the rounding left out
 __device__ __forceinline__ double log_1p(float z) {
-  return z <= 1.0f ? (double)log1p_of(z) : log_of(1.0f + z);
+  const float w = 1.0f + z;
+  return log_of(w) + (double)((z - (w - 1.0f)) * __builtin_amdgcn_rcpf(w));
 }
 
 // phi(x) = e^x - 1 - x for |x| <= 1
