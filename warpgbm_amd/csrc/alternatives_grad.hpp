@@ -80,6 +80,11 @@ __global__ __launch_bounds__(F::kMax) void alternatives_grad_lane_kernel(ScoresV
   const F f(s);
   const int64_t i = F::row(blockIdx.x);
   if (i >= s.n) return;
+  const int32_t* const classes = g.classes + i * g.class_stride;
+  const float* const grads = g.grad_list + i * g.grad_stride;
+  using Batch = EntryBatch<float>;
+  Batch b;
+  b.load(classes, g.class_step, grads, g.grad_step, 0, 1, g.k);
   typename F::Regs v;
   f.load(v, s, blockIdx.x);
   float own[F::N], all = 0.0f;
@@ -94,8 +99,11 @@ __global__ __launch_bounds__(F::kMax) void alternatives_grad_lane_kernel(ScoresV
     for (int j = 0; j < F::N; ++j) own[j] += f.cls(j) == c ? x : 0.0f;
   };
   if (g.label) add(g.label[i], g.grad_label[i]);
-  for (int32_t e = 0; e < g.k; ++e)
-    add(g.classes[i * g.class_stride + e * g.class_step], g.grad_list[i * g.grad_stride + e * g.grad_step]);
+  for (int first = 0; first < g.k; first += Batch::kSize) {
+    if (first) b.load(classes, g.class_step, grads, g.grad_step, first, 1, g.k);
+#pragma unroll
+    for (int q = 0; q < Batch::kSize; ++q) add(first + q < g.k ? b.cls[q] : -1, b.value[q]);
+  }
   const AltGradRow r = alt_grad_row(g, i, all, any);
   if (!r.live && accumulate) return;
   f.store(out, blockIdx.x, accumulate, [&](int j) {
@@ -131,25 +139,33 @@ __global__ __launch_bounds__(F::kMax) void alternatives_grad_slices_kernel(Score
   const int64_t row = F::row(blockIdx.x);
   const bool in = row < s.n;
   const int64_t i = in ? row : s.n - 1;
+  const int32_t* const classes = g.classes + i * g.class_stride;
+  const float* const grads = g.grad_list + i * g.grad_stride;
+  using Batch = EntryBatch<float>;
+  Batch b;
+  b.load(classes, g.class_step, grads, g.grad_step, f.w, f.S, k);
   typename F::Regs v;
   f.load(v, s, blockIdx.x);
   map.clear();
   __syncthreads();
-  const int32_t* const classes = g.classes + i * g.class_stride;
-  const float* const grads = g.grad_list + i * g.grad_stride;
   float sum[2] = {0.0f, 0.0f};  // of the g, and how many are not 0
   bool twice = false;
-  for (int j = f.w; j < k; j += f.S) {
-    const int32_t c = classes[j * g.class_step];
-    float x = 0.0f;
-    if ((uint32_t)c < (uint32_t)s.K) {
-      x = grads[j * g.grad_step];
-      sum[0] += x;
-      sum[1] += x != 0.0f ? 1.0f : 0.0f;
-      twice |= map.put(f, c, j);
+  for (int first = f.w; first < k; first += Batch::kSize * f.S) {
+    if (first != f.w) b.load(classes, g.class_step, grads, g.grad_step, first, f.S, k);
+#pragma unroll
+    for (int q = 0; q < Batch::kSize; ++q) {
+      const int j = first + q * f.S;
+      if (j >= k) break;
+      float x = 0.0f;
+      if ((uint32_t)b.cls[q] < (uint32_t)s.K) {
+        x = b.value[q];
+        sum[0] += x;
+        sum[1] += x != 0.0f ? 1.0f : 0.0f;
+        twice |= map.put(f, b.cls[q], j);
+      }
+      own[64 * j] = x;
+      score[64 * j] = 0.0f;
     }
-    own[64 * j] = x;
-    score[64 * j] = 0.0f;
   }
   if (__syncthreads_or(twice)) {
     // the first of the entries that name a class takes its place, and all their g

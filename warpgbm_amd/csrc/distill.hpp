@@ -139,6 +139,11 @@ __global__ __launch_bounds__(F::kMax) void distill_lane_kernel(ScoresView s, Dis
   const int t = threadIdx.x;
   const int64_t i = F::row(blockIdx.x);
   if (i >= s.n) return;
+  const int32_t* const classes = g.classes + i * g.class_stride;
+  const float* const logits = g.logits + i * g.logit_stride;
+  using Batch = EntryBatch<float>;
+  Batch b;
+  b.load(classes, g.class_step, logits, g.logit_step, 0, 1, g.k);
   const float w = g.weight ? g.weight[i] : 1.0f;
   typename F::Regs v;
   f.load(v, s, blockIdx.x);
@@ -148,19 +153,21 @@ __global__ __launch_bounds__(F::kMax) void distill_lane_kernel(ScoresView s, Dis
 #pragma unroll
   for (int j = 0; j < N; ++j) score[j][t] = F::value(v, j);
   uint32_t listed = 0;
-  const int32_t* const classes = g.classes + i * g.class_stride;
-  const float* const logits = g.logits + i * g.logit_stride;
   float m = -__builtin_inff(), lm = m;
   const int k = w != 0.0f ? g.k : 0;
-  for (int e = 0; e < k; ++e) {
-    const int32_t c = classes[e * g.class_step];
-    const float l = logits[e * g.logit_step];
-    if ((uint32_t)c >= (uint32_t)s.K || (listed >> c & 1)) continue;  // (the first one counts)
-    listed |= 1u << c;
-    logit[c][t] = l;
-    const float sc = score[c][t];
-    m = fmaxf(m, sc);
-    lm = closed(sc) ? lm : fmaxf(lm, l);
+  for (int first = 0; first < k; first += Batch::kSize) {
+    if (first) b.load(classes, g.class_step, logits, g.logit_step, first, 1, k);
+#pragma unroll
+    for (int q = 0; q < Batch::kSize; ++q) {
+      const int32_t c = b.cls[q];
+      // (the first of the entries that name a class counts)
+      if (first + q >= k || (uint32_t)c >= (uint32_t)s.K || (listed >> c & 1)) continue;
+      listed |= 1u << c;
+      logit[c][t] = b.value[q];
+      const float sc = score[c][t];
+      m = fmaxf(m, sc);
+      lm = closed(sc) ? lm : fmaxf(lm, b.value[q]);
+    }
   }
   float mr = -__builtin_inff();
 #pragma unroll
@@ -175,8 +182,8 @@ __global__ __launch_bounds__(F::kMax) void distill_lane_kernel(ScoresView s, Dis
     a.zr += e[j];
   }
   const float norm = g.rest ? (g.log_norm ? g.log_norm[i] : g.log_norm_all) : 0.0f;
-  for (uint32_t b = listed; b; b &= b - 1) {
-    const int c = __ffs(b) - 1;
+  for (uint32_t left = listed; left; left &= left - 1) {
+    const int c = __ffs(left) - 1;
     const float sc = score[c][t], l = logit[c][t];
     if (closed(sc)) {
       if (g.rest) a.out += exp_of((float)((double)l * g.inv_tau - (double)norm));
@@ -190,8 +197,8 @@ __global__ __launch_bounds__(F::kMax) void distill_lane_kernel(ScoresView s, Dis
   }
   const DistillRow r = distill_row(a, g, i, m, mr, lm, w);
   float loss = r.rest_term;
-  for (uint32_t b = listed; b; b &= b - 1) {
-    const int c = __ffs(b) - 1;
+  for (uint32_t left = listed; left; left &= left - 1) {
+    const int c = __ffs(left) - 1;
     const float sc = score[c][t];
     float grad = 0.0f;
     if (!closed(sc)) {
@@ -251,22 +258,30 @@ __global__ __launch_bounds__(F::kMax) void distill_slices_kernel(ScoresView s, D
   const int64_t row = F::row(blockIdx.x);
   const bool in = row < s.n;
   const int64_t i = in ? row : s.n - 1;
-  typename F::Regs v;
-  f.load(v, s, blockIdx.x);
-  const float w = !in ? 0.0f : g.weight ? g.weight[i] : 1.0f;
-  map.clear();
-  __syncthreads();
   const int32_t* const classes = g.classes + i * g.class_stride;
   const float* const logits = g.logits + i * g.logit_stride;
+  using Batch = EntryBatch<float>;
+  Batch b;
+  b.load(classes, g.class_step, logits, g.logit_step, f.w, f.S, k);
+  const float w = !in ? 0.0f : g.weight ? g.weight[i] : 1.0f;
+  typename F::Regs v;
+  f.load(v, s, blockIdx.x);
+  map.clear();
+  __syncthreads();
   uint32_t used = 0;  // a bit for each of this thread's entries j = f.w, f.w + f.S, ...
   bool twice = false;
-  for (int j = f.w, n = 0; j < k; j += f.S, ++n) {
-    const int32_t c = classes[j * g.class_step];
-    logit[64 * j] = logits[j * g.logit_step];
-    score[64 * j] = -__builtin_inff();
-    if (w != 0.0f && (uint32_t)c < (uint32_t)s.K) {
-      used |= 1u << n;
-      twice |= map.put(f, c, j);
+  for (int first = f.w, n = 0; first < k; first += Batch::kSize * f.S) {
+    if (n) b.load(classes, g.class_step, logits, g.logit_step, first, f.S, k);
+#pragma unroll
+    for (int q = 0; q < Batch::kSize; ++q, ++n) {
+      const int j = first + q * f.S;
+      if (j >= k) break;
+      logit[64 * j] = b.value[q];
+      score[64 * j] = -__builtin_inff();
+      if (w != 0.0f && (uint32_t)b.cls[q] < (uint32_t)s.K) {
+        used |= 1u << n;
+        twice |= map.put(f, b.cls[q], j);
+      }
     }
   }
   if (__syncthreads_or(twice)) {
@@ -324,10 +339,10 @@ __global__ __launch_bounds__(F::kMax) void distill_slices_kernel(ScoresView s, D
   float loss[1] = {0.0f};
   for (int j = f.w; j < k; j += f.S) {
     const float sc = score[64 * j];
-    Bucket b{0.0f, 0.0f};
-    if (!closed(sc)) b = distill_entry(r, g, sc, logit[64 * j]);
-    loss[0] += b.term;
-    score[64 * j] = r.scale * b.slope;
+    Bucket u{0.0f, 0.0f};
+    if (!closed(sc)) u = distill_entry(r, g, sc, logit[64 * j]);
+    loss[0] += u.term;
+    score[64 * j] = r.scale * u.slope;
   }
   f.put_all(loss, AddF(), buf + 9 * blockDim.x);
   __syncthreads();

@@ -69,6 +69,24 @@ __device__ __forceinline__ bool listed_before(const F& f, const int32_t* cls, in
   return false;
 }
 
+// Entries first, first + step, ... of a row's list (k of them), four at a time: a batch's
+// loads are in flight together, the first batch's before the row's scores are waited for.
+template <typename V>
+struct EntryBatch {
+  static constexpr int kSize = 4;
+  int32_t cls[kSize];
+  V value[kSize];
+  __device__ __forceinline__ void load(const int32_t* classes, int64_t class_step, const V* values,
+                                       int64_t value_step, int first, int step, int k) {
+#pragma unroll
+    for (int q = 0; q < kSize; ++q) {
+      const int j = first + q * step < k ? first + q * step : k - 1;
+      cls[q] = classes[j * class_step];
+      value[q] = values[j * value_step];
+    }
+  }
+};
+
 // ---------------------------------------------------------------------------
 // Lists of class-major rows in slices: the thread that has a listed class knows its
 // score, another one its entry.  They meet in LDS: a byte for each slot of each
