@@ -265,29 +265,44 @@ __global__ __launch_bounds__(F::kMax) void alternatives_candidates_kernel(Scores
   f.trim(v);
   // the chunks' maxima: a candidate is looked for in a chunk that has one
   float top[F::NC];
-  float m = -__builtin_inff(), half = m;
+  float m = -__builtin_inff();
 #pragma unroll
   for (int c = 0; c < F::NC; ++c) {
     top[c] = F::value(v, c * VE);
 #pragma unroll
-    for (int e = 1; e < VE; ++e) {
-      top[c] = fmaxf(top[c], F::value(v, c * VE + e));
-      if (F::NC == 1 && e == VE / 2 - 1) half = top[0];
-    }
+    for (int e = 1; e < VE; ++e) top[c] = fmaxf(top[c], F::value(v, c * VE + e));
     m = fmaxf(m, top[c]);
-    if (F::NC > 1 && c == F::NC / 2 - 1) half = m;
   }
   const float own = m;
   float from = 0.0f;
   if constexpr (NW == 1) {
     if (g.k > 0) {
-      // 128 parts: the halves of a lane's classes (the second one's maximum is m, or
-      // another one that is no larger)
-      float other = -__builtin_inff();
+      // two parts a lane, the halves of its classes; eight (four in float32 rows of a chunk
+      // a lane) for lists of more than half of the lanes that have classes, or nearly all
+      // parts would be in the list and most classes candidates.  64 alternatives of 20047
+      // x 257 float16 30 us, 67 with two parts; of 30000 x 3001 bfloat16 79 and 90; but of
+      // 30000 x 1000 55 and 52, and 20 of 20047 x 257 19 and 18.
+      constexpr int P = F::N < 8 ? F::N : 8;
+      uint32_t key[P];
 #pragma unroll
-      for (int j = F::N / 2; j < F::N; ++j) other = fmaxf(other, F::value(v, j));
-      const uint32_t key[2] = {order_of(half), order_of(other)};
-      from = kth_at_least<2>(key, g.k);
+      for (int p = 0; p < P; ++p) {
+        float x = F::value(v, p * F::N / P);
+#pragma unroll
+        for (int j = p * F::N / P + 1; j < (p + 1) * F::N / P; ++j) x = fmaxf(x, F::value(v, j));
+        key[p] = order_of(x);
+      }
+      const int32_t lanes = (s.K + VE - 1) / VE;
+      if (2 * g.k > (lanes < 64 ? lanes : 64)) {
+        from = kth_at_least<P>(key, g.k);
+      } else {
+        uint32_t two[2] = {key[0], key[P / 2]};
+#pragma unroll
+        for (int p = 1; p < P / 2; ++p) {
+          two[0] = key[p] > two[0] ? key[p] : two[0];
+          two[1] = key[P / 2 + p] > two[1] ? key[P / 2 + p] : two[1];
+        }
+        from = kth_at_least<2>(two, g.k);
+      }
     }
   } else {
     // 256 parts: a thread's classes, or those of four threads
