@@ -69,7 +69,8 @@ def check_alternatives(r, want, k, label=True):
     fin = w > -INF
     assert (r.log_prob.cpu()[~fin] == -INF).all()
     tol = t_lse[:, None] + U * 4 * w.abs()
-    check(torch.where(fin, r.log_prob.cpu().to(F64), 0.0), torch.where(fin, w, 0.0), tol + 1e-300,
+    # (numbers below the smallest normal one of float32 may be 0)
+    check(torch.where(fin, r.log_prob.cpu().to(F64), 0.0), torch.where(fin, w, 0.0), tol + 1e-37,
           "log_prob")
     check(r.entropy, want["entropy"], t_lse + t_down + U * want["entropy"] + 1e-37, "entropy")
     if label:
@@ -888,3 +889,147 @@ def test_refusals_on_the_gpu(gpu):
     no("log_norm", lambda: losses.distill_loss(s, c, x, log_norm=INF))
     no("with_grad", lambda: losses.distill_loss(s, c, x, grad=torch.zeros_like(s), with_grad=False))
     no("temperature", lambda: losses.distill_loss(s, c, x, temperature=0))
+
+
+# --------------------------------------------------------------------- edges of frames
+def run_all(s, k, dtype, tau, seed):
+    """Every operator on s with lists of k, against the float64 forms."""
+    from warpgbm_amd import losses
+
+    n, K = s.shape
+    g = torch.Generator().manual_seed(seed)
+    a = torch.randint(0, K, (n,), generator=g, dtype=torch.int32)
+    w = 0.5 + torch.rand(n, generator=g)
+    sd = to_gpu(s)
+    f = losses.class_alternatives(sd, min(k, K), labels=a.cuda(), temperature=tau)
+    check_alternatives(f, alternatives64(s, a, min(k, K), tau), min(k, K))
+    cls, logits, ln = lists_for(s, k, seed, tau, spare=False)
+    for norms in (None, ln):
+        got = losses.distill_loss(sd, cls.cuda(), logits.cuda(), weight=w.cuda(), temperature=tau,
+                                  log_norm=None if norms is None else norms.cuda())
+        check_distill(got, distill64(s, cls, logits, norms, w, tau), w, tau, dtype)
+    up = torch.randn((n, k), generator=g)
+    ge = torch.randn(n, generator=g)
+    got = losses.class_alternatives_grad(
+        sd, f.norm, labels=a.cuda(), grad_label_log_prob=w.cuda(), classes=cls.cuda(),
+        grad_log_prob=up.cuda(), grad_entropy=ge.cuda(), temperature=tau)
+    grad, tol = alternatives_grad64(s, a, w, cls, up, ge, tau)
+    check(got, grad, round_tol(tol, grad, dtype), "gradient")
+
+
+CLASS_EDGES = [4, 5, 8, 9, 12, 13, 16, 17, 32, 33, 40, 41, 52, 53, 64, 65, 80, 81, 104, 105, 128,
+               129, 160, 208, 209, 256, 257, 312, 313, 432, 433, 500, 512, 513]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", list(DTYPES))
+def test_edges_of_class_major_frames(gpu, dtype):
+    for K in CLASS_EDGES:
+        for n, k in ((67, 64), (130, 7)):
+            print_case("class edges", dtype, n, K, k)
+            run_all(make_scores(n, K, dtype, "class", K, masked=0.1), k, dtype, 1.0, K + k)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", list(DTYPES))
+def test_edges_of_row_major_frames(gpu, dtype):
+    """One class less and more than what a number of 16-byte chunks holds, up to rows that
+    go in tiles."""
+    VE = 4 if dtype == "f32" else 8
+    for chunks in (1, 2, 3, 4, 8, 16, 32, 64, 128, 256, 512, 1024, 2048, 4096, 8192, 16384):
+        for K in (chunks * VE - 1, chunks * VE, chunks * VE + 1):
+            n, k = (35, 17) if chunks <= 512 else (3, 64 if K % 2 else 5)
+            print_case("row edges", dtype, n, K, k)
+            run_all(make_scores(n, K, dtype, "row+" if K % 2 else "row", K, masked=0.1), k, dtype,
+                    2.0, K + k)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", list(DTYPES))
+def test_many_short_rows(gpu, dtype):
+    """Rows enough for fewer threads each, a part of a workgroup left over."""
+    for K, chunks in ((30, 8), (60, 16), (100, 32), (13, 4), (6, 2)):
+        if dtype != "f32" and K > 8:
+            K *= 2
+        n = (1 << 19) // chunks + 37
+        print_case("many", dtype, n, K)
+        run_all(make_scores(n, K, dtype, "row", K), 5, dtype, 1.0, K)
+
+
+@pytest.mark.gpu
+def test_lists_past_32_bits(gpu):
+    """The first and last rows of matrices of more than 2^31 elements against the same
+    rows alone."""
+    from warpgbm_amd import losses
+
+    for n, K, k in ((66_000, 33_000, 9), (2_200_000, 1000, 5)):
+        print_case("past 32 bits", n, K)
+        s = torch.empty((n, K), dtype=torch.bfloat16, device="cuda")
+        s.normal_(generator=torch.Generator(device="cuda").manual_seed(1))
+        rows = torch.cat([torch.arange(3), torch.arange(n - 5, n)]).cuda()
+        a = torch.arange(n, dtype=torch.int32, device="cuda") % K
+        f = losses.class_alternatives(s, k, labels=a, temperature=1.5)
+        r = losses.distill_loss(s, f.classes, f.log_prob, log_norm=0.125)
+        few = s[rows].contiguous()
+        F = losses.class_alternatives(few, k, labels=a[rows].contiguous(), temperature=1.5)
+        R = losses.distill_loss(few, F.classes, F.log_prob, log_norm=0.125)
+        up = torch.ones(n, device="cuda")
+        G = losses.class_alternatives_grad(few, F.norm, grad_entropy=up[:8], classes=F.classes,
+                                           grad_log_prob=F.log_prob, temperature=1.5)
+        for x, y in ((f.classes, F.classes), (f.log_prob, F.log_prob), (f.norm, F.norm),
+                     (f.label_log_prob, F.label_log_prob), (r.loss, R.loss), (r.grad, R.grad)):
+            assert torch.equal(x[rows], y)
+        del r
+        g = losses.class_alternatives_grad(s, f.norm, grad_entropy=up, classes=f.classes,
+                                           grad_log_prob=f.log_prob, temperature=1.5)
+        assert torch.equal(g[rows], G)
+        del s, g, f
+        torch.cuda.empty_cache()
+
+
+@pytest.mark.gpu
+def test_temperatures_at_their_limits(gpu):
+    from warpgbm_amd import losses
+
+    for order in ("row", "class"):
+        for K in (6, 60, 700):
+            s = make_scores(20, K, "f32", order, 4)
+            a = torch.zeros(20, dtype=torch.int32)
+            for tau in (1e-6, 1e-3, 1e3, 1e6):
+                print_case("temperature", order, K, tau)
+                r = losses.class_alternatives(to_gpu(s), 3, labels=a.cuda(), temperature=tau)
+                # (tau in float32)
+                t = float(torch.tensor(tau, dtype=torch.float32))
+                check_alternatives(r, alternatives64(s, a, 3, t), 3)
+                d = losses.distill_loss(to_gpu(s), r.classes, r.log_prob.clamp(min=-1e30) * tau,
+                                        log_norm=0.0, temperature=tau)
+                assert torch.isfinite(d.loss).all() and torch.isfinite(d.grad).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("order", ["row", "class"])
+def test_a_rest_next_to_its_border(gpu, order):
+    """Whether the teacher's rest is one (2^-20 or more) is decided as in float64."""
+    from warpgbm_amd import losses
+
+    for K, k in ((6, 5), (40, 12), (300, 20), (9000, 64)):
+        print_case("border", order, K, k)
+        n = 400
+        g = torch.Generator().manual_seed(K)
+        s = torch.randn((n, K), generator=g)
+        cls = torch.argsort(torch.rand((n, K), generator=g), 1)[:, :k].to(torch.int32).contiguous()
+        t = torch.log_softmax(torch.randn((n, k), generator=g, dtype=F64), 1)
+        # rests from 0.9 to 1.1 times the border
+        rest = 2.0 ** -20 * torch.linspace(0.9, 1.1, n, dtype=F64)
+        logits = (t + torch.log1p(-rest)[:, None]).float()
+        w = torch.ones(n)
+        left = 1 - logits.to(F64).exp().sum(1)
+        # (the sum's own rounding in float64)
+        assert ((left - 2.0 ** -20).abs() > 1e-13).all()
+        want = distill64(place(s, order), cls, logits, 0.0, w, 1.0)
+        got = losses.distill_loss(to_gpu(place(s, order)), cls.cuda(), logits.cuda(), log_norm=0.0)
+        check_distill(got, want, w, 1.0, "f32")
+        # the others' share of the gradient: P of them without a rest, P - Q with one
+        others = torch.ones((n, K), dtype=torch.bool).scatter_(1, cls.long(), False)
+        share = torch.where(others, got.grad.cpu().to(F64), 0.0).sum(1)
+        assert ((share - (want["P"] - want["Q"])).abs() <= U * (STEPS + 64) * want["P"] + 2e-8).all()

@@ -61,8 +61,23 @@ __device__ __forceinline__ float power_of(float v, float from, const DistillRows
   return exp2_f32((v - from) * g.scale);
 }
 
+// e^x in float64 for x up to some 1, to some 10^-14: x = n ln 2 + r, and e^r - 1 from the
+// first terms of its series at r / 1024, doubled ten times, q -> q (q + 2).  (Seldom
+// called; a longer series' coefficients would take the registers of a wave in five.)
+__device__ __forceinline__ double exp_wide(double x) {
+  const double n = rint(x * 1.44269504088896340736);
+  const double r = fma(n, -0.693147180559945286227, x) * 0x1p-10;
+  double q = fma(fma(fma(r, 1.0 / 24.0, 1.0 / 6.0), r, 0.5), r * r, r);
+#pragma unroll 1
+  for (int d = 0; d < 10; ++d) q = fma(q, q, q + q);
+  return x < -700.0 ? 0.0 : ldexp(1.0 + q, (int)n);
+}
+
+// logit(j): the logits of the row's entries j < k (-infinity: not used)
+template <typename Logit>
 __device__ __forceinline__ DistillRow distill_row(const DistillSums& a, const DistillRows& g,
-                                                  int64_t i, float m, float mr, float lm, float w) {
+                                                  int64_t i, float m, float mr, float lm, float w,
+                                                  int k, Logit logit) {
   DistillRow o{};
   o.m = safe_max(m);
   o.lm = safe_max(lm);
@@ -88,7 +103,15 @@ __device__ __forceinline__ DistillRow distill_row(const DistillSums& a, const Di
   } else {
     const float top = (float)((double)lm * g.inv_tau - norm);  // its logarithm
     const float one = counts ? exp_of(top) : 0.0f, C = counts ? more * one : 0.0f;
-    const float left = counts ? one_less_exp(top) - C - a.out : 1.0f - a.out;
+    float left = counts ? one_less_exp(top) - C - a.out : 1.0f - a.out;
+    // next to the border whether a rest is one is decided in float64 (the roundings above
+    // come to less than 100 * 2^-24)
+    if (has_rest && fabsf(left - kLeastRest) < 1e-5f) {
+      double sum = 0.0;
+#pragma unroll 1
+      for (int j = 0; j < k; ++j) sum += exp_wide((double)logit(j) * g.inv_tau - norm);
+      left = (float)(1.0 - sum);
+    }
     const bool rest = left >= kLeastRest && has_rest;
     Q = rest ? left : 0.0f;
     // what is left out of sum 1
@@ -195,7 +218,9 @@ __global__ __launch_bounds__(F::kMax) void distill_lane_kernel(ScoresView s, Dis
     a.q += l == lm ? 0.0f : el;
     a.q_ties += l == lm ? 1.0f : 0.0f;
   }
-  const DistillRow r = distill_row(a, g, i, m, mr, lm, w);
+  const DistillRow r = distill_row(a, g, i, m, mr, lm, w, N, [&](int j) {
+    return listed >> j & 1 ? logit[j][t] : -__builtin_inff();
+  });
   float loss = r.rest_term;
   for (uint32_t left = listed; left; left &= left - 1) {
     const int c = __ffs(left) - 1;
@@ -217,11 +242,11 @@ __global__ __launch_bounds__(F::kMax) void distill_lane_kernel(ScoresView s, Dis
 }
 
 // a listed class's part of the sums x[1] .. x[5]
-__device__ __forceinline__ void add_entry(const DistillRows& g, double norm, bool used, float sc,
-                                          float l, float m, float ms, float lm, float lms,
+__device__ __forceinline__ void add_entry(const DistillRows& g, double norm, float sc, float l,
+                                          float m, float ms, float lm, float lms,
                                           float (&x)[6]) {
   if (closed(sc)) {
-    if (g.rest && used) x[5] += exp_of((float)((double)l * g.inv_tau - norm));
+    if (g.rest) x[5] += exp_of((float)((double)l * g.inv_tau - norm));
     return;
   }
   const float es = power_of(sc, ms, g), el = power_of(l, lms, g);
@@ -268,29 +293,30 @@ __global__ __launch_bounds__(F::kMax) void distill_slices_kernel(ScoresView s, D
   f.load(v, s, blockIdx.x);
   map.clear();
   __syncthreads();
-  uint32_t used = 0;  // a bit for each of this thread's entries j = f.w, f.w + f.S, ...
+  // (entries that are not used have score and logit -infinity)
   bool twice = false;
-  for (int first = f.w, n = 0; first < k; first += Batch::kSize * f.S) {
-    if (n) b.load(classes, g.class_step, logits, g.logit_step, first, f.S, k);
+  for (int first = f.w; first < k; first += Batch::kSize * f.S) {
+    if (first != f.w) b.load(classes, g.class_step, logits, g.logit_step, first, f.S, k);
 #pragma unroll
-    for (int q = 0; q < Batch::kSize; ++q, ++n) {
+    for (int q = 0; q < Batch::kSize; ++q) {
       const int j = first + q * f.S;
       if (j >= k) break;
-      logit[64 * j] = b.value[q];
+      const bool used = w != 0.0f && (uint32_t)b.cls[q] < (uint32_t)s.K;
+      logit[64 * j] = used ? b.value[q] : -__builtin_inff();
       score[64 * j] = -__builtin_inff();
-      if (w != 0.0f && (uint32_t)b.cls[q] < (uint32_t)s.K) {
-        used |= 1u << n;
-        twice |= map.put(f, b.cls[q], j);
-      }
+      if (used) twice |= map.put(f, b.cls[q], j);
     }
   }
   if (__syncthreads_or(twice)) {
     // the first of the entries that name a class takes its place
-    for (int j = f.w, n = 0; j < k; j += f.S, ++n) {
+    for (int j = f.w; j < k; j += f.S) {
       const int32_t c = classes[j * g.class_step];
-      for (int o = 0; o < j; ++o)
-        if (classes[o * g.class_step] == c) used &= ~(1u << n);
-      if (used >> n & 1) map.set(f, c, j);
+      bool first = w != 0.0f && (uint32_t)c < (uint32_t)s.K;
+      for (int o = 0; o < j; ++o) first &= classes[o * g.class_step] != c;
+      if (first)
+        map.set(f, c, j);
+      else
+        logit[64 * j] = -__builtin_inff();
     }
     __syncthreads();
   }
@@ -322,8 +348,8 @@ __global__ __launch_bounds__(F::kMax) void distill_slices_kernel(ScoresView s, D
   for (int j = 0; j < F::N; ++j) z[j % 2] += power_of(F::value(v, j), mrs, g);
   float y[6] = {z[0] + z[1], 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
   const double norm = row_norm(g, i);
-  for (int j = f.w, n = 0; j < k; j += f.S, ++n)
-    add_entry(g, norm, used >> n & 1, score[64 * j], logit[64 * j], m, ms, lm, lms, y);
+  for (int j = f.w; j < k; j += f.S)
+    add_entry(g, norm, score[64 * j], logit[64 * j], m, ms, lm, lms, y);
   f.put_all(y, AddF(), buf + 3 * blockDim.x);
   __syncthreads();
   // what follows from the row as a whole costs as much as some 20 classes: the first wave
@@ -331,7 +357,8 @@ __global__ __launch_bounds__(F::kMax) void distill_slices_kernel(ScoresView s, D
   DistillRow r;
   if (f.w == 0) {
     f.join_all(y, AddF(), buf + 3 * blockDim.x);
-    r = distill_row(DistillSums{y[0], y[1], y[2], y[3], y[4], y[5]}, g, i, m, mr, lm, w);
+    r = distill_row(DistillSums{y[0], y[1], y[2], y[3], y[4], y[5]}, g, i, m, mr, lm, w, k,
+                    [&](int j) { return logit[64 * j]; });
     share[lane] = r;
   }
   __syncthreads();
@@ -382,7 +409,7 @@ __device__ __forceinline__ ListTable list_table(uint32_t* lds, int k) {
   return t;
 }
 
-// entries that are not used have class -1 and score -infinity
+// entries that are not used have class -1, and logit and score -infinity
 
 // entries that name a class again no longer count
 template <typename F>
@@ -398,7 +425,7 @@ __device__ __forceinline__ void drop_repeated(const F& f, const ListTable& t, in
   for (int j = f.entry(); j < k; j += f.entry_step(), ++n)
     if (again >> n & 1) {
       t.cls[f.entry_at(j, k)] = -1;
-      t.score[f.entry_at(j, k)] = -__builtin_inff();
+      t.logit[f.entry_at(j, k)] = t.score[f.entry_at(j, k)] = -__builtin_inff();
     }
 }
 
@@ -423,7 +450,7 @@ __device__ __forceinline__ void list_sums(const F& f, const ListTable& t, const 
   x[1] = x[2] = x[3] = x[4] = x[5] = 0.0f;
   for (int j = f.entry(); j < k; j += f.entry_step()) {
     const int at = f.entry_at(j, k);
-    add_entry(g, norm, t.cls[at] >= 0, t.score[at], t.logit[at], m, ms, lm, lms, x);
+    add_entry(g, norm, t.score[at], t.logit[at], m, ms, lm, lms, x);
   }
 }
 
@@ -462,7 +489,7 @@ __global__ __launch_bounds__(F::kMax) void distill_frame_kernel(ScoresView s, Di
     }
     const int at = f.entry_at(j, k);
     tab.cls[at] = c;
-    tab.logit[at] = l;
+    tab.logit[at] = c >= 0 ? l : -__builtin_inff();
     tab.score[at] = sc;
   }
   if (__syncthreads_or(twice)) drop_repeated(f, tab, k);
@@ -495,7 +522,8 @@ __global__ __launch_bounds__(F::kMax) void distill_frame_kernel(ScoresView s, Di
   DistillRow r;
   if (owner) {
     f.join_all(y, AddF(), tab.buf);
-    r = distill_row(DistillSums{y[0], y[1], y[2], y[3], y[4], y[5]}, g, i, m, mr, lm, w);
+    r = distill_row(DistillSums{y[0], y[1], y[2], y[3], y[4], y[5]}, g, i, m, mr, lm, w, k,
+                    [&](int j) { return tab.logit[f.entry_at(j, k)]; });
     if (F::kBarrier && threadIdx.x == 0) share = r;
   }
   if (F::kBarrier) {
@@ -554,7 +582,8 @@ __global__ __launch_bounds__(1024) void distill_long_kernel(ScoresView s, Distil
     int32_t c = w != 0.0f ? g.classes[i * g.class_stride + j * g.class_step] : -1;
     if (c < 0 || c >= s.K) c = -1;
     tab.cls[j] = c;
-    tab.logit[j] = c >= 0 ? g.logits[i * g.logit_stride + j * g.logit_step] : 0.0f;
+    tab.logit[j] =
+        c >= 0 ? g.logits[i * g.logit_stride + j * g.logit_step] : -__builtin_inff();
     tab.score[j] = c >= 0 ? score_at<T>(s, i, c) : -__builtin_inff();
   }
   __syncthreads();
@@ -611,7 +640,9 @@ __global__ __launch_bounds__(1024) void distill_long_kernel(ScoresView s, Distil
   list_sums(whole, tab, g, i, m, lm, y);
   __syncthreads();
   whole.reduce_all(y, AddF(), buf);
-  const DistillRow r = distill_row(DistillSums{y[0], y[1], y[2], y[3], y[4], y[5]}, g, i, m, mr, lm, w);
+  const DistillRow r =
+      distill_row(DistillSums{y[0], y[1], y[2], y[3], y[4], y[5]}, g, i, m, mr, lm, w, k,
+                  [&](int j) { return tab.logit[j]; });
   if (out.data && (r.live || !accumulate)) {
     for (int32_t t = 0; t < tiles; ++t) {
       const ScoresView p = tile_of(s, span, t), o = tile_of(out, span, t);

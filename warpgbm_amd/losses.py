@@ -26,6 +26,7 @@ from __future__ import annotations
 
 import ctypes as C
 import functools
+import operator
 from collections import namedtuple
 
 import numpy as np
@@ -387,8 +388,10 @@ def class_alternatives(scores, top_k, *, labels=None, temperature=1.0) -> ClassA
     top_k: 0 (no alternatives) to min(64, K)."""
     v = _matrix(scores, "scores")
     (n, K), dev = scores.shape, scores.device
-    if isinstance(top_k, bool) or not isinstance(top_k, int) or not 0 <= top_k <= min(MAX_LIST, K):
+    if isinstance(top_k, bool) or not hasattr(top_k, "__index__") or (
+            not 0 <= top_k <= min(MAX_LIST, K)):
         raise RuntimeError(f"top_k must be an integer in [0, min({MAX_LIST}, n_classes)], got {top_k}")
+    top_k = operator.index(top_k)
     tau = _temperature(temperature)
     lab = _vector(labels, "labels", torch.int32, n, dev) if labels is not None else None
     f32 = torch.float32
