@@ -1033,3 +1033,30 @@ def test_a_rest_next_to_its_border(gpu, order):
         others = torch.ones((n, K), dtype=torch.bool).scatter_(1, cls.long(), False)
         share = torch.where(others, got.grad.cpu().to(F64), 0.0).sum(1)
         assert ((share - (want["P"] - want["Q"])).abs() <= U * (STEPS + 64) * want["P"] + 2e-8).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("order", ["row", "class"])
+def test_distill_of_a_small_listed_share(gpu, order):
+    """A softened teacher whose list is a small part of it: the others' gradient is a
+    difference of shares next to 1, which the listed shares' digits give."""
+    from warpgbm_amd import losses
+
+    for n, K in ((40, 400), (12, 3000), (5, 30_000)):
+        print_case("small share", order, n, K)
+        g = torch.Generator().manual_seed(K)
+        s = place(torch.randn((n, K), generator=g), order)
+        t = 0.8 * s + 0.5 * torch.randn((n, K), generator=g)
+        logits, cls = (x[:, :2].contiguous() for x in torch.sort(t, dim=1, descending=True))
+        cls = cls.to(torch.int32)
+        ln = torch.logsumexp(t.double() / 4.0, 1).float()
+        got = losses.distill_loss(to_gpu(s), cls.cuda(), logits.cuda(), log_norm=ln.cuda(),
+                                  temperature=4.0)
+        want = distill64(s, cls, logits, ln, torch.ones(n), 4.0)
+        check_distill(got, want, torch.ones(n), 4.0, "f32")
+        # listed: p_k and q_k of a few roundings each (and log norm's, which all share);
+        # others: (listed q - listed p) r_k, the same
+        p, q, r = want["p"], want["q"], want["r"]
+        small = (torch.where(q > 0, p, 0.0).sum(1, keepdim=True) + q.sum(1, keepdim=True))
+        tol = 4.0 * U * (STEPS + 128) * torch.where(q > 0, p + q, small * r)
+        check(got.grad, want["grad"], tol + U * want["grad"].abs(), "gradient")

@@ -95,14 +95,15 @@ __device__ __forceinline__ DistillRow distill_row(const DistillSums& a, const Di
   const bool counts = lm > -__builtin_inff() || a.q != a.q;
   const double norm = g.rest ? (double)(g.log_norm ? g.log_norm[i] : g.log_norm_all) : 0.0;
   const float more = a.q + (a.q_ties - 1.0f);  // relative to the largest
-  float Q = 0.0f;
-  double log_mass = 0.0, shift;  // log q = l / tau - shift
+  float Q = 0.0f, listed = 0.0f;  // shares of the others, of the list
+  double log_mass = 0.0, shift;   // log q = l / tau - shift
   if (!g.rest) {
     o.live = o.live && counts;
     shift = (double)o.lm * g.inv_tau + (counts ? log_1p(more) : 0.0);
   } else {
     const float top = (float)((double)lm * g.inv_tau - norm);  // its logarithm
     const float one = counts ? exp_of(top) : 0.0f, C = counts ? more * one : 0.0f;
+    listed = one + C + a.out;
     float left = counts ? one_less_exp(top) - C - a.out : 1.0f - a.out;
     // next to the border whether a rest is one is decided in float64 (the roundings above
     // come to less than 100 * 2^-24)
@@ -131,7 +132,8 @@ __device__ __forceinline__ DistillRow distill_row(const DistillSums& a, const Di
     const float P = exp_of((float)log_P);
     Bucket b{P, P};
     if (Q > 0.0f) {
-      const double log_Q = log_of(Q) - log_mass;
+      // (a small list: 1 - listed would round its digits away)
+      const double log_Q = (listed < 0.5f ? (double)log1p_of(-listed) : log_of(Q)) - log_mass;
       b = bucket(P, exp_of((float)log_Q), (float)(log_P - log_Q));
     }
     o.rest_term = b.term;
