@@ -1060,3 +1060,35 @@ def test_distill_of_a_small_listed_share(gpu, order):
         small = (torch.where(q > 0, p, 0.0).sum(1, keepdim=True) + q.sum(1, keepdim=True))
         tol = 4.0 * U * (STEPS + 128) * torch.where(q > 0, p + q, small * r)
         check(got.grad, want["grad"], tol + U * want["grad"].abs(), "gradient")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("order", ["row", "class"])
+def test_distill_where_the_teacher_s_best_class_is_closed(gpu, order):
+    """The row may not take the class that has almost all of the teacher's share: what is
+    left, scaled to sum 1, keeps its digits."""
+    from warpgbm_amd import losses
+
+    for n, K in ((64, 4), (64, 40), (16, 900)):
+        print_case("closed", order, n, K)
+        g = torch.Generator().manual_seed(K)
+        s = torch.randn((n, K), generator=g)
+        t = torch.randn((n, K), generator=g)
+        t[torch.arange(n), torch.arange(n) % K] += torch.linspace(2.0, 11.0, n)
+        best = torch.sort(t, dim=1, descending=True)
+        logits = best.values[:, :3].contiguous()
+        cls = best.indices[:, :3].to(torch.int32).contiguous()
+        s[torch.arange(n), cls[:, 0].long()] = -INF
+        ln = torch.logsumexp(t.double(), 1).float()
+        got = losses.distill_loss(to_gpu(place(s, order)), cls.cuda(), logits.cuda(),
+                                  log_norm=ln.cuda())
+        w = torch.ones(n)
+        want = distill64(place(s, order), cls, logits, ln, w, 1.0)
+        check_distill(got, want, w, 1.0, "f32")
+        # sums of what is left: a few roundings of each share, not of the closed one (log_norm's
+        # own rounding is an input)
+        gap = torch.where(want["q"] > 0, (want["q"].log() + want["far"]).abs(), 0.0)
+        far_rest = torch.where(want["Q"] > 0, (want["Q"].clamp(min=1e-30).log() - want["rest"]).abs(),
+                               0.0)
+        tol = U * (STEPS * want["lost"] + 24 * (2 + (want["q"] * gap).sum(1) + far_rest))
+        check(got.loss, want["loss"], tol + U * want["loss"], "loss")

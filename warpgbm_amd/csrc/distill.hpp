@@ -106,8 +106,9 @@ __device__ __forceinline__ DistillRow distill_row(const DistillSums& a, const Di
     listed = one + C + a.out;
     float left = counts ? one_less_exp(top) - C - a.out : 1.0f - a.out;
     // next to the border whether a rest is one is decided in float64 (the roundings above
-    // come to less than 100 * 2^-24)
-    if (has_rest && fabsf(left - kLeastRest) < 1e-5f) {
+    // come to less than 100 * 2^-24); so is what is left of a list that the row may
+    // mostly not take, whose roundings the scaling to sum 1 would enlarge
+    if (has_rest && (fabsf(left - kLeastRest) < 1e-5f || a.out > 0.5f)) {
       double sum = 0.0;
 #pragma unroll 1
       for (int j = 0; j < k; ++j) sum += exp_wide((double)logit(j) * g.inv_tau - norm);
