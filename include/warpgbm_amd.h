@@ -334,7 +334,7 @@ int wgbm_balance_loss(const wgbm_scores* scores, const uint8_t* mask, int32_t to
  * 0 and norm (-inf, 0, 0). */
 int64_t wgbm_class_alternatives_workspace(const wgbm_scores* scores);
 int wgbm_class_alternatives(const wgbm_scores* scores, const int32_t* labels, int32_t top_k,
-                            float temperature, int32_t* classes, float* log_prob, float* entropy,
+                            double temperature, int32_t* classes, float* log_prob, float* entropy,
                             float* label_log_prob, float* norm, void* workspace,
                             int64_t workspace_bytes, void* stream);
 
@@ -358,7 +358,7 @@ typedef struct wgbm_alternatives_grad_args {
   int64_t grad_step;
   int32_t list_length;                /* [0, WGBM_MAX_LIST] */
   const float* grad_entropy;          /* [n_rows] or NULL */
-  float temperature;
+  double temperature;
 } wgbm_alternatives_grad_args;
 int64_t wgbm_class_alternatives_grad_workspace(const wgbm_scores* scores);
 int wgbm_class_alternatives_grad(const wgbm_scores* scores,
@@ -392,7 +392,7 @@ typedef struct wgbm_distill_args {
   const float* log_norm;   /* [n_rows] or NULL */
   float log_norm_all;
   const float* weight;     /* [n_rows] or NULL */
-  float temperature;
+  double temperature;
 } wgbm_distill_args;
 int64_t wgbm_distill_loss_workspace(const wgbm_scores* scores);
 int wgbm_distill_loss(const wgbm_scores* scores, const wgbm_distill_args* args, float* loss,

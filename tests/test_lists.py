@@ -998,9 +998,7 @@ def test_temperatures_at_their_limits(gpu):
             for tau in (1e-6, 1e-3, 1e3, 1e6):
                 print_case("temperature", order, K, tau)
                 r = losses.class_alternatives(to_gpu(s), 3, labels=a.cuda(), temperature=tau)
-                # (tau in float32)
-                t = float(torch.tensor(tau, dtype=torch.float32))
-                check_alternatives(r, alternatives64(s, a, 3, t), 3)
+                check_alternatives(r, alternatives64(s, a, 3, tau), 3)
                 d = losses.distill_loss(to_gpu(s), r.classes, r.log_prob.clamp(min=-1e30) * tau,
                                         log_norm=0.0, temperature=tau)
                 assert torch.isfinite(d.loss).all() and torch.isfinite(d.grad).all()
@@ -1079,16 +1077,17 @@ def test_distill_where_the_teacher_s_best_class_is_closed(gpu, order):
         logits = best.values[:, :3].contiguous()
         cls = best.indices[:, :3].to(torch.int32).contiguous()
         s[torch.arange(n), cls[:, 0].long()] = -INF
-        ln = torch.logsumexp(t.double(), 1).float()
+        tau = 0.7  # (not a float32)
+        ln = torch.logsumexp(t.double() / tau, 1).float()
         got = losses.distill_loss(to_gpu(place(s, order)), cls.cuda(), logits.cuda(),
-                                  log_norm=ln.cuda())
+                                  log_norm=ln.cuda(), temperature=tau)
         w = torch.ones(n)
-        want = distill64(place(s, order), cls, logits, ln, w, 1.0)
-        check_distill(got, want, w, 1.0, "f32")
+        want = distill64(place(s, order), cls, logits, ln, w, tau)
+        check_distill(got, want, w, tau, "f32")
         # sums of what is left: a few roundings of each share, not of the closed one (log_norm's
         # own rounding is an input)
         gap = torch.where(want["q"] > 0, (want["q"].log() + want["far"]).abs(), 0.0)
         far_rest = torch.where(want["Q"] > 0, (want["Q"].clamp(min=1e-30).log() - want["rest"]).abs(),
                                0.0)
-        tol = U * (STEPS * want["lost"] + 24 * (2 + (want["q"] * gap).sum(1) + far_rest))
+        tol = tau * tau * U * (STEPS * want["lost"] + 24 * (2 + (want["q"] * gap).sum(1) + far_rest))
         check(got.loss, want["loss"], tol + U * want["loss"], "loss")

@@ -53,7 +53,7 @@ SIGNATURES = {
     "wgbm_balance_loss_workspace": (_i64, [_p]),
     "wgbm_balance_loss": (C.c_int, [_p, _p, _i32, _f32, _p, _p, _p, _p, _i32, _p, _i64, _p]),
     "wgbm_class_alternatives_workspace": (_i64, [_p]),
-    "wgbm_class_alternatives": (C.c_int, [_p, _p, _i32, _f32, _p, _p, _p, _p, _p, _p, _i64, _p]),
+    "wgbm_class_alternatives": (C.c_int, [_p, _p, _i32, C.c_double, _p, _p, _p, _p, _p, _p, _i64, _p]),
     "wgbm_class_alternatives_grad_workspace": (_i64, [_p]),
     "wgbm_class_alternatives_grad": (C.c_int, [_p, _p, _p, _i32, _p, _i64, _p]),
     "wgbm_distill_loss_workspace": (_i64, [_p]),
@@ -144,7 +144,7 @@ class AlternativesGradArgs(C.Structure):
         ("grad_step", _i64),
         ("list_length", _i32),
         ("grad_entropy", _p),
-        ("temperature", _f32),
+        ("temperature", C.c_double),
     ]
 
 
@@ -161,7 +161,7 @@ class DistillArgs(C.Structure):
         ("log_norm", _p),
         ("log_norm_all", _f32),
         ("weight", _p),
-        ("temperature", _f32),
+        ("temperature", C.c_double),
     ]
 
 

@@ -169,11 +169,11 @@ int wgbm_balance_loss(const wgbm_scores* scores, const uint8_t* mask, int32_t to
 }
 
 // log2(e) / tau and 1 / tau of a temperature
-static int tempered(float temperature, const char* what, float* scale, double* inv) {
-  WGBM_REQUIRE(temperature >= 1e-6f && temperature <= 1e6f,
+static int tempered(double temperature, const char* what, float* scale, double* inv) {
+  WGBM_REQUIRE(temperature >= 1e-6 && temperature <= 1e6,
                "%s: temperature must be in [1e-6, 1e6]", what);
-  *inv = 1.0 / (double)temperature;
-  *scale = (float)(1.44269504088896340736 / (double)temperature);
+  *inv = 1.0 / temperature;
+  *scale = (float)(1.44269504088896340736 / temperature);
   return 0;
 }
 static int list_length(int32_t k, int32_t least, const char* what) {
@@ -198,7 +198,7 @@ int64_t wgbm_class_alternatives_workspace(const wgbm_scores* scores) {
 }
 
 int wgbm_class_alternatives(const wgbm_scores* scores, const int32_t* labels, int32_t top_k,
-                            float temperature, int32_t* classes, float* log_prob, float* entropy,
+                            double temperature, int32_t* classes, float* log_prob, float* entropy,
                             float* label_log_prob, float* norm, void* workspace,
                             int64_t workspace_bytes, void* stream) {
   ScoresView s;
@@ -309,7 +309,7 @@ int wgbm_distill_loss(const wgbm_scores* scores, const wgbm_distill_args* a, flo
   g.log_norm = a->rest ? a->log_norm : nullptr;
   g.log_norm_all = a->log_norm_all;
   g.weight = a->weight;
-  g.tau = a->temperature;
+  g.tau = (float)a->temperature;
   g.loss = loss;
   return distill_loss(s, g, o, accumulate != 0, workspace, S(stream));
 }
