@@ -104,7 +104,7 @@ def _like(v, scores):
     if v.row_stride == 1 and v.class_stride != 1:
         t = torch.empty_strided((n, K), (1, max(n, 2)), dtype=scores.dtype, device=scores.device)
         return t, _lib.Scores(t.data_ptr(), v.dtype, n, K, 1, max(n, 2))
-    t = torch.empty((n, K), dtype=scores.dtype, device=scores.device)
+    t = torch.empty(n, K, dtype=scores.dtype, device=scores.device)
     return t, _lib.Scores(t.data_ptr(), v.dtype, n, K, K, 1)
 
 
@@ -397,10 +397,10 @@ def class_alternatives(scores, top_k, *, labels=None, temperature=1.0) -> ClassA
     f32 = torch.float32
     lib = _lib.load()
     with _on(dev):
-        classes = torch.empty((n, top_k), dtype=torch.int32, device=dev)
-        log_prob = torch.empty((n, top_k), dtype=f32, device=dev)
+        classes = torch.empty(n, top_k, dtype=torch.int32, device=dev)
+        log_prob = torch.empty(n, top_k, dtype=f32, device=dev)
         entropy = torch.empty(n, dtype=f32, device=dev)
-        norm = torch.empty((n, 3), dtype=f32, device=dev)
+        norm = torch.empty(n, 3, dtype=f32, device=dev)
         label = torch.empty(n, dtype=f32, device=dev) if labels is not None else None
         ws, at, size = _workspace("wgbm_class_alternatives_workspace", v, dev)
         rc = lib.wgbm_class_alternatives(
