@@ -6,6 +6,12 @@
 // log1p of the sum without the largest term, 1: nothing cancels, for a row sure
 // of its class as for an even one.  Rows are read once into registers
 // (losses_frames.hpp).
+//
+// 1M x 10 float32 class-major, three alternatives: 19 us (88 MB, 4.5 TB/s: memory).  8191
+// x 16001 bfloat16, 64 alternatives: 73 us (267 MB, 3.6 TB/s): vector instructions are
+// issued in four fifths of the cycles.  1 x 50001 float32: 9.3 us, one workgroup's
+// latency.  A turn a class is what long lists of class-major rows cost: 1M x 100 float32
+// 90 us without alternatives, 116 with three, 295 with 16.
 #pragma once
 #include "losses_lists.hpp"
 

@@ -1,7 +1,7 @@
 """Losses of class scores and of paired scores, with their gradients.
 
-What a boosting round of the objectives "policy", "preference" and
-"policy_preference" fits its trees to, as operators on GPU tensors: each call
+What a boosting round of the objectives "policy", "preference",
+"policy_preference" and "distill" fits its trees to, as operators on GPU tensors: each call
 returns the per-row (per-pair) losses and the gradient with respect to the
 scores, computed by the HIP library through the C ABI of
 ``include/warpgbm_amd.h``.  The reference has no counterpart (its losses are
