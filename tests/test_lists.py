@@ -1091,3 +1091,38 @@ def test_distill_where_the_teacher_s_best_class_is_closed(gpu, order):
                                0.0)
         tol = tau * tau * U * (STEPS * want["lost"] + 24 * (2 + (want["q"] * gap).sum(1) + far_rest))
         check(got.loss, want["loss"], tol + U * want["loss"], "loss")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,order,n", [("f16", "class", 2), ("f32", "row", 1)])
+def test_rows_of_the_most_classes(gpu, dtype, order, n):
+    """2^24 classes: rows in the most tiles, and their copy where they are class-major."""
+    K = 1 << 24
+    print_case("most classes", dtype, order, n, K)
+    run_all(make_scores(n, K, dtype, order, 77), 64, dtype, 1.0, 78)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("K,order", [(90, "class"), (700, "class"), (20_001, "row")])
+def test_two_streams_at_once(gpu, K, order):
+    """Steps that run beside each other have the bits of steps that run alone."""
+    n, k = 3000, 8
+    a = torch.randint(0, K, (n,), dtype=torch.int32).cuda()
+    w = torch.ones(n).cuda()
+    inputs = [[to_gpu(make_scores(n, K, "f32", order, 80 + 2 * j + i)) for i in range(2)]
+              for j in range(2)]
+    alone = [teach(s, t, a, w, k, 2.0, 0.5) for s, t in inputs]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in inputs]
+    got = [[], []]
+    for _ in range(5):
+        for j, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                got[j].append(teach(*inputs[j], a, w, k, 2.0, 0.5))
+    torch.cuda.synchronize()
+    for j in range(2):
+        f, r, e, g = alone[j]
+        for F, R, E, G in got[j]:
+            for x, y in ((f.classes, F.classes), (f.log_prob, F.log_prob), (r.loss, R.loss),
+                         (e.entropy, E.entropy), (g, G)):
+                assert torch.equal(x, y)

@@ -11,9 +11,10 @@ Scores are [n rows, K classes] in float32, bfloat16 or float16, with either the
 classes of a row next to each other (``scores`` contiguous, or rows with a
 stride) or the rows of a class (``scores_cm.t()`` of the engine's class-major
 [K, n]).  Per-row inputs are contiguous; lists [n, k] of a row's classes have
-either order too.  A score of -inf is a class that the row may not take; a row whose scores are all -inf counts as left out.  Rows
-left out (weight 0, mask false, label outside [0, K)) are not read: their
-results and gradients are 0, whatever their scores hold.
+either order too.  A score of -inf is a class that the row may not take; a row
+whose scores are all -inf counts as left out.  Rows left out (weight 0, mask
+false, label outside [0, K)) are not read: their results and gradients are 0,
+whatever their scores hold.
 
 Launches go on torch's current stream of the scores' device; nothing
 synchronises except the construction of a :class:`PreferencePlan`.  Outputs and
