@@ -160,8 +160,8 @@ static void pick_list_slices(const ScoresView& s, Fn fn) {
 // Whether a thread takes a whole row: class-major up to 16 classes, and row-major ones
 // up to 12 (a lane's loads are 48 bytes apart at most), which share what a row costs as
 // a whole with nobody.  1M x 10 row-major, a thread a row and four: best three classes
-// float32 23 and 39 us, bfloat16 21 and 48; distillation 50 and 66, 34 and 71; gradient 44
-// and 45, 30 and 50; but of 1M x 16 float32 38 and 36, 113 and 60, 97 and 42.
+// float32 20 and 35 us, bfloat16 20 and 47; distillation 48 and 66, 33 and 71; gradient 40
+// and 43, 25 and 46; but of 1M x 16 float32 38 and 36, 113 and 60, 97 and 42.
 static inline bool thread_rows(const ScoresView& s) {
   return s.K <= (s.class_major() ? 16 : 12);
 }
