@@ -323,6 +323,13 @@ int wgbm_balance_loss(const wgbm_scores* scores, const uint8_t* mask, int32_t to
  * stride is 1 (step >= n_rows).  Temperatures are in [1e-6, 1e6] and divide the scores. */
 #define WGBM_MAX_LIST 64
 
+/* The parts that the losses with lists cut a row of row-major scores into where registers
+ * do not hold it whole, wgbm_class_alternatives_grad (grad != 0) or the other two: their
+ * number, and in *span (or NULL) the classes of each but the last, which has 8 at least
+ * and span at most.  1 and n_classes where rows are whole, -1 for scores that the losses
+ * refuse.  No device call is made. */
+int32_t wgbm_lists_tiles(const wgbm_scores* scores, int32_t grad, int32_t* span);
+
 /* With p = softmax(scores[i] / temperature): the top_k classes of largest score, in
  * descending order, the lower class first among equal scores, with log p of each
  * (classes, log_prob [n_rows][top_k]; -1 and -inf where the row has fewer classes;

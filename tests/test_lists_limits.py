@@ -1,0 +1,88 @@
+"""Losses with lists of classes at lengths, scores and arguments next to their limits:
+tiles of very long rows."""
+import ctypes as C
+
+import pytest
+import torch
+
+from conftest import print_case
+from test_lists import alternatives_grad64, round_tol
+from test_losses import DTYPES, check, make_scores, to_gpu
+
+MOST = {False: {0: 16_384, 1: 32_768}, True: {0: 4096, 1: 8192}}  # classes of a tile
+
+
+def tiles_of(K, code, grad):
+    from warpgbm_amd import _lib
+
+    span = C.c_int32()
+    v = _lib.Scores(16, code, 1, K, K, 1)
+    return _lib.load().wgbm_lists_tiles(C.byref(v), int(grad), C.byref(span)), span.value
+
+
+# --------------------------------------------------------------------- tiles of long rows
+@pytest.mark.parametrize("grad", [False, True])
+@pytest.mark.parametrize("code", [0, 1, 2])
+def test_tiles_hold_a_chunk_and_fit_their_frame(code, grad):
+    """Every class in one tile, none longer than the frame, none shorter than 8 classes:
+    the lengths next to every multiple of a tile, and some between."""
+    most = MOST[grad][min(code, 1)]
+    whole = most if grad else 4 * most
+    g = torch.Generator().manual_seed(code)
+    lengths = torch.randint(13, (1 << 24) + 1, (20_000,), generator=g).tolist()
+    for step in (most, most - 8, most - 16):
+        for at in range(0, 1 << 24, step):
+            lengths += range(max(13, at - 1), at + 9)
+    for K in lengths:
+        if K > 1 << 24:
+            continue
+        tiles, span = tiles_of(K, code, grad)
+        if K <= whole:
+            assert (tiles, span) == (1, K)
+            continue
+        last = K - (tiles - 1) * span
+        assert span % 8 == 0 and 8 <= last <= span <= most, (K, tiles, span)
+
+
+def test_tiles_of_other_scores():
+    from warpgbm_amd import _lib
+
+    entry = _lib.load().wgbm_lists_tiles
+    assert entry(C.byref(_lib.Scores(16, 0, 4, 90_000, 1, 4)), 1, None) == 1  # class-major
+    assert entry(C.byref(_lib.Scores(16, 0, 4, 90_000, 90_000, 1)), 1, None) == 22
+    assert entry(C.byref(_lib.Scores(16, 5, 4, 90_000, 90_000, 1)), 1, None) == -1
+    assert entry(None, 0, None) == -1
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,order,n,K", [
+    ("f32", "row", 2, 2_093_057), ("f32", "row+", 2, 2_093_058), ("f32", "class", 2, 2_093_059),
+    ("bf16", "row", 1, 8_380_417), ("f16", "row+", 1, 8_380_423), ("bf16", "class", 2, 2_093_057)])
+def test_gradient_of_rows_that_leave_a_few_classes_over(gpu, dtype, order, n, K):
+    """Lengths a few classes over a multiple of the tile's, with the label and an entry
+    among these."""
+    from warpgbm_amd import losses
+
+    s = make_scores(n, K, dtype, order, 7)
+    g = torch.Generator().manual_seed(K)
+    a = torch.full((n,), K - 1, dtype=torch.int32)
+    cls = torch.randint(0, K, (n, 20), generator=g, dtype=torch.int32)
+    cls[:, 3], cls[:, 4], cls[:, 5] = K - 2, K - 9, 0
+    gl, ge = torch.randn(n, generator=g), torch.randn(n, generator=g)
+    gt = torch.randn((n, 20), generator=g)
+    old = make_scores(n, K, dtype, order, 8)
+    sd = to_gpu(s)
+    f = losses.class_alternatives(sd, 0)
+    for what in ("label", "list", "added"):
+        print_case("over", dtype, order, n, K, what)
+        lists = what != "label"
+        want, tol = alternatives_grad64(s, a, gl, cls if lists else None, gt, ge, 1.0)
+        kw = dict(classes=cls.cuda(), grad_log_prob=gt.cuda()) if lists else {}
+        if what == "added":
+            kw["grad"] = to_gpu(old)
+            want = want + old.double()
+        got = losses.class_alternatives_grad(sd, f.norm, labels=a.cuda(),
+                                             grad_label_log_prob=gl.cuda(),
+                                             grad_entropy=ge.cuda(), **kw)
+        assert got.dtype == DTYPES[dtype]
+        check(got, want, round_tol(tol, want, dtype), what)

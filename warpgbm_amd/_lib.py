@@ -52,6 +52,7 @@ SIGNATURES = {
     "wgbm_policy_loss": (C.c_int, [_p, _p, _p, _p, _p, _p, _i32, _p, _i64, _p]),
     "wgbm_balance_loss_workspace": (_i64, [_p]),
     "wgbm_balance_loss": (C.c_int, [_p, _p, _i32, _f32, _p, _p, _p, _p, _i32, _p, _i64, _p]),
+    "wgbm_lists_tiles": (_i32, [_p, _i32, C.POINTER(_i32)]),
     "wgbm_class_alternatives_workspace": (_i64, [_p]),
     "wgbm_class_alternatives": (C.c_int, [_p, _p, _i32, C.c_double, _p, _p, _p, _p, _p, _p, _i64, _p]),
     "wgbm_class_alternatives_grad_workspace": (_i64, [_p]),

@@ -514,8 +514,9 @@ static int alternatives_frames(const ScoresView& s, const AltRows& g, hipStream_
   } else if (chunks <= 16384) {
     candidates(FrameTag<RowFrame<T, 1024, 16>>());
   } else {
-    int32_t span, tiles;
-    cut_tiles(s.K, AltTile<T>::N * 1024, &span, &tiles);
+    static_assert(AltTile<T>::N * 1024 == kTileChunks * VE, "a tile");
+    int32_t span;
+    const int32_t tiles = row_tiles(s, false, &span);
     hipLaunchKernelGGL((alternatives_long_kernel<T>), dim3((unsigned)s.n), dim3(1024), 0, st, s, g,
                        span, tiles);
   }

@@ -389,13 +389,14 @@ static int alternatives_grad_frames(const ScoresView& s, const AltGradRows& g,
   };
   // (nothing is summed over a row: long rows go in parts)
   using Tile = RowFrame<T, 256, 4>;
-  if (s.class_major() || s.K <= Tile::N * 256) {
+  static_assert(Tile::N * 256 == kGradTileChunks * Chunk<T>::VE, "a tile");
+  int32_t span;
+  const int32_t tiles = row_tiles(s, true, &span);
+  if (tiles == 1) {
     pick_short_frame<T>(s, [&](auto tag, int64_t blocks, int threads) {
       launch(tag, blocks, threads, 0, 1);
     });
   } else {
-    int32_t span, tiles;
-    cut_tiles(s.K, Tile::N * 256, &span, &tiles);
     launch(FrameTag<Tile>(), s.n, 256, span, tiles);
   }
   WGBM_LAUNCH_CHECK();

@@ -191,6 +191,13 @@ static int list_strides(int64_t stride, int64_t step, int64_t n, int32_t k, cons
   return 0;
 }
 
+int32_t wgbm_lists_tiles(const wgbm_scores* scores, int32_t grad, int32_t* span) {
+  ScoresView s;
+  int32_t most;
+  if (view_of(scores, "scores", &s)) return -1;
+  return row_tiles(s, grad != 0, span ? span : &most);
+}
+
 int64_t wgbm_class_alternatives_workspace(const wgbm_scores* scores) {
   ScoresView s;
   if (view_of(scores, "scores", &s)) return -1;

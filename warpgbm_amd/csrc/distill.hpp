@@ -694,8 +694,9 @@ static int distill_frames(const ScoresView& s, const DistillRows& g, const Score
                           bool accumulate, hipStream_t st) {
   if (!rows_fit(s, false)) {
     using F = RowFrame<T, 1024, 4>;
-    int32_t span, tiles;
-    cut_tiles(s.K, F::N * 1024, &span, &tiles);
+    static_assert(F::N * 1024 == kTileChunks * F::VE, "a tile");
+    int32_t span;
+    const int32_t tiles = row_tiles(s, false, &span);
     hipLaunchKernelGGL((distill_long_kernel<T>), dim3((unsigned)s.n), dim3(1024),
                        (size_t)g.k * 12 + 1024 * 4, st, s, g, out, accumulate, span, tiles);
     WGBM_LAUNCH_CHECK();

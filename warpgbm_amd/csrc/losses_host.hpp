@@ -114,12 +114,25 @@ int class_alternatives_grad(const ScoresView& s, const AltGradRows& g, const Sco
                             bool accumulate, void* ws, hipStream_t st);
 int distill_loss(const ScoresView& s, const DistillRows& g, const ScoresView& out, bool accumulate,
                  void* ws, hipStream_t st);
-// a row of more classes than registers hold in tiles of at most `most` classes, at
-// least 8 each, of whole chunks
-inline void cut_tiles(int32_t K, int32_t most, int32_t* span, int32_t* tiles) {
+// Rows of more 16-byte chunks than this are cut in tiles of chunks: of the gradient of
+// alternatives, which sums nothing over a row, and of the other two.
+constexpr int32_t kGradTileChunks = 1024, kWholeChunks = 16384, kTileChunks = 4096;
+// Tiles of a row of K classes, of `span` classes each but the last, at most `most`: as
+// even as whole chunks allow.  The last one holds 8 classes at least (a frame reads a
+// row's end by a whole chunk): where fewer would be left over, shorter tiles leave more
+// to it.
+inline int32_t cut_tiles(int32_t K, int32_t most, int32_t* span) {
   const int32_t n = (K + most - 1) / most;
   *span = ((K + n - 1) / n + 7) / 8 * 8;
-  *tiles = (K + *span - 1) / *span;
+  while (K % *span != 0 && K % *span < 8) *span -= 8;
+  return (K + *span - 1) / *span;
+}
+// the same for scores (1 tile: whole rows)
+inline int32_t row_tiles(const ScoresView& s, bool grad, int32_t* span) {
+  const int32_t VE = s.dtype == kF32 ? 4 : 8;
+  *span = s.K;
+  if (s.class_major() || (s.K + VE - 1) / VE <= (grad ? kGradTileChunks : kWholeChunks)) return 1;
+  return cut_tiles(s.K, (grad ? kGradTileChunks : kTileChunks) * VE, span);
 }
 
 // A grid's threads are counted in 32 bits: rows in registers are launched in
