@@ -1,6 +1,7 @@
 """Losses with lists of classes at lengths, scores and arguments next to their limits:
-tiles of very long rows."""
+tiles of very long rows, NaN among scores."""
 import ctypes as C
+import math
 
 import pytest
 import torch
@@ -9,6 +10,7 @@ from conftest import print_case
 from test_lists import alternatives_grad64, round_tol
 from test_losses import DTYPES, check, make_scores, to_gpu
 
+INF = math.inf
 MOST = {False: {0: 16_384, 1: 32_768}, True: {0: 4096, 1: 8192}}  # classes of a tile
 
 
@@ -86,3 +88,61 @@ def test_gradient_of_rows_that_leave_a_few_classes_over(gpu, dtype, order, n, K)
                                              grad_entropy=ge.cuda(), **kw)
         assert got.dtype == DTYPES[dtype]
         check(got, want, round_tol(tol, want, dtype), what)
+
+
+# --------------------------------------------------------------------- NaN among scores
+def rows_with_nan(K, dtype, order, seed):
+    """Rows with one NaN, one of either sign first and last, a run of them, every other
+    class, all but one, all; with classes that the row may not take; among equal scores."""
+    g = torch.Generator().manual_seed(seed)
+    s = torch.randn((13, K), generator=g)
+    nan = float("nan")
+    s[0, K // 2] = nan
+    s[1, 0], s[1, K - 1] = nan, -nan
+    s[2, K // 3:K // 3 + 40] = nan
+    s[3, ::2] = nan
+    one = s[4, K // 2].clone()
+    s[4] = nan
+    s[4, K // 2] = one
+    s[5] = nan
+    s[6, 1::2] = -INF
+    s[6, K // 2 // 2 * 2] = nan
+    s[7] = 0.5
+    s[7, K // 4] = nan
+    s[8] = -s[8].abs() - 1e3
+    s[8, K // 5] = nan
+    s = s.to(DTYPES[dtype])
+    # (NaN of a type's own, of either sign: a conversion may choose another sign)
+    bits = s.view(torch.int32 if dtype == "f32" else torch.int16)
+    quiet = {"f32": 0x7fc00000, "bf16": 0x7fc0, "f16": 0x7e00}[dtype]
+    sign = torch.iinfo(bits.dtype).min
+    bits[10, K // 2] = bits[11, K - 1] = quiet
+    bits[11, 0] = quiet + sign
+    bits[12, K // 3:K // 3 + 40] = quiet
+    return s if order == "row" else s.t().contiguous().t()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("order", ["row", "class"])
+@pytest.mark.parametrize("dtype", list(DTYPES))
+def test_nan_takes_no_place_among_the_alternatives(gpu, dtype, order):
+    """The other classes in their order; -1 only where a row has fewer of them."""
+    from warpgbm_amd import losses
+
+    for K in (3, 10, 14, 40, 130, 200, 257, 400, 512, 600, 1000, 1500, 3000, 5000, 12_000, 20_000,
+              70_001, 140_003):
+        if order == "class" and K > 3000:
+            continue
+        s = rows_with_nan(K, dtype, order, K)
+        there = ~torch.isnan(s) & (s > -INF)
+        at = torch.sort(torch.where(there, s.double(), -INF), dim=1, descending=True, stable=True)
+        for k in sorted({1, min(5, K), min(64, K)}):
+            print_case("nan", dtype, order, K, k)
+            want = torch.where(at.values[:, :k] > -INF, at.indices[:, :k], -1).to(torch.int32)
+            r = losses.class_alternatives(to_gpu(s), k)
+            assert torch.equal(r.classes.cpu(), want), (K, k)
+            lp = r.log_prob.cpu()
+            assert (lp[want < 0] == -INF).all()
+            has = torch.isnan(s).any(1)
+            assert torch.isnan(lp[has][want[has] >= 0]).all()
+            assert not torch.isnan(lp[~has]).any()
