@@ -397,7 +397,7 @@ typedef struct wgbm_distill_args {
   int32_t list_length;     /* [1, WGBM_MAX_LIST] */
   int32_t rest;
   const float* log_norm;   /* [n_rows] or NULL */
-  float log_norm_all;
+  double log_norm_all;
   const float* weight;     /* [n_rows] or NULL */
   double temperature;
 } wgbm_distill_args;

@@ -1,5 +1,5 @@
 """Losses with lists of classes at lengths, scores and arguments next to their limits:
-tiles of very long rows, NaN among scores."""
+tiles of very long rows, NaN among scores, log norms far from 0."""
 import ctypes as C
 import math
 
@@ -7,7 +7,7 @@ import pytest
 import torch
 
 from conftest import print_case
-from test_lists import alternatives_grad64, round_tol
+from test_lists import alternatives_grad64, check_distill, distill64, round_tol
 from test_losses import DTYPES, check, make_scores, to_gpu
 
 INF = math.inf
@@ -146,3 +146,27 @@ def test_nan_takes_no_place_among_the_alternatives(gpu, dtype, order):
             has = torch.isnan(s).any(1)
             assert torch.isnan(lp[has][want[has] >= 0]).all()
             assert not torch.isnan(lp[~has]).any()
+
+
+# --------------------------------------------------------------------- log norms as numbers
+@pytest.mark.gpu
+@pytest.mark.parametrize("order", ["row", "class"])
+def test_a_log_norm_for_all_rows_keeps_its_digits(gpu, order):
+    """A number is taken in float64, as temperatures are: rounded to float32, one of some
+    thousand would move every share by up to 2.4e-4 of it."""
+    from warpgbm_amd import losses
+
+    for K, k, tau, norm in ((6, 3, 1.0, 4096.3), (40, 8, 0.7, -3000.1), (300, 12, 2.0, 777.77),
+                            (900, 20, 1.0, 2049.1), (70_001, 64, 1.0, 5000.1)):
+        print_case("log norm", order, K, k, tau, norm)
+        n = 12
+        g = torch.Generator().manual_seed(K)
+        s = torch.randn((n, K), generator=g)
+        s = s if order == "row" else s.t().contiguous().t()
+        cls = torch.argsort(torch.rand((n, K), generator=g), 1)[:, :k].to(torch.int32).contiguous()
+        t = torch.log_softmax(torch.randn((n, K), generator=g, dtype=torch.float64), 1)
+        logits = (tau * (t.gather(1, cls.long()) + norm)).float()
+        w = torch.ones(n)
+        got = losses.distill_loss(to_gpu(s), cls.cuda(), logits.cuda(), log_norm=norm,
+                                  temperature=tau)
+        check_distill(got, distill64(s, cls, logits, norm, w, tau), w, tau, "f32")

@@ -160,7 +160,7 @@ class DistillArgs(C.Structure):
         ("list_length", _i32),
         ("rest", _i32),
         ("log_norm", _p),
-        ("log_norm_all", _f32),
+        ("log_norm_all", C.c_double),
         ("weight", _p),
         ("temperature", C.c_double),
     ]

@@ -79,6 +79,12 @@ __device__ __forceinline__ double exp_wide(double x) {
   return x < -700.0 ? 0.0 : ldexp(1.0 + q, (int)n);
 }
 
+// the logarithm of the teacher's sum over all classes (0 where it does not count)
+__device__ __forceinline__ double row_norm(const DistillRows& g, int64_t i) {
+  if (!g.rest) return 0.0;
+  return g.log_norm ? (double)g.log_norm[i] : g.log_norm_all;
+}
+
 // logit(j): the logits of the row's entries j < k (-infinity: not used)
 template <typename Logit>
 __device__ __forceinline__ DistillRow distill_row(const DistillSums& a, const DistillRows& g,
@@ -99,7 +105,7 @@ __device__ __forceinline__ DistillRow distill_row(const DistillSums& a, const Di
   const double lse = log_1p(a.zl_ties > 0.0f ? a.zl + (a.zl_ties - 1.0f) + B : A + (B - 1.0f));
   // shares: `one` of the largest logit, C of the other counting ones
   const bool counts = lm > -__builtin_inff() || a.q != a.q;
-  const double norm = g.rest ? (double)(g.log_norm ? g.log_norm[i] : g.log_norm_all) : 0.0;
+  const double norm = row_norm(g, i);
   const float more = a.q + (a.q_ties - 1.0f);  // relative to the largest
   float Q = 0.0f, listed = 0.0f;  // shares of the others, of the list
   double log_mass = 0.0, shift;   // log q = l / tau - shift
@@ -213,12 +219,12 @@ __global__ __launch_bounds__(F::kMax) void distill_lane_kernel(ScoresView s, Dis
     e[j] = listed >> j & 1 ? 0.0f : power_of(F::value(v, j), mrs, g);
     a.zr += e[j];
   }
-  const float norm = g.rest ? (g.log_norm ? g.log_norm[i] : g.log_norm_all) : 0.0f;
+  const double norm = row_norm(g, i);
   for (uint32_t left = listed; left; left &= left - 1) {
     const int c = __ffs(left) - 1;
     const float sc = score[c][t], l = logit[c][t];
     if (closed(sc)) {
-      if (g.rest) a.out += exp_of((float)((double)l * g.inv_tau - (double)norm));
+      if (g.rest) a.out += exp_of((float)((double)l * g.inv_tau - norm));
       continue;
     }
     const float es = power_of(sc, ms, g), el = power_of(l, lms, g);
@@ -263,9 +269,6 @@ __device__ __forceinline__ void add_entry(const DistillRows& g, double norm, flo
   x[2] += sc == m ? 1.0f : 0.0f;
   x[3] += l == lm ? 0.0f : el;
   x[4] += l == lm ? 1.0f : 0.0f;
-}
-__device__ __forceinline__ double row_norm(const DistillRows& g, int64_t i) {
-  return g.rest ? (double)(g.log_norm ? g.log_norm[i] : g.log_norm_all) : 0.0;
 }
 
 // ---------------------------------------------------------------------------

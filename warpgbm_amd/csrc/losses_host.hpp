@@ -91,7 +91,7 @@ struct DistillRows {
   int32_t k;
   bool rest;              // the classes that are not listed count
   const float* log_norm;  // null: log_norm_all for every row
-  float log_norm_all;
+  double log_norm_all;
   const float* weight;  // null: 1
   float scale;
   double inv_tau;
