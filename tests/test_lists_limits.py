@@ -170,3 +170,29 @@ def test_a_log_norm_for_all_rows_keeps_its_digits(gpu, order):
         got = losses.distill_loss(to_gpu(s), cls.cuda(), logits.cuda(), log_norm=norm,
                                   temperature=tau)
         check_distill(got, distill64(s, cls, logits, norm, w, tau), w, tau, "f32")
+
+
+# --------------------------------------------------------------------- refusals
+def test_what_is_no_number_is_refused_as_other_arguments_are():
+    from warpgbm_amd import losses
+
+    for x in (None, "warm", [1.0], (2.0, 3.0), 1j):
+        with pytest.raises(RuntimeError, match="temperature must be a number"):
+            losses._temperature(x)
+    assert losses._temperature(torch.tensor(2.0)) == 2.0 == losses._temperature(2)
+
+
+@pytest.mark.gpu
+def test_lists_refuse_what_is_no_number(gpu):
+    from warpgbm_amd import losses
+
+    s = torch.zeros((4, 8)).cuda()
+    c, x = torch.zeros((4, 2), dtype=torch.int32).cuda(), torch.zeros((4, 2)).cuda()
+    for bad in ("zero", [0.0] * 4, 1j):
+        with pytest.raises(RuntimeError, match="log_norm must be a number"):
+            losses.distill_loss(s, c, x, log_norm=bad)
+    for call in (lambda t: losses.class_alternatives(s, 2, temperature=t),
+                 lambda t: losses.class_alternatives_grad(s, torch.zeros((4, 3)).cuda(), temperature=t),
+                 lambda t: losses.distill_loss(s, c, x, temperature=t)):
+        with pytest.raises(RuntimeError, match="temperature must be a number"):
+            call(None)

@@ -234,8 +234,15 @@ def _length(t, name):
     return t.shape[1]
 
 
+def _number(x, name):
+    try:
+        return float(x)
+    except (TypeError, ValueError):
+        raise RuntimeError(f"{name} must be a number, got {x!r}") from None
+
+
 def _temperature(temperature):
-    t = float(temperature)
+    t = _number(temperature, "temperature")
     if not 1e-6 <= t <= 1e6:
         raise RuntimeError(f"temperature must be in [1e-6, 1e6], got {temperature}")
     return t
@@ -504,7 +511,7 @@ def distill_loss(scores, classes, logits, *, log_norm=None, weight=None, tempera
             norms = log_norm
             args.log_norm = _vector(log_norm, "log_norm", f32, n, dev)
         else:
-            args.log_norm_all = float(log_norm)
+            args.log_norm_all = _number(log_norm, "log_norm")
     if weight is not None:
         args.weight = _vector(weight, "weight", f32, n, dev)
     lib = _lib.load()
