@@ -181,3 +181,27 @@ def test_fit_argument_refusals():
     no(ValueError, "not an argument", "policy", advantage=y, teacher_classes=c)
     no(ValueError, "eval set", teacher_classes=c, teacher_logits=t, X_eval=X, y_eval=y,
        eval_every_n_trees=1)
+
+
+@pytest.mark.gpu
+def test_a_teacher_of_more_classes_is_not_taken_in_silence(gpu):
+    """Numbers past the student's columns name none of its classes: they are left out, and
+    the fit says so."""
+    import warnings
+
+    from warpgbm_amd import WarpGBM
+
+    new, given, _ = distill_data(600, 4, 11, True, 0.0, 1.0)
+    tc = given["teacher_classes"]
+    inside = dict(given, teacher_classes=np.where(tc < 4, tc, -1))
+    beyond = dict(given, teacher_classes=tc.copy())
+    beyond["teacher_classes"][7, 0] = 4
+    inside["teacher_classes"][7, 0] = -1
+    fits = []
+    with warnings.catch_warnings():
+        warnings.simplefilter("error", UserWarning)
+        fits.append(WarpGBM(n_estimators=2, **new, **KW).fit(**inside))
+    with pytest.warns(UserWarning, match="past the last of the 4 classes"):
+        fits.append(WarpGBM(n_estimators=2, **new, **KW).fit(**beyond))
+    assert fits[0].forest == fits[1].forest
+    assert fits[0].training_loss == fits[1].training_loss

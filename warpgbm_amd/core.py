@@ -26,6 +26,7 @@ the clipped policy loss with KL, balance and entropy terms),
 from __future__ import annotations
 
 import pickle
+import warnings
 
 import numpy as np
 import torch
@@ -465,7 +466,8 @@ class WarpGBM(BaseEstimator, RegressorMixin):
         log-probabilities.  Policies start uniform.
 
         ``"distill"``: y holds the labels, ``teacher_classes`` [n, k] (k at most 64) a
-        teacher's best classes of each row as columns of ``classes_`` (-1: none) and
+        teacher's best classes of each row as columns of ``classes_``, the sorted classes
+        of y (-1: none; numbers past the last column are left out, with a warning), and
         ``teacher_logits`` [n, k] its scores of them: the loss is their divergence at
         ``temperature`` (``warpgbm_amd.losses.distill_loss``), which counts the classes
         that are not listed as one with ``teacher_log_norm`` [n] (the logarithm of the
@@ -906,6 +908,10 @@ class WarpGBM(BaseEstimator, RegressorMixin):
         if self.objective == "distill":
             labels = torch.from_numpy(np.asarray(y).astype(np.int32)).to(dev)
             tc = given["teacher_classes"]
+            if (tc >= K).any():
+                warnings.warn(f"teacher_classes has numbers past the last of the {K} classes of y: "
+                              "these entries are left out (a teacher of other classes has other "
+                              "columns)", stacklevel=4)
             # (numbers outside the classes, -1 among them, are unused entries)
             classes = torch.from_numpy(np.where((tc >= 0) & (tc < K), tc, -1).astype(np.int32)).to(dev)
             logits, log_norm = rows(given["teacher_logits"]), rows(given["teacher_log_norm"])
