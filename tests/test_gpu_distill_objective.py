@@ -205,3 +205,38 @@ def test_a_teacher_of_more_classes_is_not_taken_in_silence(gpu):
         fits.append(WarpGBM(n_estimators=2, **new, **KW).fit(**beyond))
     assert fits[0].forest == fits[1].forest
     assert fits[0].training_loss == fits[1].training_loss
+
+
+@pytest.mark.gpu
+def test_a_forest_s_own_lists_teach_it_nothing(gpu):
+    """A forest that goes on from where its lists were taken: losses and leaves of the
+    next round are roundings."""
+    from warpgbm_amd import WarpGBM
+
+    tau, K = 2.0, 5
+    new, given, _ = distill_data(2500, K, 9, True, 0.0, tau)
+    m = WarpGBM(n_estimators=4, warm_start=True, **new, **KW).fit(**given)
+    X = given["X"]
+    lists = m.alternatives(X, K, temperature=tau)
+    assert (lists.classes >= 0).all()
+    s = scores_of(m, X)
+    m.n_estimators = 5
+    m.fit(X, given["y"], teacher_classes=lists.classes, teacher_logits=lists.log_prob * tau,
+          teacher_log_norm=np.zeros(len(X), np.float32))
+    # log p - log q of a class: the lists' rounding to float32 and, of the student, the
+    # scores' sums over four rounds and a few more steps; a gradient is at most T of it, a
+    # loss T^2 of its square
+    far = np.abs(s).max()
+    x = 2.0 ** -24 * (2 * np.abs(lists.log_prob).max() + 16 * far + 64)
+    assert len(m.training_loss) == 5
+    assert m.training_loss[3] > 1e-3 and 0 <= m.training_loss[4] <= (tau * x) ** 2
+
+    def leaves(node):
+        if "leaf_value" in node:
+            return [abs(node["leaf_value"])]
+        return leaves(node["left"]) + leaves(node["right"])
+
+    before = max(max(leaves(t)) for t in m.forest[3])
+    assert before > 1e-3
+    for tree in m.forest[4]:
+        assert max(leaves(tree)) <= tau * x
