@@ -10,8 +10,11 @@
 // As both sides sum to 1 the loss is also a sum of terms >= 0,
 //   p - q - q x = q (e^x - 1 - x) with x = log(p / q),
 // in which the rounding of log sum e^x, common to all, cancels to first order;
-// the gradient is q (e^x - 1).  Logarithms are differences in float64 of
-// float32-exact sums; the sums leave out their largest term, 1.
+// the gradient is q (e^x - 1).  Logarithms are differences in float64 of float32
+// sums.  The listed classes' sum leaves out its largest term, 1, so that a row sure of
+// one of them keeps what is left.  The others' sum has its own in: log sum e^x of a row
+// sure of one of the others is off by 2^-24, a rounding of each listed p, and P itself
+// comes from the quotient of the two sums.
 //
 // The listed classes are taken out of the rows as they sit in registers (a bit a
 // slot): what is left is the others' maximum and sum, and their gradient
@@ -101,7 +104,8 @@ __device__ __forceinline__ DistillRow distill_row(const DistillSums& a, const Di
   const float B = has_rest ? exp_of((float)drop) * a.zr : 0.0f;
   const float A = a.zl + a.zl_ties;
   o.live = w != 0.0f && !(A + B == 0.0f);
-  // without the largest term, 1, which is among the listed or among the others
+  // without the largest term, 1, where it is among the listed; among the others it is
+  // part of their sum
   const double lse = log_1p(a.zl_ties > 0.0f ? a.zl + (a.zl_ties - 1.0f) + B : A + (B - 1.0f));
   // shares: `one` of the largest logit, C of the other counting ones
   const bool counts = lm > -__builtin_inff() || a.q != a.q;
@@ -402,7 +406,8 @@ __global__ __launch_bounds__(F::kMax) void distill_slices_kernel(ScoresView s, D
 // ---------------------------------------------------------------------------
 // rows that threads share
 // ---------------------------------------------------------------------------
-// a workgroup's lists in LDS: classes (-1: not used), logits, scores of these
+// a workgroup's lists in LDS: classes, logits, scores of these (an entry that is not used
+// has class -1, and logit and score -infinity)
 struct ListTable {
   int32_t* cls;
   float* logit;
@@ -420,8 +425,6 @@ __device__ __forceinline__ ListTable list_table(uint32_t* lds, int k) {
   t.buf = (float*)(t.bits + F::kMaskWords * blockDim.x);
   return t;
 }
-
-// entries that are not used have class -1, and logit and score -infinity
 
 // entries that name a class again no longer count
 template <typename F>

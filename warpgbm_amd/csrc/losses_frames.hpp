@@ -542,14 +542,8 @@ struct ClassFrame {
     if (SLICES) __syncthreads();
     join_all(x, op, buf);
   }
-  // lists as in RowFrame, of slices: a row's entries are spread over the waves
-  static constexpr int kListRows = 64;
-  __device__ __forceinline__ int entry() const { return w; }
-  __device__ __forceinline__ int entry_step() const { return S; }
-  __device__ __forceinline__ int entry_at(int j, int) const {
-    return j * 64 + (threadIdx.x & 63);
-  }
-  // the wave and slot of class k (k / S of k < 512 by a multiplication)
+  // lists (losses_lists.hpp): the wave and slot of class k (k / S of k < 512 by a
+  // multiplication)
   __device__ __forceinline__ void locate(int32_t k, int& wave, int& slot) const {
     slot = (k * ((65535 + S) / S)) >> 16;
     wave = k - slot * S;

@@ -1,5 +1,5 @@
-// Host declarations of the losses (losses.hip, losses_balance.hip,
-// preference.hip).
+// Host declarations of the losses (losses.hip, losses_balance.hip, losses_lists.hip,
+// losses_turn.hip, preference.hip).
 #pragma once
 #include <hip/hip_runtime.h>
 #include <stdint.h>
