@@ -292,10 +292,11 @@ __global__ __launch_bounds__(F::kMax) void alternatives_candidates_kernel(Scores
       uint32_t key[P];
 #pragma unroll
       for (int p = 0; p < P; ++p) {
-        float x = -__builtin_inff();  // (of NaN alone: no class)
+        float x = F::value(v, p * F::N / P);
 #pragma unroll
-        for (int j = p * F::N / P; j < (p + 1) * F::N / P; ++j) x = fmaxf(x, F::value(v, j));
-        key[p] = order_of(x);
+        for (int j = p * F::N / P + 1; j < (p + 1) * F::N / P; ++j) x = fmaxf(x, F::value(v, j));
+        // (a part of NaN alone has no class)
+        key[p] = order_of(fmaxf(x, -__builtin_inff()));
       }
       const int32_t lanes = (s.K + VE - 1) / VE;
       if (2 * g.k > (lanes < 64 ? lanes : 64)) {
