@@ -1,5 +1,6 @@
 """Losses with lists of classes at lengths, scores and arguments next to their limits:
-tiles of very long rows, NaN among scores, log norms far from 0."""
+tiles of very long rows, NaN among scores, log norms far from 0,
+logits of -inf, launches in parts."""
 import ctypes as C
 import math
 
@@ -170,6 +171,80 @@ def test_a_log_norm_for_all_rows_keeps_its_digits(gpu, order):
         got = losses.distill_loss(to_gpu(s), cls.cuda(), logits.cuda(), log_norm=norm,
                                   temperature=tau)
         check_distill(got, distill64(s, cls, logits, norm, w, tau), w, tau, "f32")
+
+
+# --------------------------------------------------------------------- logits of -inf
+@pytest.mark.gpu
+@pytest.mark.parametrize("rest", [False, True])
+@pytest.mark.parametrize("order", ["row", "class"])
+def test_listed_classes_that_the_teacher_rules_out(gpu, order, rest):
+    """Entries of logit -inf: a share of 0, of some, of all, of closed classes; the scores'
+    probability there is to go."""
+    from warpgbm_amd import losses
+
+    for K, k in ((5, 3), (12, 5), (40, 8), (300, 20), (900, 20), (9000, 64), (70_001, 64)):
+        print_case("ruled out", order, K, k, rest)
+        n = 8
+        g = torch.Generator().manual_seed(K)
+        s = torch.randn((n, K), generator=g)
+        cls = torch.argsort(torch.rand((n, K), generator=g), 1)[:, :k].to(torch.int32).contiguous()
+        t = torch.log_softmax(torch.randn((n, K), generator=g), 1)
+        logits = t.gather(1, cls.long())
+        logits[0, 0] = logits[1, k - 1] = -INF
+        logits[2, 1:] = -INF
+        logits[3] = -INF
+        logits[4, 0] = -INF
+        s[4, cls[4, 0].long()] = -INF
+        s[5, cls[5, 0].long()] = -INF
+        logits[5, 1:] = -INF
+        w = 0.5 + torch.rand(n, generator=g)
+        s = s if order == "row" else s.t().contiguous().t()
+        norm = 0.0 if rest else None
+        got = losses.distill_loss(to_gpu(s), cls.cuda(), logits.cuda(), log_norm=norm,
+                                  weight=w.cuda())
+        want = distill64(s, cls, logits, norm, w, 1.0)
+        assert bool(want["live"][3]) == rest and bool(want["live"][5]) == rest
+        check_distill(got, want, w, 1.0, "f32")
+
+
+# --------------------------------------------------------------------- launches in parts
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,order,K", [("bf16", "row", 257), ("f32", "class", 40)])
+def test_lists_of_rows_that_go_in_parts(gpu, dtype, order, K):
+    """More rows than a launch's threads are counted for: rows at both sides of the part's
+    end and the last ones against the same rows alone, with every argument of a row."""
+    from warpgbm_amd import losses
+
+    part = ((1 << 32) - 1) // (K + 3) // 1024 * 1024
+    n, k = part + 77_777, 3
+    print_case("parts", dtype, order, n, K)
+    s = torch.empty((n, K) if order == "row" else (K, n), dtype=DTYPES[dtype], device="cuda")
+    s.normal_(generator=torch.Generator(device="cuda").manual_seed(5))
+    s = s if order == "row" else s.t()
+    at = torch.cat([torch.arange(3), torch.arange(part - 5, part + 5), torch.arange(n - 5, n)]).cuda()
+    i = torch.arange(n, device="cuda")
+    a = (i % K).to(torch.int32)
+    w, ln = 0.5 + (i % 7).float(), 2.0 + (i % 5).float()
+    few = s[at].contiguous() if order == "row" else s.t()[:, at].contiguous().t()
+    A, W, N = a[at], w[at], ln[at]
+    f = losses.class_alternatives(s, k, labels=a, temperature=1.5)
+    F = losses.class_alternatives(few, k, labels=A, temperature=1.5)
+    for x, y in zip(f, F):
+        assert torch.equal(x[at], y)
+    # (lists of either order)
+    cls = f.classes if order == "row" else f.classes.t().contiguous().t()
+    r = losses.distill_loss(s, cls, f.log_prob, log_norm=ln, weight=w)
+    R = losses.distill_loss(few, F.classes, F.log_prob, log_norm=N, weight=W)
+    assert torch.equal(r.loss[at], R.loss) and torch.equal(r.grad[at], R.grad)
+    del r
+    g = losses.class_alternatives_grad(s, f.norm, labels=a, grad_label_log_prob=w, classes=cls,
+                                       grad_log_prob=f.log_prob, grad_entropy=ln, temperature=1.5)
+    G = losses.class_alternatives_grad(few, F.norm, labels=A, grad_label_log_prob=W,
+                                       classes=F.classes, grad_log_prob=F.log_prob, grad_entropy=N,
+                                       temperature=1.5)
+    assert torch.equal(g[at], G)
+    del s, g, f
+    torch.cuda.empty_cache()
 
 
 # --------------------------------------------------------------------- refusals
