@@ -1,6 +1,6 @@
 """Losses with lists of classes at lengths, scores and arguments next to their limits:
 tiles of very long rows, NaN among scores, log norms far from 0,
-logits of -inf, launches in parts."""
+logits of -inf, lowest masks at low temperatures, launches in parts."""
 import ctypes as C
 import math
 
@@ -9,7 +9,7 @@ import torch
 
 from conftest import print_case
 from test_lists import alternatives_grad64, check_distill, distill64, round_tol
-from test_losses import DTYPES, check, make_scores, to_gpu
+from test_losses import DTYPES, STEPS, U, check, make_scores, to_gpu
 
 INF = math.inf
 MOST = {False: {0: 16_384, 1: 32_768}, True: {0: 4096, 1: 8192}}  # classes of a tile
@@ -205,6 +205,66 @@ def test_listed_classes_that_the_teacher_rules_out(gpu, order, rest):
         want = distill64(s, cls, logits, norm, w, 1.0)
         assert bool(want["live"][3]) == rest and bool(want["live"][5]) == rest
         check_distill(got, want, w, 1.0, "f32")
+
+
+# --------------------------------------------------------------------- lowest masks
+@pytest.mark.gpu
+@pytest.mark.parametrize("rest", [False, True])
+@pytest.mark.parametrize("order", ["row", "class"])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_lowest_masks_at_low_temperatures(gpu, dtype, order, rest):
+    """A class masked by the type's lowest number that the teacher takes: a divergence of
+    some 10^37, which fits, though log(q / p) at the temperature does not."""
+    from warpgbm_amd import losses
+
+    low = torch.finfo(DTYPES[dtype]).min
+    for K, k in ((4, 2), (12, 5), (40, 8), (300, 20), (900, 20), (9000, 64), (140_003, 64)):
+        for tau in (0.7, 0.05):
+            print_case("lowest", dtype, order, K, k, tau, rest)
+            n = 6
+            g = torch.Generator().manual_seed(K)
+            s = torch.randn((n, K), generator=g).to(DTYPES[dtype])
+            cls = torch.argsort(torch.rand((n, K), generator=g), 1)[:, :k].to(torch.int32).contiguous()
+            t = torch.log_softmax(torch.randn((n, K), generator=g) / tau, 1)
+            t[0] = -math.log(K)
+            logits = tau * t.gather(1, cls.long())
+            others = torch.ones((n, K), dtype=torch.bool).scatter_(1, cls.long(), False)
+            s[0, cls[0, 1].long()] = low             # an entry
+            s[1, cls[1].long()] = low                # the whole list
+            s[2, others[2]] = low                    # what is not listed
+            s[3, others[3]] = low
+            s[3, cls[3, 0].long()] = low
+            w = 0.5 + torch.rand(n, generator=g)
+            s = s if order == "row" else s.t().contiguous().t()
+            norm = 0.0 if rest else None
+            got = losses.distill_loss(to_gpu(s), cls.cuda(), logits.cuda(), log_norm=norm,
+                                      weight=w.cuda(), temperature=tau)
+            want = distill64(s, cls, logits, norm, w, tau)
+            assert 1e35 < want["loss"].max() < torch.finfo(torch.float32).max
+            # the other classes' parts of their sum from their own maximum: the log of a sum
+            # of e^(-10^39) keeps no number of them, in float64 either
+            x = s.double() / tau
+            x = torch.where(others, x, -INF)
+            r = torch.exp(x - x.max(1, keepdim=True).values)
+            r = r / r.sum(1, keepdim=True)
+            p, q, Q = want["p"], want["q"], want["Q"][:, None]
+            # A share q = e^y, y = log q, has the power of two of a float32 product: the
+            # difference's, the product's and log2(e) / tau's roundings are 2.3 |y| 2^-24 of
+            # it. Elsewhere that is a rounding of the largest share (|y| e^-|y| < 1 / e);
+            # here q multiplies log(q / p) of any size, and so does its rounding.
+            value = w.double() * tau * tau
+            y = torch.where(q > 0, q.log().abs(), 0.0)
+            gap = torch.where(q > 0, y + want["far"], 0.0)
+            gap_rest = torch.where(want["Q"] > 0, want["rest"].abs() + 30.0, 0.0)
+            tol = value * U * (STEPS * want["lost"] + (k + 16) * 4
+                               + (q * gap * (16 + 2.3 * y)).sum(1) + (k + 8) * gap_rest)
+            check(got.loss, want["loss"], tol + U * want["loss"], "loss")
+            scale = (w.double() * tau)[:, None]
+            grad = scale * (p - q - Q * r)
+            tol = scale * U * ((STEPS + 64) * (p + q + r * (want["P"][:, None] + Q))
+                               + (k + 8) * (q + r))
+            half = U if dtype == "f32" else 2.0 ** -8 * (1 + 1e-3)
+            check(got.grad, grad, tol + half * grad.abs() + 1e-37, "gradient")
 
 
 # --------------------------------------------------------------------- launches in parts

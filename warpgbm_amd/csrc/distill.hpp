@@ -49,21 +49,26 @@ struct DistillRow {
   float to_p, to_q;    // p = to_p e^(s - m), q = to_q e^(l - lm)
   double apart;        // log(p / q) = (s - l) / tau - apart
   float others;        // gradient of another class: others * e^(s - mr)
-  float rest_term;     // the others' term of the loss
-  float scale, value;  // w tau, w tau^2
+  float rest_term;     // the others' term
+  float scale;         // w tau
 };
 
-// a bucket's term and what its gradient is made of, x = log(p / q)
+// a bucket's term, times tau / 4, and what its gradient is made of, log_ratio = log(p / q).
+// (The logarithm of a class masked by the lowest finite score passes float32's range at a
+// tau below 1; tau times it is a difference of scores, and a sum of such by shares that
+// round to more than 1 fits by the 4.)
+constexpr float kTermUnit = 0.25f;
 struct Bucket {
   float term, slope;
 };
-__device__ __forceinline__ Bucket bucket(float p, float q, float x) {
+__device__ __forceinline__ Bucket bucket(float p, float q, double log_ratio, float tau) {
+  const float x = (float)log_ratio, unit = kTermUnit * tau;
   if (fabsf(x) <= 1.0f) {
     const float f = phi_small(x);
-    return {q * f, q * (x + f)};
+    return {unit * q * f, q * (x + f)};
   }
-  if (q == 0.0f) return {p, p};
-  return {p - q - q * x, p - q};
+  if (q == 0.0f) return {unit * p, p};
+  return {unit * (p - q) - q * (float)(log_ratio * (double)unit), p - q};
 }
 
 __device__ __forceinline__ float power_of(float v, float from, const DistillRows& g) {
@@ -97,7 +102,6 @@ __device__ __forceinline__ DistillRow distill_row(const DistillSums& a, const Di
   o.m = safe_max(m);
   o.lm = safe_max(lm);
   o.scale = w * g.tau;
-  o.value = o.scale * g.tau;
   const bool has_rest = mr > -__builtin_inff() || a.zr != a.zr;
   // scores: listed A, others B, relative to m
   const double drop = has_rest ? ((double)mr - (double)o.m) * g.inv_tau : 0.0;
@@ -147,11 +151,11 @@ __device__ __forceinline__ DistillRow distill_row(const DistillSums& a, const Di
     double log_P = -log_1p(A / B);
     if (!(B > 1e-30f * A)) log_P = drop + log_of(a.zr) - lse;
     const float P = exp_of((float)log_P);
-    Bucket b{P, P};
+    Bucket b{kTermUnit * g.tau * P, P};
     if (Q > 0.0f) {
       // (a small list: 1 - listed would round its digits away)
       const double log_Q = (listed < 0.5f ? (double)log1p_of(-listed) : log_of(Q)) - log_mass;
-      b = bucket(P, exp_of((float)log_Q), (float)(log_P - log_Q));
+      b = bucket(P, exp_of((float)log_Q), log_P - log_Q, g.tau);
     }
     o.rest_term = b.term;
     if (o.live) o.others = o.scale * b.slope / a.zr;
@@ -162,7 +166,7 @@ __device__ __forceinline__ DistillRow distill_row(const DistillSums& a, const Di
 __device__ __forceinline__ Bucket distill_entry(const DistillRow& r, const DistillRows& g, float s,
                                                 float l) {
   return bucket(r.to_p * power_of(s, r.m, g), r.to_q * power_of(l, r.lm, g),
-                (float)(((double)s - (double)l) * g.inv_tau - r.apart));
+                ((double)s - (double)l) * g.inv_tau - r.apart, g.tau);
 }
 // a listed class that does not count: the row may not take it
 __device__ __forceinline__ bool closed(float s) { return s == -__builtin_inff(); }
@@ -252,7 +256,7 @@ __global__ __launch_bounds__(F::kMax) void distill_lane_kernel(ScoresView s, Dis
     }
     score[c][t] = grad;
   }
-  g.loss[i] = r.live ? r.value * loss : 0.0f;
+  g.loss[i] = r.live ? r.scale / kTermUnit * loss : 0.0f;
   if (!out.data || (!r.live && accumulate)) return;
   f.store(out, blockIdx.x, accumulate, [&](int j) {
     const float x = listed >> j & 1 ? score[j][t] : r.others * e[j];
@@ -391,7 +395,7 @@ __global__ __launch_bounds__(F::kMax) void distill_slices_kernel(ScoresView s, D
   __syncthreads();
   if (f.w == 0) {
     f.join_all(loss, AddF(), buf + 9 * blockDim.x);
-    if (in) g.loss[i] = r.live ? r.value * (loss[0] + r.rest_term) : 0.0f;
+    if (in) g.loss[i] = r.live ? r.scale / kTermUnit * (loss[0] + r.rest_term) : 0.0f;
   }
   // (one store for rows that count and rows left out: lanes of a wave may hold both)
   if (!in || !out.data || (!r.live && accumulate)) return;
@@ -571,7 +575,7 @@ __global__ __launch_bounds__(F::kMax) void distill_frame_kernel(ScoresView s, Di
   }
   // (rows of several waves have their list in the first one)
   if (owner) loss[0] = lanes_reduce<(F::kListLanes)>(loss[0], AddF());
-  if (in && f.first_lane()) g.loss[i] = r.live ? r.value * (loss[0] + r.rest_term) : 0.0f;
+  if (in && f.first_lane()) g.loss[i] = r.live ? r.scale / kTermUnit * (loss[0] + r.rest_term) : 0.0f;
 }
 
 // ---------------------------------------------------------------------------
@@ -692,7 +696,7 @@ __global__ __launch_bounds__(1024) void distill_long_kernel(ScoresView s, Distil
     }
   }
   whole.reduce_all(loss, AddF(), buf);
-  if (threadIdx.x == 0) g.loss[i] = r.live ? r.value * (loss[0] + r.rest_term) : 0.0f;
+  if (threadIdx.x == 0) g.loss[i] = r.live ? r.scale / kTermUnit * (loss[0] + r.rest_term) : 0.0f;
 }
 
 template <typename T>
