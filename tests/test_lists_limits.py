@@ -1,6 +1,7 @@
 """Losses with lists of classes at lengths, scores and arguments next to their limits:
 tiles of very long rows, NaN among scores, log norms far from 0,
-logits of -inf, lowest masks at low temperatures, launches in parts."""
+logits of -inf, lowest masks at low temperatures, rows
+and teachers far from 0, launches in parts."""
 import ctypes as C
 import math
 
@@ -265,6 +266,40 @@ def test_lowest_masks_at_low_temperatures(gpu, dtype, order, rest):
                                + (k + 8) * (q + r))
             half = U if dtype == "f32" else 2.0 ** -8 * (1 + 1e-3)
             check(got.grad, grad, tol + half * grad.abs() + 1e-37, "gradient")
+
+
+# --------------------------------------------------------------------- far from 0
+FAR = [1e6, -1e10, 1e20, -1e30, torch.finfo(torch.float32).max, torch.finfo(torch.float32).min]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rest", [False, True])
+@pytest.mark.parametrize("order", ["row", "class"])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_distillation_of_rows_and_teachers_far_from_0(gpu, dtype, order, rest):
+    """Rows masked as a whole by the lowest number, and others of equal scores of any size:
+    even probabilities; lists of logits of any size, whose differences count."""
+    from warpgbm_amd import losses
+
+    for K, k in ((4, 2), (12, 5), (40, 8), (300, 20), (900, 20), (9000, 64), (140_003, 64)):
+        print_case("far", dtype, order, K, k, rest)
+        n = 2 * len(FAR)
+        g = torch.Generator().manual_seed(K)
+        s = torch.randn((n, K), generator=g)
+        t = torch.log_softmax(torch.randn((n, K), generator=g), 1)
+        cls = torch.argsort(torch.rand((n, K), generator=g), 1)[:, :k].to(torch.int32).contiguous()
+        logits = t.gather(1, cls.long())
+        for i, far in enumerate(FAR):
+            s[i] = far
+            if not rest:
+                logits[len(FAR) + i] = far
+        s = s.to(DTYPES[dtype]).clamp(torch.finfo(DTYPES[dtype]).min, torch.finfo(DTYPES[dtype]).max)
+        s = s if order == "row" else s.t().contiguous().t()
+        w = 0.5 + torch.rand(n, generator=g)
+        norm = 0.0 if rest else None
+        got = losses.distill_loss(to_gpu(s), cls.cuda(), logits.cuda(), log_norm=norm,
+                                  weight=w.cuda())
+        check_distill(got, distill64(s, cls, logits, norm, w, 1.0), w, 1.0, dtype)
 
 
 # --------------------------------------------------------------------- launches in parts

@@ -47,7 +47,9 @@ struct DistillRow {
   bool live;
   float m, lm;         // (0 where there is none)
   float to_p, to_q;    // p = to_p e^(s - m), q = to_q e^(l - lm)
-  double apart;        // log(p / q) = (s - l) / tau - apart
+  // log(p / q) = ((s - m) - (l - lm)) / tau - apart: scores and logits of any size count by
+  // their differences
+  double apart;
   float others;        // gradient of another class: others * e^(s - mr)
   float rest_term;     // the others' term
   float scale;         // w tau
@@ -116,10 +118,10 @@ __device__ __forceinline__ DistillRow distill_row(const DistillSums& a, const Di
   const double norm = row_norm(g, i);
   const float more = a.q + (a.q_ties - 1.0f);  // relative to the largest
   float Q = 0.0f, listed = 0.0f;  // shares of the others, of the list
-  double log_mass = 0.0, shift;   // log q = l / tau - shift
+  double log_mass = 0.0, top_q;   // log of the largest q
   if (!g.rest) {
     o.live = o.live && counts;
-    shift = (double)o.lm * g.inv_tau + (counts ? log_1p(more) : 0.0);
+    top_q = counts ? -log_1p(more) : 0.0;
   } else {
     const float top = (float)((double)lm * g.inv_tau - norm);  // its logarithm
     const float one = counts ? exp_of(top) : 0.0f, C = counts ? more * one : 0.0f;
@@ -141,11 +143,11 @@ __device__ __forceinline__ DistillRow distill_row(const DistillSums& a, const Di
     log_mass = (double)log1p_of(-lost);
     if (!(lost < 0.5f)) log_mass = log_of(one + C + Q);
     o.live = o.live && (counts || rest) && !(one + C + Q == 0.0f);
-    shift = norm + log_mass;
+    top_q = ((double)o.lm * g.inv_tau - norm) - log_mass;
   }
   o.to_p = exp_of((float)-lse);
-  o.to_q = exp_of((float)((double)o.lm * g.inv_tau - shift));
-  o.apart = (double)o.m * g.inv_tau + lse - shift;
+  o.to_q = exp_of((float)top_q);
+  o.apart = lse + top_q;
   // the others
   if (has_rest) {
     double log_P = -log_1p(A / B);
@@ -166,7 +168,8 @@ __device__ __forceinline__ DistillRow distill_row(const DistillSums& a, const Di
 __device__ __forceinline__ Bucket distill_entry(const DistillRow& r, const DistillRows& g, float s,
                                                 float l) {
   return bucket(r.to_p * power_of(s, r.m, g), r.to_q * power_of(l, r.lm, g),
-                ((double)s - (double)l) * g.inv_tau - r.apart, g.tau);
+                (((double)s - (double)r.m) - ((double)l - (double)r.lm)) * g.inv_tau - r.apart,
+                g.tau);
 }
 // a listed class that does not count: the row may not take it
 __device__ __forceinline__ bool closed(float s) { return s == -__builtin_inff(); }
