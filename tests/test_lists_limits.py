@@ -1,7 +1,7 @@
 """Losses with lists of classes at lengths, scores and arguments next to their limits:
 tiles of very long rows, NaN among scores, log norms far from 0,
 logits of -inf, lowest masks at low temperatures, rows
-and teachers far from 0, launches in parts."""
+and teachers far from 0, shares below float32's range, launches in parts."""
 import ctypes as C
 import math
 
@@ -300,6 +300,77 @@ def test_distillation_of_rows_and_teachers_far_from_0(gpu, dtype, order, rest):
         got = losses.distill_loss(to_gpu(s), cls.cuda(), logits.cuda(), log_norm=norm,
                                   weight=w.cuda())
         check_distill(got, distill64(s, cls, logits, norm, w, 1.0), w, 1.0, dtype)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("order", ["row", "class"])
+def test_shares_below_and_above_float32_s_range(gpu, order):
+    """A row that may take only classes to which the teacher gives e^-100 and less: they
+    are scaled to sum 1, whatever is left of the teacher. Logits with a log norm far below
+    theirs, the same."""
+    from warpgbm_amd import losses
+
+    for K, k in ((4, 3), (12, 5), (40, 8), (300, 20), (900, 20), (9000, 64), (70_001, 64)):
+        print_case("range", order, K, k)
+        n = 6
+        g = torch.Generator().manual_seed(K)
+        s = torch.randn((n, K), generator=g)
+        cls = torch.argsort(torch.rand((n, K), generator=g), 1)[:, :k].to(torch.int32).contiguous()
+        logits = torch.randn((n, k), generator=g)
+        others = torch.ones((n, K), dtype=torch.bool).scatter_(1, cls.long(), False)
+        logits[:4, 0] = torch.tensor([100.0, 200.0, 600.0, 100.0])
+        ln = torch.logsumexp(logits.double(), 1).float()
+        for i in range(4):                          # the teacher's class is closed
+            s[i, cls[i, 0].long()] = -INF
+        s[3, others[3]] = -INF                      # and all that it does not list
+        s[4, others[4]] = -INF
+        logits[4:] += torch.tensor([[100.0], [300.0]])  # shares of e^100 and e^300
+        ln[4:] = 0.0
+        w = 0.5 + torch.rand(n, generator=g)
+        s = s if order == "row" else s.t().contiguous().t()
+        got = losses.distill_loss(to_gpu(s), cls.cuda(), logits.cuda(), log_norm=ln.cuda(),
+                                  weight=w.cuda())
+        want = distill64(s, cls, logits, ln, w, 1.0)
+        assert want["live"].all()
+        check_distill(got, want, w, 1.0, "f32")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("order", ["row", "class"])
+def test_nan_shows_in_its_row_of_a_distillation(gpu, order):
+    """In a score, a logit, a log norm, a weight; not in entries that are not used or rows
+    that are left out, and in no other row."""
+    from warpgbm_amd import losses
+
+    nan = float("nan")
+    for K, k in ((4, 2), (12, 5), (40, 8), (300, 20), (900, 20), (9000, 64), (70_001, 64)):
+        print_case("nan row", order, K, k)
+        n = 16
+        g = torch.Generator().manual_seed(K)
+        s = torch.randn((n, K), generator=g)
+        cls = torch.argsort(torch.rand((n, K), generator=g), 1)[:, :k].to(torch.int32).contiguous()
+        t = torch.log_softmax(torch.randn((n, K), generator=g), 1)
+        logits, ln, w = t.gather(1, cls.long()), torch.zeros(n), torch.ones(n)
+        others = torch.ones((n, K), dtype=torch.bool).scatter_(1, cls.long(), False)
+        s[1, cls[1, 0].long()] = nan
+        s[2, int(others[2].nonzero()[0])] = nan
+        logits[3, 0] = nan
+        ln[4] = nan                       # (counts with log norms only)
+        ln[5] = nan
+        s[5, others[5]] = -INF            # (no rest, whatever the log norm)
+        w[6] = nan
+        s[8], logits[8], ln[8], w[8] = nan, nan, nan, 0.0
+        cls[9, 1], logits[9, 1] = -1, nan
+        s[10, cls[10, 0].long()], logits[10, 0] = -INF, nan   # (a closed class: of the rest)
+        s[11, cls[11, 0].long()], logits[11, 0] = -INF, nan
+        s[11, others[11]] = -INF                              # (no rest)
+        s = s if order == "row" else s.t().contiguous().t()
+        for norms, rows in ((None, {1, 2, 3, 6}), (ln, {1, 2, 3, 4, 5, 6, 10})):
+            r = losses.distill_loss(to_gpu(s), cls.cuda(), logits.cuda(), weight=w.cuda(),
+                                    log_norm=None if norms is None else norms.cuda())
+            assert set(torch.isnan(r.loss).nonzero()[:, 0].tolist()) == rows
+            assert set(torch.isnan(r.grad).any(1).nonzero()[:, 0].tolist()) == rows
+            assert r.loss[8] == 0 and (r.grad[8] == 0).all()
 
 
 # --------------------------------------------------------------------- launches in parts

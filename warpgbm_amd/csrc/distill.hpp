@@ -81,6 +81,7 @@ __device__ __forceinline__ float power_of(float v, float from, const DistillRows
 // first terms of its series at r / 1024, doubled ten times, q -> q (q + 2).  (Seldom
 // called; a longer series' coefficients would take the registers of a wave in five.)
 __device__ __forceinline__ double exp_wide(double x) {
+  x = fmin(x, 1000.0);
   const double n = rint(x * 1.44269504088896340736);
   const double r = fma(n, -0.693147180559945286227, x) * 0x1p-10;
   double q = fma(fma(fma(r, 1.0 / 24.0, 1.0 / 6.0), r, 0.5), r * r, r);
@@ -113,20 +114,18 @@ __device__ __forceinline__ DistillRow distill_row(const DistillSums& a, const Di
   // without the largest term, 1, where it is among the listed; among the others it is
   // part of their sum
   const double lse = log_1p(a.zl_ties > 0.0f ? a.zl + (a.zl_ties - 1.0f) + B : A + (B - 1.0f));
-  // shares: `one` of the largest logit, C of the other counting ones
+  // shares: `one` of the largest logit, C of the other counting ones; top its logarithm
   const bool counts = lm > -__builtin_inff() || a.q != a.q;
-  const double norm = row_norm(g, i);
   const float more = a.q + (a.q_ties - 1.0f);  // relative to the largest
-  float Q = 0.0f, listed = 0.0f;  // shares of the others, of the list
-  double log_mass = 0.0, top_q;   // log of the largest q
-  if (!g.rest) {
-    o.live = o.live && counts;
-    top_q = counts ? -log_1p(more) : 0.0;
-  } else {
-    const float top = (float)((double)lm * g.inv_tau - norm);  // its logarithm
-    const float one = counts ? exp_of(top) : 0.0f, C = counts ? more * one : 0.0f;
+  float Q = 0.0f, listed = 0.0f;               // shares of the others, of the list
+  double log_mass = 0.0, top_q = 0.0;          // log of the sum scaled to 1, of the largest q
+  bool rest = false;
+  const double norm = row_norm(g, i);
+  if (g.rest) {
+    const double top = (double)o.lm * g.inv_tau - norm;
+    const float one = counts ? exp_of((float)top) : 0.0f, C = counts ? more * one : 0.0f;
     listed = one + C + a.out;
-    float left = counts ? one_less_exp(top) - C - a.out : 1.0f - a.out;
+    float left = counts ? one_less_exp((float)top) - C - a.out : 1.0f - a.out;
     // next to the border whether a rest is one is decided in float64 (the roundings above
     // come to less than 100 * 2^-24); so is what is left of a list that the row may
     // mostly not take, whose roundings the scaling to sum 1 would enlarge
@@ -136,14 +135,20 @@ __device__ __forceinline__ DistillRow distill_row(const DistillSums& a, const Di
       for (int j = 0; j < k; ++j) sum += exp_wide((double)logit(j) * g.inv_tau - norm);
       left = (float)(1.0 - sum);
     }
-    const bool rest = left >= kLeastRest && has_rest;
-    Q = rest ? left : 0.0f;
-    // what is left out of sum 1
-    const float lost = a.out + (rest ? 0.0f : left);
-    log_mass = (double)log1p_of(-lost);
-    if (!(lost < 0.5f)) log_mass = log_of(one + C + Q);
-    o.live = o.live && (counts || rest) && !(one + C + Q == 0.0f);
-    top_q = ((double)o.lm * g.inv_tau - norm) - log_mass;
+    rest = left >= kLeastRest && has_rest;
+    if (rest) {
+      Q = left;
+      log_mass = (double)log1p_of(-a.out);
+      if (!(a.out < 0.5f)) log_mass = log_of(one + C + Q);
+      top_q = counts ? top - log_mass : 0.0;
+    }
+  }
+  // without a rest the counting shares sum to 1 whatever they were, also past float32's
+  // range (NaN of what the rest is made of shows in the results)
+  if (!rest) {
+    o.live = o.live && counts;
+    top_q = counts ? -log_1p(more) : 0.0;
+    if (norm != norm || (has_rest && a.out != a.out)) top_q = __builtin_nan("");
   }
   o.to_p = exp_of((float)-lse);
   o.to_q = exp_of((float)top_q);
