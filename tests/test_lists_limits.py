@@ -304,6 +304,38 @@ def test_distillation_of_rows_and_teachers_far_from_0(gpu, dtype, order, rest):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("order", ["row", "class"])
+def test_alternatives_of_rows_far_from_0(gpu, order):
+    """Differences of scores count: rows of few values at any distance from 0 have the bits
+    of the same rows at 0."""
+    from warpgbm_amd import losses
+
+    for K, k in ((4, 2), (12, 5), (40, 8), (300, 20), (900, 20), (9000, 64), (140_003, 64)):
+        print_case("far alternatives", order, K, k)
+        n = len(FAR)
+        g = torch.Generator().manual_seed(K)
+        near = torch.zeros((n, K))
+        far = torch.tensor(FAR)[:, None].expand(n, K).clone()
+        for i in range(n):
+            gone = torch.rand(K, generator=g) < 0.3
+            gone[i % K] = False
+            near[i, gone] = far[i, gone] = -INF
+        cls = torch.argsort(torch.rand((n, K), generator=g), 1)[:, :k].to(torch.int32).contiguous()
+        up, ge = torch.randn((n, k), generator=g).cuda(), torch.randn(n, generator=g).cuda()
+        a = torch.randint(0, K, (n,), generator=g, dtype=torch.int32).cuda()
+        got = []
+        for s in (near, far):
+            s = to_gpu(s if order == "row" else s.t().contiguous().t())
+            f = losses.class_alternatives(s, k, labels=a, temperature=0.7)
+            d = losses.class_alternatives_grad(s, f.norm, labels=a, grad_label_log_prob=ge,
+                                               classes=cls.cuda(), grad_log_prob=up,
+                                               grad_entropy=ge, temperature=0.7)
+            got.append((f.classes, f.log_prob, f.entropy, f.label_log_prob, f.norm[:, 1:], d))
+        for x, y in zip(*got):
+            assert torch.equal(x, y) and not torch.isnan(y).any()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("order", ["row", "class"])
 def test_shares_below_and_above_float32_s_range(gpu, order):
     """A row that may take only classes to which the teacher gives e^-100 and less: they
     are scaled to sum 1, whatever is left of the teacher. Logits with a log norm far below
