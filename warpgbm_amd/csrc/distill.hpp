@@ -81,7 +81,6 @@ __device__ __forceinline__ float power_of(float v, float from, const DistillRows
 // first terms of its series at r / 1024, doubled ten times, q -> q (q + 2).  (Seldom
 // called; a longer series' coefficients would take the registers of a wave in five.)
 __device__ __forceinline__ double exp_wide(double x) {
-  x = fmin(x, 1000.0);
   const double n = rint(x * 1.44269504088896340736);
   const double r = fma(n, -0.693147180559945286227, x) * 0x1p-10;
   double q = fma(fma(fma(r, 1.0 / 24.0, 1.0 / 6.0), r, 0.5), r * r, r);
@@ -106,30 +105,24 @@ __device__ __forceinline__ DistillRow distill_row(const DistillSums& a, const Di
   o.lm = safe_max(lm);
   o.scale = w * g.tau;
   const bool has_rest = mr > -__builtin_inff() || a.zr != a.zr;
-  // scores: listed A, others B, relative to m
-  const double drop = has_rest ? ((double)mr - (double)o.m) * g.inv_tau : 0.0;
-  const float B = has_rest ? exp_of((float)drop) * a.zr : 0.0f;
-  const float A = a.zl + a.zl_ties;
-  o.live = w != 0.0f && !(A + B == 0.0f);
-  // without the largest term, 1, where it is among the listed; among the others it is
-  // part of their sum
-  const double lse = log_1p(a.zl_ties > 0.0f ? a.zl + (a.zl_ties - 1.0f) + B : A + (B - 1.0f));
   // shares: `one` of the largest logit, C of the other counting ones; top its logarithm
   const bool counts = lm > -__builtin_inff() || a.q != a.q;
   const float more = a.q + (a.q_ties - 1.0f);  // relative to the largest
-  float Q = 0.0f, listed = 0.0f;               // shares of the others, of the list
-  double log_mass = 0.0, top_q = 0.0;          // log of the sum scaled to 1, of the largest q
-  bool rest = false;
-  const double norm = row_norm(g, i);
+  double top_q = 0.0, log_Q = 0.0;             // logs of the largest q, of the others' share
+  bool rest = false, odd = false;
+  o.live = true;
   if (g.rest) {
-    const double top = (double)o.lm * g.inv_tau - norm;
+    const double top = (double)o.lm * g.inv_tau - row_norm(g, i);
+    odd = top != top || (has_rest && a.out != a.out);
     const float one = counts ? exp_of((float)top) : 0.0f, C = counts ? more * one : 0.0f;
-    listed = one + C + a.out;
+    const float held = one + C;
     float left = counts ? one_less_exp((float)top) - C - a.out : 1.0f - a.out;
     // next to the border whether a rest is one is decided in float64 (the roundings above
     // come to less than 100 * 2^-24); so is what is left of a list that the row may
-    // mostly not take, whose roundings the scaling to sum 1 would enlarge
-    if (has_rest && (fabsf(left - kLeastRest) < 1e-5f || a.out > 0.5f)) {
+    // mostly not take, whose roundings the scaling to sum 1 would enlarge (shares of 2 and
+    // more, of a log norm too small, leave none)
+    if (has_rest && (fabsf(left - kLeastRest) < 1e-5f || (a.out > 0.5f && left > -1.0f))) {
+      const double norm = row_norm(g, i);
       double sum = 0.0;
 #pragma unroll 1
       for (int j = 0; j < k; ++j) sum += exp_wide((double)logit(j) * g.inv_tau - norm);
@@ -137,19 +130,30 @@ __device__ __forceinline__ DistillRow distill_row(const DistillSums& a, const Di
     }
     rest = left >= kLeastRest && has_rest;
     if (rest) {
-      Q = left;
-      log_mass = (double)log1p_of(-a.out);
-      if (!(a.out < 0.5f)) log_mass = log_of(one + C + Q);
-      top_q = counts ? top - log_mass : 0.0;
+      // what is left, scaled to sum 1 (of a small list: 1 - listed would round its digits
+      // away)
+      double log_mass = (double)log1p_of(-a.out);
+      if (!(a.out < 0.5f)) log_mass = log_of(held + left);
+      const float listed = held + a.out;
+      log_Q = (listed < 0.5f ? (double)log1p_of(-listed) : log_of(left)) - log_mass;
+      if (counts) top_q = top - log_mass;
     }
   }
   // without a rest the counting shares sum to 1 whatever they were, also past float32's
   // range (NaN of what the rest is made of shows in the results)
   if (!rest) {
-    o.live = o.live && counts;
+    o.live = counts;
     top_q = counts ? -log_1p(more) : 0.0;
-    if (norm != norm || (has_rest && a.out != a.out)) top_q = __builtin_nan("");
+    if (odd) top_q = __builtin_nan("");
   }
+  // scores: listed A, others B, relative to m
+  const double drop = has_rest ? ((double)mr - (double)o.m) * g.inv_tau : 0.0;
+  const float B = has_rest ? exp_of((float)drop) * a.zr : 0.0f;
+  const float A = a.zl + a.zl_ties;
+  o.live = o.live && w != 0.0f && !(A + B == 0.0f);
+  // without the largest term, 1, where it is among the listed; among the others it is
+  // part of their sum
+  const double lse = log_1p(a.zl_ties > 0.0f ? a.zl + (a.zl_ties - 1.0f) + B : A + (B - 1.0f));
   o.to_p = exp_of((float)-lse);
   o.to_q = exp_of((float)top_q);
   o.apart = lse + top_q;
@@ -159,11 +163,7 @@ __device__ __forceinline__ DistillRow distill_row(const DistillSums& a, const Di
     if (!(B > 1e-30f * A)) log_P = drop + log_of(a.zr) - lse;
     const float P = exp_of((float)log_P);
     Bucket b{kTermUnit * g.tau * P, P};
-    if (Q > 0.0f) {
-      // (a small list: 1 - listed would round its digits away)
-      const double log_Q = (listed < 0.5f ? (double)log1p_of(-listed) : log_of(Q)) - log_mass;
-      b = bucket(P, exp_of((float)log_Q), log_P - log_Q, g.tau);
-    }
+    if (rest) b = bucket(P, exp_of((float)log_Q), log_P - log_Q, g.tau);
     o.rest_term = b.term;
     if (o.live) o.others = o.scale * b.slope / a.zr;
   }
@@ -481,9 +481,11 @@ __device__ __forceinline__ void list_sums(const F& f, const ListTable& t, const 
   }
 }
 
+// (registers for eight waves where that takes two from the seldom loop of distill_row: 15000
+// x 3900 float32 97 us, 100 in 66 registers)
 template <typename F>
-__global__ __launch_bounds__(F::kMax) void distill_frame_kernel(ScoresView s, DistillRows g,
-                                                                ScoresView out, bool accumulate) {
+__global__ __launch_bounds__(F::kMax, F::G == 256 && F::NC == 4 ? 8 : 1) void distill_frame_kernel(
+    ScoresView s, DistillRows g, ScoresView out, bool accumulate) {
   using T = typename F::T;
   extern __shared__ uint32_t lds[];
   __shared__ DistillRow share;
