@@ -167,8 +167,15 @@ __global__ __launch_bounds__(F::kMax) void alternatives_turns_kernel(ScoresView 
 // the row is no larger than the k-th largest score, so the classes from there on
 // (some more than k in rows without an order) are copied to LDS, and a
 // candidate's place is the number of candidates with a larger key.  Rows with
-// more candidates than the copy holds (many equal scores) take their best
-// classes in turns.
+// more candidates than the copy holds take their best classes in turns from memory.
+//
+// A part is what a thread has (or four neighbouring ones): 4 to 32 classes in a row at a
+// time.  Where class numbers carry no order of scores, k parts hold little more than k
+// candidates; where the best classes lie next to each other they share parts, and the
+// candidates grow to the square.  64 best of bfloat16 rows, us, classes in any order, with
+// scores that fall as the logarithm of the class's number beside noise of a unit,
+// without noise, and all equal: 30000 x 3001 87, 133, 4270, 4340; 8191 x 16001 63, 72, 179,
+// 5940; 4099 x 32000 80, 127, 5710, 5740 (the last two of each, but for 179: turns).
 // ---------------------------------------------------------------------------
 // a number no larger than the k-th largest of the wave's M keys a lane (its upper
 // 16 bits: 2^-7 of the value), as a score
@@ -473,7 +480,15 @@ __global__ __launch_bounds__(1024) void alternatives_long_kernel(ScoresView s, A
 }
 
 // ---------------------------------------------------------------------------
-// which kernel a call takes
+// which kernel a call takes.  From 64 chunks on: as few threads as hold a row's chunks in 8
+// each, 16 where no workgroup has more.  20 best of 60M float32 (120M bfloat16) scores,
+// us, so, with a quarter of the threads and four times the chunks, and the other way round:
+//   of 1000 (2000) classes   59 (74), -, 117 (135)
+//   of 2000 (4000)           50 (57), -, 70 (86)
+//   of 4000 (8000)           47 (61), 48 (65), 126 (149)
+//   of 8000 (16000)          43 (50), -, 73 (92)
+//   of 16000 (32000)         50 (64), 43 (53), -
+// (256 threads of sixteen chunks would be faster for the last ones, 3750 rows each)
 // ---------------------------------------------------------------------------
 template <typename T>
 static int alternatives_frames(const ScoresView& s, const AltRows& g, hipStream_t st) {

@@ -344,7 +344,22 @@ __global__ __launch_bounds__(F::kMax) void alternatives_grad_list_kernel(ScoresV
   if (mine) write(lab, sa, g_label);
 }
 
-// frames of class-major rows and of row-major ones up to 1024 chunks
+// frames of class-major rows and of row-major ones up to 1024 chunks.  Nothing is summed
+// over a row, so waves wait for one another at the lists only: few threads with two chunks
+// each, up to 32 with eight, then workgroups.  Gradient with eight
+// listed classes, us, with the threads and chunks taken, half the threads and twice the
+// chunks, twice the threads and half the chunks (-: the same, or no such frame):
+//   float32                           bfloat16
+//   1M x 27        103    -  108      1M x 55        119    -  123
+//   1M x 59        154  187  194      1M x 119       186  212  228
+//   504201 x 119   132  141  192      502092 x 239   159  164  219
+//   251046 x 239   122  119  191      250520 x 479   143  134  216
+//   125260 x 479   103  116  117      125130 x 959   112  132  138
+//   60060 x 999    108    -  101      60030 x 1999   121    -  105
+//   30015 x 1999   102  105    -      30006 x 3999   130  117    -   (half: a wave a row)
+//   15003 x 3999    95  106  158      15000 x 7999   120  123  196   (half: a wave a row)
+// Without a list the order is the same, but for 16-bit rows of 257 to 1024 chunks: a wave a
+// row takes 90 and 93 us there, workgroups 104 and 107.
 template <typename T, typename Fn>
 static void pick_short_frame(const ScoresView& s, Fn fn) {
   constexpr int VE = Chunk<T>::VE;

@@ -21,9 +21,9 @@
 // needs one exponential a class.  The list's own terms are worked out an entry a
 // thread.
 //
-// 1M x 10 float32 class-major, four listed: 31 us (124 MB, 3.9 TB/s).  1M x 100, 16
+// 1M x 10 float32 class-major, four listed: 32 us (124 MB, 3.8 TB/s).  1M x 100, 16
 // listed, at a temperature of 2: 219 us (940 MB, 4.3 TB/s; vector instructions in three
-// fifths of the cycles); at 1: 181 us with one listed, 223 with 16, 314 with 32.  8191 x
+// fifths of the cycles); at 1: 181 us with one listed, 228 with 16, 313 with 32.  8191 x
 // 16001 bfloat16, 64 listed: 127 us (529 MB, 4.1 TB/s, two exponentials a class), 123 with
 // one.  256 x 1000 float32: 7 us, latency.
 #pragma once

@@ -391,7 +391,9 @@ def class_alternatives(scores, top_k, *, labels=None, temperature=1.0) -> ClassA
     (int32 [n]; None without them; 0 for a label outside [0, K)), and ``norm`` [n, 3]
     what :func:`class_alternatives_grad` takes: the largest score m,
     log(sum exp((s - m) / temperature)) and the mean of (m - s) / temperature.
-    A row without a class has entropy 0 and norm (-inf, 0, 0).
+    A row without a class has entropy 0 and norm (-inf, 0, 0).  Rows of more than some
+    hundred classes whose best ones have neighbouring numbers (classes in the order of their
+    scores), or of very many equal scores, may take tens of times as long as others.
 
     top_k: 0 (no alternatives) to min(64, K)."""
     v = _matrix(scores, "scores")
